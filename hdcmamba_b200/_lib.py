@@ -68,6 +68,20 @@ SIGNATURES = {
     "hdc_ssm_carry_fwd": (c_int, [c_int, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp]),
     "hdc_slot_step": (c_int, [c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                               c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp]),
+    "hdc_gated_scan_state_rows": (c_i64, []),
+    "hdc_gated_scan_workspace_bytes": (c_size, [c_i64, c_i64, c_i64]),
+    "hdc_gated_scan_fwd": (c_int, [c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp,
+                                   c_vp, c_size, c_i64, c_i64, c_i64, c_vp]),
+    "hdc_gated_scan_bwd_workspace_bytes": (c_size, [c_i64, c_i64, c_i64]),
+    "hdc_gated_scan_bwd": (c_int, [c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp,
+                                   c_i64, c_i64, c_vp, c_vp, c_vp, c_size, c_i64, c_i64, c_i64, c_vp]),
+    "hdc_gated_step": (c_int, [c_int, c_int, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp]),
+    "hdc_group_norm_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64]),
+    "hdc_group_norm_fwd": (c_int, [c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp,
+                                   c_size, c_i64, c_i64, c_i64, c_i64, c_float, c_int, c_vp]),
+    "hdc_group_norm_bwd_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64]),
+    "hdc_group_norm_bwd": (c_int, [c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                   c_i64, c_i64, c_vp, c_vp, c_vp, c_size, c_i64, c_i64, c_i64, c_i64, c_int, c_vp]),
     "hdc_peer_alloc": (c_int, [c_size, ctypes.POINTER(c_vp)]),
     "hdc_peer_free": (c_int, [c_vp]),
     "hdc_ipc_handle_bytes": (c_int, []),

@@ -495,3 +495,215 @@ def slot_step(q, k, v, gate, num_heads, gamma, gn_w, gn_b, R, U, k_cache, v_cach
               _p(out), out.stride(0), B, H, hd, C, _p(pos), _stream(q))
     return out
 
+
+# ------------------------------------------------------------------ gated recurrence
+_ACTS = {"none": _lib.HDC_ACT_NONE, "silu": _lib.HDC_ACT_SILU}
+
+
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
+
+
+def _f32_state(t, shape, what):
+    if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous fp32 {list(shape)} tensor")
+
+
+def _gated_args(projs, A_log, d_state, reset, rows):
+    """Checks shared by the gated-recurrence ops; A_log and reset made contiguous."""
+    if projs.dim() != len(rows) + 1 or projs.shape[-1] < 3 * d_state or d_state < 1:
+        raise ValueError(f"projs {list(projs.shape)} must be {list(rows)} rows of >= 3*d_state columns")
+    if projs.shape[-1] > 1 and projs.stride(-1) != 1:
+        raise ValueError("projs needs a unit column stride")
+    if A_log.shape != (d_state,):
+        raise ValueError(f"A_log must be [{d_state}], got {list(A_log.shape)}")
+    if reset is not None:
+        if reset.dtype not in (torch.bool, torch.uint8) or reset.shape != rows:
+            raise ValueError(f"reset must be a bool {list(rows)} tensor")
+        reset = reset.contiguous()
+    return A_log.contiguous(), reset
+
+
+def gated_scan(projs, A_log, d_state, h0=None, reset=None, out=None, return_states=False):
+    """Gated linear recurrence over whole sequences (hdc_gated_scan_fwd): the Block's SSM gates
+    (hdcmamba/model.py:189-193) with no chunk rounding, h_t = exp(d A) h_{t-1} + d b x with
+    d = softplus(dt), A = -exp(A_log).
+
+    projs: [B, L, >=3*d_state] view (unit column stride), columns dt | x | b; L may be 0.
+    h0: optional fp32 [B, d_state] state before the first step.  reset: optional bool [B, L];
+    a true step starts from a zero state.  out: optional [B, L, d_state] view (unit column
+    stride).  Returns (y in projs.dtype, h_last fp32 [B, d_state]) and, if ``return_states``,
+    the states that ``gated_scan_bwd`` needs.  For autograd use ``recurrent.gated_scan``."""
+    _cuda(projs, A_log, h0, reset, out)
+    dt = _code(projs)
+    if projs.dim() != 3:
+        raise ValueError("projs must be [B, L, cols]")
+    B, L, _ = projs.shape
+    A_log, reset = _gated_args(projs, A_log, d_state, reset, (B, L))
+    if h0 is not None:
+        h0 = h0.float().contiguous()
+        if h0.shape != (B, d_state):
+            raise ValueError(f"h0 must be [{B}, {d_state}]")
+    if out is None:
+        out = torch.empty(B, L, d_state, device=projs.device, dtype=projs.dtype)
+    else:
+        _same_dtype(projs, out)
+        if out.shape != (B, L, d_state) or (d_state > 1 and out.stride(2) != 1):
+            raise ValueError(f"out must be a [{B}, {L}, {d_state}] view with unit column stride")
+    h_last = torch.empty(B, d_state, device=projs.device, dtype=torch.float32)
+    states = None
+    lib = _lib.load()
+    if return_states:
+        rows = lib.hdc_gated_scan_state_rows()
+        states = torch.empty(B, (L + rows - 1) // rows, d_state, device=projs.device, dtype=torch.float32)
+    ws = _workspace(lib.hdc_gated_scan_workspace_bytes(B, L, d_state), projs.device)
+    _lib.call("hdc_gated_scan_fwd", dt, _code(A_log), _p(projs), projs.stride(0), projs.stride(1), _p(A_log), _p(h0),
+              _p(reset), _p(out), out.stride(0), out.stride(1), _p(h_last), _p(states), _p(ws),
+              ws.numel() if ws is not None else 0, B, L, d_state, _stream(projs))
+    return (out, h_last, states) if return_states else (out, h_last)
+
+
+def gated_scan_bwd(dy, projs, A_log, states, d_state, reset=None, dh_last=None, need_dh0=False, out=None):
+    """Gradient of ``gated_scan`` (hdc_gated_scan_bwd).  ``states`` as returned by the forward
+    on the same inputs; dy: [B, L, d_state] view (unit column stride) in projs.dtype; dh_last:
+    optional fp32 [B, d_state].  out: optional [B, L, >=3*d_state] view that receives dprojs
+    (its first 3*d_state columns).  Returns (dprojs, dA_log in A_log.dtype, dh0 fp32
+    [B, d_state] or None)."""
+    _cuda(dy, projs, A_log, states, reset, dh_last, out)
+    dt = _code(projs)
+    if projs.dim() != 3:
+        raise ValueError("projs must be [B, L, cols]")
+    B, L, _ = projs.shape
+    A_log, reset = _gated_args(projs, A_log, d_state, reset, (B, L))
+    _same_dtype(projs, dy)
+    if dy.shape != (B, L, d_state):
+        raise ValueError(f"dy must be [{B}, {L}, {d_state}]")
+    if d_state > 1 and dy.stride(2) != 1:
+        dy = dy.contiguous()
+    lib = _lib.load()
+    rows = lib.hdc_gated_scan_state_rows()
+    _f32_state(states, (B, (L + rows - 1) // rows, d_state), "states")
+    if dh_last is not None:
+        dh_last = dh_last.float().contiguous()
+        if dh_last.shape != (B, d_state):
+            raise ValueError(f"dh_last must be [{B}, {d_state}]")
+    if out is None:
+        out = torch.empty(B, L, 3 * d_state, device=projs.device, dtype=projs.dtype)
+    else:
+        _same_dtype(projs, out)
+        if out.dim() != 3 or out.shape[:2] != (B, L) or out.shape[2] < 3 * d_state or out.stride(2) != 1:
+            raise ValueError(f"out must be a [{B}, {L}, >= {3 * d_state}] view with unit column stride")
+    dA = torch.empty(d_state, device=projs.device, dtype=A_log.dtype)
+    dh0 = torch.empty(B, d_state, device=projs.device, dtype=torch.float32) if need_dh0 else None
+    ws = _workspace(lib.hdc_gated_scan_bwd_workspace_bytes(B, L, d_state), projs.device)
+    _lib.call("hdc_gated_scan_bwd", dt, _code(A_log), _p(projs), projs.stride(0), projs.stride(1), _p(A_log),
+              _p(states), _p(reset), _p(dy), dy.stride(0), dy.stride(1), _p(dh_last), _p(out), out.stride(0),
+              out.stride(1), _p(dA), _p(dh0), _p(ws), ws.numel() if ws is not None else 0, B, L, d_state,
+              _stream(projs))
+    return out, dA, dh0
+
+
+def gated_step(projs, A_log, h, d_state, reset=None, out=None, h_out=None):
+    """One step of ``gated_scan`` per sequence (hdc_gated_step): projs [B, >=3*d_state] (unit
+    column stride), h fp32 [B, d_state], updated in place unless ``h_out`` is given; reset:
+    optional bool [B].  Returns (y [B, d_state] in projs.dtype, the new state)."""
+    _cuda(projs, A_log, h, reset, out, h_out)
+    dt = _code(projs)
+    if projs.dim() != 2:
+        raise ValueError("projs must be [B, cols]")
+    B = projs.shape[0]
+    A_log, reset = _gated_args(projs, A_log, d_state, reset, (B,))
+    _f32_state(h, (B, d_state), "h")
+    if h_out is None:
+        h_out = h
+    else:
+        _f32_state(h_out, (B, d_state), "h_out")
+    if out is None:
+        out = torch.empty(B, d_state, device=projs.device, dtype=projs.dtype)
+    else:
+        _same_dtype(projs, out)
+        if out.shape != (B, d_state) or (d_state > 1 and out.stride(1) != 1):
+            raise ValueError(f"out must be a [{B}, {d_state}] view with unit column stride")
+    _lib.call("hdc_gated_step", dt, _code(A_log), _p(projs), projs.stride(0), _p(A_log), _p(h), _p(reset), _p(h_out),
+              _p(out), out.stride(0), B, d_state, _stream(projs))
+    return out, h_out
+
+
+# ------------------------------------------------------------------ group norm + activation
+def _positions(x):
+    """x [N, ..., C] as a [N, S, C] view with unit channel stride (a copy only when the
+    strides of the positions do not allow one)."""
+    if x.dim() < 2:
+        raise ValueError(f"group_norm_act needs [N, ..., C], got {list(x.shape)}")
+    if x.dim() != 3:
+        S = 1
+        for n in x.shape[1:-1]:
+            S *= n
+        x = x.reshape(x.shape[0], S, x.shape[-1])
+    return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
+
+
+def _norm_params(x, num_groups, weight, bias):
+    C = x.shape[-1]
+    if num_groups < 1 or C < 1 or C % num_groups != 0:
+        raise ValueError(f"{C} channels do not split into {num_groups} groups")
+    for t, what in ((weight, "weight"), (bias, "bias")):
+        if t is not None and t.shape != (C,):
+            raise ValueError(f"{what} must be [{C}], got {list(t.shape)}")
+    if weight is not None and bias is not None:
+        _same_dtype(weight, bias)
+    ref = weight if weight is not None else bias
+    return (_code(ref) if ref is not None else _code(x), weight.contiguous() if weight is not None else None,
+            bias.contiguous() if bias is not None else None)
+
+
+def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", stats=False):
+    """Group norm with an activation, channels last (hdc_group_norm_fwd): x [N, ..., C],
+    statistics of each sample and group of C / num_groups neighbouring channels over all
+    positions in between ([N, C]: over the group's channels alone, as the Block's GroupNorm
+    per head and token, hdcmamba/model.py:285-292).  act: "none" or "silu".  Returns y (and
+    fp32 mean, rstd [N, num_groups] if ``stats``).  For autograd use
+    ``recurrent.group_norm_act``."""
+    _cuda(x, weight, bias)
+    dt = _code(x)
+    if act not in _ACTS:
+        raise ValueError(f"act must be one of {sorted(_ACTS)}")
+    x3 = _positions(x)
+    pd, weight, bias = _norm_params(x, num_groups, weight, bias)
+    N, S, C = x3.shape
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    mean = rstd = None
+    if stats:
+        mean = torch.empty(N, num_groups, device=x.device, dtype=torch.float32)
+        rstd = torch.empty(N, num_groups, device=x.device, dtype=torch.float32)
+    ws = _workspace(_lib.load().hdc_group_norm_workspace_bytes(N, S, C, num_groups), x.device)
+    _lib.call("hdc_group_norm_fwd", dt, pd, _p(x3), x3.stride(0), x3.stride(1), _p(weight), _p(bias), _p(y), S * C, C,
+              _p(mean), _p(rstd), _p(ws), ws.numel() if ws is not None else 0, N, S, C, num_groups, float(eps),
+              _ACTS[act], _stream(x))
+    return (y, mean, rstd) if stats else y
+
+
+def group_norm_act_bwd(dy, x, mean, rstd, num_groups, weight=None, bias=None, act="none", need_params=True):
+    """Gradient of ``group_norm_act`` (hdc_group_norm_bwd) from the forward's mean and rstd.
+    Returns (dx in x.dtype, dweight, dbias in the parameters' type, None for a parameter that
+    is None or when ``need_params`` is false)."""
+    _cuda(dy, x, mean, rstd, weight, bias)
+    dt = _code(x)
+    if act not in _ACTS:
+        raise ValueError(f"act must be one of {sorted(_ACTS)}")
+    _same_dtype(x, dy)
+    if dy.shape != x.shape:
+        raise ValueError(f"dy {list(dy.shape)} must have x's shape {list(x.shape)}")
+    x3, d3 = _positions(x), _positions(dy)
+    pd, weight, bias = _norm_params(x, num_groups, weight, bias)
+    N, S, C = x3.shape
+    _f32_state(mean, (N, num_groups), "mean")
+    _f32_state(rstd, (N, num_groups), "rstd")
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    dw = torch.empty_like(weight) if need_params and weight is not None else None
+    db = torch.empty_like(bias) if need_params and bias is not None else None
+    ws = _workspace(_lib.load().hdc_group_norm_bwd_workspace_bytes(N, S, C, num_groups), x.device)
+    _lib.call("hdc_group_norm_bwd", dt, pd, _p(d3), d3.stride(0), d3.stride(1), _p(x3), x3.stride(0), x3.stride(1),
+              _p(mean), _p(rstd), _p(weight), _p(bias), _p(dx), S * C, C, _p(dw), _p(db), _p(ws),
+              ws.numel() if ws is not None else 0, N, S, C, num_groups, _ACTS[act], _stream(x))
+    return dx, dw, db

@@ -356,6 +356,75 @@ int hdc_slot_step(int dtype, const void* q, const void* k, const void* v, const 
                   const int32_t* pos, hdc_stream_t stream);
 
 /*
+ * Gated linear recurrence with gradient and single-token step.  The Block's diagonal SSM
+ * gates (hdcmamba/model.py:189-193) without the reference's chunks and bf16 rounding points:
+ * any length and width, a carried fp32 state, resets at document starts.  Per batch b and
+ * channel j < ds, projs columns [0,ds) dt, [ds,2ds) x, [2ds,3ds) b:
+ *   d_t = softplus(dt_t) (dt itself above 20), A = -exp(A_log), a_t = exp(d_t A),
+ *   h_t = a_t h_{t-1} + d_t b_t x_t,  y_t = h_t.
+ * dtype is that of projs, y, dy and dprojs; a_dtype that of A_log and dA_log.  fp32 arithmetic.
+ *   projs  : row (b, t) starts at projs + b*proj_sb + t*proj_st (elements; rows may overlap).
+ *   h0     : NULL (zeros) or fp32 [B, ds], the state before the first step.
+ *   reset  : NULL or uint8 [B, L] contiguous; where non-zero, step t starts from a zero state
+ *            whatever h_{t-1} holds (infinities and NaN included).
+ *   y      : element (b, t, j) at y + b*y_sb + t*y_st + j; must not overlap projs.
+ *   h_last : NULL or fp32 [B, ds], the state after the last step (h0 or zeros when L = 0).
+ *   states : NULL, or fp32 [B, ceil(L / R), ds] with R = hdc_gated_scan_state_rows(): the
+ *            state before steps 0, R, 2R, ..., which the gradient starts from.
+ *   workspace : hdc_gated_scan_workspace_bytes(B, L, ds) bytes, 16-byte aligned.
+ * hdc_gated_scan_bwd: dy as y (a gradient of y), dh_last NULL or fp32 [B, ds]; writes dprojs
+ *   (columns d dt | d x | d b, row (b, t) at dprojs + b*dp_sb + t*dp_st), dA_log [ds] and,
+ *   unless NULL, dh0 fp32 [B, ds].  Sums over b and t are taken in a fixed order.
+ * hdc_gated_step: one step per sequence from projs rows [B, >=3ds]; h / h_out fp32 [B, ds]
+ *   (h_out may be h), reset NULL or uint8 [B].
+ * B in [0, 65535], L in [0, 2^30], ds in [1, 2^20].  Pointers need their type's alignment;
+ * 16-byte aligned rows take the wide loads.
+ */
+int64_t hdc_gated_scan_state_rows(void);
+size_t hdc_gated_scan_workspace_bytes(int64_t B, int64_t L, int64_t ds);
+int hdc_gated_scan_fwd(int dtype, int a_dtype, const void* projs, int64_t proj_sb, int64_t proj_st,
+                       const void* A_log, const float* h0, const uint8_t* reset, void* y, int64_t y_sb,
+                       int64_t y_st, float* h_last, float* states, void* workspace, size_t workspace_bytes,
+                       int64_t B, int64_t L, int64_t ds, hdc_stream_t stream);
+size_t hdc_gated_scan_bwd_workspace_bytes(int64_t B, int64_t L, int64_t ds);
+int hdc_gated_scan_bwd(int dtype, int a_dtype, const void* projs, int64_t proj_sb, int64_t proj_st,
+                       const void* A_log, const float* states, const uint8_t* reset, const void* dy,
+                       int64_t dy_sb, int64_t dy_st, const float* dh_last, void* dprojs, int64_t dp_sb,
+                       int64_t dp_st, void* dA_log, float* dh0, void* workspace, size_t workspace_bytes,
+                       int64_t B, int64_t L, int64_t ds, hdc_stream_t stream);
+int hdc_gated_step(int dtype, int a_dtype, const void* projs, int64_t proj_sb, const void* A_log,
+                   const float* h, const uint8_t* reset, float* h_out, void* y, int64_t y_sb, int64_t B,
+                   int64_t ds, hdc_stream_t stream);
+
+/*
+ * Group norm with an activation, channels last, with gradient: x [N, S, C], statistics (mean
+ * and biased variance, fp32) of each sample and group of C / G channels over the S positions,
+ *   y = act((x - mean) * rstd * weight_c + bias_c),  rstd = 1 / sqrt(var + eps).
+ * S = 1 is nn.GroupNorm as the Block applies it per head and token
+ * (hdcmamba/model.py:285-292); S > 1 its form over positions.  dtype is that of x, y, dy, dx;
+ * p_dtype that of weight, bias, dweight, dbias ([C]; weight NULL = ones, bias NULL = zeros).
+ *   x      : element (n, s, c) at x + n*x_sn + s*x_ss + c (elements); y, dy, dx likewise.
+ *   mean, rstd : fp32 [N, G]; both NULL in the forward when no gradient follows.
+ *   act    : HDC_ACT_NONE or HDC_ACT_SILU.
+ * hdc_group_norm_bwd: dx and, unless NULL, dweight / dbias from dy and the forward's mean and
+ *   rstd; sums in a fixed order.  dx may be dy or x itself.
+ * C in [1, 65536], G a divisor of C, N and S in [0, 2^30], N*G < 2^31.  Pointers need their
+ * type's alignment; 16-byte aligned rows take the wide loads.  workspace: the
+ * *_workspace_bytes of the shape, 16-byte aligned.
+ */
+size_t hdc_group_norm_workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G);
+int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t x_sn, int64_t x_ss,
+                       const void* weight, const void* bias, void* y, int64_t y_sn, int64_t y_ss,
+                       float* mean, float* rstd, void* workspace, size_t workspace_bytes, int64_t N,
+                       int64_t S, int64_t C, int64_t G, float eps, int act, hdc_stream_t stream);
+size_t hdc_group_norm_bwd_workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G);
+int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_t dy_sn, int64_t dy_ss,
+                       const void* x, int64_t x_sn, int64_t x_ss, const float* mean, const float* rstd,
+                       const void* weight, const void* bias, void* dx, int64_t dx_sn, int64_t dx_ss,
+                       void* dweight, void* dbias, void* workspace, size_t workspace_bytes, int64_t N,
+                       int64_t S, int64_t C, int64_t G, int act, hdc_stream_t stream);
+
+/*
  * Peer-memory exchange for sequence parallelism (one process per GPU, NVLink / NVSwitch).
  * No reference counterpart: it replaces the all-gathers of the sequence-parallel runner
  * with direct peer stores where the data flow is one-directional (rank r needs the carries
