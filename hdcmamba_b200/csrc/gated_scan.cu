@@ -10,12 +10,34 @@
 // (c_t = s_t = 0 where t is a reset.)  All arithmetic is in fp32; only y and dprojs are
 // rounded, once, to the activation type.
 //
-// Schedule: one thread per (batch, channel) walks the sequence.
-#include "common.cuh"
+// Forward schedule (bound by HBM: 3 values read and 1 written per step and channel): the
+// sequence is cut into tiles of 64 steps x 128 bytes of channels (64 bf16, 32 fp32).  A step is
+// the map h -> a h + u, and maps compose: (P, H) then (P', H') is (P' P, P' H + H'), so each
+// tile is scanned from a zero state, and the state entering it is added afterwards through P:
+//   * a warp owns 8 steps of the tile, a lane one 4-byte word of channels; its a and u stay in
+//     registers between the local scan and the outputs, so every input is read once;
+//   * the 8 warps' maps are composed through shared memory, and the tile's map is published in
+//     the workspace;
+//   * the state entering the tile is composed from at most 31 published entries: the state at
+//     the end of the last whole 256 tiles, the maps of the whole 16-tile spans after it, and the
+//     maps of the tiles after those.  Which entries is a matter of the tile's index alone, so
+//     the result does not depend on timing.
+// CTAs take tiles by ticket, time-major: a tile waits only for tiles with smaller tickets,
+// which running CTAs hold, so the waits end (they are bounded all the same).  An entry is one
+// 64-bit word per channel, (P, H); the workspace is set to all ones before the launch, which
+// no published P is, so the word is its own flag.  The next tile is in flight (cp.async)
+// while one is computed.
+// P < 0 marks a map that a reset has cut off from what came before (P is otherwise >= 0).
+#include <type_traits>
+
+#include "tc.cuh"
 
 namespace hdc {
 
-constexpr int kStateRows = 128;  // rows per saved state
+constexpr int kStateRows = 64;       // rows per tile = rows per saved state
+constexpr int kWarps = 8, kRows = 8;  // warps per tile, steps per warp
+constexpr int kSpan = 16;            // tiles per span, spans per chain link
+static_assert(kWarps * kRows == kStateRows, "a tile is one state interval");
 
 struct ScanParams {
   const void* projs; int64_t psb, pst;
@@ -29,6 +51,14 @@ struct ScanParams {
   void* dprojs; int64_t gsb, gst;
   float* dA_part; float* dh0; float* hbuf;
   int B, L, ds, NT;
+  // tiles
+  int nch;          // channel groups
+  int NG;           // channel groups of all batches
+  int64_t ntiles;   // NG * NT
+  unsigned* ticket;  // NULL: a single tile in time, taken by block index, nothing published
+  uint64_t* ent;    // [NG][NT + spans + links][CW] published entries
+  int nent;         // entries per group
+  int out_vec;      // the outputs' rows allow whole words
 };
 
 __device__ __forceinline__ float ld_param(const void* p, int bf16, int i) {
@@ -38,25 +68,421 @@ __device__ __forceinline__ float ld_param(const void* p, int bf16, int i) {
 // softplus with the Block's threshold (hdcmamba/model.py:192), exact for small exp(x) too
 __device__ __forceinline__ float softplus_acc(float x) { return x > 20.0f ? x : log1pf(expf(x)); }
 
+// ---------------------------------------------------------------- one word of channels
+// The channels of a lane: one fp32 value, or two bf16 values computed as a pair
+// (fma.rn.f32x2 and friends: two fp32 operations per issued instruction).
+template <int V> struct Fv { float v[V]; };
+template <typename T> constexpr int kVec = 4 / sizeof(T);
+template <typename T> constexpr int kCW = 32 * kVec<T>;  // channels per tile
+
+__device__ __forceinline__ uint64_t f2_bits(const Fv<2>& a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.v[0]), "f"(a.v[1]));
+  return r;
+}
+__device__ __forceinline__ Fv<2> bits_f2(uint64_t b) {
+  Fv<2> r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.v[0]), "=f"(r.v[1]) : "l"(b));
+  return r;
+}
+__device__ __forceinline__ Fv<1> fma(const Fv<1>& a, const Fv<1>& b, const Fv<1>& c) {
+  return {{fmaf(a.v[0], b.v[0], c.v[0])}};
+}
+__device__ __forceinline__ Fv<1> operator*(const Fv<1>& a, const Fv<1>& b) { return {{a.v[0] * b.v[0]}}; }
+__device__ __forceinline__ Fv<1> operator+(const Fv<1>& a, const Fv<1>& b) { return {{a.v[0] + b.v[0]}}; }
+__device__ __forceinline__ Fv<2> fma(const Fv<2>& a, const Fv<2>& b, const Fv<2>& c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+  return bits_f2(r);
+}
+__device__ __forceinline__ Fv<2> operator*(const Fv<2>& a, const Fv<2>& b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return bits_f2(r);
+}
+__device__ __forceinline__ Fv<2> operator+(const Fv<2>& a, const Fv<2>& b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return bits_f2(r);
+}
+template <int V> __device__ __forceinline__ Fv<V> all(float x) {
+  Fv<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = x;
+  return r;
+}
+__device__ __forceinline__ Fv<1> word_f(uint32_t w, float) { return {{__uint_as_float(w)}}; }
+__device__ __forceinline__ Fv<2> word_f(uint32_t w, __nv_bfloat16) {
+  return {{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)}};
+}
+__device__ __forceinline__ uint32_t f_word(const Fv<1>& a) { return __float_as_uint(a.v[0]); }
+__device__ __forceinline__ uint32_t f_word(const Fv<2>& a) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a.v[0], a.v[1]);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// store a word of channels c, c+1, ... (< ds); vec: the row allows the whole word
 template <typename T>
-__global__ void __launch_bounds__(128) gated_scan_fwd_kernel(ScanParams p) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (int64_t)p.B * p.ds) return;
-  const int b = (int)(i / p.ds), j = (int)(i - (int64_t)b * p.ds);
-  const float A = -expf(ld_param(p.A_log, p.a_bf16, j));
-  const T* in = static_cast<const T*>(p.projs) + b * p.psb + j;
-  T* y = static_cast<T*>(p.y) + b * p.ysb + j;
-  const uint8_t* rs = p.reset ? p.reset + (int64_t)b * p.L : nullptr;
-  float h = p.h0 ? p.h0[i] : 0.f;
-  for (int t = 0; t < p.L; ++t) {
-    if (p.states && t % kStateRows == 0) p.states[((int64_t)b * p.NT + t / kStateRows) * p.ds + j] = h;
-    const T* r = in + t * p.pst;
-    const float d = softplus_acc(to_f(r[0]));
-    const float u = d * to_f(r[2 * p.ds]) * to_f(r[p.ds]);
-    h = (rs && rs[t]) ? u : fmaf(expf(d * A), h, u);
-    y[t * p.yst] = from_f<T>(h);
+__device__ __forceinline__ void st_word(T* row, int c, int ds, int vec, const Fv<kVec<T>>& v) {
+  if (vec && c + kVec<T> <= ds) {
+    *reinterpret_cast<uint32_t*>(row + c) = f_word(v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i)
+      if (c + i < ds) row[c + i] = from_f<T>(v.v[i]);
   }
-  if (p.h_last) p.h_last[i] = h;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// d = softplus(x) and a = exp(d A) for the lane's channels.
+//   fp32: the library's exp and log1p.
+//   bf16 inputs: softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) by the hardware's 2^x, and
+//   log1p(e) = e p(e) on [0, 1] with p of degree 7, fitted here for the least relative error
+//   (weighted least squares on Chebyshev points, weights iterated to equal errors: 2e-7, 3e-7
+//   with fp32 evaluation; the bf16 input itself is 2^-9 off).  e p(e) keeps its relative accuracy
+//   for small e, where log(1 + e) loses it.  A2 = A log2(e).
+__device__ __forceinline__ void gates(const Fv<1>& x, const Fv<1>& A, const Fv<1>&, Fv<1>& d, Fv<1>& a) {
+  d.v[0] = softplus_acc(x.v[0]);
+  a.v[0] = expf(d.v[0] * A.v[0]);
+}
+__device__ __forceinline__ void gates(const Fv<2>& x, const Fv<2>&, const Fv<2>& A2, Fv<2>& d, Fv<2>& a) {
+  Fv<2> e, m;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    e.v[i] = ex2(-1.4426950408889634f * fabsf(x.v[i]));
+    m.v[i] = x.v[i] < 0.f ? 0.f : x.v[i];  // not fmaxf: NaN stays NaN
+  }
+  Fv<2> p = all<2>(-0.008539206348359585f);
+  p = fma(p, e, all<2>(0.04408962279558182f));
+  p = fma(p, e, all<2>(-0.10768169909715652f));
+  p = fma(p, e, all<2>(0.17745240032672882f));
+  p = fma(p, e, all<2>(-0.24495463073253632f));
+  p = fma(p, e, all<2>(0.33275479078292847f));
+  p = fma(p, e, all<2>(-0.4999740421772003f));
+  p = fma(p, e, all<2>(0.9999998211860657f));
+  d = fma(p, e, m);
+  const Fv<2> l = d * A2;
+  a.v[0] = ex2(l.v[0]);
+  a.v[1] = ex2(l.v[1]);
+}
+
+// ---------------------------------------------------------------- maps h -> P h + H
+template <int V> struct Map { Fv<V> P, H; };
+template <int V> __device__ __forceinline__ Map<V> identity_map() { return {all<V>(1.f), all<V>(0.f)}; }
+// m applied to a state
+template <int V> __device__ __forceinline__ Fv<V> apply(const Map<V>& m, const Fv<V>& h) {
+  Fv<V> r = fma(m.P, h, m.H);
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = m.P.v[i] < 0.f ? m.H.v[i] : r.v[i];
+  return r;
+}
+// first m, then n
+template <int V> __device__ __forceinline__ Map<V> then(const Map<V>& m, const Map<V>& n) {
+  Map<V> r;
+  r.H = apply(n, m.H);
+  r.P = m.P * n.P;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.P.v[i] = (m.P.v[i] < 0.f || n.P.v[i] < 0.f) ? -1.f : r.P.v[i];
+  return r;
+}
+// a lane's map in shared memory: 8 bytes per channel
+template <int V> __device__ __forceinline__ void st_map(char* p, int lane, const Map<V>& m) {
+  float* f = reinterpret_cast<float*>(p) + lane * 2 * V;
+  if constexpr (V == 2) *reinterpret_cast<float4*>(f) = make_float4(m.P.v[0], m.H.v[0], m.P.v[1], m.H.v[1]);
+  else *reinterpret_cast<float2*>(f) = make_float2(m.P.v[0], m.H.v[0]);
+}
+template <int V> __device__ __forceinline__ Map<V> ld_map(const char* p, int lane) {
+  const float* f = reinterpret_cast<const float*>(p) + lane * 2 * V;
+  if constexpr (V == 2) {
+    const float4 q = *reinterpret_cast<const float4*>(f);
+    return {{{q.x, q.z}}, {{q.y, q.w}}};
+  } else {
+    const float2 q = *reinterpret_cast<const float2*>(f);
+    return {{{q.x}}, {{q.y}}};
+  }
+}
+
+// ---------------------------------------------------------------- published entries
+constexpr uint32_t kUnset = 0xffffffffu;  // P of a word that is not published
+template <int V> __device__ __forceinline__ void publish(uint64_t* e, int lane, const Map<V>& m) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    uint32_t P = __float_as_uint(m.P.v[i]);
+    if (P == kUnset) P = 0x7fffffffu;  // a NaN stays one
+    const uint64_t w = ((uint64_t)__float_as_uint(m.H.v[i]) << 32) | P;
+    asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(e + lane * V + i), "l"(w) : "memory");
+  }
+}
+__device__ __forceinline__ uint64_t ld_entry(const uint64_t* e) {
+  uint64_t w;
+  asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(w) : "l"(e) : "memory");
+  return w;
+}
+// Compose n <= 4 neighbouring entries, each waited for (2 s in all, then error 61 and zeros).
+template <int V> __device__ __forceinline__ Map<V> take(const uint64_t* e, int n, int lane) {
+  uint64_t w[4][V];
+  uint64_t t0 = 0;
+  bool late = false;
+  while (true) {
+    bool ok = true;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (k < n) {
+          w[k][i] = ld_entry(e + (int64_t)k * 32 * V + lane * V + i);
+          ok = ok && (uint32_t)w[k][i] != kUnset;
+        }
+    if (__all_sync(0xffffffffu, ok)) break;
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    late = now - t0 > 2000000000ull;
+    if (__any_sync(0xffffffffu, late)) {
+      if (lane == 0) atomicCAS(&g_dev_error, 0, 61);
+      break;
+    }
+  }
+  Map<V> m = identity_map<V>();
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (k < n) {
+      Map<V> q;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const bool set = (uint32_t)w[k][i] != kUnset;
+        q.P.v[i] = set ? __uint_as_float((uint32_t)w[k][i]) : 0.f;
+        q.H.v[i] = set ? __uint_as_float((uint32_t)(w[k][i] >> 32)) : 0.f;
+      }
+      m = then(m, q);
+    }
+  return m;
+}
+// Entry indices of a group: tiles, then spans of 16 tiles, then links of 16 spans.
+__device__ __forceinline__ int span_at(int NT, int k) { return NT + k; }
+__device__ __forceinline__ int link_at(int NT, int k) { return NT + (NT + kSpan - 1) / kSpan + k; }
+
+// This warp's part of what precedes tile q of its group: warps 0..3 compose the link and the
+// whole spans (up to 16 entries), warps 4..7 the tiles of the span that q is in (up to 15).
+template <int V>
+__device__ __forceinline__ Map<V> before_tile(const uint64_t* ent, int NT, int q, int warp, int lane) {
+  constexpr int CW = 32 * V;
+  if (warp >= 4) {
+    const int n = min(4, q % kSpan - (warp - 4) * 4);
+    if (n <= 0) return identity_map<V>();
+    return take<V>(ent + (int64_t)(q - q % kSpan + (warp - 4) * 4) * CW, n, lane);
+  }
+  const int link = q / (kSpan * kSpan), s0 = link * kSpan, ns = q / kSpan - s0;
+  Map<V> m = identity_map<V>();
+  if (warp == 0 && link > 0) m = take<V>(ent + (int64_t)link_at(NT, link - 1) * CW, 1, lane);
+  const int n = min(4, ns - warp * 4);
+  if (n > 0) m = then(m, take<V>(ent + (int64_t)span_at(NT, s0 + warp * 4) * CW, n, lane));
+  return m;
+}
+
+// ---------------------------------------------------------------- staging
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool ok, std::integral_constant<int, 16>) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool ok, std::integral_constant<int, 4>) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+// The warp's 8 rows of 128 bytes from base (row stride st elements), rows >= nv and channels >=
+// nc as zeros.  CB: bytes per copy (rows allow 16 or 4), 0: element by element, not asynchronous.
+template <typename T, int CB>
+__device__ __forceinline__ void stage_rows(char* dst, const T* base, int64_t st, int nv, int nc, int lane) {
+  if constexpr (CB == 0) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      T v[kVec<T>];
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i) {
+        const int c = lane * kVec<T> + i;
+        v[i] = r < nv && c < nc ? base[r * st + c] : from_f<T>(0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i) reinterpret_cast<T*>(dst + r * 128)[lane * kVec<T> + i] = v[i];
+    }
+  } else {
+    constexpr int per_row = 128 / CB, rows = 32 / per_row;  // rows per warp-wide copy
+    const int r0 = lane / per_row, x = lane % per_row;
+    const bool in = x * (CB / (int)sizeof(T)) < nc;
+    const uint32_t d = smem_u32(dst) + r0 * 128 + x * CB;
+    const char* s = reinterpret_cast<const char*>(base) + x * CB;
+#pragma unroll
+    for (int k = 0; k < kRows / rows; ++k) {
+      const bool ok = in && r0 + k * rows < nv;
+      cp_async(d + k * rows * 128, ok ? s + (r0 + k * rows) * st * (int64_t)sizeof(T) : reinterpret_cast<const char*>(base),
+               ok, std::integral_constant<int, CB>());
+    }
+  }
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+struct Tile {
+  int q, g, b, c0;  // index in time, group, batch, first channel
+};
+template <typename T> __device__ __forceinline__ Tile tile_of(const ScanParams& p, int64_t id) {
+  Tile t;
+  t.q = (int)(id / p.NG);
+  t.g = (int)(id - (int64_t)t.q * p.NG);
+  t.b = t.g / p.nch;
+  t.c0 = (t.g - t.b * p.nch) * kCW<T>;
+  return t;
+}
+__device__ __forceinline__ int64_t next_tile(const ScanParams& p, int64_t last) {
+  if (!p.ticket) return last + gridDim.x;
+  return (int64_t)(unsigned)(atomicAdd(p.ticket, 1u) + 1u);  // the counter starts at all ones
+}
+// the warp's reset flags as a mask (bit r: step r of its rows)
+__device__ __forceinline__ uint32_t reset_byte(const ScanParams& p, int b, int t, int nv, int lane) {
+  return lane < nv ? p.reset[(int64_t)b * p.L + t + lane] : 0;
+}
+
+template <typename T, bool RESET, int CB>
+__global__ void __launch_bounds__(kWarps * 32, 4) gated_scan_fwd_kernel(const ScanParams p) {
+  constexpr int V = kVec<T>, CW = kCW<T>, kRegion = 3 * kRows * 128;
+  extern __shared__ __align__(128) char raw[];  // [2][warp][dt, x, b][row][128 bytes]
+  __shared__ __align__(16) float s_h[CW];
+  __shared__ __align__(16) char s_tile[CW * 8];
+  __shared__ int64_t s_next[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int cl = lane * V;  // the lane's first channel of the tile
+
+  // what a lane holds for a staged tile besides the copies
+  struct Ahead { float A[V]; uint32_t rb; };
+  auto stage = [&](const Tile& t, char* buf, Ahead& n) {
+    const int t0 = t.q * kStateRows + warp * kRows;
+    const int nv = min(kRows, p.L - t0), nc = p.ds - t.c0;
+    const T* in = static_cast<const T*>(p.projs) + t.b * p.psb + t0 * p.pst + t.c0;
+    char* reg = buf + warp * kRegion;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) stage_rows<T, CB>(reg + k * kRows * 128, in + k * p.ds, p.pst, nv, nc, lane);
+    cp_commit();
+#pragma unroll
+    for (int i = 0; i < V; ++i) n.A[i] = cl + i < nc ? ld_param(p.A_log, p.a_bf16, t.c0 + cl + i) : 0.f;
+    if (RESET) n.rb = reset_byte(p, t.b, t0, nv, lane);
+  };
+
+  if (threadIdx.x == 0) s_next[0] = p.ticket ? next_tile(p, 0) : blockIdx.x;
+  __syncthreads();
+  int64_t id = s_next[0];
+  Ahead ahead = {};
+  int s = 0;
+  if (id < p.ntiles) stage(tile_of<T>(p, id), raw, ahead);
+  for (; id < p.ntiles; s ^= 1) {
+    const Tile t = tile_of<T>(p, id);
+    if (threadIdx.x == 0) s_next[s ^ 1] = next_tile(p, id);
+    char* buf = raw + s * kWarps * kRegion;
+    char* mine = buf + warp * kRegion;
+    const int t0 = t.q * kStateRows + warp * kRows, nv = min(kRows, p.L - t0);
+    Fv<V> A, A2;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      A.v[i] = -expf(ahead.A[i]);
+      A2.v[i] = A.v[i] * 1.4426950408889634f;
+    }
+    const uint32_t cut = RESET ? __ballot_sync(0xffffffffu, ahead.rb != 0) : 0;
+    cp_wait_all();
+    __syncwarp();
+
+    // local scan of the warp's steps from a zero state
+    Fv<V> a[kRows], u[kRows];
+    Map<V> m = identity_map<V>();
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(mine + r * 128) + lane;
+      const Fv<V> dt = word_f(w[0], T()), x = word_f(w[kRows * 32], T()), b = word_f(w[2 * kRows * 32], T());
+      Fv<V> d;
+      // past the end the staged zeros give u = 0, and A = 0 gives a = 1: the identity
+      gates(dt, r < nv ? A : all<V>(0.f), r < nv ? A2 : all<V>(0.f), d, a[r]);
+      u[r] = d * b * x;
+      if (RESET && ((cut >> r) & 1)) {
+        m.H = u[r];
+        m.P = all<V>(-1.f);
+      } else {
+        m.H = fma(a[r], m.H, u[r]);
+        if (!RESET || !(m.P.v[0] < 0.f)) m.P = m.P * a[r];
+      }
+    }
+    __syncwarp();
+    st_map<V>(mine, lane, m);
+    __syncthreads();
+
+    const int64_t nid = s_next[s ^ 1];
+    if (nid < p.ntiles) stage(tile_of<T>(p, nid), raw + (s ^ 1) * kWarps * kRegion, ahead);
+
+    // the tile's map, published; then the state entering the tile
+    Fv<V> h;
+    if (p.ticket) {
+      uint64_t* ent = p.ent + (int64_t)t.g * p.nent * CW;
+      if (warp == 0) {
+        Map<V> all8 = ld_map<V>(buf, lane);
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) all8 = then(all8, ld_map<V>(buf + k * kRegion, lane));
+        if (t.q + 1 < p.NT) publish<V>(ent + (int64_t)t.q * CW, lane, all8);
+        st_map<V>(s_tile, lane, all8);
+      }
+      st_map<V>(mine + 512, lane, before_tile<V>(ent, p.NT, t.q, warp, lane));
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int c = t.c0 + cl + i;
+          h.v[i] = p.h0 && c < p.ds ? p.h0[(int64_t)t.b * p.ds + c] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) h = apply(ld_map<V>(buf + k * kRegion + 512, lane), h);
+#pragma unroll
+        for (int i = 0; i < V; ++i) s_h[cl + i] = h.v[i];
+        if (t.q % (kSpan * kSpan) == kSpan * kSpan - 1 && t.q + 1 < p.NT) {  // the end of a link
+          const Map<V> end = {all<V>(-1.f), apply(ld_map<V>(s_tile, lane), h)};
+          publish<V>(ent + (int64_t)link_at(p.NT, t.q / (kSpan * kSpan)) * CW, lane, end);
+        }
+      } else if (warp == 1 && t.q % kSpan == kSpan - 1 && t.q + 1 < p.NT) {  // the end of a span
+        Map<V> sp = identity_map<V>();
+#pragma unroll
+        for (int k = 4; k < kWarps; ++k) sp = then(sp, ld_map<V>(buf + k * kRegion + 512, lane));
+        publish<V>(ent + (int64_t)span_at(p.NT, t.q / kSpan) * CW, lane, then(sp, ld_map<V>(s_tile, lane)));
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < V; ++i) h.v[i] = s_h[cl + i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = t.c0 + cl + i;
+        h.v[i] = p.h0 && c < p.ds ? p.h0[(int64_t)t.b * p.ds + c] : 0.f;
+      }
+    }
+    if (p.states && warp == 0) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = t.c0 + cl + i;
+        if (c < p.ds) p.states[((int64_t)t.b * p.NT + t.q) * p.ds + c] = h.v[i];
+      }
+    }
+    for (int k = 0; k < warp; ++k) h = apply(ld_map<V>(buf + k * kRegion, lane), h);
+
+    T* y = static_cast<T*>(p.y) + t.b * p.ysb + t0 * p.yst + t.c0;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      h = RESET && ((cut >> r) & 1) ? u[r] : fma(a[r], h, u[r]);
+      if (r < nv) st_word<T>(y + r * p.yst, cl, p.ds - t.c0, p.out_vec, h);
+    }
+    if (p.h_last && t.q == p.NT - 1 && warp == kWarps - 1) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = t.c0 + cl + i;
+        if (c < p.ds) p.h_last[(int64_t)t.b * p.ds + c] = h.v[i];
+      }
+    }
+    id = nid;
+  }
 }
 
 template <typename T>
@@ -139,6 +565,49 @@ static bool off_type(const void* p, int dtype) {
   return (reinterpret_cast<uintptr_t>(p) & (dtype == HDC_F32 ? 3u : 1u)) != 0;
 }
 
+// ---------------------------------------------------------------- plans
+// every row of a tensor (batch stride sb, row stride st, in elements) starts on `align` bytes
+static int rows_allow(const void* p, int64_t sb, int64_t st, int es, int align) {
+  return reinterpret_cast<uintptr_t>(p) % align == 0 && sb * es % align == 0 && st * es % align == 0;
+}
+static int64_t scan_entries(int64_t NT) {
+  return NT + (NT + kSpan - 1) / kSpan + (NT + kSpan * kSpan - 1) / (kSpan * kSpan);
+}
+// the ticket, then the entries (channels rounded up to the wider of the two tiles)
+static size_t scan_ws(int64_t B, int64_t L, int64_t ds) {
+  const int64_t NT = (L + kStateRows - 1) / kStateRows;
+  if (B < 1 || ds < 1 || NT < 2) return 0;
+  return 16 + (size_t)(B * ((ds + 63) / 64 * 64)) * scan_entries(NT) * 8;
+}
+static void scan_plan(ScanParams& p, int CW, void* ws) {
+  p.nch = (p.ds + CW - 1) / CW;
+  p.NG = p.B * p.nch;
+  p.ntiles = (int64_t)p.NG * p.NT;
+  p.nent = (int)scan_entries(p.NT);
+  p.ticket = p.NT > 1 ? static_cast<unsigned*>(ws) : nullptr;
+  p.ent = p.NT > 1 ? reinterpret_cast<uint64_t*>(static_cast<char*>(ws) + 16) : nullptr;
+}
+static int scan_clear(const ScanParams& p, cudaStream_t s, const char* what) {
+  if (!p.ticket) return 0;
+  const cudaError_t e = cudaMemsetAsync(p.ticket, 0xff, scan_ws(p.B, p.L, p.ds), s);
+  return e == cudaSuccess ? 0 : fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+}
+template <typename T, bool RESET, int CB>
+static void scan_fwd_launch(const ScanParams& p, cudaStream_t s) {
+  constexpr int smem = 2 * kWarps * 3 * kRows * 128;
+  auto k = gated_scan_fwd_kernel<T, RESET, CB>;
+  cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const int64_t most = (int64_t)num_sms() * 4;
+  k<<<(unsigned)(p.ntiles < most ? p.ntiles : most), kWarps * 32, smem, s>>>(p);
+}
+template <typename T>
+static void scan_fwd_launch(const ScanParams& p, int cb, cudaStream_t s) {
+  constexpr int least = sizeof(T) == 4 ? 4 : 0;  // fp32 rows always allow 4 bytes
+  if (cb == 16) p.reset ? scan_fwd_launch<T, true, 16>(p, s) : scan_fwd_launch<T, false, 16>(p, s);
+  else if (cb == 4) p.reset ? scan_fwd_launch<T, true, 4>(p, s) : scan_fwd_launch<T, false, 4>(p, s);
+  else p.reset ? scan_fwd_launch<T, true, least>(p, s) : scan_fwd_launch<T, false, least>(p, s);
+}
+
 }  // namespace hdc
 
 using namespace hdc;
@@ -156,20 +625,35 @@ extern "C" int hdc_gated_scan_fwd(int dtype, int a_dtype, const void* projs, int
       off_type(h_last, HDC_F32) || off_type(states, HDC_F32))
     return fail(HDC_E_ALIGN, "gated_scan: a pointer is not aligned to its type");
   if (y_st < ds && L > 1) return fail(HDC_E_SHAPE, "gated_scan: y rows overlap (y_st=%lld)", (long long)y_st);
-  if (workspace_bytes < hdc_gated_scan_workspace_bytes(B, L, ds))
-    return fail(HDC_E_WORKSPACE, "gated_scan: workspace of %zu bytes is too small", workspace_bytes);
+  const size_t need = scan_ws(B, L, ds);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(HDC_E_WORKSPACE, "gated_scan: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  if (!aligned16(workspace)) return fail(HDC_E_ALIGN, "gated_scan: the workspace is not 16-byte aligned");
+  if (B * ((ds + 31) / 32) > (int64_t(1) << 30) || B * ((ds + 31) / 32) * ((L + kStateRows - 1) / kStateRows) > (int64_t(1) << 31))
+    return fail(HDC_E_SHAPE, "gated_scan: B=%lld x L=%lld x d_state=%lld is too large", (long long)B, (long long)L, (long long)ds);
   ScanParams p{};
   p.projs = projs; p.psb = proj_sb; p.pst = proj_st; p.A_log = A_log; p.a_bf16 = a_dtype == HDC_BF16;
   p.h0 = h0; p.reset = reset; p.y = y; p.ysb = y_sb; p.yst = y_st; p.h_last = h_last; p.states = states;
   p.B = (int)B; p.L = (int)L; p.ds = (int)ds; p.NT = (int)((L + kStateRows - 1) / kStateRows);
   auto s = reinterpret_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)((B * ds + 127) / 128);
-  if (dtype == HDC_F32) gated_scan_fwd_kernel<float><<<grid, 128, 0, s>>>(p);
-  else gated_scan_fwd_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(p);
+  if (L == 0) {  // nothing to scan: the state stays as it is
+    if (!h_last) return HDC_OK;
+    const cudaError_t e = h0 ? cudaMemcpyAsync(h_last, h0, (size_t)B * ds * 4, cudaMemcpyDeviceToDevice, s)
+                             : cudaMemsetAsync(h_last, 0, (size_t)B * ds * 4, s);
+    return e == cudaSuccess ? HDC_OK : fail((int)e, "gated_scan: %s", cudaGetErrorString(e));
+  }
+  const int es = dtype == HDC_F32 ? 4 : 2;
+  scan_plan(p, 128 / es, workspace);
+  p.out_vec = rows_allow(y, y_sb, y_st, es, 4);
+  if (int e = scan_clear(p, s, "gated_scan")) return e;
+  const int cb = rows_allow(projs, proj_sb, proj_st, es, 16) && ds * es % 16 == 0 ? 16
+                 : rows_allow(projs, proj_sb, proj_st, es, 4) && ds * es % 4 == 0 ? 4 : 0;
+  if (dtype == HDC_F32) scan_fwd_launch<float>(p, cb, s);
+  else scan_fwd_launch<__nv_bfloat16>(p, cb, s);
   return launch_status("gated_scan_fwd_kernel");
 }
 
-extern "C" size_t hdc_gated_scan_workspace_bytes(int64_t B, int64_t L, int64_t ds) { return 0; }
+extern "C" size_t hdc_gated_scan_workspace_bytes(int64_t B, int64_t L, int64_t ds) { return scan_ws(B, L, ds); }
 
 extern "C" size_t hdc_gated_scan_bwd_workspace_bytes(int64_t B, int64_t L, int64_t ds) {
   if (B < 1 || L < 0 || ds < 1) return 0;
