@@ -37,6 +37,10 @@ namespace hdc {
 constexpr int kStateRows = 64;       // rows per tile = rows per saved state
 constexpr int kWarps = 8, kRows = 8;  // warps per tile, steps per warp
 constexpr int kSpan = 16;            // tiles per span, spans per chain link
+#ifndef FC
+#define FC 4
+#endif
+constexpr int kFwdCtas = FC;          // resident forward CTAs per SM
 static_assert(kWarps * kRows == kStateRows, "a tile is one state interval");
 
 struct ScanParams {
@@ -120,6 +124,9 @@ __device__ __forceinline__ uint32_t f_word(const Fv<2>& a) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a.v[0], a.v[1]);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// a word of dt = -inf
+__device__ __forceinline__ uint32_t no_step(float) { return 0xff800000u; }
+__device__ __forceinline__ uint32_t no_step(__nv_bfloat16) { return 0xff80ff80u; }
 // store a word of channels c, c+1, ... (< ds); vec: the row allows the whole word
 template <typename T>
 __device__ __forceinline__ void st_word(T* row, int c, int ds, int vec, const Fv<kVec<T>>& v) {
@@ -154,8 +161,22 @@ __device__ __forceinline__ void gates(const Fv<2>& x, const Fv<2>&, const Fv<2>&
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     e.v[i] = ex2(-1.4426950408889634f * fabsf(x.v[i]));
-    m.v[i] = x.v[i] < 0.f ? 0.f : x.v[i];  // not fmaxf: NaN stays NaN
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(m.v[i]) : "f"(x.v[i]));  // NaN stays NaN
   }
+#ifdef SCALARP
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float q = -0.008539206348359585f, z = e.v[i];
+    q = fmaf(q, z, 0.04408962279558182f);
+    q = fmaf(q, z, -0.10768169909715652f);
+    q = fmaf(q, z, 0.17745240032672882f);
+    q = fmaf(q, z, -0.24495463073253632f);
+    q = fmaf(q, z, 0.33275479078292847f);
+    q = fmaf(q, z, -0.4999740421772003f);
+    q = fmaf(q, z, 0.9999998211860657f);
+    d.v[i] = fmaf(q, z, m.v[i]);
+  }
+#else
   Fv<2> p = all<2>(-0.008539206348359585f);
   p = fma(p, e, all<2>(0.04408962279558182f));
   p = fma(p, e, all<2>(-0.10768169909715652f));
@@ -165,6 +186,7 @@ __device__ __forceinline__ void gates(const Fv<2>& x, const Fv<2>&, const Fv<2>&
   p = fma(p, e, all<2>(-0.4999740421772003f));
   p = fma(p, e, all<2>(0.9999998211860657f));
   d = fma(p, e, m);
+#endif
   const Fv<2> l = d * A2;
   a.v[0] = ex2(l.v[0]);
   a.v[1] = ex2(l.v[1]);
@@ -173,33 +195,37 @@ __device__ __forceinline__ void gates(const Fv<2>& x, const Fv<2>&, const Fv<2>&
 // ---------------------------------------------------------------- maps h -> P h + H
 template <int V> struct Map { Fv<V> P, H; };
 template <int V> __device__ __forceinline__ Map<V> identity_map() { return {all<V>(1.f), all<V>(0.f)}; }
-// m applied to a state
-template <int V> __device__ __forceinline__ Fv<V> apply(const Map<V>& m, const Fv<V>& h) {
+// m applied to a state (RESET: maps may be cut off)
+template <bool RESET, int V> __device__ __forceinline__ Fv<V> apply(const Map<V>& m, const Fv<V>& h) {
   Fv<V> r = fma(m.P, h, m.H);
+  if (RESET) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = m.P.v[i] < 0.f ? m.H.v[i] : r.v[i];
+    for (int i = 0; i < V; ++i) r.v[i] = m.P.v[i] < 0.f ? m.H.v[i] : r.v[i];
+  }
   return r;
 }
 // first m, then n
-template <int V> __device__ __forceinline__ Map<V> then(const Map<V>& m, const Map<V>& n) {
+template <bool RESET, int V> __device__ __forceinline__ Map<V> then(const Map<V>& m, const Map<V>& n) {
   Map<V> r;
-  r.H = apply(n, m.H);
+  r.H = apply<RESET>(n, m.H);
   r.P = m.P * n.P;
+  if (RESET) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) r.P.v[i] = (m.P.v[i] < 0.f || n.P.v[i] < 0.f) ? -1.f : r.P.v[i];
+    for (int i = 0; i < V; ++i) r.P.v[i] = (m.P.v[i] < 0.f || n.P.v[i] < 0.f) ? -1.f : r.P.v[i];
+  }
   return r;
 }
 // a lane's map in shared memory: 8 bytes per channel
 template <int V> __device__ __forceinline__ void st_map(char* p, int lane, const Map<V>& m) {
   float* f = reinterpret_cast<float*>(p) + lane * 2 * V;
-  if constexpr (V == 2) *reinterpret_cast<float4*>(f) = make_float4(m.P.v[0], m.H.v[0], m.P.v[1], m.H.v[1]);
+  if constexpr (V == 2) *reinterpret_cast<float4*>(f) = make_float4(m.P.v[0], m.P.v[1], m.H.v[0], m.H.v[1]);
   else *reinterpret_cast<float2*>(f) = make_float2(m.P.v[0], m.H.v[0]);
 }
 template <int V> __device__ __forceinline__ Map<V> ld_map(const char* p, int lane) {
   const float* f = reinterpret_cast<const float*>(p) + lane * 2 * V;
   if constexpr (V == 2) {
     const float4 q = *reinterpret_cast<const float4*>(f);
-    return {{{q.x, q.z}}, {{q.y, q.w}}};
+    return {{{q.x, q.y}}, {{q.z, q.w}}};
   } else {
     const float2 q = *reinterpret_cast<const float2*>(f);
     return {{{q.x}}, {{q.y}}};
@@ -209,79 +235,78 @@ template <int V> __device__ __forceinline__ Map<V> ld_map(const char* p, int lan
 // ---------------------------------------------------------------- published entries
 constexpr uint32_t kUnset = 0xffffffffu;  // P of a word that is not published
 template <int V> __device__ __forceinline__ void publish(uint64_t* e, int lane, const Map<V>& m) {
+  uint64_t w[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     uint32_t P = __float_as_uint(m.P.v[i]);
     if (P == kUnset) P = 0x7fffffffu;  // a NaN stays one
-    const uint64_t w = ((uint64_t)__float_as_uint(m.H.v[i]) << 32) | P;
-    asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(e + lane * V + i), "l"(w) : "memory");
+    w[i] = ((uint64_t)__float_as_uint(m.H.v[i]) << 32) | P;
   }
+  if constexpr (V == 2)
+    asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(e + lane * 2), "l"(w[0]), "l"(w[1]) : "memory");
+  else asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(e + lane), "l"(w[0]) : "memory");
 }
-__device__ __forceinline__ uint64_t ld_entry(const uint64_t* e) {
-  uint64_t w;
-  asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(w) : "l"(e) : "memory");
-  return w;
+__device__ __forceinline__ void ld_entry(const uint64_t* e, uint64_t (&w)[1]) {
+  asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(w[0]) : "l"(e) : "memory");
 }
-// Compose n <= 4 neighbouring entries, each waited for (2 s in all, then error 61 and zeros).
-template <int V> __device__ __forceinline__ Map<V> take(const uint64_t* e, int n, int lane) {
+__device__ __forceinline__ void ld_entry(const uint64_t* e, uint64_t (&w)[2]) {
+  asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(w[0]), "=l"(w[1]) : "l"(e) : "memory");
+}
+// Compose n in 1..4 neighbouring entries, waited for (some 2 s, then error 61; what is missing
+// then counts as zeros).  e: entry 0 of them, ch: the lane's first channel.  While an entry is
+// missing, one word of each is polled, not the whole entries.
+constexpr long long kWaitCycles = 4000000000ll;
+template <bool RESET, int V> __device__ __forceinline__ Map<V> take(const uint64_t* e, int ch, int n, int lane) {
   uint64_t w[4][V];
-  uint64_t t0 = 0;
-  bool late = false;
+  long long t0 = 0;
   while (true) {
     bool ok = true;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
+      if (k < n) ld_entry(e + (int64_t)k * 32 * V + ch, w[k]);
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (k < n) {
-          w[k][i] = ld_entry(e + (int64_t)k * 32 * V + lane * V + i);
-          ok = ok && (uint32_t)w[k][i] != kUnset;
-        }
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) ok = ok && (k >= n || (uint32_t)w[k][i] != kUnset);
     if (__all_sync(0xffffffffu, ok)) break;
-    const uint64_t now = globaltimer_ns();
-    if (t0 == 0) t0 = now;
-    late = now - t0 > 2000000000ull;
+    if (t0 == 0) t0 = clock64();
+    bool late = false;
+    if (lane < n) {
+      uint64_t one[1];
+      do {
+        __nanosleep(32);
+        ld_entry(e + (int64_t)lane * 32 * V, one);
+        late = clock64() - t0 > kWaitCycles;
+      } while ((uint32_t)one[0] == kUnset && !late);
+    }
     if (__any_sync(0xffffffffu, late)) {
       if (lane == 0) atomicCAS(&g_dev_error, 0, 61);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if ((uint32_t)w[k][i] == kUnset) w[k][i] = 0;
       break;
     }
   }
-  Map<V> m = identity_map<V>();
+  Map<V> m;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (k < n) {
       Map<V> q;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const bool set = (uint32_t)w[k][i] != kUnset;
-        q.P.v[i] = set ? __uint_as_float((uint32_t)w[k][i]) : 0.f;
-        q.H.v[i] = set ? __uint_as_float((uint32_t)(w[k][i] >> 32)) : 0.f;
+        q.P.v[i] = __uint_as_float((uint32_t)w[k][i]);
+        q.H.v[i] = __uint_as_float((uint32_t)(w[k][i] >> 32));
       }
-      m = then(m, q);
+      m = k == 0 ? q : then<RESET>(m, q);
     }
   return m;
 }
-// Entry indices of a group: tiles, then spans of 16 tiles, then links of 16 spans.
+// Entries of a group: tiles, then spans of 16 tiles, then links of 16 spans (P unused, H the
+// state itself).
 __device__ __forceinline__ int span_at(int NT, int k) { return NT + k; }
 __device__ __forceinline__ int link_at(int NT, int k) { return NT + (NT + kSpan - 1) / kSpan + k; }
-
-// This warp's part of what precedes tile q of its group: warps 0..3 compose the link and the
-// whole spans (up to 16 entries), warps 4..7 the tiles of the span that q is in (up to 15).
-template <int V>
-__device__ __forceinline__ Map<V> before_tile(const uint64_t* ent, int NT, int q, int warp, int lane) {
-  constexpr int CW = 32 * V;
-  if (warp >= 4) {
-    const int n = min(4, q % kSpan - (warp - 4) * 4);
-    if (n <= 0) return identity_map<V>();
-    return take<V>(ent + (int64_t)(q - q % kSpan + (warp - 4) * 4) * CW, n, lane);
-  }
-  const int link = q / (kSpan * kSpan), s0 = link * kSpan, ns = q / kSpan - s0;
-  Map<V> m = identity_map<V>();
-  if (warp == 0 && link > 0) m = take<V>(ent + (int64_t)link_at(NT, link - 1) * CW, 1, lane);
-  const int n = min(4, ns - warp * 4);
-  if (n > 0) m = then(m, take<V>(ent + (int64_t)span_at(NT, s0 + warp * 4) * CW, n, lane));
-  return m;
-}
 
 // ---------------------------------------------------------------- staging
 __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool ok, std::integral_constant<int, 16>) {
@@ -290,117 +315,131 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool ok,
 __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool ok, std::integral_constant<int, 4>) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
 }
-// The warp's 8 rows of 128 bytes from base (row stride st elements), rows >= nv and channels >=
-// nc as zeros.  CB: bytes per copy (rows allow 16 or 4), 0: element by element, not asynchronous.
-template <typename T, int CB>
-__device__ __forceinline__ void stage_rows(char* dst, const T* base, int64_t st, int nv, int nc, int lane) {
-  if constexpr (CB == 0) {
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      T v[kVec<T>];
-#pragma unroll
-      for (int i = 0; i < kVec<T>; ++i) {
-        const int c = lane * kVec<T> + i;
-        v[i] = r < nv && c < nc ? base[r * st + c] : from_f<T>(0.f);
-      }
-#pragma unroll
-      for (int i = 0; i < kVec<T>; ++i) reinterpret_cast<T*>(dst + r * 128)[lane * kVec<T> + i] = v[i];
-    }
-  } else {
-    constexpr int per_row = 128 / CB, rows = 32 / per_row;  // rows per warp-wide copy
-    const int r0 = lane / per_row, x = lane % per_row;
-    const bool in = x * (CB / (int)sizeof(T)) < nc;
-    const uint32_t d = smem_u32(dst) + r0 * 128 + x * CB;
-    const char* s = reinterpret_cast<const char*>(base) + x * CB;
-#pragma unroll
-    for (int k = 0; k < kRows / rows; ++k) {
-      const bool ok = in && r0 + k * rows < nv;
-      cp_async(d + k * rows * 128, ok ? s + (r0 + k * rows) * st * (int64_t)sizeof(T) : reinterpret_cast<const char*>(base),
-               ok, std::integral_constant<int, CB>());
-    }
-  }
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
-struct Tile {
-  int q, g, b, c0;  // index in time, group, batch, first channel
+// Copies of one warp's 8 rows of 128 bytes of a tile, rows >= nv and channels >= nc as zeros.
+// CB: bytes per copy (16 or 4, as the rows allow), or 0: element by element, not asynchronous.
+template <typename T, int CB> struct Rows {
+  static constexpr int kPer = CB ? 128 / CB : 32, kAt = 32 / kPer, kN = kRows / kAt;
+  uint32_t dst;   // the lane's place in a region
+  int r0, x;      // its first row and first byte of the rows
+  __device__ explicit Rows(int lane) : r0(lane / kPer), x(lane % kPer * (CB ? CB : 4)) { dst = r0 * 128 + x; }
+  // tile: the tile's first element; row0: the warp's first row in it; st: row stride (elements);
+  // `arrays` consecutive regions, their sources `apart` elements from each other
+  template <int arrays>
+  __device__ __forceinline__ void copy(char* region, const T* tile, int row0, int64_t st, int64_t apart, int nv,
+                                       int nc) const {
+    if constexpr (CB == 0) {
+      const int c = x / (int)sizeof(T);
+#pragma unroll
+      for (int k = 0; k < arrays; ++k)
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+          for (int i = 0; i < kVec<T>; ++i)
+            reinterpret_cast<T*>(region + (k * kRows + r) * 128)[c + i] =
+                r < nv && c + i < nc ? tile[k * apart + (row0 + r) * st + c + i] : from_f<T>(0.f);
+    } else {
+      const uint32_t d = smem_u32(region) + dst;
+      const bool in = x < nc * (int)sizeof(T);
+      const char* src[kN];
+      bool ok[kN];
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        ok[i] = in && r0 + i * kAt < nv;
+        src[i] = reinterpret_cast<const char*>(tile) + (ok[i] ? (row0 + r0 + i * kAt) * st * (int64_t)sizeof(T) + x : 0);
+      }
+#pragma unroll
+      for (int k = 0; k < arrays; ++k)
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+          cp_async(d + (k * kRows + i * kAt) * 128, src[i] + k * apart * (int64_t)sizeof(T), ok[i],
+                   std::integral_constant<int, CB>());
+    }
+  }
 };
+
+// A tile as broadcast through shared memory: index in time, group, batch, first channel; q < 0: none
+using Tile = int4;
 template <typename T> __device__ __forceinline__ Tile tile_of(const ScanParams& p, int64_t id) {
-  Tile t;
-  t.q = (int)(id / p.NG);
-  t.g = (int)(id - (int64_t)t.q * p.NG);
-  t.b = t.g / p.nch;
-  t.c0 = (t.g - t.b * p.nch) * kCW<T>;
-  return t;
+  if (id >= p.ntiles) return make_int4(-1, 0, 0, 0);
+  const unsigned q = (unsigned)id / (unsigned)p.NG, g = (unsigned)id - q * p.NG, b = g / (unsigned)p.nch;
+  return make_int4((int)q, (int)g, (int)b, (int)(g - b * p.nch) * kCW<T>);
 }
 __device__ __forceinline__ int64_t next_tile(const ScanParams& p, int64_t last) {
   if (!p.ticket) return last + gridDim.x;
   return (int64_t)(unsigned)(atomicAdd(p.ticket, 1u) + 1u);  // the counter starts at all ones
 }
-// the warp's reset flags as a mask (bit r: step r of its rows)
-__device__ __forceinline__ uint32_t reset_byte(const ScanParams& p, int b, int t, int nv, int lane) {
-  return lane < nv ? p.reset[(int64_t)b * p.L + t + lane] : 0;
-}
 
 template <typename T, bool RESET, int CB>
-__global__ void __launch_bounds__(kWarps * 32, 4) gated_scan_fwd_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(kWarps * 32, kFwdCtas) gated_scan_fwd_kernel(const __grid_constant__ ScanParams p) {
   constexpr int V = kVec<T>, CW = kCW<T>, kRegion = 3 * kRows * 128;
   extern __shared__ __align__(128) char raw[];  // [2][warp][dt, x, b][row][128 bytes]
-  __shared__ __align__(16) float s_h[CW];
-  __shared__ __align__(16) char s_tile[CW * 8];
-  __shared__ int64_t s_next[2];
+  __shared__ __align__(16) float s_A[2][CW];
+  __shared__ Tile s_next[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int cl = lane * V;  // the lane's first channel of the tile
+  const Rows<T, CB> rows(lane);
+  int64_t id = 0;  // thread 0's
 
-  // what a lane holds for a staged tile besides the copies
-  struct Ahead { float A[V]; uint32_t rb; };
-  auto stage = [&](const Tile& t, char* buf, Ahead& n) {
-    const int t0 = t.q * kStateRows + warp * kRows;
-    const int nv = min(kRows, p.L - t0), nc = p.ds - t.c0;
-    const T* in = static_cast<const T*>(p.projs) + t.b * p.psb + t0 * p.pst + t.c0;
-    char* reg = buf + warp * kRegion;
-#pragma unroll
-    for (int k = 0; k < 3; ++k) stage_rows<T, CB>(reg + k * kRows * 128, in + k * p.ds, p.pst, nv, nc, lane);
+  uint32_t rb = 0;  // the staged tile's reset flag of step `lane` of the warp
+  auto stage = [&](const Tile& t, int s) {
+    const int t0 = t.x * kStateRows, nv = p.L - t0 - warp * kRows, nc = p.ds - t.w;
+    const T* tile = static_cast<const T*>(p.projs) + t.z * p.psb + t0 * p.pst + t.w;
+    rows.template copy<3>(raw + (s * kWarps + warp) * kRegion, tile, warp * kRows, p.pst, p.ds, nv, nc);
     cp_commit();
+    if (RESET) rb = lane < min(nv, kRows) ? p.reset[(int64_t)t.z * p.L + t0 + warp * kRows + lane] : 0;
+    if (warp == 3) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) n.A[i] = cl + i < nc ? ld_param(p.A_log, p.a_bf16, t.c0 + cl + i) : 0.f;
-    if (RESET) n.rb = reset_byte(p, t.b, t0, nv, lane);
+      for (int i = 0; i < V; ++i) s_A[s][cl + i] = cl + i < nc ? -expf(ld_param(p.A_log, p.a_bf16, t.w + cl + i)) : 0.f;
+    }
   };
 
-  if (threadIdx.x == 0) s_next[0] = p.ticket ? next_tile(p, 0) : blockIdx.x;
+  if (threadIdx.x == 0) {
+    id = p.ticket ? next_tile(p, 0) : blockIdx.x;
+    s_next[0] = tile_of<T>(p, id);
+  }
   __syncthreads();
-  int64_t id = s_next[0];
-  Ahead ahead = {};
-  int s = 0;
-  if (id < p.ntiles) stage(tile_of<T>(p, id), raw, ahead);
-  for (; id < p.ntiles; s ^= 1) {
-    const Tile t = tile_of<T>(p, id);
-    if (threadIdx.x == 0) s_next[s ^ 1] = next_tile(p, id);
+  Tile t = s_next[0];
+  if (t.x >= 0) stage(t, 0);
+  __syncthreads();
+  bool first = true;
+  for (int s = 0; t.x >= 0; s ^= 1) {
+    // The next ticket, early enough to stage its tile below.  The first time only after the loads:
+    // a CTA that starts early would else take two neighbouring tiles, and the tiles after
+    // the second one would wait until it is done with the first.
+    if (first) cp_wait_all();
+    first = false;
+    if (threadIdx.x == 0) {
+      id = next_tile(p, id);
+      s_next[s ^ 1] = tile_of<T>(p, id);
+    }
     char* buf = raw + s * kWarps * kRegion;
     char* mine = buf + warp * kRegion;
-    const int t0 = t.q * kStateRows + warp * kRows, nv = min(kRows, p.L - t0);
-    Fv<V> A, A2;
+    const int t0 = t.x * kStateRows + warp * kRows, nv = p.L - t0, nc = p.ds - t.w;
+    const uint32_t cut = RESET ? __ballot_sync(0xffffffffu, rb != 0) : 0;
+    Fv<V> A;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      A.v[i] = -expf(ahead.A[i]);
-      A2.v[i] = A.v[i] * 1.4426950408889634f;
-    }
-    const uint32_t cut = RESET ? __ballot_sync(0xffffffffu, ahead.rb != 0) : 0;
+    for (int i = 0; i < V; ++i) A.v[i] = s_A[s][cl + i];
+    const Fv<V> A2 = A * all<V>(1.4426950408889634f);
     cp_wait_all();
     __syncwarp();
+    if (nv < kRows) {  // steps past the end: dt = -inf (and x = b = 0) is the identity, a = 1, u = 0
+      for (int r = max(nv, 0); r < kRows; ++r) reinterpret_cast<uint32_t*>(mine + r * 128)[lane] = no_step(T());
+    }
 
     // local scan of the warp's steps from a zero state
     Fv<V> a[kRows], u[kRows];
     Map<V> m = identity_map<V>();
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(mine) + lane;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(mine + r * 128) + lane;
-      const Fv<V> dt = word_f(w[0], T()), x = word_f(w[kRows * 32], T()), b = word_f(w[2 * kRows * 32], T());
+      const Fv<V> dt = word_f(w[r * 32], T()), x = word_f(w[(kRows + r) * 32], T());
+      const Fv<V> b = word_f(w[(2 * kRows + r) * 32], T());
       Fv<V> d;
-      // past the end the staged zeros give u = 0, and A = 0 gives a = 1: the identity
-      gates(dt, r < nv ? A : all<V>(0.f), r < nv ? A2 : all<V>(0.f), d, a[r]);
-      u[r] = d * b * x;
+      gates(dt, A, A2, d, a[r]);
+      u[r] = d * (b * x);
       if (RESET && ((cut >> r) & 1)) {
         m.H = u[r];
         m.P = all<V>(-1.f);
@@ -413,75 +452,82 @@ __global__ void __launch_bounds__(kWarps * 32, 4) gated_scan_fwd_kernel(const Sc
     st_map<V>(mine, lane, m);
     __syncthreads();
 
-    const int64_t nid = s_next[s ^ 1];
-    if (nid < p.ntiles) stage(tile_of<T>(p, nid), raw + (s ^ 1) * kWarps * kRegion, ahead);
+    const Tile nt = s_next[s ^ 1];
+    if (nt.x >= 0) stage(nt, s ^ 1);
 
     // the tile's map, published; then the state entering the tile
     Fv<V> h;
+#pragma unroll
+    for (int i = 0; i < V; ++i) h.v[i] = p.h0 && cl + i < nc ? p.h0[(int64_t)t.z * p.ds + t.w + cl + i] : 0.f;
     if (p.ticket) {
-      uint64_t* ent = p.ent + (int64_t)t.g * p.nent * CW;
+      uint64_t* ent = p.ent + (int64_t)t.y * p.nent * CW;
+      const int in_span = t.x % kSpan, span = t.x / kSpan, link = span / kSpan, in_link = span % kSpan;
+      Map<V> tile_map;
       if (warp == 0) {
-        Map<V> all8 = ld_map<V>(buf, lane);
+        tile_map = ld_map<V>(buf, lane);
 #pragma unroll
-        for (int k = 1; k < kWarps; ++k) all8 = then(all8, ld_map<V>(buf + k * kRegion, lane));
-        if (t.q + 1 < p.NT) publish<V>(ent + (int64_t)t.q * CW, lane, all8);
-        st_map<V>(s_tile, lane, all8);
+        for (int k = 1; k < kWarps; ++k) tile_map = then<RESET>(tile_map, ld_map<V>(buf + k * kRegion, lane));
+        if (t.x + 1 < p.NT) publish<V>(ent + (int64_t)t.x * CW, lane, tile_map);
       }
-      st_map<V>(mine + 512, lane, before_tile<V>(ent, p.NT, t.q, warp, lane));
-      __syncthreads();
-      if (warp == 0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int c = t.c0 + cl + i;
-          h.v[i] = p.h0 && c < p.ds ? p.h0[(int64_t)t.b * p.ds + c] : 0.f;
-        }
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k) h = apply(ld_map<V>(buf + k * kRegion + 512, lane), h);
-#pragma unroll
-        for (int i = 0; i < V; ++i) s_h[cl + i] = h.v[i];
-        if (t.q % (kSpan * kSpan) == kSpan * kSpan - 1 && t.q + 1 < p.NT) {  // the end of a link
-          const Map<V> end = {all<V>(-1.f), apply(ld_map<V>(s_tile, lane), h)};
-          publish<V>(ent + (int64_t)link_at(p.NT, t.q / (kSpan * kSpan)) * CW, lane, end);
-        }
-      } else if (warp == 1 && t.q % kSpan == kSpan - 1 && t.q + 1 < p.NT) {  // the end of a span
-        Map<V> sp = identity_map<V>();
-#pragma unroll
-        for (int k = 4; k < kWarps; ++k) sp = then(sp, ld_map<V>(buf + k * kRegion + 512, lane));
-        publish<V>(ent + (int64_t)span_at(p.NT, t.q / kSpan) * CW, lane, then(sp, ld_map<V>(s_tile, lane)));
+      // warps 0..3 compose the whole spans of the link that the tile is in, warps 4..7 the tiles
+      // of the span that it is in, four entries each
+      const int from = warp % 4 * 4, n = min(4, (warp < 4 ? in_link : in_span) - from);
+      if (n > 0) {
+        const int at = warp < 4 ? span_at(p.NT, link * kSpan + from) : span * kSpan + from;
+        st_map<V>(mine + 512, lane, take<RESET, V>(ent + (int64_t)at * CW, cl, n, lane));
       }
-      __syncthreads();
+      if (in_span == kSpan - 1 && t.x + 1 < p.NT && warp >= 4) {
+        // the end of a span: its map is published before this tile waits for earlier spans, or
+        // each span would wait for the one before
+        named_bar_sync(1, 128);
+        if (warp == 4) {
+          Map<V> sp = ld_map<V>(buf + 4 * kRegion + 512, lane);
 #pragma unroll
-      for (int i = 0; i < V; ++i) h.v[i] = s_h[cl + i];
+          for (int k = 5; k < kWarps; ++k) sp = then<RESET>(sp, ld_map<V>(buf + k * kRegion + 512, lane));
+#pragma unroll
+          for (int k = 0; k < kWarps; ++k) sp = then<RESET>(sp, ld_map<V>(buf + k * kRegion, lane));
+          publish<V>(ent + (int64_t)span_at(p.NT, span) * CW, lane, sp);
+        }
+      }
+      if (link > 0) h = take<false, V>(ent + (int64_t)link_at(p.NT, link - 1) * CW, cl, 1, lane).H;
+      __syncthreads();
+      const int outer = (in_link + 3) / 4, inner = (in_span + 3) / 4;
+      for (int k = 0; k < outer; ++k) h = apply<RESET>(ld_map<V>(buf + k * kRegion + 512, lane), h);
+      for (int k = 4; k < 4 + inner; ++k) h = apply<RESET>(ld_map<V>(buf + k * kRegion + 512, lane), h);
+      if (warp == 0 && in_span == kSpan - 1 && in_link == kSpan - 1 && t.x + 1 < p.NT)  // the end of a link
+        publish<V>(ent + (int64_t)link_at(p.NT, link) * CW, lane, {all<V>(0.f), apply<RESET>(tile_map, h)});
     } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = t.c0 + cl + i;
-        h.v[i] = p.h0 && c < p.ds ? p.h0[(int64_t)t.b * p.ds + c] : 0.f;
-      }
+      __syncthreads();
     }
     if (p.states && warp == 0) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = t.c0 + cl + i;
-        if (c < p.ds) p.states[((int64_t)t.b * p.NT + t.q) * p.ds + c] = h.v[i];
-      }
+      for (int i = 0; i < V; ++i)
+        if (cl + i < nc) p.states[((int64_t)t.z * p.NT + t.x) * p.ds + t.w + cl + i] = h.v[i];
     }
-    for (int k = 0; k < warp; ++k) h = apply(ld_map<V>(buf + k * kRegion, lane), h);
+    for (int k = 0; k < warp; ++k) h = apply<RESET>(ld_map<V>(buf + k * kRegion, lane), h);
 
-    T* y = static_cast<T*>(p.y) + t.b * p.ysb + t0 * p.yst + t.c0;
+    T* y = static_cast<T*>(p.y) + t.z * p.ysb + t0 * p.yst + t.w;
+    if (p.out_vec && nv >= kRows && nc >= CW) {
+      char* row = reinterpret_cast<char*>(y + cl);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      h = RESET && ((cut >> r) & 1) ? u[r] : fma(a[r], h, u[r]);
-      if (r < nv) st_word<T>(y + r * p.yst, cl, p.ds - t.c0, p.out_vec, h);
-    }
-    if (p.h_last && t.q == p.NT - 1 && warp == kWarps - 1) {
+      for (int r = 0; r < kRows; ++r) {
+        h = RESET && ((cut >> r) & 1) ? u[r] : fma(a[r], h, u[r]);
+        *reinterpret_cast<uint32_t*>(row) = f_word(h);
+        row += p.yst * (int64_t)sizeof(T);
+      }
+    } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = t.c0 + cl + i;
-        if (c < p.ds) p.h_last[(int64_t)t.b * p.ds + c] = h.v[i];
+      for (int r = 0; r < kRows; ++r) {
+        h = RESET && ((cut >> r) & 1) ? u[r] : fma(a[r], h, u[r]);
+        if (r < nv) st_word<T>(y + r * p.yst, cl, nc, p.out_vec, h);
       }
     }
-    id = nid;
+    if (p.h_last && t.x == p.NT - 1 && warp == kWarps - 1) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (cl + i < nc) p.h_last[(int64_t)t.z * p.ds + t.w + cl + i] = h.v[i];
+    }
+    t = nt;
   }
 }
 
@@ -597,7 +643,7 @@ static void scan_fwd_launch(const ScanParams& p, cudaStream_t s) {
   constexpr int smem = 2 * kWarps * 3 * kRows * 128;
   auto k = gated_scan_fwd_kernel<T, RESET, CB>;
   cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  const int64_t most = (int64_t)num_sms() * 4;
+  const int64_t most = (int64_t)num_sms() * kFwdCtas;
   k<<<(unsigned)(p.ntiles < most ? p.ntiles : most), kWarps * 32, smem, s>>>(p);
 }
 template <typename T>
