@@ -10,11 +10,11 @@
 // (c_t = s_t = 0 where t is a reset.)  All arithmetic is in fp32; only y and dprojs are
 // rounded, once, to the activation type.
 //
-// Forward schedule (bound by HBM: 3 values read and 1 written per step and channel): the
-// sequence is cut into tiles of 64 steps x 128 bytes of channels (64 bf16, 32 fp32).  A step is
-// the map h -> a h + u, and maps compose: (P, H) then (P', H') is (P' P, P' H + H'), so each
+// Schedule of the scans (bound by HBM: 3 values read and 1 written per step and channel forward,
+// 4 and 3 backward).  The sequence is cut into tiles of 64 steps x a few dozen channels.  A step
+// is the map h -> a h + u, and maps compose: (P, H) then (P', H') is (P' P, P' H + H'), so each
 // tile is scanned from a zero state, and the state entering it is added afterwards through P:
-//   * a warp owns 8 steps of the tile, a lane one 4-byte word of channels; its a and u stay in
+//   * a warp owns 8 steps of the tile, a lane a few neighbouring channels; its a and u stay in
 //     registers between the local scan and the outputs, so every input is read once;
 //   * the 8 warps' maps are composed through shared memory, and the tile's map is published in
 //     the workspace;
@@ -22,6 +22,8 @@
 //     the end of the last whole 256 tiles, the maps of the whole 16-tile spans after it, and the
 //     maps of the tiles after those.  Which entries is a matter of the tile's index alone, so
 //     the result does not depend on timing.
+// The gradient is the same scan from the end, of the maps c -> a (dy + c), on the same tiles;
+// the states inside a tile are scanned again from the one that the forward saved at its start.
 // CTAs take tiles by ticket, time-major: a tile waits only for tiles with smaller tickets,
 // which running CTAs hold, so the waits end (they are bounded all the same).  An entry is one
 // 64-bit word per channel, (P, H); the workspace is set to all ones before the launch, which
@@ -37,10 +39,6 @@ namespace hdc {
 constexpr int kStateRows = 64;       // rows per tile = rows per saved state
 constexpr int kWarps = 8, kRows = 8;  // warps per tile, steps per warp
 constexpr int kSpan = 16;            // tiles per span, spans per chain link
-#ifndef FC
-#define FC 4
-#endif
-constexpr int kFwdCtas = FC;          // resident forward CTAs per SM
 static_assert(kWarps * kRows == kStateRows, "a tile is one state interval");
 
 struct ScanParams {
@@ -53,7 +51,8 @@ struct ScanParams {
   const void* dy; int64_t dsb, dst;
   const float* dh_last;
   void* dprojs; int64_t gsb, gst;
-  float* dA_part; float* dh0; float* hbuf;
+  float* dA_part;   // [NT][NG][CW]: each tile's sum of s d
+  float* dh0;
   int B, L, ds, NT;
   // tiles
   int nch;          // channel groups
@@ -62,7 +61,8 @@ struct ScanParams {
   unsigned* ticket;  // NULL: a single tile in time, taken by block index, nothing published
   uint64_t* ent;    // [NG][NT + spans + links][CW] published entries
   int nent;         // entries per group
-  int out_vec;      // the outputs' rows allow whole words
+  int CW;           // channels per tile
+  int out_vec;      // the outputs' rows allow whole lanes
 };
 
 __device__ __forceinline__ float ld_param(const void* p, int bf16, int i) {
@@ -72,42 +72,63 @@ __device__ __forceinline__ float ld_param(const void* p, int bf16, int i) {
 // softplus with the Block's threshold (hdcmamba/model.py:192), exact for small exp(x) too
 __device__ __forceinline__ float softplus_acc(float x) { return x > 20.0f ? x : log1pf(expf(x)); }
 
-// ---------------------------------------------------------------- one word of channels
-// The channels of a lane: one fp32 value, or two bf16 values computed as a pair
-// (fma.rn.f32x2 and friends: two fp32 operations per issued instruction).
+// ---------------------------------------------------------------- a lane's channels
+// V neighbouring channels of a lane: W words of 4 bytes (fp32: V = W, bf16: V = 2 W), computed
+// as pairs where V is even (fma.rn.f32x2 and friends: two fp32 operations per issued instruction).
 template <int V> struct Fv { float v[V]; };
-template <typename T> constexpr int kVec = 4 / sizeof(T);
-template <typename T> constexpr int kCW = 32 * kVec<T>;  // channels per tile
+template <typename T, int W> constexpr int kV = W * 4 / (int)sizeof(T);
 
-__device__ __forceinline__ uint64_t f2_bits(const Fv<2>& a) {
+__device__ __forceinline__ uint64_t pair_bits(float a, float b) {
   uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.v[0]), "f"(a.v[1]));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ Fv<2> bits_f2(uint64_t b) {
-  Fv<2> r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.v[0]), "=f"(r.v[1]) : "l"(b));
-  return r;
+__device__ __forceinline__ void bits_pair(uint64_t r, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
 }
-__device__ __forceinline__ Fv<1> fma(const Fv<1>& a, const Fv<1>& b, const Fv<1>& c) {
-  return {{fmaf(a.v[0], b.v[0], c.v[0])}};
+template <int V> __device__ __forceinline__ Fv<V> fma(const Fv<V>& a, const Fv<V>& b, const Fv<V>& c) {
+  Fv<V> o;
+  if constexpr (V == 1) {
+    o.v[0] = fmaf(a.v[0], b.v[0], c.v[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      uint64_t r;
+      asm("fma.rn.f32x2 %0, %1, %2, %3;"
+          : "=l"(r)
+          : "l"(pair_bits(a.v[i], a.v[i + 1])), "l"(pair_bits(b.v[i], b.v[i + 1])), "l"(pair_bits(c.v[i], c.v[i + 1])));
+      bits_pair(r, o.v[i], o.v[i + 1]);
+    }
+  }
+  return o;
 }
-__device__ __forceinline__ Fv<1> operator*(const Fv<1>& a, const Fv<1>& b) { return {{a.v[0] * b.v[0]}}; }
-__device__ __forceinline__ Fv<1> operator+(const Fv<1>& a, const Fv<1>& b) { return {{a.v[0] + b.v[0]}}; }
-__device__ __forceinline__ Fv<2> fma(const Fv<2>& a, const Fv<2>& b, const Fv<2>& c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
-  return bits_f2(r);
+template <int V> __device__ __forceinline__ Fv<V> operator*(const Fv<V>& a, const Fv<V>& b) {
+  Fv<V> o;
+  if constexpr (V == 1) {
+    o.v[0] = a.v[0] * b.v[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      uint64_t r;
+      asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a.v[i], a.v[i + 1])), "l"(pair_bits(b.v[i], b.v[i + 1])));
+      bits_pair(r, o.v[i], o.v[i + 1]);
+    }
+  }
+  return o;
 }
-__device__ __forceinline__ Fv<2> operator*(const Fv<2>& a, const Fv<2>& b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
-  return bits_f2(r);
-}
-__device__ __forceinline__ Fv<2> operator+(const Fv<2>& a, const Fv<2>& b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
-  return bits_f2(r);
+template <int V> __device__ __forceinline__ Fv<V> operator+(const Fv<V>& a, const Fv<V>& b) {
+  Fv<V> o;
+  if constexpr (V == 1) {
+    o.v[0] = a.v[0] + b.v[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      uint64_t r;
+      asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a.v[i], a.v[i + 1])), "l"(pair_bits(b.v[i], b.v[i + 1])));
+      bits_pair(r, o.v[i], o.v[i + 1]);
+    }
+  }
+  return o;
 }
 template <int V> __device__ __forceinline__ Fv<V> all(float x) {
   Fv<V> r;
@@ -115,29 +136,54 @@ template <int V> __device__ __forceinline__ Fv<V> all(float x) {
   for (int i = 0; i < V; ++i) r.v[i] = x;
   return r;
 }
-__device__ __forceinline__ Fv<1> word_f(uint32_t w, float) { return {{__uint_as_float(w)}}; }
-__device__ __forceinline__ Fv<2> word_f(uint32_t w, __nv_bfloat16) {
-  return {{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)}};
+// a lane's channels from and to its words
+template <typename T, int W> __device__ __forceinline__ Fv<kV<T, W>> ld_words(const char* p) {
+  uint32_t w[W];
+  if constexpr (W == 2) {
+    const uint2 q = *reinterpret_cast<const uint2*>(p);
+    w[0] = q.x; w[1] = q.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+  Fv<kV<T, W>> r;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      r.v[i] = __uint_as_float(w[i]);
+    } else {
+      r.v[2 * i] = __uint_as_float(w[i] << 16);
+      r.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  return r;
 }
-__device__ __forceinline__ uint32_t f_word(const Fv<1>& a) { return __float_as_uint(a.v[0]); }
-__device__ __forceinline__ uint32_t f_word(const Fv<2>& a) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a.v[0], a.v[1]);
-  return *reinterpret_cast<const uint32_t*>(&h);
+template <typename T, int W> __device__ __forceinline__ void st_words(void* p, const Fv<kV<T, W>>& f) {
+  uint32_t w[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = __float_as_uint(f.v[i]);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f.v[2 * i], f.v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  if constexpr (W == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(p) = w[0];
 }
-// a word of dt = -inf
-__device__ __forceinline__ uint32_t no_step(float) { return 0xff800000u; }
-__device__ __forceinline__ uint32_t no_step(__nv_bfloat16) { return 0xff80ff80u; }
-// store a word of channels c, c+1, ... (< ds); vec: the row allows the whole word
-template <typename T>
-__device__ __forceinline__ void st_word(T* row, int c, int ds, int vec, const Fv<kVec<T>>& v) {
-  if (vec && c + kVec<T> <= ds) {
-    *reinterpret_cast<uint32_t*>(row + c) = f_word(v);
+// channels c, c+1, ... (those < nc) of a row; vec: the row allows whole lanes
+template <typename T, int W>
+__device__ __forceinline__ void st_row(T* row, int c, int nc, int vec, const Fv<kV<T, W>>& f) {
+  if (vec && c + kV<T, W> <= nc) {
+    st_words<T, W>(row + c, f);
   } else {
 #pragma unroll
-    for (int i = 0; i < kVec<T>; ++i)
-      if (c + i < ds) row[c + i] = from_f<T>(v.v[i]);
+    for (int i = 0; i < kV<T, W>; ++i)
+      if (c + i < nc) row[c + i] = from_f<T>(f.v[i]);
   }
 }
+// a word of dt = -inf
+template <typename T> constexpr uint32_t kNoStep = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -145,51 +191,65 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// d = softplus(x) and a = exp(d A) for the lane's channels.
+// d = softplus(x).
 //   fp32: the library's exp and log1p.
 //   bf16 inputs: softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) by the hardware's 2^x, and
 //   log1p(e) = e p(e) on [0, 1] with p of degree 7, fitted here for the least relative error
 //   (weighted least squares on Chebyshev points, weights iterated to equal errors: 2e-7, 3e-7
 //   with fp32 evaluation; the bf16 input itself is 2^-9 off).  e p(e) keeps its relative accuracy
-//   for small e, where log(1 + e) loses it.  A2 = A log2(e).
-__device__ __forceinline__ void gates(const Fv<1>& x, const Fv<1>& A, const Fv<1>&, Fv<1>& d, Fv<1>& a) {
-  d.v[0] = softplus_acc(x.v[0]);
-  a.v[0] = expf(d.v[0] * A.v[0]);
+//   for small e, where log(1 + e) loses it.
+// e: exp(-|x|) as computed on the way (bf16).
+template <typename T, int V> __device__ __forceinline__ Fv<V> gate(const Fv<V>& x, Fv<V>& e) {
+  if constexpr (sizeof(T) == 4) {
+    Fv<V> d;
+#pragma unroll
+    for (int i = 0; i < V; ++i) d.v[i] = softplus_acc(x.v[i]);
+    return d;
+  } else {
+    Fv<V> m;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      e.v[i] = ex2(-1.4426950408889634f * fabsf(x.v[i]));
+      asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(m.v[i]) : "f"(x.v[i]));  // NaN stays NaN
+    }
+    Fv<V> p = all<V>(-0.008539206348359585f);
+    p = fma(p, e, all<V>(0.04408962279558182f));
+    p = fma(p, e, all<V>(-0.10768169909715652f));
+    p = fma(p, e, all<V>(0.17745240032672882f));
+    p = fma(p, e, all<V>(-0.24495463073253632f));
+    p = fma(p, e, all<V>(0.33275479078292847f));
+    p = fma(p, e, all<V>(-0.4999740421772003f));
+    p = fma(p, e, all<V>(0.9999998211860657f));
+    return fma(p, e, m);
+  }
 }
-__device__ __forceinline__ void gates(const Fv<2>& x, const Fv<2>&, const Fv<2>& A2, Fv<2>& d, Fv<2>& a) {
-  Fv<2> e, m;
+// a = exp(d A); A2 = A log2(e)
+template <typename T, int V> __device__ __forceinline__ Fv<V> decay(const Fv<V>& d, const Fv<V>& A, const Fv<V>& A2) {
+  Fv<V> a;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    e.v[i] = ex2(-1.4426950408889634f * fabsf(x.v[i]));
-    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(m.v[i]) : "f"(x.v[i]));  // NaN stays NaN
-  }
-#ifdef SCALARP
+    for (int i = 0; i < V; ++i) a.v[i] = expf(d.v[i] * A.v[i]);
+  } else {
+    const Fv<V> l = d * A2;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float q = -0.008539206348359585f, z = e.v[i];
-    q = fmaf(q, z, 0.04408962279558182f);
-    q = fmaf(q, z, -0.10768169909715652f);
-    q = fmaf(q, z, 0.17745240032672882f);
-    q = fmaf(q, z, -0.24495463073253632f);
-    q = fmaf(q, z, 0.33275479078292847f);
-    q = fmaf(q, z, -0.4999740421772003f);
-    q = fmaf(q, z, 0.9999998211860657f);
-    d.v[i] = fmaf(q, z, m.v[i]);
+    for (int i = 0; i < V; ++i) a.v[i] = ex2(l.v[i]);
   }
-#else
-  Fv<2> p = all<2>(-0.008539206348359585f);
-  p = fma(p, e, all<2>(0.04408962279558182f));
-  p = fma(p, e, all<2>(-0.10768169909715652f));
-  p = fma(p, e, all<2>(0.17745240032672882f));
-  p = fma(p, e, all<2>(-0.24495463073253632f));
-  p = fma(p, e, all<2>(0.33275479078292847f));
-  p = fma(p, e, all<2>(-0.4999740421772003f));
-  p = fma(p, e, all<2>(0.9999998211860657f));
-  d = fma(p, e, m);
-#endif
-  const Fv<2> l = d * A2;
-  a.v[0] = ex2(l.v[0]);
-  a.v[1] = ex2(l.v[1]);
+  return a;
+}
+// sigmoid(x); e = exp(-|x|) (bf16)
+template <typename T, int V> __device__ __forceinline__ Fv<V> sigmoid(const Fv<V>& x, const Fv<V>& e) {
+  Fv<V> s;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      s.v[i] = 1.f / (1.f + expf(-x.v[i]));
+    } else {
+      float r;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e.v[i]));
+      s.v[i] = x.v[i] < 0.f ? e.v[i] * r : r;
+    }
+  }
+  return s;
 }
 
 // ---------------------------------------------------------------- maps h -> P h + H
@@ -215,25 +275,38 @@ template <bool RESET, int V> __device__ __forceinline__ Map<V> then(const Map<V>
   }
   return r;
 }
-// a lane's map in shared memory: 8 bytes per channel
+// a lane's V values in shared memory, slot k of arrays of 32 lanes
+template <int V> __device__ __forceinline__ void st_f(char* p, int k, int lane, const Fv<V>& f) {
+  float* q = reinterpret_cast<float*>(p) + (k * 32 + lane) * V;
+  if constexpr (V == 4) *reinterpret_cast<float4*>(q) = make_float4(f.v[0], f.v[1], f.v[2], f.v[3]);
+  else if constexpr (V == 2) *reinterpret_cast<float2*>(q) = make_float2(f.v[0], f.v[1]);
+  else *q = f.v[0];
+}
+template <int V> __device__ __forceinline__ Fv<V> ld_f(const char* p, int k, int lane) {
+  const float* q = reinterpret_cast<const float*>(p) + (k * 32 + lane) * V;
+  if constexpr (V == 4) {
+    const float4 t = *reinterpret_cast<const float4*>(q);
+    return {{t.x, t.y, t.z, t.w}};
+  } else if constexpr (V == 2) {
+    const float2 t = *reinterpret_cast<const float2*>(q);
+    return {{t.x, t.y}};
+  } else {
+    return {{*q}};
+  }
+}
+// a map in the slots k and k + 1
+template <int V> constexpr int kMapBytes = 2 * 32 * V * 4;
 template <int V> __device__ __forceinline__ void st_map(char* p, int lane, const Map<V>& m) {
-  float* f = reinterpret_cast<float*>(p) + lane * 2 * V;
-  if constexpr (V == 2) *reinterpret_cast<float4*>(f) = make_float4(m.P.v[0], m.P.v[1], m.H.v[0], m.H.v[1]);
-  else *reinterpret_cast<float2*>(f) = make_float2(m.P.v[0], m.H.v[0]);
+  st_f<V>(p, 0, lane, m.P);
+  st_f<V>(p, 1, lane, m.H);
 }
 template <int V> __device__ __forceinline__ Map<V> ld_map(const char* p, int lane) {
-  const float* f = reinterpret_cast<const float*>(p) + lane * 2 * V;
-  if constexpr (V == 2) {
-    const float4 q = *reinterpret_cast<const float4*>(f);
-    return {{{q.x, q.y}}, {{q.z, q.w}}};
-  } else {
-    const float2 q = *reinterpret_cast<const float2*>(f);
-    return {{{q.x}}, {{q.y}}};
-  }
+  return {ld_f<V>(p, 0, lane), ld_f<V>(p, 1, lane)};
 }
 
 // ---------------------------------------------------------------- published entries
 constexpr uint32_t kUnset = 0xffffffffu;  // P of a word that is not published
+// entry e (its first word), the lane's words
 template <int V> __device__ __forceinline__ void publish(uint64_t* e, int lane, const Map<V>& m) {
   uint64_t w[V];
 #pragma unroll
@@ -242,28 +315,36 @@ template <int V> __device__ __forceinline__ void publish(uint64_t* e, int lane, 
     if (P == kUnset) P = 0x7fffffffu;  // a NaN stays one
     w[i] = ((uint64_t)__float_as_uint(m.H.v[i]) << 32) | P;
   }
-  if constexpr (V == 2)
-    asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(e + lane * 2), "l"(w[0]), "l"(w[1]) : "memory");
-  else asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(e + lane), "l"(w[0]) : "memory");
+  if constexpr (V == 1) {
+    asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(e + lane), "l"(w[0]) : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2)
+      asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(e + lane * V + i), "l"(w[i]), "l"(w[i + 1])
+                   : "memory");
+  }
 }
-__device__ __forceinline__ void ld_entry(const uint64_t* e, uint64_t (&w)[1]) {
-  asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(w[0]) : "l"(e) : "memory");
-}
-__device__ __forceinline__ void ld_entry(const uint64_t* e, uint64_t (&w)[2]) {
-  asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(w[0]), "=l"(w[1]) : "l"(e) : "memory");
+template <int V> __device__ __forceinline__ void ld_entry(const uint64_t* e, uint64_t (&w)[V]) {
+  if constexpr (V == 1) {
+    asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(w[0]) : "l"(e) : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2)
+      asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(w[i]), "=l"(w[i + 1]) : "l"(e + i) : "memory");
+  }
 }
 // Compose n in 1..4 neighbouring entries, waited for (some 2 s, then error 61; what is missing
-// then counts as zeros).  e: entry 0 of them, ch: the lane's first channel.  While an entry is
-// missing, one word of each is polled, not the whole entries.
+// then counts as zeros).  e: entry 0 of them.  While an entry is missing, one word of each is
+// polled, not the whole entries.
 constexpr long long kWaitCycles = 4000000000ll;
-template <bool RESET, int V> __device__ __forceinline__ Map<V> take(const uint64_t* e, int ch, int n, int lane) {
+template <bool RESET, int V> __device__ __forceinline__ Map<V> take(const uint64_t* e, int n, int lane) {
   uint64_t w[4][V];
   long long t0 = 0;
   while (true) {
     bool ok = true;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (k < n) ld_entry(e + (int64_t)k * 32 * V + ch, w[k]);
+      if (k < n) ld_entry<V>(e + (k * 32 + lane) * V, w[k]);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -275,7 +356,7 @@ template <bool RESET, int V> __device__ __forceinline__ Map<V> take(const uint64
       uint64_t one[1];
       do {
         __nanosleep(32);
-        ld_entry(e + (int64_t)lane * 32 * V, one);
+        ld_entry<1>(e + lane * 32 * V, one);
         late = clock64() - t0 > kWaitCycles;
       } while ((uint32_t)one[0] == kUnset && !late);
     }
@@ -303,10 +384,57 @@ template <bool RESET, int V> __device__ __forceinline__ Map<V> take(const uint64
     }
   return m;
 }
-// Entries of a group: tiles, then spans of 16 tiles, then links of 16 spans (P unused, H the
-// state itself).
-__device__ __forceinline__ int span_at(int NT, int k) { return NT + k; }
-__device__ __forceinline__ int link_at(int NT, int k) { return NT + (NT + kSpan - 1) / kSpan + k; }
+
+// The exchange between tiles, the same for both directions.  q: the tile's index in the order
+// of the scan.  maps: the 8 warps' maps in shared memory, warp w's at maps + w * stride, composed
+// in the order of the scan (REV: from the last warp to the first).  pre: this warp's slot at
+// pre + warp * pre_stride.  All threads call it (it synchronises the CTA once, after the maps'
+// own barrier); h: the state entering the sequence, returned as the state entering the tile.
+template <bool RESET, bool REV, int V>
+__device__ __forceinline__ Fv<V> enter_tile(const ScanParams& p, int g, int q, const char* maps, int stride, char* pre,
+                                            int pre_stride, Fv<V> h, int warp, int lane) {
+  constexpr int CW = 32 * V;
+  uint64_t* ent = p.ent + (int64_t)g * p.nent * CW;
+  // entries of a group: tiles, then spans of 16 tiles, then links of 16 spans (P unused, H the
+  // state at their end)
+  uint64_t* spans = ent + (int64_t)p.NT * CW;
+  uint64_t* links = spans + (int64_t)((p.NT + kSpan - 1) / kSpan) * CW;
+  const int in_span = q % kSpan, span = q / kSpan, link = span / kSpan, in_link = span % kSpan;
+  const bool more = q + 1 < p.NT;
+  auto tile_map = [&]() {
+    Map<V> m = ld_map<V>(maps + (REV ? kWarps - 1 : 0) * stride, lane);
+#pragma unroll
+    for (int k = 1; k < kWarps; ++k) m = then<RESET>(m, ld_map<V>(maps + (REV ? kWarps - 1 - k : k) * stride, lane));
+    return m;
+  };
+  if (warp == 0 && more) publish<V>(ent + (int64_t)q * CW, lane, tile_map());
+  // warps 0..3 compose the whole spans of the link that the tile is in, warps 4..7 the tiles of
+  // the span that it is in, four entries each
+  const int from = warp % 4 * 4, n = min(4, (warp < 4 ? in_link : in_span) - from);
+  if (n > 0) {
+    const uint64_t* e = warp < 4 ? spans + (int64_t)(link * kSpan + from) * CW : ent + (int64_t)(span * kSpan + from) * CW;
+    st_map<V>(pre + warp * pre_stride, lane, take<RESET, V>(e, n, lane));
+  }
+  if (in_span == kSpan - 1 && more && warp >= 4) {
+    // the end of a span: its map is published before this tile waits for earlier spans, or
+    // each span would wait for the one before
+    named_bar_sync(1, 128);
+    if (warp == 4) {
+      Map<V> m = ld_map<V>(pre + 4 * pre_stride, lane);
+#pragma unroll
+      for (int k = 5; k < kWarps; ++k) m = then<RESET>(m, ld_map<V>(pre + k * pre_stride, lane));
+      publish<V>(spans + (int64_t)span * CW, lane, then<RESET>(m, tile_map()));
+    }
+  }
+  if (link > 0) h = take<false, V>(links + (int64_t)(link - 1) * CW, 1, lane).H;
+  __syncthreads();
+  const int outer = (in_link + 3) / 4, inner = (in_span + 3) / 4;
+  for (int k = 0; k < outer; ++k) h = apply<RESET>(ld_map<V>(pre + k * pre_stride, lane), h);
+  for (int k = 4; k < 4 + inner; ++k) h = apply<RESET>(ld_map<V>(pre + k * pre_stride, lane), h);
+  if (warp == 0 && in_span == kSpan - 1 && in_link == kSpan - 1 && more)  // the end of a link
+    publish<V>(links + (int64_t)link * CW, lane, {all<V>(0.f), apply<RESET>(tile_map(), h)});
+  return h;
+}
 
 // ---------------------------------------------------------------- staging
 __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool ok, std::integral_constant<int, 16>) {
@@ -318,69 +446,84 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool ok,
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
-// Copies of one warp's 8 rows of 128 bytes of a tile, rows >= nv and channels >= nc as zeros.
-// CB: bytes per copy (16 or 4, as the rows allow), or 0: element by element, not asynchronous.
-template <typename T, int CB> struct Rows {
-  static constexpr int kPer = CB ? 128 / CB : 32, kAt = 32 / kPer, kN = kRows / kAt;
-  uint32_t dst;   // the lane's place in a region
-  int r0, x;      // its first row and first byte of the rows
-  __device__ explicit Rows(int lane) : r0(lane / kPer), x(lane % kPer * (CB ? CB : 4)) { dst = r0 * 128 + x; }
+// Copies of one warp's 8 rows (128 W bytes each) of a tile, rows >= nv and channels >= nc as
+// zeros.  CB: bytes per copy (16 or 4, as the rows allow), or 0: element by element, not
+// asynchronous.
+template <typename T, int W, int CB> struct Rows {
+  static constexpr int kBytes = 128 * W, kCopy = CB ? CB : 4;
+  static constexpr int kPer = kBytes / kCopy;               // copies per row
+  static constexpr int kAt = kPer < 32 ? 32 / kPer : 1;     // rows per warp-wide copy
+  static constexpr int kX = kPer > 32 ? kPer / 32 : 1;      // warp-wide copies per row
+  int r0, x;  // the lane's first row and first byte of a row
+  __device__ explicit Rows(int lane) : r0(kPer < 32 ? lane / kPer : 0), x((kPer < 32 ? lane % kPer : lane) * kCopy) {}
   // tile: the tile's first element; row0: the warp's first row in it; st: row stride (elements);
   // `arrays` consecutive regions, their sources `apart` elements from each other
   template <int arrays>
   __device__ __forceinline__ void copy(char* region, const T* tile, int row0, int64_t st, int64_t apart, int nv,
                                        int nc) const {
-    if constexpr (CB == 0) {
-      const int c = x / (int)sizeof(T);
 #pragma unroll
-      for (int k = 0; k < arrays; ++k)
+    for (int i = 0; i < kRows / kAt; ++i)
 #pragma unroll
-        for (int r = 0; r < kRows; ++r)
+      for (int j = 0; j < kX; ++j) {
+        const int r = r0 + i * kAt, xb = x + j * 32 * kCopy;
+        const bool ok = r < nv && xb < nc * (int)sizeof(T);
+        if constexpr (CB == 0) {
+          constexpr int per = 4 / (int)sizeof(T);
+          const int c = xb / (int)sizeof(T);
 #pragma unroll
-          for (int i = 0; i < kVec<T>; ++i)
-            reinterpret_cast<T*>(region + (k * kRows + r) * 128)[c + i] =
-                r < nv && c + i < nc ? tile[k * apart + (row0 + r) * st + c + i] : from_f<T>(0.f);
-    } else {
-      const uint32_t d = smem_u32(region) + dst;
-      const bool in = x < nc * (int)sizeof(T);
-      const char* src[kN];
-      bool ok[kN];
+          for (int k = 0; k < arrays; ++k)
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        ok[i] = in && r0 + i * kAt < nv;
-        src[i] = reinterpret_cast<const char*>(tile) + (ok[i] ? (row0 + r0 + i * kAt) * st * (int64_t)sizeof(T) + x : 0);
+            for (int e = 0; e < per; ++e)
+              reinterpret_cast<T*>(region + (k * kRows + r) * kBytes)[c + e] =
+                  r < nv && c + e < nc ? tile[k * apart + (row0 + r) * st + c + e] : from_f<T>(0.f);
+        } else {
+          const char* src = reinterpret_cast<const char*>(tile) + (ok ? (row0 + r) * st * (int64_t)sizeof(T) + xb : 0);
+          const uint32_t dst = smem_u32(region) + r * kBytes + xb;
+#pragma unroll
+          for (int k = 0; k < arrays; ++k)
+            cp_async(dst + k * kRows * kBytes, src + k * apart * (int64_t)sizeof(T), ok, std::integral_constant<int, CB>());
+        }
       }
-#pragma unroll
-      for (int k = 0; k < arrays; ++k)
-#pragma unroll
-        for (int i = 0; i < kN; ++i)
-          cp_async(d + (k * kRows + i * kAt) * 128, src[i] + k * apart * (int64_t)sizeof(T), ok[i],
-                   std::integral_constant<int, CB>());
-    }
   }
 };
 
-// A tile as broadcast through shared memory: index in time, group, batch, first channel; q < 0: none
+// A tile as broadcast through shared memory: index in the scan's order, group, batch, first
+// channel; x < 0: none
 using Tile = int4;
-template <typename T> __device__ __forceinline__ Tile tile_of(const ScanParams& p, int64_t id) {
+__device__ __forceinline__ Tile tile_of(const ScanParams& p, int64_t id, int CW) {
   if (id >= p.ntiles) return make_int4(-1, 0, 0, 0);
   const unsigned q = (unsigned)id / (unsigned)p.NG, g = (unsigned)id - q * p.NG, b = g / (unsigned)p.nch;
-  return make_int4((int)q, (int)g, (int)b, (int)(g - b * p.nch) * kCW<T>);
+  return make_int4((int)q, (int)g, (int)b, (int)(g - b * p.nch) * CW);
 }
 __device__ __forceinline__ int64_t next_tile(const ScanParams& p, int64_t last) {
   if (!p.ticket) return last + gridDim.x;
   return (int64_t)(unsigned)(atomicAdd(p.ticket, 1u) + 1u);  // the counter starts at all ones
 }
+// the lane's channels of a [.., ds] fp32 row (nc of them in the tile), zeros where there is none
+template <int V> __device__ __forceinline__ Fv<V> ld_state(const float* row, int cl, int nc) {
+  Fv<V> h;
+#pragma unroll
+  for (int i = 0; i < V; ++i) h.v[i] = row && cl + i < nc ? row[cl + i] : 0.f;
+  return h;
+}
+template <int V> __device__ __forceinline__ void st_state(float* row, int cl, int nc, const Fv<V>& h) {
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (cl + i < nc) row[cl + i] = h.v[i];
+}
 
-template <typename T, bool RESET, int CB>
-__global__ void __launch_bounds__(kWarps * 32, kFwdCtas) gated_scan_fwd_kernel(const __grid_constant__ ScanParams p) {
-  constexpr int V = kVec<T>, CW = kCW<T>, kRegion = 3 * kRows * 128;
-  extern __shared__ __align__(128) char raw[];  // [2][warp][dt, x, b][row][128 bytes]
+template <int W> constexpr int kFwdCtas = W == 2 ? 2 : 4;  // resident forward CTAs per SM
+
+template <typename T, int W, bool RESET, int CB>
+__global__ void __launch_bounds__(kWarps * 32, kFwdCtas<W>) gated_scan_fwd_kernel(const __grid_constant__ ScanParams p) {
+  constexpr int V = kV<T, W>, CW = 32 * V, RB = 128 * W, kRegion = 3 * kRows * RB;
+  static_assert(2 * kMapBytes<V> <= kRegion, "maps fit into a warp's staged rows");
+  extern __shared__ __align__(128) char raw[];  // [2][warp][dt, x, b][row][RB bytes]
   __shared__ __align__(16) float s_A[2][CW];
   __shared__ Tile s_next[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int cl = lane * V;  // the lane's first channel of the tile
-  const Rows<T, CB> rows(lane);
+  const Rows<T, W, CB> rows(lane);
   int64_t id = 0;  // thread 0's
 
   uint32_t rb = 0;  // the staged tile's reset flag of step `lane` of the warp
@@ -398,7 +541,7 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas) gated_scan_fwd_kernel(c
 
   if (threadIdx.x == 0) {
     id = p.ticket ? next_tile(p, 0) : blockIdx.x;
-    s_next[0] = tile_of<T>(p, id);
+    s_next[0] = tile_of(p, id, CW);
   }
   __syncthreads();
   Tile t = s_next[0];
@@ -413,32 +556,33 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas) gated_scan_fwd_kernel(c
     first = false;
     if (threadIdx.x == 0) {
       id = next_tile(p, id);
-      s_next[s ^ 1] = tile_of<T>(p, id);
+      s_next[s ^ 1] = tile_of(p, id, CW);
     }
     char* buf = raw + s * kWarps * kRegion;
     char* mine = buf + warp * kRegion;
     const int t0 = t.x * kStateRows + warp * kRows, nv = p.L - t0, nc = p.ds - t.w;
     const uint32_t cut = RESET ? __ballot_sync(0xffffffffu, rb != 0) : 0;
-    Fv<V> A;
-#pragma unroll
-    for (int i = 0; i < V; ++i) A.v[i] = s_A[s][cl + i];
+    const Fv<V> A = ld_f<V>(reinterpret_cast<char*>(s_A[s]), 0, lane);
     const Fv<V> A2 = A * all<V>(1.4426950408889634f);
     cp_wait_all();
     __syncwarp();
     if (nv < kRows) {  // steps past the end: dt = -inf (and x = b = 0) is the identity, a = 1, u = 0
-      for (int r = max(nv, 0); r < kRows; ++r) reinterpret_cast<uint32_t*>(mine + r * 128)[lane] = no_step(T());
+      for (int r = max(nv, 0); r < kRows; ++r)
+#pragma unroll
+        for (int k = 0; k < W; ++k) reinterpret_cast<uint32_t*>(mine + r * RB)[lane * W + k] = kNoStep<T>;
     }
 
     // local scan of the warp's steps from a zero state
     Fv<V> a[kRows], u[kRows];
     Map<V> m = identity_map<V>();
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(mine) + lane;
+    const char* w = mine + lane * 4 * W;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const Fv<V> dt = word_f(w[r * 32], T()), x = word_f(w[(kRows + r) * 32], T());
-      const Fv<V> b = word_f(w[(2 * kRows + r) * 32], T());
-      Fv<V> d;
-      gates(dt, A, A2, d, a[r]);
+      const Fv<V> dt = ld_words<T, W>(w + r * RB), x = ld_words<T, W>(w + (kRows + r) * RB);
+      const Fv<V> b = ld_words<T, W>(w + (2 * kRows + r) * RB);
+      Fv<V> e;
+      const Fv<V> d = gate<T>(dt, e);
+      a[r] = decay<T>(d, A, A2);
       u[r] = d * (b * x);
       if (RESET && ((cut >> r) & 1)) {
         m.H = u[r];
@@ -455,55 +599,13 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas) gated_scan_fwd_kernel(c
     const Tile nt = s_next[s ^ 1];
     if (nt.x >= 0) stage(nt, s ^ 1);
 
-    // the tile's map, published; then the state entering the tile
-    Fv<V> h;
-#pragma unroll
-    for (int i = 0; i < V; ++i) h.v[i] = p.h0 && cl + i < nc ? p.h0[(int64_t)t.z * p.ds + t.w + cl + i] : 0.f;
-    if (p.ticket) {
-      uint64_t* ent = p.ent + (int64_t)t.y * p.nent * CW;
-      const int in_span = t.x % kSpan, span = t.x / kSpan, link = span / kSpan, in_link = span % kSpan;
-      Map<V> tile_map;
-      if (warp == 0) {
-        tile_map = ld_map<V>(buf, lane);
-#pragma unroll
-        for (int k = 1; k < kWarps; ++k) tile_map = then<RESET>(tile_map, ld_map<V>(buf + k * kRegion, lane));
-        if (t.x + 1 < p.NT) publish<V>(ent + (int64_t)t.x * CW, lane, tile_map);
-      }
-      // warps 0..3 compose the whole spans of the link that the tile is in, warps 4..7 the tiles
-      // of the span that it is in, four entries each
-      const int from = warp % 4 * 4, n = min(4, (warp < 4 ? in_link : in_span) - from);
-      if (n > 0) {
-        const int at = warp < 4 ? span_at(p.NT, link * kSpan + from) : span * kSpan + from;
-        st_map<V>(mine + 512, lane, take<RESET, V>(ent + (int64_t)at * CW, cl, n, lane));
-      }
-      if (in_span == kSpan - 1 && t.x + 1 < p.NT && warp >= 4) {
-        // the end of a span: its map is published before this tile waits for earlier spans, or
-        // each span would wait for the one before
-        named_bar_sync(1, 128);
-        if (warp == 4) {
-          Map<V> sp = ld_map<V>(buf + 4 * kRegion + 512, lane);
-#pragma unroll
-          for (int k = 5; k < kWarps; ++k) sp = then<RESET>(sp, ld_map<V>(buf + k * kRegion + 512, lane));
-#pragma unroll
-          for (int k = 0; k < kWarps; ++k) sp = then<RESET>(sp, ld_map<V>(buf + k * kRegion, lane));
-          publish<V>(ent + (int64_t)span_at(p.NT, span) * CW, lane, sp);
-        }
-      }
-      if (link > 0) h = take<false, V>(ent + (int64_t)link_at(p.NT, link - 1) * CW, cl, 1, lane).H;
-      __syncthreads();
-      const int outer = (in_link + 3) / 4, inner = (in_span + 3) / 4;
-      for (int k = 0; k < outer; ++k) h = apply<RESET>(ld_map<V>(buf + k * kRegion + 512, lane), h);
-      for (int k = 4; k < 4 + inner; ++k) h = apply<RESET>(ld_map<V>(buf + k * kRegion + 512, lane), h);
-      if (warp == 0 && in_span == kSpan - 1 && in_link == kSpan - 1 && t.x + 1 < p.NT)  // the end of a link
-        publish<V>(ent + (int64_t)link_at(p.NT, link) * CW, lane, {all<V>(0.f), apply<RESET>(tile_map, h)});
-    } else {
-      __syncthreads();
-    }
-    if (p.states && warp == 0) {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (cl + i < nc) p.states[((int64_t)t.z * p.NT + t.x) * p.ds + t.w + cl + i] = h.v[i];
-    }
+    // the state entering the tile, then the warp's steps
+    const int64_t at = (int64_t)t.z * p.ds + t.w;
+    Fv<V> h = ld_state<V>(p.h0 ? p.h0 + at : nullptr, cl, nc);
+    if (p.ticket)
+      h = enter_tile<RESET, false, V>(p, t.y, t.x, buf, kRegion, buf + kMapBytes<V>, kRegion, h, warp, lane);
+    else __syncthreads();  // s_A of the next tile
+    if (p.states && warp == 0) st_state<V>(p.states + ((int64_t)t.z * p.NT + t.x) * p.ds + t.w, cl, nc, h);
     for (int k = 0; k < warp; ++k) h = apply<RESET>(ld_map<V>(buf + k * kRegion, lane), h);
 
     T* y = static_cast<T*>(p.y) + t.z * p.ysb + t0 * p.yst + t.w;
@@ -512,73 +614,198 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas) gated_scan_fwd_kernel(c
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         h = RESET && ((cut >> r) & 1) ? u[r] : fma(a[r], h, u[r]);
-        *reinterpret_cast<uint32_t*>(row) = f_word(h);
+        st_words<T, W>(row, h);
         row += p.yst * (int64_t)sizeof(T);
       }
     } else {
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         h = RESET && ((cut >> r) & 1) ? u[r] : fma(a[r], h, u[r]);
-        if (r < nv) st_word<T>(y + r * p.yst, cl, nc, p.out_vec, h);
+        if (r < nv) st_row<T, W>(y + r * p.yst, cl, nc, p.out_vec, h);
       }
     }
-    if (p.h_last && t.x == p.NT - 1 && warp == kWarps - 1) {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (cl + i < nc) p.h_last[(int64_t)t.z * p.ds + t.w + cl + i] = h.v[i];
-    }
+    if (p.h_last && t.x == p.NT - 1 && warp == kWarps - 1) st_state<V>(p.h_last + at, cl, nc, h);
     t = nt;
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(128) gated_scan_bwd_kernel(ScanParams p) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (int64_t)p.B * p.ds) return;
-  const int b = (int)(i / p.ds), j = (int)(i - (int64_t)b * p.ds);
-  const float A = -expf(ld_param(p.A_log, p.a_bf16, j));
-  const T* in = static_cast<const T*>(p.projs) + b * p.psb + j;
-  const T* dy = static_cast<const T*>(p.dy) + b * p.dsb + j;
-  T* out = static_cast<T*>(p.dprojs) + b * p.gsb + j;
-  const uint8_t* rs = p.reset ? p.reset + (int64_t)b * p.L : nullptr;
-  float* hb = p.hbuf + (int64_t)b * p.L * p.ds + j;
-  float h = 0.f;
-  for (int t = 0; t < p.L; ++t) {
-    if (t % kStateRows == 0) h = p.states[((int64_t)b * p.NT + t / kStateRows) * p.ds + j];
-    hb[(int64_t)t * p.ds] = h;
-    const T* r = in + t * p.pst;
-    const float d = softplus_acc(to_f(r[0]));
-    const float u = d * to_f(r[2 * p.ds]) * to_f(r[p.ds]);
-    h = (rs && rs[t]) ? u : fmaf(expf(d * A), h, u);
+template <int W> constexpr int kBwdCtas = 2;  // resident backward CTAs per SM
+// shared memory of the backward: two staged tiles, the warps' forward maps and backward maps
+// (P shared), the exchange's slots, the warps' sums for dA
+template <int V, int W> constexpr int kBwdMaps = 2 * kWarps * 4 * kRows * 128 * W;
+template <int V, int W> constexpr int kBwdSmem = kBwdMaps<V, W> + kWarps * 32 * V * (16 + 8 + 4);
+
+template <typename T, int W, bool RESET, int CB>
+__global__ void __launch_bounds__(kWarps * 32, kBwdCtas<W>) gated_scan_bwd_kernel(const __grid_constant__ ScanParams p) {
+  constexpr int V = kV<T, W>, CW = 32 * V, RB = 128 * W, kRegion = 4 * kRows * RB;
+  extern __shared__ __align__(128) char raw[];  // [2][warp][dt, x, b, dy][row][RB bytes]
+  char* fmap = raw + kBwdMaps<V, W>;            // [warp] forward maps (P, H)
+  char* bmap = fmap + kWarps * kMapBytes<V>;    // [warp] backward maps (P, C)
+  char* pre = bmap + kWarps * kMapBytes<V>;     // [warp] exchange
+  char* sums = pre + kWarps * kMapBytes<V>;     // [warp] sums of s d
+  __shared__ __align__(16) float s_A[2][CW];
+  __shared__ Tile s_next[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int cl = lane * V;
+  const Rows<T, W, CB> rows(lane);
+  int64_t id = 0;  // thread 0's
+
+  uint32_t rb = 0;
+  auto stage = [&](const Tile& t, int s) {
+    const int t0 = (p.NT - 1 - t.x) * kStateRows, nv = p.L - t0 - warp * kRows, nc = p.ds - t.w;
+    char* reg = raw + (s * kWarps + warp) * kRegion;
+    const T* tile = static_cast<const T*>(p.projs) + t.z * p.psb + t0 * p.pst + t.w;
+    rows.template copy<3>(reg, tile, warp * kRows, p.pst, p.ds, nv, nc);
+    const T* dyt = static_cast<const T*>(p.dy) + t.z * p.dsb + t0 * p.dst + t.w;
+    rows.template copy<1>(reg + 3 * kRows * RB, dyt, warp * kRows, p.dst, 0, nv, nc);
+    cp_commit();
+    if (RESET) rb = lane < min(nv, kRows) ? p.reset[(int64_t)t.z * p.L + t0 + warp * kRows + lane] : 0;
+    if (warp == 3) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) s_A[s][cl + i] = cl + i < nc ? -expf(ld_param(p.A_log, p.a_bf16, t.w + cl + i)) : 0.f;
+    }
+  };
+  // the sum of the warps' s d of the tile before, in their order
+  auto write_dA = [&](const Tile& t) {
+    Fv<V> v = ld_f<V>(sums, 0, lane);
+#pragma unroll
+    for (int k = 1; k < kWarps; ++k) v = v + ld_f<V>(sums, k, lane);
+    st_f<V>(reinterpret_cast<char*>(p.dA_part + ((int64_t)t.x * p.NG + t.y) * CW), 0, lane, v);
+  };
+
+  if (threadIdx.x == 0) {
+    id = p.ticket ? next_tile(p, 0) : blockIdx.x;
+    s_next[0] = tile_of(p, id, CW);
   }
-  float c = p.dh_last ? p.dh_last[i] : 0.f;
-  float dA = 0.f;
-  for (int t = p.L - 1; t >= 0; --t) {
-    const T* r = in + t * p.pst;
-    const float dt = to_f(r[0]), x = to_f(r[p.ds]), bb = to_f(r[2 * p.ds]);
-    const float d = softplus_acc(dt), sg = 1.f / (1.f + expf(-dt));
-    const float g = to_f(dy[t * p.dst]) + c;
-    const bool cut = rs && rs[t];
-    c = cut ? 0.f : expf(d * A) * g;
-    const float s = cut ? 0.f : c * hb[(int64_t)t * p.ds];
-    dA = fmaf(s, d * A, dA);
-    T* o = out + t * p.gst;
-    o[0] = from_f<T>(fmaf(g * bb, x, s * A) * sg);
-    o[p.ds] = from_f<T>(g * d * bb);
-    o[2 * p.ds] = from_f<T>(g * d * x);
+  __syncthreads();
+  Tile t = s_next[0], before = make_int4(-1, 0, 0, 0);
+  if (t.x >= 0) stage(t, 0);
+  __syncthreads();
+  for (int s = 0; t.x >= 0; s ^= 1) {
+    if (before.x < 0) cp_wait_all();  // the first time the next ticket waits for the loads, as in the forward
+    if (threadIdx.x == 0) {
+      id = next_tile(p, id);
+      s_next[s ^ 1] = tile_of(p, id, CW);
+    }
+    char* mine = raw + (s * kWarps + warp) * kRegion;
+    const int tt = p.NT - 1 - t.x, t0 = tt * kStateRows + warp * kRows, nv = p.L - t0, nc = p.ds - t.w;
+    const uint32_t cut = RESET ? __ballot_sync(0xffffffffu, rb != 0) : 0;
+    Fv<V> h = ld_state<V>(p.states + ((int64_t)t.z * p.NT + tt) * p.ds + t.w, cl, nc);
+    const Fv<V> A = ld_f<V>(reinterpret_cast<char*>(s_A[s]), 0, lane);
+    const Fv<V> A2 = A * all<V>(1.4426950408889634f);
+    cp_wait_all();
+    __syncwarp();
+    if (nv < kRows) {  // steps past the end are the identity
+      for (int r = max(nv, 0); r < kRows; ++r)
+#pragma unroll
+        for (int k = 0; k < W; ++k) reinterpret_cast<uint32_t*>(mine + r * RB)[lane * W + k] = kNoStep<T>;
+    }
+
+    // local scans of the warp's steps, forward and backward
+    Fv<V> a[kRows], d[kRows];
+    Map<V> m = identity_map<V>();
+    Fv<V> c = all<V>(0.f);
+    const char* w = mine + lane * 4 * W;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const Fv<V> dt = ld_words<T, W>(w + r * RB), x = ld_words<T, W>(w + (kRows + r) * RB);
+      const Fv<V> b = ld_words<T, W>(w + (2 * kRows + r) * RB);
+      Fv<V> e;
+      d[r] = gate<T>(dt, e);
+      a[r] = decay<T>(d[r], A, A2);
+      const Fv<V> u = d[r] * (b * x);
+      if (RESET && ((cut >> r) & 1)) {
+        m.H = u;
+        m.P = all<V>(-1.f);
+      } else {
+        m.H = fma(a[r], m.H, u);
+        if (!RESET || !(m.P.v[0] < 0.f)) m.P = m.P * a[r];
+      }
+    }
+#pragma unroll
+    for (int r = kRows - 1; r >= 0; --r) {
+      c = a[r] * (ld_words<T, W>(w + (3 * kRows + r) * RB) + c);
+      if (RESET && ((cut >> r) & 1)) c = all<V>(0.f);
+    }
+    st_map<V>(fmap + warp * kMapBytes<V>, lane, m);
+    st_map<V>(bmap + warp * kMapBytes<V>, lane, {m.P, c});
+    __syncthreads();
+
+    const Tile nt = s_next[s ^ 1];
+    if (nt.x >= 0) stage(nt, s ^ 1);
+    if (warp == 2 && before.x >= 0) write_dA(before);
+
+    // what enters the tile from its end, then the warp's part of both scans
+    const int64_t at = (int64_t)t.z * p.ds + t.w;
+    c = ld_state<V>(p.dh_last ? p.dh_last + at : nullptr, cl, nc);
+    for (int k = 0; k < warp; ++k) h = apply<RESET>(ld_map<V>(fmap + k * kMapBytes<V>, lane), h);
+    if (p.ticket) c = enter_tile<RESET, true, V>(p, t.y, t.x, bmap, kMapBytes<V>, pre, kMapBytes<V>, c, warp, lane);
+    else __syncthreads();  // s_A of the next tile, the sums
+    for (int k = kWarps - 1; k > warp; --k) c = apply<RESET>(ld_map<V>(bmap + k * kMapBytes<V>, lane), c);
+
+    Fv<V> q[kRows];  // a_t h_{t-1}, 0 at a reset
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const Fv<V> x = ld_words<T, W>(w + (kRows + r) * RB), b = ld_words<T, W>(w + (2 * kRows + r) * RB);
+      q[r] = RESET && ((cut >> r) & 1) ? all<V>(0.f) : a[r] * h;
+      h = fma(d[r], b * x, q[r]);
+    }
+    Fv<V> sum = all<V>(0.f);
+    T* out = static_cast<T*>(p.dprojs) + t.z * p.gsb + t0 * p.gst + t.w;
+    const bool whole = p.out_vec && nv >= kRows && nc >= CW;
+#pragma unroll
+    for (int r = kRows - 1; r >= 0; --r) {
+      const Fv<V> dt = ld_words<T, W>(w + r * RB), x = ld_words<T, W>(w + (kRows + r) * RB);
+      const Fv<V> b = ld_words<T, W>(w + (2 * kRows + r) * RB);
+      const Fv<V> g = ld_words<T, W>(w + (3 * kRows + r) * RB) + c;
+      c = a[r] * g;
+      if (RESET && ((cut >> r) & 1)) c = all<V>(0.f);
+      Fv<V> e;
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) e.v[i] = ex2(-1.4426950408889634f * fabsf(dt.v[i]));
+      }
+      const Fv<V> gd = g * d[r], sr = g * q[r];
+      const Fv<V> ddt = fma(sr, A, g * (b * x)) * sigmoid<T>(dt, e);
+      if (whole) {
+        sum = fma(sr, d[r], sum);
+        T* o = out + r * p.gst + cl;
+        st_words<T, W>(o, ddt);
+        st_words<T, W>(o + p.ds, gd * b);
+        st_words<T, W>(o + 2 * p.ds, gd * x);
+      } else if (r < nv) {
+        sum = fma(sr, d[r], sum);
+        T* o = out + r * p.gst;
+        st_row<T, W>(o, cl, nc, p.out_vec, ddt);
+        st_row<T, W>(o + p.ds, cl, nc, p.out_vec, gd * b);
+        st_row<T, W>(o + 2 * p.ds, cl, nc, p.out_vec, gd * x);
+      }
+    }
+    if (p.dh0 && tt == 0 && warp == 0) st_state<V>(p.dh0 + at, cl, nc, c);
+    st_f<V>(sums, warp, lane, sum);
+    __syncthreads();  // the maps and slots are read, the sums written
+    before = t;
+    t = nt;
   }
-  if (p.dh0) p.dh0[i] = c;
-  p.dA_part[i] = dA;
+  if (warp == 2 && before.x >= 0) write_dA(before);
 }
 
-// dA_log[j] = sum over the parts, in their order
-__global__ void gated_scan_dA_kernel(const float* part, int parts, int ds, void* dA, int bf16) {
-  const int j = blockIdx.x * blockDim.x + threadIdx.x;
-  if (j >= ds) return;
-  float s = 0.f;
-  for (int k = 0; k < parts; ++k) s += part[(int64_t)k * ds + j];
-  if (bf16) static_cast<__nv_bfloat16*>(dA)[j] = __float2bfloat16_rn(s);
-  else static_cast<float*>(dA)[j] = s;
+// dA_log[j] = A_j times the sum of the parts ([q][b][channel], channels padded to cpad), in their
+// order: 8 strands per channel (32 channels a CTA), then the strands
+__global__ void __launch_bounds__(256) gated_scan_dA_kernel(const float* part, int64_t parts, int cpad, int ds,
+                                                            const void* A_log, int a_bf16, void* dA) {
+  __shared__ float s[8][32];
+  const int j = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+  float v = 0.f;
+  if (j < ds)
+    for (int64_t i = k; i < parts; i += 8) v += part[i * cpad + j];
+  s[k][threadIdx.x & 31] = v;
+  __syncthreads();
+  if (k != 0 || j >= ds) return;
+  for (int i = 1; i < 8; ++i) v += s[i][threadIdx.x];
+  v *= -expf(ld_param(A_log, a_bf16, j));
+  if (a_bf16) static_cast<__nv_bfloat16*>(dA)[j] = __float2bfloat16_rn(v);
+  else static_cast<float*>(dA)[j] = v;
 }
 
 template <typename T>
@@ -613,19 +840,23 @@ static bool off_type(const void* p, int dtype) {
 
 // ---------------------------------------------------------------- plans
 // every row of a tensor (batch stride sb, row stride st, in elements) starts on `align` bytes
-static int rows_allow(const void* p, int64_t sb, int64_t st, int es, int align) {
+static bool rows_allow(const void* p, int64_t sb, int64_t st, int es, int align) {
   return reinterpret_cast<uintptr_t>(p) % align == 0 && sb * es % align == 0 && st * es % align == 0;
 }
+static int64_t tiles_in_time(int64_t L) { return (L + kStateRows - 1) / kStateRows; }
 static int64_t scan_entries(int64_t NT) {
   return NT + (NT + kSpan - 1) / kSpan + (NT + kSpan * kSpan - 1) / (kSpan * kSpan);
 }
-// the ticket, then the entries (channels rounded up to the wider of the two tiles)
+// channels rounded up to the widest tile
+static int64_t scan_pad(int64_t ds) { return (ds + 127) / 128 * 128; }
+// the ticket, then the entries
 static size_t scan_ws(int64_t B, int64_t L, int64_t ds) {
-  const int64_t NT = (L + kStateRows - 1) / kStateRows;
+  const int64_t NT = tiles_in_time(L);
   if (B < 1 || ds < 1 || NT < 2) return 0;
-  return 16 + (size_t)(B * ((ds + 63) / 64 * 64)) * scan_entries(NT) * 8;
+  return 16 + (size_t)(B * scan_pad(ds)) * scan_entries(NT) * 8;
 }
 static void scan_plan(ScanParams& p, int CW, void* ws) {
+  p.CW = CW;
   p.nch = (p.ds + CW - 1) / CW;
   p.NG = p.B * p.nch;
   p.ntiles = (int64_t)p.NG * p.NT;
@@ -635,23 +866,48 @@ static void scan_plan(ScanParams& p, int CW, void* ws) {
 }
 static int scan_clear(const ScanParams& p, cudaStream_t s, const char* what) {
   if (!p.ticket) return 0;
-  const cudaError_t e = cudaMemsetAsync(p.ticket, 0xff, scan_ws(p.B, p.L, p.ds), s);
+  const size_t n = 16 + (size_t)p.NG * p.CW * p.nent * 8;
+  const cudaError_t e = cudaMemsetAsync(p.ticket, 0xff, n, s);
   return e == cudaSuccess ? 0 : fail((int)e, "%s: %s", what, cudaGetErrorString(e));
 }
-template <typename T, bool RESET, int CB>
-static void scan_fwd_launch(const ScanParams& p, cudaStream_t s) {
-  constexpr int smem = 2 * kWarps * 3 * kRows * 128;
-  auto k = gated_scan_fwd_kernel<T, RESET, CB>;
-  cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  const int64_t most = (int64_t)num_sms() * kFwdCtas;
-  k<<<(unsigned)(p.ntiles < most ? p.ntiles : most), kWarps * 32, smem, s>>>(p);
+// sizes that the kernels' 32-bit indices hold
+static int scan_fits(const char* what, int64_t B, int64_t L, int64_t ds) {
+  const int64_t groups = B * ((ds + 31) / 32);
+  if (groups > (int64_t(1) << 30) || groups * tiles_in_time(L) > (int64_t(1) << 31) - 4096)
+    return fail(HDC_E_SHAPE, "%s: B=%lld x L=%lld x d_state=%lld is too large", what, (long long)B, (long long)L,
+                (long long)ds);
+  return 0;
 }
-template <typename T>
-static void scan_fwd_launch(const ScanParams& p, int cb, cudaStream_t s) {
+// Words per lane: two (tiles of 128 bf16 or 64 fp32 channels) halve the instructions per channel
+// that a tile costs beside the arithmetic; one where half of a wide tile would be empty.
+static int scan_words(int64_t ds, int es) { return ds * es % 256 == 0 || ds * es > 1024 ? 2 : 1; }
+
+template <typename T, int W, bool RESET, int CB, bool BWD>
+static void scan_launch(const ScanParams& p, cudaStream_t s) {
+  constexpr int V = kV<T, W>;
+  constexpr int smem = BWD ? kBwdSmem<V, W> : 2 * kWarps * 3 * kRows * 128 * W;
+  const int64_t most = (int64_t)num_sms() * (BWD ? kBwdCtas<W> : kFwdCtas<W>);
+  const unsigned grid = (unsigned)(p.ntiles < most ? p.ntiles : most);
+  if constexpr (BWD) {
+    cudaFuncSetAttribute(gated_scan_bwd_kernel<T, W, RESET, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    gated_scan_bwd_kernel<T, W, RESET, CB><<<grid, kWarps * 32, smem, s>>>(p);
+  } else {
+    cudaFuncSetAttribute(gated_scan_fwd_kernel<T, W, RESET, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    gated_scan_fwd_kernel<T, W, RESET, CB><<<grid, kWarps * 32, smem, s>>>(p);
+  }
+}
+template <typename T, int W, bool BWD>
+static void scan_launch(const ScanParams& p, int cb, cudaStream_t s) {
   constexpr int least = sizeof(T) == 4 ? 4 : 0;  // fp32 rows always allow 4 bytes
-  if (cb == 16) p.reset ? scan_fwd_launch<T, true, 16>(p, s) : scan_fwd_launch<T, false, 16>(p, s);
-  else if (cb == 4) p.reset ? scan_fwd_launch<T, true, 4>(p, s) : scan_fwd_launch<T, false, 4>(p, s);
-  else p.reset ? scan_fwd_launch<T, true, least>(p, s) : scan_fwd_launch<T, false, least>(p, s);
+  if (cb == 16) p.reset ? scan_launch<T, W, true, 16, BWD>(p, s) : scan_launch<T, W, false, 16, BWD>(p, s);
+  else if (cb == 4) p.reset ? scan_launch<T, W, true, 4, BWD>(p, s) : scan_launch<T, W, false, 4, BWD>(p, s);
+  else p.reset ? scan_launch<T, W, true, least, BWD>(p, s) : scan_launch<T, W, false, least, BWD>(p, s);
+}
+template <bool BWD>
+static void scan_launch(const ScanParams& p, int dtype, int W, int cb, cudaStream_t s) {
+  constexpr int most = BWD ? 1 : 2;
+  if (dtype == HDC_F32) W == 2 ? scan_launch<float, most, BWD>(p, cb, s) : scan_launch<float, 1, BWD>(p, cb, s);
+  else W == 2 ? scan_launch<__nv_bfloat16, most, BWD>(p, cb, s) : scan_launch<__nv_bfloat16, 1, BWD>(p, cb, s);
 }
 
 }  // namespace hdc
@@ -675,12 +931,11 @@ extern "C" int hdc_gated_scan_fwd(int dtype, int a_dtype, const void* projs, int
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(HDC_E_WORKSPACE, "gated_scan: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   if (!aligned16(workspace)) return fail(HDC_E_ALIGN, "gated_scan: the workspace is not 16-byte aligned");
-  if (B * ((ds + 31) / 32) > (int64_t(1) << 30) || B * ((ds + 31) / 32) * ((L + kStateRows - 1) / kStateRows) > (int64_t(1) << 31))
-    return fail(HDC_E_SHAPE, "gated_scan: B=%lld x L=%lld x d_state=%lld is too large", (long long)B, (long long)L, (long long)ds);
+  if (int e = scan_fits("gated_scan", B, L, ds)) return e;
   ScanParams p{};
   p.projs = projs; p.psb = proj_sb; p.pst = proj_st; p.A_log = A_log; p.a_bf16 = a_dtype == HDC_BF16;
   p.h0 = h0; p.reset = reset; p.y = y; p.ysb = y_sb; p.yst = y_st; p.h_last = h_last; p.states = states;
-  p.B = (int)B; p.L = (int)L; p.ds = (int)ds; p.NT = (int)((L + kStateRows - 1) / kStateRows);
+  p.B = (int)B; p.L = (int)L; p.ds = (int)ds; p.NT = (int)tiles_in_time(L);
   auto s = reinterpret_cast<cudaStream_t>(stream);
   if (L == 0) {  // nothing to scan: the state stays as it is
     if (!h_last) return HDC_OK;
@@ -688,22 +943,22 @@ extern "C" int hdc_gated_scan_fwd(int dtype, int a_dtype, const void* projs, int
                              : cudaMemsetAsync(h_last, 0, (size_t)B * ds * 4, s);
     return e == cudaSuccess ? HDC_OK : fail((int)e, "gated_scan: %s", cudaGetErrorString(e));
   }
-  const int es = dtype == HDC_F32 ? 4 : 2;
-  scan_plan(p, 128 / es, workspace);
-  p.out_vec = rows_allow(y, y_sb, y_st, es, 4);
+  const int es = dtype == HDC_F32 ? 4 : 2, W = scan_words(ds, es);
+  scan_plan(p, 128 * W / es, workspace);
+  p.out_vec = rows_allow(y, y_sb, y_st, es, 4 * W);
   if (int e = scan_clear(p, s, "gated_scan")) return e;
   const int cb = rows_allow(projs, proj_sb, proj_st, es, 16) && ds * es % 16 == 0 ? 16
                  : rows_allow(projs, proj_sb, proj_st, es, 4) && ds * es % 4 == 0 ? 4 : 0;
-  if (dtype == HDC_F32) scan_fwd_launch<float>(p, cb, s);
-  else scan_fwd_launch<__nv_bfloat16>(p, cb, s);
+  scan_launch<false>(p, dtype, W, cb, s);
   return launch_status("gated_scan_fwd_kernel");
 }
 
 extern "C" size_t hdc_gated_scan_workspace_bytes(int64_t B, int64_t L, int64_t ds) { return scan_ws(B, L, ds); }
 
+// the forward's, then the tiles' parts of dA
 extern "C" size_t hdc_gated_scan_bwd_workspace_bytes(int64_t B, int64_t L, int64_t ds) {
-  if (B < 1 || L < 0 || ds < 1) return 0;
-  return (size_t)B * ds * 4 * (1 + L);
+  if (B < 1 || L < 1 || ds < 1) return 0;
+  return scan_ws(B, L, ds) + (size_t)tiles_in_time(L) * B * scan_pad(ds) * 4;
 }
 
 extern "C" int hdc_gated_scan_bwd(int dtype, int a_dtype, const void* projs, int64_t proj_sb, int64_t proj_st,
@@ -723,20 +978,32 @@ extern "C" int hdc_gated_scan_bwd(int dtype, int a_dtype, const void* projs, int
   const size_t need = hdc_gated_scan_bwd_workspace_bytes(B, L, ds);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(HDC_E_WORKSPACE, "gated_scan_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  if (!aligned16(workspace)) return fail(HDC_E_ALIGN, "gated_scan_bwd: the workspace is not 16-byte aligned");
+  if (int e = scan_fits("gated_scan_bwd", B, L, ds)) return e;
   ScanParams p{};
   p.projs = projs; p.psb = proj_sb; p.pst = proj_st; p.A_log = A_log; p.a_bf16 = a_dtype == HDC_BF16;
   p.reset = reset; p.states = const_cast<float*>(states); p.dy = dy; p.dsb = dy_sb; p.dst = dy_st;
   p.dh_last = dh_last; p.dprojs = dprojs; p.gsb = dp_sb; p.gst = dp_st; p.dh0 = dh0;
-  p.dA_part = static_cast<float*>(workspace); p.hbuf = p.dA_part + B * ds;
-  p.B = (int)B; p.L = (int)L; p.ds = (int)ds; p.NT = (int)((L + kStateRows - 1) / kStateRows);
+  p.B = (int)B; p.L = (int)L; p.ds = (int)ds; p.NT = (int)tiles_in_time(L);
   auto s = reinterpret_cast<cudaStream_t>(stream);
-  if (B > 0) {
-    const unsigned grid = (unsigned)((B * ds + 127) / 128);
-    if (dtype == HDC_F32) gated_scan_bwd_kernel<float><<<grid, 128, 0, s>>>(p);
-    else gated_scan_bwd_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(p);
+  const int es = dtype == HDC_F32 ? 4 : 2, W = 1;
+  scan_plan(p, 128 * W / es, workspace);
+  if (B > 0 && L > 0) {
+    p.dA_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + scan_ws(B, L, ds));
+    p.out_vec = rows_allow(dprojs, dp_sb, dp_st, es, 4 * W) && ds * es % (4 * W) == 0;
+    if (int e = scan_clear(p, s, "gated_scan_bwd")) return e;
+    const bool in = ds * es % 4 == 0 && rows_allow(projs, proj_sb, proj_st, es, 4) && rows_allow(dy, dy_sb, dy_st, es, 4);
+    const int cb = in && ds * es % 16 == 0 && rows_allow(projs, proj_sb, proj_st, es, 16) &&
+                   rows_allow(dy, dy_sb, dy_st, es, 16) ? 16 : in ? 4 : 0;
+    scan_launch<true>(p, dtype, W, cb, s);
     if (int e = launch_status("gated_scan_bwd_kernel")) return e;
+  } else if (dh0 && B > 0) {  // no steps: the gradient passes through
+    const cudaError_t e = dh_last ? cudaMemcpyAsync(dh0, dh_last, (size_t)B * ds * 4, cudaMemcpyDeviceToDevice, s)
+                                  : cudaMemsetAsync(dh0, 0, (size_t)B * ds * 4, s);
+    if (e != cudaSuccess) return fail((int)e, "gated_scan_bwd: %s", cudaGetErrorString(e));
   }
-  gated_scan_dA_kernel<<<(unsigned)((ds + 127) / 128), 128, 0, s>>>(p.dA_part, (int)B, (int)ds, dA_log, p.a_bf16);
+  gated_scan_dA_kernel<<<(unsigned)((ds + 31) / 32), 256, 0, s>>>(p.dA_part, (int64_t)p.NT * B, p.nch * p.CW, (int)ds,
+                                                                  A_log, p.a_bf16, dA_log);
   return launch_status("gated_scan_dA_kernel");
 }
 
