@@ -7,7 +7,20 @@
 // S = 1 is the Block's norm of each head and token (hdcmamba/model.py:285-292).
 // Statistics and sums are fp32; y, dx, dw, db are rounded once to their types.
 //
-// Schedule: one CTA per (n, g).
+// Schedules (bound by HBM: x read and y written; x, dy read and dx written):
+//   * one position (S = 1): a group is Cg neighbouring values.  A few lanes (LG, a power of two)
+//     hold one group of one sample in registers, with its mean, its centred squares (or the two
+//     sums of the gradient) summed by shuffles; a CTA covers whole samples, and a thread keeps its
+//     channels from sample to sample, so that weight and bias stay in registers and dw and db
+//     accumulate there.  One pass over the data.
+//   * otherwise two passes: a CTA takes a slice of a sample's positions, a thread a few channels
+//     of every RL-th of them.  First each slice's statistics (or sums of the gradient), then, with
+//     the slices of a sample joined in their order, the outputs; the second reading of the
+//     input comes from L2 where it fits (126 MB).
+// Statistics never cancel: a thread takes blocks of rows, each with its own mean and centred
+// squares, and blocks, threads and slices are joined by
+//   n = n1 + n2, mean = mean1 + (mean2 - mean1) n2/n, M2 = M2_1 + M2_2 + (mean2 - mean1)^2 n1 n2/n.
+// Channels per load: as many as 16 bytes, the rows' alignment and (S = 1) the group allow.
 #include "common.cuh"
 
 namespace hdc {
@@ -19,9 +32,14 @@ struct GnParams {
   float* mean; float* rstd;
   const void* dy; int64_t dsn, dss;
   void* dx; int64_t gsn, gss;
-  float* part;  // [N, 2, C] sums of dz xh and dz
+  float* part;     // gradient: sums of dz xh and of dz per channel, [part][2][C]
+  float2* stats;   // two passes: (mean, M2) of each slice, [N][slices][G]
+  void* dw; void* db;
   int N, S, C, G, Cg;
   float eps; int silu;
+  int slices, rows;  // two passes: slices per sample, positions per slice
+  int cb;            // two passes: channels per CTA (whole groups, or all)
+  int whole;         // the rows allow whole loads (else one by one, with the same arithmetic)
 };
 
 __device__ __forceinline__ float gn_param(const void* p, int bf16, int i, float none) {
@@ -29,6 +47,515 @@ __device__ __forceinline__ float gn_param(const void* p, int bf16, int i, float 
   return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];
 }
 
+// VE neighbouring values as loaded, at once or (rows that do not allow it) one by one
+template <typename T, int VE> struct Raw { static constexpr int kW = VE * (int)sizeof(T) >= 4 ? VE * (int)sizeof(T) / 4 : 1; uint32_t w[kW]; };
+template <typename T, int VE> __device__ __forceinline__ Raw<T, VE> ld_raw(const T* p, int whole) {
+  Raw<T, VE> r;
+  constexpr int bytes = VE * (int)sizeof(T);
+  if (VE > 1 && !whole) {
+#pragma unroll
+    for (int i = 0; i < Raw<T, VE>::kW; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        r.w[i] = __float_as_uint(p[i]);
+      } else {
+        const unsigned short* q = reinterpret_cast<const unsigned short*>(p) + 2 * i;
+        r.w[i] = q[0] | (uint32_t)q[VE > 1 ? 1 : 0] << 16;
+      }
+    }
+    return r;
+  }
+  if constexpr (bytes == 16) {
+    const uint4 q = ldg16(p);
+    r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
+  } else if constexpr (bytes == 8) {
+    const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
+    r.w[0] = q.x; r.w[1] = q.y;
+  } else if constexpr (bytes == 4) {
+    r.w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  } else {
+    r.w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
+  }
+  return r;
+}
+template <typename T, int VE> __device__ __forceinline__ void unpack(const Raw<T, VE>& r, float (&f)[VE]) {
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    if constexpr (sizeof(T) == 4) f[i] = __uint_as_float(r.w[i]);
+    else f[i] = __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
+  }
+}
+template <typename T, int VE> __device__ __forceinline__ void st_vec(T* p, const float (&f)[VE], int whole) {
+  constexpr int bytes = VE * (int)sizeof(T);
+  if (VE > 1 && !whole) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) p[i] = from_f<T>(f[i]);
+    return;
+  }
+  if constexpr (bytes == 2) {
+    *p = from_f<T>(f[0]);
+  } else {
+    uint32_t w[bytes / 4];
+#pragma unroll
+    for (int i = 0; i < bytes / 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[i] = __float_as_uint(f[i]);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    if constexpr (bytes == 16) stg16(p, make_uint4(w[0], w[1], w[2], w[3]));
+    else if constexpr (bytes == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
+  }
+}
+
+// sigmoid: hardware 2^x and reciprocal for bf16 tensors (a few 2^-23 off), the library's for fp32
+template <typename T> __device__ __forceinline__ float gn_sigmoid(float z) {
+  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-z));
+  else return __fdividef(1.f, 1.f + __expf(-z));
+}
+template <typename T> __device__ __forceinline__ float gn_act(float z, int silu) {
+  return silu ? z * gn_sigmoid<T>(z) : z;
+}
+// dz from dy
+template <typename T> __device__ __forceinline__ float gn_dact(float dy, float z, int silu) {
+  if (!silu) return dy;
+  const float q = gn_sigmoid<T>(z);
+  return dy * (q * fmaf(z, 1.f - q, 1.f));
+}
+__device__ __forceinline__ float gn_rstd(float M2, float n, float eps) { return 1.f / sqrtf(M2 / n + eps); }
+
+// ---------------------------------------------------------------- one position per sample
+// The lanes of a group: LG of them, CPL loads of VE channels each: channel (k LG + l) VE + i of
+// the group.  Threads: (sample of the CTA, group, lane), groups from blockIdx.y * gpc.
+template <int LG> __device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = LG / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T, int VE, int CPL, int U, bool BWD, int LG>
+__global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnParams p, int gpc, int spc) {
+  const int l = threadIdx.x % LG, gi = threadIdx.x / LG % gpc, sr = threadIdx.x / LG / gpc;
+  const int g = blockIdx.y * gpc + gi;
+  const bool live = g < p.G && sr < spc;
+  const int gc = live ? g : 0, c0 = gc * p.Cg;
+  constexpr int M = VE * CPL;
+  int ch[CPL];
+  bool in[CPL];
+  float w[M], b[M];
+#pragma unroll
+  for (int k = 0; k < CPL; ++k) {
+    const int c = (k * LG + l) * VE;
+    in[k] = live && c < p.Cg;
+    ch[k] = c0 + (c < p.Cg ? c : 0);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      w[k * VE + i] = gn_param(p.w, p.p_bf16, ch[k] + i, 1.f);
+      b[k * VE + i] = gn_param(p.b, p.p_bf16, ch[k] + i, 0.f);
+    }
+  }
+  const float inv = 1.f / (float)p.Cg;
+  float dw[BWD ? M : 1], db[BWD ? M : 1];
+#pragma unroll
+  for (int i = 0; i < (BWD ? M : 1); ++i) dw[i] = db[i] = 0.f;
+
+  const int64_t step = (int64_t)gridDim.x * spc;
+  for (int64_t n0 = (int64_t)blockIdx.x * spc; n0 < p.N; n0 += step * U) {
+    Raw<T, VE> xr[U][CPL], dr[BWD ? U : 1][CPL];
+    float mu[U], rs[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t n = n0 + u * step + sr;
+      const bool ok = live && n < p.N;
+      const int64_t nn = ok ? n : 0;
+#pragma unroll
+      for (int k = 0; k < CPL; ++k) {
+        xr[u][k] = ld_raw<T, VE>(static_cast<const T*>(p.x) + nn * p.xsn + ch[k], p.whole);
+        if constexpr (BWD) dr[u][k] = ld_raw<T, VE>(static_cast<const T*>(p.dy) + nn * p.dsn + ch[k], p.whole);
+      }
+      if constexpr (BWD) {
+        mu[u] = p.mean[nn * p.G + gc];
+        rs[u] = p.rstd[nn * p.G + gc];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t n = n0 + u * step + sr;
+      const bool ok = live && n < p.N;
+      float x[M];
+#pragma unroll
+      for (int k = 0; k < CPL; ++k) {
+        float f[VE];
+        unpack<T, VE>(xr[u][k], f);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) x[k * VE + i] = f[i];
+      }
+      if constexpr (!BWD) {
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < CPL; ++k)
+#pragma unroll
+          for (int i = 0; i < VE; ++i) s += in[k] ? x[k * VE + i] : 0.f;
+        const float mean = group_sum<LG>(s) / (float)p.Cg;
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < CPL; ++k)
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            x[k * VE + i] -= mean;
+            s = in[k] ? fmaf(x[k * VE + i], x[k * VE + i], s) : s;
+          }
+        const float rstd = gn_rstd(group_sum<LG>(s), (float)p.Cg, p.eps);
+        if (ok) {
+#pragma unroll
+          for (int k = 0; k < CPL; ++k)
+            if (in[k]) {
+              float f[VE];
+#pragma unroll
+              for (int i = 0; i < VE; ++i)
+                f[i] = gn_act<T>(fmaf(x[k * VE + i] * rstd, w[k * VE + i], b[k * VE + i]), p.silu);
+              st_vec<T, VE>(static_cast<T*>(p.y) + n * p.ysn + ch[k], f, p.whole);
+            }
+          if (l == 0 && p.mean) {
+            p.mean[n * p.G + g] = mean;
+            p.rstd[n * p.G + g] = rstd;
+          }
+        }
+      } else {
+        float e[M], se = 0.f, sx = 0.f;
+#pragma unroll
+        for (int k = 0; k < CPL; ++k) {
+          float f[VE];
+          unpack<T, VE>(dr[u][k], f);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            const int m = k * VE + i;
+            x[m] = (x[m] - mu[u]) * rs[u];
+            const float dz = gn_dact<T>(f[i], fmaf(x[m], w[m], b[m]), p.silu);
+            if (ok && in[k]) {
+              dw[m] = fmaf(dz, x[m], dw[m]);
+              db[m] += dz;
+              e[m] = dz * w[m];
+              se += e[m];
+              sx = fmaf(e[m], x[m], sx);
+            }
+          }
+        }
+        se = group_sum<LG>(se) * inv;
+        sx = group_sum<LG>(sx) * inv;
+        if (ok) {
+#pragma unroll
+          for (int k = 0; k < CPL; ++k)
+            if (in[k]) {
+              float f[VE];
+#pragma unroll
+              for (int i = 0; i < VE; ++i) f[i] = rs[u] * (e[k * VE + i] - se - x[k * VE + i] * sx);
+              st_vec<T, VE>(static_cast<T*>(p.dx) + n * p.gsn + ch[k], f, p.whole);
+            }
+        }
+      }
+    }
+  }
+  if constexpr (BWD) {  // the CTA's sums over its samples, in their order
+    extern __shared__ float sh[];  // [spc][gpc * LG][M]
+    const int per = gpc * LG, q = threadIdx.x % per;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+      if (sr < spc) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) sh[((size_t)sr * M + i) * per + q] = which ? db[i] : dw[i];
+      }
+      __syncthreads();
+      if (sr == 0 && live) {
+#pragma unroll
+        for (int k = 0; k < CPL; ++k)
+          if (in[k])
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+              float v = 0.f;
+              for (int r = 0; r < spc; ++r) v += sh[((size_t)r * M + k * VE + i) * per + q];
+              p.part[((int64_t)blockIdx.x * 2 + which) * p.C + ch[k] + i] = v;
+            }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- several positions per sample
+// CTA (slice, sample, channel block): thread = (row lane, chunk of VE channels).
+struct GnStat { float n, mean, M2; };
+__device__ __forceinline__ GnStat join(const GnStat& a, const GnStat& b) {
+  const float n = a.n + b.n;
+  if (n == 0.f) return a;
+  const float d = b.mean - a.mean, f = b.n / n;
+  return {n, fmaf(d, f, a.mean), a.M2 + b.M2 + d * d * (a.n * f)};
+}
+constexpr int kGnThreads = 256;
+// row lanes of a CTA: threads per chunk of channels (one when a thread has several chunks)
+__host__ __device__ inline int gn_lanes(int nchunk) { return nchunk < kGnThreads ? kGnThreads / nchunk : 1; }
+
+template <typename T, int VE>
+__global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(const __grid_constant__ GnParams p) {
+  extern __shared__ float sh[];  // [2][row lanes][cb]: mean, M2
+  const int c_lo = blockIdx.y * p.cb, cw = min(p.cb, p.C - c_lo), nchunk = cw / VE;
+  const int RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
+  const int n = blockIdx.x / p.slices, slice = blockIdx.x - n * p.slices, r0 = slice * p.rows, rows = min(p.rows, p.S - r0);
+  constexpr int U = 8;
+  if (rl < RL)
+  for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
+    const T* x = static_cast<const T*>(p.x) + n * p.xsn + (int64_t)r0 * p.xss + c_lo + k * VE;
+    float mean[VE], M2[VE], cnt = 0.f;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) mean[i] = M2[i] = 0.f;
+    int r = rl;
+    for (; r + (U - 1) * RL < rows; r += U * RL) {
+      Raw<T, VE> raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
+      float v[U][VE];
+#pragma unroll
+      for (int u = 0; u < U; ++u) unpack<T, VE>(raw[u], v[u]);
+      const float total = cnt + U, f = U / total, g = cnt * f;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        float s = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) s += v[u][i];
+        const float m = s * (1.f / U), d = m - mean[i];
+        s = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) s = fmaf(v[u][i] - m, v[u][i] - m, s);
+        M2[i] += fmaf(d * d, g, s);
+        mean[i] = fmaf(d, f, mean[i]);
+      }
+      cnt = total;
+    }
+    for (; r < rows; r += RL) {
+      float v[VE];
+      unpack<T, VE>(ld_raw<T, VE>(x + (int64_t)r * p.xss, p.whole), v);
+      const float total = cnt + 1.f, f = 1.f / total;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const float d = v[i] - mean[i];
+        mean[i] = fmaf(d, f, mean[i]);
+        M2[i] = fmaf(d * d, cnt * f, M2[i]);
+      }
+      cnt = total;
+    }
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      sh[rl * cw + k * VE + i] = mean[i];
+      sh[(RL + rl) * cw + k * VE + i] = M2[i];
+    }
+  }
+  __syncthreads();
+  // channels over the row lanes, then groups over their channels
+  auto count = [&](int q) { return rows > q ? (float)((rows - q - 1) / RL + 1) : 0.f; };
+  for (int c = threadIdx.x; c < cw; c += kGnThreads) {
+    GnStat a = {count(0), sh[c], sh[RL * cw + c]};
+    for (int q = 1; q < RL; ++q) a = join(a, {count(q), sh[q * cw + c], sh[(RL + q) * cw + c]});
+    sh[c] = a.mean;  // only this thread reads and writes this channel here
+    sh[RL * cw + c] = a.M2;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int gi = threadIdx.x >> 5; gi < cw / p.Cg; gi += kGnThreads / 32) {
+    GnStat a = {0.f, 0.f, 0.f};
+    for (int c = lane; c < p.Cg; c += 32) a = join(a, {(float)rows, sh[gi * p.Cg + c], sh[RL * cw + gi * p.Cg + c]});
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      a = join(a, {__shfl_down_sync(0xffffffffu, a.n, o), __shfl_down_sync(0xffffffffu, a.mean, o),
+                   __shfl_down_sync(0xffffffffu, a.M2, o)});
+    if (lane == 0) p.stats[(int64_t)blockIdx.x * p.G + c_lo / p.Cg + gi] = make_float2(a.mean, a.M2);
+  }
+}
+
+template <typename T, int VE>
+__global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(const __grid_constant__ GnParams p) {
+  extern __shared__ float sh[];  // [2][groups of the block]: mean, rstd
+  const int c_lo = blockIdx.y * p.cb, cw = min(p.cb, p.C - c_lo), nchunk = cw / VE, ng = cw / p.Cg;
+  const int n = blockIdx.x / p.slices, slice = blockIdx.x - n * p.slices, r0 = slice * p.rows, rows = min(p.rows, p.S - r0);
+  for (int gi = threadIdx.x; gi < ng; gi += kGnThreads) {
+    const float2* st = p.stats + (int64_t)n * p.slices * p.G + c_lo / p.Cg + gi;
+    GnStat a = {0.f, 0.f, 0.f};
+    for (int q = 0; q < p.slices; ++q) {
+      const float2 v = st[(int64_t)q * p.G];
+      a = join(a, {(float)min(p.rows, p.S - q * p.rows) * (float)p.Cg, v.x, v.y});
+    }
+    const float rstd = gn_rstd(a.M2, a.n, p.eps);
+    sh[gi] = a.mean;
+    sh[ng + gi] = rstd;
+    if (p.mean && slice == 0) {
+      p.mean[(int64_t)n * p.G + c_lo / p.Cg + gi] = a.mean;
+      p.rstd[(int64_t)n * p.G + c_lo / p.Cg + gi] = rstd;
+    }
+  }
+  __syncthreads();
+  const int RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
+  if (rl >= RL) return;
+  for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
+    float mean[VE], sc[VE], b[VE];
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      const int c = k * VE + i;
+      mean[i] = sh[c / p.Cg];
+      sc[i] = sh[ng + c / p.Cg] * gn_param(p.w, p.p_bf16, c_lo + c, 1.f);
+      b[i] = gn_param(p.b, p.p_bf16, c_lo + c, 0.f);
+    }
+    const T* x = static_cast<const T*>(p.x) + n * p.xsn + (int64_t)r0 * p.xss + c_lo + k * VE;
+    T* y = static_cast<T*>(p.y) + n * p.ysn + (int64_t)r0 * p.yss + c_lo + k * VE;
+    constexpr int U = 4;
+    for (int r = rl; r < rows; r += U * RL) {
+      Raw<T, VE> raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + u * RL < rows) raw[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + u * RL < rows) {
+          float v[VE];
+          unpack<T, VE>(raw[u], v);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) v[i] = gn_act<T>(fmaf(v[i] - mean[i], sc[i], b[i]), p.silu);
+          st_vec<T, VE>(y + (int64_t)(r + u * RL) * p.yss, v, p.whole);
+        }
+    }
+  }
+}
+
+// The gradient's sums per channel of each slice: part[n * slices + slice][2][C]
+template <typename T, int VE>
+__global__ void __launch_bounds__(kGnThreads) gn_sums_kernel(const __grid_constant__ GnParams p) {
+  extern __shared__ float sh[];  // [2][row lanes][cb]
+  const int c_lo = blockIdx.y * p.cb, cw = min(p.cb, p.C - c_lo), nchunk = cw / VE;
+  const int RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
+  const int n = blockIdx.x / p.slices, slice = blockIdx.x - n * p.slices, r0 = slice * p.rows, rows = min(p.rows, p.S - r0);
+  if (rl < RL)
+  for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
+    float mean[VE], rstd[VE], w[VE], b[VE], a0[VE], a1[VE];
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      const int c = c_lo + k * VE + i;
+      mean[i] = p.mean[(int64_t)n * p.G + c / p.Cg];
+      rstd[i] = p.rstd[(int64_t)n * p.G + c / p.Cg];
+      w[i] = gn_param(p.w, p.p_bf16, c, 1.f);
+      b[i] = gn_param(p.b, p.p_bf16, c, 0.f);
+      a0[i] = a1[i] = 0.f;
+    }
+    const T* x = static_cast<const T*>(p.x) + n * p.xsn + (int64_t)r0 * p.xss + c_lo + k * VE;
+    const T* dy = static_cast<const T*>(p.dy) + n * p.dsn + (int64_t)r0 * p.dss + c_lo + k * VE;
+    constexpr int U = 4;
+    for (int r = rl; r < rows; r += U * RL) {
+      Raw<T, VE> xr[U], dr[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + u * RL < rows) {
+          xr[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
+          dr[u] = ld_raw<T, VE>(dy + (int64_t)(r + u * RL) * p.dss, p.whole);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + u * RL < rows) {
+          float v[VE], d[VE];
+          unpack<T, VE>(xr[u], v);
+          unpack<T, VE>(dr[u], d);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            const float xh = (v[i] - mean[i]) * rstd[i];
+            const float dz = gn_dact<T>(d[i], fmaf(xh, w[i], b[i]), p.silu);
+            a0[i] = fmaf(dz, xh, a0[i]);
+            a1[i] += dz;
+          }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      sh[rl * cw + k * VE + i] = a0[i];
+      sh[(RL + rl) * cw + k * VE + i] = a1[i];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * cw; i += kGnThreads) {
+    const int which = i >= cw, c = which ? i - cw : i;
+    float v = 0.f;
+    for (int q = 0; q < RL; ++q) v += sh[(which * RL + q) * cw + c];
+    p.part[((int64_t)blockIdx.x * 2 + which) * p.C + c_lo + c] = v;
+  }
+}
+
+template <typename T, int VE>
+__global__ void __launch_bounds__(kGnThreads) gn_dx_kernel(const __grid_constant__ GnParams p) {
+  extern __shared__ float sh[];  // [2][cb] channel sums times w, then [2][groups]
+  const int c_lo = blockIdx.y * p.cb, cw = min(p.cb, p.C - c_lo), nchunk = cw / VE, ng = cw / p.Cg;
+  const int n = blockIdx.x / p.slices, slice = blockIdx.x - n * p.slices, r0 = slice * p.rows, rows = min(p.rows, p.S - r0);
+  float* gs = sh + 2 * cw;
+  for (int i = threadIdx.x; i < 2 * cw; i += kGnThreads) {
+    const int which = i >= cw, c = which ? i - cw : i;
+    const float* q = p.part + ((int64_t)n * p.slices * 2 + which) * p.C + c_lo + c;
+    float v = 0.f;
+    for (int k = 0; k < p.slices; ++k) v += q[(int64_t)k * 2 * p.C];
+    sh[i] = v * gn_param(p.w, p.p_bf16, c_lo + c, 1.f);
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  const float inv = 1.f / ((float)p.S * (float)p.Cg);
+  for (int i = threadIdx.x >> 5; i < 2 * ng; i += kGnThreads / 32) {
+    const int which = i >= ng, gi = which ? i - ng : i;
+    float v = 0.f;
+    for (int c = lane; c < p.Cg; c += 32) v += sh[which * cw + gi * p.Cg + c];
+    v = warp_sum(v);
+    if (lane == 0) gs[i] = v * inv;
+  }
+  __syncthreads();
+  const int RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
+  if (rl >= RL) return;
+  for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
+    float mean[VE], rstd[VE], w[VE], b[VE], sx[VE], se[VE];
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      const int c = c_lo + k * VE + i, gi = (k * VE + i) / p.Cg;
+      mean[i] = p.mean[(int64_t)n * p.G + c / p.Cg];
+      rstd[i] = p.rstd[(int64_t)n * p.G + c / p.Cg];
+      w[i] = gn_param(p.w, p.p_bf16, c, 1.f);
+      b[i] = gn_param(p.b, p.p_bf16, c, 0.f);
+      sx[i] = gs[gi];
+      se[i] = gs[ng + gi];
+    }
+    const T* x = static_cast<const T*>(p.x) + n * p.xsn + (int64_t)r0 * p.xss + c_lo + k * VE;
+    const T* dy = static_cast<const T*>(p.dy) + n * p.dsn + (int64_t)r0 * p.dss + c_lo + k * VE;
+    T* dx = static_cast<T*>(p.dx) + n * p.gsn + (int64_t)r0 * p.gss + c_lo + k * VE;
+    constexpr int U = 4;
+    for (int r = rl; r < rows; r += U * RL) {
+      Raw<T, VE> xr[U], dr[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + u * RL < rows) {
+          xr[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
+          dr[u] = ld_raw<T, VE>(dy + (int64_t)(r + u * RL) * p.dss, p.whole);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + u * RL < rows) {
+          float v[VE], d[VE];
+          unpack<T, VE>(xr[u], v);
+          unpack<T, VE>(dr[u], d);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            const float xh = (v[i] - mean[i]) * rstd[i];
+            const float dz = gn_dact<T>(d[i], fmaf(xh, w[i], b[i]), p.silu);
+            v[i] = rstd[i] * (fmaf(dz, w[i], -se[i]) - xh * sx[i]);
+          }
+          st_vec<T, VE>(dx + (int64_t)(r + u * RL) * p.gss, v, p.whole);
+        }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- groups of more than 4096 channels
+// One CTA per (n, g), the group read again for each of its sums.
 __device__ __forceinline__ float block_sum(float v) {
   __shared__ float red[8];
   v = warp_sum(v);
@@ -41,7 +568,7 @@ __device__ __forceinline__ float block_sum(float v) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) gn_fwd_kernel(GnParams p) {
+__global__ void __launch_bounds__(256) gn_any_fwd_kernel(GnParams p) {
   const int n = blockIdx.x / p.G, g = blockIdx.x - n * p.G;
   const T* x = static_cast<const T*>(p.x) + n * p.xsn + g * p.Cg;
   T* y = static_cast<T*>(p.y) + n * p.ysn + g * p.Cg;
@@ -69,7 +596,7 @@ __global__ void __launch_bounds__(256) gn_fwd_kernel(GnParams p) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) gn_bwd_kernel(GnParams p) {
+__global__ void __launch_bounds__(256) gn_any_bwd_kernel(GnParams p) {
   const int n = blockIdx.x / p.G, g = blockIdx.x - n * p.G;
   const T* x = static_cast<const T*>(p.x) + n * p.xsn + g * p.Cg;
   const T* dy = static_cast<const T*>(p.dy) + n * p.dsn + g * p.Cg;
@@ -116,16 +643,148 @@ __global__ void __launch_bounds__(256) gn_bwd_kernel(GnParams p) {
   }
 }
 
-// dw[c], db[c]: sums of the parts in their order (blockIdx.y: 0 dw, 1 db)
-__global__ void gn_param_grad_kernel(const float* part, int parts, int C, void* dw, void* db, int bf16) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= C) return;
+// dw[c] (blockIdx.y 0) and db[c] (1): sums of the parts, 8 strands per channel, then the strands
+__global__ void __launch_bounds__(256) gn_param_grad_kernel(const float* part, int64_t parts, int C, void* dw, void* db,
+                                                            int bf16) {
+  __shared__ float s[8][32];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
   void* out = blockIdx.y ? db : dw;
   if (!out) return;
-  float s = 0.f;
-  for (int k = 0; k < parts; ++k) s += part[((int64_t)k * 2 + blockIdx.y) * C + c];
-  if (bf16) static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn(s);
-  else static_cast<float*>(out)[c] = s;
+  float v = 0.f;
+  if (c < C) {
+#pragma unroll 4
+    for (int64_t i = k; i < parts; i += 8) v += part[(i * 2 + blockIdx.y) * C + c];
+  }
+  s[k][threadIdx.x & 31] = v;
+  __syncthreads();
+  if (k != 0 || c >= C) return;
+  for (int i = 1; i < 8; ++i) v += s[i][threadIdx.x];
+  if (bf16) static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn(v);
+  else static_cast<float*>(out)[c] = v;
+}
+
+// ---------------------------------------------------------------- plans
+constexpr int kGnMostCg = 4096;  // channels of a group in the kernels above
+
+// One position: loads of ve channels, LG lanes and CPL loads per group.
+struct GnRowPlan { bool ok; int lg, cpl, gpc, spc, gy; int64_t ctas; };
+static GnRowPlan gn_row_plan(int64_t N, int64_t S, int64_t G, int64_t Cg, int ve) {
+  GnRowPlan r{};
+  const int64_t chunks = Cg / ve;
+  r.lg = 1;
+  while (r.lg < 32 && r.lg < chunks) r.lg *= 2;
+  r.cpl = 1;
+  while ((int64_t)r.lg * r.cpl < chunks) r.cpl *= 2;
+  r.ok = S == 1 && r.cpl <= 8 && r.cpl * ve <= 32;
+  const int most = 256 / r.lg;  // groups (of any sample) per CTA
+  r.gy = (int)((G + most - 1) / most);
+  r.gpc = (int)((G + r.gy - 1) / r.gy);
+  r.spc = most / r.gpc;
+  const int64_t need = (N + r.spc - 1) / r.spc, fill = (int64_t)148 * 8 / (r.gy < 8 ? r.gy : 8);
+  r.ctas = need < fill ? need : fill;
+  return r;
+}
+// The workspace is sized without knowing the type: for the most CTAs of any width.
+static int64_t gn_row_parts(int64_t N, int64_t G, int64_t Cg) {
+  int64_t most = 0;
+  for (int ve = 1; ve <= 8; ve *= 2)
+    if (Cg % ve == 0) {
+      const GnRowPlan r = gn_row_plan(N, 1, G, Cg, ve);
+      if (r.ok && r.ctas > most) most = r.ctas;
+    }
+  return most;
+}
+// Two passes: slices per sample so that a few CTAs per SM run, each of 32 positions or more.
+struct GnPlan { int64_t slices, rows, cb, gz; };
+static GnPlan gn_plan(int64_t N, int64_t S, int64_t C, int64_t G) {
+  GnPlan r{};
+  const int64_t Cg = C / G;
+  r.cb = C;
+  if (C > 512) {  // blocks of whole groups, about 512 channels
+    int64_t g = 512 / Cg;
+    if (g < 1) g = 1;
+    r.cb = g * Cg;
+  }
+  r.gz = (C + r.cb - 1) / r.cb;
+  const int64_t want = (148 * 8 + N * r.gz - 1) / (N * r.gz);
+  int64_t rows = (S + want - 1) / want;
+  if (rows < 32) rows = 32;
+  if (rows > S) rows = S;
+  r.rows = rows;
+  r.slices = (S + rows - 1) / rows;
+  return r;
+}
+// Channels per load: as many as 16 bytes hold and divide d (the group's channels, or the row's).
+// The layout does not enter, so that it does not change the arithmetic; whether the rows allow
+// such loads does (whole).
+static int gn_width(int es, int64_t d) {
+  int ve = 16 / es;
+  while (d % ve != 0) ve /= 2;
+  return ve;
+}
+static int gn_whole(int es, int ve, const void* const* ptr, const int64_t* stride, int n) {
+  bool ok = true;
+  for (int i = 0; i < n; ++i)
+    ok = ok && reinterpret_cast<uintptr_t>(ptr[i]) % (ve * es) == 0 && stride[2 * i] % ve == 0 && stride[2 * i + 1] % ve == 0;
+  return ok;
+}
+
+template <typename T, int VE, int CPL, bool BWD, int LG>
+static void gn_row_launch(const GnParams& p, const GnRowPlan& r, cudaStream_t s) {
+  constexpr int M = VE * CPL, U = M <= 8 ? (BWD ? 2 : 4) : M <= 16 ? 2 : 1;
+  const int threads = (r.gpc * r.lg * r.spc + 31) / 32 * 32;
+  const size_t smem = BWD ? (size_t)r.spc * r.gpc * r.lg * M * 4 : 0;
+  gn_row_kernel<T, VE, CPL, U, BWD, LG><<<dim3((unsigned)r.ctas, (unsigned)r.gy), threads, smem, s>>>(p, r.gpc, r.spc);
+}
+template <typename T, int VE, int CPL, bool BWD>
+static void gn_row_lanes(const GnParams& p, const GnRowPlan& r, cudaStream_t s) {
+  if constexpr (CPL > 1) {
+    gn_row_launch<T, VE, CPL, BWD, 32>(p, r, s);
+  } else {
+    switch (r.lg) {
+      case 1: return gn_row_launch<T, VE, 1, BWD, 1>(p, r, s);
+      case 2: return gn_row_launch<T, VE, 1, BWD, 2>(p, r, s);
+      case 4: return gn_row_launch<T, VE, 1, BWD, 4>(p, r, s);
+      case 8: return gn_row_launch<T, VE, 1, BWD, 8>(p, r, s);
+      case 16: return gn_row_launch<T, VE, 1, BWD, 16>(p, r, s);
+      default: return gn_row_launch<T, VE, 1, BWD, 32>(p, r, s);
+    }
+  }
+}
+template <typename T, int VE, bool BWD>
+static void gn_row_loads(const GnParams& p, const GnRowPlan& r, cudaStream_t s) {
+  if (r.cpl == 1) return gn_row_lanes<T, VE, 1, BWD>(p, r, s);
+  if (r.cpl == 2) return gn_row_lanes<T, VE, 2, BWD>(p, r, s);
+  if (r.cpl == 4) return gn_row_lanes<T, VE, 4, BWD>(p, r, s);
+  if constexpr (VE <= 4) return gn_row_lanes<T, VE, 8, BWD>(p, r, s);
+}
+template <typename T, bool BWD> static void gn_rows(const GnParams& p, const GnRowPlan& r, int ve, cudaStream_t s) {
+  if (ve == 1) return gn_row_loads<T, 1, BWD>(p, r, s);
+  if (ve == 2) return gn_row_loads<T, 2, BWD>(p, r, s);
+  if (ve == 4) return gn_row_loads<T, 4, BWD>(p, r, s);
+  if constexpr (sizeof(T) == 2) return gn_row_loads<T, 8, BWD>(p, r, s);
+}
+
+enum GnPass { kStats, kApply, kSums, kDx };
+template <typename T, int VE> static void gn_pass(GnPass pass, const GnParams& p, const GnPlan& r, cudaStream_t s) {
+  const dim3 grid((unsigned)(r.slices * p.N), (unsigned)r.gz);
+  const size_t lanes = gn_lanes((int)(r.cb / VE));
+  switch (pass) {
+    case kStats: gn_stats_kernel<T, VE><<<grid, kGnThreads, 2 * lanes * r.cb * 4, s>>>(p); break;
+    case kApply: gn_apply_kernel<T, VE><<<grid, kGnThreads, 2 * (r.cb / p.Cg) * 4, s>>>(p); break;
+    case kSums: gn_sums_kernel<T, VE><<<grid, kGnThreads, 2 * lanes * r.cb * 4, s>>>(p); break;
+    case kDx: gn_dx_kernel<T, VE><<<grid, kGnThreads, 2 * (r.cb + r.cb / p.Cg) * 4, s>>>(p); break;
+  }
+}
+template <typename T> static void gn_pass(GnPass pass, const GnParams& p, const GnPlan& r, int ve, cudaStream_t s) {
+  if (ve == 1) return gn_pass<T, 1>(pass, p, r, s);
+  if (ve == 2) return gn_pass<T, 2>(pass, p, r, s);
+  if (ve == 4) return gn_pass<T, 4>(pass, p, r, s);
+  if constexpr (sizeof(T) == 2) return gn_pass<T, 8>(pass, p, r, s);
+}
+static void gn_pass(GnPass pass, int dtype, const GnParams& p, const GnPlan& r, int ve, cudaStream_t s) {
+  if (dtype == HDC_F32) gn_pass<float>(pass, p, r, ve, s);
+  else gn_pass<__nv_bfloat16>(pass, p, r, ve, s);
 }
 
 static bool gn_off(const void* p, int dtype) {
@@ -147,7 +806,12 @@ static int gn_check(const char* what, int dtype, int p_dtype, int64_t N, int64_t
 
 using namespace hdc;
 
-extern "C" size_t hdc_group_norm_workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G) { return 0; }
+extern "C" size_t hdc_group_norm_workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G) {
+  if (N < 1 || S < 1 || C < 1 || G < 1 || C % G != 0 || C / G > kGnMostCg) return 0;
+  // one position takes no second pass with wider loads if it takes none with single channels
+  if (gn_row_plan(N, S, G, C / G, 1).ok) return 0;
+  return (size_t)N * gn_plan(N, S, C, G).slices * G * 8;
+}
 
 extern "C" int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t x_sn, int64_t x_ss, const void* weight,
                                   const void* bias, void* y, int64_t y_sn, int64_t y_ss, float* mean, float* rstd,
@@ -157,23 +821,52 @@ extern "C" int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t
   if (N == 0 || S == 0) return HDC_OK;
   if (!x || !y || (!mean != !rstd)) return fail(HDC_E_NULL, "group_norm: null pointer");
   if (gn_off(x, dtype) || gn_off(y, dtype) || gn_off(weight, p_dtype) || gn_off(bias, p_dtype) ||
-      gn_off(mean, HDC_F32) || gn_off(rstd, HDC_F32))
+      gn_off(mean, HDC_F32) || gn_off(rstd, HDC_F32) || !aligned16(workspace))
     return fail(HDC_E_ALIGN, "group_norm: a pointer is not aligned to its type");
-  if (workspace_bytes < hdc_group_norm_workspace_bytes(N, S, C, G))
-    return fail(HDC_E_WORKSPACE, "group_norm: workspace of %zu bytes is too small", workspace_bytes);
+  const size_t need = hdc_group_norm_workspace_bytes(N, S, C, G);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(HDC_E_WORKSPACE, "group_norm: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   GnParams p{};
   p.x = x; p.xsn = x_sn; p.xss = x_ss; p.w = weight; p.b = bias; p.p_bf16 = p_dtype == HDC_BF16;
-  p.y = y; p.ysn = y_sn; p.yss = y_ss; p.mean = mean; p.rstd = rstd;
+  p.y = y; p.ysn = y_sn; p.yss = y_ss; p.mean = mean; p.rstd = rstd; p.stats = static_cast<float2*>(workspace);
   p.N = (int)N; p.S = (int)S; p.C = (int)C; p.G = (int)G; p.Cg = (int)(C / G); p.eps = eps;
   p.silu = act == HDC_ACT_SILU;
   auto s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == HDC_F32) gn_fwd_kernel<float><<<(unsigned)(N * G), 256, 0, s>>>(p);
-  else gn_fwd_kernel<__nv_bfloat16><<<(unsigned)(N * G), 256, 0, s>>>(p);
-  return launch_status("gn_fwd_kernel");
+  const int es = dtype == HDC_F32 ? 4 : 2;
+  if (p.Cg > kGnMostCg) {
+    if (dtype == HDC_F32) gn_any_fwd_kernel<float><<<(unsigned)(N * G), 256, 0, s>>>(p);
+    else gn_any_fwd_kernel<__nv_bfloat16><<<(unsigned)(N * G), 256, 0, s>>>(p);
+    return launch_status("gn_any_fwd_kernel");
+  }
+  const void* ptr[] = {x, y};
+  const int64_t stride[] = {N > 1 ? x_sn : 0, S > 1 ? x_ss : 0, N > 1 ? y_sn : 0, S > 1 ? y_ss : 0};
+  int ve = gn_width(es, p.Cg);
+  const GnRowPlan row = gn_row_plan(N, S, G, p.Cg, ve);
+  if (row.ok) {
+    p.whole = gn_whole(es, ve, ptr, stride, 2);
+    if (dtype == HDC_F32) gn_rows<float, false>(p, row, ve, s);
+    else gn_rows<__nv_bfloat16, false>(p, row, ve, s);
+    return launch_status("gn_row_kernel");
+  }
+  const GnPlan plan = gn_plan(N, S, C, G);
+  p.slices = (int)plan.slices; p.rows = (int)plan.rows; p.cb = (int)plan.cb;
+  ve = gn_width(es, plan.cb | C);
+  p.whole = gn_whole(es, ve, ptr, stride, 2);
+  gn_pass(kStats, dtype, p, plan, ve, s);
+  if (int e = launch_status("gn_stats_kernel")) return e;
+  gn_pass(kApply, dtype, p, plan, ve, s);
+  return launch_status("gn_apply_kernel");
 }
 
 extern "C" size_t hdc_group_norm_bwd_workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G) {
-  return N > 0 && S > 0 && C > 0 ? (size_t)N * 2 * C * 4 : 0;
+  if (N < 1 || S < 1 || C < 1 || G < 1 || C % G != 0) return 0;
+  if (C / G > kGnMostCg) return (size_t)N * 2 * C * 4;
+  int64_t parts = S == 1 ? gn_row_parts(N, G, C / G) : 0;
+  if (!gn_row_plan(N, S, G, C / G, 1).ok) {
+    const int64_t two = N * gn_plan(N, S, C, G).slices;
+    if (two > parts) parts = two;
+  }
+  return (size_t)parts * 2 * C * 4;
 }
 
 extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_t dy_sn, int64_t dy_ss, const void* x,
@@ -186,7 +879,7 @@ extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_
   if (!empty && (!dy || !x || !mean || !rstd || !dx)) return fail(HDC_E_NULL, "group_norm_bwd: null pointer");
   if (gn_off(dy, dtype) || gn_off(x, dtype) || gn_off(dx, dtype) || gn_off(weight, p_dtype) || gn_off(bias, p_dtype) ||
       gn_off(dweight, p_dtype) || gn_off(dbias, p_dtype) || gn_off(mean, HDC_F32) || gn_off(rstd, HDC_F32) ||
-      gn_off(workspace, HDC_F32))
+      !aligned16(workspace))
     return fail(HDC_E_ALIGN, "group_norm_bwd: a pointer is not aligned to its type");
   const size_t need = hdc_group_norm_bwd_workspace_bytes(N, S, C, G);
   if (need > 0 && (!workspace || workspace_bytes < need))
@@ -197,13 +890,39 @@ extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_
   p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd); p.part = static_cast<float*>(workspace);
   p.N = (int)N; p.S = (int)S; p.C = (int)C; p.G = (int)G; p.Cg = (int)(C / G); p.silu = act == HDC_ACT_SILU;
   auto s = reinterpret_cast<cudaStream_t>(stream);
-  if (!empty) {
-    if (dtype == HDC_F32) gn_bwd_kernel<float><<<(unsigned)(N * G), 256, 0, s>>>(p);
-    else gn_bwd_kernel<__nv_bfloat16><<<(unsigned)(N * G), 256, 0, s>>>(p);
-    if (int e = launch_status("gn_bwd_kernel")) return e;
+  const int es = dtype == HDC_F32 ? 4 : 2;
+  int64_t parts = 0;
+  if (!empty && p.Cg > kGnMostCg) {
+    if (dtype == HDC_F32) gn_any_bwd_kernel<float><<<(unsigned)(N * G), 256, 0, s>>>(p);
+    else gn_any_bwd_kernel<__nv_bfloat16><<<(unsigned)(N * G), 256, 0, s>>>(p);
+    if (int e = launch_status("gn_any_bwd_kernel")) return e;
+    parts = N;
+  } else if (!empty) {
+    const void* ptr[] = {x, dy, dx};
+    const int64_t stride[] = {N > 1 ? x_sn : 0,  S > 1 ? x_ss : 0,  N > 1 ? dy_sn : 0,
+                              S > 1 ? dy_ss : 0, N > 1 ? dx_sn : 0, S > 1 ? dx_ss : 0};
+    int ve = gn_width(es, p.Cg);
+    const GnRowPlan row = gn_row_plan(N, S, G, p.Cg, ve);
+    if (row.ok) {
+      p.whole = gn_whole(es, ve, ptr, stride, 3);
+      if (dtype == HDC_F32) gn_rows<float, true>(p, row, ve, s);
+      else gn_rows<__nv_bfloat16, true>(p, row, ve, s);
+      if (int e = launch_status("gn_row_kernel")) return e;
+      parts = row.ctas;
+    } else {
+      const GnPlan plan = gn_plan(N, S, C, G);
+      p.slices = (int)plan.slices; p.rows = (int)plan.rows; p.cb = (int)plan.cb;
+      ve = gn_width(es, plan.cb | C);
+      p.whole = gn_whole(es, ve, ptr, stride, 3);
+      gn_pass(kSums, dtype, p, plan, ve, s);
+      if (int e = launch_status("gn_sums_kernel")) return e;
+      gn_pass(kDx, dtype, p, plan, ve, s);
+      if (int e = launch_status("gn_dx_kernel")) return e;
+      parts = N * plan.slices;
+    }
   }
   if (!dweight && !dbias) return HDC_OK;
-  gn_param_grad_kernel<<<dim3((unsigned)((C + 127) / 128), 2), 128, 0, s>>>(p.part, empty ? 0 : (int)N, (int)C,
-                                                                           dweight, dbias, p.p_bf16);
+  gn_param_grad_kernel<<<dim3((unsigned)((C + 31) / 32), 2), 256, 0, s>>>(p.part, parts, (int)C, dweight, dbias,
+                                                                          p.p_bf16);
   return launch_status("gn_param_grad_kernel");
 }

@@ -46,6 +46,9 @@ SHAPES = [
     # few and many positions
     (2, 2, 32, 4), (3, 5, 64, 8), (4, 16, 30, 3), (2, 49, 320, 32), (1, 64, 1, 1), (3, 77, 10, 2), (2, 225, 96, 8),
     (1, 1000, 640, 32), (2, 4096, 40, 4), (1, 5000, 33, 11), (1, 20000, 64, 2), (6, 300, 256, 1), (40, 130, 128, 32),
+    # groups too wide for one CTA's channels, and at the limits of the lanes of one position
+    (2, 3, 10000, 2), (3, 1, 5000, 1), (3, 1, 256, 1), (3, 1, 257, 1), (3, 1, 1024, 1), (5, 1, 1032, 1), (4, 1, 255, 1),
+    (3, 10, 1500, 1), (2, 33, 2049, 3),
 ]
 
 
