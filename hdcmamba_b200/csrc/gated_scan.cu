@@ -33,6 +33,7 @@
 #include <type_traits>
 
 #include "tc.cuh"
+#include "vec.cuh"
 
 namespace hdc {
 
@@ -75,67 +76,8 @@ __device__ __forceinline__ float softplus_acc(float x) { return x > 20.0f ? x : 
 // ---------------------------------------------------------------- a lane's channels
 // V neighbouring channels of a lane: W words of 4 bytes (fp32: V = W, bf16: V = 2 W), computed
 // as pairs where V is even (fma.rn.f32x2 and friends: two fp32 operations per issued instruction).
-template <int V> struct Fv { float v[V]; };
 template <typename T, int W> constexpr int kV = W * 4 / (int)sizeof(T);
 
-__device__ __forceinline__ uint64_t pair_bits(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void bits_pair(uint64_t r, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
-}
-template <int V> __device__ __forceinline__ Fv<V> fma(const Fv<V>& a, const Fv<V>& b, const Fv<V>& c) {
-  Fv<V> o;
-  if constexpr (V == 1) {
-    o.v[0] = fmaf(a.v[0], b.v[0], c.v[0]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i += 2) {
-      uint64_t r;
-      asm("fma.rn.f32x2 %0, %1, %2, %3;"
-          : "=l"(r)
-          : "l"(pair_bits(a.v[i], a.v[i + 1])), "l"(pair_bits(b.v[i], b.v[i + 1])), "l"(pair_bits(c.v[i], c.v[i + 1])));
-      bits_pair(r, o.v[i], o.v[i + 1]);
-    }
-  }
-  return o;
-}
-template <int V> __device__ __forceinline__ Fv<V> operator*(const Fv<V>& a, const Fv<V>& b) {
-  Fv<V> o;
-  if constexpr (V == 1) {
-    o.v[0] = a.v[0] * b.v[0];
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i += 2) {
-      uint64_t r;
-      asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a.v[i], a.v[i + 1])), "l"(pair_bits(b.v[i], b.v[i + 1])));
-      bits_pair(r, o.v[i], o.v[i + 1]);
-    }
-  }
-  return o;
-}
-template <int V> __device__ __forceinline__ Fv<V> operator+(const Fv<V>& a, const Fv<V>& b) {
-  Fv<V> o;
-  if constexpr (V == 1) {
-    o.v[0] = a.v[0] + b.v[0];
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i += 2) {
-      uint64_t r;
-      asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(a.v[i], a.v[i + 1])), "l"(pair_bits(b.v[i], b.v[i + 1])));
-      bits_pair(r, o.v[i], o.v[i + 1]);
-    }
-  }
-  return o;
-}
-template <int V> __device__ __forceinline__ Fv<V> all(float x) {
-  Fv<V> r;
-#pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = x;
-  return r;
-}
 // a lane's channels from and to its words
 template <typename T, int W> __device__ __forceinline__ Fv<kV<T, W>> ld_words(const char* p) {
   uint32_t w[W];
@@ -184,12 +126,6 @@ __device__ __forceinline__ void st_row(T* row, int c, int nc, int vec, const Fv<
 }
 // a word of dt = -inf
 template <typename T> constexpr uint32_t kNoStep = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
-
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 
 // d = softplus(x).
 //   fp32: the library's exp and log1p.
@@ -244,8 +180,7 @@ template <typename T, int V> __device__ __forceinline__ Fv<V> sigmoid(const Fv<V
     if constexpr (sizeof(T) == 4) {
       s.v[i] = 1.f / (1.f + expf(-x.v[i]));
     } else {
-      float r;
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e.v[i]));
+      const float r = rcp(1.f + e.v[i]);
       s.v[i] = x.v[i] < 0.f ? e.v[i] * r : r;
     }
   }

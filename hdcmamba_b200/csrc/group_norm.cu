@@ -21,7 +21,7 @@
 // squares, and blocks, threads and slices are joined by
 //   n = n1 + n2, mean = mean1 + (mean2 - mean1) n2/n, M2 = M2_1 + M2_2 + (mean2 - mean1)^2 n1 n2/n.
 // Channels per load: as many as 16 bytes, the rows' alignment and (S = 1) the group allow.
-#include "common.cuh"
+#include "vec.cuh"
 
 namespace hdc {
 
@@ -34,6 +34,8 @@ struct GnParams {
   void* dx; int64_t gsn, gss;
   float* part;     // gradient: sums of dz xh and of dz per channel, [part][2][C]
   float2* stats;   // two passes: (mean, M2) of each slice, [N][slices][G]
+  float* sums;     // two passes, gradient: part over the slices, [N][2][C]
+  float* gmean;    // and the groups' means of e xh and of e, [N][2][G]
   void* dw; void* db;
   int N, S, C, G, Cg;
   float eps; int silu;
@@ -77,30 +79,32 @@ template <typename T, int VE> __device__ __forceinline__ Raw<T, VE> ld_raw(const
   }
   return r;
 }
-template <typename T, int VE> __device__ __forceinline__ void unpack(const Raw<T, VE>& r, float (&f)[VE]) {
+template <typename T, int VE> __device__ __forceinline__ Fv<VE> unpack(const Raw<T, VE>& r) {
+  Fv<VE> f;
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
-    if constexpr (sizeof(T) == 4) f[i] = __uint_as_float(r.w[i]);
-    else f[i] = __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
+    if constexpr (sizeof(T) == 4) f.v[i] = __uint_as_float(r.w[i]);
+    else f.v[i] = __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
   }
+  return f;
 }
-template <typename T, int VE> __device__ __forceinline__ void st_vec(T* p, const float (&f)[VE], int whole) {
+template <typename T, int VE> __device__ __forceinline__ void st_vec(T* p, const Fv<VE>& f, int whole) {
   constexpr int bytes = VE * (int)sizeof(T);
   if (VE > 1 && !whole) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) p[i] = from_f<T>(f[i]);
+    for (int i = 0; i < VE; ++i) p[i] = from_f<T>(f.v[i]);
     return;
   }
   if constexpr (bytes == 2) {
-    *p = from_f<T>(f[0]);
+    *p = from_f<T>(f.v[0]);
   } else {
     uint32_t w[bytes / 4];
 #pragma unroll
     for (int i = 0; i < bytes / 4; ++i) {
       if constexpr (sizeof(T) == 4) {
-        w[i] = __float_as_uint(f[i]);
+        w[i] = __float_as_uint(f.v[i]);
       } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f.v[2 * i], f.v[2 * i + 1]);
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
       }
     }
@@ -111,31 +115,55 @@ template <typename T, int VE> __device__ __forceinline__ void st_vec(T* p, const
 }
 
 // sigmoid: hardware 2^x and reciprocal for bf16 tensors (a few 2^-23 off), the library's for fp32
-template <typename T> __device__ __forceinline__ float gn_sigmoid(float z) {
-  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-z));
-  else return __fdividef(1.f, 1.f + __expf(-z));
+template <typename T, int V> __device__ __forceinline__ Fv<V> gn_sigmoid(const Fv<V>& z) {
+  Fv<V> q;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) q.v[i] = 1.f / (1.f + expf(-z.v[i]));
+  } else {
+    q = z * all<V>(-1.4426950408889634f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) q.v[i] = ex2(q.v[i]);
+    q = q + all<V>(1.f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) q.v[i] = rcp(q.v[i]);
+  }
+  return q;
 }
-template <typename T> __device__ __forceinline__ float gn_act(float z, int silu) {
+template <typename T, int V> __device__ __forceinline__ Fv<V> gn_act(const Fv<V>& z, int silu) {
   return silu ? z * gn_sigmoid<T>(z) : z;
 }
 // dz from dy
-template <typename T> __device__ __forceinline__ float gn_dact(float dy, float z, int silu) {
+template <typename T, int V> __device__ __forceinline__ Fv<V> gn_dact(const Fv<V>& dy, const Fv<V>& z, int silu) {
   if (!silu) return dy;
-  const float q = gn_sigmoid<T>(z);
-  return dy * (q * fmaf(z, 1.f - q, 1.f));
+  const Fv<V> q = gn_sigmoid<T>(z);
+  return dy * (q * fma(z, fma(q, all<V>(-1.f), all<V>(1.f)), all<V>(1.f)));
+}
+template <int V> __device__ __forceinline__ float sum_of(const Fv<V>& f) {
+  float s = f.v[0];
+#pragma unroll
+  for (int i = 1; i < V; ++i) s += f.v[i];
+  return s;
+}
+template <int V> __device__ __forceinline__ Fv<V> gn_params(const void* p, int bf16, int c, float none) {
+  Fv<V> f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) f.v[i] = gn_param(p, bf16, c + i, none);
+  return f;
 }
 __device__ __forceinline__ float gn_rstd(float M2, float n, float eps) { return 1.f / sqrtf(M2 / n + eps); }
 
 // ---------------------------------------------------------------- one position per sample
 // The lanes of a group: LG of them, CPL loads of VE channels each: channel (k LG + l) VE + i of
 // the group.  Threads: (sample of the CTA, group, lane), groups from blockIdx.y * gpc.
+// FULL: the lanes' loads are exactly the group.
 template <int LG> __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
   for (int o = LG / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-template <typename T, int VE, int CPL, int U, bool BWD, int LG>
+template <typename T, int VE, int CPL, int U, bool BWD, int LG, bool FULL>
 __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnParams p, int gpc, int spc) {
   const int l = threadIdx.x % LG, gi = threadIdx.x / LG % gpc, sr = threadIdx.x / LG / gpc;
   const int g = blockIdx.y * gpc + gi;
@@ -144,22 +172,18 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
   constexpr int M = VE * CPL;
   int ch[CPL];
   bool in[CPL];
-  float w[M], b[M];
+  Fv<VE> w[CPL], b[CPL], dw[BWD ? CPL : 1], db[BWD ? CPL : 1];
 #pragma unroll
   for (int k = 0; k < CPL; ++k) {
     const int c = (k * LG + l) * VE;
-    in[k] = live && c < p.Cg;
-    ch[k] = c0 + (c < p.Cg ? c : 0);
-#pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      w[k * VE + i] = gn_param(p.w, p.p_bf16, ch[k] + i, 1.f);
-      b[k * VE + i] = gn_param(p.b, p.p_bf16, ch[k] + i, 0.f);
-    }
+    in[k] = FULL || c < p.Cg;
+    ch[k] = c0 + (in[k] ? c : 0);
+    w[k] = gn_params<VE>(p.w, p.p_bf16, ch[k], 1.f);
+    b[k] = gn_params<VE>(p.b, p.p_bf16, ch[k], 0.f);
+    if constexpr (BWD) dw[k] = db[k] = all<VE>(0.f);
   }
   const float inv = 1.f / (float)p.Cg;
-  float dw[BWD ? M : 1], db[BWD ? M : 1];
-#pragma unroll
-  for (int i = 0; i < (BWD ? M : 1); ++i) dw[i] = db[i] = 0.f;
+  if constexpr (BWD) let_next_start();
 
   const int64_t step = (int64_t)gridDim.x * spc;
   for (int64_t n0 = (int64_t)blockIdx.x * spc; n0 < p.N; n0 += step * U) {
@@ -168,8 +192,7 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t n = n0 + u * step + sr;
-      const bool ok = live && n < p.N;
-      const int64_t nn = ok ? n : 0;
+      const int64_t nn = live && n < p.N ? n : 0;
 #pragma unroll
       for (int k = 0; k < CPL; ++k) {
         xr[u][k] = ld_raw<T, VE>(static_cast<const T*>(p.x) + nn * p.xsn + ch[k], p.whole);
@@ -184,63 +207,46 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
     for (int u = 0; u < U; ++u) {
       const int64_t n = n0 + u * step + sr;
       const bool ok = live && n < p.N;
-      float x[M];
-#pragma unroll
-      for (int k = 0; k < CPL; ++k) {
-        float f[VE];
-        unpack<T, VE>(xr[u][k], f);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) x[k * VE + i] = f[i];
-      }
+      Fv<VE> x[CPL];
       if constexpr (!BWD) {
         float s = 0.f;
 #pragma unroll
-        for (int k = 0; k < CPL; ++k)
-#pragma unroll
-          for (int i = 0; i < VE; ++i) s += in[k] ? x[k * VE + i] : 0.f;
+        for (int k = 0; k < CPL; ++k) {
+          x[k] = unpack<T, VE>(xr[u][k]);
+          s += in[k] ? sum_of(x[k]) : 0.f;
+        }
         const float mean = group_sum<LG>(s) / (float)p.Cg;
         s = 0.f;
 #pragma unroll
-        for (int k = 0; k < CPL; ++k)
-#pragma unroll
-          for (int i = 0; i < VE; ++i) {
-            x[k * VE + i] -= mean;
-            s = in[k] ? fmaf(x[k * VE + i], x[k * VE + i], s) : s;
-          }
+        for (int k = 0; k < CPL; ++k) {
+          x[k] = x[k] + all<VE>(-mean);
+          s += in[k] ? sum_of(x[k] * x[k]) : 0.f;
+        }
         const float rstd = gn_rstd(group_sum<LG>(s), (float)p.Cg, p.eps);
         if (ok) {
 #pragma unroll
           for (int k = 0; k < CPL; ++k)
-            if (in[k]) {
-              float f[VE];
-#pragma unroll
-              for (int i = 0; i < VE; ++i)
-                f[i] = gn_act<T>(fmaf(x[k * VE + i] * rstd, w[k * VE + i], b[k * VE + i]), p.silu);
-              st_vec<T, VE>(static_cast<T*>(p.y) + n * p.ysn + ch[k], f, p.whole);
-            }
+            if (in[k])
+              st_vec<T, VE>(static_cast<T*>(p.y) + n * p.ysn + ch[k],
+                            gn_act<T>(fma(x[k] * all<VE>(rstd), w[k], b[k]), p.silu), p.whole);
           if (l == 0 && p.mean) {
             p.mean[n * p.G + g] = mean;
             p.rstd[n * p.G + g] = rstd;
           }
         }
       } else {
-        float e[M], se = 0.f, sx = 0.f;
+        Fv<VE> e[CPL];
+        float se = 0.f, sx = 0.f;
 #pragma unroll
         for (int k = 0; k < CPL; ++k) {
-          float f[VE];
-          unpack<T, VE>(dr[u][k], f);
-#pragma unroll
-          for (int i = 0; i < VE; ++i) {
-            const int m = k * VE + i;
-            x[m] = (x[m] - mu[u]) * rs[u];
-            const float dz = gn_dact<T>(f[i], fmaf(x[m], w[m], b[m]), p.silu);
-            if (ok && in[k]) {
-              dw[m] = fmaf(dz, x[m], dw[m]);
-              db[m] += dz;
-              e[m] = dz * w[m];
-              se += e[m];
-              sx = fmaf(e[m], x[m], sx);
-            }
+          x[k] = (unpack<T, VE>(xr[u][k]) + all<VE>(-mu[u])) * all<VE>(rs[u]);
+          const Fv<VE> dz = gn_dact<T>(unpack<T, VE>(dr[u][k]), fma(x[k], w[k], b[k]), p.silu);
+          e[k] = dz * w[k];
+          if (ok && in[k]) {
+            dw[k] = fma(dz, x[k], dw[k]);
+            db[k] = db[k] + dz;
+            se += sum_of(e[k]);
+            sx += sum_of(e[k] * x[k]);
           }
         }
         se = group_sum<LG>(se) * inv;
@@ -248,25 +254,22 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
         if (ok) {
 #pragma unroll
           for (int k = 0; k < CPL; ++k)
-            if (in[k]) {
-              float f[VE];
-#pragma unroll
-              for (int i = 0; i < VE; ++i) f[i] = rs[u] * (e[k * VE + i] - se - x[k * VE + i] * sx);
-              st_vec<T, VE>(static_cast<T*>(p.dx) + n * p.gsn + ch[k], f, p.whole);
-            }
+            if (in[k])
+              st_vec<T, VE>(static_cast<T*>(p.dx) + n * p.gsn + ch[k],
+                            fma(x[k], all<VE>(-sx), e[k] + all<VE>(-se)) * all<VE>(rs[u]), p.whole);
         }
       }
     }
   }
   if constexpr (BWD) {  // the CTA's sums over its samples, in their order
-    extern __shared__ float sh[];  // [spc][gpc * LG][M]
+    extern __shared__ float sh[];  // [spc][M][gpc * LG]
     const int per = gpc * LG, q = threadIdx.x % per;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
       if (sr < spc) {
 #pragma unroll
-        for (int i = 0; i < M; ++i) sh[((size_t)sr * M + i) * per + q] = which ? db[i] : dw[i];
+        for (int i = 0; i < M; ++i) sh[((size_t)sr * M + i) * per + q] = (which ? db[i / VE] : dw[i / VE]).v[i % VE];
       }
       __syncthreads();
       if (sr == 0 && live) {
@@ -285,143 +288,174 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
 }
 
 // ---------------------------------------------------------------- several positions per sample
-// CTA (slice, sample, channel block): thread = (row lane, chunk of VE channels).
-struct GnStat { float n, mean, M2; };
-__device__ __forceinline__ GnStat join(const GnStat& a, const GnStat& b) {
-  const float n = a.n + b.n;
-  if (n == 0.f) return a;
-  const float d = b.mean - a.mean, f = b.n / n;
-  return {n, fmaf(d, f, a.mean), a.M2 + b.M2 + d * d * (a.n * f)};
-}
+// CTA (sample and slice, channel block): thread = (row lane, chunk of VE channels).
 constexpr int kGnThreads = 256;
 // row lanes of a CTA: threads per chunk of channels (one when a thread has several chunks)
 __host__ __device__ inline int gn_lanes(int nchunk) { return nchunk < kGnThreads ? kGnThreads / nchunk : 1; }
 
+// A CTA's place: sample n, slice of its positions from r0 (rows of them), channels c_lo .. c_lo + cw
+struct GnPlace {
+  int n, slice, r0, rows, c_lo, cw;
+  __device__ explicit GnPlace(const GnParams& p) {
+    n = blockIdx.x / p.slices;
+    slice = blockIdx.x - n * p.slices;
+    r0 = slice * p.rows;
+    rows = min(p.rows, p.S - r0);
+    c_lo = blockIdx.y * p.cb;
+    cw = min(p.cb, p.C - c_lo);
+  }
+};
+
+// (mean, M2) of each slice and group
 template <typename T, int VE>
 __global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(const __grid_constant__ GnParams p) {
-  extern __shared__ float sh[];  // [2][row lanes][cb]: mean, M2
-  const int c_lo = blockIdx.y * p.cb, cw = min(p.cb, p.C - c_lo), nchunk = cw / VE;
-  const int RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
-  const int n = blockIdx.x / p.slices, slice = blockIdx.x - n * p.slices, r0 = slice * p.rows, rows = min(p.rows, p.S - r0);
-  constexpr int U = 8;
+  extern __shared__ float sh[];  // [2][row lanes][cw]: mean, M2
+  const GnPlace at(p);
+  const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
+  constexpr int U = 4;
+  let_next_start();
   if (rl < RL)
-  for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
-    const T* x = static_cast<const T*>(p.x) + n * p.xsn + (int64_t)r0 * p.xss + c_lo + k * VE;
-    float mean[VE], M2[VE], cnt = 0.f;
-#pragma unroll
-    for (int i = 0; i < VE; ++i) mean[i] = M2[i] = 0.f;
-    int r = rl;
-    for (; r + (U - 1) * RL < rows; r += U * RL) {
+    for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
+      const T* x = static_cast<const T*>(p.x) + at.n * p.xsn + (int64_t)(at.r0 + rl) * p.xss + at.c_lo + k * VE;
+      const int64_t hop = RL * p.xss;
+      Fv<VE> mean = all<VE>(0.f), M2 = all<VE>(0.f);
+      float blocks = 0.f;  // of U rows
+      int r = rl;
       Raw<T, VE> raw[U];
+      auto load = [&]() {
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
-      float v[U][VE];
+        for (int u = 0; u < U; ++u) raw[u] = ld_raw<T, VE>(x + u * hop, p.whole);
+        x += U * hop;
+      };
+      bool more = r + (U - 1) * RL < at.rows;
+      if (more) load();
+      while (more) {
+        Fv<VE> v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) unpack<T, VE>(raw[u], v[u]);
-      const float total = cnt + U, f = U / total, g = cnt * f;
+        for (int u = 0; u < U; ++u) v[u] = unpack<T, VE>(raw[u]);
+        r += U * RL;
+        more = r + (U - 1) * RL < at.rows;
+        if (more) load();
+        Fv<VE> m = (v[0] + v[1]) + (v[2] + v[3]);
+        m = m * all<VE>(1.f / U);
+        const Fv<VE> neg = m * all<VE>(-1.f);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const Fv<VE> d = v[u] + neg;
+          M2 = fma(d, d, M2);
+        }
+        blocks += 1.f;
+        const float f = 1.f / blocks;
+        const Fv<VE> d = fma(mean, all<VE>(-1.f), m);
+        mean = fma(d, all<VE>(f), mean);
+        M2 = fma(d * d, all<VE>(U * (blocks - 1.f) * f), M2);
+      }
+      float cnt = blocks * U;
+      for (; r < at.rows; r += RL) {
+        const Fv<VE> d = fma(mean, all<VE>(-1.f), unpack<T, VE>(ld_raw<T, VE>(x, p.whole)));
+        x += hop;
+        const float f = 1.f / (cnt + 1.f);
+        mean = fma(d, all<VE>(f), mean);
+        M2 = fma(d * d, all<VE>(cnt * f), M2);
+        cnt += 1.f;
+      }
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        float s = 0.f;
-#pragma unroll
-        for (int u = 0; u < U; ++u) s += v[u][i];
-        const float m = s * (1.f / U), d = m - mean[i];
-        s = 0.f;
-#pragma unroll
-        for (int u = 0; u < U; ++u) s = fmaf(v[u][i] - m, v[u][i] - m, s);
-        M2[i] += fmaf(d * d, g, s);
-        mean[i] = fmaf(d, f, mean[i]);
+        sh[rl * at.cw + k * VE + i] = mean.v[i];
+        sh[(RL + rl) * at.cw + k * VE + i] = M2.v[i];
       }
-      cnt = total;
     }
-    for (; r < rows; r += RL) {
-      float v[VE];
-      unpack<T, VE>(ld_raw<T, VE>(x + (int64_t)r * p.xss, p.whole), v);
-      const float total = cnt + 1.f, f = 1.f / total;
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const float d = v[i] - mean[i];
-        mean[i] = fmaf(d, f, mean[i]);
-        M2[i] = fmaf(d * d, cnt * f, M2[i]);
-      }
-      cnt = total;
+  __syncthreads();
+  // channels over the row lanes (lane q has the rows q, q + RL, ...)
+  const float inv = 1.f / (float)at.rows;
+  for (int c = threadIdx.x; c < at.cw; c += kGnThreads) {
+    const int lanes = min(RL, at.rows), base = at.rows / RL, extra = at.rows - base * RL;
+    float m = 0.f;
+    for (int q = 0; q < lanes; ++q) m = fmaf((float)(base + (q < extra)), sh[q * at.cw + c], m);
+    m *= inv;
+    float M2 = 0.f;
+    for (int q = 0; q < lanes; ++q) {
+      const float d = sh[q * at.cw + c] - m;
+      M2 += fmaf((float)(base + (q < extra)) * d, d, sh[(RL + q) * at.cw + c]);
     }
-#pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      sh[rl * cw + k * VE + i] = mean[i];
-      sh[(RL + rl) * cw + k * VE + i] = M2[i];
-    }
+    sh[c] = m;  // only this thread reads and writes this channel here
+    sh[RL * at.cw + c] = M2;
   }
   __syncthreads();
-  // channels over the row lanes, then groups over their channels
-  auto count = [&](int q) { return rows > q ? (float)((rows - q - 1) / RL + 1) : 0.f; };
-  for (int c = threadIdx.x; c < cw; c += kGnThreads) {
-    GnStat a = {count(0), sh[c], sh[RL * cw + c]};
-    for (int q = 1; q < RL; ++q) a = join(a, {count(q), sh[q * cw + c], sh[(RL + q) * cw + c]});
-    sh[c] = a.mean;  // only this thread reads and writes this channel here
-    sh[RL * cw + c] = a.M2;
-  }
-  __syncthreads();
+  // groups over their channels
   const int lane = threadIdx.x & 31;
-  for (int gi = threadIdx.x >> 5; gi < cw / p.Cg; gi += kGnThreads / 32) {
-    GnStat a = {0.f, 0.f, 0.f};
-    for (int c = lane; c < p.Cg; c += 32) a = join(a, {(float)rows, sh[gi * p.Cg + c], sh[RL * cw + gi * p.Cg + c]});
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      a = join(a, {__shfl_down_sync(0xffffffffu, a.n, o), __shfl_down_sync(0xffffffffu, a.mean, o),
-                   __shfl_down_sync(0xffffffffu, a.M2, o)});
-    if (lane == 0) p.stats[(int64_t)blockIdx.x * p.G + c_lo / p.Cg + gi] = make_float2(a.mean, a.M2);
+  for (int gi = threadIdx.x >> 5; gi < at.cw / p.Cg; gi += kGnThreads / 32) {
+    const float* m = sh + gi * p.Cg;
+    float mean = 0.f;
+    for (int c = lane; c < p.Cg; c += 32) mean += m[c];
+    mean = warp_sum(mean) / (float)p.Cg;
+    float M2 = 0.f;
+    for (int c = lane; c < p.Cg; c += 32) {
+      const float d = m[c] - mean;
+      M2 += fmaf((float)at.rows * d, d, m[RL * at.cw + c]);
+    }
+    M2 = warp_sum(M2);
+    if (lane == 0) p.stats[(int64_t)blockIdx.x * p.G + at.c_lo / p.Cg + gi] = make_float2(mean, M2);
+  }
+}
+
+// mean and rstd of each (n, g) from its slices: one warp each
+__global__ void __launch_bounds__(256) gn_join_kernel(const __grid_constant__ GnParams p) {
+  let_next_start();
+  wait_for_previous();
+  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (i >= (int64_t)p.N * p.G) return;
+  const int n = (int)(i / p.G), g = (int)(i - (int64_t)n * p.G);
+  const float2* st = p.stats + (int64_t)n * p.slices * p.G + g;
+  const float total = (float)p.S * (float)p.Cg;
+  float mean = 0.f;
+  for (int q = lane; q < p.slices; q += 32)
+    mean = fmaf((float)min(p.rows, p.S - q * p.rows) * (float)p.Cg, st[(int64_t)q * p.G].x, mean);
+  mean = warp_sum(mean) / total;
+  float M2 = 0.f;
+  for (int q = lane; q < p.slices; q += 32) {
+    const float2 v = st[(int64_t)q * p.G];
+    const float d = v.x - mean;
+    M2 += fmaf((float)min(p.rows, p.S - q * p.rows) * (float)p.Cg * d, d, v.y);
+  }
+  M2 = warp_sum(M2);
+  if (lane == 0) {
+    p.mean[i] = mean;
+    p.rstd[i] = gn_rstd(M2, total, p.eps);
   }
 }
 
 template <typename T, int VE>
 __global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(const __grid_constant__ GnParams p) {
-  extern __shared__ float sh[];  // [2][groups of the block]: mean, rstd
-  const int c_lo = blockIdx.y * p.cb, cw = min(p.cb, p.C - c_lo), nchunk = cw / VE, ng = cw / p.Cg;
-  const int n = blockIdx.x / p.slices, slice = blockIdx.x - n * p.slices, r0 = slice * p.rows, rows = min(p.rows, p.S - r0);
-  for (int gi = threadIdx.x; gi < ng; gi += kGnThreads) {
-    const float2* st = p.stats + (int64_t)n * p.slices * p.G + c_lo / p.Cg + gi;
-    GnStat a = {0.f, 0.f, 0.f};
-    for (int q = 0; q < p.slices; ++q) {
-      const float2 v = st[(int64_t)q * p.G];
-      a = join(a, {(float)min(p.rows, p.S - q * p.rows) * (float)p.Cg, v.x, v.y});
-    }
-    const float rstd = gn_rstd(a.M2, a.n, p.eps);
-    sh[gi] = a.mean;
-    sh[ng + gi] = rstd;
-    if (p.mean && slice == 0) {
-      p.mean[(int64_t)n * p.G + c_lo / p.Cg + gi] = a.mean;
-      p.rstd[(int64_t)n * p.G + c_lo / p.Cg + gi] = rstd;
-    }
-  }
-  __syncthreads();
-  const int RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
+  const GnPlace at(p);
+  const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
   if (rl >= RL) return;
   for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
-    float mean[VE], sc[VE], b[VE];
+    const int c0 = at.c_lo + k * VE;
+    const Fv<VE> w = gn_params<VE>(p.w, p.p_bf16, c0, 1.f), b = gn_params<VE>(p.b, p.p_bf16, c0, 0.f);
+    wait_for_previous();
+    Fv<VE> neg, sc;
 #pragma unroll
     for (int i = 0; i < VE; ++i) {
-      const int c = k * VE + i;
-      mean[i] = sh[c / p.Cg];
-      sc[i] = sh[ng + c / p.Cg] * gn_param(p.w, p.p_bf16, c_lo + c, 1.f);
-      b[i] = gn_param(p.b, p.p_bf16, c_lo + c, 0.f);
+      const int64_t j = (int64_t)at.n * p.G + (c0 + i) / p.Cg;
+      neg.v[i] = -p.mean[j];
+      sc.v[i] = p.rstd[j];
     }
-    const T* x = static_cast<const T*>(p.x) + n * p.xsn + (int64_t)r0 * p.xss + c_lo + k * VE;
-    T* y = static_cast<T*>(p.y) + n * p.ysn + (int64_t)r0 * p.yss + c_lo + k * VE;
+    sc = sc * w;
+    const T* x = static_cast<const T*>(p.x) + at.n * p.xsn + (int64_t)at.r0 * p.xss + c0;
+    T* y = static_cast<T*>(p.y) + at.n * p.ysn + (int64_t)at.r0 * p.yss + c0;
     constexpr int U = 4;
-    for (int r = rl; r < rows; r += U * RL) {
+    for (int r = rl; r < at.rows; r += U * RL) {
       Raw<T, VE> raw[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (r + u * RL < rows) raw[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
+        if (r + u * RL < at.rows) raw[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (r + u * RL < rows) {
-          float v[VE];
-          unpack<T, VE>(raw[u], v);
-#pragma unroll
-          for (int i = 0; i < VE; ++i) v[i] = gn_act<T>(fmaf(v[i] - mean[i], sc[i], b[i]), p.silu);
-          st_vec<T, VE>(y + (int64_t)(r + u * RL) * p.yss, v, p.whole);
-        }
+        if (r + u * RL < at.rows)
+          st_vec<T, VE>(y + (int64_t)(r + u * RL) * p.yss, gn_act<T>(fma(unpack<T, VE>(raw[u]) + neg, sc, b), p.silu),
+                        p.whole);
     }
   }
 }
@@ -429,126 +463,130 @@ __global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(const __grid_const
 // The gradient's sums per channel of each slice: part[n * slices + slice][2][C]
 template <typename T, int VE>
 __global__ void __launch_bounds__(kGnThreads) gn_sums_kernel(const __grid_constant__ GnParams p) {
-  extern __shared__ float sh[];  // [2][row lanes][cb]
-  const int c_lo = blockIdx.y * p.cb, cw = min(p.cb, p.C - c_lo), nchunk = cw / VE;
-  const int RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
-  const int n = blockIdx.x / p.slices, slice = blockIdx.x - n * p.slices, r0 = slice * p.rows, rows = min(p.rows, p.S - r0);
+  extern __shared__ float sh[];  // [2][row lanes][cw]
+  const GnPlace at(p);
+  const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
+  let_next_start();
   if (rl < RL)
-  for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
-    float mean[VE], rstd[VE], w[VE], b[VE], a0[VE], a1[VE];
+    for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
+      const int c0 = at.c_lo + k * VE;
+      const Fv<VE> w = gn_params<VE>(p.w, p.p_bf16, c0, 1.f), b = gn_params<VE>(p.b, p.p_bf16, c0, 0.f);
+      Fv<VE> neg, rstd, a0 = all<VE>(0.f), a1 = all<VE>(0.f);
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      const int c = c_lo + k * VE + i;
-      mean[i] = p.mean[(int64_t)n * p.G + c / p.Cg];
-      rstd[i] = p.rstd[(int64_t)n * p.G + c / p.Cg];
-      w[i] = gn_param(p.w, p.p_bf16, c, 1.f);
-      b[i] = gn_param(p.b, p.p_bf16, c, 0.f);
-      a0[i] = a1[i] = 0.f;
-    }
-    const T* x = static_cast<const T*>(p.x) + n * p.xsn + (int64_t)r0 * p.xss + c_lo + k * VE;
-    const T* dy = static_cast<const T*>(p.dy) + n * p.dsn + (int64_t)r0 * p.dss + c_lo + k * VE;
-    constexpr int U = 4;
-    for (int r = rl; r < rows; r += U * RL) {
-      Raw<T, VE> xr[U], dr[U];
+      for (int i = 0; i < VE; ++i) {
+        const int64_t j = (int64_t)at.n * p.G + (c0 + i) / p.Cg;
+        neg.v[i] = -p.mean[j];
+        rstd.v[i] = p.rstd[j];
+      }
+      const T* x = static_cast<const T*>(p.x) + at.n * p.xsn + (int64_t)at.r0 * p.xss + c0;
+      const T* dy = static_cast<const T*>(p.dy) + at.n * p.dsn + (int64_t)at.r0 * p.dss + c0;
+      constexpr int U = 4;
+      for (int r = rl; r < at.rows; r += U * RL) {
+        Raw<T, VE> xr[U], dr[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (r + u * RL < rows) {
-          xr[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
-          dr[u] = ld_raw<T, VE>(dy + (int64_t)(r + u * RL) * p.dss, p.whole);
-        }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (r + u * RL < rows) {
-          float v[VE], d[VE];
-          unpack<T, VE>(xr[u], v);
-          unpack<T, VE>(dr[u], d);
-#pragma unroll
-          for (int i = 0; i < VE; ++i) {
-            const float xh = (v[i] - mean[i]) * rstd[i];
-            const float dz = gn_dact<T>(d[i], fmaf(xh, w[i], b[i]), p.silu);
-            a0[i] = fmaf(dz, xh, a0[i]);
-            a1[i] += dz;
+        for (int u = 0; u < U; ++u)
+          if (r + u * RL < at.rows) {
+            xr[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
+            dr[u] = ld_raw<T, VE>(dy + (int64_t)(r + u * RL) * p.dss, p.whole);
           }
-        }
-    }
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      sh[rl * cw + k * VE + i] = a0[i];
-      sh[(RL + rl) * cw + k * VE + i] = a1[i];
+        for (int u = 0; u < U; ++u)
+          if (r + u * RL < at.rows) {
+            const Fv<VE> xh = (unpack<T, VE>(xr[u]) + neg) * rstd;
+            const Fv<VE> dz = gn_dact<T>(unpack<T, VE>(dr[u]), fma(xh, w, b), p.silu);
+            a0 = fma(dz, xh, a0);
+            a1 = a1 + dz;
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        sh[rl * at.cw + k * VE + i] = a0.v[i];
+        sh[(RL + rl) * at.cw + k * VE + i] = a1.v[i];
+      }
     }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * at.cw; i += kGnThreads) {
+    const int which = i >= at.cw, c = which ? i - at.cw : i;
+    float v = 0.f;
+    for (int q = 0; q < RL; ++q) v += sh[(which * RL + q) * at.cw + c];
+    p.part[((int64_t)blockIdx.x * 2 + which) * p.C + at.c_lo + c] = v;
+  }
+}
+
+// CTA (sample, block of whole groups): the sample's sums over its slices, to sums[n][2][C], and
+// from them the means of e xh and of e of each group, to gmean[n][2][G].
+__global__ void __launch_bounds__(256) gn_mid_kernel(const __grid_constant__ GnParams p, int block) {
+  extern __shared__ float sh[];  // [strands][2 cw], then [2 cw]
+  let_next_start();
+  wait_for_previous();
+  const int n = blockIdx.x, c_lo = blockIdx.y * block, cw = min(block, p.C - c_lo), items = 2 * cw;
+  const int per = min(items, 256), strands = 256 / per, st = threadIdx.x / per;
+  if (st < strands)
+    for (int i = threadIdx.x - st * per; i < items; i += per) {
+      const int which = i >= cw, c = which ? i - cw : i;
+      const float* q = p.part + ((int64_t)n * p.slices * 2 + which) * p.C + c_lo + c;
+      float v = 0.f;
+#pragma unroll 8
+      for (int k = st; k < p.slices; k += strands) v += q[(int64_t)k * 2 * p.C];
+      sh[st * items + i] = v;
+    }
+  __syncthreads();
+  float* tot = sh + strands * items;
+  for (int i = threadIdx.x; i < items; i += 256) {
+    float v = sh[i];
+    for (int k = 1; k < strands; ++k) v += sh[k * items + i];
+    const int which = i >= cw, c = which ? i - cw : i;
+    p.sums[((int64_t)n * 2 + which) * p.C + c_lo + c] = v;
+    tot[i] = v * gn_param(p.w, p.p_bf16, c_lo + c, 1.f);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * cw; i += kGnThreads) {
-    const int which = i >= cw, c = which ? i - cw : i;
+  const int lane = threadIdx.x & 31, ng = cw / p.Cg;
+  const float inv = 1.f / ((float)p.S * (float)p.Cg);
+  for (int i = threadIdx.x >> 5; i < 2 * ng; i += 8) {
+    const int which = i >= ng, gi = which ? i - ng : i;
     float v = 0.f;
-    for (int q = 0; q < RL; ++q) v += sh[(which * RL + q) * cw + c];
-    p.part[((int64_t)blockIdx.x * 2 + which) * p.C + c_lo + c] = v;
+    for (int c = lane; c < p.Cg; c += 32) v += tot[which * cw + gi * p.Cg + c];
+    v = warp_sum(v);
+    if (lane == 0) p.gmean[((int64_t)n * 2 + which) * p.G + c_lo / p.Cg + gi] = v * inv;
   }
 }
 
 template <typename T, int VE>
 __global__ void __launch_bounds__(kGnThreads) gn_dx_kernel(const __grid_constant__ GnParams p) {
-  extern __shared__ float sh[];  // [2][cb] channel sums times w, then [2][groups]
-  const int c_lo = blockIdx.y * p.cb, cw = min(p.cb, p.C - c_lo), nchunk = cw / VE, ng = cw / p.Cg;
-  const int n = blockIdx.x / p.slices, slice = blockIdx.x - n * p.slices, r0 = slice * p.rows, rows = min(p.rows, p.S - r0);
-  float* gs = sh + 2 * cw;
-  for (int i = threadIdx.x; i < 2 * cw; i += kGnThreads) {
-    const int which = i >= cw, c = which ? i - cw : i;
-    const float* q = p.part + ((int64_t)n * p.slices * 2 + which) * p.C + c_lo + c;
-    float v = 0.f;
-    for (int k = 0; k < p.slices; ++k) v += q[(int64_t)k * 2 * p.C];
-    sh[i] = v * gn_param(p.w, p.p_bf16, c_lo + c, 1.f);
-  }
-  __syncthreads();
-  const int lane = threadIdx.x & 31;
-  const float inv = 1.f / ((float)p.S * (float)p.Cg);
-  for (int i = threadIdx.x >> 5; i < 2 * ng; i += kGnThreads / 32) {
-    const int which = i >= ng, gi = which ? i - ng : i;
-    float v = 0.f;
-    for (int c = lane; c < p.Cg; c += 32) v += sh[which * cw + gi * p.Cg + c];
-    v = warp_sum(v);
-    if (lane == 0) gs[i] = v * inv;
-  }
-  __syncthreads();
-  const int RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
+  const GnPlace at(p);
+  const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
   if (rl >= RL) return;
   for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
-    float mean[VE], rstd[VE], w[VE], b[VE], sx[VE], se[VE];
+    const int c0 = at.c_lo + k * VE;
+    const Fv<VE> w = gn_params<VE>(p.w, p.p_bf16, c0, 1.f), b = gn_params<VE>(p.b, p.p_bf16, c0, 0.f);
+    wait_for_previous();
+    Fv<VE> neg, rstd, sx, se;
 #pragma unroll
     for (int i = 0; i < VE; ++i) {
-      const int c = c_lo + k * VE + i, gi = (k * VE + i) / p.Cg;
-      mean[i] = p.mean[(int64_t)n * p.G + c / p.Cg];
-      rstd[i] = p.rstd[(int64_t)n * p.G + c / p.Cg];
-      w[i] = gn_param(p.w, p.p_bf16, c, 1.f);
-      b[i] = gn_param(p.b, p.p_bf16, c, 0.f);
-      sx[i] = gs[gi];
-      se[i] = gs[ng + gi];
+      const int g = (c0 + i) / p.Cg;
+      neg.v[i] = -p.mean[(int64_t)at.n * p.G + g];
+      rstd.v[i] = p.rstd[(int64_t)at.n * p.G + g];
+      sx.v[i] = -p.gmean[((int64_t)at.n * 2) * p.G + g];
+      se.v[i] = -p.gmean[((int64_t)at.n * 2 + 1) * p.G + g];
     }
-    const T* x = static_cast<const T*>(p.x) + n * p.xsn + (int64_t)r0 * p.xss + c_lo + k * VE;
-    const T* dy = static_cast<const T*>(p.dy) + n * p.dsn + (int64_t)r0 * p.dss + c_lo + k * VE;
-    T* dx = static_cast<T*>(p.dx) + n * p.gsn + (int64_t)r0 * p.gss + c_lo + k * VE;
+    const T* x = static_cast<const T*>(p.x) + at.n * p.xsn + (int64_t)at.r0 * p.xss + c0;
+    const T* dy = static_cast<const T*>(p.dy) + at.n * p.dsn + (int64_t)at.r0 * p.dss + c0;
+    T* dx = static_cast<T*>(p.dx) + at.n * p.gsn + (int64_t)at.r0 * p.gss + c0;
     constexpr int U = 4;
-    for (int r = rl; r < rows; r += U * RL) {
+    for (int r = rl; r < at.rows; r += U * RL) {
       Raw<T, VE> xr[U], dr[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (r + u * RL < rows) {
+        if (r + u * RL < at.rows) {
           xr[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
           dr[u] = ld_raw<T, VE>(dy + (int64_t)(r + u * RL) * p.dss, p.whole);
         }
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (r + u * RL < rows) {
-          float v[VE], d[VE];
-          unpack<T, VE>(xr[u], v);
-          unpack<T, VE>(dr[u], d);
-#pragma unroll
-          for (int i = 0; i < VE; ++i) {
-            const float xh = (v[i] - mean[i]) * rstd[i];
-            const float dz = gn_dact<T>(d[i], fmaf(xh, w[i], b[i]), p.silu);
-            v[i] = rstd[i] * (fmaf(dz, w[i], -se[i]) - xh * sx[i]);
-          }
-          st_vec<T, VE>(dx + (int64_t)(r + u * RL) * p.gss, v, p.whole);
+        if (r + u * RL < at.rows) {
+          const Fv<VE> xh = (unpack<T, VE>(xr[u]) + neg) * rstd;
+          const Fv<VE> dz = gn_dact<T>(unpack<T, VE>(dr[u]), fma(xh, w, b), p.silu);
+          st_vec<T, VE>(dx + (int64_t)(r + u * RL) * p.gss, fma(xh, sx, fma(dz, w, se)) * rstd, p.whole);
         }
     }
   }
@@ -649,6 +687,7 @@ __global__ void __launch_bounds__(256) gn_param_grad_kernel(const float* part, i
   __shared__ float s[8][32];
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
   void* out = blockIdx.y ? db : dw;
+  wait_for_previous();
   if (!out) return;
   float v = 0.f;
   if (c < C) {
@@ -734,7 +773,9 @@ static void gn_row_launch(const GnParams& p, const GnRowPlan& r, cudaStream_t s)
   constexpr int M = VE * CPL, U = M <= 8 ? (BWD ? 2 : 4) : M <= 16 ? 2 : 1;
   const int threads = (r.gpc * r.lg * r.spc + 31) / 32 * 32;
   const size_t smem = BWD ? (size_t)r.spc * r.gpc * r.lg * M * 4 : 0;
-  gn_row_kernel<T, VE, CPL, U, BWD, LG><<<dim3((unsigned)r.ctas, (unsigned)r.gy), threads, smem, s>>>(p, r.gpc, r.spc);
+  const dim3 grid((unsigned)r.ctas, (unsigned)r.gy);
+  if (LG * M == p.Cg) gn_row_kernel<T, VE, CPL, U, BWD, LG, true><<<grid, threads, smem, s>>>(p, r.gpc, r.spc);
+  else gn_row_kernel<T, VE, CPL, U, BWD, LG, false><<<grid, threads, smem, s>>>(p, r.gpc, r.spc);
 }
 template <typename T, int VE, int CPL, bool BWD>
 static void gn_row_lanes(const GnParams& p, const GnRowPlan& r, cudaStream_t s) {
@@ -768,12 +809,12 @@ template <typename T, bool BWD> static void gn_rows(const GnParams& p, const GnR
 enum GnPass { kStats, kApply, kSums, kDx };
 template <typename T, int VE> static void gn_pass(GnPass pass, const GnParams& p, const GnPlan& r, cudaStream_t s) {
   const dim3 grid((unsigned)(r.slices * p.N), (unsigned)r.gz);
-  const size_t lanes = gn_lanes((int)(r.cb / VE));
+  const size_t smem = (size_t)2 * gn_lanes((int)(r.cb / VE)) * r.cb * 4;
   switch (pass) {
-    case kStats: gn_stats_kernel<T, VE><<<grid, kGnThreads, 2 * lanes * r.cb * 4, s>>>(p); break;
-    case kApply: gn_apply_kernel<T, VE><<<grid, kGnThreads, 2 * (r.cb / p.Cg) * 4, s>>>(p); break;
-    case kSums: gn_sums_kernel<T, VE><<<grid, kGnThreads, 2 * lanes * r.cb * 4, s>>>(p); break;
-    case kDx: gn_dx_kernel<T, VE><<<grid, kGnThreads, 2 * (r.cb + r.cb / p.Cg) * 4, s>>>(p); break;
+    case kStats: gn_stats_kernel<T, VE><<<grid, kGnThreads, smem, s>>>(p); break;
+    case kApply: launch_dependent(gn_apply_kernel<T, VE>, grid, kGnThreads, 0, s, p); break;
+    case kSums: gn_sums_kernel<T, VE><<<grid, kGnThreads, smem, s>>>(p); break;
+    case kDx: launch_dependent(gn_dx_kernel<T, VE>, grid, kGnThreads, 0, s, p); break;
   }
 }
 template <typename T> static void gn_pass(GnPass pass, const GnParams& p, const GnPlan& r, int ve, cudaStream_t s) {
@@ -810,7 +851,8 @@ extern "C" size_t hdc_group_norm_workspace_bytes(int64_t N, int64_t S, int64_t C
   if (N < 1 || S < 1 || C < 1 || G < 1 || C % G != 0 || C / G > kGnMostCg) return 0;
   // one position takes no second pass with wider loads if it takes none with single channels
   if (gn_row_plan(N, S, G, C / G, 1).ok) return 0;
-  return (size_t)N * gn_plan(N, S, C, G).slices * G * 8;
+  // the slices' statistics, then the samples' mean and rstd when the caller does not want them
+  return (size_t)N * G * 8 * (gn_plan(N, S, C, G).slices + 1);
 }
 
 extern "C" int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t x_sn, int64_t x_ss, const void* weight,
@@ -852,8 +894,14 @@ extern "C" int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t
   p.slices = (int)plan.slices; p.rows = (int)plan.rows; p.cb = (int)plan.cb;
   ve = gn_width(es, plan.cb | C);
   p.whole = gn_whole(es, ve, ptr, stride, 2);
+  if (!p.mean) {
+    p.mean = reinterpret_cast<float*>(p.stats + N * plan.slices * G);
+    p.rstd = p.mean + N * G;
+  }
   gn_pass(kStats, dtype, p, plan, ve, s);
   if (int e = launch_status("gn_stats_kernel")) return e;
+  launch_dependent(gn_join_kernel, dim3((unsigned)((N * G + 7) / 8)), 256, 0, s, p);
+  if (int e = launch_status("gn_join_kernel")) return e;
   gn_pass(kApply, dtype, p, plan, ve, s);
   return launch_status("gn_apply_kernel");
 }
@@ -861,12 +909,16 @@ extern "C" int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t
 extern "C" size_t hdc_group_norm_bwd_workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G) {
   if (N < 1 || S < 1 || C < 1 || G < 1 || C % G != 0) return 0;
   if (C / G > kGnMostCg) return (size_t)N * 2 * C * 4;
-  int64_t parts = S == 1 ? gn_row_parts(N, G, C / G) : 0;
-  if (!gn_row_plan(N, S, G, C / G, 1).ok) {
-    const int64_t two = N * gn_plan(N, S, C, G).slices;
-    if (two > parts) parts = two;
-  }
-  return (size_t)parts * 2 * C * 4;
+  const size_t one = S == 1 ? (size_t)gn_row_parts(N, G, C / G) * 2 * C * 4 : 0;
+  if (gn_row_plan(N, S, G, C / G, 1).ok) return one;
+  // the slices' sums, the samples' sums, the groups' means
+  const size_t two = (size_t)N * 2 * 4 * ((gn_plan(N, S, C, G).slices + 1) * C + G);
+  return one > two ? one : two;
+}
+// the middle step's channels per CTA: whole groups, some 64 channels
+static int gn_mid_block(int C, int Cg) {
+  const int b = Cg >= 64 ? Cg : 64 / Cg * Cg;
+  return b < C ? b : C;
 }
 
 extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_t dy_sn, int64_t dy_ss, const void* x,
@@ -914,15 +966,22 @@ extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_
       p.slices = (int)plan.slices; p.rows = (int)plan.rows; p.cb = (int)plan.cb;
       ve = gn_width(es, plan.cb | C);
       p.whole = gn_whole(es, ve, ptr, stride, 3);
+      p.sums = p.part + N * plan.slices * 2 * C;
+      p.gmean = p.sums + N * 2 * C;
       gn_pass(kSums, dtype, p, plan, ve, s);
       if (int e = launch_status("gn_sums_kernel")) return e;
+      const int block = gn_mid_block(p.C, p.Cg), items = 2 * block, strands = items < 256 ? 256 / items : 1;
+      launch_dependent(gn_mid_kernel, dim3((unsigned)N, (unsigned)((C + block - 1) / block)), 256,
+                       (size_t)(strands + 1) * items * 4, s, p, block);
+      if (int e = launch_status("gn_mid_kernel")) return e;
       gn_pass(kDx, dtype, p, plan, ve, s);
       if (int e = launch_status("gn_dx_kernel")) return e;
-      parts = N * plan.slices;
+      p.part = p.sums;
+      parts = N;
     }
   }
   if (!dweight && !dbias) return HDC_OK;
-  gn_param_grad_kernel<<<dim3((unsigned)((C + 31) / 32), 2), 256, 0, s>>>(p.part, parts, (int)C, dweight, dbias,
-                                                                          p.p_bf16);
+  launch_dependent(gn_param_grad_kernel, dim3((unsigned)((C + 31) / 32), 2), 256, 0, s, p.part, parts, (int)C, dweight,
+                   dbias, p.p_bf16);
   return launch_status("gn_param_grad_kernel");
 }
