@@ -140,10 +140,19 @@ template <typename T, int V> __device__ __forceinline__ Fv<V> gn_dact(const Fv<V
   return dy * (q * fma(z, fma(q, all<V>(-1.f), all<V>(1.f)), all<V>(1.f)));
 }
 template <int V> __device__ __forceinline__ float sum_of(const Fv<V>& f) {
-  float s = f.v[0];
+  if constexpr (V >= 4) {  // halves added as pairs
+    Fv<V / 2> a, b;
 #pragma unroll
-  for (int i = 1; i < V; ++i) s += f.v[i];
-  return s;
+    for (int i = 0; i < V / 2; ++i) {
+      a.v[i] = f.v[i];
+      b.v[i] = f.v[V / 2 + i];
+    }
+    return sum_of(a + b);
+  } else if constexpr (V == 2) {
+    return f.v[0] + f.v[1];
+  } else {
+    return f.v[0];
+  }
 }
 template <int V> __device__ __forceinline__ Fv<V> gn_params(const void* p, int bf16, int c, float none) {
   Fv<V> f;
@@ -151,7 +160,13 @@ template <int V> __device__ __forceinline__ Fv<V> gn_params(const void* p, int b
   for (int i = 0; i < V; ++i) f.v[i] = gn_param(p, bf16, c + i, none);
   return f;
 }
-__device__ __forceinline__ float gn_rstd(float M2, float n, float eps) { return 1.f / sqrtf(M2 / n + eps); }
+// s / n given inv = 1 / n: one correction makes up for inv's rounding (a constant group's mean is
+// its value)
+__device__ __forceinline__ float over(float s, float n, float inv) {
+  const float m = s * inv;
+  return fmaf(fmaf(-m, n, s), inv, m);
+}
+__device__ __forceinline__ float gn_rstd(float M2, float inv, float eps) { return rsqrtf(fmaf(M2, inv, eps)); }
 
 // ---------------------------------------------------------------- one position per sample
 // The lanes of a group: LG of them, CPL loads of VE channels each: channel (k LG + l) VE + i of
@@ -185,28 +200,41 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
   const float inv = 1.f / (float)p.Cg;
   if constexpr (BWD) let_next_start();
 
-  const int64_t step = (int64_t)gridDim.x * spc;
-  for (int64_t n0 = (int64_t)blockIdx.x * spc; n0 < p.N; n0 += step * U) {
+  // The thread's samples: first, first + step, ...  All threads of the CTA take the same number of
+  // turns (the shuffles want whole warps); a turn past the last sample, or a thread without a
+  // group, reads the thread's first sample (or sample 0) again and stores nothing.
+  const int64_t step = (int64_t)gridDim.x * spc, cta0 = (int64_t)blockIdx.x * spc;
+  const bool any = live && cta0 + sr < p.N;
+  const int64_t first = any ? cta0 + sr : 0;
+  const int turns = (int)((p.N - cta0 + step - 1) / step);                          // of the CTA
+  const int whole_turns = any && first + (turns - 1) * step < p.N ? turns : any ? turns - 1 : 0;  // of the thread
+  const T* xp = static_cast<const T*>(p.x) + first * p.xsn;
+  const T* dp = static_cast<const T*>(p.dy) + first * p.dsn;
+  T* op = (BWD ? static_cast<T*>(p.dx) : static_cast<T*>(p.y)) + first * (BWD ? p.gsn : p.ysn);
+  float* mp = p.mean ? p.mean + first * p.G + gc : nullptr;
+  float* rp = p.mean ? p.rstd + first * p.G + gc : nullptr;
+  const int64_t xs = step * p.xsn, ds = step * p.dsn, os = step * (BWD ? p.gsn : p.ysn), gs = step * p.G;
+  const bool stats = !BWD && l == 0 && mp;
+
+  for (int i = 0; i < turns; i += U) {
     Raw<T, VE> xr[U][CPL], dr[BWD ? U : 1][CPL];
     float mu[U], rs[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t n = n0 + u * step + sr;
-      const int64_t nn = live && n < p.N ? n : 0;
+      const int64_t at = i + u < whole_turns ? i + u : 0;
 #pragma unroll
       for (int k = 0; k < CPL; ++k) {
-        xr[u][k] = ld_raw<T, VE>(static_cast<const T*>(p.x) + nn * p.xsn + ch[k], p.whole);
-        if constexpr (BWD) dr[u][k] = ld_raw<T, VE>(static_cast<const T*>(p.dy) + nn * p.dsn + ch[k], p.whole);
+        xr[u][k] = ld_raw<T, VE>(xp + at * xs + ch[k], p.whole);
+        if constexpr (BWD) dr[u][k] = ld_raw<T, VE>(dp + at * ds + ch[k], p.whole);
       }
       if constexpr (BWD) {
-        mu[u] = p.mean[nn * p.G + gc];
-        rs[u] = p.rstd[nn * p.G + gc];
+        mu[u] = __ldg(mp + at * gs);
+        rs[u] = __ldg(rp + at * gs);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t n = n0 + u * step + sr;
-      const bool ok = live && n < p.N;
+      const bool ok = i + u < whole_turns;
       Fv<VE> x[CPL];
       if constexpr (!BWD) {
         float s = 0.f;
@@ -215,23 +243,22 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
           x[k] = unpack<T, VE>(xr[u][k]);
           s += in[k] ? sum_of(x[k]) : 0.f;
         }
-        const float mean = group_sum<LG>(s) / (float)p.Cg;
+        const float mean = over(group_sum<LG>(s), (float)p.Cg, inv);
         s = 0.f;
 #pragma unroll
         for (int k = 0; k < CPL; ++k) {
           x[k] = x[k] + all<VE>(-mean);
           s += in[k] ? sum_of(x[k] * x[k]) : 0.f;
         }
-        const float rstd = gn_rstd(group_sum<LG>(s), (float)p.Cg, p.eps);
+        const float rstd = gn_rstd(group_sum<LG>(s), inv, p.eps);
         if (ok) {
 #pragma unroll
           for (int k = 0; k < CPL; ++k)
             if (in[k])
-              st_vec<T, VE>(static_cast<T*>(p.y) + n * p.ysn + ch[k],
-                            gn_act<T>(fma(x[k] * all<VE>(rstd), w[k], b[k]), p.silu), p.whole);
-          if (l == 0 && p.mean) {
-            p.mean[n * p.G + g] = mean;
-            p.rstd[n * p.G + g] = rstd;
+              st_vec<T, VE>(op + (i + u) * os + ch[k], gn_act<T>(fma(x[k] * all<VE>(rstd), w[k], b[k]), p.silu), p.whole);
+          if (stats) {
+            mp[(i + u) * gs] = mean;
+            rp[(i + u) * gs] = rstd;
           }
         }
       } else {
@@ -255,7 +282,7 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
 #pragma unroll
           for (int k = 0; k < CPL; ++k)
             if (in[k])
-              st_vec<T, VE>(static_cast<T*>(p.dx) + n * p.gsn + ch[k],
+              st_vec<T, VE>(op + (i + u) * os + ch[k],
                             fma(x[k], all<VE>(-sx), e[k] + all<VE>(-se)) * all<VE>(rs[u]), p.whole);
         }
       }
@@ -306,10 +333,55 @@ struct GnPlace {
   }
 };
 
-// (mean, M2) of each slice and group
+// neg = -mean and rstd of the channels c0 .. c0 + VE - 1, from arrays indexed by group
+template <int VE>
+__device__ __forceinline__ void gn_groups(const float* mean, const float* rstd, int c0, int Cg, Fv<VE>& neg, Fv<VE>& rs) {
+  int g = c0 / Cg, end = (g + 1) * Cg;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    if (c0 + i >= end) ++g, end += Cg;
+    neg.v[i] = -mean[g];
+    rs.v[i] = rstd[g];
+  }
+}
+
+// The slice's outputs; mean and rstd indexed by the block's groups.
 template <typename T, int VE>
-__global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(const __grid_constant__ GnParams p) {
-  extern __shared__ float sh[];  // [2][row lanes][cw]: mean, M2
+__device__ __forceinline__ void gn_apply_rows(const GnParams& p, const GnPlace& at, const float* gmean, const float* grstd) {
+  const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
+  if (rl >= RL) return;
+  for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
+    const int c0 = at.c_lo + k * VE;
+    const Fv<VE> w = gn_params<VE>(p.w, p.p_bf16, c0, 1.f), b = gn_params<VE>(p.b, p.p_bf16, c0, 0.f);
+    wait_for_previous();
+    Fv<VE> neg, sc;
+    gn_groups<VE>(gmean, grstd, k * VE, p.Cg, neg, sc);
+    sc = sc * w;
+    const T* x = static_cast<const T*>(p.x) + at.n * p.xsn + (int64_t)(at.r0 + rl) * p.xss + c0;
+    T* y = static_cast<T*>(p.y) + at.n * p.ysn + (int64_t)(at.r0 + rl) * p.yss + c0;
+    const int64_t xh = RL * p.xss, yh = RL * p.yss;
+    constexpr int U = 4;
+    int r = rl;
+    for (; r + (U - 1) * RL < at.rows; r += U * RL) {
+      Raw<T, VE> raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = ld_raw<T, VE>(x + u * xh, p.whole);
+      x += U * xh;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        st_vec<T, VE>(y + u * yh, gn_act<T>(fma(unpack<T, VE>(raw[u]) + neg, sc, b), p.silu), p.whole);
+      y += U * yh;
+    }
+    for (; r < at.rows; r += RL, x += xh, y += yh)
+      st_vec<T, VE>(y, gn_act<T>(fma(unpack<T, VE>(ld_raw<T, VE>(x, p.whole)) + neg, sc, b), p.silu), p.whole);
+  }
+}
+
+// (mean, M2) of each slice and group; ONE (a single slice): mean and rstd, and the outputs too,
+// the second reading from L1 or L2.
+template <typename T, int VE, bool ONE>
+__global__ void __launch_bounds__(kGnThreads, 3) gn_stats_kernel(const __grid_constant__ GnParams p) {
+  extern __shared__ float sh[];  // [2][row lanes][cw]: mean, M2; ONE: [2][groups]
   const GnPlace at(p);
   const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
   constexpr int U = 4;
@@ -345,7 +417,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(const __grid_const
           M2 = fma(d, d, M2);
         }
         blocks += 1.f;
-        const float f = 1.f / blocks;
+        const float f = rcp(blocks);  // off by 2^-23: the mean by that much of a block's deviation
         const Fv<VE> d = fma(mean, all<VE>(-1.f), m);
         mean = fma(d, all<VE>(f), mean);
         M2 = fma(d * d, all<VE>(U * (blocks - 1.f) * f), M2);
@@ -354,7 +426,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(const __grid_const
       for (; r < at.rows; r += RL) {
         const Fv<VE> d = fma(mean, all<VE>(-1.f), unpack<T, VE>(ld_raw<T, VE>(x, p.whole)));
         x += hop;
-        const float f = 1.f / (cnt + 1.f);
+        const float f = rcp(cnt + 1.f);
         mean = fma(d, all<VE>(f), mean);
         M2 = fma(d * d, all<VE>(cnt * f), M2);
         cnt += 1.f;
@@ -367,35 +439,57 @@ __global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(const __grid_const
     }
   __syncthreads();
   // channels over the row lanes (lane q has the rows q, q + RL, ...)
-  const float inv = 1.f / (float)at.rows;
+  const int lanes = min(RL, at.rows), base = at.rows / RL, extra = at.rows - base * RL;
+  const float nr = (float)at.rows, n0 = (float)base, n1 = (float)(base + 1);
   for (int c = threadIdx.x; c < at.cw; c += kGnThreads) {
-    const int lanes = min(RL, at.rows), base = at.rows / RL, extra = at.rows - base * RL;
     float m = 0.f;
-    for (int q = 0; q < lanes; ++q) m = fmaf((float)(base + (q < extra)), sh[q * at.cw + c], m);
-    m *= inv;
+    for (int q = 0; q < lanes; ++q) m = fmaf(q < extra ? n1 : n0, sh[q * at.cw + c], m);
+    m = over(m, nr, 1.f / nr);
     float M2 = 0.f;
     for (int q = 0; q < lanes; ++q) {
       const float d = sh[q * at.cw + c] - m;
-      M2 += fmaf((float)(base + (q < extra)) * d, d, sh[(RL + q) * at.cw + c]);
+      M2 += fmaf((q < extra ? n1 : n0) * d, d, sh[(RL + q) * at.cw + c]);
     }
     sh[c] = m;  // only this thread reads and writes this channel here
     sh[RL * at.cw + c] = M2;
   }
   __syncthreads();
-  // groups over their channels
-  const int lane = threadIdx.x & 31;
-  for (int gi = threadIdx.x >> 5; gi < at.cw / p.Cg; gi += kGnThreads / 32) {
-    const float* m = sh + gi * p.Cg;
-    float mean = 0.f;
-    for (int c = lane; c < p.Cg; c += 32) mean += m[c];
-    mean = warp_sum(mean) / (float)p.Cg;
-    float M2 = 0.f;
-    for (int c = lane; c < p.Cg; c += 32) {
+  // groups over their channels: a few lanes each
+  const int ng = at.cw / p.Cg;
+  const float nc = (float)p.Cg, invc = 1.f / nc;
+  int lg = 1;
+  while (lg < 32 && lg < p.Cg) lg *= 2;
+  const int l = threadIdx.x & (lg - 1);
+  float* gmean = sh + 2 * RL * at.cw;
+  for (int g0 = 0; g0 < ng; g0 += kGnThreads / lg) {
+    const int gi = g0 + threadIdx.x / lg;
+    const float* m = sh + min(gi, ng - 1) * p.Cg;
+    float mean = 0.f, M2 = 0.f;
+    for (int c = l; c < p.Cg; c += lg) mean += m[c];
+    for (int o = lg / 2; o > 0; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
+    mean = over(mean, nc, invc);
+    for (int c = l; c < p.Cg; c += lg) {
       const float d = m[c] - mean;
-      M2 += fmaf((float)at.rows * d, d, m[RL * at.cw + c]);
+      M2 += fmaf(nr * d, d, m[RL * at.cw + c]);
     }
-    M2 = warp_sum(M2);
-    if (lane == 0) p.stats[(int64_t)blockIdx.x * p.G + at.c_lo / p.Cg + gi] = make_float2(mean, M2);
+    for (int o = lg / 2; o > 0; o >>= 1) M2 += __shfl_xor_sync(0xffffffffu, M2, o);
+    if (l == 0 && gi < ng) {
+      if constexpr (ONE) {
+        const float rstd = gn_rstd(M2, invc / nr, p.eps);
+        gmean[gi] = mean;
+        gmean[ng + gi] = rstd;
+        if (p.mean) {
+          p.mean[(int64_t)at.n * p.G + at.c_lo / p.Cg + gi] = mean;
+          p.rstd[(int64_t)at.n * p.G + at.c_lo / p.Cg + gi] = rstd;
+        }
+      } else {
+        p.stats[(int64_t)blockIdx.x * p.G + at.c_lo / p.Cg + gi] = make_float2(mean, M2);
+      }
+    }
+  }
+  if constexpr (ONE) {
+    __syncthreads();
+    gn_apply_rows<T, VE>(p, at, gmean, gmean + ng);
   }
 }
 
@@ -422,82 +516,96 @@ __global__ void __launch_bounds__(256) gn_join_kernel(const __grid_constant__ Gn
   M2 = warp_sum(M2);
   if (lane == 0) {
     p.mean[i] = mean;
-    p.rstd[i] = gn_rstd(M2, total, p.eps);
+    p.rstd[i] = gn_rstd(M2, 1.f / total, p.eps);
   }
 }
 
 template <typename T, int VE>
-__global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(const __grid_constant__ GnParams p) {
+__global__ void __launch_bounds__(kGnThreads, 3) gn_apply_kernel(const __grid_constant__ GnParams p) {
   const GnPlace at(p);
+  const int64_t g0 = (int64_t)at.n * p.G + at.c_lo / p.Cg;
+  gn_apply_rows<T, VE>(p, at, p.mean + g0, p.rstd + g0);
+}
+
+// The slice's dx; the means of e xh and of e indexed by the block's groups.
+template <typename T, int VE>
+__device__ __forceinline__ void gn_dx_rows(const GnParams& p, const GnPlace& at, const float* mx, const float* me) {
   const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
   if (rl >= RL) return;
+  const int64_t g0 = (int64_t)at.n * p.G + at.c_lo / p.Cg;
   for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
     const int c0 = at.c_lo + k * VE;
     const Fv<VE> w = gn_params<VE>(p.w, p.p_bf16, c0, 1.f), b = gn_params<VE>(p.b, p.p_bf16, c0, 0.f);
+    Fv<VE> neg, rstd, sx, se;
+    gn_groups<VE>(p.mean + g0, p.rstd + g0, k * VE, p.Cg, neg, rstd);
     wait_for_previous();
-    Fv<VE> neg, sc;
-#pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      const int64_t j = (int64_t)at.n * p.G + (c0 + i) / p.Cg;
-      neg.v[i] = -p.mean[j];
-      sc.v[i] = p.rstd[j];
-    }
-    sc = sc * w;
-    const T* x = static_cast<const T*>(p.x) + at.n * p.xsn + (int64_t)at.r0 * p.xss + c0;
-    T* y = static_cast<T*>(p.y) + at.n * p.ysn + (int64_t)at.r0 * p.yss + c0;
+    gn_groups<VE>(mx, me, k * VE, p.Cg, sx, se);
+    se = se * all<VE>(-1.f);
+    const T* x = static_cast<const T*>(p.x) + at.n * p.xsn + (int64_t)(at.r0 + rl) * p.xss + c0;
+    const T* dy = static_cast<const T*>(p.dy) + at.n * p.dsn + (int64_t)(at.r0 + rl) * p.dss + c0;
+    T* dx = static_cast<T*>(p.dx) + at.n * p.gsn + (int64_t)(at.r0 + rl) * p.gss + c0;
+    const int64_t xh = RL * p.xss, dh = RL * p.dss, gh = RL * p.gss;
+    auto one = [&](const Raw<T, VE>& xr, const Raw<T, VE>& dr, T* to) {
+      const Fv<VE> v = (unpack<T, VE>(xr) + neg) * rstd;
+      const Fv<VE> dz = gn_dact<T>(unpack<T, VE>(dr), fma(v, w, b), p.silu);
+      st_vec<T, VE>(to, fma(v, sx, fma(dz, w, se)) * rstd, p.whole);
+    };
     constexpr int U = 4;
-    for (int r = rl; r < at.rows; r += U * RL) {
-      Raw<T, VE> raw[U];
+    int r = rl;
+    for (; r + (U - 1) * RL < at.rows; r += U * RL) {
+      Raw<T, VE> xr[U], dr[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (r + u * RL < at.rows) raw[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
+      for (int u = 0; u < U; ++u) {
+        xr[u] = ld_raw<T, VE>(x + u * xh, p.whole);
+        dr[u] = ld_raw<T, VE>(dy + u * dh, p.whole);
+      }
+      x += U * xh, dy += U * dh;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (r + u * RL < at.rows)
-          st_vec<T, VE>(y + (int64_t)(r + u * RL) * p.yss, gn_act<T>(fma(unpack<T, VE>(raw[u]) + neg, sc, b), p.silu),
-                        p.whole);
+      for (int u = 0; u < U; ++u) one(xr[u], dr[u], dx + u * gh);
+      dx += U * gh;
     }
+    for (; r < at.rows; r += RL, x += xh, dy += dh, dx += gh)
+      one(ld_raw<T, VE>(x, p.whole), ld_raw<T, VE>(dy, p.whole), dx);
   }
 }
 
-// The gradient's sums per channel of each slice: part[n * slices + slice][2][C]
-template <typename T, int VE>
-__global__ void __launch_bounds__(kGnThreads) gn_sums_kernel(const __grid_constant__ GnParams p) {
-  extern __shared__ float sh[];  // [2][row lanes][cw]
+// The gradient's sums per channel of each slice: part[n * slices + slice][2][C]; ONE: dx too.
+template <typename T, int VE, bool ONE>
+__global__ void __launch_bounds__(kGnThreads, 2) gn_sums_kernel(const __grid_constant__ GnParams p) {
+  extern __shared__ float sh[];  // [2][row lanes][cw]; ONE: [2][cw], [2][groups]
   const GnPlace at(p);
   const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
+  const int64_t g0 = (int64_t)at.n * p.G + at.c_lo / p.Cg;
   let_next_start();
   if (rl < RL)
     for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
       const int c0 = at.c_lo + k * VE;
       const Fv<VE> w = gn_params<VE>(p.w, p.p_bf16, c0, 1.f), b = gn_params<VE>(p.b, p.p_bf16, c0, 0.f);
       Fv<VE> neg, rstd, a0 = all<VE>(0.f), a1 = all<VE>(0.f);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const int64_t j = (int64_t)at.n * p.G + (c0 + i) / p.Cg;
-        neg.v[i] = -p.mean[j];
-        rstd.v[i] = p.rstd[j];
-      }
-      const T* x = static_cast<const T*>(p.x) + at.n * p.xsn + (int64_t)at.r0 * p.xss + c0;
-      const T* dy = static_cast<const T*>(p.dy) + at.n * p.dsn + (int64_t)at.r0 * p.dss + c0;
+      gn_groups<VE>(p.mean + g0, p.rstd + g0, k * VE, p.Cg, neg, rstd);
+      const T* x = static_cast<const T*>(p.x) + at.n * p.xsn + (int64_t)(at.r0 + rl) * p.xss + c0;
+      const T* dy = static_cast<const T*>(p.dy) + at.n * p.dsn + (int64_t)(at.r0 + rl) * p.dss + c0;
+      const int64_t xh = RL * p.xss, dh = RL * p.dss;
+      auto one = [&](const Raw<T, VE>& xr, const Raw<T, VE>& dr) {
+        const Fv<VE> v = (unpack<T, VE>(xr) + neg) * rstd;
+        const Fv<VE> dz = gn_dact<T>(unpack<T, VE>(dr), fma(v, w, b), p.silu);
+        a0 = fma(dz, v, a0);
+        a1 = a1 + dz;
+      };
       constexpr int U = 4;
-      for (int r = rl; r < at.rows; r += U * RL) {
+      int r = rl;
+      for (; r + (U - 1) * RL < at.rows; r += U * RL) {
         Raw<T, VE> xr[U], dr[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (r + u * RL < at.rows) {
-            xr[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
-            dr[u] = ld_raw<T, VE>(dy + (int64_t)(r + u * RL) * p.dss, p.whole);
-          }
+        for (int u = 0; u < U; ++u) {
+          xr[u] = ld_raw<T, VE>(x + u * xh, p.whole);
+          dr[u] = ld_raw<T, VE>(dy + u * dh, p.whole);
+        }
+        x += U * xh, dy += U * dh;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (r + u * RL < at.rows) {
-            const Fv<VE> xh = (unpack<T, VE>(xr[u]) + neg) * rstd;
-            const Fv<VE> dz = gn_dact<T>(unpack<T, VE>(dr[u]), fma(xh, w, b), p.silu);
-            a0 = fma(dz, xh, a0);
-            a1 = a1 + dz;
-          }
+        for (int u = 0; u < U; ++u) one(xr[u], dr[u]);
       }
+      for (; r < at.rows; r += RL, x += xh, dy += dh) one(ld_raw<T, VE>(x, p.whole), ld_raw<T, VE>(dy, p.whole));
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         sh[rl * at.cw + k * VE + i] = a0.v[i];
@@ -505,11 +613,28 @@ __global__ void __launch_bounds__(kGnThreads) gn_sums_kernel(const __grid_consta
       }
     }
   __syncthreads();
+  float* tot = sh + 2 * RL * at.cw;
   for (int i = threadIdx.x; i < 2 * at.cw; i += kGnThreads) {
     const int which = i >= at.cw, c = which ? i - at.cw : i;
     float v = 0.f;
     for (int q = 0; q < RL; ++q) v += sh[(which * RL + q) * at.cw + c];
     p.part[((int64_t)blockIdx.x * 2 + which) * p.C + at.c_lo + c] = v;
+    if constexpr (ONE) tot[i] = v * gn_param(p.w, p.p_bf16, at.c_lo + c, 1.f);
+  }
+  if constexpr (ONE) {
+    __syncthreads();
+    const int lane = threadIdx.x & 31, ng = at.cw / p.Cg;
+    float* gm = tot + 2 * at.cw;
+    const float inv = 1.f / ((float)p.S * (float)p.Cg);
+    for (int i = threadIdx.x >> 5; i < 2 * ng; i += kGnThreads / 32) {
+      const int which = i >= ng, gi = which ? i - ng : i;
+      float v = 0.f;
+      for (int c = lane; c < p.Cg; c += 32) v += tot[which * at.cw + gi * p.Cg + c];
+      v = warp_sum(v);
+      if (lane == 0) gm[i] = v * inv;
+    }
+    __syncthreads();
+    gn_dx_rows<T, VE>(p, at, gm, gm + ng);
   }
 }
 
@@ -552,44 +677,10 @@ __global__ void __launch_bounds__(256) gn_mid_kernel(const __grid_constant__ GnP
 }
 
 template <typename T, int VE>
-__global__ void __launch_bounds__(kGnThreads) gn_dx_kernel(const __grid_constant__ GnParams p) {
+__global__ void __launch_bounds__(kGnThreads, 2) gn_dx_kernel(const __grid_constant__ GnParams p) {
   const GnPlace at(p);
-  const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
-  if (rl >= RL) return;
-  for (int k = threadIdx.x - rl * per; k < nchunk; k += per) {
-    const int c0 = at.c_lo + k * VE;
-    const Fv<VE> w = gn_params<VE>(p.w, p.p_bf16, c0, 1.f), b = gn_params<VE>(p.b, p.p_bf16, c0, 0.f);
-    wait_for_previous();
-    Fv<VE> neg, rstd, sx, se;
-#pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      const int g = (c0 + i) / p.Cg;
-      neg.v[i] = -p.mean[(int64_t)at.n * p.G + g];
-      rstd.v[i] = p.rstd[(int64_t)at.n * p.G + g];
-      sx.v[i] = -p.gmean[((int64_t)at.n * 2) * p.G + g];
-      se.v[i] = -p.gmean[((int64_t)at.n * 2 + 1) * p.G + g];
-    }
-    const T* x = static_cast<const T*>(p.x) + at.n * p.xsn + (int64_t)at.r0 * p.xss + c0;
-    const T* dy = static_cast<const T*>(p.dy) + at.n * p.dsn + (int64_t)at.r0 * p.dss + c0;
-    T* dx = static_cast<T*>(p.dx) + at.n * p.gsn + (int64_t)at.r0 * p.gss + c0;
-    constexpr int U = 4;
-    for (int r = rl; r < at.rows; r += U * RL) {
-      Raw<T, VE> xr[U], dr[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (r + u * RL < at.rows) {
-          xr[u] = ld_raw<T, VE>(x + (int64_t)(r + u * RL) * p.xss, p.whole);
-          dr[u] = ld_raw<T, VE>(dy + (int64_t)(r + u * RL) * p.dss, p.whole);
-        }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (r + u * RL < at.rows) {
-          const Fv<VE> xh = (unpack<T, VE>(xr[u]) + neg) * rstd;
-          const Fv<VE> dz = gn_dact<T>(unpack<T, VE>(dr[u]), fma(xh, w, b), p.silu);
-          st_vec<T, VE>(dx + (int64_t)(r + u * RL) * p.gss, fma(xh, sx, fma(dz, w, se)) * rstd, p.whole);
-        }
-    }
-  }
+  const int64_t g0 = (int64_t)at.n * 2 * p.G + at.c_lo / p.Cg;
+  gn_dx_rows<T, VE>(p, at, p.gmean + g0, p.gmean + g0 + p.G);
 }
 
 // ---------------------------------------------------------------- groups of more than 4096 channels
@@ -619,7 +710,7 @@ __global__ void __launch_bounds__(256) gn_any_fwd_kernel(GnParams p) {
     const float d = to_f(x[(i / p.Cg) * p.xss + i % p.Cg]) - mean;
     s = fmaf(d, d, s);
   }
-  const float rstd = 1.f / sqrtf(block_sum(s) / (float)M + p.eps);
+  const float rstd = rsqrtf(block_sum(s) / (float)M + p.eps);
   if (threadIdx.x == 0 && p.mean) {
     p.mean[blockIdx.x] = mean;
     p.rstd[blockIdx.x] = rstd;
@@ -707,7 +798,7 @@ constexpr int kGnMostCg = 4096;  // channels of a group in the kernels above
 
 // One position: loads of ve channels, LG lanes and CPL loads per group.
 struct GnRowPlan { bool ok; int lg, cpl, gpc, spc, gy; int64_t ctas; };
-static GnRowPlan gn_row_plan(int64_t N, int64_t S, int64_t G, int64_t Cg, int ve) {
+static GnRowPlan gn_row_plan(int64_t N, int64_t S, int64_t G, int64_t Cg, int ve, bool bwd = false) {
   GnRowPlan r{};
   const int64_t chunks = Cg / ve;
   r.lg = 1;
@@ -719,7 +810,8 @@ static GnRowPlan gn_row_plan(int64_t N, int64_t S, int64_t G, int64_t Cg, int ve
   r.gy = (int)((G + most - 1) / most);
   r.gpc = (int)((G + r.gy - 1) / r.gy);
   r.spc = most / r.gpc;
-  const int64_t need = (N + r.spc - 1) / r.spc, fill = (int64_t)148 * 8 / (r.gy < 8 ? r.gy : 8);
+  // one wave of the CTAs that are resident: a thread's parameters are loaded once
+  const int64_t need = (N + r.spc - 1) / r.spc, fill = ((int64_t)148 * (bwd ? 2 : 4) + r.gy - 1) / r.gy;
   r.ctas = need < fill ? need : fill;
   return r;
 }
@@ -728,29 +820,39 @@ static int64_t gn_row_parts(int64_t N, int64_t G, int64_t Cg) {
   int64_t most = 0;
   for (int ve = 1; ve <= 8; ve *= 2)
     if (Cg % ve == 0) {
-      const GnRowPlan r = gn_row_plan(N, 1, G, Cg, ve);
+      const GnRowPlan r = gn_row_plan(N, 1, G, Cg, ve, true);
       if (r.ok && r.ctas > most) most = r.ctas;
     }
   return most;
 }
-// Two passes: slices per sample so that a few CTAs per SM run, each of 32 positions or more.
-struct GnPlan { int64_t slices, rows, cb, gz; };
+// Several positions.  One pass when a sample's block of channels is small enough to be read again
+// from L1 (64 KB), the blocks then about 64 channels wide for more CTAs; else slices of each
+// sample, 32 positions or more, in one wave of three CTAs per SM: a CTA's fixed cost (joining its
+// threads' sums) is that of some 30 rows.
+struct GnPlan { int64_t slices, rows, cb, gz; bool one; };
+static int64_t gn_block(int64_t C, int64_t Cg, int64_t want) {  // whole groups, about `want` channels
+  if (C <= want) return C;
+  return Cg >= want ? Cg : want / Cg * Cg;
+}
 static GnPlan gn_plan(int64_t N, int64_t S, int64_t C, int64_t G) {
   GnPlan r{};
   const int64_t Cg = C / G;
-  r.cb = C;
-  if (C > 512) {  // blocks of whole groups, about 512 channels
-    int64_t g = 512 / Cg;
-    if (g < 1) g = 1;
-    r.cb = g * Cg;
+  r.cb = gn_block(C, Cg, 64);
+  r.one = S * r.cb <= 32768 && r.cb <= 1024;
+  if (r.one && N * ((C + r.cb - 1) / r.cb) > 592) {  // CTAs enough: wider blocks
+    const int64_t wide = gn_block(C, Cg, 256);
+    if (S * wide <= 32768) r.cb = wide;
   }
+  if (!r.one) r.cb = gn_block(C, Cg, 512);
   r.gz = (C + r.cb - 1) / r.cb;
-  const int64_t want = (148 * 8 + N * r.gz - 1) / (N * r.gz);
-  int64_t rows = (S + want - 1) / want;
-  if (rows < 32) rows = 32;
-  if (rows > S) rows = S;
-  r.rows = rows;
-  r.slices = (S + rows - 1) / rows;
+  r.rows = S;
+  r.slices = 1;
+  if (!r.one) {
+    const int64_t want = (148 * 3) / (N * r.gz) > 0 ? (148 * 3) / (N * r.gz) : 1;
+    r.rows = (S + want - 1) / want;
+    if (r.rows < 32) r.rows = S < 32 ? S : 32;
+    r.slices = (S + r.rows - 1) / r.rows;
+  }
   return r;
 }
 // Channels per load: as many as 16 bytes hold and divide d (the group's channels, or the row's).
@@ -809,11 +911,21 @@ template <typename T, bool BWD> static void gn_rows(const GnParams& p, const GnR
 enum GnPass { kStats, kApply, kSums, kDx };
 template <typename T, int VE> static void gn_pass(GnPass pass, const GnParams& p, const GnPlan& r, cudaStream_t s) {
   const dim3 grid((unsigned)(r.slices * p.N), (unsigned)r.gz);
-  const size_t smem = (size_t)2 * gn_lanes((int)(r.cb / VE)) * r.cb * 4;
+  // the row lanes' values of the widest block; a narrower last one has no more of them
+  const size_t values = (size_t)2 * gn_lanes((int)(r.cb / VE)) * r.cb > 2 * kGnThreads * VE
+                            ? (size_t)2 * gn_lanes((int)(r.cb / VE)) * r.cb : 2 * kGnThreads * VE;
+  const size_t groups = 2 * (r.cb / p.Cg), smem = (values + (r.one ? groups : 0)) * 4;
+  const size_t smem_sums = (values + (r.one ? 2 * r.cb + groups : 0)) * 4;
   switch (pass) {
-    case kStats: gn_stats_kernel<T, VE><<<grid, kGnThreads, smem, s>>>(p); break;
+    case kStats:
+      if (r.one) gn_stats_kernel<T, VE, true><<<grid, kGnThreads, smem, s>>>(p);
+      else gn_stats_kernel<T, VE, false><<<grid, kGnThreads, smem, s>>>(p);
+      break;
     case kApply: launch_dependent(gn_apply_kernel<T, VE>, grid, kGnThreads, 0, s, p); break;
-    case kSums: gn_sums_kernel<T, VE><<<grid, kGnThreads, smem, s>>>(p); break;
+    case kSums:
+      if (r.one) gn_sums_kernel<T, VE, true><<<grid, kGnThreads, smem_sums, s>>>(p);
+      else gn_sums_kernel<T, VE, false><<<grid, kGnThreads, smem_sums, s>>>(p);
+      break;
     case kDx: launch_dependent(gn_dx_kernel<T, VE>, grid, kGnThreads, 0, s, p); break;
   }
 }
@@ -851,6 +963,7 @@ extern "C" size_t hdc_group_norm_workspace_bytes(int64_t N, int64_t S, int64_t C
   if (N < 1 || S < 1 || C < 1 || G < 1 || C % G != 0 || C / G > kGnMostCg) return 0;
   // one position takes no second pass with wider loads if it takes none with single channels
   if (gn_row_plan(N, S, G, C / G, 1).ok) return 0;
+  if (gn_plan(N, S, C, G).one) return 0;
   // the slices' statistics, then the samples' mean and rstd when the caller does not want them
   return (size_t)N * G * 8 * (gn_plan(N, S, C, G).slices + 1);
 }
@@ -894,12 +1007,13 @@ extern "C" int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t
   p.slices = (int)plan.slices; p.rows = (int)plan.rows; p.cb = (int)plan.cb;
   ve = gn_width(es, plan.cb | C);
   p.whole = gn_whole(es, ve, ptr, stride, 2);
-  if (!p.mean) {
+  if (!p.mean && !plan.one) {
     p.mean = reinterpret_cast<float*>(p.stats + N * plan.slices * G);
     p.rstd = p.mean + N * G;
   }
   gn_pass(kStats, dtype, p, plan, ve, s);
   if (int e = launch_status("gn_stats_kernel")) return e;
+  if (plan.one) return HDC_OK;
   launch_dependent(gn_join_kernel, dim3((unsigned)((N * G + 7) / 8)), 256, 0, s, p);
   if (int e = launch_status("gn_join_kernel")) return e;
   gn_pass(kApply, dtype, p, plan, ve, s);
@@ -954,7 +1068,7 @@ extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_
     const int64_t stride[] = {N > 1 ? x_sn : 0,  S > 1 ? x_ss : 0,  N > 1 ? dy_sn : 0,
                               S > 1 ? dy_ss : 0, N > 1 ? dx_sn : 0, S > 1 ? dx_ss : 0};
     int ve = gn_width(es, p.Cg);
-    const GnRowPlan row = gn_row_plan(N, S, G, p.Cg, ve);
+    const GnRowPlan row = gn_row_plan(N, S, G, p.Cg, ve, true);
     if (row.ok) {
       p.whole = gn_whole(es, ve, ptr, stride, 3);
       if (dtype == HDC_F32) gn_rows<float, true>(p, row, ve, s);
@@ -970,14 +1084,16 @@ extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_
       p.gmean = p.sums + N * 2 * C;
       gn_pass(kSums, dtype, p, plan, ve, s);
       if (int e = launch_status("gn_sums_kernel")) return e;
+      parts = N;
       const int block = gn_mid_block(p.C, p.Cg), items = 2 * block, strands = items < 256 ? 256 / items : 1;
+      if (!plan.one) {
       launch_dependent(gn_mid_kernel, dim3((unsigned)N, (unsigned)((C + block - 1) / block)), 256,
                        (size_t)(strands + 1) * items * 4, s, p, block);
       if (int e = launch_status("gn_mid_kernel")) return e;
       gn_pass(kDx, dtype, p, plan, ve, s);
       if (int e = launch_status("gn_dx_kernel")) return e;
       p.part = p.sums;
-      parts = N;
+      }
     }
   }
   if (!dweight && !dbias) return HDC_OK;
