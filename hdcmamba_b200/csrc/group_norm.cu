@@ -21,298 +21,9 @@
 // squares, and blocks, threads and slices are joined by
 //   n = n1 + n2, mean = mean1 + (mean2 - mean1) n2/n, M2 = M2_1 + M2_2 + (mean2 - mean1)^2 n1 n2/n.
 // Channels per load: as many as 16 bytes, the rows' alignment and (S = 1) the group allow.
-#include "vec.cuh"
+#include "group_norm.cuh"
 
 namespace hdc {
-
-struct GnParams {
-  const void* x; int64_t xsn, xss;
-  const void* w; const void* b; int p_bf16;
-  void* y; int64_t ysn, yss;
-  float* mean; float* rstd;
-  const void* dy; int64_t dsn, dss;
-  void* dx; int64_t gsn, gss;
-  float* part;     // gradient: sums of dz xh and of dz per channel, [part][2][C]
-  float2* stats;   // two passes: (mean, M2) of each slice, [N][slices][G]
-  float* sums;     // two passes, gradient: part over the slices, [N][2][C]
-  float* gmean;    // and the groups' means of e xh and of e, [N][2][G]
-  void* dw; void* db;
-  int N, S, C, G, Cg;
-  float eps; int silu;
-  int slices, rows;  // two passes: slices per sample, positions per slice
-  int cb;            // two passes: channels per CTA (whole groups, or all)
-  int whole;         // the rows allow whole loads (else one by one, with the same arithmetic)
-};
-
-__device__ __forceinline__ float gn_param(const void* p, int bf16, int i, float none) {
-  if (!p) return none;
-  return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];
-}
-
-// VE neighbouring values as loaded, at once or (rows that do not allow it) one by one
-template <typename T, int VE> struct Raw { static constexpr int kW = VE * (int)sizeof(T) >= 4 ? VE * (int)sizeof(T) / 4 : 1; uint32_t w[kW]; };
-template <typename T, int VE> __device__ __forceinline__ Raw<T, VE> ld_raw(const T* p, int whole) {
-  Raw<T, VE> r;
-  constexpr int bytes = VE * (int)sizeof(T);
-  if (VE > 1 && !whole) {
-#pragma unroll
-    for (int i = 0; i < Raw<T, VE>::kW; ++i) {
-      if constexpr (sizeof(T) == 4) {
-        r.w[i] = __float_as_uint(p[i]);
-      } else {
-        const unsigned short* q = reinterpret_cast<const unsigned short*>(p) + 2 * i;
-        r.w[i] = q[0] | (uint32_t)q[VE > 1 ? 1 : 0] << 16;
-      }
-    }
-    return r;
-  }
-  if constexpr (bytes == 16) {
-    const uint4 q = ldg16(p);
-    r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
-  } else if constexpr (bytes == 8) {
-    const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
-    r.w[0] = q.x; r.w[1] = q.y;
-  } else if constexpr (bytes == 4) {
-    r.w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-  } else {
-    r.w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
-  }
-  return r;
-}
-template <typename T, int VE> __device__ __forceinline__ Fv<VE> unpack(const Raw<T, VE>& r) {
-  Fv<VE> f;
-#pragma unroll
-  for (int i = 0; i < VE; ++i) {
-    if constexpr (sizeof(T) == 4) f.v[i] = __uint_as_float(r.w[i]);
-    else f.v[i] = __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
-  }
-  return f;
-}
-template <typename T, int VE> __device__ __forceinline__ void st_vec(T* p, const Fv<VE>& f, int whole) {
-  constexpr int bytes = VE * (int)sizeof(T);
-  if (VE > 1 && !whole) {
-#pragma unroll
-    for (int i = 0; i < VE; ++i) p[i] = from_f<T>(f.v[i]);
-    return;
-  }
-  if constexpr (bytes == 2) {
-    *p = from_f<T>(f.v[0]);
-  } else {
-    uint32_t w[bytes / 4];
-#pragma unroll
-    for (int i = 0; i < bytes / 4; ++i) {
-      if constexpr (sizeof(T) == 4) {
-        w[i] = __float_as_uint(f.v[i]);
-      } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(f.v[2 * i], f.v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-    }
-    if constexpr (bytes == 16) stg16(p, make_uint4(w[0], w[1], w[2], w[3]));
-    else if constexpr (bytes == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t*>(p) = w[0];
-  }
-}
-
-// sigmoid: hardware 2^x and reciprocal for bf16 tensors (a few 2^-23 off), the library's for fp32
-template <typename T, int V> __device__ __forceinline__ Fv<V> gn_sigmoid(const Fv<V>& z) {
-  Fv<V> q;
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) q.v[i] = 1.f / (1.f + expf(-z.v[i]));
-  } else {
-    q = z * all<V>(-1.4426950408889634f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) q.v[i] = ex2(q.v[i]);
-    q = q + all<V>(1.f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) q.v[i] = rcp(q.v[i]);
-  }
-  return q;
-}
-template <typename T, int V> __device__ __forceinline__ Fv<V> gn_act(const Fv<V>& z, int silu) {
-  return silu ? z * gn_sigmoid<T>(z) : z;
-}
-// dz from dy
-template <typename T, int V> __device__ __forceinline__ Fv<V> gn_dact(const Fv<V>& dy, const Fv<V>& z, int silu) {
-  if (!silu) return dy;
-  const Fv<V> q = gn_sigmoid<T>(z);
-  return dy * (q * fma(z, fma(q, all<V>(-1.f), all<V>(1.f)), all<V>(1.f)));
-}
-template <int V> __device__ __forceinline__ float sum_of(const Fv<V>& f) {
-  if constexpr (V >= 4) {  // halves added as pairs
-    Fv<V / 2> a, b;
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      a.v[i] = f.v[i];
-      b.v[i] = f.v[V / 2 + i];
-    }
-    return sum_of(a + b);
-  } else if constexpr (V == 2) {
-    return f.v[0] + f.v[1];
-  } else {
-    return f.v[0];
-  }
-}
-template <int V> __device__ __forceinline__ Fv<V> gn_params(const void* p, int bf16, int c, float none) {
-  Fv<V> f;
-#pragma unroll
-  for (int i = 0; i < V; ++i) f.v[i] = gn_param(p, bf16, c + i, none);
-  return f;
-}
-// s / n given inv = 1 / n: one correction makes up for inv's rounding (a constant group's mean is
-// its value)
-__device__ __forceinline__ float over(float s, float n, float inv) {
-  const float m = s * inv;
-  return fmaf(fmaf(-m, n, s), inv, m);
-}
-__device__ __forceinline__ float gn_rstd(float M2, float inv, float eps) { return rsqrtf(fmaf(M2, inv, eps)); }
-
-// ---------------------------------------------------------------- one position per sample
-// The lanes of a group: LG of them, CPL loads of VE channels each: channel (k LG + l) VE + i of
-// the group.  Threads: (sample of the CTA, group, lane), groups from blockIdx.y * gpc.
-// FULL: the lanes' loads are exactly the group.
-template <int LG> __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int o = LG / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-template <typename T, int VE, int CPL, int U, bool BWD, int LG, bool FULL>
-__global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnParams p, int gpc, int spc) {
-  const int l = threadIdx.x % LG, gi = threadIdx.x / LG % gpc, sr = threadIdx.x / LG / gpc;
-  const int g = blockIdx.y * gpc + gi;
-  const bool live = g < p.G && sr < spc;
-  const int gc = live ? g : 0, c0 = gc * p.Cg;
-  constexpr int M = VE * CPL;
-  int ch[CPL];
-  bool in[CPL];
-  Fv<VE> w[CPL], b[CPL], dw[BWD ? CPL : 1], db[BWD ? CPL : 1];
-#pragma unroll
-  for (int k = 0; k < CPL; ++k) {
-    const int c = (k * LG + l) * VE;
-    in[k] = FULL || c < p.Cg;
-    ch[k] = c0 + (in[k] ? c : 0);
-    w[k] = gn_params<VE>(p.w, p.p_bf16, ch[k], 1.f);
-    b[k] = gn_params<VE>(p.b, p.p_bf16, ch[k], 0.f);
-    if constexpr (BWD) dw[k] = db[k] = all<VE>(0.f);
-  }
-  const float inv = 1.f / (float)p.Cg;
-  if constexpr (BWD) let_next_start();
-
-  // The thread's samples: first, first + step, ...  All threads of the CTA take the same number of
-  // turns (the shuffles want whole warps); a turn past the last sample, or a thread without a
-  // group, reads the thread's first sample (or sample 0) again and stores nothing.
-  const int64_t step = (int64_t)gridDim.x * spc, cta0 = (int64_t)blockIdx.x * spc;
-  const bool any = live && cta0 + sr < p.N;
-  const int64_t first = any ? cta0 + sr : 0;
-  const int turns = (int)((p.N - cta0 + step - 1) / step);                          // of the CTA
-  const int whole_turns = any && first + (turns - 1) * step < p.N ? turns : any ? turns - 1 : 0;  // of the thread
-  const T* xp = static_cast<const T*>(p.x) + first * p.xsn;
-  const T* dp = static_cast<const T*>(p.dy) + first * p.dsn;
-  T* op = (BWD ? static_cast<T*>(p.dx) : static_cast<T*>(p.y)) + first * (BWD ? p.gsn : p.ysn);
-  float* mp = p.mean ? p.mean + first * p.G + gc : nullptr;
-  float* rp = p.mean ? p.rstd + first * p.G + gc : nullptr;
-  const int64_t xs = step * p.xsn, ds = step * p.dsn, os = step * (BWD ? p.gsn : p.ysn), gs = step * p.G;
-  const bool stats = !BWD && l == 0 && mp;
-
-  for (int i = 0; i < turns; i += U) {
-    Raw<T, VE> xr[U][CPL], dr[BWD ? U : 1][CPL];
-    float mu[U], rs[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = i + u < whole_turns ? i + u : 0;
-#pragma unroll
-      for (int k = 0; k < CPL; ++k) {
-        xr[u][k] = ld_raw<T, VE>(xp + at * xs + ch[k], p.whole);
-        if constexpr (BWD) dr[u][k] = ld_raw<T, VE>(dp + at * ds + ch[k], p.whole);
-      }
-      if constexpr (BWD) {
-        mu[u] = __ldg(mp + at * gs);
-        rs[u] = __ldg(rp + at * gs);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool ok = i + u < whole_turns;
-      Fv<VE> x[CPL];
-      if constexpr (!BWD) {
-        float s = 0.f;
-#pragma unroll
-        for (int k = 0; k < CPL; ++k) {
-          x[k] = unpack<T, VE>(xr[u][k]);
-          s += in[k] ? sum_of(x[k]) : 0.f;
-        }
-        const float mean = over(group_sum<LG>(s), (float)p.Cg, inv);
-        s = 0.f;
-#pragma unroll
-        for (int k = 0; k < CPL; ++k) {
-          x[k] = x[k] + all<VE>(-mean);
-          s += in[k] ? sum_of(x[k] * x[k]) : 0.f;
-        }
-        const float rstd = gn_rstd(group_sum<LG>(s), inv, p.eps);
-        if (ok) {
-#pragma unroll
-          for (int k = 0; k < CPL; ++k)
-            if (in[k])
-              st_vec<T, VE>(op + (i + u) * os + ch[k], gn_act<T>(fma(x[k] * all<VE>(rstd), w[k], b[k]), p.silu), p.whole);
-          if (stats) {
-            mp[(i + u) * gs] = mean;
-            rp[(i + u) * gs] = rstd;
-          }
-        }
-      } else {
-        Fv<VE> e[CPL];
-        float se = 0.f, sx = 0.f;
-#pragma unroll
-        for (int k = 0; k < CPL; ++k) {
-          x[k] = (unpack<T, VE>(xr[u][k]) + all<VE>(-mu[u])) * all<VE>(rs[u]);
-          const Fv<VE> dz = gn_dact<T>(unpack<T, VE>(dr[u][k]), fma(x[k], w[k], b[k]), p.silu);
-          e[k] = dz * w[k];
-          if (ok && in[k]) {
-            dw[k] = fma(dz, x[k], dw[k]);
-            db[k] = db[k] + dz;
-            se += sum_of(e[k]);
-            sx += sum_of(e[k] * x[k]);
-          }
-        }
-        se = group_sum<LG>(se) * inv;
-        sx = group_sum<LG>(sx) * inv;
-        if (ok) {
-#pragma unroll
-          for (int k = 0; k < CPL; ++k)
-            if (in[k])
-              st_vec<T, VE>(op + (i + u) * os + ch[k],
-                            fma(x[k], all<VE>(-sx), e[k] + all<VE>(-se)) * all<VE>(rs[u]), p.whole);
-        }
-      }
-    }
-  }
-  if constexpr (BWD) {  // the CTA's sums over its samples, in their order
-    extern __shared__ float sh[];  // [spc][M][gpc * LG]
-    const int per = gpc * LG, q = threadIdx.x % per;
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      __syncthreads();
-      if (sr < spc) {
-#pragma unroll
-        for (int i = 0; i < M; ++i) sh[((size_t)sr * M + i) * per + q] = (which ? db[i / VE] : dw[i / VE]).v[i % VE];
-      }
-      __syncthreads();
-      if (sr == 0 && live) {
-#pragma unroll
-        for (int k = 0; k < CPL; ++k)
-          if (in[k])
-#pragma unroll
-            for (int i = 0; i < VE; ++i) {
-              float v = 0.f;
-              for (int r = 0; r < spc; ++r) v += sh[((size_t)r * M + k * VE + i) * per + q];
-              p.part[((int64_t)blockIdx.x * 2 + which) * p.C + ch[k] + i] = v;
-            }
-      }
-    }
-  }
-}
 
 // ---------------------------------------------------------------- several positions per sample
 // CTA (sample and slice, channel block): thread = (row lane, chunk of VE channels).
@@ -346,7 +57,7 @@ __device__ __forceinline__ void gn_groups(const float* mean, const float* rstd, 
 }
 
 // The slice's outputs; mean and rstd indexed by the block's groups.
-template <typename T, int VE>
+template <typename T, int VE, bool WHOLE>
 __device__ __forceinline__ void gn_apply_rows(const GnParams& p, const GnPlace& at, const float* gmean, const float* grstd) {
   const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
   if (rl >= RL) return;
@@ -365,21 +76,21 @@ __device__ __forceinline__ void gn_apply_rows(const GnParams& p, const GnPlace& 
     for (; r + (U - 1) * RL < at.rows; r += U * RL) {
       Raw<T, VE> raw[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = ld_raw<T, VE>(x + u * xh, p.whole);
+      for (int u = 0; u < U; ++u) raw[u] = ld_raw<T, VE, WHOLE>(x + u * xh);
       x += U * xh;
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        st_vec<T, VE>(y + u * yh, gn_act<T>(fma(unpack<T, VE>(raw[u]) + neg, sc, b), p.silu), p.whole);
+        st_vec<T, VE, WHOLE>(y + u * yh, gn_act<T>(fma(unpack<T, VE>(raw[u]) + neg, sc, b), p.silu));
       y += U * yh;
     }
     for (; r < at.rows; r += RL, x += xh, y += yh)
-      st_vec<T, VE>(y, gn_act<T>(fma(unpack<T, VE>(ld_raw<T, VE>(x, p.whole)) + neg, sc, b), p.silu), p.whole);
+      st_vec<T, VE, WHOLE>(y, gn_act<T>(fma(unpack<T, VE>(ld_raw<T, VE, WHOLE>(x)) + neg, sc, b), p.silu));
   }
 }
 
 // (mean, M2) of each slice and group; ONE (a single slice): mean and rstd, and the outputs too,
 // the second reading from L1 or L2.
-template <typename T, int VE, bool ONE>
+template <typename T, int VE, bool WHOLE, bool ONE>
 __global__ void __launch_bounds__(kGnThreads, 3) gn_stats_kernel(const __grid_constant__ GnParams p) {
   extern __shared__ float sh[];  // [2][row lanes][cw]: mean, M2; ONE: [2][groups]
   const GnPlace at(p);
@@ -396,7 +107,7 @@ __global__ void __launch_bounds__(kGnThreads, 3) gn_stats_kernel(const __grid_co
       Raw<T, VE> raw[U];
       auto load = [&]() {
 #pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = ld_raw<T, VE>(x + u * hop, p.whole);
+        for (int u = 0; u < U; ++u) raw[u] = ld_raw<T, VE, WHOLE>(x + u * hop);
         x += U * hop;
       };
       bool more = r + (U - 1) * RL < at.rows;
@@ -424,7 +135,7 @@ __global__ void __launch_bounds__(kGnThreads, 3) gn_stats_kernel(const __grid_co
       }
       float cnt = blocks * U;
       for (; r < at.rows; r += RL) {
-        const Fv<VE> d = fma(mean, all<VE>(-1.f), unpack<T, VE>(ld_raw<T, VE>(x, p.whole)));
+        const Fv<VE> d = fma(mean, all<VE>(-1.f), unpack<T, VE>(ld_raw<T, VE, WHOLE>(x)));
         x += hop;
         const float f = rcp(cnt + 1.f);
         mean = fma(d, all<VE>(f), mean);
@@ -489,7 +200,7 @@ __global__ void __launch_bounds__(kGnThreads, 3) gn_stats_kernel(const __grid_co
   }
   if constexpr (ONE) {
     __syncthreads();
-    gn_apply_rows<T, VE>(p, at, gmean, gmean + ng);
+    gn_apply_rows<T, VE, WHOLE>(p, at, gmean, gmean + ng);
   }
 }
 
@@ -520,15 +231,15 @@ __global__ void __launch_bounds__(256) gn_join_kernel(const __grid_constant__ Gn
   }
 }
 
-template <typename T, int VE>
+template <typename T, int VE, bool WHOLE>
 __global__ void __launch_bounds__(kGnThreads, 3) gn_apply_kernel(const __grid_constant__ GnParams p) {
   const GnPlace at(p);
   const int64_t g0 = (int64_t)at.n * p.G + at.c_lo / p.Cg;
-  gn_apply_rows<T, VE>(p, at, p.mean + g0, p.rstd + g0);
+  gn_apply_rows<T, VE, WHOLE>(p, at, p.mean + g0, p.rstd + g0);
 }
 
 // The slice's dx; the means of e xh and of e indexed by the block's groups.
-template <typename T, int VE>
+template <typename T, int VE, bool WHOLE>
 __device__ __forceinline__ void gn_dx_rows(const GnParams& p, const GnPlace& at, const float* mx, const float* me) {
   const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
   if (rl >= RL) return;
@@ -548,7 +259,7 @@ __device__ __forceinline__ void gn_dx_rows(const GnParams& p, const GnPlace& at,
     auto one = [&](const Raw<T, VE>& xr, const Raw<T, VE>& dr, T* to) {
       const Fv<VE> v = (unpack<T, VE>(xr) + neg) * rstd;
       const Fv<VE> dz = gn_dact<T>(unpack<T, VE>(dr), fma(v, w, b), p.silu);
-      st_vec<T, VE>(to, fma(v, sx, fma(dz, w, se)) * rstd, p.whole);
+      st_vec<T, VE, WHOLE>(to, fma(v, sx, fma(dz, w, se)) * rstd);
     };
     constexpr int U = 4;
     int r = rl;
@@ -556,8 +267,8 @@ __device__ __forceinline__ void gn_dx_rows(const GnParams& p, const GnPlace& at,
       Raw<T, VE> xr[U], dr[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        xr[u] = ld_raw<T, VE>(x + u * xh, p.whole);
-        dr[u] = ld_raw<T, VE>(dy + u * dh, p.whole);
+        xr[u] = ld_raw<T, VE, WHOLE>(x + u * xh);
+        dr[u] = ld_raw<T, VE, WHOLE>(dy + u * dh);
       }
       x += U * xh, dy += U * dh;
 #pragma unroll
@@ -565,12 +276,12 @@ __device__ __forceinline__ void gn_dx_rows(const GnParams& p, const GnPlace& at,
       dx += U * gh;
     }
     for (; r < at.rows; r += RL, x += xh, dy += dh, dx += gh)
-      one(ld_raw<T, VE>(x, p.whole), ld_raw<T, VE>(dy, p.whole), dx);
+      one(ld_raw<T, VE, WHOLE>(x), ld_raw<T, VE, WHOLE>(dy), dx);
   }
 }
 
 // The gradient's sums per channel of each slice: part[n * slices + slice][2][C]; ONE: dx too.
-template <typename T, int VE, bool ONE>
+template <typename T, int VE, bool WHOLE, bool ONE>
 __global__ void __launch_bounds__(kGnThreads, 2) gn_sums_kernel(const __grid_constant__ GnParams p) {
   extern __shared__ float sh[];  // [2][row lanes][cw]; ONE: [2][cw], [2][groups]
   const GnPlace at(p);
@@ -598,14 +309,14 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_sums_kernel(const __grid_con
         Raw<T, VE> xr[U], dr[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          xr[u] = ld_raw<T, VE>(x + u * xh, p.whole);
-          dr[u] = ld_raw<T, VE>(dy + u * dh, p.whole);
+          xr[u] = ld_raw<T, VE, WHOLE>(x + u * xh);
+          dr[u] = ld_raw<T, VE, WHOLE>(dy + u * dh);
         }
         x += U * xh, dy += U * dh;
 #pragma unroll
         for (int u = 0; u < U; ++u) one(xr[u], dr[u]);
       }
-      for (; r < at.rows; r += RL, x += xh, dy += dh) one(ld_raw<T, VE>(x, p.whole), ld_raw<T, VE>(dy, p.whole));
+      for (; r < at.rows; r += RL, x += xh, dy += dh) one(ld_raw<T, VE, WHOLE>(x), ld_raw<T, VE, WHOLE>(dy));
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         sh[rl * at.cw + k * VE + i] = a0.v[i];
@@ -634,7 +345,7 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_sums_kernel(const __grid_con
       if (lane == 0) gm[i] = v * inv;
     }
     __syncthreads();
-    gn_dx_rows<T, VE>(p, at, gm, gm + ng);
+    gn_dx_rows<T, VE, WHOLE>(p, at, gm, gm + ng);
   }
 }
 
@@ -676,11 +387,11 @@ __global__ void __launch_bounds__(256) gn_mid_kernel(const __grid_constant__ GnP
   }
 }
 
-template <typename T, int VE>
+template <typename T, int VE, bool WHOLE>
 __global__ void __launch_bounds__(kGnThreads, 2) gn_dx_kernel(const __grid_constant__ GnParams p) {
   const GnPlace at(p);
   const int64_t g0 = (int64_t)at.n * 2 * p.G + at.c_lo / p.Cg;
-  gn_dx_rows<T, VE>(p, at, p.gmean + g0, p.gmean + g0 + p.G);
+  gn_dx_rows<T, VE, WHOLE>(p, at, p.gmean + g0, p.gmean + g0 + p.G);
 }
 
 // ---------------------------------------------------------------- groups of more than 4096 channels
@@ -796,8 +507,6 @@ __global__ void __launch_bounds__(256) gn_param_grad_kernel(const float* part, i
 // ---------------------------------------------------------------- plans
 constexpr int kGnMostCg = 4096;  // channels of a group in the kernels above
 
-// One position: loads of ve channels, LG lanes and CPL loads per group.
-struct GnRowPlan { bool ok; int lg, cpl, gpc, spc, gy; int64_t ctas; };
 static GnRowPlan gn_row_plan(int64_t N, int64_t S, int64_t G, int64_t Cg, int ve, bool bwd = false) {
   GnRowPlan r{};
   const int64_t chunks = Cg / ve;
@@ -870,46 +579,9 @@ static int gn_whole(int es, int ve, const void* const* ptr, const int64_t* strid
   return ok;
 }
 
-template <typename T, int VE, int CPL, bool BWD, int LG>
-static void gn_row_launch(const GnParams& p, const GnRowPlan& r, cudaStream_t s) {
-  constexpr int M = VE * CPL, U = M <= 8 ? (BWD ? 2 : 4) : M <= 16 ? 2 : 1;
-  const int threads = (r.gpc * r.lg * r.spc + 31) / 32 * 32;
-  const size_t smem = BWD ? (size_t)r.spc * r.gpc * r.lg * M * 4 : 0;
-  const dim3 grid((unsigned)r.ctas, (unsigned)r.gy);
-  if (LG * M == p.Cg) gn_row_kernel<T, VE, CPL, U, BWD, LG, true><<<grid, threads, smem, s>>>(p, r.gpc, r.spc);
-  else gn_row_kernel<T, VE, CPL, U, BWD, LG, false><<<grid, threads, smem, s>>>(p, r.gpc, r.spc);
-}
-template <typename T, int VE, int CPL, bool BWD>
-static void gn_row_lanes(const GnParams& p, const GnRowPlan& r, cudaStream_t s) {
-  if constexpr (CPL > 1) {
-    gn_row_launch<T, VE, CPL, BWD, 32>(p, r, s);
-  } else {
-    switch (r.lg) {
-      case 1: return gn_row_launch<T, VE, 1, BWD, 1>(p, r, s);
-      case 2: return gn_row_launch<T, VE, 1, BWD, 2>(p, r, s);
-      case 4: return gn_row_launch<T, VE, 1, BWD, 4>(p, r, s);
-      case 8: return gn_row_launch<T, VE, 1, BWD, 8>(p, r, s);
-      case 16: return gn_row_launch<T, VE, 1, BWD, 16>(p, r, s);
-      default: return gn_row_launch<T, VE, 1, BWD, 32>(p, r, s);
-    }
-  }
-}
-template <typename T, int VE, bool BWD>
-static void gn_row_loads(const GnParams& p, const GnRowPlan& r, cudaStream_t s) {
-  if (r.cpl == 1) return gn_row_lanes<T, VE, 1, BWD>(p, r, s);
-  if (r.cpl == 2) return gn_row_lanes<T, VE, 2, BWD>(p, r, s);
-  if (r.cpl == 4) return gn_row_lanes<T, VE, 4, BWD>(p, r, s);
-  if constexpr (VE <= 4) return gn_row_lanes<T, VE, 8, BWD>(p, r, s);
-}
-template <typename T, bool BWD> static void gn_rows(const GnParams& p, const GnRowPlan& r, int ve, cudaStream_t s) {
-  if (ve == 1) return gn_row_loads<T, 1, BWD>(p, r, s);
-  if (ve == 2) return gn_row_loads<T, 2, BWD>(p, r, s);
-  if (ve == 4) return gn_row_loads<T, 4, BWD>(p, r, s);
-  if constexpr (sizeof(T) == 2) return gn_row_loads<T, 8, BWD>(p, r, s);
-}
-
 enum GnPass { kStats, kApply, kSums, kDx };
-template <typename T, int VE> static void gn_pass(GnPass pass, const GnParams& p, const GnPlan& r, cudaStream_t s) {
+template <typename T, int VE, bool WHOLE>
+static void gn_pass(GnPass pass, const GnParams& p, const GnPlan& r, cudaStream_t s) {
   const dim3 grid((unsigned)(r.slices * p.N), (unsigned)r.gz);
   // the row lanes' values of the widest block; a narrower last one has no more of them
   const size_t values = (size_t)2 * gn_lanes((int)(r.cb / VE)) * r.cb > 2 * kGnThreads * VE
@@ -918,16 +590,20 @@ template <typename T, int VE> static void gn_pass(GnPass pass, const GnParams& p
   const size_t smem_sums = (values + (r.one ? 2 * r.cb + groups : 0)) * 4;
   switch (pass) {
     case kStats:
-      if (r.one) gn_stats_kernel<T, VE, true><<<grid, kGnThreads, smem, s>>>(p);
-      else gn_stats_kernel<T, VE, false><<<grid, kGnThreads, smem, s>>>(p);
+      if (r.one) gn_stats_kernel<T, VE, WHOLE, true><<<grid, kGnThreads, smem, s>>>(p);
+      else gn_stats_kernel<T, VE, WHOLE, false><<<grid, kGnThreads, smem, s>>>(p);
       break;
-    case kApply: launch_dependent(gn_apply_kernel<T, VE>, grid, kGnThreads, 0, s, p); break;
+    case kApply: launch_dependent(gn_apply_kernel<T, VE, WHOLE>, grid, kGnThreads, 0, s, p); break;
     case kSums:
-      if (r.one) gn_sums_kernel<T, VE, true><<<grid, kGnThreads, smem_sums, s>>>(p);
-      else gn_sums_kernel<T, VE, false><<<grid, kGnThreads, smem_sums, s>>>(p);
+      if (r.one) gn_sums_kernel<T, VE, WHOLE, true><<<grid, kGnThreads, smem_sums, s>>>(p);
+      else gn_sums_kernel<T, VE, WHOLE, false><<<grid, kGnThreads, smem_sums, s>>>(p);
       break;
-    case kDx: launch_dependent(gn_dx_kernel<T, VE>, grid, kGnThreads, 0, s, p); break;
+    case kDx: launch_dependent(gn_dx_kernel<T, VE, WHOLE>, grid, kGnThreads, 0, s, p); break;
   }
+}
+template <typename T, int VE> static void gn_pass(GnPass pass, const GnParams& p, const GnPlan& r, cudaStream_t s) {
+  if (VE == 1 || p.whole) gn_pass<T, VE, true>(pass, p, r, s);
+  else gn_pass<T, VE, VE == 1>(pass, p, r, s);
 }
 template <typename T> static void gn_pass(GnPass pass, const GnParams& p, const GnPlan& r, int ve, cudaStream_t s) {
   if (ve == 1) return gn_pass<T, 1>(pass, p, r, s);
@@ -999,8 +675,7 @@ extern "C" int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t
   const GnRowPlan row = gn_row_plan(N, S, G, p.Cg, ve);
   if (row.ok) {
     p.whole = gn_whole(es, ve, ptr, stride, 2);
-    if (dtype == HDC_F32) gn_rows<float, false>(p, row, ve, s);
-    else gn_rows<__nv_bfloat16, false>(p, row, ve, s);
+    gn_rows_fwd(dtype, p, row, ve, s);
     return launch_status("gn_row_kernel");
   }
   const GnPlan plan = gn_plan(N, S, C, G);
@@ -1071,8 +746,7 @@ extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_
     const GnRowPlan row = gn_row_plan(N, S, G, p.Cg, ve, true);
     if (row.ok) {
       p.whole = gn_whole(es, ve, ptr, stride, 3);
-      if (dtype == HDC_F32) gn_rows<float, true>(p, row, ve, s);
-      else gn_rows<__nv_bfloat16, true>(p, row, ve, s);
+      gn_rows_bwd(dtype, p, row, ve, s);
       if (int e = launch_status("gn_row_kernel")) return e;
       parts = row.ctas;
     } else {
