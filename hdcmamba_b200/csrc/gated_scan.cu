@@ -134,15 +134,14 @@ template <typename T> constexpr uint32_t kNoStep = sizeof(T) == 4 ? 0xff800000u 
 //   (weighted least squares on Chebyshev points, weights iterated to equal errors: 2e-7, 3e-7
 //   with fp32 evaluation; the bf16 input itself is 2^-9 off).  e p(e) keeps its relative accuracy
 //   for small e, where log(1 + e) loses it.
-// e: exp(-|x|) as computed on the way (bf16).
-template <typename T, int V> __device__ __forceinline__ Fv<V> gate(const Fv<V>& x, Fv<V>& e) {
+template <typename T, int V> __device__ __forceinline__ Fv<V> gate(const Fv<V>& x) {
   if constexpr (sizeof(T) == 4) {
     Fv<V> d;
 #pragma unroll
     for (int i = 0; i < V; ++i) d.v[i] = softplus_acc(x.v[i]);
     return d;
   } else {
-    Fv<V> m;
+    Fv<V> e, m;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       e.v[i] = ex2(-1.4426950408889634f * fabsf(x.v[i]));
@@ -172,17 +171,19 @@ template <typename T, int V> __device__ __forceinline__ Fv<V> decay(const Fv<V>&
   }
   return a;
 }
-// sigmoid(x); e = exp(-|x|) (bf16)
-template <typename T, int V> __device__ __forceinline__ Fv<V> sigmoid(const Fv<V>& x, const Fv<V>& e) {
+// sigmoid(x) = 1 / (1 + exp(-x)); bf16: 0 where exp(-x) overflows (x < -88)
+template <typename T, int V> __device__ __forceinline__ Fv<V> sigmoid(const Fv<V>& x) {
   Fv<V> s;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if constexpr (sizeof(T) == 4) {
-      s.v[i] = 1.f / (1.f + expf(-x.v[i]));
-    } else {
-      const float r = rcp(1.f + e.v[i]);
-      s.v[i] = x.v[i] < 0.f ? e.v[i] * r : r;
-    }
+    for (int i = 0; i < V; ++i) s.v[i] = 1.f / (1.f + expf(-x.v[i]));
+  } else {
+    s = x * all<V>(-1.4426950408889634f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s.v[i] = ex2(s.v[i]);
+    s = s + all<V>(1.f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s.v[i] = rcp(s.v[i]);
   }
   return s;
 }
@@ -320,6 +321,19 @@ template <bool RESET, int V> __device__ __forceinline__ Map<V> take(const uint64
   return m;
 }
 
+// The composition of the 8 warps' maps, and its publication by one warp.
+template <bool RESET, bool REV, int V> __device__ __forceinline__ Map<V> tile_map_of(const char* maps, int stride, int lane) {
+  Map<V> m = ld_map<V>(maps + (REV ? kWarps - 1 : 0) * stride, lane);
+#pragma unroll
+  for (int k = 1; k < kWarps; ++k) m = then<RESET>(m, ld_map<V>(maps + (REV ? kWarps - 1 - k : k) * stride, lane));
+  return m;
+}
+template <bool RESET, bool REV, int V>
+__device__ __forceinline__ void publish_tile(const ScanParams& p, int g, int q, const char* maps, int stride, int lane) {
+  if (q + 1 < p.NT)
+    publish<V>(p.ent + ((int64_t)g * p.nent + q) * 32 * V, lane, tile_map_of<RESET, REV, V>(maps, stride, lane));
+}
+
 // The exchange between tiles, the same for both directions.  q: the tile's index in the order
 // of the scan.  maps: the 8 warps' maps in shared memory, warp w's at maps + w * stride, composed
 // in the order of the scan (REV: from the last warp to the first).  pre: this warp's slot at
@@ -336,13 +350,7 @@ __device__ __forceinline__ Fv<V> enter_tile(const ScanParams& p, int g, int q, c
   uint64_t* links = spans + (int64_t)((p.NT + kSpan - 1) / kSpan) * CW;
   const int in_span = q % kSpan, span = q / kSpan, link = span / kSpan, in_link = span % kSpan;
   const bool more = q + 1 < p.NT;
-  auto tile_map = [&]() {
-    Map<V> m = ld_map<V>(maps + (REV ? kWarps - 1 : 0) * stride, lane);
-#pragma unroll
-    for (int k = 1; k < kWarps; ++k) m = then<RESET>(m, ld_map<V>(maps + (REV ? kWarps - 1 - k : k) * stride, lane));
-    return m;
-  };
-  if (warp == 0 && more) publish<V>(ent + (int64_t)q * CW, lane, tile_map());
+  auto tile_map = [&]() { return tile_map_of<RESET, REV, V>(maps, stride, lane); };
   // warps 0..3 compose the whole spans of the link that the tile is in, warps 4..7 the tiles of
   // the span that it is in, four entries each
   const int from = warp % 4 * 4, n = min(4, (warp < 4 ? in_link : in_span) - from);
@@ -484,14 +492,17 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas<W>) gated_scan_fwd_kerne
   __syncthreads();
   bool first = true;
   for (int s = 0; t.x >= 0; s ^= 1) {
-    // The next ticket, early enough to stage its tile below.  The first time only after the loads:
-    // a CTA that starts early would else take two neighbouring tiles, and the tiles after
-    // the second one would wait until it is done with the first.
-    if (first) cp_wait_all();
-    first = false;
-    if (threadIdx.x == 0) {
-      id = next_tile(p, id);
-      s_next[s ^ 1] = tile_of(p, id, CW);
+    // The tile after this one is known by now (its ticket was taken during the tile before), except
+    // the first time, and then it is asked for only after the loads: a CTA that starts early
+    // would else take two neighbouring tiles, and the tiles after the second one would wait until
+    // it is done with the first.
+    if (first) {
+      cp_wait_all();
+      if (threadIdx.x == 0) {
+        id = next_tile(p, id);
+        s_next[1] = tile_of(p, id, CW);
+      }
+      first = false;
     }
     char* buf = raw + s * kWarps * kRegion;
     char* mine = buf + warp * kRegion;
@@ -515,8 +526,7 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas<W>) gated_scan_fwd_kerne
     for (int r = 0; r < kRows; ++r) {
       const Fv<V> dt = ld_words<T, W>(w + r * RB), x = ld_words<T, W>(w + (kRows + r) * RB);
       const Fv<V> b = ld_words<T, W>(w + (2 * kRows + r) * RB);
-      Fv<V> e;
-      const Fv<V> d = gate<T>(dt, e);
+      const Fv<V> d = gate<T>(dt);
       a[r] = decay<T>(d, A, A2);
       u[r] = d * (b * x);
       if (RESET && ((cut >> r) & 1)) {
@@ -532,6 +542,8 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas<W>) gated_scan_fwd_kerne
     __syncthreads();
 
     const Tile nt = s_next[s ^ 1];
+    if (threadIdx.x == 0) id = next_tile(p, id);
+    if (p.ticket && warp == 0) publish_tile<RESET, false, V>(p, t.y, t.x, buf, kRegion, lane);
     if (nt.x >= 0) stage(nt, s ^ 1);
 
     // the state entering the tile, then the warp's steps
@@ -560,6 +572,7 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas<W>) gated_scan_fwd_kerne
       }
     }
     if (p.h_last && t.x == p.NT - 1 && warp == kWarps - 1) st_state<V>(p.h_last + at, cl, nc, h);
+    if (threadIdx.x == 0) s_next[s] = tile_of(p, id, CW);
     t = nt;
   }
 }
@@ -617,10 +630,12 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas<W>) gated_scan_bwd_kerne
   if (t.x >= 0) stage(t, 0);
   __syncthreads();
   for (int s = 0; t.x >= 0; s ^= 1) {
-    if (before.x < 0) cp_wait_all();  // the first time the next ticket waits for the loads, as in the forward
-    if (threadIdx.x == 0) {
-      id = next_tile(p, id);
-      s_next[s ^ 1] = tile_of(p, id, CW);
+    if (before.x < 0) {  // the first time, as in the forward
+      cp_wait_all();
+      if (threadIdx.x == 0) {
+        id = next_tile(p, id);
+        s_next[1] = tile_of(p, id, CW);
+      }
     }
     char* mine = raw + (s * kWarps + warp) * kRegion;
     const int tt = p.NT - 1 - t.x, t0 = tt * kStateRows + warp * kRows, nv = p.L - t0, nc = p.ds - t.w;
@@ -645,28 +660,28 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas<W>) gated_scan_bwd_kerne
     for (int r = 0; r < kRows; ++r) {
       const Fv<V> dt = ld_words<T, W>(w + r * RB), x = ld_words<T, W>(w + (kRows + r) * RB);
       const Fv<V> b = ld_words<T, W>(w + (2 * kRows + r) * RB);
-      Fv<V> e;
-      d[r] = gate<T>(dt, e);
+      d[r] = gate<T>(dt);
       a[r] = decay<T>(d[r], A, A2);
       const Fv<V> u = d[r] * (b * x);
+      // the backward map from zero: c = sum of dy_r times the decays up to step r, until a reset
       if (RESET && ((cut >> r) & 1)) {
         m.H = u;
         m.P = all<V>(-1.f);
       } else {
         m.H = fma(a[r], m.H, u);
-        if (!RESET || !(m.P.v[0] < 0.f)) m.P = m.P * a[r];
+        if (!RESET || !(m.P.v[0] < 0.f)) {
+          m.P = m.P * a[r];
+          c = fma(m.P, ld_words<T, W>(w + (3 * kRows + r) * RB), c);
+        }
       }
-    }
-#pragma unroll
-    for (int r = kRows - 1; r >= 0; --r) {
-      c = a[r] * (ld_words<T, W>(w + (3 * kRows + r) * RB) + c);
-      if (RESET && ((cut >> r) & 1)) c = all<V>(0.f);
     }
     st_map<V>(fmap + warp * kMapBytes<V>, lane, m);
     st_map<V>(bmap + warp * kMapBytes<V>, lane, {m.P, c});
     __syncthreads();
 
     const Tile nt = s_next[s ^ 1];
+    if (threadIdx.x == 0) id = next_tile(p, id);
+    if (p.ticket && warp == 0) publish_tile<RESET, true, V>(p, t.y, t.x, bmap, kMapBytes<V>, lane);
     if (nt.x >= 0) stage(nt, s ^ 1);
     if (warp == 2 && before.x >= 0) write_dA(before);
 
@@ -695,13 +710,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas<W>) gated_scan_bwd_kerne
       const Fv<V> g = ld_words<T, W>(w + (3 * kRows + r) * RB) + c;
       c = a[r] * g;
       if (RESET && ((cut >> r) & 1)) c = all<V>(0.f);
-      Fv<V> e;
-      if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) e.v[i] = ex2(-1.4426950408889634f * fabsf(dt.v[i]));
-      }
       const Fv<V> gd = g * d[r], sr = g * q[r];
-      const Fv<V> ddt = fma(sr, A, g * (b * x)) * sigmoid<T>(dt, e);
+      const Fv<V> ddt = fma(sr, A, g * (b * x)) * sigmoid<T>(dt);
       if (whole) {
         sum = fma(sr, d[r], sum);
         T* o = out + r * p.gst + cl;
@@ -718,6 +728,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas<W>) gated_scan_bwd_kerne
     }
     if (p.dh0 && tt == 0 && warp == 0) st_state<V>(p.dh0 + at, cl, nc, c);
     st_f<V>(sums, warp, lane, sum);
+    if (threadIdx.x == 0) s_next[s] = tile_of(p, id, CW);
     __syncthreads();  // the maps and slots are read, the sums written
     before = t;
     t = nt;

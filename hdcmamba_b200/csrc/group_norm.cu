@@ -28,6 +28,7 @@ namespace hdc {
 // ---------------------------------------------------------------- several positions per sample
 // CTA (sample and slice, channel block): thread = (row lane, chunk of VE channels).
 constexpr int kGnThreads = 256;
+constexpr int kGnFwdCtas = 3, kGnBwdCtas = 2;  // resident CTAs per SM of the two-pass kernels
 // row lanes of a CTA: threads per chunk of channels (one when a thread has several chunks)
 __host__ __device__ inline int gn_lanes(int nchunk) { return nchunk < kGnThreads ? kGnThreads / nchunk : 1; }
 
@@ -91,7 +92,7 @@ __device__ __forceinline__ void gn_apply_rows(const GnParams& p, const GnPlace& 
 // (mean, M2) of each slice and group; ONE (a single slice): mean and rstd, and the outputs too,
 // the second reading from L1 or L2.
 template <typename T, int VE, bool WHOLE, bool ONE>
-__global__ void __launch_bounds__(kGnThreads, 3) gn_stats_kernel(const __grid_constant__ GnParams p) {
+__global__ void __launch_bounds__(kGnThreads, kGnFwdCtas) gn_stats_kernel(const __grid_constant__ GnParams p) {
   extern __shared__ float sh[];  // [2][row lanes][cw]: mean, M2; ONE: [2][groups]
   const GnPlace at(p);
   const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(256) gn_join_kernel(const __grid_constant__ Gn
 }
 
 template <typename T, int VE, bool WHOLE>
-__global__ void __launch_bounds__(kGnThreads, 3) gn_apply_kernel(const __grid_constant__ GnParams p) {
+__global__ void __launch_bounds__(kGnThreads, kGnFwdCtas) gn_apply_kernel(const __grid_constant__ GnParams p) {
   const GnPlace at(p);
   const int64_t g0 = (int64_t)at.n * p.G + at.c_lo / p.Cg;
   gn_apply_rows<T, VE, WHOLE>(p, at, p.mean + g0, p.rstd + g0);
@@ -282,7 +283,7 @@ __device__ __forceinline__ void gn_dx_rows(const GnParams& p, const GnPlace& at,
 
 // The gradient's sums per channel of each slice: part[n * slices + slice][2][C]; ONE: dx too.
 template <typename T, int VE, bool WHOLE, bool ONE>
-__global__ void __launch_bounds__(kGnThreads, 2) gn_sums_kernel(const __grid_constant__ GnParams p) {
+__global__ void __launch_bounds__(kGnThreads, kGnBwdCtas) gn_sums_kernel(const __grid_constant__ GnParams p) {
   extern __shared__ float sh[];  // [2][row lanes][cw]; ONE: [2][cw], [2][groups]
   const GnPlace at(p);
   const int nchunk = at.cw / VE, RL = gn_lanes(nchunk), per = min(nchunk, kGnThreads), rl = threadIdx.x / per;
@@ -388,7 +389,7 @@ __global__ void __launch_bounds__(256) gn_mid_kernel(const __grid_constant__ GnP
 }
 
 template <typename T, int VE, bool WHOLE>
-__global__ void __launch_bounds__(kGnThreads, 2) gn_dx_kernel(const __grid_constant__ GnParams p) {
+__global__ void __launch_bounds__(kGnThreads, kGnBwdCtas) gn_dx_kernel(const __grid_constant__ GnParams p) {
   const GnPlace at(p);
   const int64_t g0 = (int64_t)at.n * 2 * p.G + at.c_lo / p.Cg;
   gn_dx_rows<T, VE, WHOLE>(p, at, p.gmean + g0, p.gmean + g0 + p.G);
@@ -536,14 +537,19 @@ static int64_t gn_row_parts(int64_t N, int64_t G, int64_t Cg) {
 }
 // Several positions.  One pass when a sample's block of channels is small enough to be read again
 // from L1 (64 KB), the blocks then about 64 channels wide for more CTAs; else slices of each
-// sample, 32 positions or more, in one wave of three CTAs per SM: a CTA's fixed cost (joining its
+// sample, 32 positions or more, in one wave of the resident CTAs: a CTA's fixed cost (joining its
 // threads' sums) is that of some 30 rows.
 struct GnPlan { int64_t slices, rows, cb, gz; bool one; };
-static int64_t gn_block(int64_t C, int64_t Cg, int64_t want) {  // whole groups, about `want` channels
-  if (C <= want) return C;
-  return Cg >= want ? Cg : want / Cg * Cg;
+// Whole groups, about `want` channels, a multiple of the channels that a load of the full row
+// could take (so that blocks do not narrow the loads).
+static int64_t gn_block(int64_t C, int64_t Cg, int64_t want) {
+  int64_t step = Cg;
+  for (int ve = 2; ve <= 8 && C % ve == 0; ve *= 2)
+    while (step % ve != 0) step *= 2;
+  if (C <= want || C <= step) return C;
+  return step >= want ? step : want / step * step;
 }
-static GnPlan gn_plan(int64_t N, int64_t S, int64_t C, int64_t G) {
+static GnPlan gn_plan(int64_t N, int64_t S, int64_t C, int64_t G, bool bwd) {
   GnPlan r{};
   const int64_t Cg = C / G;
   r.cb = gn_block(C, Cg, 64);
@@ -557,7 +563,7 @@ static GnPlan gn_plan(int64_t N, int64_t S, int64_t C, int64_t G) {
   r.rows = S;
   r.slices = 1;
   if (!r.one) {
-    const int64_t want = (148 * 3) / (N * r.gz) > 0 ? (148 * 3) / (N * r.gz) : 1;
+    const int64_t ctas = 148 * (bwd ? kGnBwdCtas : kGnFwdCtas), want = ctas >= N * r.gz ? ctas / (N * r.gz) : 1;
     r.rows = (S + want - 1) / want;
     if (r.rows < 32) r.rows = S < 32 ? S : 32;
     r.slices = (S + r.rows - 1) / r.rows;
@@ -639,9 +645,9 @@ extern "C" size_t hdc_group_norm_workspace_bytes(int64_t N, int64_t S, int64_t C
   if (N < 1 || S < 1 || C < 1 || G < 1 || C % G != 0 || C / G > kGnMostCg) return 0;
   // one position takes no second pass with wider loads if it takes none with single channels
   if (gn_row_plan(N, S, G, C / G, 1).ok) return 0;
-  if (gn_plan(N, S, C, G).one) return 0;
+  if (gn_plan(N, S, C, G, false).one) return 0;
   // the slices' statistics, then the samples' mean and rstd when the caller does not want them
-  return (size_t)N * G * 8 * (gn_plan(N, S, C, G).slices + 1);
+  return (size_t)N * G * 8 * (gn_plan(N, S, C, G, false).slices + 1);
 }
 
 extern "C" int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t x_sn, int64_t x_ss, const void* weight,
@@ -678,7 +684,7 @@ extern "C" int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t
     gn_rows_fwd(dtype, p, row, ve, s);
     return launch_status("gn_row_kernel");
   }
-  const GnPlan plan = gn_plan(N, S, C, G);
+  const GnPlan plan = gn_plan(N, S, C, G, false);
   p.slices = (int)plan.slices; p.rows = (int)plan.rows; p.cb = (int)plan.cb;
   ve = gn_width(es, plan.cb | C);
   p.whole = gn_whole(es, ve, ptr, stride, 2);
@@ -701,7 +707,7 @@ extern "C" size_t hdc_group_norm_bwd_workspace_bytes(int64_t N, int64_t S, int64
   const size_t one = S == 1 ? (size_t)gn_row_parts(N, G, C / G) * 2 * C * 4 : 0;
   if (gn_row_plan(N, S, G, C / G, 1).ok) return one;
   // the slices' sums, the samples' sums, the groups' means
-  const size_t two = (size_t)N * 2 * 4 * ((gn_plan(N, S, C, G).slices + 1) * C + G);
+  const size_t two = (size_t)N * 2 * 4 * ((gn_plan(N, S, C, G, true).slices + 1) * C + G);
   return one > two ? one : two;
 }
 // the middle step's channels per CTA: whole groups, some 64 channels
@@ -750,7 +756,7 @@ extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_
       if (int e = launch_status("gn_row_kernel")) return e;
       parts = row.ctas;
     } else {
-      const GnPlan plan = gn_plan(N, S, C, G);
+      const GnPlan plan = gn_plan(N, S, C, G, true);
       p.slices = (int)plan.slices; p.rows = (int)plan.rows; p.cb = (int)plan.cb;
       ve = gn_width(es, plan.cb | C);
       p.whole = gn_whole(es, ve, ptr, stride, 3);

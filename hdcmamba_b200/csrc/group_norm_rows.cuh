@@ -58,21 +58,35 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
   const int64_t xs = step * p.xsn, ds = step * p.dsn, os = step * (BWD ? p.gsn : p.ysn), gs = step * p.G;
   const bool stats = !BWD && l == 0 && mp;
 
+  struct Turn {
+    Raw<T, VE> x[CPL], dy[BWD ? CPL : 1];
+    float mu, rs;
+  };
+  auto load = [&](int i) {
+    const int64_t at = i < whole_turns ? i : 0;
+    Turn t;
+#pragma unroll
+    for (int k = 0; k < CPL; ++k) {
+      t.x[k] = ld_raw<T, VE, WHOLE>(xp + at * xs + ch[k]);
+      if constexpr (BWD) t.dy[k] = ld_raw<T, VE, WHOLE>(dp + at * ds + ch[k]);
+    }
+    if constexpr (BWD) {
+      t.mu = __ldg(mp + at * gs);
+      t.rs = __ldg(rp + at * gs);
+    }
+    return t;
+  };
+  // the loads of the next U turns are in flight during U turns
+  Turn next[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) next[u] = load(u);
   for (int i = 0; i < turns; i += U) {
-    Raw<T, VE> xr[U][CPL], dr[BWD ? U : 1][CPL];
-    float mu[U], rs[U];
+    Turn now[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = i + u < whole_turns ? i + u : 0;
+    for (int u = 0; u < U; ++u) now[u] = next[u];
+    if (i + U < turns) {
 #pragma unroll
-      for (int k = 0; k < CPL; ++k) {
-        xr[u][k] = ld_raw<T, VE, WHOLE>(xp + at * xs + ch[k]);
-        if constexpr (BWD) dr[u][k] = ld_raw<T, VE, WHOLE>(dp + at * ds + ch[k]);
-      }
-      if constexpr (BWD) {
-        mu[u] = __ldg(mp + at * gs);
-        rs[u] = __ldg(rp + at * gs);
-      }
+      for (int u = 0; u < U; ++u) next[u] = load(i + U + u);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -82,7 +96,7 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
         float s = 0.f;
 #pragma unroll
         for (int k = 0; k < CPL; ++k) {
-          x[k] = unpack<T, VE>(xr[u][k]);
+          x[k] = unpack<T, VE>(now[u].x[k]);
           s += in[k] ? sum_of(x[k]) : 0.f;
         }
         const float mean = over(group_sum<LG>(s, lg), (float)p.Cg, inv);
@@ -108,8 +122,8 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
         float se = 0.f, sx = 0.f;
 #pragma unroll
         for (int k = 0; k < CPL; ++k) {
-          x[k] = (unpack<T, VE>(xr[u][k]) + all<VE>(-mu[u])) * all<VE>(rs[u]);
-          const Fv<VE> dz = gn_dact<T>(unpack<T, VE>(dr[u][k]), fma(x[k], w[k], b[k]), p.silu);
+          x[k] = (unpack<T, VE>(now[u].x[k]) + all<VE>(-now[u].mu)) * all<VE>(now[u].rs);
+          const Fv<VE> dz = gn_dact<T>(unpack<T, VE>(now[u].dy[k]), fma(x[k], w[k], b[k]), p.silu);
           e[k] = dz * w[k];
           if (ok && in[k]) {
             dw[k] = fma(dz, x[k], dw[k]);
@@ -125,7 +139,7 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
           for (int k = 0; k < CPL; ++k)
             if (in[k])
               st_vec<T, VE, WHOLE>(op + (i + u) * os + ch[k],
-                            fma(x[k], all<VE>(-sx), e[k] + all<VE>(-se)) * all<VE>(rs[u]));
+                            fma(x[k], all<VE>(-sx), e[k] + all<VE>(-se)) * all<VE>(now[u].rs));
         }
       }
     }
@@ -158,7 +172,7 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
 
 template <typename T, int VE, bool WHOLE, int CPL, bool BWD, int LG, bool FULL>
 static void gn_row_launch(const GnParams& p, const GnRowPlan& r, cudaStream_t s) {
-  constexpr int M = VE * CPL, U = M <= 8 ? (BWD ? 2 : 4) : M <= 16 ? 2 : 1;
+  constexpr int M = VE * CPL, U = M <= 8 ? 2 : 1;
   const int threads = (r.gpc * r.lg * r.spc + 31) / 32 * 32;
   const size_t smem = BWD ? (size_t)r.spc * r.gpc * r.lg * M * 4 : 0;
   gn_row_kernel<T, VE, WHOLE, CPL, U, BWD, LG, FULL>
