@@ -30,6 +30,7 @@
 // no published P is, so the word is its own flag.  The next tile is in flight (cp.async)
 // while one is computed.
 // P < 0 marks a map that a reset has cut off from what came before (P is otherwise >= 0).
+#include <atomic>
 #include <type_traits>
 
 #include "tc.cuh"
@@ -62,6 +63,7 @@ struct ScanParams {
   unsigned* ticket;  // NULL: a single tile in time, taken by block index, nothing published
   uint64_t* ent;    // [NG][NT + spans + links][CW] published entries
   int nent;         // entries per group
+  uint64_t div_NG, div_nch;  // 2^64 / d rounded up (0: d = 1)
   int CW;           // channels per tile
   int out_vec;      // the outputs' rows allow whole lanes
 };
@@ -430,12 +432,15 @@ template <typename T, int W, int CB> struct Rows {
   }
 };
 
+// n / d for n, d < 2^32 from m = 2^64 / d rounded up: n m = 2^64 n/d + n e with e < d, n e < 2^64
+__device__ __forceinline__ unsigned quotient(unsigned n, uint64_t m) { return m ? (unsigned)__umul64hi(m, n) : n; }
+
 // A tile as broadcast through shared memory: index in the scan's order, group, batch, first
 // channel; x < 0: none
 using Tile = int4;
 __device__ __forceinline__ Tile tile_of(const ScanParams& p, int64_t id, int CW) {
   if (id >= p.ntiles) return make_int4(-1, 0, 0, 0);
-  const unsigned q = (unsigned)id / (unsigned)p.NG, g = (unsigned)id - q * p.NG, b = g / (unsigned)p.nch;
+  const unsigned q = quotient((unsigned)id, p.div_NG), g = (unsigned)id - q * p.NG, b = quotient(g, p.div_nch);
   return make_int4((int)q, (int)g, (int)b, (int)(g - b * p.nch) * CW);
 }
 __device__ __forceinline__ int64_t next_tile(const ScanParams& p, int64_t last) {
@@ -455,31 +460,33 @@ template <int V> __device__ __forceinline__ void st_state(float* row, int cl, in
     if (cl + i < nc) row[cl + i] = h.v[i];
 }
 
-template <int W> constexpr int kFwdCtas = W == 2 ? 2 : 4;  // resident forward CTAs per SM
+// Resident forward CTAs per SM.  Two words per lane need 128 registers; one needs 64 in bf16 (32768 x
+// 64: 15.1 us with four, 16.7 with three) and more in fp32 (3 x 1537 x 333: 17.0 us with three, 19.3
+// with four).
+template <typename T, int W> constexpr int kFwdCtas = W == 2 ? 2 : sizeof(T) == 4 ? 3 : 4;
 
 template <typename T, int W, bool RESET, int CB>
-__global__ void __launch_bounds__(kWarps * 32, kFwdCtas<W>) gated_scan_fwd_kernel(const __grid_constant__ ScanParams p) {
+__global__ void __launch_bounds__(kWarps * 32, kFwdCtas<T, W>) gated_scan_fwd_kernel(const __grid_constant__ ScanParams p) {
   constexpr int V = kV<T, W>, CW = 32 * V, RB = 128 * W, kRegion = 3 * kRows * RB;
   static_assert(2 * kMapBytes<V> <= kRegion, "maps fit into a warp's staged rows");
   extern __shared__ __align__(128) char raw[];  // [2][warp][dt, x, b][row][RB bytes]
-  __shared__ __align__(16) float s_A[2][CW];
   __shared__ Tile s_next[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int cl = lane * V;  // the lane's first channel of the tile
   const Rows<T, W, CB> rows(lane);
   int64_t id = 0;  // thread 0's
 
-  uint32_t rb = 0;  // the staged tile's reset flag of step `lane` of the warp
+  // of the staged tile: the reset flag of step `lane` of the warp, A_log of the lane's channels
+  uint32_t rb = 0;
+  Fv<V> A_next = all<V>(0.f);
   auto stage = [&](const Tile& t, int s) {
     const int t0 = t.x * kStateRows, nv = p.L - t0 - warp * kRows, nc = p.ds - t.w;
     const T* tile = static_cast<const T*>(p.projs) + t.z * p.psb + t0 * p.pst + t.w;
     rows.template copy<3>(raw + (s * kWarps + warp) * kRegion, tile, warp * kRows, p.pst, p.ds, nv, nc);
     cp_commit();
     if (RESET) rb = lane < min(nv, kRows) ? p.reset[(int64_t)t.z * p.L + t0 + warp * kRows + lane] : 0;
-    if (warp == 3) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) s_A[s][cl + i] = cl + i < nc ? -expf(ld_param(p.A_log, p.a_bf16, t.w + cl + i)) : 0.f;
-    }
+    for (int i = 0; i < V; ++i) A_next.v[i] = cl + i < nc ? ld_param(p.A_log, p.a_bf16, t.w + cl + i) : 0.f;
   };
 
   if (threadIdx.x == 0) {
@@ -489,7 +496,6 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas<W>) gated_scan_fwd_kerne
   __syncthreads();
   Tile t = s_next[0];
   if (t.x >= 0) stage(t, 0);
-  __syncthreads();
   bool first = true;
   for (int s = 0; t.x >= 0; s ^= 1) {
     // The tile after this one is known by now (its ticket was taken during the tile before), except
@@ -508,7 +514,9 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas<W>) gated_scan_fwd_kerne
     char* mine = buf + warp * kRegion;
     const int t0 = t.x * kStateRows + warp * kRows, nv = p.L - t0, nc = p.ds - t.w;
     const uint32_t cut = RESET ? __ballot_sync(0xffffffffu, rb != 0) : 0;
-    const Fv<V> A = ld_f<V>(reinterpret_cast<char*>(s_A[s]), 0, lane);
+    Fv<V> A;
+#pragma unroll
+    for (int i = 0; i < V; ++i) A.v[i] = -expf(A_next.v[i]);
     const Fv<V> A2 = A * all<V>(1.4426950408889634f);
     cp_wait_all();
     __syncwarp();
@@ -551,7 +559,6 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas<W>) gated_scan_fwd_kerne
     Fv<V> h = ld_state<V>(p.h0 ? p.h0 + at : nullptr, cl, nc);
     if (p.ticket)
       h = enter_tile<RESET, false, V>(p, t.y, t.x, buf, kRegion, buf + kMapBytes<V>, kRegion, h, warp, lane);
-    else __syncthreads();  // s_A of the next tile
     if (p.states && warp == 0) st_state<V>(p.states + ((int64_t)t.z * p.NT + t.x) * p.ds + t.w, cl, nc, h);
     for (int k = 0; k < warp; ++k) h = apply<RESET>(ld_map<V>(buf + k * kRegion, lane), h);
 
@@ -577,21 +584,20 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas<W>) gated_scan_fwd_kerne
   }
 }
 
-template <int W> constexpr int kBwdCtas = 2;  // resident backward CTAs per SM
+constexpr int kBwdCtas = 2;  // resident backward CTAs per SM (three: 80 registers, spills, 244 us for 184)
 // shared memory of the backward: two staged tiles, the warps' forward maps and backward maps
 // (P shared), the exchange's slots, the warps' sums for dA
 template <int V, int W> constexpr int kBwdMaps = 2 * kWarps * 4 * kRows * 128 * W;
 template <int V, int W> constexpr int kBwdSmem = kBwdMaps<V, W> + kWarps * 32 * V * (16 + 8 + 4);
 
 template <typename T, int W, bool RESET, int CB>
-__global__ void __launch_bounds__(kWarps * 32, kBwdCtas<W>) gated_scan_bwd_kernel(const __grid_constant__ ScanParams p) {
+__global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gated_scan_bwd_kernel(const __grid_constant__ ScanParams p) {
   constexpr int V = kV<T, W>, CW = 32 * V, RB = 128 * W, kRegion = 4 * kRows * RB;
   extern __shared__ __align__(128) char raw[];  // [2][warp][dt, x, b, dy][row][RB bytes]
   char* fmap = raw + kBwdMaps<V, W>;            // [warp] forward maps (P, H)
   char* bmap = fmap + kWarps * kMapBytes<V>;    // [warp] backward maps (P, C)
   char* pre = bmap + kWarps * kMapBytes<V>;     // [warp] exchange
   char* sums = pre + kWarps * kMapBytes<V>;     // [warp] sums of s d
-  __shared__ __align__(16) float s_A[2][CW];
   __shared__ Tile s_next[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int cl = lane * V;
@@ -599,6 +605,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas<W>) gated_scan_bwd_kerne
   int64_t id = 0;  // thread 0's
 
   uint32_t rb = 0;
+  Fv<V> A_next = all<V>(0.f);
   auto stage = [&](const Tile& t, int s) {
     const int t0 = (p.NT - 1 - t.x) * kStateRows, nv = p.L - t0 - warp * kRows, nc = p.ds - t.w;
     char* reg = raw + (s * kWarps + warp) * kRegion;
@@ -608,10 +615,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas<W>) gated_scan_bwd_kerne
     rows.template copy<1>(reg + 3 * kRows * RB, dyt, warp * kRows, p.dst, 0, nv, nc);
     cp_commit();
     if (RESET) rb = lane < min(nv, kRows) ? p.reset[(int64_t)t.z * p.L + t0 + warp * kRows + lane] : 0;
-    if (warp == 3) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) s_A[s][cl + i] = cl + i < nc ? -expf(ld_param(p.A_log, p.a_bf16, t.w + cl + i)) : 0.f;
-    }
+    for (int i = 0; i < V; ++i) A_next.v[i] = cl + i < nc ? ld_param(p.A_log, p.a_bf16, t.w + cl + i) : 0.f;
   };
   // the sum of the warps' s d of the tile before, in their order
   auto write_dA = [&](const Tile& t) {
@@ -628,7 +633,6 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas<W>) gated_scan_bwd_kerne
   __syncthreads();
   Tile t = s_next[0], before = make_int4(-1, 0, 0, 0);
   if (t.x >= 0) stage(t, 0);
-  __syncthreads();
   for (int s = 0; t.x >= 0; s ^= 1) {
     if (before.x < 0) {  // the first time, as in the forward
       cp_wait_all();
@@ -641,7 +645,9 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas<W>) gated_scan_bwd_kerne
     const int tt = p.NT - 1 - t.x, t0 = tt * kStateRows + warp * kRows, nv = p.L - t0, nc = p.ds - t.w;
     const uint32_t cut = RESET ? __ballot_sync(0xffffffffu, rb != 0) : 0;
     Fv<V> h = ld_state<V>(p.states + ((int64_t)t.z * p.NT + tt) * p.ds + t.w, cl, nc);
-    const Fv<V> A = ld_f<V>(reinterpret_cast<char*>(s_A[s]), 0, lane);
+    Fv<V> A;
+#pragma unroll
+    for (int i = 0; i < V; ++i) A.v[i] = -expf(A_next.v[i]);
     const Fv<V> A2 = A * all<V>(1.4426950408889634f);
     cp_wait_all();
     __syncwarp();
@@ -690,7 +696,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas<W>) gated_scan_bwd_kerne
     c = ld_state<V>(p.dh_last ? p.dh_last + at : nullptr, cl, nc);
     for (int k = 0; k < warp; ++k) h = apply<RESET>(ld_map<V>(fmap + k * kMapBytes<V>, lane), h);
     if (p.ticket) c = enter_tile<RESET, true, V>(p, t.y, t.x, bmap, kMapBytes<V>, pre, kMapBytes<V>, c, warp, lane);
-    else __syncthreads();  // s_A of the next tile, the sums
+    else __syncthreads();  // the sums of the tile before
     for (int k = kWarps - 1; k > warp; --k) c = apply<RESET>(ld_map<V>(bmap + k * kMapBytes<V>, lane), c);
 
     Fv<V> q[kRows];  // a_t h_{t-1}, 0 at a reset
@@ -807,6 +813,8 @@ static void scan_plan(ScanParams& p, int CW, void* ws) {
   p.NG = p.B * p.nch;
   p.ntiles = (int64_t)p.NG * p.NT;
   p.nent = (int)scan_entries(p.NT);
+  p.div_NG = p.NG > 1 ? ~uint64_t(0) / p.NG + 1 : 0;
+  p.div_nch = p.nch > 1 ? ~uint64_t(0) / p.nch + 1 : 0;
   p.ticket = p.NT > 1 ? static_cast<unsigned*>(ws) : nullptr;
   p.ent = p.NT > 1 ? reinterpret_cast<uint64_t*>(static_cast<char*>(ws) + 16) : nullptr;
 }
@@ -832,15 +840,21 @@ template <typename T, int W, bool RESET, int CB, bool BWD>
 static void scan_launch(const ScanParams& p, cudaStream_t s) {
   constexpr int V = kV<T, W>;
   constexpr int smem = BWD ? kBwdSmem<V, W> : 2 * kWarps * 3 * kRows * 128 * W;
-  const int64_t most = (int64_t)num_sms() * (BWD ? kBwdCtas<W> : kFwdCtas<W>);
+  const int64_t most = (int64_t)num_sms() * (BWD ? kBwdCtas : kFwdCtas<T, W>);
   const unsigned grid = (unsigned)(p.ntiles < most ? p.ntiles : most);
-  if constexpr (BWD) {
-    cudaFuncSetAttribute(gated_scan_bwd_kernel<T, W, RESET, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    gated_scan_bwd_kernel<T, W, RESET, CB><<<grid, kWarps * 32, smem, s>>>(p);
-  } else {
-    cudaFuncSetAttribute(gated_scan_fwd_kernel<T, W, RESET, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    gated_scan_fwd_kernel<T, W, RESET, CB><<<grid, kWarps * 32, smem, s>>>(p);
+  auto k = [] {
+    if constexpr (BWD) return gated_scan_bwd_kernel<T, W, RESET, CB>;
+    else return gated_scan_fwd_kernel<T, W, RESET, CB>;
+  }();
+  static std::atomic<uint64_t> ready{0};  // devices whose limit of shared memory is set
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    ready.fetch_or(bit, std::memory_order_relaxed);
   }
+  k<<<grid, kWarps * 32, smem, s>>>(p);
 }
 template <typename T, int W, bool BWD>
 static void scan_launch(const ScanParams& p, int cb, cudaStream_t s) {

@@ -497,6 +497,11 @@ def slot_step(q, k, v, gate, num_heads, gamma, gn_w, gn_b, R, U, k_cache, v_cach
 
 
 # ------------------------------------------------------------------ gated recurrence
+def _a(t):
+    """A tensor's address as a plain int (ctypes converts it), None for none."""
+    return t.data_ptr() if t is not None else None
+
+
 _ACTS = {"none": _lib.HDC_ACT_NONE, "silu": _lib.HDC_ACT_SILU}
 
 
@@ -557,9 +562,9 @@ def gated_scan(projs, A_log, d_state, h0=None, reset=None, out=None, return_stat
         rows = lib.hdc_gated_scan_state_rows()
         states = torch.empty(B, (L + rows - 1) // rows, d_state, device=projs.device, dtype=torch.float32)
     ws = _workspace(lib.hdc_gated_scan_workspace_bytes(B, L, d_state), projs.device)
-    _lib.call("hdc_gated_scan_fwd", dt, _code(A_log), _p(projs), projs.stride(0), projs.stride(1), _p(A_log), _p(h0),
-              _p(reset), _p(out), out.stride(0), out.stride(1), _p(h_last), _p(states), _p(ws),
-              ws.numel() if ws is not None else 0, B, L, d_state, _stream(projs))
+    _lib.call("hdc_gated_scan_fwd", dt, _code(A_log), _a(projs), projs.stride(0), projs.stride(1), _a(A_log), _a(h0),
+              _a(reset), _a(out), out.stride(0), out.stride(1), _a(h_last), _a(states), _a(ws),
+              ws.numel() if ws is not None else 0, B, L, d_state, torch.cuda.current_stream(projs.device).cuda_stream)
     return (out, h_last, states) if return_states else (out, h_last)
 
 
@@ -596,10 +601,10 @@ def gated_scan_bwd(dy, projs, A_log, states, d_state, reset=None, dh_last=None, 
     dA = torch.empty(d_state, device=projs.device, dtype=A_log.dtype)
     dh0 = torch.empty(B, d_state, device=projs.device, dtype=torch.float32) if need_dh0 else None
     ws = _workspace(lib.hdc_gated_scan_bwd_workspace_bytes(B, L, d_state), projs.device)
-    _lib.call("hdc_gated_scan_bwd", dt, _code(A_log), _p(projs), projs.stride(0), projs.stride(1), _p(A_log),
-              _p(states), _p(reset), _p(dy), dy.stride(0), dy.stride(1), _p(dh_last), _p(out), out.stride(0),
-              out.stride(1), _p(dA), _p(dh0), _p(ws), ws.numel() if ws is not None else 0, B, L, d_state,
-              _stream(projs))
+    _lib.call("hdc_gated_scan_bwd", dt, _code(A_log), _a(projs), projs.stride(0), projs.stride(1), _a(A_log),
+              _a(states), _a(reset), _a(dy), dy.stride(0), dy.stride(1), _a(dh_last), _a(out), out.stride(0),
+              out.stride(1), _a(dA), _a(dh0), _a(ws), ws.numel() if ws is not None else 0, B, L, d_state,
+              torch.cuda.current_stream(projs.device).cuda_stream)
     return out, dA, dh0
 
 
@@ -624,8 +629,8 @@ def gated_step(projs, A_log, h, d_state, reset=None, out=None, h_out=None):
         _same_dtype(projs, out)
         if out.shape != (B, d_state) or (d_state > 1 and out.stride(1) != 1):
             raise ValueError(f"out must be a [{B}, {d_state}] view with unit column stride")
-    _lib.call("hdc_gated_step", dt, _code(A_log), _p(projs), projs.stride(0), _p(A_log), _p(h), _p(reset), _p(h_out),
-              _p(out), out.stride(0), B, d_state, _stream(projs))
+    _lib.call("hdc_gated_step", dt, _code(A_log), _a(projs), projs.stride(0), _a(A_log), _a(h), _a(reset), _a(h_out),
+              _a(out), out.stride(0), B, d_state, torch.cuda.current_stream(projs.device).cuda_stream)
     return out, h_out
 
 
@@ -677,9 +682,9 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
         mean = torch.empty(N, num_groups, device=x.device, dtype=torch.float32)
         rstd = torch.empty(N, num_groups, device=x.device, dtype=torch.float32)
     ws = _workspace(_lib.load().hdc_group_norm_workspace_bytes(N, S, C, num_groups), x.device)
-    _lib.call("hdc_group_norm_fwd", dt, pd, _p(x3), x3.stride(0), x3.stride(1), _p(weight), _p(bias), _p(y), S * C, C,
-              _p(mean), _p(rstd), _p(ws), ws.numel() if ws is not None else 0, N, S, C, num_groups, float(eps),
-              _ACTS[act], _stream(x))
+    _lib.call("hdc_group_norm_fwd", dt, pd, _a(x3), x3.stride(0), x3.stride(1), _a(weight), _a(bias), _a(y), S * C, C,
+              _a(mean), _a(rstd), _a(ws), ws.numel() if ws is not None else 0, N, S, C, num_groups, float(eps),
+              _ACTS[act], torch.cuda.current_stream(x.device).cuda_stream)
     return (y, mean, rstd) if stats else y
 
 
@@ -703,7 +708,7 @@ def group_norm_act_bwd(dy, x, mean, rstd, num_groups, weight=None, bias=None, ac
     dw = torch.empty_like(weight) if need_params and weight is not None else None
     db = torch.empty_like(bias) if need_params and bias is not None else None
     ws = _workspace(_lib.load().hdc_group_norm_bwd_workspace_bytes(N, S, C, num_groups), x.device)
-    _lib.call("hdc_group_norm_bwd", dt, pd, _p(d3), d3.stride(0), d3.stride(1), _p(x3), x3.stride(0), x3.stride(1),
-              _p(mean), _p(rstd), _p(weight), _p(bias), _p(dx), S * C, C, _p(dw), _p(db), _p(ws),
-              ws.numel() if ws is not None else 0, N, S, C, num_groups, _ACTS[act], _stream(x))
+    _lib.call("hdc_group_norm_bwd", dt, pd, _a(d3), d3.stride(0), d3.stride(1), _a(x3), x3.stride(0), x3.stride(1),
+              _a(mean), _a(rstd), _a(weight), _a(bias), _a(dx), S * C, C, _a(dw), _a(db), _a(ws),
+              ws.numel() if ws is not None else 0, N, S, C, num_groups, _ACTS[act], torch.cuda.current_stream(x.device).cuda_stream)
     return dx, dw, db
