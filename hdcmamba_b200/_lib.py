@@ -108,6 +108,8 @@ class HdcError(RuntimeError):
 def load():
     """Load the shared library once (raises OSError if it is absent)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):

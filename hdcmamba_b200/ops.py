@@ -5,10 +5,17 @@ caching allocator on the current stream, and launches through ``_lib.call``.
 Only CUDA tensors are accepted: there is no CPU path.
 """
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
+
+try:  # the stream's address without a Stream object (0.2 us for 2.3)
+    from torch._C import _cuda_getCurrentRawStream as _current_raw_stream
+except ImportError:  # pragma: no cover
+    def _current_raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
 
 _DT = {torch.float32: _lib.HDC_F32, torch.bfloat16: _lib.HDC_BF16}
 
@@ -497,6 +504,17 @@ def slot_step(q, k, v, gate, num_heads, gamma, gn_w, gn_b, R, U, k_cache, v_cach
 
 
 # ------------------------------------------------------------------ gated recurrence
+@functools.lru_cache(maxsize=4096)
+def _size(name, *sizes):
+    """A size that the library computes from sizes alone."""
+    return int(getattr(_lib.load(), name)(*sizes))
+
+
+def _raw_stream(t):
+    """The current stream of t's device as an int."""
+    return _current_raw_stream(t.device.index)
+
+
 def _a(t):
     """A tensor's address as a plain int (ctypes converts it), None for none."""
     return t.data_ptr() if t is not None else None
@@ -557,14 +575,13 @@ def gated_scan(projs, A_log, d_state, h0=None, reset=None, out=None, return_stat
             raise ValueError(f"out must be a [{B}, {L}, {d_state}] view with unit column stride")
     h_last = torch.empty(B, d_state, device=projs.device, dtype=torch.float32)
     states = None
-    lib = _lib.load()
     if return_states:
-        rows = lib.hdc_gated_scan_state_rows()
+        rows = _size("hdc_gated_scan_state_rows")
         states = torch.empty(B, (L + rows - 1) // rows, d_state, device=projs.device, dtype=torch.float32)
-    ws = _workspace(lib.hdc_gated_scan_workspace_bytes(B, L, d_state), projs.device)
+    ws = _workspace(_size("hdc_gated_scan_workspace_bytes", B, L, d_state), projs.device)
     _lib.call("hdc_gated_scan_fwd", dt, _code(A_log), _a(projs), projs.stride(0), projs.stride(1), _a(A_log), _a(h0),
               _a(reset), _a(out), out.stride(0), out.stride(1), _a(h_last), _a(states), _a(ws),
-              ws.numel() if ws is not None else 0, B, L, d_state, torch.cuda.current_stream(projs.device).cuda_stream)
+              ws.numel() if ws is not None else 0, B, L, d_state, _raw_stream(projs))
     return (out, h_last, states) if return_states else (out, h_last)
 
 
@@ -585,8 +602,7 @@ def gated_scan_bwd(dy, projs, A_log, states, d_state, reset=None, dh_last=None, 
         raise ValueError(f"dy must be [{B}, {L}, {d_state}]")
     if d_state > 1 and dy.stride(2) != 1:
         dy = dy.contiguous()
-    lib = _lib.load()
-    rows = lib.hdc_gated_scan_state_rows()
+    rows = _size("hdc_gated_scan_state_rows")
     _f32_state(states, (B, (L + rows - 1) // rows, d_state), "states")
     if dh_last is not None:
         dh_last = dh_last.float().contiguous()
@@ -600,11 +616,11 @@ def gated_scan_bwd(dy, projs, A_log, states, d_state, reset=None, dh_last=None, 
             raise ValueError(f"out must be a [{B}, {L}, >= {3 * d_state}] view with unit column stride")
     dA = torch.empty(d_state, device=projs.device, dtype=A_log.dtype)
     dh0 = torch.empty(B, d_state, device=projs.device, dtype=torch.float32) if need_dh0 else None
-    ws = _workspace(lib.hdc_gated_scan_bwd_workspace_bytes(B, L, d_state), projs.device)
+    ws = _workspace(_size("hdc_gated_scan_bwd_workspace_bytes", B, L, d_state), projs.device)
     _lib.call("hdc_gated_scan_bwd", dt, _code(A_log), _a(projs), projs.stride(0), projs.stride(1), _a(A_log),
               _a(states), _a(reset), _a(dy), dy.stride(0), dy.stride(1), _a(dh_last), _a(out), out.stride(0),
               out.stride(1), _a(dA), _a(dh0), _a(ws), ws.numel() if ws is not None else 0, B, L, d_state,
-              torch.cuda.current_stream(projs.device).cuda_stream)
+              _raw_stream(projs))
     return out, dA, dh0
 
 
@@ -630,7 +646,7 @@ def gated_step(projs, A_log, h, d_state, reset=None, out=None, h_out=None):
         if out.shape != (B, d_state) or (d_state > 1 and out.stride(1) != 1):
             raise ValueError(f"out must be a [{B}, {d_state}] view with unit column stride")
     _lib.call("hdc_gated_step", dt, _code(A_log), _a(projs), projs.stride(0), _a(A_log), _a(h), _a(reset), _a(h_out),
-              _a(out), out.stride(0), B, d_state, torch.cuda.current_stream(projs.device).cuda_stream)
+              _a(out), out.stride(0), B, d_state, _raw_stream(projs))
     return out, h_out
 
 
@@ -681,10 +697,10 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     if stats:
         mean = torch.empty(N, num_groups, device=x.device, dtype=torch.float32)
         rstd = torch.empty(N, num_groups, device=x.device, dtype=torch.float32)
-    ws = _workspace(_lib.load().hdc_group_norm_workspace_bytes(N, S, C, num_groups), x.device)
+    ws = _workspace(_size("hdc_group_norm_workspace_bytes", N, S, C, num_groups), x.device)
     _lib.call("hdc_group_norm_fwd", dt, pd, _a(x3), x3.stride(0), x3.stride(1), _a(weight), _a(bias), _a(y), S * C, C,
               _a(mean), _a(rstd), _a(ws), ws.numel() if ws is not None else 0, N, S, C, num_groups, float(eps),
-              _ACTS[act], torch.cuda.current_stream(x.device).cuda_stream)
+              _ACTS[act], _raw_stream(x))
     return (y, mean, rstd) if stats else y
 
 
@@ -707,8 +723,8 @@ def group_norm_act_bwd(dy, x, mean, rstd, num_groups, weight=None, bias=None, ac
     dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     dw = torch.empty_like(weight) if need_params and weight is not None else None
     db = torch.empty_like(bias) if need_params and bias is not None else None
-    ws = _workspace(_lib.load().hdc_group_norm_bwd_workspace_bytes(N, S, C, num_groups), x.device)
+    ws = _workspace(_size("hdc_group_norm_bwd_workspace_bytes", N, S, C, num_groups), x.device)
     _lib.call("hdc_group_norm_bwd", dt, pd, _a(d3), d3.stride(0), d3.stride(1), _a(x3), x3.stride(0), x3.stride(1),
               _a(mean), _a(rstd), _a(weight), _a(bias), _a(dx), S * C, C, _a(dw), _a(db), _a(ws),
-              ws.numel() if ws is not None else 0, N, S, C, num_groups, _ACTS[act], torch.cuda.current_stream(x.device).cuda_stream)
+              ws.numel() if ws is not None else 0, N, S, C, num_groups, _ACTS[act], _raw_stream(x))
     return dx, dw, db

@@ -18,13 +18,18 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import ops
 from .model import _require_cuda, fused_norm_conv1d_trainable
 
 __all__ = ["gated_scan", "group_norm_act", "GatedScanFunction", "GroupNormActFunction", "GatedRecurrentBlock",
            "RecurrentState"]
+
+
+def _first_order_only():
+    """Gradients of the gradients are not implemented: an error rather than missing terms."""
+    if torch.is_grad_enabled():  # only with create_graph=True
+        raise RuntimeError("hdcmamba_b200: gated_scan and group_norm_act are differentiable once (create_graph=False)")
 
 
 class GatedScanFunction(torch.autograd.Function):
@@ -40,8 +45,8 @@ class GatedScanFunction(torch.autograd.Function):
         return y, h_last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh_last):
+        _first_order_only()
         projs, A_log, states, reset = ctx.saved_tensors
         ds = ctx.d_state
         if dy is None:
@@ -77,8 +82,8 @@ class GroupNormActFunction(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _first_order_only()
         x, weight, bias, mean, rstd = ctx.saved_tensors
         dx, dw, db = ops.group_norm_act_bwd(dy, x, mean, rstd, ctx.num_groups, weight, bias, act=ctx.act,
                                             need_params=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
