@@ -30,6 +30,17 @@
 // no published P is, so the word is its own flag.  The next tile is in flight (cp.async)
 // while one is computed.
 // P < 0 marks a map that a reset has cut off from what came before (P is otherwise >= 0).
+//
+// Why tiles of 64 steps: what a tile keeps between its two halves (a and u: 8 bytes per step and
+// channel) has to stay on the SM, in registers, and 16 to 32 warps of it fill them.  Measured
+// (device time, inputs out of L2, against 6550 GB/s): 8 x 4096 x 1280 bf16 forward 87 us (59%),
+// backward 184 us (49%); 1 x 32768 x 768 bf16 forward 91 us (34%); 1 x 32768 x 64 bf16 15 us;
+// 3 x 1537 x 333 fp32 forward 17 us, backward 30 us.  With many channels the issue slots bind (55 to
+// 65% busy, the rest waits of dependent instructions between 16 warps; without the exchange the
+// forward of the same bytes takes 44 us per 201 MB); with few, each round of tiles waits for the
+// slowest map before it, some 4 us of a round's 8.  Tried and slower: tickets that run the maps a
+// few hundred tiles ahead of the outputs (inputs read again from L2: 105 us for 91), one word per
+// lane (above), three backward CTAs per SM (spills).
 #include <atomic>
 #include <type_traits>
 
@@ -743,23 +754,27 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gated_scan_bwd_kernel(c
 }
 
 // dA_log[j] = A_j times the sum of the parts ([q][b][channel], channels padded to cpad), in their
-// order: 8 strands per channel (32 channels a CTA), then the strands
-__global__ void __launch_bounds__(256) gated_scan_dA_kernel(const float* part, int64_t parts, int cpad, int ds,
-                                                            const void* A_log, int a_bf16, void* dA) {
-  __shared__ float s[8][32];
-  const int j = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+// order: 32 strands per channel (32 channels a CTA), then the strands.
+__global__ void __launch_bounds__(1024) gated_scan_dA_kernel(const float* part, int64_t parts, int cpad, int ds,
+                                                             const void* A_log, int a_bf16, void* dA) {
+  __shared__ float s[32][33];
+  const int x = threadIdx.x & 31, k = threadIdx.x >> 5, j = blockIdx.x * 32 + x;
   float v = 0.f;
-  if (j < ds)
-    for (int64_t i = k; i < parts; i += 8) v += part[i * cpad + j];
-  s[k][threadIdx.x & 31] = v;
+  if (j < ds) {
+#pragma unroll 8
+    for (int64_t i = k; i < parts; i += 32) v += part[i * cpad + j];
+  }
+  s[k][x] = v;
   __syncthreads();
   if (k != 0 || j >= ds) return;
-  for (int i = 1; i < 8; ++i) v += s[i][threadIdx.x];
+  for (int i = 1; i < 32; ++i) v += s[i][x];
   v *= -expf(ld_param(A_log, a_bf16, j));
   if (a_bf16) static_cast<__nv_bfloat16*>(dA)[j] = __float2bfloat16_rn(v);
   else static_cast<float*>(dA)[j] = v;
 }
 
+// One step per sequence: a thread per channel, 20 bytes (bf16) each.  Bound by the launch up to a
+// few hundred thousand channels (1 x 768: 1.6 us, 256 x 2048: 4.3 us, 1.3 us of it traffic).
 template <typename T>
 __global__ void __launch_bounds__(128) gated_step_kernel(const T* projs, int64_t psb, const void* A_log, int a_bf16,
                                                          const float* h, const uint8_t* reset, float* h_out, T* y,
@@ -832,8 +847,10 @@ static int scan_fits(const char* what, int64_t B, int64_t L, int64_t ds) {
                 (long long)ds);
   return 0;
 }
-// Words per lane: two (tiles of 128 bf16 or 64 fp32 channels) halve the instructions per channel
-// that a tile costs beside the arithmetic; one where half of a wide tile would be empty.
+// Words per lane in the forward: two (tiles of 128 bf16 or 64 fp32 channels) halve what a tile costs
+// beside its arithmetic (8 x 4096 x 1280 bf16: 87 us for 95, 1 x 32768 x 768: 91 for 93); one where
+// much of a wide tile would be empty (the 64 channels of a Block's d_state: half of it).  The
+// backward holds more per channel (two words spill 500 bytes) and takes one.
 static int scan_words(int64_t ds, int es) { return ds * es % 256 == 0 || ds * es > 1024 ? 2 : 1; }
 
 template <typename T, int W, bool RESET, int CB, bool BWD>
@@ -962,7 +979,7 @@ extern "C" int hdc_gated_scan_bwd(int dtype, int a_dtype, const void* projs, int
                                   : cudaMemsetAsync(dh0, 0, (size_t)B * ds * 4, s);
     if (e != cudaSuccess) return fail((int)e, "gated_scan_bwd: %s", cudaGetErrorString(e));
   }
-  gated_scan_dA_kernel<<<(unsigned)((ds + 31) / 32), 256, 0, s>>>(p.dA_part, (int64_t)p.NT * B, p.nch * p.CW, (int)ds,
+  gated_scan_dA_kernel<<<(unsigned)((ds + 31) / 32), 1024, 0, s>>>(p.dA_part, (int64_t)p.NT * B, p.nch * p.CW, (int)ds,
                                                                   A_log, p.a_bf16, dA_log);
   return launch_status("gated_scan_dA_kernel");
 }

@@ -28,7 +28,8 @@ namespace hdc {
 // ---------------------------------------------------------------- several positions per sample
 // CTA (sample and slice, channel block): thread = (row lane, chunk of VE channels).
 constexpr int kGnThreads = 256;
-constexpr int kGnFwdCtas = 3, kGnBwdCtas = 2;  // resident CTAs per SM of the two-pass kernels
+// resident CTAs per SM of the two-pass kernels (forward with four: 39 us for 34, 16 x 4096 x 320)
+constexpr int kGnFwdCtas = 3, kGnBwdCtas = 2;
 // row lanes of a CTA: threads per chunk of channels (one when a thread has several chunks)
 __host__ __device__ inline int gn_lanes(int nchunk) { return nchunk < kGnThreads ? kGnThreads / nchunk : 1; }
 
@@ -484,23 +485,23 @@ __global__ void __launch_bounds__(256) gn_any_bwd_kernel(GnParams p) {
   }
 }
 
-// dw[c] (blockIdx.y 0) and db[c] (1): sums of the parts, 8 strands per channel, then the strands
-__global__ void __launch_bounds__(256) gn_param_grad_kernel(const float* part, int64_t parts, int C, void* dw, void* db,
-                                                            int bf16) {
-  __shared__ float s[8][32];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+// dw[c] (blockIdx.y 0) and db[c] (1): sums of the parts, 32 strands per channel, then the strands
+__global__ void __launch_bounds__(1024) gn_param_grad_kernel(const float* part, int64_t parts, int C, void* dw, void* db,
+                                                             int bf16) {
+  __shared__ float s[32][33];
+  const int x = threadIdx.x & 31, k = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
   void* out = blockIdx.y ? db : dw;
   wait_for_previous();
   if (!out) return;
   float v = 0.f;
   if (c < C) {
-#pragma unroll 4
-    for (int64_t i = k; i < parts; i += 8) v += part[(i * 2 + blockIdx.y) * C + c];
+#pragma unroll 8
+    for (int64_t i = k; i < parts; i += 32) v += part[(i * 2 + blockIdx.y) * C + c];
   }
-  s[k][threadIdx.x & 31] = v;
+  s[k][x] = v;
   __syncthreads();
   if (k != 0 || c >= C) return;
-  for (int i = 1; i < 8; ++i) v += s[i][threadIdx.x];
+  for (int i = 1; i < 32; ++i) v += s[i][x];
   if (bf16) static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn(v);
   else static_cast<float*>(out)[c] = v;
 }
@@ -535,10 +536,12 @@ static int64_t gn_row_parts(int64_t N, int64_t G, int64_t Cg) {
     }
   return most;
 }
-// Several positions.  One pass when a sample's block of channels is small enough to be read again
-// from L1 (64 KB), the blocks then about 64 channels wide for more CTAs; else slices of each
-// sample, 32 positions or more, in one wave of the resident CTAs: a CTA's fixed cost (joining its
-// threads' sums) is that of some 30 rows.
+// Several positions.  One pass when a sample's block of some 64 channels is small enough (64 KB in
+// bf16) to be read again from L1 (2 x 225 x 96: 6.0 us forward, 7.2 backward; in two passes 7.6 and
+// 10.5).  Else slices of each sample, 32 positions or more, in one wave of the resident CTAs: a
+// CTA's fixed cost (joining its threads' sums) is that of some 30 rows, and a second wave starts
+// late (432 backward CTAs for 296 places: 60 us, 296: 46 us, 4 x 16384 x 128 fp32).  Also tried: the
+// block held in the shared memory of a cluster and read once (16 x 4096 x 320 bf16: 51 us for 34).
 struct GnPlan { int64_t slices, rows, cb, gz; bool one; };
 // Whole groups, about `want` channels, a multiple of the channels that a load of the full row
 // could take (so that blocks do not narrow the loads).
@@ -554,10 +557,6 @@ static GnPlan gn_plan(int64_t N, int64_t S, int64_t C, int64_t G, bool bwd) {
   const int64_t Cg = C / G;
   r.cb = gn_block(C, Cg, 64);
   r.one = S * r.cb <= 32768 && r.cb <= 1024;
-  if (r.one && N * ((C + r.cb - 1) / r.cb) > 592) {  // CTAs enough: wider blocks
-    const int64_t wide = gn_block(C, Cg, 256);
-    if (S * wide <= 32768) r.cb = wide;
-  }
   if (!r.one) r.cb = gn_block(C, Cg, 512);
   r.gz = (C + r.cb - 1) / r.cb;
   r.rows = S;
@@ -765,19 +764,19 @@ extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_
       gn_pass(kSums, dtype, p, plan, ve, s);
       if (int e = launch_status("gn_sums_kernel")) return e;
       parts = N;
-      const int block = gn_mid_block(p.C, p.Cg), items = 2 * block, strands = items < 256 ? 256 / items : 1;
       if (!plan.one) {
-      launch_dependent(gn_mid_kernel, dim3((unsigned)N, (unsigned)((C + block - 1) / block)), 256,
-                       (size_t)(strands + 1) * items * 4, s, p, block);
-      if (int e = launch_status("gn_mid_kernel")) return e;
-      gn_pass(kDx, dtype, p, plan, ve, s);
-      if (int e = launch_status("gn_dx_kernel")) return e;
-      p.part = p.sums;
+        const int block = gn_mid_block(p.C, p.Cg), items = 2 * block, strands = items < 256 ? 256 / items : 1;
+        launch_dependent(gn_mid_kernel, dim3((unsigned)N, (unsigned)((C + block - 1) / block)), 256,
+                         (size_t)(strands + 1) * items * 4, s, p, block);
+        if (int e = launch_status("gn_mid_kernel")) return e;
+        gn_pass(kDx, dtype, p, plan, ve, s);
+        if (int e = launch_status("gn_dx_kernel")) return e;
+        p.part = p.sums;
       }
     }
   }
   if (!dweight && !dbias) return HDC_OK;
-  launch_dependent(gn_param_grad_kernel, dim3((unsigned)((C + 31) / 32), 2), 256, 0, s, p.part, parts, (int)C, dweight,
+  launch_dependent(gn_param_grad_kernel, dim3((unsigned)((C + 31) / 32), 2), 1024, 0, s, p.part, parts, (int)C, dweight,
                    dbias, p.p_bf16);
   return launch_status("gn_param_grad_kernel");
 }
