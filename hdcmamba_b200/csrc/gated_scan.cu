@@ -171,6 +171,10 @@ template <typename T, int V> __device__ __forceinline__ Fv<V> gate(const Fv<V>& 
     return fma(p, e, m);
   }
 }
+// A = -exp(A_log)
+template <typename T> __device__ __forceinline__ float rate(float A_log) {
+  return sizeof(T) == 4 ? -expf(A_log) : -ex2(1.4426950408889634f * A_log);
+}
 // a = exp(d A); A2 = A log2(e)
 template <typename T, int V> __device__ __forceinline__ Fv<V> decay(const Fv<V>& d, const Fv<V>& A, const Fv<V>& A2) {
   Fv<V> a;
@@ -527,7 +531,7 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas<T, W>) gated_scan_fwd_ke
     const uint32_t cut = RESET ? __ballot_sync(0xffffffffu, rb != 0) : 0;
     Fv<V> A;
 #pragma unroll
-    for (int i = 0; i < V; ++i) A.v[i] = -expf(A_next.v[i]);
+    for (int i = 0; i < V; ++i) A.v[i] = rate<T>(A_next.v[i]);
     const Fv<V> A2 = A * all<V>(1.4426950408889634f);
     cp_wait_all();
     __syncwarp();
@@ -658,7 +662,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gated_scan_bwd_kernel(c
     Fv<V> h = ld_state<V>(p.states + ((int64_t)t.z * p.NT + tt) * p.ds + t.w, cl, nc);
     Fv<V> A;
 #pragma unroll
-    for (int i = 0; i < V; ++i) A.v[i] = -expf(A_next.v[i]);
+    for (int i = 0; i < V; ++i) A.v[i] = rate<T>(A_next.v[i]);
     const Fv<V> A2 = A * all<V>(1.4426950408889634f);
     cp_wait_all();
     __syncwarp();
@@ -669,7 +673,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gated_scan_bwd_kernel(c
     }
 
     // local scans of the warp's steps, forward and backward
-    Fv<V> a[kRows], d[kRows];
+    Fv<V> a[kRows], d[kRows], bx[kRows];
     Map<V> m = identity_map<V>();
     Fv<V> c = all<V>(0.f);
     const char* w = mine + lane * 4 * W;
@@ -679,7 +683,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gated_scan_bwd_kernel(c
       const Fv<V> b = ld_words<T, W>(w + (2 * kRows + r) * RB);
       d[r] = gate<T>(dt);
       a[r] = decay<T>(d[r], A, A2);
-      const Fv<V> u = d[r] * (b * x);
+      bx[r] = b * x;
+      const Fv<V> u = d[r] * bx[r];
       // the backward map from zero: c = sum of dy_r times the decays up to step r, until a reset
       if (RESET && ((cut >> r) & 1)) {
         m.H = u;
@@ -713,9 +718,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gated_scan_bwd_kernel(c
     Fv<V> q[kRows];  // a_t h_{t-1}, 0 at a reset
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const Fv<V> x = ld_words<T, W>(w + (kRows + r) * RB), b = ld_words<T, W>(w + (2 * kRows + r) * RB);
       q[r] = RESET && ((cut >> r) & 1) ? all<V>(0.f) : a[r] * h;
-      h = fma(d[r], b * x, q[r]);
+      h = fma(d[r], bx[r], q[r]);
     }
     Fv<V> sum = all<V>(0.f);
     T* out = static_cast<T*>(p.dprojs) + t.z * p.gsb + t0 * p.gst + t.w;
@@ -728,7 +732,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gated_scan_bwd_kernel(c
       c = a[r] * g;
       if (RESET && ((cut >> r) & 1)) c = all<V>(0.f);
       const Fv<V> gd = g * d[r], sr = g * q[r];
-      const Fv<V> ddt = fma(sr, A, g * (b * x)) * sigmoid<T>(dt);
+      const Fv<V> ddt = fma(sr, A, g * bx[r]) * sigmoid<T>(dt);
       if (whole) {
         sum = fma(sr, d[r], sum);
         T* o = out + r * p.gst + cl;
@@ -847,11 +851,12 @@ static int scan_fits(const char* what, int64_t B, int64_t L, int64_t ds) {
                 (long long)ds);
   return 0;
 }
-// Words per lane in the forward: two (tiles of 128 bf16 or 64 fp32 channels) halve what a tile costs
-// beside its arithmetic (8 x 4096 x 1280 bf16: 87 us for 95, 1 x 32768 x 768: 91 for 93); one where
-// much of a wide tile would be empty (the 64 channels of a Block's d_state: half of it).  The
-// backward holds more per channel (two words spill 500 bytes) and takes one.
-static int scan_words(int64_t ds, int es) { return ds * es % 256 == 0 || ds * es > 1024 ? 2 : 1; }
+// Words per lane in the forward: in bf16 two (tiles of 128 channels) halve what a tile costs beside
+// its arithmetic (8 x 4096 x 1280: 87 us for 95, 1 x 32768 x 768: 91 for 93); one where much of a
+// wide tile would be empty (the 64 channels of a Block's d_state: half of it), and in fp32, whose
+// exp and log1p take the registers (3 x 1537 x 333: 17 us with one, 19 with two).  The backward
+// holds more per channel (two words spill 500 bytes) and takes one.
+static int scan_words(int64_t ds, int es) { return es == 2 && (ds % 128 == 0 || ds > 512) ? 2 : 1; }
 
 template <typename T, int W, bool RESET, int CB, bool BWD>
 static void scan_launch(const ScanParams& p, cudaStream_t s) {
@@ -883,7 +888,7 @@ static void scan_launch(const ScanParams& p, int cb, cudaStream_t s) {
 template <bool BWD>
 static void scan_launch(const ScanParams& p, int dtype, int W, int cb, cudaStream_t s) {
   constexpr int most = BWD ? 1 : 2;
-  if (dtype == HDC_F32) W == 2 ? scan_launch<float, most, BWD>(p, cb, s) : scan_launch<float, 1, BWD>(p, cb, s);
+  if (dtype == HDC_F32) scan_launch<float, 1, BWD>(p, cb, s);
   else W == 2 ? scan_launch<__nv_bfloat16, most, BWD>(p, cb, s) : scan_launch<__nv_bfloat16, 1, BWD>(p, cb, s);
 }
 
