@@ -592,7 +592,6 @@ def gated_scan_bwd(dy, projs, A_log, states, d_state, reset=None, dh_last=None, 
     (its first 3*d_state columns).  Returns (dprojs, dA_log in A_log.dtype, dh0 fp32
     [B, d_state] or None)."""
     _cuda(dy, projs, A_log, states, reset, dh_last, out)
-    dt = _code(projs)
     if projs.dim() != 3:
         raise ValueError("projs must be [B, L, cols]")
     B, L, _ = projs.shape
@@ -600,27 +599,34 @@ def gated_scan_bwd(dy, projs, A_log, states, d_state, reset=None, dh_last=None, 
     _same_dtype(projs, dy)
     if dy.shape != (B, L, d_state):
         raise ValueError(f"dy must be [{B}, {L}, {d_state}]")
-    if d_state > 1 and dy.stride(2) != 1:
-        dy = dy.contiguous()
     rows = _size("hdc_gated_scan_state_rows")
     _f32_state(states, (B, (L + rows - 1) // rows, d_state), "states")
     if dh_last is not None:
         dh_last = dh_last.float().contiguous()
         if dh_last.shape != (B, d_state):
             raise ValueError(f"dh_last must be [{B}, {d_state}]")
-    if out is None:
-        out = torch.empty(B, L, 3 * d_state, device=projs.device, dtype=projs.dtype)
-    else:
+    if out is not None:
         _same_dtype(projs, out)
         if out.dim() != 3 or out.shape[:2] != (B, L) or out.shape[2] < 3 * d_state or out.stride(2) != 1:
             raise ValueError(f"out must be a [{B}, {L}, >= {3 * d_state}] view with unit column stride")
-    dA = torch.empty(d_state, device=projs.device, dtype=A_log.dtype)
-    dh0 = torch.empty(B, d_state, device=projs.device, dtype=torch.float32) if need_dh0 else None
-    ws = _workspace(_size("hdc_gated_scan_bwd_workspace_bytes", B, L, d_state), projs.device)
-    _lib.call("hdc_gated_scan_bwd", dt, _code(A_log), _a(projs), projs.stride(0), projs.stride(1), _a(A_log),
+    return _gated_scan_bwd(dy, projs, A_log, states, d_state, reset, dh_last, need_dh0, out)
+
+
+def _gated_scan_bwd(dy, projs, A_log, states, d_state, reset, dh_last, need_dh0, out):
+    """``gated_scan_bwd`` on arguments that have been checked (A_log, reset, dh_last contiguous)."""
+    B, L, _ = projs.shape
+    dev = projs.device
+    if d_state > 1 and dy.stride(2) != 1:
+        dy = dy.contiguous()
+    if out is None:
+        out = torch.empty(B, L, 3 * d_state, device=dev, dtype=projs.dtype)
+    dA = torch.empty_like(A_log)
+    dh0 = torch.empty(B, d_state, device=dev, dtype=torch.float32) if need_dh0 else None
+    nbytes = _size("hdc_gated_scan_bwd_workspace_bytes", B, L, d_state)
+    ws = _workspace(nbytes, dev)
+    _lib.call("hdc_gated_scan_bwd", _code(projs), _code(A_log), _a(projs), projs.stride(0), projs.stride(1), _a(A_log),
               _a(states), _a(reset), _a(dy), dy.stride(0), dy.stride(1), _a(dh_last), _a(out), out.stride(0),
-              out.stride(1), _a(dA), _a(dh0), _a(ws), ws.numel() if ws is not None else 0, B, L, d_state,
-              _raw_stream(projs))
+              out.stride(1), _a(dA), _a(dh0), _a(ws), nbytes, B, L, d_state, _raw_stream(projs))
     return out, dA, dh0
 
 
@@ -709,22 +715,30 @@ def group_norm_act_bwd(dy, x, mean, rstd, num_groups, weight=None, bias=None, ac
     Returns (dx in x.dtype, dweight, dbias in the parameters' type, None for a parameter that
     is None or when ``need_params`` is false)."""
     _cuda(dy, x, mean, rstd, weight, bias)
-    dt = _code(x)
+    _code(x)
     if act not in _ACTS:
         raise ValueError(f"act must be one of {sorted(_ACTS)}")
     _same_dtype(x, dy)
     if dy.shape != x.shape:
         raise ValueError(f"dy {list(dy.shape)} must have x's shape {list(x.shape)}")
-    x3, d3 = _positions(x), _positions(dy)
-    pd, weight, bias = _norm_params(x, num_groups, weight, bias)
-    N, S, C = x3.shape
+    _, weight, bias = _norm_params(x, num_groups, weight, bias)
+    N = x.shape[0]
     _f32_state(mean, (N, num_groups), "mean")
     _f32_state(rstd, (N, num_groups), "rstd")
+    return _group_norm_bwd(dy, x, mean, rstd, num_groups, weight, bias, act, need_params)
+
+
+def _group_norm_bwd(dy, x, mean, rstd, num_groups, weight, bias, act, need_params):
+    """``group_norm_act_bwd`` on arguments that have been checked (weight, bias contiguous)."""
+    x3, d3 = _positions(x), _positions(dy)
+    N, S, C = x3.shape
+    ref = weight if weight is not None else bias if bias is not None else x
     dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     dw = torch.empty_like(weight) if need_params and weight is not None else None
     db = torch.empty_like(bias) if need_params and bias is not None else None
-    ws = _workspace(_size("hdc_group_norm_bwd_workspace_bytes", N, S, C, num_groups), x.device)
-    _lib.call("hdc_group_norm_bwd", dt, pd, _a(d3), d3.stride(0), d3.stride(1), _a(x3), x3.stride(0), x3.stride(1),
-              _a(mean), _a(rstd), _a(weight), _a(bias), _a(dx), S * C, C, _a(dw), _a(db), _a(ws),
-              ws.numel() if ws is not None else 0, N, S, C, num_groups, _ACTS[act], _raw_stream(x))
+    nbytes = _size("hdc_group_norm_bwd_workspace_bytes", N, S, C, num_groups)
+    ws = _workspace(nbytes, x.device)
+    _lib.call("hdc_group_norm_bwd", _code(x), _code(ref), _a(d3), d3.stride(0), d3.stride(1), _a(x3), x3.stride(0),
+              x3.stride(1), _a(mean), _a(rstd), _a(weight), _a(bias), _a(dx), S * C, C, _a(dw), _a(db), _a(ws), nbytes,
+              N, S, C, num_groups, _ACTS[act], _raw_stream(x))
     return dx, dw, db

@@ -38,6 +38,7 @@ class GatedScanFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, projs, A_log, h0, reset, d_state):
+        A_log, reset = A_log.contiguous(), reset.contiguous() if reset is not None else None
         y, h_last, states = ops.gated_scan(projs, A_log, d_state, h0=h0, reset=reset, return_states=True)
         ctx.save_for_backward(projs, A_log, states, reset)
         ctx.d_state, ctx.h0_dtype = d_state, h0.dtype if h0 is not None else None
@@ -55,8 +56,10 @@ class GatedScanFunction(torch.autograd.Function):
         if projs.shape[2] > 3 * ds:  # columns the recurrence does not read have a zero gradient
             out = torch.zeros(projs.shape, device=projs.device, dtype=projs.dtype)
         need_dh0 = ctx.h0_dtype is not None and ctx.needs_input_grad[2]
-        dprojs, dA, dh0 = ops.gated_scan_bwd(dy, projs, A_log, states, ds, reset=reset, dh_last=dh_last,
-                                             need_dh0=need_dh0, out=out)
+        if dh_last is not None:
+            dh_last = dh_last.contiguous()
+        # the forward has checked the arguments
+        dprojs, dA, dh0 = ops._gated_scan_bwd(dy, projs, A_log, states, ds, reset, dh_last, need_dh0, out)
         return dprojs, dA, dh0.to(ctx.h0_dtype) if dh0 is not None else None, None, None
 
 
@@ -76,6 +79,8 @@ class GroupNormActFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, num_groups, eps, act):
+        weight = weight.contiguous() if weight is not None else None
+        bias = bias.contiguous() if bias is not None else None
         y, mean, rstd = ops.group_norm_act(x, num_groups, weight, bias, eps=eps, act=act, stats=True)
         ctx.save_for_backward(x, weight, bias, mean, rstd)
         ctx.num_groups, ctx.act = num_groups, act
@@ -85,8 +90,9 @@ class GroupNormActFunction(torch.autograd.Function):
     def backward(ctx, dy):
         _first_order_only()
         x, weight, bias, mean, rstd = ctx.saved_tensors
-        dx, dw, db = ops.group_norm_act_bwd(dy, x, mean, rstd, ctx.num_groups, weight, bias, act=ctx.act,
-                                            need_params=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        # the forward has checked the arguments
+        dx, dw, db = ops._group_norm_bwd(dy, x, mean, rstd, ctx.num_groups, weight, bias, ctx.act,
+                                         ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
         return dx, dw, db, None, None, None
 
 

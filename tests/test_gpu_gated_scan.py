@@ -360,6 +360,17 @@ def test_autograd_inputs():
         assert recurrent.gated_scan(p, a, ds)[0].grad_fn is None
 
 
+def test_second_order_raises():
+    projs, A_log = inputs(1, 20, 16, F32)
+    p = projs.clone().requires_grad_()
+    y, _ = recurrent.gated_scan(p, A_log, 16)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(y.sum(), p, create_graph=True)
+    z = recurrent.group_norm_act(p, 3, act="silu")
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(z.sum(), p, create_graph=True)
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals():
     projs, A_log = inputs(2, 10, 16, F32)
