@@ -34,8 +34,8 @@
 // Why tiles of 64 steps: what a tile keeps between its two halves (a and u: 8 bytes per step and
 // channel) has to stay on the SM, in registers, and 16 to 32 warps of it fill them.  Measured
 // (device time, inputs out of L2, against 6550 GB/s): 8 x 4096 x 1280 bf16 forward 87 us (59%),
-// backward 184 us (49%); 1 x 32768 x 768 bf16 forward 91 us (34%); 1 x 32768 x 64 bf16 15 us;
-// 3 x 1537 x 333 fp32 forward 17 us, backward 30 us.  With many channels the issue slots bind (55 to
+// backward 171 us (52%); 1 x 32768 x 768 bf16 forward 92 us (33%); 1 x 32768 x 64 bf16 15 us;
+// 3 x 1537 x 333 fp32 forward 17 us, backward 29 us.  With many channels the issue slots bind (55 to
 // 65% busy, the rest waits of dependent instructions between 16 warps; without the exchange the
 // forward of the same bytes takes 44 us per 201 MB); with few, each round of tiles waits for the
 // slowest map before it, some 4 us of a round's 8.  Tried and slower: tickets that run the maps a
@@ -310,7 +310,8 @@ template <bool RESET, int V> __device__ __forceinline__ Map<V> take(const uint64
       do {
         __nanosleep(32);
         ld_entry<1>(e + lane * 32 * V, one);
-        late = clock64() - t0 > kWaitCycles;
+        // a wait that has run out elsewhere ends this one too, so that the kernel ends soon
+        late = clock64() - t0 > kWaitCycles || *static_cast<volatile int*>(&g_dev_error) == 61;
       } while ((uint32_t)one[0] == kUnset && !late);
     }
     if (__any_sync(0xffffffffu, late)) {
@@ -599,7 +600,8 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas<T, W>) gated_scan_fwd_ke
   }
 }
 
-constexpr int kBwdCtas = 2;  // resident backward CTAs per SM (three: 80 registers, spills, 244 us for 184)
+// resident backward CTAs per SM (three: 80 registers and spills, 244 us for 184, 8 x 4096 x 1280)
+constexpr int kBwdCtas = 2;
 // shared memory of the backward: two staged tiles, the warps' forward maps and backward maps
 // (P shared), the exchange's slots, the warps' sums for dA
 template <int V, int W> constexpr int kBwdMaps = 2 * kWarps * 4 * kRows * 128 * W;

@@ -20,7 +20,10 @@
 // Statistics never cancel: a thread takes blocks of rows, each with its own mean and centred
 // squares, and blocks, threads and slices are joined by
 //   n = n1 + n2, mean = mean1 + (mean2 - mean1) n2/n, M2 = M2_1 + M2_2 + (mean2 - mean1)^2 n1 n2/n.
-// Channels per load: as many as 16 bytes, the rows' alignment and (S = 1) the group allow.
+// Channels per load: as many as 16 bytes hold and the row (S = 1: the group) divides into.
+// Measured (device time, against 6550 GB/s): 16 x 4096 x 320 bf16 forward 34 us (38%): statistics
+// 16, joining 3, outputs 15, each bound by the latency of its loads at 24 warps per SM;
+// 4 x 16384 x 128 fp32 forward 25 us (40%), backward 46 us (33%); 2 x 225 x 96 bf16 6.2 and 7.5 us.
 #include "group_norm.cuh"
 
 namespace hdc {

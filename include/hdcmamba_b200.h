@@ -368,17 +368,22 @@ int hdc_slot_step(int dtype, const void* q, const void* k, const void* v, const 
  *   reset  : NULL or uint8 [B, L] contiguous; where non-zero, step t starts from a zero state
  *            whatever h_{t-1} holds (infinities and NaN included).
  *   y      : element (b, t, j) at y + b*y_sb + t*y_st + j; must not overlap projs.
- *   h_last : NULL or fp32 [B, ds], the state after the last step (h0 or zeros when L = 0).
+ *   h_last : NULL or fp32 [B, ds], the state after the last step (h0 or zeros when L = 0); must
+ *            not overlap h0.
  *   states : NULL, or fp32 [B, ceil(L / R), ds] with R = hdc_gated_scan_state_rows(): the
  *            state before steps 0, R, 2R, ..., which the gradient starts from.
  *   workspace : hdc_gated_scan_workspace_bytes(B, L, ds) bytes, 16-byte aligned.
  * hdc_gated_scan_bwd: dy as y (a gradient of y), dh_last NULL or fp32 [B, ds]; writes dprojs
  *   (columns d dt | d x | d b, row (b, t) at dprojs + b*dp_sb + t*dp_st), dA_log [ds] and,
- *   unless NULL, dh0 fp32 [B, ds].  Sums over b and t are taken in a fixed order.
+ *   unless NULL, dh0 fp32 [B, ds] (not overlapping dh_last).  Sums over b and t are taken in a
+ *   fixed order.
  * hdc_gated_step: one step per sequence from projs rows [B, >=3ds]; h / h_out fp32 [B, ds]
  *   (h_out may be h), reset NULL or uint8 [B].
- * B in [0, 65535], L in [0, 2^30], ds in [1, 2^20].  Pointers need their type's alignment;
- * 16-byte aligned rows take the wide loads.
+ * B in [0, 65535], L in [0, 2^30], ds in [1, 2^20], B * ceil(ds / 32) * ceil(L / 64) < 2^31.
+ * Pointers need their type's alignment; 16-byte aligned rows take the wide loads.  Tiles of a
+ * sequence hand their results on inside the kernel; every wait is bounded (~2 s) and reports 61
+ * through hdc_device_error() (the outputs are then invalid, and later waits of such calls give
+ * up early until the error is cleared).
  */
 int64_t hdc_gated_scan_state_rows(void);
 size_t hdc_gated_scan_workspace_bytes(int64_t B, int64_t L, int64_t ds);
