@@ -33,11 +33,11 @@
 //
 // Why tiles of 64 steps: what a tile keeps between its two halves (a and u: 8 bytes per step and
 // channel) has to stay on the SM, in registers, and 16 to 32 warps of it fill them.  Measured
-// (device time, inputs out of L2, against 6550 GB/s): 8 x 4096 x 1280 bf16 forward 87 us (59%),
-// backward 171 us (52%); 1 x 32768 x 768 bf16 forward 92 us (33%); 1 x 32768 x 64 bf16 15 us;
+// (device time, inputs out of L2, against 6550 GB/s): 8 x 4096 x 1280 bf16 forward 94 us (55%),
+// backward 174 us (51%); 1 x 32768 x 768 bf16 forward 92 us (33%); 1 x 32768 x 64 bf16 15 us;
 // 3 x 1537 x 333 fp32 forward 17 us, backward 29 us.  With many channels the issue slots bind (55 to
 // 65% busy, the rest waits of dependent instructions between 16 warps; without the exchange the
-// forward of the same bytes takes 44 us per 201 MB); with few, each round of tiles waits for the
+// forward takes 44 us per 201 MB); with few, each round of tiles waits for the
 // slowest map before it, some 4 us of a round's 8.  Tried and slower: tickets that run the maps a
 // few hundred tiles ahead of the outputs (inputs read again from L2: 105 us for 91), one word per
 // lane (above), three backward CTAs per SM (spills).
@@ -175,17 +175,14 @@ template <typename T, int V> __device__ __forceinline__ Fv<V> gate(const Fv<V>& 
 template <typename T> __device__ __forceinline__ float rate(float A_log) {
   return sizeof(T) == 4 ? -expf(A_log) : -ex2(1.4426950408889634f * A_log);
 }
-// a = exp(d A); A2 = A log2(e)
-template <typename T, int V> __device__ __forceinline__ Fv<V> decay(const Fv<V>& d, const Fv<V>& A, const Fv<V>& A2) {
+// a = exp(d A), by the library's exp in both types: its error compounds over the steps that a
+// state remembers, and the hardware's 2^x doubles the error of the fp32 states and of dA_log (8 x
+// 4096 x 1280 bf16 forward 87 us with it, 94 without; backward 168 and 174).
+template <int V> __device__ __forceinline__ Fv<V> decay(const Fv<V>& d, const Fv<V>& A) {
+  const Fv<V> l = d * A;
   Fv<V> a;
-  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) a.v[i] = expf(d.v[i] * A.v[i]);
-  } else {
-    const Fv<V> l = d * A2;
-#pragma unroll
-    for (int i = 0; i < V; ++i) a.v[i] = ex2(l.v[i]);
-  }
+  for (int i = 0; i < V; ++i) a.v[i] = expf(l.v[i]);
   return a;
 }
 // sigmoid(x) = 1 / (1 + exp(-x)); bf16: 0 where exp(-x) overflows (x < -88)
@@ -533,7 +530,6 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas<T, W>) gated_scan_fwd_ke
     Fv<V> A;
 #pragma unroll
     for (int i = 0; i < V; ++i) A.v[i] = rate<T>(A_next.v[i]);
-    const Fv<V> A2 = A * all<V>(1.4426950408889634f);
     cp_wait_all();
     __syncwarp();
     if (nv < kRows) {  // steps past the end: dt = -inf (and x = b = 0) is the identity, a = 1, u = 0
@@ -551,7 +547,7 @@ __global__ void __launch_bounds__(kWarps * 32, kFwdCtas<T, W>) gated_scan_fwd_ke
       const Fv<V> dt = ld_words<T, W>(w + r * RB), x = ld_words<T, W>(w + (kRows + r) * RB);
       const Fv<V> b = ld_words<T, W>(w + (2 * kRows + r) * RB);
       const Fv<V> d = gate<T>(dt);
-      a[r] = decay<T>(d, A, A2);
+      a[r] = decay(d, A);
       u[r] = d * (b * x);
       if (RESET && ((cut >> r) & 1)) {
         m.H = u[r];
@@ -665,7 +661,6 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gated_scan_bwd_kernel(c
     Fv<V> A;
 #pragma unroll
     for (int i = 0; i < V; ++i) A.v[i] = rate<T>(A_next.v[i]);
-    const Fv<V> A2 = A * all<V>(1.4426950408889634f);
     cp_wait_all();
     __syncwarp();
     if (nv < kRows) {  // steps past the end are the identity
@@ -684,7 +679,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBwdCtas) gated_scan_bwd_kernel(c
       const Fv<V> dt = ld_words<T, W>(w + r * RB), x = ld_words<T, W>(w + (kRows + r) * RB);
       const Fv<V> b = ld_words<T, W>(w + (2 * kRows + r) * RB);
       d[r] = gate<T>(dt);
-      a[r] = decay<T>(d[r], A, A2);
+      a[r] = decay(d[r], A);
       bx[r] = b * x;
       const Fv<V> u = d[r] * bx[r];
       // the backward map from zero: c = sum of dy_r times the decays up to step r, until a reset
@@ -854,10 +849,11 @@ static int scan_fits(const char* what, int64_t B, int64_t L, int64_t ds) {
   return 0;
 }
 // Words per lane in the forward: in bf16 two (tiles of 128 channels) halve what a tile costs beside
-// its arithmetic (8 x 4096 x 1280: 87 us for 95, 1 x 32768 x 768: 91 for 93); one where much of a
-// wide tile would be empty (the 64 channels of a Block's d_state: half of it), and in fp32, whose
-// exp and log1p take the registers (3 x 1537 x 333: 17 us with one, 19 with two).  The backward
-// holds more per channel (two words spill 500 bytes) and takes one.
+// its arithmetic (before decay() took the library's exp, 8 x 4096 x 1280: 87 us for 95, 1 x 32768 x
+// 768: 91 for 93); one where much of a wide tile would be empty (the 64 channels of a Block's
+// d_state: half of it), and in fp32, whose exp and log1p take the registers (3 x 1537 x 333: 17 us
+// with one, 19 with two).  The backward holds more per channel (two words spill 500 bytes) and
+// takes one.
 static int scan_words(int64_t ds, int es) { return es == 2 && (ds % 128 == 0 || ds > 512) ? 2 : 1; }
 
 template <typename T, int W, bool RESET, int CB, bool BWD>
