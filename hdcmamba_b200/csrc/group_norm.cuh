@@ -15,7 +15,6 @@ struct GnParams {
   float2* stats;   // two passes: (mean, M2) of each slice, [N][slices][G]
   float* sums;     // two passes, gradient: part over the slices, [N][2][C]
   float* gmean;    // and the groups' means of e xh and of e, [N][2][G]
-  void* dw; void* db;
   int N, S, C, G, Cg;
   float eps; int silu;
   int slices, rows;  // two passes: slices per sample, positions per slice
