@@ -33,6 +33,10 @@ SIGNATURES = {
     "hdc_ln_conv_bwd_workspace_bytes": (c_size, [c_i64, c_i64, c_i64]),
     "hdc_ln_conv_bwd": (c_int, [c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_size,
                                 c_i64, c_i64, c_i64, c_vp]),
+    "hdc_ln_conv_train_fwd": (c_int, [c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64,
+                                      c_float, c_vp]),
+    "hdc_ln_conv_train_bwd": (c_int, [c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                      c_vp, c_size, c_i64, c_i64, c_i64, c_vp]),
     "hdc_ssm_chunk_stats": (c_int, [c_int, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp]),
     "hdc_ssm_scan_fwd": (c_int, [c_int, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64,
                                  c_i64, c_vp]),

@@ -31,7 +31,8 @@ namespace hdc {
 
 struct LnConvParams {
   const void* x; const void* nw; const void* nb; const void* cw; const void* cb;
-  const void* halo; void* out; __nv_bfloat16* mean; __nv_bfloat16* rstd;
+  const void* halo; void* out;
+  void* mean; void* rstd; int stat_f32;  // row statistics: bf16, or fp32 where stat_f32
   // sequence parallelism: the halo arrives from another GPU; the CTAs that read it wait
   // (bounded) until *halo_flag reaches *halo_gen (nullptr: no wait)
   const uint32_t* halo_flag; const uint32_t* halo_gen;
@@ -348,8 +349,14 @@ __global__ void __launch_bounds__(512) ln_conv_kernel(LnConvParams p) {
       issue(k + p.nst - 1);
     }
     if (p.mean && warp == 0 && lane < nv) {
-      p.mean[(size_t)b * p.L + t0 + lane] = __float2bfloat16_rn(mean);
-      p.rstd[(size_t)b * p.L + t0 + lane] = __float2bfloat16_rn(rs);
+      const size_t i = (size_t)b * p.L + t0 + lane;
+      if (p.stat_f32) {
+        static_cast<float*>(p.mean)[i] = mean;
+        static_cast<float*>(p.rstd)[i] = rs;
+      } else {
+        static_cast<__nv_bfloat16*>(p.mean)[i] = __float2bfloat16_rn(mean);
+        static_cast<__nv_bfloat16*>(p.rstd)[i] = __float2bfloat16_rn(rs);
+      }
     }
     T* orow = out + (size_t)t0 * p.D + cc * VEC;
     if (nv == R) conv_rows(std::true_type{}, tile_a + cc * 16, orow, R, rs, mrs);
@@ -405,8 +412,8 @@ static int ln_conv_dispatch(LnConvParams p, int64_t B, cudaStream_t stream) {
 using namespace hdc;
 
 static int ln_conv_fwd(int dtype, const void* x, const void* norm_w, const void* norm_b, const void* conv_w,
-                       const void* conv_b, const void* halo, void* out, void* mean, void* rstd, int64_t B,
-                       int64_t L, int64_t D, float eps, int act, const uint32_t* halo_flag,
+                       const void* conv_b, const void* halo, void* out, void* mean, void* rstd, int stat_f32,
+                       int64_t B, int64_t L, int64_t D, float eps, int act, const uint32_t* halo_flag,
                        const uint32_t* halo_gen, hdc_stream_t stream) {
   if (dtype != HDC_F32 && dtype != HDC_BF16) return fail(HDC_E_DTYPE, "ln_conv: dtype %d", dtype);
   if (!x || !norm_w || !norm_b || !conv_w || !conv_b || !out) return fail(HDC_E_NULL, "ln_conv: null pointer");
@@ -422,7 +429,7 @@ static int ln_conv_fwd(int dtype, const void* x, const void* norm_w, const void*
   if (x == out) return fail(HDC_E_SHAPE, "ln_conv: out must not alias x");
   LnConvParams p{};
   p.x = x; p.nw = norm_w; p.nb = norm_b; p.cw = conv_w; p.cb = conv_b; p.halo = halo; p.out = out;
-  p.mean = static_cast<__nv_bfloat16*>(mean); p.rstd = static_cast<__nv_bfloat16*>(rstd);
+  p.mean = mean; p.rstd = rstd; p.stat_f32 = stat_f32;
   p.L = (int)L; p.D = (int)D; p.eps = eps; p.act = act;
   p.halo_flag = halo_flag; p.halo_gen = halo_gen;
   auto s = reinterpret_cast<cudaStream_t>(stream);
@@ -433,8 +440,18 @@ extern "C" int hdc_ln_conv_fwd(int dtype, const void* x, const void* norm_w, con
                                const void* conv_w, const void* conv_b, const void* halo, void* out,
                                void* mean, void* rstd, int64_t B, int64_t L, int64_t D, float eps,
                                int act, hdc_stream_t stream) {
-  return ln_conv_fwd(dtype, x, norm_w, norm_b, conv_w, conv_b, halo, out, mean, rstd, B, L, D, eps, act, nullptr,
+  return ln_conv_fwd(dtype, x, norm_w, norm_b, conv_w, conv_b, halo, out, mean, rstd, 0, B, L, D, eps, act, nullptr,
                      nullptr, stream);
+}
+
+extern "C" int hdc_ln_conv_train_fwd(int dtype, const void* x, const void* norm_w, const void* norm_b,
+                                     const void* conv_w, const void* conv_b, void* out, float* mean, float* rstd,
+                                     int64_t B, int64_t L, int64_t D, float eps, hdc_stream_t stream) {
+  if (!mean || !rstd) return fail(HDC_E_NULL, "ln_conv_train: null pointer");
+  if (((reinterpret_cast<uintptr_t>(mean) | reinterpret_cast<uintptr_t>(rstd)) & 3u) != 0)
+    return fail(HDC_E_ALIGN, "ln_conv_train: mean or rstd is not aligned to its type");
+  return ln_conv_fwd(dtype, x, norm_w, norm_b, conv_w, conv_b, nullptr, out, mean, rstd, 1, B, L, D, eps,
+                     HDC_ACT_NONE, nullptr, nullptr, stream);
 }
 
 extern "C" int hdc_ln_conv_fwd_halo_flag(int dtype, const void* x, const void* norm_w, const void* norm_b,
@@ -443,6 +460,6 @@ extern "C" int hdc_ln_conv_fwd_halo_flag(int dtype, const void* x, const void* n
                                          int act, const uint32_t* halo_flag, const uint32_t* halo_gen,
                                          hdc_stream_t stream) {
   if (!halo || !halo_flag || !halo_gen) return fail(HDC_E_NULL, "ln_conv_halo_flag: halo, flag and gen required");
-  return ln_conv_fwd(dtype, x, norm_w, norm_b, conv_w, conv_b, halo, out, mean, rstd, B, L, D, eps, act, halo_flag,
+  return ln_conv_fwd(dtype, x, norm_w, norm_b, conv_w, conv_b, halo, out, mean, rstd, 0, B, L, D, eps, act, halo_flag,
                      halo_gen, stream);
 }

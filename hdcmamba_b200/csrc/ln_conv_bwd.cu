@@ -8,6 +8,13 @@
 //   d_nw     = sum_t dn xhat,  d_nb = sum_t dn,  d_cb = sum_t go[t]
 //   d_cw[k]  = sum_t go[t] xhat[t-3+k] nw        (rows t-3+k < 0 contribute nothing, and
 //                                                 the norm bias is not part of the term)
+// The training form (hdc_ln_conv_train_bwd) is the derivative of the forward itself, on fp32
+// mean / rstd.  The normalised rows are n[t] = xhat[t] nw + nb, nb before the sequence, so what
+// the formulas above leave out is the same for every row and comes from d_cb = sum_t go[t]:
+//   d_cw[k] = sum_t go[t] n[t-3+k] = (d_cw[k] above) + nb d_cb
+//   d_nb    = sum_{t >= -3} dn[t]  = d_cb (cw0 + cw1 + cw2 + cw3)
+// (the rows before the sequence have xhat = 0 and no dx, so d_nw and dx have nothing missing).  The
+// kernel that adds up the CTAs' sums applies both in fp32; the rest is shared.
 // Schedule (HBM-bound: read go, x; write dx):
 //   * one CTA walks a contiguous L-segment of one batch row; thread g owns channels
 //     [4g, 4g+4), loaded / stored as one 8-byte (bf16) or 16-byte (fp32) vector;
@@ -27,10 +34,15 @@
 namespace hdc {
 
 struct LnConvBwdParams {
-  const void* go; const void* x; const __nv_bfloat16* mean; const __nv_bfloat16* rstd;
+  const void* go; const void* x; const void* mean; const void* rstd; int stat_f32;
   const void* nw; const void* cw; void* dx; float* part;
   int L, D, seg_len, segs_per_b;
 };
+
+// row statistic i: bf16, or fp32 where the training form keeps it so
+__device__ __forceinline__ float ld_stat(const void* p, int f32, size_t i) {
+  return f32 ? static_cast<const float*>(p)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
 
 template <typename T>
 __device__ __forceinline__ void ld4(const T* p, float* f);
@@ -75,8 +87,9 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_kernel(LnConvBwdParams p) {
   const T* go = static_cast<const T*>(p.go) + (size_t)b * p.L * rowD + cc;
   const T* x = static_cast<const T*>(p.x) + (size_t)b * p.L * rowD + cc;
   T* dx = static_cast<T*>(p.dx) + (size_t)b * p.L * rowD + cc;
-  const __nv_bfloat16* mean = p.mean + (size_t)b * p.L;
-  const __nv_bfloat16* rstd = p.rstd + (size_t)b * p.L;
+  const size_t stat0 = (size_t)b * p.L;
+  auto mean = [&](int t) { return ld_stat(p.mean, p.stat_f32, stat0 + t); };
+  auto rstd = [&](int t) { return ld_stat(p.rstd, p.stat_f32, stat0 + t); };
   const float invD = 1.0f / (float)p.D;
 
   float nw[4], cw[4][4];  // cw[e][k]
@@ -92,7 +105,7 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_kernel(LnConvBwdParams p) {
     if (act && t >= 0) {
       float v[4];
       ld4<T>(x + (size_t)t * rowD, v);
-      const float m = __bfloat162float(mean[t]), r = __bfloat162float(rstd[t]);
+      const float m = mean(t), r = rstd(t);
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] = (v[e] - m) * r * nw[e];
     } else {
@@ -121,7 +134,7 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_kernel(LnConvBwdParams p) {
       if (t < l1) {
         load_go(t + 3, G[(u + 3) & 3]);
         float v[4];
-        const float m = __bfloat162float(mean[t]), r = __bfloat162float(rstd[t]);
+        const float m = mean(t), r = rstd(t);
         rs[u] = r;
         if (act) ld4<T>(x + (size_t)t * rowD, v);
         else v[0] = v[1] = v[2] = v[3] = 0.f;
@@ -275,8 +288,9 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_staged_kernel(LnConvBwdParams
   const T* gob = static_cast<const T*>(p.go) + (size_t)b * p.L * rowD;
   const T* xb = static_cast<const T*>(p.x) + (size_t)b * p.L * rowD;
   T* dx = static_cast<T*>(p.dx) + (size_t)b * p.L * rowD + cc;
-  const __nv_bfloat16* mean = p.mean + (size_t)b * p.L;
-  const __nv_bfloat16* rstd = p.rstd + (size_t)b * p.L;
+  const size_t stat0 = (size_t)b * p.L;
+  auto mean = [&](int t) { return ld_stat(p.mean, p.stat_f32, stat0 + t); };
+  auto rstd = [&](int t) { return ld_stat(p.rstd, p.stat_f32, stat0 + t); };
   const float invD = 1.0f / (float)p.D;
   const int ntiles = (l1 - l0 + TR - 1) / TR;
 
@@ -328,7 +342,7 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_staged_kernel(LnConvBwdParams
     if (t >= 0) {
       uint64_t v[2];
       ldg4<T>(xb + (size_t)t * rowD + cc, v);
-      const float m = __bfloat162float(mean[t]), rr = __bfloat162float(rstd[t]);
+      const float m = mean(t), rr = rstd(t);
       const uint64_t r2 = f2_make(rr, rr), mr2 = f2_make(-m * rr, -m * rr);
 #pragma unroll
       for (int j = 0; j < 2; ++j) X[r + 1][j] = f2_mul(f2_fma(v[j], r2, mr2), nw2[j]);
@@ -347,8 +361,8 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_staged_kernel(LnConvBwdParams
     // row statistics of the tile: lane i holds row i's (TR <= 32)
     float mt = 0.f, rt = 0.f;
     if (lane < nrows) {
-      mt = __bfloat162float(mean[t0 + lane]);
-      rt = __bfloat162float(rstd[t0 + lane]);
+      mt = mean(t0 + lane);
+      rt = rstd(t0 + lane);
     }
     // a timed-out wait ends the loop for every warp together at the group barrier below
     const bool got = mbar_wait_warp(&bars[st], (uint32_t)((k / NST) & 1), 34);
@@ -472,16 +486,27 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_staged_kernel(LnConvBwdParams
 }
 
 // sums the per-CTA partials [nseg][7][D] in CTA order and casts to T:
-// dnw [D], dnb [D], dcb [D], dcw [D][4]
+// dnw [D], dnb [D], dcb [D], dcw [D][4]; nb, cw: the training form's terms (nullptr: without them)
 template <typename T>
-__global__ void ln_conv_bwd_reduce_kernel(const float* part, int nseg, int D, T* dnw, T* dnb, T* dcw, T* dcb) {
+__global__ void ln_conv_bwd_reduce_kernel(const float* part, int nseg, int D, const T* nb, const T* cw, T* dnw, T* dnb,
+                                          T* dcw, T* dcb) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;  // (row of 7, channel)
   if (i >= 7 * D) return;
   const int k = i / D, d = i - k * D;
-  float s = 0.f;
-  // 16 loads in flight per thread (few threads: 7 D of them); the adds stay in CTA order
+  auto sum_row = [&](int row) {
+    float s = 0.f;
+    // 16 loads in flight per thread (few threads: 7 D of them); the adds stay in CTA order
 #pragma unroll 16
-  for (int c = 0; c < nseg; ++c) s += part[(size_t)c * 7 * D + i];
+    for (int c = 0; c < nseg; ++c) s += part[((size_t)c * 7 + row) * D + d];
+    return s;
+  };
+  float s = sum_row(nb && k == 1 ? 2 : k);
+  if (nb && k == 1) {
+    const T* w = cw + (size_t)d * 4;
+    s *= (to_f(w[0]) + to_f(w[1])) + (to_f(w[2]) + to_f(w[3]));
+  } else if (nb && k >= 3) {
+    s = fmaf(to_f(nb[d]), sum_row(2), s);
+  }
   const T v = from_f<T>(s);
   if (k == 0) dnw[d] = v;
   else if (k == 1) dnb[d] = v;
@@ -516,10 +541,11 @@ extern "C" size_t hdc_ln_conv_bwd_workspace_bytes(int64_t B, int64_t L, int64_t 
   return (size_t)B * spb * 7 * D * sizeof(float);
 }
 
-extern "C" int hdc_ln_conv_bwd(int dtype, const void* grad_out, const void* x, const void* mean, const void* rstd,
-                               const void* norm_w, const void* conv_w, void* dx, void* dnorm_w, void* dnorm_b,
-                               void* dconv_w, void* dconv_b, void* workspace, size_t workspace_bytes, int64_t B,
-                               int64_t L, int64_t D, hdc_stream_t stream) {
+// norm_b: the training form (fp32 mean and rstd); nullptr: the reference's formulas (bf16)
+static int ln_conv_bwd(int dtype, const void* grad_out, const void* x, const void* mean, const void* rstd,
+                       const void* norm_w, const void* norm_b, const void* conv_w, void* dx, void* dnorm_w,
+                       void* dnorm_b, void* dconv_w, void* dconv_b, void* workspace, size_t workspace_bytes, int64_t B,
+                       int64_t L, int64_t D, hdc_stream_t stream) {
   if (dtype != HDC_F32 && dtype != HDC_BF16) return fail(HDC_E_DTYPE, "ln_conv_bwd: dtype %d", dtype);
   if (!grad_out || !x || !mean || !rstd || !norm_w || !conv_w || !dx || !dnorm_w || !dnorm_b || !dconv_w ||
       !dconv_b || !workspace)
@@ -533,8 +559,8 @@ extern "C" int hdc_ln_conv_bwd(int dtype, const void* grad_out, const void* x, c
       !aligned16(workspace))
     return fail(HDC_E_ALIGN, "ln_conv_bwd: pointers must be 16-byte aligned");
   LnConvBwdParams p{};
-  p.go = grad_out; p.x = x; p.mean = static_cast<const __nv_bfloat16*>(mean);
-  p.rstd = static_cast<const __nv_bfloat16*>(rstd); p.nw = norm_w; p.cw = conv_w; p.dx = dx;
+  p.go = grad_out; p.x = x; p.mean = mean; p.rstd = rstd; p.stat_f32 = norm_b != nullptr;
+  p.nw = norm_w; p.cw = conv_w; p.dx = dx;
   p.part = static_cast<float*>(workspace); p.L = (int)L; p.D = (int)D;
   bwd_plan(B, L, D, &p.seg_len, &p.segs_per_b);
   const int nseg = (int)(B * p.segs_per_b);
@@ -563,16 +589,38 @@ extern "C" int hdc_ln_conv_bwd(int dtype, const void* grad_out, const void* x, c
     else go(ln_conv_bwd_staged_kernel<T, 2, 4>);
     return launch_status("ln_conv_bwd_kernel");
   };
+  auto reduce = [&](auto tag) {
+    using T = decltype(tag);
+    ln_conv_bwd_reduce_kernel<T><<<rgrid, 256, 0, s>>>(
+        p.part, nseg, (int)D, static_cast<const T*>(norm_b), static_cast<const T*>(conv_w), static_cast<T*>(dnorm_w),
+        static_cast<T*>(dnorm_b), static_cast<T*>(dconv_w), static_cast<T*>(dconv_b));
+  };
   if (dtype == HDC_F32) {
     if (int e = launch_main(float{})) return e;
-    ln_conv_bwd_reduce_kernel<float><<<rgrid, 256, 0, s>>>(p.part, nseg, (int)D, static_cast<float*>(dnorm_w),
-                                                           static_cast<float*>(dnorm_b), static_cast<float*>(dconv_w),
-                                                           static_cast<float*>(dconv_b));
+    reduce(float{});
   } else {
     if (int e = launch_main(__nv_bfloat16{})) return e;
-    ln_conv_bwd_reduce_kernel<__nv_bfloat16><<<rgrid, 256, 0, s>>>(
-        p.part, nseg, (int)D, static_cast<__nv_bfloat16*>(dnorm_w), static_cast<__nv_bfloat16*>(dnorm_b),
-        static_cast<__nv_bfloat16*>(dconv_w), static_cast<__nv_bfloat16*>(dconv_b));
+    reduce(__nv_bfloat16{});
   }
   return launch_status("ln_conv_bwd_reduce_kernel");
+}
+
+extern "C" int hdc_ln_conv_bwd(int dtype, const void* grad_out, const void* x, const void* mean, const void* rstd,
+                               const void* norm_w, const void* conv_w, void* dx, void* dnorm_w, void* dnorm_b,
+                               void* dconv_w, void* dconv_b, void* workspace, size_t workspace_bytes, int64_t B,
+                               int64_t L, int64_t D, hdc_stream_t stream) {
+  return ln_conv_bwd(dtype, grad_out, x, mean, rstd, norm_w, nullptr, conv_w, dx, dnorm_w, dnorm_b, dconv_w, dconv_b,
+                     workspace, workspace_bytes, B, L, D, stream);
+}
+
+extern "C" int hdc_ln_conv_train_bwd(int dtype, const void* grad_out, const void* x, const float* mean,
+                                     const float* rstd, const void* norm_w, const void* norm_b, const void* conv_w,
+                                     void* dx, void* dnorm_w, void* dnorm_b, void* dconv_w, void* dconv_b,
+                                     void* workspace, size_t workspace_bytes, int64_t B, int64_t L, int64_t D,
+                                     hdc_stream_t stream) {
+  if (!norm_b) return fail(HDC_E_NULL, "ln_conv_train_bwd: null pointer");
+  if (!aligned16(norm_b) || ((reinterpret_cast<uintptr_t>(mean) | reinterpret_cast<uintptr_t>(rstd)) & 3u) != 0)
+    return fail(HDC_E_ALIGN, "ln_conv_train_bwd: norm_b must be 16-byte aligned, mean and rstd aligned to their type");
+  return ln_conv_bwd(dtype, grad_out, x, mean, rstd, norm_w, norm_b, conv_w, dx, dnorm_w, dnorm_b, dconv_w, dconv_b,
+                     workspace, workspace_bytes, B, L, D, stream);
 }

@@ -111,6 +111,50 @@ def ln_conv_bwd(grad_out, x, mean, rstd, norm_w, conv_w):
     return dx, dnw, dnb, dcw, dcb
 
 
+def _ln_conv_params(x, *params):
+    """Parameters in x's type, contiguous (conv weights [D, 4] or [D, 1, 4] as [D, 4])."""
+    D = x.shape[2]
+    return tuple((p.reshape(D, 4) if p.dim() > 1 else p).to(x.dtype).contiguous() for p in params)
+
+
+def ln_conv_train(x, norm_w, norm_b, conv_w, conv_b, eps=1e-5):
+    """``ln_conv`` without activation for training a layer of one's own
+    (hdc_ln_conv_train_fwd): returns (out, mean, rstd), the row statistics in fp32 [B, L]."""
+    _cuda(x, norm_w, norm_b, conv_w, conv_b)
+    dt = _code(x)
+    B, L, D = x.shape
+    x = x.contiguous()
+    nw, nb, cw, cb = _ln_conv_params(x, norm_w, norm_b, conv_w, conv_b)
+    out = torch.empty_like(x)
+    mean = torch.empty(B, L, device=x.device, dtype=torch.float32)
+    rstd = torch.empty(B, L, device=x.device, dtype=torch.float32)
+    _lib.call("hdc_ln_conv_train_fwd", dt, _p(x), _p(nw), _p(nb), _p(cw), _p(cb), _p(out), _p(mean), _p(rstd),
+              B, L, D, float(eps), _stream(x))
+    return out, mean, rstd
+
+
+def ln_conv_train_bwd(grad_out, x, mean, rstd, norm_w, norm_b, conv_w):
+    """The derivative of ``ln_conv_train`` (hdc_ln_conv_train_bwd), the norm bias and the rows
+    before the sequence included.  Returns (dx, d_norm_w, d_norm_b, d_conv_w [D, 4], d_conv_b)
+    in x.dtype."""
+    _cuda(grad_out, x, mean, rstd, norm_w, norm_b, conv_w)
+    dt = _code(x)
+    B, L, D = x.shape
+    _same_dtype(x, grad_out)
+    if grad_out.shape != x.shape:
+        raise ValueError(f"grad_out {list(grad_out.shape)} must have x's shape {list(x.shape)}")
+    _f32_state(mean, (B, L), "mean")
+    _f32_state(rstd, (B, L), "rstd")
+    grad_out, x = grad_out.contiguous(), x.contiguous()
+    nw, nb, cw = _ln_conv_params(x, norm_w, norm_b, conv_w)
+    dx, dnw, dnb, dcw, dcb = (torch.empty_like(t) for t in (x, nw, nw, cw, nw))
+    ws = torch.empty(max(int(_lib.load().hdc_ln_conv_bwd_workspace_bytes(B, L, D)), 16), device=x.device,
+                     dtype=torch.uint8)
+    _lib.call("hdc_ln_conv_train_bwd", dt, _p(grad_out), _p(x), _p(mean), _p(rstd), _p(nw), _p(nb), _p(cw), _p(dx),
+              _p(dnw), _p(dnb), _p(dcw), _p(dcb), _p(ws), ws.numel(), B, L, D, _stream(x))
+    return dx, dnw, dnb, dcw, dcb
+
+
 def _row_view(t, what):
     """(batch stride, row stride) of a [B, L, cols] view whose last dim is unit-stride."""
     if t.dim() != 3 or t.stride(2) != 1:

@@ -4,7 +4,10 @@ The Block's SSM and slot kernels follow the reference's forward and have no grad
 (hdcmamba/model.py:175-295).  ``gated_scan`` and ``group_norm_act`` are the operators to
 train such a layer with: the SSM's gates as one exact recurrence over the sequence, and the
 GroupNorm of each head with SiLU, both with hand-written backward kernels.
-``GatedRecurrentBlock`` joins them with the Block's trainable LayerNorm + conv:
+``GatedRecurrentBlock`` joins them with the Block's LayerNorm + conv.  That one's gradient here
+(``norm_conv1d``) is the derivative of its forward; ``fused_norm_conv1d_trainable`` keeps the
+reference's formulas, which leave the norm bias and the rows before the sequence out of two
+gradients (hdcmamba/model.py:74-124):
 
     blk = GatedRecurrentBlock(d_model=768, num_heads=12).cuda().bfloat16()
     loss = blk(x, reset=starts).float().square().mean(); loss.backward()   # training
@@ -20,16 +23,44 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import ops
-from .model import _require_cuda, fused_norm_conv1d_trainable
+from .model import _require_cuda
 
-__all__ = ["gated_scan", "group_norm_act", "GatedScanFunction", "GroupNormActFunction", "GatedRecurrentBlock",
-           "RecurrentState"]
+__all__ = ["norm_conv1d", "gated_scan", "group_norm_act", "NormConv1dFunction", "GatedScanFunction",
+           "GroupNormActFunction", "GatedRecurrentBlock", "RecurrentState"]
 
 
 def _first_order_only():
     """Gradients of the gradients are not implemented: an error rather than missing terms."""
     if torch.is_grad_enabled():  # only with create_graph=True
-        raise RuntimeError("hdcmamba_b200: gated_scan and group_norm_act are differentiable once (create_graph=False)")
+        raise RuntimeError("hdcmamba_b200: norm_conv1d, gated_scan and group_norm_act are differentiable once (create_graph=False)")
+
+
+class NormConv1dFunction(torch.autograd.Function):
+    """(x, norm_w, norm_b, conv_w [D, 4], conv_b, eps) -> LayerNorm + causal depthwise conv1d
+    (hdc_ln_conv_train_fwd / hdc_ln_conv_train_bwd); all in x's type."""
+
+    @staticmethod
+    def forward(ctx, x, norm_w, norm_b, conv_w, conv_b, eps):
+        out, mean, rstd = ops.ln_conv_train(x, norm_w, norm_b, conv_w, conv_b, eps)
+        ctx.save_for_backward(x, norm_w, norm_b, conv_w, mean, rstd)
+        return out
+
+    @staticmethod
+    def backward(ctx, dy):
+        _first_order_only()
+        x, norm_w, norm_b, conv_w, mean, rstd = ctx.saved_tensors
+        return (*ops.ln_conv_train_bwd(dy, x, mean, rstd, norm_w, norm_b, conv_w), None)
+
+
+def norm_conv1d(x, norm, conv):
+    """Differentiable LayerNorm + causal depthwise conv1d (width 4) of x [B, L, D] with the
+    parameters of an ``nn.LayerNorm`` and an ``nn.Conv1d``; rows before the sequence are zeros
+    before the norm."""
+    _require_cuda(x)
+    params = [p.to(x.dtype) for p in (norm.weight, norm.bias, conv.weight.squeeze(1), conv.bias)]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params)):
+        return NormConv1dFunction.apply(x, *params, norm.eps)
+    return ops.ln_conv(x, *params, norm.eps)
 
 
 class GatedScanFunction(torch.autograd.Function):
@@ -145,7 +176,7 @@ class GatedRecurrentBlock(nn.Module):
                               "silu").reshape(y.shape)
 
     def _run(self, x, reset, h0):
-        x_conv = fused_norm_conv1d_trainable(x, self.norm, self.conv1d)
+        x_conv = norm_conv1d(x, self.norm, self.conv1d)
         y, h = gated_scan(self.in_proj(x_conv), self.A_log, self.d_state, h0=h0, reset=reset)
         return x + self.out_proj(self._heads(y)), h
 

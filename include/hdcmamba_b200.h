@@ -97,6 +97,23 @@ int hdc_ln_conv_bwd(int dtype, const void* grad_out, const void* x, const void* 
                     int64_t L, int64_t D, hdc_stream_t stream);
 
 /*
+ * LayerNorm + conv for training a layer of one's own: hdc_ln_conv_fwd without activation and halo,
+ * with fp32 row statistics mean / rstd [B, L], and the derivative of that forward.  Unlike
+ * hdc_ln_conv_bwd, the conv-weight gradient has the norm bias's part, and the conv-weight and
+ * norm-bias gradients have that of the three rows before the sequence (whose LayerNorm is norm_b).
+ * Otherwise as hdc_ln_conv_fwd and hdc_ln_conv_bwd (sizes, alignment, workspace, sums in a fixed
+ * order, gradients stored in dtype); norm_b 16-byte aligned.
+ */
+int hdc_ln_conv_train_fwd(int dtype, const void* x, const void* norm_w, const void* norm_b,
+                          const void* conv_w, const void* conv_b, void* out, float* mean, float* rstd,
+                          int64_t B, int64_t L, int64_t D, float eps, hdc_stream_t stream);
+int hdc_ln_conv_train_bwd(int dtype, const void* grad_out, const void* x, const float* mean,
+                          const float* rstd, const void* norm_w, const void* norm_b, const void* conv_w,
+                          void* dx, void* dnorm_w, void* dnorm_b, void* dconv_w, void* dconv_b,
+                          void* workspace, size_t workspace_bytes, int64_t B, int64_t L, int64_t D,
+                          hdc_stream_t stream);
+
+/*
  * Diagonal SSM chunk statistics (pass 1 of the chunked scan).
  * Replaces _ssm_intra_v2's last_state / chunk_decay outputs (hdcmamba/model.py:175-198,
  * launched at 345-350).  For batch b and chunk n (C steps), per channel j < ds:
