@@ -73,6 +73,7 @@ SIGNATURES = {
     "hdc_slot_step": (c_int, [c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                               c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp]),
     "hdc_gated_scan_state_rows": (c_i64, []),
+    "hdc_gated_scan_wait_limit": (c_int, [ctypes.c_uint64]),
     "hdc_gated_scan_workspace_bytes": (c_size, [c_i64, c_i64, c_i64]),
     "hdc_gated_scan_fwd": (c_int, [c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp,
                                    c_vp, c_size, c_i64, c_i64, c_i64, c_vp]),

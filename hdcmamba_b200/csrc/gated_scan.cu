@@ -25,7 +25,9 @@
 // The gradient is the same scan from the end, of the maps c -> a (dy + c), on the same tiles;
 // the states inside a tile are scanned again from the one that the forward saved at its start.
 // CTAs take tiles by ticket, time-major: a tile waits only for tiles with smaller tickets,
-// which running CTAs hold, so the waits end (they are bounded all the same).  An entry is one
+// which running CTAs hold, so the waits end.  They are bounded all the same: a call whose wait
+// runs out ends soon (a word of its workspace says so to its other waits), reports it, and what
+// the missing entry would have reached is NaN; later calls know nothing of it.  An entry is one
 // 64-bit word per channel, (P, H); the workspace is set to all ones before the launch, which
 // no published P is, so the word is its own flag.  The next tile is in flight (cp.async)
 // while one is computed.
@@ -72,6 +74,8 @@ struct ScanParams {
   int NG;           // channel groups of all batches
   int64_t ntiles;   // NG * NT
   unsigned* ticket;  // NULL: a single tile in time, taken by block index, nothing published
+                     // ticket[1]: all ones, 0 once a wait of this call has run out
+  uint64_t wait_ns;  // limit of a wait
   uint64_t* ent;    // [NG][NT + spans + links][CW] published entries
   int nent;         // entries per group
   uint64_t div_NG, div_nch;  // 2^64 / d rounded up (0: d = 1)
@@ -283,13 +287,13 @@ template <int V> __device__ __forceinline__ void ld_entry(const uint64_t* e, uin
       asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(w[i]), "=l"(w[i + 1]) : "l"(e + i) : "memory");
   }
 }
-// Compose n in 1..4 neighbouring entries, waited for (some 2 s, then error 61; what is missing
-// then counts as zeros).  e: entry 0 of them.  While an entry is missing, one word of each is
+// Compose n in 1..4 neighbouring entries, waited for (up to p.wait_ns, then error 61; what is
+// missing then is NaN).  e: entry 0 of them.  While an entry is missing, one word of each is
 // polled, not the whole entries.
-constexpr long long kWaitCycles = 4000000000ll;
-template <bool RESET, int V> __device__ __forceinline__ Map<V> take(const uint64_t* e, int n, int lane) {
+template <bool RESET, int V>
+__device__ __forceinline__ Map<V> take(const ScanParams& p, const uint64_t* e, int n, int lane) {
   uint64_t w[4][V];
-  long long t0 = 0;
+  uint64_t t0 = 0;
   while (true) {
     bool ok = true;
 #pragma unroll
@@ -300,24 +304,27 @@ template <bool RESET, int V> __device__ __forceinline__ Map<V> take(const uint64
 #pragma unroll
       for (int i = 0; i < V; ++i) ok = ok && (k >= n || (uint32_t)w[k][i] != kUnset);
     if (__all_sync(0xffffffffu, ok)) break;
-    if (t0 == 0) t0 = clock64();
+    if (t0 == 0) t0 = globaltimer_ns();
     bool late = false;
     if (lane < n) {
       uint64_t one[1];
       do {
         __nanosleep(32);
         ld_entry<1>(e + lane * 32 * V, one);
-        // a wait that has run out elsewhere ends this one too, so that the kernel ends soon
-        late = clock64() - t0 > kWaitCycles || *static_cast<volatile int*>(&g_dev_error) == 61;
+        // a wait of this call that has run out elsewhere ends this one too, so that it ends soon
+        late = globaltimer_ns() - t0 >= p.wait_ns || *static_cast<volatile unsigned*>(p.ticket + 1) == 0;
       } while ((uint32_t)one[0] == kUnset && !late);
     }
     if (__any_sync(0xffffffffu, late)) {
-      if (lane == 0) atomicCAS(&g_dev_error, 0, 61);
+      if (lane == 0) {
+        atomicExch(p.ticket + 1, 0u);
+        atomicCAS(&g_dev_error, 0, 61);
+      }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          if ((uint32_t)w[k][i] == kUnset) w[k][i] = 0;
+          if ((uint32_t)w[k][i] == kUnset) w[k][i] = 0x7fffffff7fffffffull;
       break;
     }
   }
@@ -371,7 +378,7 @@ __device__ __forceinline__ Fv<V> enter_tile(const ScanParams& p, int g, int q, c
   const int from = warp % 4 * 4, n = min(4, (warp < 4 ? in_link : in_span) - from);
   if (n > 0) {
     const uint64_t* e = warp < 4 ? spans + (int64_t)(link * kSpan + from) * CW : ent + (int64_t)(span * kSpan + from) * CW;
-    st_map<V>(pre + warp * pre_stride, lane, take<RESET, V>(e, n, lane));
+    st_map<V>(pre + warp * pre_stride, lane, take<RESET, V>(p, e, n, lane));
   }
   if (in_span == kSpan - 1 && more && warp >= 4) {
     // the end of a span: its map is published before this tile waits for earlier spans, or
@@ -384,7 +391,7 @@ __device__ __forceinline__ Fv<V> enter_tile(const ScanParams& p, int g, int q, c
       publish<V>(spans + (int64_t)span * CW, lane, then<RESET>(m, tile_map()));
     }
   }
-  if (link > 0) h = take<false, V>(links + (int64_t)(link - 1) * CW, 1, lane).H;
+  if (link > 0) h = take<false, V>(p, links + (int64_t)(link - 1) * CW, 1, lane).H;
   __syncthreads();
   const int outer = (in_link + 3) / 4, inner = (in_span + 3) / 4;
   for (int k = 0; k < outer; ++k) h = apply<RESET>(ld_map<V>(pre + k * pre_stride, lane), h);
@@ -817,13 +824,17 @@ static int64_t scan_entries(int64_t NT) {
 }
 // channels rounded up to the widest tile
 static int64_t scan_pad(int64_t ds) { return (ds + 127) / 128 * 128; }
-// the ticket, then the entries
+// the ticket and the word beside it (16 bytes), then the entries
 static size_t scan_ws(int64_t B, int64_t L, int64_t ds) {
   const int64_t NT = tiles_in_time(L);
   if (B < 1 || ds < 1 || NT < 2) return 0;
   return 16 + (size_t)(B * scan_pad(ds)) * scan_entries(NT) * 8;
 }
+constexpr uint64_t kMostWaitNs = 2000000000ull;
+static std::atomic<uint64_t> g_wait_ns{kMostWaitNs};
+
 static void scan_plan(ScanParams& p, int CW, void* ws) {
+  p.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
   p.CW = CW;
   p.nch = (p.ds + CW - 1) / CW;
   p.NG = p.B * p.nch;
@@ -895,6 +906,14 @@ static void scan_launch(const ScanParams& p, int dtype, int W, int cb, cudaStrea
 using namespace hdc;
 
 extern "C" int64_t hdc_gated_scan_state_rows(void) { return kStateRows; }
+
+extern "C" int hdc_gated_scan_wait_limit(uint64_t ns) {
+  if (ns > kMostWaitNs)
+    return fail(HDC_E_SHAPE, "gated_scan_wait_limit: %llu ns (at most %llu)", (unsigned long long)ns,
+                (unsigned long long)kMostWaitNs);
+  g_wait_ns.store(ns, std::memory_order_relaxed);
+  return HDC_OK;
+}
 
 extern "C" int hdc_gated_scan_fwd(int dtype, int a_dtype, const void* projs, int64_t proj_sb, int64_t proj_st,
                                   const void* A_log, const float* h0, const uint8_t* reset, void* y, int64_t y_sb,

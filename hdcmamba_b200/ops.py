@@ -47,6 +47,17 @@ def _same_dtype(ref, *ts):
             raise TypeError(f"hdcmamba_b200: dtype mismatch ({t.dtype} vs {ref.dtype})")
 
 
+def check_device():
+    """Synchronise the current device and raise HdcError if a bounded wait inside a kernel has run
+    out since the last check (the error is cleared): the outputs of the call that waited are
+    invalid.  Kernels report such a wait on the device only, so a training loop calls this once
+    in a while (say with each checkpoint)."""
+    torch.cuda.synchronize()
+    code = _lib.load().hdc_device_error(1)
+    if code != 0:
+        raise _lib.HdcError(f"a bounded wait inside a kernel has run out (code {code}); the outputs of that call are invalid")
+
+
 # ------------------------------------------------------------------ LN + conv
 def ln_conv(x, norm_w, norm_b, conv_w, conv_b, eps=1e-5, act="none", halo=None, stats=False, halo_flag=None):
     """LayerNorm + causal depthwise conv1d (width 4), optional SiLU.
@@ -600,7 +611,8 @@ def gated_scan(projs, A_log, d_state, h0=None, reset=None, out=None, return_stat
     h0: optional fp32 [B, d_state] state before the first step.  reset: optional bool [B, L];
     a true step starts from a zero state.  out: optional [B, L, d_state] view (unit column
     stride).  Returns (y in projs.dtype, h_last fp32 [B, d_state]) and, if ``return_states``,
-    the states that ``gated_scan_bwd`` needs.  For autograd use ``recurrent.gated_scan``."""
+    the states that ``gated_scan_bwd`` needs.  For autograd use ``recurrent.gated_scan``.
+    Waits between the tiles of a sequence are bounded: see ``check_device``."""
     _cuda(projs, A_log, h0, reset, out)
     dt = _code(projs)
     if projs.dim() != 3:

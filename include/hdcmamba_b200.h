@@ -398,11 +398,13 @@ int hdc_slot_step(int dtype, const void* q, const void* k, const void* v, const 
  *   (h_out may be h), reset NULL or uint8 [B].
  * B in [0, 65535], L in [0, 2^30], ds in [1, 2^20], B * ceil(ds / 32) * ceil(L / 64) < 2^31.
  * Pointers need their type's alignment; 16-byte aligned rows take the wide loads.  Tiles of a
- * sequence hand their results on inside the kernel; every wait is bounded (~2 s) and reports 61
- * through hdc_device_error() (the outputs are then invalid, and later waits of such calls give
- * up early until the error is cleared).
+ * sequence hand their results on inside the kernel; every wait is bounded.  A call whose wait runs
+ * out reports 61 through hdc_device_error(), and what the missing result would have reached is NaN;
+ * other calls are not affected.  hdc_gated_scan_wait_limit: the limit of the waits of later calls
+ * of this process in ns, from 0 (no waiting) to 2e9, which it is at the start.
  */
 int64_t hdc_gated_scan_state_rows(void);
+int hdc_gated_scan_wait_limit(uint64_t ns);
 size_t hdc_gated_scan_workspace_bytes(int64_t B, int64_t L, int64_t ds);
 int hdc_gated_scan_fwd(int dtype, int a_dtype, const void* projs, int64_t proj_sb, int64_t proj_st,
                        const void* A_log, const float* h0, const uint8_t* reset, void* y, int64_t y_sb,
