@@ -32,7 +32,7 @@ namespace hdc {
 struct LnConvParams {
   const void* x; const void* nw; const void* nb; const void* cw; const void* cb;
   const void* halo; void* out;
-  void* mean; void* rstd; int stat_f32;  // row statistics: bf16, or fp32 where stat_f32
+  void* mean; void* rstd;  // row statistics: bf16, or fp32 where STAT32
   // sequence parallelism: the halo arrives from another GPU; the CTAs that read it wait
   // (bounded) until *halo_flag reaches *halo_gen (nullptr: no wait)
   const uint32_t* halo_flag; const uint32_t* halo_gen;
@@ -142,7 +142,9 @@ __device__ __forceinline__ float warp_sum16(float* v, int lane) {
   return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
 }
 
-template <typename T, bool SILU>
+// STAT32: the training form's fp32 row statistics (as a template: a branch at run time costs the
+// other form 40 bytes of spills)
+template <typename T, bool SILU, bool STAT32>
 __global__ void __launch_bounds__(512) ln_conv_kernel(LnConvParams p) {
   constexpr int VEC = Vec<T>::N, NP = VEC / 2, R = LNC_ROWS;
   extern __shared__ uint8_t smem_raw[];
@@ -350,7 +352,7 @@ __global__ void __launch_bounds__(512) ln_conv_kernel(LnConvParams p) {
     }
     if (p.mean && warp == 0 && lane < nv) {
       const size_t i = (size_t)b * p.L + t0 + lane;
-      if (p.stat_f32) {
+      if constexpr (STAT32) {
         static_cast<float*>(p.mean)[i] = mean;
         static_cast<float*>(p.rstd)[i] = rs;
       } else {
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(512) ln_conv_kernel(LnConvParams p) {
   }
 }
 
-template <typename T, bool SILU>
+template <typename T, bool SILU, bool STAT32>
 static int launch_ln_conv(LnConvParams p, int64_t B, cudaStream_t stream) {
   const int G = p.D / Vec<T>::N;
   const int threads = (G + 31) / 32 * 32;
@@ -381,9 +383,10 @@ static int launch_ln_conv(LnConvParams p, int64_t B, cudaStream_t stream) {
   while (smem_of(nst) > 227 * 1024 && nst > 2) --nst;
   const size_t smem = smem_of(nst);
   if (smem > 227 * 1024) return fail(HDC_E_SHAPE, "ln_conv: D=%d needs %zu bytes of shared memory", p.D, smem);
-  cudaFuncSetAttribute(ln_conv_kernel<T, SILU>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  constexpr auto kernel = ln_conv_kernel<T, SILU, STAT32>;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   int occ = 0;
-  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, ln_conv_kernel<T, SILU>, threads, smem);
+  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, threads, smem);
   if (occ < 1) occ = 1;
   const int64_t target = (int64_t)num_sms() * occ;
   // rounded down, so B * segs_per_b stays within one wave of resident CTAs
@@ -395,16 +398,17 @@ static int launch_ln_conv(LnConvParams p, int64_t B, cudaStream_t stream) {
   p.segs_per_b = (int)segs_per_b;
   p.total_segs = (int)(B * segs_per_b);
   p.nst = nst;
-  ln_conv_kernel<T, SILU><<<p.total_segs, threads, smem, stream>>>(p);
+  kernel<<<p.total_segs, threads, smem, stream>>>(p);
   return launch_status("ln_conv_kernel");
 }
 
 template <typename T>
-static int ln_conv_dispatch(LnConvParams p, int64_t B, cudaStream_t stream) {
+static int ln_conv_dispatch(LnConvParams p, bool stat32, int64_t B, cudaStream_t stream) {
   const int G = p.D / Vec<T>::N;
-  if (G <= 512)
-    return p.act == HDC_ACT_SILU ? launch_ln_conv<T, true>(p, B, stream) : launch_ln_conv<T, false>(p, B, stream);
-  return fail(HDC_E_SHAPE, "ln_conv: D=%d too large", p.D);
+  if (G > 512) return fail(HDC_E_SHAPE, "ln_conv: D=%d too large", p.D);
+  if (stat32) return launch_ln_conv<T, false, true>(p, B, stream);
+  return p.act == HDC_ACT_SILU ? launch_ln_conv<T, true, false>(p, B, stream)
+                               : launch_ln_conv<T, false, false>(p, B, stream);
 }
 
 }  // namespace hdc
@@ -412,7 +416,7 @@ static int ln_conv_dispatch(LnConvParams p, int64_t B, cudaStream_t stream) {
 using namespace hdc;
 
 static int ln_conv_fwd(int dtype, const void* x, const void* norm_w, const void* norm_b, const void* conv_w,
-                       const void* conv_b, const void* halo, void* out, void* mean, void* rstd, int stat_f32,
+                       const void* conv_b, const void* halo, void* out, void* mean, void* rstd, bool stat32,
                        int64_t B, int64_t L, int64_t D, float eps, int act, const uint32_t* halo_flag,
                        const uint32_t* halo_gen, hdc_stream_t stream) {
   if (dtype != HDC_F32 && dtype != HDC_BF16) return fail(HDC_E_DTYPE, "ln_conv: dtype %d", dtype);
@@ -429,18 +433,19 @@ static int ln_conv_fwd(int dtype, const void* x, const void* norm_w, const void*
   if (x == out) return fail(HDC_E_SHAPE, "ln_conv: out must not alias x");
   LnConvParams p{};
   p.x = x; p.nw = norm_w; p.nb = norm_b; p.cw = conv_w; p.cb = conv_b; p.halo = halo; p.out = out;
-  p.mean = mean; p.rstd = rstd; p.stat_f32 = stat_f32;
+  p.mean = mean; p.rstd = rstd;
   p.L = (int)L; p.D = (int)D; p.eps = eps; p.act = act;
   p.halo_flag = halo_flag; p.halo_gen = halo_gen;
   auto s = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == HDC_F32 ? ln_conv_dispatch<float>(p, B, s) : ln_conv_dispatch<__nv_bfloat16>(p, B, s);
+  return dtype == HDC_F32 ? ln_conv_dispatch<float>(p, stat32, B, s)
+                          : ln_conv_dispatch<__nv_bfloat16>(p, stat32, B, s);
 }
 
 extern "C" int hdc_ln_conv_fwd(int dtype, const void* x, const void* norm_w, const void* norm_b,
                                const void* conv_w, const void* conv_b, const void* halo, void* out,
                                void* mean, void* rstd, int64_t B, int64_t L, int64_t D, float eps,
                                int act, hdc_stream_t stream) {
-  return ln_conv_fwd(dtype, x, norm_w, norm_b, conv_w, conv_b, halo, out, mean, rstd, 0, B, L, D, eps, act, nullptr,
+  return ln_conv_fwd(dtype, x, norm_w, norm_b, conv_w, conv_b, halo, out, mean, rstd, false, B, L, D, eps, act, nullptr,
                      nullptr, stream);
 }
 
@@ -450,7 +455,7 @@ extern "C" int hdc_ln_conv_train_fwd(int dtype, const void* x, const void* norm_
   if (!mean || !rstd) return fail(HDC_E_NULL, "ln_conv_train: null pointer");
   if (((reinterpret_cast<uintptr_t>(mean) | reinterpret_cast<uintptr_t>(rstd)) & 3u) != 0)
     return fail(HDC_E_ALIGN, "ln_conv_train: mean or rstd is not aligned to its type");
-  return ln_conv_fwd(dtype, x, norm_w, norm_b, conv_w, conv_b, nullptr, out, mean, rstd, 1, B, L, D, eps,
+  return ln_conv_fwd(dtype, x, norm_w, norm_b, conv_w, conv_b, nullptr, out, mean, rstd, true, B, L, D, eps,
                      HDC_ACT_NONE, nullptr, nullptr, stream);
 }
 
@@ -460,6 +465,6 @@ extern "C" int hdc_ln_conv_fwd_halo_flag(int dtype, const void* x, const void* n
                                          int act, const uint32_t* halo_flag, const uint32_t* halo_gen,
                                          hdc_stream_t stream) {
   if (!halo || !halo_flag || !halo_gen) return fail(HDC_E_NULL, "ln_conv_halo_flag: halo, flag and gen required");
-  return ln_conv_fwd(dtype, x, norm_w, norm_b, conv_w, conv_b, halo, out, mean, rstd, 0, B, L, D, eps, act, halo_flag,
-                     halo_gen, stream);
+  return ln_conv_fwd(dtype, x, norm_w, norm_b, conv_w, conv_b, halo, out, mean, rstd, false, B, L, D, eps, act,
+                     halo_flag, halo_gen, stream);
 }

@@ -34,15 +34,10 @@
 namespace hdc {
 
 struct LnConvBwdParams {
-  const void* go; const void* x; const void* mean; const void* rstd; int stat_f32;
+  const void* go; const void* x; const void* mean; const void* rstd;
   const void* nw; const void* cw; void* dx; float* part;
   int L, D, seg_len, segs_per_b;
 };
-
-// row statistic i: bf16, or fp32 where the training form keeps it so
-__device__ __forceinline__ float ld_stat(const void* p, int f32, size_t i) {
-  return f32 ? static_cast<const float*>(p)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
 
 template <typename T>
 __device__ __forceinline__ void ld4(const T* p, float* f);
@@ -72,7 +67,8 @@ __device__ __forceinline__ void st4<__nv_bfloat16>(__nv_bfloat16* p, const float
   *reinterpret_cast<uint2*>(p) = v;
 }
 
-template <typename T>
+// S: the type of the row statistics (the training form's are fp32)
+template <typename T, typename S>
 __global__ void __launch_bounds__(512) ln_conv_bwd_kernel(LnConvBwdParams p) {
   __shared__ float red[2][4][2][16];  // [half][row of the group][sum][warp]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nwarps = blockDim.x >> 5;
@@ -87,9 +83,8 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_kernel(LnConvBwdParams p) {
   const T* go = static_cast<const T*>(p.go) + (size_t)b * p.L * rowD + cc;
   const T* x = static_cast<const T*>(p.x) + (size_t)b * p.L * rowD + cc;
   T* dx = static_cast<T*>(p.dx) + (size_t)b * p.L * rowD + cc;
-  const size_t stat0 = (size_t)b * p.L;
-  auto mean = [&](int t) { return ld_stat(p.mean, p.stat_f32, stat0 + t); };
-  auto rstd = [&](int t) { return ld_stat(p.rstd, p.stat_f32, stat0 + t); };
+  const S* mean = static_cast<const S*>(p.mean) + (size_t)b * p.L;
+  const S* rstd = static_cast<const S*>(p.rstd) + (size_t)b * p.L;
   const float invD = 1.0f / (float)p.D;
 
   float nw[4], cw[4][4];  // cw[e][k]
@@ -105,7 +100,7 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_kernel(LnConvBwdParams p) {
     if (act && t >= 0) {
       float v[4];
       ld4<T>(x + (size_t)t * rowD, v);
-      const float m = mean(t), r = rstd(t);
+      const float m = to_f(mean[t]), r = to_f(rstd[t]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] = (v[e] - m) * r * nw[e];
     } else {
@@ -134,7 +129,7 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_kernel(LnConvBwdParams p) {
       if (t < l1) {
         load_go(t + 3, G[(u + 3) & 3]);
         float v[4];
-        const float m = mean(t), r = rstd(t);
+        const float m = to_f(mean[t]), r = to_f(rstd[t]);
         rs[u] = r;
         if (act) ld4<T>(x + (size_t)t * rowD, v);
         else v[0] = v[1] = v[2] = v[3] = 0.f;
@@ -265,7 +260,7 @@ __device__ __forceinline__ void stg4_if(T* p, const uint64_t* f, bool pred) {
   }
 }
 
-template <typename T, int NST, int TR>
+template <typename T, typename S, int NST, int TR>
 __global__ void __launch_bounds__(512) ln_conv_bwd_staged_kernel(LnConvBwdParams p) {
   static_assert(TR % 4 == 0 && TR <= 32, "tiles of whole 4-row groups, one row per lane");
   __shared__ __align__(16) float red[2][8][16];  // [half][value: 4 x sum dn nw, 4 x sum dn nw xhat][warp]
@@ -288,9 +283,8 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_staged_kernel(LnConvBwdParams
   const T* gob = static_cast<const T*>(p.go) + (size_t)b * p.L * rowD;
   const T* xb = static_cast<const T*>(p.x) + (size_t)b * p.L * rowD;
   T* dx = static_cast<T*>(p.dx) + (size_t)b * p.L * rowD + cc;
-  const size_t stat0 = (size_t)b * p.L;
-  auto mean = [&](int t) { return ld_stat(p.mean, p.stat_f32, stat0 + t); };
-  auto rstd = [&](int t) { return ld_stat(p.rstd, p.stat_f32, stat0 + t); };
+  const S* mean = static_cast<const S*>(p.mean) + (size_t)b * p.L;
+  const S* rstd = static_cast<const S*>(p.rstd) + (size_t)b * p.L;
   const float invD = 1.0f / (float)p.D;
   const int ntiles = (l1 - l0 + TR - 1) / TR;
 
@@ -342,7 +336,7 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_staged_kernel(LnConvBwdParams
     if (t >= 0) {
       uint64_t v[2];
       ldg4<T>(xb + (size_t)t * rowD + cc, v);
-      const float m = mean(t), rr = rstd(t);
+      const float m = to_f(mean[t]), rr = to_f(rstd[t]);
       const uint64_t r2 = f2_make(rr, rr), mr2 = f2_make(-m * rr, -m * rr);
 #pragma unroll
       for (int j = 0; j < 2; ++j) X[r + 1][j] = f2_mul(f2_fma(v[j], r2, mr2), nw2[j]);
@@ -361,8 +355,8 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_staged_kernel(LnConvBwdParams
     // row statistics of the tile: lane i holds row i's (TR <= 32)
     float mt = 0.f, rt = 0.f;
     if (lane < nrows) {
-      mt = mean(t0 + lane);
-      rt = rstd(t0 + lane);
+      mt = to_f(mean[t0 + lane]);
+      rt = to_f(rstd[t0 + lane]);
     }
     // a timed-out wait ends the loop for every warp together at the group barrier below
     const bool got = mbar_wait_warp(&bars[st], (uint32_t)((k / NST) & 1), 34);
@@ -485,33 +479,48 @@ __global__ void __launch_bounds__(512) ln_conv_bwd_staged_kernel(LnConvBwdParams
   }
 }
 
-// sums the per-CTA partials [nseg][7][D] in CTA order and casts to T:
-// dnw [D], dnb [D], dcb [D], dcw [D][4]; nb, cw: the training form's terms (nullptr: without them)
-template <typename T>
-__global__ void ln_conv_bwd_reduce_kernel(const float* part, int nseg, int D, const T* nb, const T* cw, T* dnw, T* dnb,
-                                          T* dcw, T* dcb) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;  // (row of 7, channel)
-  if (i >= 7 * D) return;
-  const int k = i / D, d = i - k * D;
-  auto sum_row = [&](int row) {
-    float s = 0.f;
-    // 16 loads in flight per thread (few threads: 7 D of them); the adds stay in CTA order
+// one of the 7 D sums over the CTAs' partials [nseg][7][D], in CTA order
+__device__ __forceinline__ float sum_parts(const float* part, int nseg, int D, int i) {
+  float s = 0.f;
+  // 16 loads in flight per thread (few threads: 7 D of them); the adds stay in CTA order
 #pragma unroll 16
-    for (int c = 0; c < nseg; ++c) s += part[((size_t)c * 7 + row) * D + d];
-    return s;
-  };
-  float s = sum_row(nb && k == 1 ? 2 : k);
-  if (nb && k == 1) {
-    const T* w = cw + (size_t)d * 4;
-    s *= (to_f(w[0]) + to_f(w[1])) + (to_f(w[2]) + to_f(w[3]));
-  } else if (nb && k >= 3) {
-    s = fmaf(to_f(nb[d]), sum_row(2), s);
-  }
+  for (int c = 0; c < nseg; ++c) s += part[(size_t)c * 7 * D + i];
+  return s;
+}
+// sum k of channel d, cast to T: dnw [D], dnb [D], dcb [D], dcw [D][4]
+template <typename T>
+__device__ __forceinline__ void store_sum(int k, int d, float s, T* dnw, T* dnb, T* dcw, T* dcb) {
   const T v = from_f<T>(s);
   if (k == 0) dnw[d] = v;
   else if (k == 1) dnb[d] = v;
   else if (k == 2) dcb[d] = v;
   else dcw[(size_t)d * 4 + (k - 3)] = v;
+}
+template <typename T>
+__global__ void ln_conv_bwd_reduce_kernel(const float* part, int nseg, int D, T* dnw, T* dnb, T* dcw, T* dcb) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;  // (row of 7, channel)
+  if (i >= 7 * D) return;
+  store_sum(i / D, i % D, sum_parts(part, nseg, D, i), dnw, dnb, dcw, dcb);
+}
+// The training form: warp k of a CTA has sum k of 32 channels, and d_cb gives the terms that the
+// partials leave out.
+template <typename T>
+__global__ void __launch_bounds__(224) ln_conv_train_reduce_kernel(const float* part, int nseg, int D, const T* nb,
+                                                                   const T* cw, T* dnw, T* dnb, T* dcw, T* dcb) {
+  __shared__ float dcb_sum[32];
+  const int k = threadIdx.x >> 5, lane = threadIdx.x & 31, d = blockIdx.x * 32 + lane;
+  float s = d < D ? sum_parts(part, nseg, D, k * D + d) : 0.f;
+  if (k == 2) dcb_sum[lane] = s;
+  __syncthreads();
+  if (d >= D) return;
+  const float g = dcb_sum[lane];
+  if (k == 1) {
+    const T* w = cw + (size_t)d * 4;
+    s = g * ((to_f(w[0]) + to_f(w[1])) + (to_f(w[2]) + to_f(w[3])));
+  } else if (k >= 3) {
+    s = fmaf(to_f(nb[d]), g, s);
+  }
+  store_sum(k, d, s, dnw, dnb, dcw, dcb);
 }
 
 constexpr int kBwdMaxD = 2048;  // 512 threads x 4 channels
@@ -559,7 +568,7 @@ static int ln_conv_bwd(int dtype, const void* grad_out, const void* x, const voi
       !aligned16(workspace))
     return fail(HDC_E_ALIGN, "ln_conv_bwd: pointers must be 16-byte aligned");
   LnConvBwdParams p{};
-  p.go = grad_out; p.x = x; p.mean = mean; p.rstd = rstd; p.stat_f32 = norm_b != nullptr;
+  p.go = grad_out; p.x = x; p.mean = mean; p.rstd = rstd;
   p.nw = norm_w; p.cw = conv_w; p.dx = dx;
   p.part = static_cast<float*>(workspace); p.L = (int)L; p.D = (int)D;
   bwd_plan(B, L, D, &p.seg_len, &p.segs_per_b);
@@ -577,32 +586,29 @@ static int ln_conv_bwd(int dtype, const void* grad_out, const void* x, const voi
   if (smem_of(TR, nst) > 200 * 1024) TR = 4;
   if (smem_of(TR, nst) > 200 * 1024) nst = 2;
   const size_t smem = smem_of(TR, nst);
-  auto launch_main = [&](auto tag) -> int {
+  auto launch = [&](auto tag, auto stat) -> int {
     using T = decltype(tag);
+    using S = decltype(stat);
     auto go = [&](auto kernel) {
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
       kernel<<<nseg, threads, smem, s>>>(p);
     };
-    if (!staged) ln_conv_bwd_kernel<T><<<nseg, threads, 0, s>>>(p);
-    else if (nst == 3 && TR == 8) go(ln_conv_bwd_staged_kernel<T, 3, 8>);
-    else if (nst == 3) go(ln_conv_bwd_staged_kernel<T, 3, 4>);
-    else go(ln_conv_bwd_staged_kernel<T, 2, 4>);
-    return launch_status("ln_conv_bwd_kernel");
+    if (!staged) ln_conv_bwd_kernel<T, S><<<nseg, threads, 0, s>>>(p);
+    else if (nst == 3 && TR == 8) go(ln_conv_bwd_staged_kernel<T, S, 3, 8>);
+    else if (nst == 3) go(ln_conv_bwd_staged_kernel<T, S, 3, 4>);
+    else go(ln_conv_bwd_staged_kernel<T, S, 2, 4>);
+    if (int e = launch_status("ln_conv_bwd_kernel")) return e;
+    T *nwo = static_cast<T*>(dnorm_w), *nbo = static_cast<T*>(dnorm_b), *cwo = static_cast<T*>(dconv_w),
+      *cbo = static_cast<T*>(dconv_b);
+    if (norm_b)
+      ln_conv_train_reduce_kernel<T><<<(int)((D + 31) / 32), 224, 0, s>>>(
+          p.part, nseg, (int)D, static_cast<const T*>(norm_b), static_cast<const T*>(conv_w), nwo, nbo, cwo, cbo);
+    else
+      ln_conv_bwd_reduce_kernel<T><<<rgrid, 256, 0, s>>>(p.part, nseg, (int)D, nwo, nbo, cwo, cbo);
+    return launch_status("ln_conv_bwd_reduce_kernel");
   };
-  auto reduce = [&](auto tag) {
-    using T = decltype(tag);
-    ln_conv_bwd_reduce_kernel<T><<<rgrid, 256, 0, s>>>(
-        p.part, nseg, (int)D, static_cast<const T*>(norm_b), static_cast<const T*>(conv_w), static_cast<T*>(dnorm_w),
-        static_cast<T*>(dnorm_b), static_cast<T*>(dconv_w), static_cast<T*>(dconv_b));
-  };
-  if (dtype == HDC_F32) {
-    if (int e = launch_main(float{})) return e;
-    reduce(float{});
-  } else {
-    if (int e = launch_main(__nv_bfloat16{})) return e;
-    reduce(__nv_bfloat16{});
-  }
-  return launch_status("ln_conv_bwd_reduce_kernel");
+  if (norm_b) return dtype == HDC_F32 ? launch(float{}, float{}) : launch(__nv_bfloat16{}, float{});
+  return dtype == HDC_F32 ? launch(float{}, __nv_bfloat16{}) : launch(__nv_bfloat16{}, __nv_bfloat16{});
 }
 
 extern "C" int hdc_ln_conv_bwd(int dtype, const void* grad_out, const void* x, const void* mean, const void* rstd,
