@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnBwdCtas) gn_sums_kernel(const _
 // CTA (sample, block of whole groups): the sample's sums over its slices, to sums[n][2][C], and
 // from them the means of e xh and of e of each group, to gmean[n][2][G].
 __global__ void __launch_bounds__(256) gn_mid_kernel(const __grid_constant__ GnParams p, int block) {
-  extern __shared__ float sh[];  // [strands][2 cw], then [2 cw]
+  extern __shared__ float sh[];  // [strands][2 cw]; then the sums times the weight in the first of them
   let_next_start();
   wait_for_previous();
   const int n = blockIdx.x, c_lo = blockIdx.y * block, cw = min(block, p.C - c_lo), items = 2 * cw;
@@ -372,8 +372,8 @@ __global__ void __launch_bounds__(256) gn_mid_kernel(const __grid_constant__ GnP
       sh[st * items + i] = v;
     }
   __syncthreads();
-  float* tot = sh + strands * items;
-  for (int i = threadIdx.x; i < items; i += 256) {
+  float* tot = sh;
+  for (int i = threadIdx.x; i < items; i += 256) {  // item i of every strand is this thread's alone
     float v = sh[i];
     for (int k = 1; k < strands; ++k) v += sh[k * items + i];
     const int which = i >= cw, c = which ? i - cw : i;
@@ -768,9 +768,12 @@ extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_
       if (int e = launch_status("gn_sums_kernel")) return e;
       parts = N;
       if (!plan.one) {
-        const int block = gn_mid_block(p.C, p.Cg), items = 2 * block, strands = items < 256 ? 256 / items : 1;
+        // shared memory: at most 256 threads' strands of any block, or the items of a wide one (32 KB
+        // for the widest group, within the 48 KB that a launch may ask for)
+        const int block = gn_mid_block(p.C, p.Cg), items = 2 * block;
+        static_assert(2 * kGnMostCg * 4 <= 48 * 1024, "the middle step's sums of a group");
         launch_dependent(gn_mid_kernel, dim3((unsigned)N, (unsigned)((C + block - 1) / block)), 256,
-                         (size_t)(strands + 1) * items * 4, s, p, block);
+                         (size_t)(items < 256 ? 256 : items) * 4, s, p, block);
         if (int e = launch_status("gn_mid_kernel")) return e;
         gn_pass(kDx, dtype, p, plan, ve, s);
         if (int e = launch_status("gn_dx_kernel")) return e;
