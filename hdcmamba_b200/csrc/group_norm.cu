@@ -547,11 +547,18 @@ static int64_t gn_row_parts(int64_t N, int64_t G, int64_t Cg) {
 // block held in the shared memory of a cluster and read once (16 x 4096 x 320 bf16: 51 us for 34).
 struct GnPlan { int64_t slices, rows, cb, gz; bool one; };
 // Whole groups, about `want` channels, a multiple of the channels that a load of the full row
-// could take (so that blocks do not narrow the loads).
+// could take (so that blocks do not narrow the loads) as long as the block's sums, two floats a
+// channel where a thread has several chunks, stay within the 48 KB that a launch may ask for: wide
+// odd groups take narrower loads instead (gn_width goes by the block too).
+constexpr int64_t kGnMostBlock = 48 * 1024 / 8;
+static_assert(kGnMostCg <= kGnMostBlock, "a block holds at least one group");
 static int64_t gn_block(int64_t C, int64_t Cg, int64_t want) {
   int64_t step = Cg;
-  for (int ve = 2; ve <= 8 && C % ve == 0; ve *= 2)
-    while (step % ve != 0) step *= 2;
+  for (int ve = 2; ve <= 8 && C % ve == 0; ve *= 2) {  // step is a multiple of ve / 2
+    if (step % ve == 0) continue;
+    if (2 * step > kGnMostBlock) break;
+    step *= 2;
+  }
   if (C <= want || C <= step) return C;
   return step >= want ? step : want / step * step;
 }
