@@ -529,16 +529,6 @@ static GnRowPlan gn_row_plan(int64_t N, int64_t S, int64_t G, int64_t Cg, int ve
   r.ctas = need < fill ? need : fill;
   return r;
 }
-// The workspace is sized without knowing the type: for the most CTAs of any width.
-static int64_t gn_row_parts(int64_t N, int64_t G, int64_t Cg) {
-  int64_t most = 0;
-  for (int ve = 1; ve <= 8; ve *= 2)
-    if (Cg % ve == 0) {
-      const GnRowPlan r = gn_row_plan(N, 1, G, Cg, ve, true);
-      if (r.ok && r.ctas > most) most = r.ctas;
-    }
-  return most;
-}
 // Several positions.  One pass when a sample's block of some 64 channels is small enough (64 KB in
 // bf16) to be read again from L1 (2 x 225 x 96: 6.0 us forward, 7.2 backward; in two passes 7.6 and
 // 10.5).  Else slices of each sample, 32 positions or more, in one wave of the resident CTAs: a
@@ -578,6 +568,23 @@ static GnPlan gn_plan(int64_t N, int64_t S, int64_t C, int64_t G, bool bwd) {
     r.slices = (S + r.rows - 1) / r.rows;
   }
   return r;
+}
+static int gn_width(int es, int64_t d);
+// What a call of element size es needs in its workspace (that of a shape is the larger one of both
+// types').  Forward: the slices' statistics, then the samples' mean and rstd when the caller does not
+// want them.  Gradient: the row CTAs' sums, or the slices' sums, the samples' sums (where a sample
+// has several slices) and the groups' means.
+static size_t gn_fwd_ws(int es, int64_t N, int64_t S, int64_t C, int64_t G) {
+  if (C / G > kGnMostCg || gn_row_plan(N, S, G, C / G, gn_width(es, C / G)).ok) return 0;
+  const GnPlan r = gn_plan(N, S, C, G, false);
+  return r.one ? 0 : (size_t)N * G * 8 * (r.slices + 1);
+}
+static size_t gn_bwd_ws(int es, int64_t N, int64_t S, int64_t C, int64_t G) {
+  if (C / G > kGnMostCg) return (size_t)N * 2 * C * 4;
+  const GnRowPlan row = gn_row_plan(N, S, G, C / G, gn_width(es, C / G), true);
+  if (row.ok) return (size_t)row.ctas * 2 * C * 4;
+  const GnPlan r = gn_plan(N, S, C, G, true);
+  return (size_t)N * 2 * 4 * ((r.slices > 1 ? r.slices + 1 : 1) * C + (r.one ? 0 : G));
 }
 // Channels per load: as many as 16 bytes hold and divide d (the group's channels, or the row's).
 // The layout does not enter, so that it does not change the arithmetic; whether the rows allow
@@ -651,12 +658,9 @@ static int gn_check(const char* what, int dtype, int p_dtype, int64_t N, int64_t
 using namespace hdc;
 
 extern "C" size_t hdc_group_norm_workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G) {
-  if (N < 1 || S < 1 || C < 1 || G < 1 || C % G != 0 || C / G > kGnMostCg) return 0;
-  // one position takes no second pass with wider loads if it takes none with single channels
-  if (gn_row_plan(N, S, G, C / G, 1).ok) return 0;
-  if (gn_plan(N, S, C, G, false).one) return 0;
-  // the slices' statistics, then the samples' mean and rstd when the caller does not want them
-  return (size_t)N * G * 8 * (gn_plan(N, S, C, G, false).slices + 1);
+  if (N < 1 || S < 1 || C < 1 || G < 1 || C % G != 0) return 0;
+  const size_t a = gn_fwd_ws(2, N, S, C, G), b = gn_fwd_ws(4, N, S, C, G);
+  return a > b ? a : b;
 }
 
 extern "C" int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t x_sn, int64_t x_ss, const void* weight,
@@ -712,12 +716,8 @@ extern "C" int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t
 
 extern "C" size_t hdc_group_norm_bwd_workspace_bytes(int64_t N, int64_t S, int64_t C, int64_t G) {
   if (N < 1 || S < 1 || C < 1 || G < 1 || C % G != 0) return 0;
-  if (C / G > kGnMostCg) return (size_t)N * 2 * C * 4;
-  const size_t one = S == 1 ? (size_t)gn_row_parts(N, G, C / G) * 2 * C * 4 : 0;
-  if (gn_row_plan(N, S, G, C / G, 1).ok) return one;
-  // the slices' sums, the samples' sums, the groups' means
-  const size_t two = (size_t)N * 2 * 4 * ((gn_plan(N, S, C, G, true).slices + 1) * C + G);
-  return one > two ? one : two;
+  const size_t a = gn_bwd_ws(2, N, S, C, G), b = gn_bwd_ws(4, N, S, C, G);
+  return a > b ? a : b;
 }
 // the middle step's channels per CTA: whole groups, some 64 channels
 static int gn_mid_block(int C, int Cg) {
@@ -769,7 +769,8 @@ extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_
       p.slices = (int)plan.slices; p.rows = (int)plan.rows; p.cb = (int)plan.cb;
       ve = gn_width(es, plan.cb | C);
       p.whole = gn_whole(es, ve, ptr, stride, 3);
-      p.sums = p.part + N * plan.slices * 2 * C;
+      // a single slice's sums are the sample's: the middle step writes them where it read them
+      p.sums = plan.slices > 1 ? p.part + N * plan.slices * 2 * C : p.part;
       p.gmean = p.sums + N * 2 * C;
       gn_pass(kSums, dtype, p, plan, ve, s);
       if (int e = launch_status("gn_sums_kernel")) return e;
