@@ -175,9 +175,11 @@ template <typename T, int V> __device__ __forceinline__ Fv<V> gate(const Fv<V>& 
     return fma(p, e, m);
   }
 }
-// A = -exp(A_log)
+// A = -exp(A_log), kept finite: -inf times the closed gate of a step past the end (d = 0) would be
+// NaN, and its decay is 1 (NaN stays NaN)
+__device__ __forceinline__ float finite_rate(float A) { return A < -3.402823466e38f ? -3.402823466e38f : A; }
 template <typename T> __device__ __forceinline__ float rate(float A_log) {
-  return sizeof(T) == 4 ? -expf(A_log) : -ex2(1.4426950408889634f * A_log);
+  return finite_rate(sizeof(T) == 4 ? -expf(A_log) : -ex2(1.4426950408889634f * A_log));
 }
 // a = exp(d A), by the library's exp in both types: its error compounds over the steps that a
 // state remembers, and the hardware's 2^x doubles the error of the fp32 states and of dA_log (8 x
@@ -776,7 +778,7 @@ __global__ void __launch_bounds__(1024) gated_scan_dA_kernel(const float* part, 
   __syncthreads();
   if (k != 0 || j >= ds) return;
   for (int i = 1; i < 32; ++i) v += s[i][x];
-  v *= -expf(ld_param(A_log, a_bf16, j));
+  v *= finite_rate(-expf(ld_param(A_log, a_bf16, j)));
   if (a_bf16) static_cast<__nv_bfloat16*>(dA)[j] = __float2bfloat16_rn(v);
   else static_cast<float*>(dA)[j] = v;
 }
@@ -790,7 +792,7 @@ __global__ void __launch_bounds__(128) gated_step_kernel(const T* projs, int64_t
   const int j = blockIdx.x * blockDim.x + threadIdx.x, b = blockIdx.y;
   if (j >= ds) return;
   const T* r = projs + b * psb + j;
-  const float A = -expf(ld_param(A_log, a_bf16, j));
+  const float A = finite_rate(-expf(ld_param(A_log, a_bf16, j)));
   const float d = softplus_acc(to_f(r[0]));
   const float u = d * to_f(r[2 * ds]) * to_f(r[ds]);
   const int64_t i = (int64_t)b * ds + j;
