@@ -81,7 +81,7 @@ __device__ __forceinline__ void gn_apply_rows(const GnParams& p, const GnPlace& 
     for (; r + (U - 1) * RL < at.rows; r += U * RL) {
       Raw<T, VE> raw[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = ld_raw<T, VE, WHOLE>(x + u * xh);
+      for (int u = 0; u < U; ++u) raw[u] = ld_raw<T, VE, WHOLE, true>(x + u * xh);
       x += U * xh;
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -89,7 +89,7 @@ __device__ __forceinline__ void gn_apply_rows(const GnParams& p, const GnPlace& 
       y += U * yh;
     }
     for (; r < at.rows; r += RL, x += xh, y += yh)
-      st_vec<T, VE, WHOLE>(y, gn_act<T>(fma(unpack<T, VE>(ld_raw<T, VE, WHOLE>(x)) + neg, sc, b), p.silu));
+      st_vec<T, VE, WHOLE>(y, gn_act<T>(fma(unpack<T, VE>(ld_raw<T, VE, WHOLE, true>(x)) + neg, sc, b), p.silu));
   }
 }
 
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnFwdCtas) gn_stats_kernel(const 
       Raw<T, VE> raw[U];
       auto load = [&]() {
 #pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = ld_raw<T, VE, WHOLE>(x + u * hop);
+        for (int u = 0; u < U; ++u) raw[u] = ld_raw<T, VE, WHOLE, true>(x + u * hop);
         x += U * hop;
       };
       bool more = r + (U - 1) * RL < at.rows;
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnFwdCtas) gn_stats_kernel(const 
       }
       float cnt = blocks * U;
       for (; r < at.rows; r += RL) {
-        const Fv<VE> d = fma(mean, all<VE>(-1.f), unpack<T, VE>(ld_raw<T, VE, WHOLE>(x)));
+        const Fv<VE> d = fma(mean, all<VE>(-1.f), unpack<T, VE>(ld_raw<T, VE, WHOLE, true>(x)));
         x += hop;
         const float f = rcp(cnt + 1.f);
         mean = fma(d, all<VE>(f), mean);
@@ -272,8 +272,8 @@ __device__ __forceinline__ void gn_dx_rows(const GnParams& p, const GnPlace& at,
       Raw<T, VE> xr[U], dr[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        xr[u] = ld_raw<T, VE, WHOLE>(x + u * xh);
-        dr[u] = ld_raw<T, VE, WHOLE>(dy + u * dh);
+        xr[u] = ld_raw<T, VE, WHOLE, false>(x + u * xh);
+        dr[u] = ld_raw<T, VE, WHOLE, false>(dy + u * dh);
       }
       x += U * xh, dy += U * dh;
 #pragma unroll
@@ -281,7 +281,7 @@ __device__ __forceinline__ void gn_dx_rows(const GnParams& p, const GnPlace& at,
       dx += U * gh;
     }
     for (; r < at.rows; r += RL, x += xh, dy += dh, dx += gh)
-      one(ld_raw<T, VE, WHOLE>(x), ld_raw<T, VE, WHOLE>(dy), dx);
+      one(ld_raw<T, VE, WHOLE, false>(x), ld_raw<T, VE, WHOLE, false>(dy), dx);
   }
 }
 
@@ -314,14 +314,14 @@ __global__ void __launch_bounds__(kGnThreads, kGnBwdCtas) gn_sums_kernel(const _
         Raw<T, VE> xr[U], dr[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          xr[u] = ld_raw<T, VE, WHOLE>(x + u * xh);
-          dr[u] = ld_raw<T, VE, WHOLE>(dy + u * dh);
+          xr[u] = ld_raw<T, VE, WHOLE, !ONE>(x + u * xh);
+          dr[u] = ld_raw<T, VE, WHOLE, !ONE>(dy + u * dh);
         }
         x += U * xh, dy += U * dh;
 #pragma unroll
         for (int u = 0; u < U; ++u) one(xr[u], dr[u]);
       }
-      for (; r < at.rows; r += RL, x += xh, dy += dh) one(ld_raw<T, VE, WHOLE>(x), ld_raw<T, VE, WHOLE>(dy));
+      for (; r < at.rows; r += RL, x += xh, dy += dh) one(ld_raw<T, VE, WHOLE, !ONE>(x), ld_raw<T, VE, WHOLE, !ONE>(dy));
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         sh[rl * at.cw + k * VE + i] = a0.v[i];

@@ -27,9 +27,11 @@ __device__ __forceinline__ float gn_param(const void* p, int bf16, int i, float 
   return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];
 }
 
-// VE neighbouring values as loaded, at once or (rows that do not allow it) one by one
+// VE neighbouring values as loaded, at once or (rows that do not allow it) one by one.  RO: nothing
+// writes them while the kernel runs (the gradient's dx may be x or dy itself, so kernels that write
+// dx load both the ordinary way).
 template <typename T, int VE> struct Raw { static constexpr int kW = VE * (int)sizeof(T) >= 4 ? VE * (int)sizeof(T) / 4 : 1; uint32_t w[kW]; };
-template <typename T, int VE, bool WHOLE> __device__ __forceinline__ Raw<T, VE> ld_raw(const T* p) {
+template <typename T, int VE, bool WHOLE, bool RO> __device__ __forceinline__ Raw<T, VE> ld_raw(const T* p) {
   Raw<T, VE> r;
   constexpr int bytes = VE * (int)sizeof(T);
   if constexpr (VE > 1 && !WHOLE) {
@@ -45,15 +47,20 @@ template <typename T, int VE, bool WHOLE> __device__ __forceinline__ Raw<T, VE> 
     return r;
   }
   if constexpr (bytes == 16) {
-    const uint4 q = ldg16(p);
+    uint4 q;
+    if constexpr (RO) q = ldg16(p);
+    else asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p) : "memory");
     r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
   } else if constexpr (bytes == 8) {
-    const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2* at = reinterpret_cast<const uint2*>(p);
+    const uint2 q = RO ? __ldg(at) : *at;
     r.w[0] = q.x; r.w[1] = q.y;
   } else if constexpr (bytes == 4) {
-    r.w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    const uint32_t* at = reinterpret_cast<const uint32_t*>(p);
+    r.w[0] = RO ? __ldg(at) : *at;
   } else {
-    r.w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
+    const unsigned short* at = reinterpret_cast<const unsigned short*>(p);
+    r.w[0] = RO ? __ldg(at) : *at;
   }
   return r;
 }

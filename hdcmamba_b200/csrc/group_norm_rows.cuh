@@ -74,8 +74,8 @@ __global__ void __launch_bounds__(256) gn_row_kernel(const __grid_constant__ GnP
     Turn t;
 #pragma unroll
     for (int k = 0; k < CPL; ++k) {
-      t.x[k] = ld_raw<T, VE, WHOLE>(xp + at * xs + ch[k]);
-      if constexpr (BWD) t.dy[k] = ld_raw<T, VE, WHOLE>(dp + at * ds + ch[k]);
+      t.x[k] = ld_raw<T, VE, WHOLE, !BWD>(xp + at * xs + ch[k]);
+      if constexpr (BWD) t.dy[k] = ld_raw<T, VE, WHOLE, !BWD>(dp + at * ds + ch[k]);
     }
     if constexpr (BWD) {
       t.mu = __ldg(mp + at * gs);
