@@ -74,8 +74,7 @@ struct ScanParams {
   int NG;           // channel groups of all batches
   int64_t ntiles;   // NG * NT
   unsigned* ticket;  // NULL: a single tile in time, taken by block index, nothing published
-                     // ticket[1]: all ones, 0 once a wait of this call has run out
-  uint64_t wait_ns;  // limit of a wait
+                     // ticket[kGaveUp]: all ones, 0 once a wait of this call has run out
   uint64_t* ent;    // [NG][NT + spans + links][CW] published entries
   int nent;         // entries per group
   uint64_t div_NG, div_nch;  // 2^64 / d rounded up (0: d = 1)
@@ -289,13 +288,19 @@ template <int V> __device__ __forceinline__ void ld_entry(const uint64_t* e, uin
       asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(w[i]), "=l"(w[i + 1]) : "l"(e + i) : "memory");
   }
 }
-// Compose n in 1..4 neighbouring entries, waited for (up to p.wait_ns, then error 61; what is
+// The limit of a wait in clock cycles, some 2 per ns (a variable of the device and not a parameter of
+// the launch: read only while waiting, it leaves the rest of the kernel as it is; gradient of 8 x
+// 4096 x 1280 184 us as a parameter, 180 so).
+constexpr long long kMostWaitNs = 2000000000ll;
+static __device__ long long g_wait_cycles = 2 * kMostWaitNs;
+constexpr int kGaveUp = 1;  // word of the workspace's header
+// Compose n in 1..4 neighbouring entries, waited for (up to the limit, then error 61; what is
 // missing then is NaN).  e: entry 0 of them.  While an entry is missing, one word of each is
 // polled, not the whole entries.
 template <bool RESET, int V>
 __device__ __forceinline__ Map<V> take(const ScanParams& p, const uint64_t* e, int n, int lane) {
   uint64_t w[4][V];
-  uint64_t t0 = 0;
+  long long t0 = 0;
   while (true) {
     bool ok = true;
 #pragma unroll
@@ -306,20 +311,23 @@ __device__ __forceinline__ Map<V> take(const ScanParams& p, const uint64_t* e, i
 #pragma unroll
       for (int i = 0; i < V; ++i) ok = ok && (k >= n || (uint32_t)w[k][i] != kUnset);
     if (__all_sync(0xffffffffu, ok)) break;
-    if (t0 == 0) t0 = globaltimer_ns();
+    if (t0 == 0) t0 = clock64();
     bool late = false;
     if (lane < n) {
       uint64_t one[1];
       do {
         __nanosleep(32);
         ld_entry<1>(e + lane * 32 * V, one);
-        // a wait of this call that has run out elsewhere ends this one too, so that it ends soon
-        late = globaltimer_ns() - t0 >= p.wait_ns || *static_cast<volatile unsigned*>(p.ticket + 1) == 0;
+        // a wait of this call that has run out elsewhere ends this one too (looked at after some
+        // 0.1 ms only: waits are of a few us, and the word lies beside the ticket)
+        const long long waited = clock64() - t0;
+        late = waited >= *static_cast<volatile long long*>(&g_wait_cycles) ||
+               (waited > 200000 && *static_cast<volatile unsigned*>(p.ticket + kGaveUp) == 0);
       } while ((uint32_t)one[0] == kUnset && !late);
     }
     if (__any_sync(0xffffffffu, late)) {
       if (lane == 0) {
-        atomicExch(p.ticket + 1, 0u);
+        atomicExch(p.ticket + kGaveUp, 0u);
         atomicCAS(&g_dev_error, 0, 61);
       }
 #pragma unroll
@@ -826,17 +834,14 @@ static int64_t scan_entries(int64_t NT) {
 }
 // channels rounded up to the widest tile
 static int64_t scan_pad(int64_t ds) { return (ds + 127) / 128 * 128; }
-// the ticket and the word beside it (16 bytes), then the entries
+// the ticket and the word beside it, then the entries, each (256 bytes or more) on whole lines
+constexpr int kScanHeader = 256;
 static size_t scan_ws(int64_t B, int64_t L, int64_t ds) {
   const int64_t NT = tiles_in_time(L);
   if (B < 1 || ds < 1 || NT < 2) return 0;
-  return 16 + (size_t)(B * scan_pad(ds)) * scan_entries(NT) * 8;
+  return kScanHeader + (size_t)(B * scan_pad(ds)) * scan_entries(NT) * 8;
 }
-constexpr uint64_t kMostWaitNs = 2000000000ull;
-static std::atomic<uint64_t> g_wait_ns{kMostWaitNs};
-
 static void scan_plan(ScanParams& p, int CW, void* ws) {
-  p.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
   p.CW = CW;
   p.nch = (p.ds + CW - 1) / CW;
   p.NG = p.B * p.nch;
@@ -845,11 +850,11 @@ static void scan_plan(ScanParams& p, int CW, void* ws) {
   p.div_NG = p.NG > 1 ? ~uint64_t(0) / p.NG + 1 : 0;
   p.div_nch = p.nch > 1 ? ~uint64_t(0) / p.nch + 1 : 0;
   p.ticket = p.NT > 1 ? static_cast<unsigned*>(ws) : nullptr;
-  p.ent = p.NT > 1 ? reinterpret_cast<uint64_t*>(static_cast<char*>(ws) + 16) : nullptr;
+  p.ent = p.NT > 1 ? reinterpret_cast<uint64_t*>(static_cast<char*>(ws) + kScanHeader) : nullptr;
 }
 static int scan_clear(const ScanParams& p, cudaStream_t s, const char* what) {
   if (!p.ticket) return 0;
-  const size_t n = 16 + (size_t)p.NG * p.CW * p.nent * 8;
+  const size_t n = kScanHeader + (size_t)p.NG * p.CW * p.nent * 8;
   const cudaError_t e = cudaMemsetAsync(p.ticket, 0xff, n, s);
   return e == cudaSuccess ? 0 : fail((int)e, "%s: %s", what, cudaGetErrorString(e));
 }
@@ -910,11 +915,11 @@ using namespace hdc;
 extern "C" int64_t hdc_gated_scan_state_rows(void) { return kStateRows; }
 
 extern "C" int hdc_gated_scan_wait_limit(uint64_t ns) {
-  if (ns > kMostWaitNs)
-    return fail(HDC_E_SHAPE, "gated_scan_wait_limit: %llu ns (at most %llu)", (unsigned long long)ns,
-                (unsigned long long)kMostWaitNs);
-  g_wait_ns.store(ns, std::memory_order_relaxed);
-  return HDC_OK;
+  if (ns > (uint64_t)kMostWaitNs)
+    return fail(HDC_E_SHAPE, "gated_scan_wait_limit: %llu ns (at most %lld)", (unsigned long long)ns, kMostWaitNs);
+  const long long cycles = 2 * (long long)ns;
+  const cudaError_t e = cudaMemcpyToSymbol(g_wait_cycles, &cycles, sizeof cycles);
+  return e == cudaSuccess ? HDC_OK : fail((int)e, "gated_scan_wait_limit: %s", cudaGetErrorString(e));
 }
 
 extern "C" int hdc_gated_scan_fwd(int dtype, int a_dtype, const void* projs, int64_t proj_sb, int64_t proj_st,

@@ -400,8 +400,9 @@ int hdc_slot_step(int dtype, const void* q, const void* k, const void* v, const 
  * Pointers need their type's alignment; 16-byte aligned rows take the wide loads.  Tiles of a
  * sequence hand their results on inside the kernel; every wait is bounded.  A call whose wait runs
  * out reports 61 through hdc_device_error(), and what the missing result would have reached is NaN;
- * other calls are not affected.  hdc_gated_scan_wait_limit: the limit of the waits of later calls
- * of this process in ns, from 0 (no waiting) to 2e9, which it is at the start.
+ * other calls are not affected.  hdc_gated_scan_wait_limit: the limit of the waits on the current
+ * device in ns, from 0 (no waiting) to 2e9, which it is at the start; it synchronises as
+ * cudaMemcpyToSymbol does.
  */
 int64_t hdc_gated_scan_state_rows(void);
 int hdc_gated_scan_wait_limit(uint64_t ns);
