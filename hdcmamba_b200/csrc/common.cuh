@@ -14,6 +14,14 @@ void set_error(const char* fmt, ...);
 int fail(int code, const char* fmt, ...);
 int launch_status(const char* what);  // also counts the launch (hdc_launch_count)
 
+// The rows (i, j) of an output, i < n at stride si, j < m at stride sj, w elements each, lie apart: one
+// stride steps over all that the other reaches.
+inline bool rows_apart(int64_t n, int64_t si, int64_t m, int64_t sj, int64_t w) {
+  if (n < 2) return m < 2 || sj >= w;
+  if (m < 2) return si >= w;
+  return (sj >= w && si >= (m - 1) * sj + w) || (si >= w && sj >= (n - 1) * si + w);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---------------------------------------------------------------- element types

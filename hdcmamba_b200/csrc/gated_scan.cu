@@ -932,7 +932,8 @@ extern "C" int hdc_gated_scan_fwd(int dtype, int a_dtype, const void* projs, int
   if (off_type(projs, dtype) || off_type(y, dtype) || off_type(A_log, a_dtype) || off_type(h0, HDC_F32) ||
       off_type(h_last, HDC_F32) || off_type(states, HDC_F32))
     return fail(HDC_E_ALIGN, "gated_scan: a pointer is not aligned to its type");
-  if (y_st < ds && L > 1) return fail(HDC_E_SHAPE, "gated_scan: y rows overlap (y_st=%lld)", (long long)y_st);
+  if (L > 0 && !rows_apart(B, y_sb, L, y_st, ds))
+    return fail(HDC_E_SHAPE, "gated_scan: y rows overlap (y_sb=%lld, y_st=%lld)", (long long)y_sb, (long long)y_st);
   const size_t need = scan_ws(B, L, ds);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(HDC_E_WORKSPACE, "gated_scan: workspace of %zu bytes, %zu needed", workspace_bytes, need);
@@ -979,8 +980,9 @@ extern "C" int hdc_gated_scan_bwd(int dtype, int a_dtype, const void* projs, int
       off_type(dA_log, a_dtype) || off_type(states, HDC_F32) || off_type(dh_last, HDC_F32) || off_type(dh0, HDC_F32) ||
       off_type(workspace, HDC_F32))
     return fail(HDC_E_ALIGN, "gated_scan_bwd: a pointer is not aligned to its type");
-  if (dp_st < 3 * ds && L > 1)
-    return fail(HDC_E_SHAPE, "gated_scan_bwd: dprojs rows overlap (dp_st=%lld)", (long long)dp_st);
+  if (B > 0 && L > 0 && !rows_apart(B, dp_sb, L, dp_st, 3 * ds))
+    return fail(HDC_E_SHAPE, "gated_scan_bwd: dprojs rows overlap (dp_sb=%lld, dp_st=%lld)", (long long)dp_sb,
+                (long long)dp_st);
   const size_t need = hdc_gated_scan_bwd_workspace_bytes(B, L, ds);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(HDC_E_WORKSPACE, "gated_scan_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);

@@ -673,6 +673,8 @@ extern "C" int hdc_group_norm_fwd(int dtype, int p_dtype, const void* x, int64_t
   if (gn_off(x, dtype) || gn_off(y, dtype) || gn_off(weight, p_dtype) || gn_off(bias, p_dtype) ||
       gn_off(mean, HDC_F32) || gn_off(rstd, HDC_F32) || !aligned16(workspace))
     return fail(HDC_E_ALIGN, "group_norm: a pointer is not aligned to its type");
+  if (!rows_apart(N, y_sn, S, y_ss, C))
+    return fail(HDC_E_SHAPE, "group_norm: y rows overlap (y_sn=%lld, y_ss=%lld)", (long long)y_sn, (long long)y_ss);
   const size_t need = hdc_group_norm_workspace_bytes(N, S, C, G);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(HDC_E_WORKSPACE, "group_norm: workspace of %zu bytes, %zu needed", workspace_bytes, need);
@@ -737,6 +739,9 @@ extern "C" int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_
       gn_off(dweight, p_dtype) || gn_off(dbias, p_dtype) || gn_off(mean, HDC_F32) || gn_off(rstd, HDC_F32) ||
       !aligned16(workspace))
     return fail(HDC_E_ALIGN, "group_norm_bwd: a pointer is not aligned to its type");
+  if (!empty && !rows_apart(N, dx_sn, S, dx_ss, C))
+    return fail(HDC_E_SHAPE, "group_norm_bwd: dx rows overlap (dx_sn=%lld, dx_ss=%lld)", (long long)dx_sn,
+                (long long)dx_ss);
   const size_t need = hdc_group_norm_bwd_workspace_bytes(N, S, C, G);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(HDC_E_WORKSPACE, "group_norm_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);

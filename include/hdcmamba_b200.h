@@ -397,7 +397,8 @@ int hdc_slot_step(int dtype, const void* q, const void* k, const void* v, const 
  * hdc_gated_step: one step per sequence from projs rows [B, >=3ds]; h / h_out fp32 [B, ds]
  *   (h_out may be h), reset NULL or uint8 [B].
  * B in [0, 65535], L in [0, 2^30], ds in [1, 2^20], B * ceil(ds / 32) * ceil(L / 64) < 2^31.
- * Pointers need their type's alignment; 16-byte aligned rows take the wide loads.  Tiles of a
+ * Rows of y and of dprojs must not overlap (one of the two strides steps over all that the other
+ * reaches).  Pointers need their type's alignment; 16-byte aligned rows take the wide loads.  Tiles of a
  * sequence hand their results on inside the kernel; every wait is bounded.  A call whose wait runs
  * out reports 61 through hdc_device_error(), and what the missing result would have reached is NaN;
  * other calls are not affected.  hdc_gated_scan_wait_limit: the limit of the waits on the current
@@ -433,7 +434,8 @@ int hdc_gated_step(int dtype, int a_dtype, const void* projs, int64_t proj_sb, c
  *   act    : HDC_ACT_NONE or HDC_ACT_SILU.
  * hdc_group_norm_bwd: dx and, unless NULL, dweight / dbias from dy and the forward's mean and
  *   rstd; sums in a fixed order.  dx may be dy or x itself.
- * C in [1, 65536], G a divisor of C, N and S in [0, 2^30], N*G < 2^31.  Pointers need their
+ * C in [1, 65536], G a divisor of C, N and S in [0, 2^30], N*G < 2^31.  Rows of y and of dx must not
+ * overlap (one of the two strides steps over all that the other reaches).  Pointers need their
  * type's alignment; 16-byte aligned rows take the wide loads.  workspace: the
  * *_workspace_bytes of the shape, 16-byte aligned.
  */
