@@ -511,6 +511,9 @@ __global__ void __launch_bounds__(1024) gn_param_grad_kernel(const float* part, 
 
 // ---------------------------------------------------------------- plans
 constexpr int kGnMostCg = 4096;  // channels of a group in the kernels above
+// SMs that the schedules fill: B200's, as a constant, so that the sizes of the workspaces and the
+// order of the sums are a matter of the shape alone
+constexpr int kGnSms = 148;
 
 static GnRowPlan gn_row_plan(int64_t N, int64_t S, int64_t G, int64_t Cg, int ve, bool bwd = false) {
   GnRowPlan r{};
@@ -525,7 +528,7 @@ static GnRowPlan gn_row_plan(int64_t N, int64_t S, int64_t G, int64_t Cg, int ve
   r.gpc = (int)((G + r.gy - 1) / r.gy);
   r.spc = most / r.gpc;
   // one wave of the CTAs that are resident: a thread's parameters are loaded once
-  const int64_t need = (N + r.spc - 1) / r.spc, fill = ((int64_t)148 * (bwd ? 2 : 4) + r.gy - 1) / r.gy;
+  const int64_t need = (N + r.spc - 1) / r.spc, fill = ((int64_t)kGnSms * (bwd ? 2 : 4) + r.gy - 1) / r.gy;
   r.ctas = need < fill ? need : fill;
   return r;
 }
@@ -562,7 +565,7 @@ static GnPlan gn_plan(int64_t N, int64_t S, int64_t C, int64_t G, bool bwd) {
   r.rows = S;
   r.slices = 1;
   if (!r.one) {
-    const int64_t ctas = 148 * (bwd ? kGnBwdCtas : kGnFwdCtas), want = ctas >= N * r.gz ? ctas / (N * r.gz) : 1;
+    const int64_t ctas = kGnSms * (bwd ? kGnBwdCtas : kGnFwdCtas), want = ctas >= N * r.gz ? ctas / (N * r.gz) : 1;
     r.rows = (S + want - 1) / want;
     if (r.rows < 32) r.rows = S < 32 ? S : 32;
     r.slices = (S + r.rows - 1) / r.rows;

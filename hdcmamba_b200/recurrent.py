@@ -175,21 +175,21 @@ class GatedRecurrentBlock(nn.Module):
         return group_norm_act(y.reshape(-1, self.d_state), self.num_heads, gn.weight, gn.bias, gn.eps,
                               "silu").reshape(y.shape)
 
-    def _run(self, x, reset, h0):
+    def _run(self, x, reset):
         x_conv = norm_conv1d(x, self.norm, self.conv1d)
-        y, h = gated_scan(self.in_proj(x_conv), self.A_log, self.d_state, h0=h0, reset=reset)
+        y, h = gated_scan(self.in_proj(x_conv), self.A_log, self.d_state, reset=reset)
         return x + self.out_proj(self._heads(y)), h
 
     def forward(self, x, reset=None):
         """x [B, L, d_model] -> [B, L, d_model]."""
         _require_cuda(x)
-        return self._run(x, reset, None)[0]
+        return self._run(x, reset)[0]
 
     @torch.no_grad()
     def prefill(self, x, reset=None):
         """(forward(x), the state after it) for ``step``."""
         _require_cuda(x)
-        y, h = self._run(x, reset, None)
+        y, h = self._run(x, reset)
         return y, RecurrentState(window=self._window(x), h=h)
 
     def _window(self, x):
