@@ -35,14 +35,14 @@
 //
 // Why tiles of 64 steps: what a tile keeps between its two halves (a and u: 8 bytes per step and
 // channel) has to stay on the SM, in registers, and 16 to 32 warps of it fill them.  Measured
-// (device time, inputs out of L2, against 6550 GB/s): 8 x 4096 x 1280 bf16 forward 94 us (55%),
-// backward 174 us (51%); 1 x 32768 x 768 bf16 forward 92 us (33%); 1 x 32768 x 64 bf16 15 us;
-// 3 x 1537 x 333 fp32 forward 17 us, backward 29 us.  With many channels the issue slots bind (55 to
-// 65% busy, the rest waits of dependent instructions between 16 warps; without the exchange the
-// forward takes 44 us per 201 MB); with few, each round of tiles waits for the
-// slowest map before it, some 4 us of a round's 8.  Tried and slower: tickets that run the maps a
+// (device time, inputs out of L2, against 6550 GB/s): 8 x 4096 x 1280 bf16 forward 94 us (54%),
+// backward 175 us (51%); 1 x 32768 x 768 bf16 forward 93 us (33%); 1 x 32768 x 64 bf16 17 us;
+// 3 x 1537 x 333 fp32 forward 17 us, backward 29 us.  With many channels nothing is saturated: 16
+// warps of dependent instructions, with the barriers and the loads between them, fill 54 to 57% of the
+// issue slots (without the exchange the forward takes 44 us per 201 MB); with few channels each
+// round of tiles waits for the slowest map before it, some 4 us of a round's 8.  Tried and slower: tickets that run the maps a
 // few hundred tiles ahead of the outputs (inputs read again from L2: 105 us for 91), one word per
-// lane (above), three backward CTAs per SM (spills).
+// lane everywhere (scan_words), three backward CTAs per SM (spills).
 #include <atomic>
 #include <type_traits>
 
@@ -867,10 +867,11 @@ static int scan_fits(const char* what, int64_t B, int64_t L, int64_t ds) {
   return 0;
 }
 // Words per lane in the forward: in bf16 two (tiles of 128 channels) halve what a tile costs beside
-// its arithmetic (before decay() took the library's exp, 8 x 4096 x 1280: 87 us for 95, 1 x 32768 x
-// 768: 91 for 93); one where much of a wide tile would be empty (the 64 channels of a Block's
-// d_state: half of it), and in fp32, whose exp and log1p take the registers (3 x 1537 x 333: 17 us
-// with one, 19 with two).  The backward holds more per channel (two words spill 500 bytes) and
+// its arithmetic (us with two and with one: 8 x 4096 x 1280 94 and 101, 32 x 1024 x 512 40 and 43, 1 x
+// 32768 x 768 93 and 95, 1 x 8192 x 2048 55 and 55); one where much of a wide tile would be empty (1 x
+// 32768 x 64 23 and 17, 4 x 4096 x 192 20 and 17, x 320 24 and 21, x 448 30 and 26; past 512 channels
+// from 4 x 4096 x 520 36 and 32 to x 601 53 and 54), and in fp32, whose exp and log1p take the registers
+// (3 x 1537 x 333: 17 us with one, 19 with two).  The backward holds more per channel (two words spill 500 bytes) and
 // takes one.
 static int scan_words(int64_t ds, int es) { return es == 2 && (ds % 128 == 0 || ds > 512) ? 2 : 1; }
 
