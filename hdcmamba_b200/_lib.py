@@ -87,6 +87,21 @@ SIGNATURES = {
     "hdc_group_norm_bwd_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64]),
     "hdc_group_norm_bwd": (c_int, [c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp,
                                    c_i64, c_i64, c_vp, c_vp, c_vp, c_size, c_i64, c_i64, c_i64, c_i64, c_int, c_vp]),
+    "hdc_decay_attn_segments": (c_i64, [c_i64, c_i64, c_i64]),
+    "hdc_decay_attn_fwd": (c_int, [c_int, *[c_vp, c_i64, c_i64, c_i64] * 3, c_vp, c_vp, c_float, c_vp, c_i64, c_i64,
+                                   c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp]),
+    "hdc_decay_attn_bwd_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64]),
+    "hdc_decay_attn_bwd": (c_int, [c_int, *[c_vp, c_i64, c_i64, c_i64] * 4, c_vp, c_vp, c_vp, c_float,
+                                   *[c_vp, c_i64, c_i64, c_i64] * 3, c_vp, c_vp, c_size, c_i64, c_i64, c_i64, c_i64,
+                                   c_vp]),
+    "hdc_decay_attn_step": (c_int, [c_int, *[c_vp, c_i64, c_i64] * 3, c_vp, c_vp, c_float, c_vp, c_i64, c_i64, c_vp,
+                                    c_i64, c_i64, c_i64, c_vp]),
+    "hdc_embedding_fwd": (c_int, [c_int, c_vp, c_int, c_vp, c_i64, c_vp, c_i64, c_float, c_i64, c_i64, c_i64, c_vp]),
+    "hdc_embedding_bwd_workspace_bytes": (c_size, [c_i64, c_i64, c_i64]),
+    "hdc_embedding_bwd": (c_int, [c_int, c_vp, c_int, c_vp, c_i64, c_vp, c_i64, c_float, c_i64, c_vp, c_size, c_i64,
+                                  c_i64, c_i64, c_vp]),
+    "hdc_clip_grads_workspace_bytes": (c_size, [c_i64]),
+    "hdc_clip_grads": (c_int, [c_i64, c_vp, c_vp, c_vp, c_vp, c_float, c_vp, c_vp, c_size, c_vp]),
     "hdc_peer_alloc": (c_int, [c_size, ctypes.POINTER(c_vp)]),
     "hdc_peer_free": (c_int, [c_vp]),
     "hdc_ipc_handle_bytes": (c_int, []),

@@ -1,0 +1,284 @@
+// Decayed linear attention: entry points, the joining of segments, and the single-token step.
+// The mathematics stands in decay_attn.cuh.
+#include "decay_attn.cuh"
+
+namespace hdc {
+
+// ---------------------------------------------------------------- segments joined
+// states[n] holds segment n's own sum; afterwards the state that enters it: run_{n+1} = e^len run_n + own_n
+// in the order of the pass, from `from` (or zeros); `to` (or NULL) takes the state behind the last one.
+// A thread per V elements of a state walks the segments; the loads of kAhead of them are in flight.
+template <int V>
+__global__ void __launch_bounds__(128) attn_join_kernel(float* states, const float* from, float* to, const float* g,
+                                                        int H, int L, int DD, int nseg, int seg, int backwards) {
+  constexpr int kAhead = 8;
+  const int64_t bh = blockIdx.x;
+  const int i = (blockIdx.y * blockDim.x + threadIdx.x) * V;
+  if (i >= DD) return;
+  const float d = g[bh % H];
+  const float whole = decay_pow(d, seg), rest = decay_pow(d, L - (nseg - 1) * seg);
+  float run[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) run[e] = from ? from[bh * DD + i + e] : 0.f;
+  float* s = states + bh * nseg * DD + i;
+  for (int n0 = 0; n0 < nseg; n0 += kAhead) {
+    float own[kAhead][V];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (n0 + k < nseg) {
+        const float* src = s + (int64_t)(backwards ? nseg - 1 - n0 - k : n0 + k) * DD;
+        if constexpr (V == 4) *reinterpret_cast<float4*>(own[k]) = *reinterpret_cast<const float4*>(src);
+        else own[k][0] = src[0];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int n = backwards ? nseg - 1 - n0 - k : n0 + k;
+      if (n0 + k < nseg) {
+        float* dst = s + (int64_t)n * DD;
+        if constexpr (V == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(run);
+        else dst[0] = run[0];
+        const float keep = n == nseg - 1 ? rest : whole;
+#pragma unroll
+        for (int e = 0; e < V; ++e) run[e] = fmaf(keep, run[e], own[k][e]);
+      }
+    }
+  }
+  if (!to) return;
+#pragma unroll
+  for (int e = 0; e < V; ++e) to[bh * DD + i + e] = run[e];
+}
+
+// ---------------------------------------------------------------- one token
+// S <- e S + k v', o = scale q' S.  A CTA per state and 4 * kCols columns: a thread has 4 columns of
+// every kRows-th row, all its loads in flight at once; the rows' parts of o are added in shared memory.
+// Bound by the state's traffic (read and written once) at large batches, by one load's latency and the
+// launch at small ones.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(128) attn_step_kernel(AttnView q, AttnView k, AttnView v, AttnView o, const float* g,
+                                                        const float* state, float* state_out, float scale, int H,
+                                                        int D) {
+  constexpr int kCols = 8, kRows = 16;
+  __shared__ float part[kRows][kCols * 4 + 1];
+  const int64_t bh = blockIdx.x;
+  const int b = (int)(bh / H), h = (int)(bh % H);
+  const int cg = threadIdx.x % kCols, rg = threadIdx.x / kCols;
+  const int c = (blockIdx.y * kCols + cg) * 4;
+  const T* qp = static_cast<const T*>(q.p) + b * q.sb + h * q.sh;
+  const T* kp = static_cast<const T*>(k.p) + b * k.sb + h * k.sh;
+  const T* vp = static_cast<const T*>(v.p) + b * v.sb + h * v.sh;
+  const float e = expf(g[h]);
+  float vv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) vv[j] = c + j < D ? to_f(vp[c + j]) : 0.f;
+  const float* s = state + bh * D * D;
+  float* t = state_out + bh * D * D;
+#pragma unroll
+  for (int i = 0; i < 128 / kRows; ++i) {
+    const int r = rg + i * kRows;
+    if (r >= D) continue;
+    const float kk = to_f(kp[r]), qq = to_f(qp[r]);
+    float x[4];
+    if constexpr (VEC) {
+      if (c >= D) continue;
+      const float4 w = *reinterpret_cast<const float4*>(s + r * D + c);
+      x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = c + j < D ? s[r * D + c + j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = fmaf(e, x[j], kk * vv[j]);
+      acc[j] = fmaf(qq, x[j], acc[j]);
+    }
+    if constexpr (VEC) {
+      *reinterpret_cast<float4*>(t + r * D + c) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < D) t[r * D + c + j] = x[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) part[rg][cg * 4 + j] = acc[j];
+  __syncthreads();
+  const int col = blockIdx.y * kCols * 4 + threadIdx.x;
+  if (threadIdx.x >= kCols * 4 || col >= D) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) sum += part[i][threadIdx.x];
+  static_cast<T*>(const_cast<void*>(o.p))[b * o.sb + h * o.sh + col] = from_f<T>(scale * sum);
+}
+
+// ---------------------------------------------------------------- plans and checks
+// Tokens of a segment, a function of the sizes alone (so that a forward and its gradient agree, and
+// results do not depend on the device's SM count): enough segments for some kCtas CTAs.
+static int64_t attn_seg(int64_t B, int64_t L, int64_t H) {
+  constexpr int64_t kCtas = 148 * 3;
+  const int64_t chunks = (L + kAttnChunk - 1) / kAttnChunk;
+  if (chunks < 1 || B < 1 || H < 1) return kAttnChunk;
+  int64_t want = kCtas / (B * H);
+  if (want < 1) want = 1;
+  if (want > chunks) want = chunks;
+  return (chunks + want - 1) / want * kAttnChunk;
+}
+static int64_t attn_nseg(int64_t B, int64_t L, int64_t H) {
+  const int64_t seg = attn_seg(B, L, H);
+  return (L + seg - 1) / seg;
+}
+
+static int attn_check(const char* what, int dtype, int64_t B, int64_t L, int64_t H, int64_t D) {
+  if (dtype != HDC_F32 && dtype != HDC_BF16) return fail(HDC_E_DTYPE, "%s: dtype %d", what, dtype);
+  if (B < 0 || L < 0 || H < 1 || D < 1 || D > 128 || L > (int64_t(1) << 30) || B > (int64_t(1) << 30) ||
+      H > (int64_t(1) << 20) || B * H * attn_nseg(B, L, H) >= (int64_t(1) << 31))
+    return fail(HDC_E_SHAPE, "%s: B=%lld, L=%lld in [0, 2^30], H=%lld in [1, 2^20], D=%lld in [1, 128]", what,
+                (long long)B, (long long)L, (long long)H, (long long)D);
+  return 0;
+}
+
+static bool off_type(const void* p, int dtype) {
+  return (reinterpret_cast<uintptr_t>(p) & (dtype == HDC_F32 ? 3u : 1u)) != 0;
+}
+
+// the heads' rows [B, L, H] of D elements of an output lie apart: by growing stride, each steps over all
+// that the ones before reach
+static bool heads_apart(const AttnView& v, int64_t B, int64_t L, int64_t H, int64_t D) {
+  int64_t n[3] = {B, L, H}, s[3] = {v.sb, v.st, v.sh};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] < 2) s[i] = 0;
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2 - i; ++j)
+      if (s[j] > s[j + 1]) {
+        int64_t t = s[j]; s[j] = s[j + 1]; s[j + 1] = t;
+        t = n[j]; n[j] = n[j + 1]; n[j + 1] = t;
+      }
+  int64_t reach = D;
+  for (int i = 0; i < 3; ++i) {
+    if (n[i] < 2) continue;
+    if (s[i] < reach) return false;
+    reach += (n[i] - 1) * s[i];
+  }
+  return true;
+}
+
+static int join(float* states, const float* from, float* to, const AttnParams& p, int64_t bh, int backwards,
+                cudaStream_t s) {
+  const int DD = p.D * p.D;
+  const bool vec = p.D % 2 == 0 && aligned16(states) && aligned16(from);
+  const int per = vec ? 512 : 128;
+  const dim3 grid((unsigned)bh, (unsigned)((DD + per - 1) / per));
+  if (vec) attn_join_kernel<4><<<grid, 128, 0, s>>>(states, from, to, p.g, p.H, p.L, DD, p.nseg, p.seg, backwards);
+  else attn_join_kernel<1><<<grid, 128, 0, s>>>(states, from, to, p.g, p.H, p.L, DD, p.nseg, p.seg, backwards);
+  return launch_status("attn_join_kernel");
+}
+
+static int copy_state(const char* what, const float* from, float* to, int64_t n, cudaStream_t s) {
+  if (!to) return HDC_OK;
+  const cudaError_t e = from ? cudaMemcpyAsync(to, from, (size_t)n * 4, cudaMemcpyDeviceToDevice, s)
+                             : cudaMemsetAsync(to, 0, (size_t)n * 4, s);
+  return e == cudaSuccess ? HDC_OK : fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+}
+
+}  // namespace hdc
+
+using namespace hdc;
+
+extern "C" int64_t hdc_decay_attn_segments(int64_t B, int64_t L, int64_t H) {
+  return L < 1 || B < 1 || H < 1 ? 0 : attn_nseg(B, L, H);
+}
+
+extern "C" int hdc_decay_attn_fwd(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,
+                                  int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
+                                  int64_t v_sh, const float* log_decay, const float* state_in, float scale, void* o,
+                                  int64_t o_sb, int64_t o_st, int64_t o_sh, float* state_out, float* states, int64_t B,
+                                  int64_t L, int64_t H, int64_t D, hdc_stream_t stream) {
+  if (int e = attn_check("decay_attn", dtype, B, L, H, D)) return e;
+  if (B == 0) return HDC_OK;
+  auto s = reinterpret_cast<cudaStream_t>(stream);
+  if (off_type(q, dtype) || off_type(k, dtype) || off_type(v, dtype) || off_type(o, dtype) ||
+      off_type(log_decay, HDC_F32) || off_type(state_in, HDC_F32) || off_type(state_out, HDC_F32) ||
+      off_type(states, HDC_F32))
+    return fail(HDC_E_ALIGN, "decay_attn: a pointer is not aligned to its type");
+  if (L == 0) return copy_state("decay_attn", state_in, state_out, B * H * D * D, s);
+  if (!q || !k || !v || !o || !log_decay || !states) return fail(HDC_E_NULL, "decay_attn: null pointer");
+  const AttnView Q{q, q_sb, q_st, q_sh}, K{k, k_sb, k_st, k_sh}, V{v, v_sb, v_st, v_sh}, O{o, o_sb, o_st, o_sh};
+  if (!heads_apart(O, B, L, H, D)) return fail(HDC_E_SHAPE, "decay_attn: rows of o overlap");
+  AttnParams p{};
+  p.g = log_decay; p.H = (int)H; p.L = (int)L; p.D = (int)D;
+  p.seg = (int)attn_seg(B, L, H); p.nseg = (int)attn_nseg(B, L, H);
+  p.pass[0] = {Q, K, V, O, states, 0, 0, scale, scale, 1.f};
+  const int64_t bh = B * H;
+  const bool f32 = dtype == HDC_F32;
+  if (int e = f32 ? attn_sums_f32(p, bh, s) : attn_sums_bf16(p, bh, s)) return e;
+  if (int e = join(states, state_in, state_out, p, bh, 0, s)) return e;
+  return f32 ? attn_out_f32(p, bh, 1, s) : attn_out_bf16(p, bh, 1, s);
+}
+
+extern "C" size_t hdc_decay_attn_bwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t D) {
+  return L < 1 || B < 1 || H < 1 || D < 1 ? 0 : (size_t)(B * H * attn_nseg(B, L, H)) * D * D * 4;
+}
+
+extern "C" int hdc_decay_attn_bwd(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,
+                                  int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
+                                  int64_t v_sh, const void* dout, int64_t do_sb, int64_t do_st, int64_t do_sh,
+                                  const float* log_decay, const float* states, const float* dstate_out, float scale,
+                                  void* dq, int64_t dq_sb, int64_t dq_st, int64_t dq_sh, void* dk, int64_t dk_sb,
+                                  int64_t dk_st, int64_t dk_sh, void* dv, int64_t dv_sb, int64_t dv_st, int64_t dv_sh,
+                                  float* dstate_in, void* workspace, size_t workspace_bytes, int64_t B, int64_t L,
+                                  int64_t H, int64_t D, hdc_stream_t stream) {
+  if (int e = attn_check("decay_attn_bwd", dtype, B, L, H, D)) return e;
+  if (B == 0) return HDC_OK;
+  auto s = reinterpret_cast<cudaStream_t>(stream);
+  if (off_type(q, dtype) || off_type(k, dtype) || off_type(v, dtype) || off_type(dout, dtype) || off_type(dq, dtype) ||
+      off_type(dk, dtype) || off_type(dv, dtype) || off_type(log_decay, HDC_F32) || off_type(states, HDC_F32) ||
+      off_type(dstate_out, HDC_F32) || off_type(dstate_in, HDC_F32))
+    return fail(HDC_E_ALIGN, "decay_attn_bwd: a pointer is not aligned to its type");
+  if (L == 0) return copy_state("decay_attn_bwd", dstate_out, dstate_in, B * H * D * D, s);
+  if (!q || !k || !v || !dout || !dq || !dk || !dv || !log_decay || !states)
+    return fail(HDC_E_NULL, "decay_attn_bwd: null pointer");
+  const size_t need = hdc_decay_attn_bwd_workspace_bytes(B, L, H, D);
+  if (!workspace || workspace_bytes < need)
+    return fail(HDC_E_WORKSPACE, "decay_attn_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  if (!aligned16(workspace)) return fail(HDC_E_ALIGN, "decay_attn_bwd: the workspace is not 16-byte aligned");
+  const AttnView Q{q, q_sb, q_st, q_sh}, K{k, k_sb, k_st, k_sh}, V{v, v_sb, v_st, v_sh}, DO{dout, do_sb, do_st, do_sh};
+  const AttnView DQ{dq, dq_sb, dq_st, dq_sh}, DK{dk, dk_sb, dk_st, dk_sh}, DV{dv, dv_sb, dv_st, dv_sh};
+  if (!heads_apart(DQ, B, L, H, D) || !heads_apart(DK, B, L, H, D) || !heads_apart(DV, B, L, H, D))
+    return fail(HDC_E_SHAPE, "decay_attn_bwd: rows of dq, dk or dv overlap");
+  float* grads = static_cast<float*>(workspace);
+  AttnParams p{};
+  p.g = log_decay; p.H = (int)H; p.L = (int)L; p.D = (int)D;
+  p.seg = (int)attn_seg(B, L, H); p.nseg = (int)attn_nseg(B, L, H);
+  const int64_t bh = B * H;
+  const bool f32 = dtype == HDC_F32;
+  p.pass[0] = {K, Q, DO, DV, grads, 0, 1, scale, 1.f, scale};
+  if (int e = f32 ? attn_sums_f32(p, bh, s) : attn_sums_bf16(p, bh, s)) return e;
+  if (int e = join(grads, dstate_out, dstate_in, p, bh, 1, s)) return e;
+  p.pass[1] = {V, DO, Q, DK, grads, 1, 1, scale, 1.f, scale};
+  p.pass[2] = {DO, V, K, DQ, const_cast<float*>(states), 1, 0, scale, scale, 1.f};
+  return f32 ? attn_out_f32(p, bh, 3, s) : attn_out_bf16(p, bh, 3, s);
+}
+
+extern "C" int hdc_decay_attn_step(int dtype, const void* q, int64_t q_sb, int64_t q_sh, const void* k, int64_t k_sb,
+                                   int64_t k_sh, const void* v, int64_t v_sb, int64_t v_sh, const float* log_decay,
+                                   const float* state, float scale, void* o, int64_t o_sb, int64_t o_sh,
+                                   float* state_out, int64_t B, int64_t H, int64_t D, hdc_stream_t stream) {
+  if (int e = attn_check("decay_attn_step", dtype, B, 1, H, D)) return e;
+  if (B == 0) return HDC_OK;
+  if (!q || !k || !v || !o || !log_decay || !state || !state_out)
+    return fail(HDC_E_NULL, "decay_attn_step: null pointer");
+  if (off_type(q, dtype) || off_type(k, dtype) || off_type(v, dtype) || off_type(o, dtype) ||
+      off_type(log_decay, HDC_F32) || off_type(state, HDC_F32) || off_type(state_out, HDC_F32))
+    return fail(HDC_E_ALIGN, "decay_attn_step: a pointer is not aligned to its type");
+  const AttnView Q{q, q_sb, 0, q_sh}, K{k, k_sb, 0, k_sh}, V{v, v_sb, 0, v_sh}, O{o, o_sb, 0, o_sh};
+  if (!heads_apart(O, B, 1, H, D)) return fail(HDC_E_SHAPE, "decay_attn_step: rows of o overlap");
+  auto s = reinterpret_cast<cudaStream_t>(stream);
+  const dim3 grid((unsigned)(B * H), (unsigned)((D + 31) / 32));
+  const bool vec = D % 4 == 0 && aligned16(state) && aligned16(state_out);
+  auto launch = [&](auto kernel) {
+    kernel<<<grid, 128, 0, s>>>(Q, K, V, O, log_decay, state, state_out, scale, (int)H, (int)D);
+  };
+  if (dtype == HDC_F32) vec ? launch(attn_step_kernel<float, true>) : launch(attn_step_kernel<float, false>);
+  else vec ? launch(attn_step_kernel<__nv_bfloat16, true>) : launch(attn_step_kernel<__nv_bfloat16, false>);
+  return launch_status("attn_step_kernel");
+}

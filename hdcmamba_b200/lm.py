@@ -18,6 +18,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .model import HdcMamba9v3Block, HdcMamba9v3Model, final_layer_norm
+from .training import embedding
 
 
 class HdcMambaLM(nn.Module):
@@ -38,7 +39,7 @@ class HdcMambaLM(nn.Module):
         self.norm = nn.LayerNorm(d_model)
 
     def hidden(self, ids):
-        h = self.embedding(ids)  # a fresh activation: the layers update it in place
+        h = embedding(ids, self.embedding.weight)  # a fresh activation: the layers update it in place
         if self.use_model:
             return self.backbone._forward(h, owns_input=True)
         for layer in self.layers:

@@ -3,7 +3,8 @@
 The Block's SSM and slot kernels follow the reference's forward and have no gradient
 (hdcmamba/model.py:175-295).  ``gated_scan`` and ``group_norm_act`` are the operators to
 train such a layer with: the SSM's gates as one exact recurrence over the sequence, and the
-GroupNorm of each head with SiLU, both with hand-written backward kernels.
+GroupNorm of each head with SiLU, both with hand-written backward kernels.  ``decay_attention``
+is the slot memory's counterpart: linear attention with a decay for each head.
 ``GatedRecurrentBlock`` joins them with the Block's LayerNorm + conv.  That one's gradient here
 (``norm_conv1d``) is the derivative of its forward; ``fused_norm_conv1d_trainable`` keeps the
 reference's formulas, which leave the norm bias and the rows before the sequence out of two
@@ -25,14 +26,15 @@ import torch.nn.functional as F
 from . import ops
 from .model import _require_cuda
 
-__all__ = ["norm_conv1d", "gated_scan", "group_norm_act", "NormConv1dFunction", "GatedScanFunction",
-           "GroupNormActFunction", "GatedRecurrentBlock", "RecurrentState"]
+__all__ = ["norm_conv1d", "gated_scan", "group_norm_act", "decay_attention", "NormConv1dFunction", "GatedScanFunction",
+           "GroupNormActFunction", "DecayAttentionFunction", "GatedRecurrentBlock", "RecurrentState"]
 
 
 def _first_order_only():
     """Gradients of the gradients are not implemented: an error rather than missing terms."""
     if torch.is_grad_enabled():  # only with create_graph=True
-        raise RuntimeError("hdcmamba_b200: norm_conv1d, gated_scan and group_norm_act are differentiable once (create_graph=False)")
+        raise RuntimeError("hdcmamba_b200: norm_conv1d, gated_scan, group_norm_act, decay_attention and embedding are "
+                           "differentiable once (create_graph=False)")
 
 
 class NormConv1dFunction(torch.autograd.Function):
@@ -133,6 +135,45 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none"):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return GroupNormActFunction.apply(x, weight, bias, num_groups, eps, act)
     return ops.group_norm_act(x, num_groups, weight, bias, eps=eps, act=act)
+
+
+class DecayAttentionFunction(torch.autograd.Function):
+    """(q, k, v, log_decay, state, scale) -> (o, state after); gradients for q, k, v and state
+    (hdc_decay_attn_fwd / hdc_decay_attn_bwd)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, scale):
+        ctx.scale, ctx.state_dtype = scale, state.dtype if state is not None else None
+        state = state.float().contiguous() if state is not None else None
+        o, after, states = ops.decay_attention(q, k, v, log_decay, scale, state, return_states=True)
+        ctx.save_for_backward(q, k, v, log_decay, states)
+        ctx.set_materialize_grads(False)
+        return o, after
+
+    @staticmethod
+    def backward(ctx, do, dafter):
+        _first_order_only()
+        q, k, v, log_decay, states = ctx.saved_tensors
+        if do is None:
+            do = torch.zeros(q.shape, device=q.device, dtype=q.dtype)
+        if dafter is not None:
+            dafter = dafter.contiguous()
+        # the forward has checked the arguments
+        dq, dk, dv, dstate = ops._decay_attention_bwd(ops._code(q), do, q, k, v, log_decay.float().contiguous(), states,
+                                                      ctx.scale, dafter, ctx.needs_input_grad[4])
+        return dq, dk, dv, None, dstate.to(ctx.state_dtype) if dstate is not None else None, None
+
+
+def decay_attention(q, k, v, log_decay, scale=1.0, state=None):
+    """Differentiable ``ops.decay_attention``: (o, state after the last token).  The states carry
+    gradients, so a sequence can be trained window by window; the decays are constants."""
+    _require_cuda(q)
+    if log_decay.requires_grad:
+        raise ValueError("decay_attention has no gradient for log_decay: pass a constant (log_decay.detach())")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    (state is not None and state.requires_grad)):
+        return DecayAttentionFunction.apply(q, k, v, log_decay, state, scale)
+    return ops.decay_attention(q, k, v, log_decay, scale, state)
 
 
 @dataclass

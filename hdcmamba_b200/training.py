@@ -1,0 +1,66 @@
+"""What a training step of an LM needs beside its layers (hdcmamba_b200/recurrent.py): the token
+embedding with its gradient, and clipping by the norm over all gradients.
+
+    h = embedding(ids, lm.embedding.weight)           # rows, differentiable
+    loss.backward()
+    norm = clip_grad_norm_(model.parameters(), 1.0)   # stays on the device
+    optimizer.step()
+
+There is no CPU path: CPU inputs raise.
+"""
+import torch
+
+from . import ops
+from .model import _require_cuda
+from .recurrent import _first_order_only
+
+__all__ = ["embedding", "clip_grad_norm_", "EmbeddingFunction"]
+
+
+class EmbeddingFunction(torch.autograd.Function):
+    """(ids, weight, scale, padding_idx) -> rows of weight; gradient for weight
+    (hdc_embedding_fwd / hdc_embedding_bwd)."""
+
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.rows, ctx.scale, ctx.padding_idx = weight.shape[0], scale, padding_idx
+        return ops.embedding(ids, weight, scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        _first_order_only()
+        (ids,) = ctx.saved_tensors
+        return None, ops.embedding_bwd(dy, ids, ctx.rows, ctx.scale, ctx.padding_idx), None, None
+
+
+def embedding(ids, weight, scale=1.0, padding_idx=None):
+    """Differentiable ``ops.embedding``: ids.shape + [D].  ``padding_idx``: an id whose tokens take no
+    part in the gradient (their rows are looked up like any other)."""
+    _require_cuda(ids)
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError(f"padding_idx {padding_idx} is outside the table of {weight.shape[0]} rows")
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return EmbeddingFunction.apply(ids, weight, scale, padding_idx)
+    return ops.embedding(ids, weight, scale)
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm):
+    """Scale the gradients of ``parameters`` (a tensor or an iterable) in place so that the norm over all
+    of them is at most ``max_norm``; returns the norm before (fp32 on the device, which the host does
+    not wait for).  Gradients are fp32 or bf16, mixed as they come; parameters without one are left out."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    if all(g.is_contiguous() for g in grads):
+        return ops.clip_grads(grads, max_norm)
+    # gradients in another order of memory: scaled in a copy
+    rows = [g.contiguous() for g in grads]
+    norm = ops.clip_grads(rows, max_norm)
+    for g, r in zip(grads, rows):
+        if r is not g:
+            g.copy_(r)
+    return norm

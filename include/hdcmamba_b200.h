@@ -452,6 +452,80 @@ int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_t dy_sn, in
                        int64_t S, int64_t C, int64_t G, int act, hdc_stream_t stream);
 
 /*
+ * Linear attention with a decay for each head, with gradient and single-token step: the Block's slot
+ * memory (hdcmamba/model.py:236-272) without its feature map, chunks and bf16 rounding points.  Per batch
+ * and head, from S_{-1} = state_in (or zeros):
+ *   S_t = exp(log_decay_h) S_{t-1} + k_t v_t',   o_t = scale * q_t' S_t.
+ * dtype is that of q, k, v, o, dout, dq, dk, dv: element (b, t, h, d) of q at
+ * q + b*q_sb + t*q_st + h*q_sh + d (elements; any strides, 0 for heads that share k or v), the others
+ * likewise.  log_decay fp32 [H], constants (no gradient), meant to be <= 0.  States fp32 [B, H, D, D],
+ * row i belonging to k's element i.  Products of bf16 tensors run on the tensor cores with fp32 sums; a
+ * token's infinities and NaN may also reach the up to 63 tokens before it.
+ *   state_in, state_out : NULL or fp32 [B, H, D, D]; may be the same.
+ *   states : fp32 [B, H, hdc_decay_attn_segments(B, L, H), D, D]: the states between the sequence's
+ *            segments, which the gradient starts from.
+ * hdc_decay_attn_bwd: states as the forward left them; dstate_out NULL or the gradient of state_out;
+ *   writes dq, dk, dv and, unless NULL, dstate_in (may be dstate_out).  workspace:
+ *   hdc_decay_attn_bwd_workspace_bytes, 16-byte aligned.
+ * hdc_decay_attn_step: one token per sequence, q [B, H, D] (strides q_sb, q_sh); state_out may be state.
+ * D in [1, 128], B, L in [0, 2^30], H in [1, 2^20], B * H * segments < 2^31.  Rows of o, dq, dk and dv must
+ * not overlap, nor the outputs the inputs.  Pointers need their type's alignment; 16-byte aligned heads
+ * take the wide loads.  Results do not depend on timing.
+ */
+int64_t hdc_decay_attn_segments(int64_t B, int64_t L, int64_t H);
+int hdc_decay_attn_fwd(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,
+                       int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
+                       int64_t v_sh, const float* log_decay, const float* state_in, float scale, void* o,
+                       int64_t o_sb, int64_t o_st, int64_t o_sh, float* state_out, float* states, int64_t B,
+                       int64_t L, int64_t H, int64_t D, hdc_stream_t stream);
+size_t hdc_decay_attn_bwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t D);
+int hdc_decay_attn_bwd(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,
+                       int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
+                       int64_t v_sh, const void* dout, int64_t do_sb, int64_t do_st, int64_t do_sh,
+                       const float* log_decay, const float* states, const float* dstate_out, float scale,
+                       void* dq, int64_t dq_sb, int64_t dq_st, int64_t dq_sh, void* dk, int64_t dk_sb,
+                       int64_t dk_st, int64_t dk_sh, void* dv, int64_t dv_sb, int64_t dv_st, int64_t dv_sh,
+                       float* dstate_in, void* workspace, size_t workspace_bytes, int64_t B, int64_t L,
+                       int64_t H, int64_t D, hdc_stream_t stream);
+int hdc_decay_attn_step(int dtype, const void* q, int64_t q_sb, int64_t q_sh, const void* k, int64_t k_sb,
+                        int64_t k_sh, const void* v, int64_t v_sb, int64_t v_sh, const float* log_decay,
+                        const float* state, float scale, void* o, int64_t o_sb, int64_t o_sh,
+                        float* state_out, int64_t B, int64_t H, int64_t D, hdc_stream_t stream);
+
+/*
+ * Token embedding with gradient (the LM wrappers' nn.Embedding, train.py:116-137):
+ *   y_n = scale * table[id_n],   dtable[v] = scale * sum over id_n = v of dy_n   (every row written).
+ * dtype is that of table, y, dy and dtable; sums in fp32, over a row's tokens in their order.
+ *   ids : [N] of id_bytes = 4 or 8 (int32, int64).  An id outside [0, rows) gives a row of NaN, no part
+ *         of the gradient, and 71 through hdc_device_error().
+ *   table : row v at table + v*table_st (elements); y, dy, dtable likewise.
+ *   skip_id : an id that takes no part in the gradient (padding); -1 for none.
+ * N, rows in [0 or 1, 2^30], D in [1, 65536].  Rows of y and of dtable must not overlap.  Pointers need
+ * their type's alignment; 16-byte aligned rows take the wide loads.  workspace:
+ * hdc_embedding_bwd_workspace_bytes, 16-byte aligned.
+ */
+int hdc_embedding_fwd(int dtype, const void* ids, int id_bytes, const void* table, int64_t table_st, void* y,
+                      int64_t y_st, float scale, int64_t N, int64_t rows, int64_t D, hdc_stream_t stream);
+size_t hdc_embedding_bwd_workspace_bytes(int64_t N, int64_t rows, int64_t D);
+int hdc_embedding_bwd(int dtype, const void* ids, int id_bytes, const void* dy, int64_t dy_st, void* dtable,
+                      int64_t dtable_st, float scale, int64_t skip_id, void* workspace, size_t workspace_bytes,
+                      int64_t N, int64_t rows, int64_t D, hdc_stream_t stream);
+
+/*
+ * The norm over all gradients of a model and the gradients scaled to it (the clipping of a training loop):
+ *   norm = sqrt(sum of all squares),  out = grad * min(1, max_norm / (norm + 1e-6)).
+ * n tensors (0 to 2^20), each contiguous with numels[i] elements of dtypes[i]; dtypes, grads, outs and
+ * numels are host arrays that the call has read when it returns.  outs NULL: the norm alone.  outs[i] may
+ * be grads[i], but may not overlap another tensor's output or gradient.  norm: device fp32.  A norm that is
+ * not finite scales as the formula says (infinity: zeros, and NaN where the gradient is infinite; NaN: NaN).
+ * workspace: hdc_clip_grads_workspace_bytes(n), 16-byte aligned.  Sums in a fixed order.
+ */
+size_t hdc_clip_grads_workspace_bytes(int64_t n);
+int hdc_clip_grads(int64_t n, const int* dtypes, const void* const* grads, void* const* outs,
+                   const int64_t* numels, float max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                   hdc_stream_t stream);
+
+/*
  * Peer-memory exchange for sequence parallelism (one process per GPU, NVLink / NVSwitch).
  * No reference counterpart: it replaces the all-gathers of the sequence-parallel runner
  * with direct peer stores where the data flow is one-directional (rank r needs the carries
