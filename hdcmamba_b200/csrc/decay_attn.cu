@@ -141,6 +141,11 @@ static bool off_type(const void* p, int dtype) {
   return (reinterpret_cast<uintptr_t>(p) & (dtype == HDC_F32 ? 3u : 1u)) != 0;
 }
 
+// a tensor's view; the stride of a dimension of one does not count
+static AttnView view_of(const void* p, int64_t sb, int64_t st, int64_t sh, int64_t B, int64_t L, int64_t H) {
+  return {p, B > 1 ? sb : 0, L > 1 ? st : 0, H > 1 ? sh : 0};
+}
+
 // the heads' rows [B, L, H] of D elements of an output lie apart: by growing stride, each steps over all
 // that the ones before reach
 static bool heads_apart(const AttnView& v, int64_t B, int64_t L, int64_t H, int64_t D) {
@@ -202,7 +207,9 @@ extern "C" int hdc_decay_attn_fwd(int dtype, const void* q, int64_t q_sb, int64_
     return fail(HDC_E_ALIGN, "decay_attn: a pointer is not aligned to its type");
   if (L == 0) return copy_state("decay_attn", state_in, state_out, B * H * D * D, s);
   if (!q || !k || !v || !o || !log_decay || !states) return fail(HDC_E_NULL, "decay_attn: null pointer");
-  const AttnView Q{q, q_sb, q_st, q_sh}, K{k, k_sb, k_st, k_sh}, V{v, v_sb, v_st, v_sh}, O{o, o_sb, o_st, o_sh};
+  auto view = [&](const void* t, int64_t sb, int64_t st, int64_t sh) { return view_of(t, sb, st, sh, B, L, H); };
+  const AttnView Q = view(q, q_sb, q_st, q_sh), K = view(k, k_sb, k_st, k_sh), V = view(v, v_sb, v_st, v_sh),
+                 O = view(o, o_sb, o_st, o_sh);
   if (!heads_apart(O, B, L, H, D)) return fail(HDC_E_SHAPE, "decay_attn: rows of o overlap");
   AttnParams p{};
   p.g = log_decay; p.H = (int)H; p.L = (int)L; p.D = (int)D;
@@ -241,8 +248,10 @@ extern "C" int hdc_decay_attn_bwd(int dtype, const void* q, int64_t q_sb, int64_
   if (!workspace || workspace_bytes < need)
     return fail(HDC_E_WORKSPACE, "decay_attn_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   if (!aligned16(workspace)) return fail(HDC_E_ALIGN, "decay_attn_bwd: the workspace is not 16-byte aligned");
-  const AttnView Q{q, q_sb, q_st, q_sh}, K{k, k_sb, k_st, k_sh}, V{v, v_sb, v_st, v_sh}, DO{dout, do_sb, do_st, do_sh};
-  const AttnView DQ{dq, dq_sb, dq_st, dq_sh}, DK{dk, dk_sb, dk_st, dk_sh}, DV{dv, dv_sb, dv_st, dv_sh};
+  auto view = [&](const void* t, int64_t sb, int64_t st, int64_t sh) { return view_of(t, sb, st, sh, B, L, H); };
+  const AttnView Q = view(q, q_sb, q_st, q_sh), K = view(k, k_sb, k_st, k_sh), V = view(v, v_sb, v_st, v_sh),
+                 DO = view(dout, do_sb, do_st, do_sh);
+  const AttnView DQ = view(dq, dq_sb, dq_st, dq_sh), DK = view(dk, dk_sb, dk_st, dk_sh), DV = view(dv, dv_sb, dv_st, dv_sh);
   if (!heads_apart(DQ, B, L, H, D) || !heads_apart(DK, B, L, H, D) || !heads_apart(DV, B, L, H, D))
     return fail(HDC_E_SHAPE, "decay_attn_bwd: rows of dq, dk or dv overlap");
   float* grads = static_cast<float*>(workspace);

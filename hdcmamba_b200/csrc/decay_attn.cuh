@@ -31,6 +31,7 @@ struct AttnPass {
   float* states;  // [B * H][nseg][D * D]: the state that enters each segment (the sums' kernel: each segment's own)
   int transposed, backwards;
   float sa, si, su;
+  int out_vec;  // out takes 16-byte stores
 };
 
 struct AttnParams {
@@ -42,10 +43,10 @@ struct AttnParams {
 // exp(g d), 1 for d = 0 whatever g is
 __device__ __forceinline__ float decay_pow(float g, int d) { return d == 0 ? 1.f : expf(g * (float)d); }
 
-// csrc/decay_attn_f32.cu: fp32 tensors
-int attn_sums_f32(const AttnParams& p, int64_t bh, cudaStream_t s);
-int attn_out_f32(const AttnParams& p, int64_t bh, int passes, cudaStream_t s);
-int attn_sums_bf16(const AttnParams& p, int64_t bh, cudaStream_t s);
-int attn_out_bf16(const AttnParams& p, int64_t bh, int passes, cudaStream_t s);
+// csrc/decay_attn_f32.cu, csrc/decay_attn_bf16.cu: the segments' own states (pass 0), and passes' outputs
+int attn_sums_f32(AttnParams& p, int64_t bh, cudaStream_t s);
+int attn_out_f32(AttnParams& p, int64_t bh, int passes, cudaStream_t s);
+int attn_sums_bf16(AttnParams& p, int64_t bh, cudaStream_t s);
+int attn_out_bf16(AttnParams& p, int64_t bh, int passes, cudaStream_t s);
 
 }  // namespace hdc

@@ -7,12 +7,12 @@ namespace hdc {
 
 constexpr int kPitchP = kAttnChunk + 4;
 
-template <typename T, int DP>
+template <int DP>
 __device__ __forceinline__ void load_rows(float* s, const AttnView& v, int64_t at, int t0, int n, int D) {
   for (int i = threadIdx.x; i < kAttnChunk * DP; i += 256) {
     const int r = i / DP, c = i % DP;
     float x = 0.f;
-    if (r < n && c < D) x = to_f(static_cast<const T*>(v.p)[at + (int64_t)(t0 + r) * v.st + c]);
+    if (r < n && c < D) x = static_cast<const float*>(v.p)[at + (int64_t)(t0 + r) * v.st + c];
     s[r * (DP + 4) + c] = x;
   }
 }
@@ -23,7 +23,7 @@ __device__ __forceinline__ float4 at4(const float* s, int r, int c) {
 }
 
 // 256 threads as 16 x 16: each has 4 x 4 values of a product's 64 x 64 (DP = 128: of each quarter).
-template <typename T, int DP, bool OUT>
+template <int DP, bool OUT>
 __global__ void __launch_bounds__(256) attn_simt_kernel(AttnParams p) {
   extern __shared__ float4 smem4[];
   constexpr int NT = DP / 64;
@@ -52,9 +52,9 @@ __global__ void __launch_bounds__(256) attn_simt_kernel(AttnParams p) {
   const int chunks = (end - begin + kAttnChunk - 1) / kAttnChunk;
   for (int q = 0; q < chunks; ++q) {
     const int t0 = begin + (a.backwards ? chunks - 1 - q : q) * kAttnChunk, n = min(kAttnChunk, end - t0);
-    load_rows<T, DP>(Y, a.y, ay, t0, n, D);
-    load_rows<T, DP>(Z, a.z, az, t0, n, D);
-    if (OUT) load_rows<T, DP>(X, a.x, ax, t0, n, D);
+    load_rows<DP>(Y, a.y, ay, t0, n, D);
+    load_rows<DP>(Z, a.z, az, t0, n, D);
+    if (OUT) load_rows<DP>(X, a.x, ax, t0, n, D);
     __syncthreads();
     if (OUT) {
       float s[4][4] = {};
@@ -117,12 +117,12 @@ __global__ void __launch_bounds__(256) attn_simt_kernel(AttnParams p) {
             }
           }
         }
-        T* out = static_cast<T*>(const_cast<void*>(a.out.p)) + b * a.out.sb + h * a.out.sh;
+        float* out = static_cast<float*>(const_cast<void*>(a.out.p)) + b * a.out.sb + h * a.out.sh;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (ty * 4 + i < n && c0 + j < D) out[(int64_t)(t0 + ty * 4 + i) * a.out.st + c0 + j] = from_f<T>(o[i][j]);
+            if (ty * 4 + i < n && c0 + j < D) out[(int64_t)(t0 + ty * 4 + i) * a.out.st + c0 + j] = o[i][j];
       }
       __syncthreads();
     }
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(256) attn_simt_kernel(AttnParams p) {
     for (int i = threadIdx.x; i < D * D; i += 256) state[i] = R[i / D * (DP + 4) + i % D];
 }
 
-template <typename T, int DP, bool OUT>
+template <int DP, bool OUT>
 static int attn_launch(const AttnParams& p, int64_t bh, int passes, cudaStream_t s) {
   constexpr int smem = 4 * (kAttnChunk * (DP + 4) * (OUT ? 3 : 2) + DP * (DP + 4) + (OUT ? kAttnChunk * kPitchP : 0));
   static std::atomic<uint64_t> ready{0};  // devices whose limit of shared memory is set
@@ -162,24 +162,18 @@ static int attn_launch(const AttnParams& p, int64_t bh, int passes, cudaStream_t
   cudaGetDevice(&dev);
   const uint64_t bit = uint64_t(1) << (dev & 63);
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    cudaFuncSetAttribute(attn_simt_kernel<T, DP, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaFuncSetAttribute(attn_simt_kernel<DP, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  attn_simt_kernel<T, DP, OUT><<<dim3((unsigned)(bh * p.nseg), 1, passes), 256, smem, s>>>(p);
+  attn_simt_kernel<DP, OUT><<<dim3((unsigned)(bh * p.nseg), 1, passes), 256, smem, s>>>(p);
   return launch_status(OUT ? "attn_simt_kernel" : "attn_simt_kernel (sums)");
 }
 
-int attn_sums_f32(const AttnParams& p, int64_t bh, cudaStream_t s) {
-  return p.D <= 64 ? attn_launch<float, 64, false>(p, bh, 1, s) : attn_launch<float, 128, false>(p, bh, 1, s);
+int attn_sums_f32(AttnParams& p, int64_t bh, cudaStream_t s) {
+  return p.D <= 64 ? attn_launch<64, false>(p, bh, 1, s) : attn_launch<128, false>(p, bh, 1, s);
 }
-int attn_out_f32(const AttnParams& p, int64_t bh, int passes, cudaStream_t s) {
-  return p.D <= 64 ? attn_launch<float, 64, true>(p, bh, passes, s) : attn_launch<float, 128, true>(p, bh, passes, s);
-}
-int attn_sums_bf16(const AttnParams& p, int64_t bh, cudaStream_t s) {
-  return p.D <= 64 ? attn_launch<__nv_bfloat16, 64, false>(p, bh, 1, s) : attn_launch<__nv_bfloat16, 128, false>(p, bh, 1, s);
-}
-int attn_out_bf16(const AttnParams& p, int64_t bh, int passes, cudaStream_t s) {
-  return p.D <= 64 ? attn_launch<__nv_bfloat16, 64, true>(p, bh, passes, s) : attn_launch<__nv_bfloat16, 128, true>(p, bh, passes, s);
+int attn_out_f32(AttnParams& p, int64_t bh, int passes, cudaStream_t s) {
+  return p.D <= 64 ? attn_launch<64, true>(p, bh, passes, s) : attn_launch<128, true>(p, bh, passes, s);
 }
 
 }  // namespace hdc
