@@ -19,17 +19,15 @@
 #include <atomic>
 
 #include "decay_attn.cuh"
+#include "vec.cuh"
 
 namespace hdc {
 
 using bf16 = __nv_bfloat16;
 
-// shared-memory tile [rows][DP] of bf16 in 16-byte units, swizzled so that eight neighbouring rows of one
-// unit lie in different banks
-template <int DP> __device__ __forceinline__ int unit_at(int row, int unit) {
-  if constexpr (DP == 32) return row * 4 + (unit ^ ((row >> 1) & 3));
-  else return row * (DP / 8) + (unit ^ (row & 7));
-}
+// A tile in shared memory: rows of DP values and 16 bytes more, so that eight neighbouring rows of one 16-byte
+// unit lie in different banks and every address is a lane's base and a constant.
+template <int DP> constexpr int kPitch = DP * 2 + 16;
 
 __device__ __forceinline__ uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -47,35 +45,28 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma0(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // from zero
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ float lo_f(uint32_t v) { return __uint_as_float(v << 16); }
-__device__ __forceinline__ float hi_f(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
-
-// One tile's rows [t0, t0 + n) to shared memory, zeros behind them.  CB: bytes that every row's pieces allow.
-template <int DP, int CB, int THREADS>
-__device__ __forceinline__ void load_tile(bf16* s, const bf16* p, int64_t st, int n, int D) {
-  constexpr int E = CB / 2;  // elements of a copy
-  constexpr int PER = DP / E;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < kAttnChunk * PER; i += THREADS) {
-    const int r = i / PER, c = i % PER * E;
-    if (c >= D) continue;
-    bf16* dst = s + unit_at<DP>(r, c / 8) * 8 + c % 8;
-    const bf16* src = p + (r < n ? r * st + c : 0);
-    if constexpr (CB == 2) {
-      *dst = r < n ? *src : __float2bfloat16(0.f);
-    } else {
-      const uint32_t d = shared_at(dst);
-      const int bytes = r < n ? CB : 0;
-      if constexpr (CB == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(bytes) : "memory");
-      else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(bytes) : "memory");
-    }
-  }
+// pairs of fp32 values: one instruction for two
+__device__ __forceinline__ void scale2(float& x, float& y, float f, float h) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(x, y)), "l"(pair_bits(f, h)));
+  bits_pair(r, x, y);
 }
-
+// (x, y) minus the two bf16 values of v
+__device__ __forceinline__ void less2(float& x, float& y, uint32_t v) {
+  uint64_t r;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(x, y)), "l"(pair_bits(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u))));
+  bits_pair(r, x, y);
+}
 template <bool FIRST, typename A, typename B> __device__ __forceinline__ auto& first_if(A& a, B& b) {
   if constexpr (FIRST) return a;
   else return b;
@@ -84,22 +75,65 @@ template <bool FIRST, typename A, typename B> __device__ __forceinline__ auto& f
 template <int DP> struct AttnShape {
   static constexpr int kWarps = DP == 128 ? 8 : 4;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kTile = kAttnChunk * DP;                   // elements of a tile
+  static constexpr int kTile = kAttnChunk * kPitch<DP>;           // bytes of a tile
   static constexpr int kStateCols = DP == 32 ? 16 : DP;           // a warp's columns of the state (16 rows)
   static constexpr int kOutCols = DP == 128 ? 64 : DP;            // a warp's columns of the outputs (16 tokens)
-  static constexpr int smem(bool out) { return 2 * ((out ? 3 : 2) * 2 * kTile + (out ? 2 * DP * DP : 0)); }
+  static constexpr int tiles(bool out) { return out ? 3 : 2; }    // of a stage
+  static constexpr int smem(bool out) { return 2 * tiles(out) * kTile + (out ? 2 * DP * kPitch<DP> : 0); }
   static constexpr int ctas(bool out) { return DP == 128 ? 1 : out ? 3 : 4; }
 };
+
+// One tile's rows, n of them from p on, to shared memory, zeros behind them.  CB: bytes that every row's pieces
+// allow.  Columns from D on are not touched.
+template <int DP, int CB, int T>
+__device__ __forceinline__ void load_tile(char* s, const bf16* p, int64_t st, int n, int D) {
+  constexpr int E = CB / 2, PER = DP / E, ROWS = T / PER > 0 ? T / PER : 1;
+  if constexpr (CB == 16) {
+    const int row = threadIdx.x / PER, col = threadIdx.x % PER * E;
+    if (col >= D) return;
+    uint32_t d = shared_at(s) + row * kPitch<DP> + col * 2;
+    const char* src = reinterpret_cast<const char*>(p + row * st + col);
+    const int64_t step = ROWS * st * 2;
+    if (n == kAttnChunk) {
+#pragma unroll
+      for (int m = 0; m < kAttnChunk / ROWS; ++m, src += step)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + m * ROWS * kPitch<DP>), "l"(src) : "memory");
+    } else {
+#pragma unroll
+      for (int m = 0; m < kAttnChunk / ROWS; ++m, src += step) {
+        const bool in = row + m * ROWS < n;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + m * ROWS * kPitch<DP>),
+                     "l"(in ? src : reinterpret_cast<const char*>(p)), "r"(in ? 16 : 0) : "memory");
+      }
+    }
+  } else {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kAttnChunk * PER; i += T) {
+      const int row = i / PER, col = i % PER * E;
+      if (col >= D) continue;
+      char* dst = s + row * kPitch<DP> + col * 2;
+      const bf16* src = p + (row < n ? row * st + col : 0);
+      if constexpr (CB == 2) {
+        *reinterpret_cast<bf16*>(dst) = row < n ? *src : __float2bfloat16(0.f);
+      } else {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(shared_at(dst)), "l"(src), "r"(row < n ? 4 : 0) : "memory");
+      }
+    }
+  }
+}
 
 template <int DP, bool OUT, int CB>
 __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(OUT)) attn_mma_kernel(const __grid_constant__ AttnParams p) {
   using Sh = AttnShape<DP>;
-  constexpr int T = Sh::kThreads, KD = DP / 16, SN = Sh::kStateCols / 8, ON = Sh::kOutCols / 8;
-  constexpr int SPLITS = OUT ? 2 : 3;
+  constexpr int T = Sh::kThreads, KD = DP / 16, SN = Sh::kStateCols / 8, ON = Sh::kOutCols / 8, PT = kPitch<DP>;
+  constexpr int SPLITS = OUT ? 2 : 3, STAGE = Sh::tiles(OUT) * Sh::kTile;
   extern __shared__ uint4 smem16[];
   __shared__ float pw[kAttnChunk + 1];
-  bf16* tiles = reinterpret_cast<bf16*>(smem16);
-  bf16* rbuf = tiles + (OUT ? 3 : 2) * 2 * Sh::kTile;
+  // in(i) si and up(j) su of a whole chunk; a short one of n tokens reads the one that counts from the chunk's
+  // end 64 - n further on
+  __shared__ float entry[2 * kAttnChunk], update[2 * kAttnChunk];
+  char* tiles = reinterpret_cast<char*>(smem16);
+  char* rbuf = tiles + 2 * STAGE;
   const AttnPass& a = p.pass[blockIdx.z];
   const int D = p.D, back = a.backwards;
   const int64_t bh = blockIdx.x / p.nseg;
@@ -112,15 +146,21 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
   const bf16* zp = static_cast<const bf16*>(a.z.p) + b * a.z.sb + h * a.z.sh;
   const bf16* xp = OUT ? static_cast<const bf16*>(a.x.p) + b * a.x.sb + h * a.x.sh : nullptr;
 
-  for (int i = threadIdx.x; i <= kAttnChunk; i += T) pw[i] = decay_pow(p.g[h], i);
+  const float gd = p.g[h];
+  for (int i = threadIdx.x; i < 2 * kAttnChunk; i += T) {
+    if (i <= kAttnChunk) pw[i] = decay_pow(gd, i);
+    const bool in = i < kAttnChunk;
+    entry[i] = in ? a.si * decay_pow(gd, back ? kAttnChunk - 1 - i : i + 1) : 0.f;
+    update[i] = in ? a.su * decay_pow(gd, back ? i + 1 : kAttnChunk - 1 - i) : 0.f;
+  }
   if (D < DP)  // columns that no copy reaches
-    for (int i = threadIdx.x; i < (OUT ? 3 : 2) * 2 * Sh::kTile / 8; i += T) smem16[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < 2 * STAGE / 16; i += T) smem16[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
 
   auto chunk_at = [&](int q) { return begin + (back ? chunks - 1 - q : q) * kAttnChunk; };
   auto load = [&](int q) {
     const int t0 = chunk_at(q), n = min(kAttnChunk, end - t0);
-    bf16* s = tiles + (q & 1) * (OUT ? 3 : 2) * Sh::kTile;
+    char* s = tiles + (q & 1) * STAGE;
     load_tile<DP, CB, T>(s, yp + (int64_t)t0 * a.y.st, a.y.st, n, D);
     load_tile<DP, CB, T>(s + Sh::kTile, zp + (int64_t)t0 * a.z.st, a.z.st, n, D);
     if (OUT) load_tile<DP, CB, T>(s + 2 * Sh::kTile, xp + (int64_t)t0 * a.x.st, a.x.st, n, D);
@@ -136,14 +176,11 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
   float R[SN][4];
   float* state = a.states + (bh * p.nseg + seg) * D * D;
   auto keep_copy = [&](int q) {  // bf16(R) for the next chunk's product
-    bf16* rb = rbuf + (q & 1) * DP * DP;
+    char* rb = rbuf + (q & 1) * DP * PT + (sr + g) * PT + sc * 2 + c * 4;
 #pragma unroll
     for (int n = 0; n < SN; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = sr + g + 8 * e, col = sc + 8 * n + 2 * c;
-        *reinterpret_cast<uint32_t*>(rb + unit_at<DP>(row, col / 8) * 8 + col % 8) = pack2(R[n][2 * e], R[n][2 * e + 1]);
-      }
+      for (int e = 0; e < 2; ++e) *reinterpret_cast<uint32_t*>(rb + e * 8 * PT + n * 16) = pack2(R[n][2 * e], R[n][2 * e + 1]);
   };
 #pragma unroll
   for (int n = 0; n < SN; ++n)
@@ -168,129 +205,148 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
       }
     }
   }
+  const float* far = pw + (back ? -16 * r - 15 : 16 * r - 7);
+  // one chunk: few products, whose roundings would not average out in the outputs, so P is split as well
+  const bool fine = p.L <= kAttnChunk;
 
-  // addresses of the four 8 x 8 blocks that a lane fetches: rows first (la), or columns first (lb)
-  const int la_row = lane % 8 + 8 * ((lane / 8) % 2), la_unit = lane / 16;
-  const int lb_row = lane % 8 + 8 * (lane / 16), lb_unit = (lane / 8) % 2;
+  // a lane's address of four 8 x 8 blocks: rows first (la), or columns first (lb)
+  const uint32_t la = (lane % 8 + 8 * ((lane / 8) % 2)) * PT + lane / 16 * 16;
+  const uint32_t lb = (lane % 8 + 8 * (lane / 16)) * PT + (lane / 8) % 2 * 16;
+  const uint32_t tiles_at = shared_at(tiles), rbuf_at = shared_at(rbuf) + la + oc * 2;
 
   for (int q = 0; q < chunks; ++q) {
-    const int t0 = chunk_at(q), n_rows = min(kAttnChunk, end - t0);
+    const int t0 = chunk_at(q), n_rows = min(kAttnChunk, end - t0), shift = kAttnChunk - n_rows;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();  // this chunk's tiles and bf16(R) are there; the other tiles and copy are no longer read
     if (q + 1 < chunks) load(q + 1);
-    bf16* Ys = tiles + (q & 1) * (OUT ? 3 : 2) * Sh::kTile;
-    const uint32_t Y = shared_at(Ys), Z = Y + Sh::kTile * 2, X = Z + Sh::kTile * 2;
-    uint32_t P[4][4];
+    char* stage = tiles + (q & 1) * STAGE;
+    const uint32_t Y = tiles_at + (q & 1) * STAGE, Z = Y + Sh::kTile, X = Z + Sh::kTile;
     float O[OUT ? ON : 1][4];
+    uint32_t x[OUT ? KD : 1][4];
     if constexpr (OUT) {
-      const uint32_t Rb = shared_at(rbuf + (q & 1) * DP * DP);
-#pragma unroll
-      for (int n = 0; n < ON; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) O[n][e] = 0.f;
+      const uint32_t Rb = rbuf_at + (q & 1) * DP * PT, Xa = X + 16 * r * PT + la;
 #pragma unroll
       for (int k = 0; k < KD; ++k) {
-        uint32_t x[4];
-        ldm4(x, X + unit_at<DP>(16 * r + la_row, 2 * k + la_unit) * 16);
+        ldm4(x[k], Xa + k * 32);
 #pragma unroll
         for (int n = 0; n < ON; n += 2) {
           uint32_t w[4];
-          ldm4t(w, Rb + unit_at<DP>(16 * k + la_row, oc / 8 + n + la_unit) * 16);
-          mma(O[n], x, w[0], w[1]);
-          mma(O[n + 1], x, w[2], w[3]);
-        }
-      }
-      const int i0 = 16 * r + g, i1 = i0 + 8;
-      const float f0 = a.si * pw[back ? max(n_rows - 1 - i0, 0) : i0 + 1], f1 = a.si * pw[back ? max(n_rows - 1 - i1, 0) : i1 + 1];
-#pragma unroll
-      for (int n = 0; n < ON; ++n) { O[n][0] *= f0; O[n][1] *= f0; O[n][2] *= f1; O[n][3] *= f1; }
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        if (back ? s < r : s > r) continue;
-        float S[2][4] = {};
-#pragma unroll
-        for (int k = 0; k < KD; ++k) {
-          uint32_t x[4], w[4];
-          ldm4(x, X + unit_at<DP>(16 * r + la_row, 2 * k + la_unit) * 16);
-          ldm4(w, Y + unit_at<DP>(16 * s + lb_row, 2 * k + lb_unit) * 16);
-          mma(S[0], x, w[0], w[1]);
-          mma(S[1], x, w[2], w[3]);
-        }
-        if (s == r) {
-#pragma unroll
-          for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) S[m][e] *= diag[m * 4 + e];
-        } else {
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            const float far = pw[back ? 16 * (s - r) + 8 * m - 15 : 16 * (r - s) - 8 * m - 7];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) S[m][e] *= far * near4[e];
+          ldm4t(w, Rb + 16 * k * PT + n * 16);
+          if (k == 0) {
+            mma0(O[n], x[k], w[0], w[1]);
+            mma0(O[n + 1], x[k], w[2], w[3]);
+          } else {
+            mma(O[n], x[k], w[0], w[1]);
+            mma(O[n + 1], x[k], w[2], w[3]);
           }
         }
-        P[s][0] = pack2(S[0][0], S[0][1]);
-        P[s][1] = pack2(S[0][2], S[0][3]);
-        P[s][2] = pack2(S[1][0], S[1][1]);
-        P[s][3] = pack2(S[1][2], S[1][3]);
+      }
+      const float* in = entry + 16 * r + g + (back ? shift : 0);
+      const float f0 = in[0], f1 = in[8];
+#pragma unroll
+      for (int n = 0; n < ON; ++n) {
+        scale2(O[n][0], O[n][1], f0, f0);
+        scale2(O[n][2], O[n][3], f1, f1);
       }
     }
     // the state decays over the chunk; the sums' kernel adds a chunk's products up apart
     const float keep = pw[n_rows];
     float U[OUT ? 1 : SN][4];
 #pragma unroll
-    for (int n = 0; n < SN; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        R[n][e] *= keep;
-        if constexpr (!OUT) U[n][e] = 0.f;
-      }
+    for (int n = 0; n < SN; ++n) {
+      scale2(R[n][0], R[n][1], keep, keep);
+      scale2(R[n][2], R[n][3], keep, keep);
+    }
     auto& acc = first_if<OUT>(R, U);
+    const float* up = update + 2 * c + (back ? 0 : shift);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      uint32_t y[4], part[SPLITS][4];
-      ldm4t(y, Y + unit_at<DP>(16 * s + lb_row, sr / 8 + lb_unit) * 16);
-      float w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = 16 * s + 2 * c + (e & 1) + 8 * (e >> 1);
-        w[e] = a.su * pw[back ? j + 1 : max(n_rows - 1 - j, 0)];
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {  // y[0], y[1]: tokens 2 c, 2 c + 1; y[2], y[3]: 8 further
-        float lo = lo_f(y[e]) * w[e & 2], hi = hi_f(y[e]) * w[(e & 2) + 1];
-#pragma unroll
-        for (int k = 0; k < SPLITS; ++k) {
-          part[k][e] = pack2(lo, hi);
-          lo -= lo_f(part[k][e]);
-          hi -= hi_f(part[k][e]);
-        }
-      }
       const bool mine = OUT && !(back ? s < r : s > r);
+      uint32_t P[4], P2[4];
+      if constexpr (OUT) {
+        if (mine) {
+          float S[2][4];
 #pragma unroll
-      for (int n = 0; n < SN; n += 2) {
-        uint32_t w4[4];
-        ldm4t(w4, Z + unit_at<DP>(16 * s + la_row, sc / 8 + n + la_unit) * 16);
+          for (int k = 0; k < KD; ++k) {
+            uint32_t w[4];
+            ldm4(w, Y + lb + 16 * s * PT + k * 32);
+            if (k == 0) {
+              mma0(S[0], x[k], w[0], w[1]);
+              mma0(S[1], x[k], w[2], w[3]);
+            } else {
+              mma(S[0], x[k], w[0], w[1]);
+              mma(S[1], x[k], w[2], w[3]);
+            }
+          }
+          if (s == r) {
 #pragma unroll
-        for (int k = SPLITS - 1; k >= 0; --k) {
-          mma(acc[n], part[k], w4[0], w4[1]);
-          mma(acc[n + 1], part[k], w4[2], w4[3]);
-        }
-        if constexpr (OUT && DP == 64) {  // the outputs' columns are the state's
-          if (mine) {
-            mma(O[n], P[s], w4[0], w4[1]);
-            mma(O[n + 1], P[s], w4[2], w4[3]);
+            for (int m = 0; m < 2; ++m) {
+              scale2(S[m][0], S[m][1], diag[m * 4], diag[m * 4 + 1]);
+              scale2(S[m][2], S[m][3], diag[m * 4 + 2], diag[m * 4 + 3]);
+            }
+          } else {
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              const float f = back ? far[16 * s + 8 * m] : far[-16 * s - 8 * m];
+              float e[4] = {near4[0], near4[1], near4[2], near4[3]};
+              scale2(e[0], e[1], f, f);
+              scale2(e[2], e[3], f, f);
+              scale2(S[m][0], S[m][1], e[0], e[1]);
+              scale2(S[m][2], S[m][3], e[2], e[3]);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) P[e] = pack2(S[e >> 1][2 * (e & 1)], S[e >> 1][2 * (e & 1) + 1]);
+          if (fine) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              less2(S[e >> 1][2 * (e & 1)], S[e >> 1][2 * (e & 1) + 1], P[e]);
+              P2[e] = pack2(S[e >> 1][2 * (e & 1)], S[e >> 1][2 * (e & 1) + 1]);
+            }
           }
         }
       }
-      if constexpr (OUT && DP != 64) {
+      uint32_t y[4], part[SPLITS][4], z[SN][2];
+      ldm4t(y, Y + lb + 16 * s * PT + sr * 2);
+#pragma unroll
+      for (int n = 0; n < SN; n += 2) {
+        uint32_t w[4];
+        ldm4t(w, Z + la + 16 * s * PT + sc * 2 + n * 16);
+        z[n][0] = w[0]; z[n][1] = w[1]; z[n + 1][0] = w[2]; z[n + 1][1] = w[3];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // y[0], y[1]: tokens 2 c, 2 c + 1 of the 16; y[2], y[3]: 8 further
+        float lo = __uint_as_float(y[e] << 16), hi = __uint_as_float(y[e] & 0xffff0000u);
+        scale2(lo, hi, up[16 * s + 4 * (e & 2)], up[16 * s + 4 * (e & 2) + 1]);
+#pragma unroll
+        for (int k = 0; k < SPLITS; ++k) {
+          part[k][e] = pack2(lo, hi);
+          if (k + 1 < SPLITS) less2(lo, hi, part[k][e]);
+        }
+      }
+#pragma unroll
+      for (int k = SPLITS - 1; k >= 0; --k)
+#pragma unroll
+        for (int n = 0; n < SN; ++n) {
+          if (!OUT && s == 0 && k == SPLITS - 1) mma0(acc[n], part[k], z[n][0], z[n][1]);
+          else mma(acc[n], part[k], z[n][0], z[n][1]);
+        }
+      if constexpr (OUT) {
         if (mine) {
 #pragma unroll
           for (int n = 0; n < ON; n += 2) {
-            uint32_t w4[4];
-            ldm4t(w4, Z + unit_at<DP>(16 * s + la_row, oc / 8 + n + la_unit) * 16);
-            mma(O[n], P[s], w4[0], w4[1]);
-            mma(O[n + 1], P[s], w4[2], w4[3]);
+            uint32_t w[4];
+            if constexpr (DP == 64) {  // the outputs' columns are the state's
+              w[0] = z[n][0]; w[1] = z[n][1]; w[2] = z[n + 1][0]; w[3] = z[n + 1][1];
+            } else {
+              ldm4t(w, Z + la + 16 * s * PT + oc * 2 + n * 16);
+            }
+            mma(O[n], P, w[0], w[1]);
+            mma(O[n + 1], P, w[2], w[3]);
+            if (fine) {
+              mma(O[n], P2, w[0], w[1]);
+              mma(O[n + 1], P2, w[2], w[3]);
+            }
           }
         }
       }
@@ -301,29 +357,33 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
 #pragma unroll
         for (int e = 0; e < 4; ++e) R[n][e] += U[n][e];
     } else {
-      keep_copy(q + 1);
+      if (q + 1 < chunks) keep_copy(q + 1);
       bf16* out = static_cast<bf16*>(const_cast<void*>(a.out.p)) + b * a.out.sb + h * a.out.sh + (int64_t)t0 * a.out.st;
       // through the strip's own rows of X, which no other warp reads (wide heads: the strip's second warp)
-      bf16* Xs = Ys + 2 * Sh::kTile;
+      char* Xs = stage + 2 * Sh::kTile + 16 * r * PT + oc * 2;
       if constexpr (DP == 128) asm volatile("bar.sync %0, 64;" ::"r"(1 + r) : "memory");
       else __syncwarp();
 #pragma unroll
       for (int n = 0; n < ON; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<uint32_t*>(Xs + unit_at<DP>(16 * r + g + 8 * e, oc / 8 + n) * 8 + 2 * c) = pack2(O[n][2 * e], O[n][2 * e + 1]);
+          *reinterpret_cast<uint32_t*>(Xs + (g + 8 * e) * PT + n * 16 + c * 4) = pack2(O[n][2 * e], O[n][2 * e + 1]);
       __syncwarp();
       if (a.out_vec) {
+        const int col = lane % ON * 8;
+        if (oc + col < D) {
 #pragma unroll
-        for (int i = lane; i < 16 * ON; i += 32) {
-          const int row = 16 * r + i / ON, col = oc + i % ON * 8;
-          if (row < n_rows && col < D)
-            stg16(out + row * a.out.st + col, *reinterpret_cast<const uint4*>(Xs + unit_at<DP>(row, col / 8) * 8));
+          for (int m = 0; m < ON / 2; ++m) {
+            const int row = lane / ON + m * (32 / ON);
+            if (16 * r + row < n_rows)
+              stg16(out + (16 * r + row) * a.out.st + oc + col, *reinterpret_cast<const uint4*>(Xs + row * PT + col * 2));
+          }
         }
       } else {
         for (int i = lane; i < 16 * 8 * ON; i += 32) {
-          const int row = 16 * r + i / (8 * ON), col = oc + i % (8 * ON);
-          if (row < n_rows && col < D) out[row * a.out.st + col] = Xs[unit_at<DP>(row, col / 8) * 8 + col % 8];
+          const int row = i / (8 * ON), col = i % (8 * ON);
+          if (16 * r + row < n_rows && oc + col < D)
+            out[(16 * r + row) * a.out.st + oc + col] = *reinterpret_cast<const bf16*>(Xs + row * PT + col * 2);
         }
       }
     }
