@@ -118,6 +118,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_host = None
 _lock = threading.Lock()
 
 
@@ -141,6 +142,19 @@ def load():
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+def host():
+    """The module of the operators whose host path is C++ (csrc/host.cpp), loaded once."""
+    global _host
+    if _host is None:
+        load()
+        if not os.path.exists(os.path.join(HERE, "_host.so")):
+            raise OSError(f"{HERE}/_host.so is missing: build it with `python -m hdcmamba_b200.build`")
+        from . import _host as m
+        m.set_error(HdcError)
+        _host = m
+    return _host
 
 
 def call(name, *args):

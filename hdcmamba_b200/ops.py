@@ -804,34 +804,6 @@ def _group_norm_bwd(dy, x, mean, rstd, num_groups, weight, bias, act, need_param
 
 
 # ------------------------------------------------------------------ linear attention with a decay for each head
-def _heads(t, shape, what):
-    """t as a tensor of ``shape`` [..., H, D] whose last dim has unit stride."""
-    if t.shape != shape:
-        raise ValueError(f"{what} must be {list(shape)}, got {list(t.shape)}")
-    if shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{what} needs a unit stride within a head")
-
-
-def _decay_args(q, k, v, log_decay, dims, *states):
-    """Checks shared by the decayed-attention ops; returns (dtype code, log_decay as fp32)."""
-    _cuda(q, k, v, log_decay, *states)
-    dt = _code(q)
-    _same_dtype(q, k, v)
-    if q.dim() != dims:
-        raise ValueError("q must be [B, L, H, D]" if dims == 4 else "q must be [B, H, D]")
-    H, D = q.shape[-2:]
-    if not 1 <= D <= 128 or H < 1:
-        raise ValueError(f"heads of 1 to 128 elements are supported, got H={H}, D={D}")
-    for t, what in ((q, "q"), (k, "k"), (v, "v")):
-        _heads(t, q.shape, what)
-    if log_decay.shape != (H,):
-        raise ValueError(f"log_decay must be [{H}], got {list(log_decay.shape)}")
-    for s in states:
-        if s is not None:
-            _f32_state(s, (q.shape[0], H, D, D), "a state")
-    return dt, log_decay.float().contiguous()
-
-
 def decay_attention(q, k, v, log_decay, scale=1.0, state=None, out=None, return_states=False):
     """Linear attention with a decay for each head over whole sequences (hdc_decay_attn_fwd): the
     Block's slot memory (hdcmamba/model.py:236-272) without its feature map and chunk rounding,
@@ -844,19 +816,7 @@ def decay_attention(q, k, v, log_decay, scale=1.0, state=None, out=None, return_
     optional [B, L, H, D] view.  Returns (o, the state after the last token) and, if
     ``return_states``, the states that ``decay_attention_bwd`` needs.  For autograd use
     ``recurrent.decay_attention``."""
-    dt, g = _decay_args(q, k, v, log_decay, 4, state)
-    B, L, H, D = q.shape
-    if out is None:
-        out = torch.empty(B, L, H, D, device=q.device, dtype=q.dtype)
-    else:
-        _cuda(out)
-        _same_dtype(q, out)
-        _heads(out, q.shape, "out")
-    after = torch.empty(B, H, D, D, device=q.device, dtype=torch.float32)
-    states = torch.empty(B, H, _size("hdc_decay_attn_segments", B, L, H), D, D, device=q.device, dtype=torch.float32)
-    _lib.call("hdc_decay_attn_fwd", dt, _a(q), *q.stride()[:3], _a(k), *k.stride()[:3], _a(v), *v.stride()[:3], _a(g),
-              _a(state), float(scale), _a(out), *out.stride()[:3], _a(after), _a(states), B, L, H, D, _raw_stream(q))
-    return (out, after, states) if return_states else (out, after)
+    return _lib.host().decay_attention(q, k, v, log_decay, scale, state, out, return_states)
 
 
 def decay_attention_bwd(do, q, k, v, log_decay, states, scale=1.0, dstate=None, need_dstate=False):
@@ -864,84 +824,23 @@ def decay_attention_bwd(do, q, k, v, log_decay, states, scale=1.0, dstate=None, 
     the same inputs; do: [B, L, H, D] view in q.dtype; dstate: optional gradient of the returned state,
     contiguous fp32 [B, H, D, D].  Returns (dq, dk, dv, the gradient of the state before the first token
     or None)."""
-    _cuda(do, states)
-    dt, g = _decay_args(q, k, v, log_decay, 4, dstate)
-    B, L, H, D = q.shape
-    _same_dtype(q, do)
-    _heads(do, q.shape, "do")
-    _f32_state(states, (B, H, _size("hdc_decay_attn_segments", B, L, H), D, D), "states")
-    return _decay_attention_bwd(dt, do, q, k, v, g, states, scale, dstate, need_dstate)
-
-
-def _decay_attention_bwd(dt, do, q, k, v, g, states, scale, dstate, need_dstate):
-    """``decay_attention_bwd`` on arguments that have been checked."""
-    B, L, H, D = q.shape
-    dev = q.device
-    if D > 1 and do.stride(3) != 1:
-        do = do.contiguous()
-    dq, dk, dv = (torch.empty(B, L, H, D, device=dev, dtype=q.dtype) for _ in range(3))
-    before = torch.empty(B, H, D, D, device=dev, dtype=torch.float32) if need_dstate else None
-    nbytes = _size("hdc_decay_attn_bwd_workspace_bytes", B, L, H, D)
-    ws = _workspace(nbytes, dev)
-    rows = (L * H * D, H * D, D)
-    _lib.call("hdc_decay_attn_bwd", dt, _a(q), *q.stride()[:3], _a(k), *k.stride()[:3], _a(v), *v.stride()[:3], _a(do),
-              *do.stride()[:3], _a(g), _a(states), _a(dstate), float(scale), _a(dq), *rows, _a(dk), *rows, _a(dv),
-              *rows, _a(before), _a(ws), nbytes, B, L, H, D, _raw_stream(q))
-    return dq, dk, dv, before
+    return _lib.host().decay_attention_bwd(do, q, k, v, log_decay, states, scale, dstate, need_dstate)
 
 
 def decay_attention_step(q, k, v, log_decay, state, scale=1.0, out=None, state_out=None):
     """One token per sequence of ``decay_attention`` (hdc_decay_attn_step): q, k, v [B, H, D] views (unit
     stride within a head), state contiguous fp32 [B, H, D, D], updated in place unless ``state_out`` is
     given.  Returns (o [B, H, D], the new state)."""
-    dt, g = _decay_args(q, k, v, log_decay, 3, state, state_out)
-    B, H, D = q.shape
-    if state_out is None:
-        state_out = state
-    if out is None:
-        out = torch.empty(B, H, D, device=q.device, dtype=q.dtype)
-    else:
-        _cuda(out)
-        _same_dtype(q, out)
-        _heads(out, q.shape, "out")
-    _lib.call("hdc_decay_attn_step", dt, _a(q), *q.stride()[:2], _a(k), *k.stride()[:2], _a(v), *v.stride()[:2], _a(g),
-              _a(state), float(scale), _a(out), *out.stride()[:2], _a(state_out), B, H, D, _raw_stream(q))
-    return out, state_out
+    return _lib.host().decay_attention_step(q, k, v, log_decay, state, scale, out, state_out)
 
 
 # ------------------------------------------------------------------ token embedding
-_ID_BYTES = {torch.int64: 8, torch.int32: 4}
-
-
-def _embedding_args(ids, table, what):
-    if ids.dtype not in _ID_BYTES:
-        raise TypeError(f"hdcmamba_b200: ids must be int64 or int32, got {ids.dtype}")
-    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
-        raise ValueError(f"{what} must be [rows, D], got {list(table.shape)}")
-    if table.shape[1] > 1 and table.stride(1) != 1:
-        raise ValueError(f"{what} needs a unit column stride")
-    return ids.reshape(-1) if ids.is_contiguous() else ids.contiguous().view(-1)
-
-
 def embedding(ids, weight, scale=1.0, out=None):
     """Rows of ``weight`` [rows, D] (unit column stride) by ``ids`` (int64 or int32, any shape), times
     ``scale`` (hdc_embedding_fwd; the LM wrappers' nn.Embedding, train.py:116-137): ids.shape + [D] in
     weight's type.  out: optional contiguous tensor of that shape.  An id outside the table gives a row
     of NaN and an error in ``check_device``.  For autograd use ``training.embedding``."""
-    _cuda(ids, weight, out)
-    dt = _code(weight)
-    flat = _embedding_args(ids, weight, "weight")
-    rows, D = weight.shape
-    shape = (*ids.shape, D)
-    if out is None:
-        out = torch.empty(shape, device=weight.device, dtype=weight.dtype)
-    else:
-        _same_dtype(weight, out)
-        if out.shape != shape or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {list(shape)} tensor")
-    _lib.call("hdc_embedding_fwd", dt, _a(flat), _ID_BYTES[ids.dtype], _a(weight), weight.stride(0), _a(out), D,
-              float(scale), flat.numel(), rows, D, _raw_stream(weight))
-    return out
+    return _lib.host().embedding(ids, weight, scale, out)
 
 
 def embedding_bwd(dy, ids, rows, scale=1.0, padding_idx=None, out=None):
@@ -949,61 +848,14 @@ def embedding_bwd(dy, ids, rows, scale=1.0, padding_idx=None, out=None):
     Tokens are sorted by id and each row's sum is taken in their order in fp32, so the result does not
     depend on timing; rows that no token has are zeros.  padding_idx: optional id that takes no part.
     out: optional [rows, D] view (unit column stride).  Returns [rows, D] in dy's type."""
-    _cuda(dy, ids, out)
-    dt = _code(dy)
-    if dy.dim() < 1 or dy.shape[:-1] != ids.shape or dy.shape[-1] < 1:
-        raise ValueError(f"dy {list(dy.shape)} must be ids' shape {list(ids.shape)} and columns")
-    D = dy.shape[-1]
-    if out is None:
-        out = torch.empty(rows, D, device=dy.device, dtype=dy.dtype)
-    else:
-        _same_dtype(dy, out)
-        if out.shape != (rows, D):
-            raise ValueError(f"out must be [{rows}, {D}]")
-    flat = _embedding_args(ids, out, "out")
-    d2 = dy.reshape(-1, D)
-    if D > 1 and d2.stride(1) != 1:
-        d2 = d2.contiguous()
-    nbytes = _size("hdc_embedding_bwd_workspace_bytes", flat.numel(), rows, D)
-    ws = _workspace(nbytes, dy.device)
-    _lib.call("hdc_embedding_bwd", dt, _a(flat), _ID_BYTES[ids.dtype], _a(d2), d2.stride(0), _a(out), out.stride(0),
-              float(scale), -1 if padding_idx is None else int(padding_idx), _a(ws), nbytes, flat.numel(), rows, D,
-              _raw_stream(dy))
-    return out
+    return _lib.host().embedding_bwd(dy, ids, rows, scale, padding_idx, out)
 
 
 # ------------------------------------------------------------------ gradient norm and clipping
 def clip_grads(grads, max_norm, out=None):
-    """The norm over all elements of ``grads`` (contiguous fp32 and bf16 tensors of one device), and
-    ``out[i] = grads[i] * min(1, max_norm / (norm + 1e-6))``, in place unless ``out`` (a list of
+    """The norm over all elements of ``grads`` (a list of contiguous fp32 and bf16 tensors of one device),
+    and ``out[i] = grads[i] * min(1, max_norm / (norm + 1e-6))``, in place unless ``out`` (a list of
     contiguous tensors of the same types and sizes) is given (hdc_clip_grads).  max_norm None: the norm
     alone.  Returns the norm, fp32 on the device; the host does not wait for it.  ``training.clip_grad_norm_``
     takes parameters."""
-    grads = list(grads)
-    n = len(grads)
-    outs = grads if out is None else list(out)
-    if len(outs) != n:
-        raise ValueError(f"{len(outs)} outputs for {n} gradients")
-    if n == 0:
-        raise ValueError("clip_grads needs at least one gradient")
-    dev = grads[0].device
-    _cuda(*grads)
-    codes, sizes = [], []
-    for g, o in zip(grads, outs):
-        if g.device != dev or o.device != dev:
-            raise ValueError(f"gradients and outputs must be on one device ({dev}, got {g.device}, {o.device})")
-        if not g.is_contiguous() or not o.is_contiguous():
-            raise ValueError("clip_grads needs contiguous tensors")
-        if o is not g and (o.dtype != g.dtype or o.numel() != g.numel()):
-            raise ValueError(f"an output {list(o.shape)} {o.dtype} does not match its gradient {list(g.shape)} {g.dtype}")
-        codes.append(_code(g))
-        sizes.append(g.numel())
-    norm = torch.empty((), device=dev, dtype=torch.float32)
-    ws = _workspace(_size("hdc_clip_grads_workspace_bytes", n), dev)
-    ptrs = ctypes.c_void_p * n
-    at = ptrs(*[g.data_ptr() for g in grads])
-    to = at if out is None else ptrs(*[o.data_ptr() for o in outs])
-    _lib.call("hdc_clip_grads", n, (ctypes.c_int * n)(*codes), at, to if max_norm is not None else None,
-              (ctypes.c_int64 * n)(*sizes), float(max_norm) if max_norm is not None else 0.0, _a(norm), _a(ws),
-              ws.numel(), _current_raw_stream(dev.index))
-    return norm
+    return _lib.host().clip_grads(grads, max_norm, out)

@@ -23,11 +23,11 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import ops
+from . import _lib, ops
 from .model import _require_cuda
 
 __all__ = ["norm_conv1d", "gated_scan", "group_norm_act", "decay_attention", "NormConv1dFunction", "GatedScanFunction",
-           "GroupNormActFunction", "DecayAttentionFunction", "GatedRecurrentBlock", "RecurrentState"]
+           "GroupNormActFunction", "GatedRecurrentBlock", "RecurrentState"]
 
 
 def _first_order_only():
@@ -137,33 +137,6 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none"):
     return ops.group_norm_act(x, num_groups, weight, bias, eps=eps, act=act)
 
 
-class DecayAttentionFunction(torch.autograd.Function):
-    """(q, k, v, log_decay, state, scale) -> (o, state after); gradients for q, k, v and state
-    (hdc_decay_attn_fwd / hdc_decay_attn_bwd)."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, log_decay, state, scale):
-        ctx.scale, ctx.state_dtype = scale, state.dtype if state is not None else None
-        state = state.float().contiguous() if state is not None else None
-        o, after, states = ops.decay_attention(q, k, v, log_decay, scale, state, return_states=True)
-        ctx.save_for_backward(q, k, v, log_decay, states)
-        ctx.set_materialize_grads(False)
-        return o, after
-
-    @staticmethod
-    def backward(ctx, do, dafter):
-        _first_order_only()
-        q, k, v, log_decay, states = ctx.saved_tensors
-        if do is None:
-            do = torch.zeros(q.shape, device=q.device, dtype=q.dtype)
-        if dafter is not None:
-            dafter = dafter.contiguous()
-        # the forward has checked the arguments
-        dq, dk, dv, dstate = ops._decay_attention_bwd(ops._code(q), do, q, k, v, log_decay.float().contiguous(), states,
-                                                      ctx.scale, dafter, ctx.needs_input_grad[4])
-        return dq, dk, dv, None, dstate.to(ctx.state_dtype) if dstate is not None else None, None
-
-
 def decay_attention(q, k, v, log_decay, scale=1.0, state=None):
     """Differentiable ``ops.decay_attention``: (o, state after the last token).  The states carry
     gradients, so a sequence can be trained window by window; the decays are constants."""
@@ -172,7 +145,7 @@ def decay_attention(q, k, v, log_decay, scale=1.0, state=None):
         raise ValueError("decay_attention has no gradient for log_decay: pass a constant (log_decay.detach())")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                     (state is not None and state.requires_grad)):
-        return DecayAttentionFunction.apply(q, k, v, log_decay, state, scale)
+        return _lib.host().decay_attention_train(q, k, v, log_decay, state, scale)  # a C++ autograd node
     return ops.decay_attention(q, k, v, log_decay, scale, state)
 
 

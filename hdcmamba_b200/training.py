@@ -10,28 +10,10 @@ There is no CPU path: CPU inputs raise.
 """
 import torch
 
-from . import ops
+from . import _lib, ops
 from .model import _require_cuda
-from .recurrent import _first_order_only
 
-__all__ = ["embedding", "clip_grad_norm_", "EmbeddingFunction"]
-
-
-class EmbeddingFunction(torch.autograd.Function):
-    """(ids, weight, scale, padding_idx) -> rows of weight; gradient for weight
-    (hdc_embedding_fwd / hdc_embedding_bwd)."""
-
-    @staticmethod
-    def forward(ctx, ids, weight, scale, padding_idx):
-        ctx.save_for_backward(ids)
-        ctx.rows, ctx.scale, ctx.padding_idx = weight.shape[0], scale, padding_idx
-        return ops.embedding(ids, weight, scale)
-
-    @staticmethod
-    def backward(ctx, dy):
-        _first_order_only()
-        (ids,) = ctx.saved_tensors
-        return None, ops.embedding_bwd(dy, ids, ctx.rows, ctx.scale, ctx.padding_idx), None, None
+__all__ = ["embedding", "clip_grad_norm_"]
 
 
 def embedding(ids, weight, scale=1.0, padding_idx=None):
@@ -41,7 +23,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"padding_idx {padding_idx} is outside the table of {weight.shape[0]} rows")
     if torch.is_grad_enabled() and weight.requires_grad:
-        return EmbeddingFunction.apply(ids, weight, scale, padding_idx)
+        return _lib.host().embedding_train(ids, weight, scale, padding_idx)  # a C++ autograd node
     return ops.embedding(ids, weight, scale)
 
 

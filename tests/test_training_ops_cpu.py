@@ -28,20 +28,10 @@ def test_cpu_tensors_raise():
         ops.clip_grads([], 1.0)
 
 
-@pytest.fixture
-def on_gpu(monkeypatch):
-    """The checks behind the one for the device, with CPU tensors; a launch would fail the test."""
-    monkeypatch.setattr(ops, "_cuda", lambda *t: None)
-    monkeypatch.setattr(recurrent, "_require_cuda", lambda *t: None)
-    monkeypatch.setattr(training, "_require_cuda", lambda *t: None)
-
-    def no_launch(*a):
-        raise AssertionError("a launch")
-
-    monkeypatch.setattr(_lib, "call", no_launch)
+# CPU tensors: sizes and types are looked at before the device, so a call that they allow ends there (RuntimeError)
 
 
-def test_attention_refusals(on_gpu):
+def test_attention_refusals():
     q, g, s = torch.zeros(2, 5, 3, 8), torch.zeros(3), torch.zeros(2, 3, 8, 8)
     bad = [
         dict(q=q.half(), k=q.half(), v=q.half()), dict(k=q.bfloat16()), dict(k=torch.zeros(2, 4, 3, 8)),
@@ -55,8 +45,6 @@ def test_attention_refusals(on_gpu):
     for kw in bad:
         with pytest.raises((ValueError, TypeError)):
             ops.decay_attention(**(dict(q=q, k=q, v=q, log_decay=g) | kw))
-    with pytest.raises(ValueError, match="log_decay"):
-        recurrent.decay_attention(q, q, q, g.clone().requires_grad_())
     n = ops._size("hdc_decay_attn_segments", 2, 5, 3)
     st = torch.zeros(2, 3, n, 8, 8)
     for kw in (dict(do=q.bfloat16()), dict(do=q[:, :4]), dict(states=st[:, :2]), dict(states=st.double()),
@@ -69,7 +57,7 @@ def test_attention_refusals(on_gpu):
             ops.decay_attention_step(**(dict(q=r, k=r, v=r, log_decay=g, state=s) | kw))
 
 
-def test_embedding_refusals(on_gpu):
+def test_embedding_refusals():
     ids, w = torch.zeros(4, dtype=torch.int64), torch.zeros(10, 8)
     for kw in (dict(ids=ids.float()), dict(ids=ids.short()), dict(weight=w.half()), dict(weight=w.t()), dict(weight=w[0]),
                dict(weight=w[:, :0]), dict(out=torch.zeros(4, 9)), dict(out=torch.zeros(4, 8).bfloat16()),
@@ -81,12 +69,9 @@ def test_embedding_refusals(on_gpu):
                dict(out=torch.zeros(10, 8).bfloat16())):
         with pytest.raises((ValueError, TypeError)):
             ops.embedding_bwd(**(dict(dy=dy, ids=ids, rows=10) | kw))
-    for bad in (-1, 10):
-        with pytest.raises(ValueError, match="padding_idx"):
-            training.embedding(ids, w, padding_idx=bad)
 
 
-def test_clip_refusals(on_gpu):
+def test_clip_refusals():
     x = torch.zeros(4, 5)
     for grads, out in (([x.t()], None), ([x.half()], None), ([x], [x.bfloat16()]), ([x], [torch.zeros(21)]), ([x], []),
                        ([x], [torch.zeros(5, 4).t()]), ([x, x.long()], None)):
@@ -106,6 +91,26 @@ def attn_fwd(**kw):
     v = dict(dtype=1, q=A, k=A, v=A, st=(64, 32, 8), g=A, s0=None, o=A, ost=(64, 32, 8), s1=None, states=A, B=2, L=2, H=4, D=8) | kw
     return rc("hdc_decay_attn_fwd", v["dtype"], v["q"], *v["st"], v["k"], *v["st"], v["v"], *v["st"], v["g"], v["s0"], 1.0, v["o"],
               *v["ost"], v["s1"], v["states"], v["B"], v["L"], v["H"], v["D"], None)[0]
+
+
+def test_checks_beside_the_operators(monkeypatch):
+    monkeypatch.setattr(recurrent, "_require_cuda", lambda *t: None)
+    monkeypatch.setattr(training, "_require_cuda", lambda *t: None)
+    q, g = torch.zeros(2, 5, 3, 8), torch.zeros(3)
+    with pytest.raises(ValueError, match="log_decay"):
+        recurrent.decay_attention(q, q, q, g.requires_grad_())
+    for bad in (-1, 10):
+        with pytest.raises(ValueError, match="padding_idx"):
+            training.embedding(torch.zeros(4, dtype=torch.int64), torch.zeros(10, 8), padding_idx=bad)
+    for bad in (None, 3, "q"):
+        with pytest.raises(TypeError):
+            ops.decay_attention(bad, q, q, g)
+        with pytest.raises(TypeError):
+            ops.clip_grads([q, bad], 1.0)
+    with pytest.raises(TypeError):
+        ops.decay_attention(q, q, q, g, scale="1")
+    with pytest.raises(TypeError):
+        ops.clip_grads(5, 1.0)
 
 
 def test_c_checks_attention():
