@@ -9,6 +9,8 @@
 // end), of which every warp takes an equal part, so that neither a frequent id nor a wide table leaves
 // warps idle: a token costs one row read, a row's end one row written (zeros where no token has it).
 // A row cut by a part's border leaves fp32 partial sums that a last kernel adds in the parts' order.
+#include <atomic>
+
 #include "tc.cuh"
 #include "vec.cuh"
 
@@ -24,57 +26,88 @@ __device__ __forceinline__ int64_t id_at(const void* ids, int64_t n) {
 // ---------------------------------------------------------------- lookup
 constexpr int kLoads = 4;
 
-// nv: vectors of V elements of a row.  Block i takes vectors [i * 256 * kLoads, ...) of all rows' vectors.
-template <typename T, typename I, int V>
-__global__ void __launch_bounds__(256) embedding_kernel(const void* ids, const T* table, int64_t table_st, T* y,
-                                                        int64_t y_st, int64_t N, int64_t rows, int nv, float scale) {
-  const int64_t first = (int64_t)blockIdx.x * 256 * kLoads;
-  const int64_t n0 = first / nv;
-  const unsigned off = (unsigned)(first - n0 * nv) + threadIdx.x;
-  uint4 w[kLoads];
-  T e[kLoads];
-  int64_t id[kLoads];
-#pragma unroll
-  for (int u = 0; u < kLoads; ++u) {
-    const unsigned k = off + u * 256;
-    const int64_t n = n0 + k / (unsigned)nv;
-    id[u] = n < N ? id_at<I>(ids, n) : -1;
-    if (n < N && (id[u] < 0 || id[u] >= rows)) atomicCAS(&g_dev_error, 0, kBadId);
+// One 16-byte vector (V > 1) or element of an output row from its table row; a bad id gives NaN.
+template <typename T, int V> struct Cell {
+  uint4 w;
+  T e;
+  __device__ __forceinline__ void load(const T* src, bool ok) {
+    if constexpr (V == 1) e = ok ? *src : from_f<T>(0.f);
+    else w = ldg16_pred(src, ok);
   }
-#pragma unroll
-  for (int u = 0; u < kLoads; ++u) {
-    const unsigned c = (off + u * 256) % (unsigned)nv;
-    const bool ok = id[u] >= 0 && id[u] < rows;
-    const T* src = table + id[u] * table_st + (int64_t)c * V;
-    if constexpr (V == 1) e[u] = ok ? *src : from_f<T>(0.f);
-    else w[u] = ldg16_pred(ok ? src : table, ok);
-  }
-#pragma unroll
-  for (int u = 0; u < kLoads; ++u) {
-    const unsigned k = off + u * 256, c = k % (unsigned)nv;
-    const int64_t n = n0 + k / (unsigned)nv;
-    if (n >= N) continue;
-    const float by = id[u] >= 0 && id[u] < rows ? scale : __int_as_float(0x7fffffff);
-    T* dst = y + n * y_st + (int64_t)c * V;
+  __device__ __forceinline__ void store(T* dst, float by) const {
     if constexpr (V == 1) {
-      *dst = from_f<T>(by * to_f(e[u]));
+      *dst = from_f<T>(by * to_f(e));
     } else {
       float f[V];
-      unpack16<T>(w[u], f);
+      unpack16<T>(w, f);
 #pragma unroll
       for (int i = 0; i < V; ++i) f[i] *= by;
       stg16(dst, pack16<T>(f));
     }
   }
+};
+
+// A group of `lanes` lanes (a power of two) copies a row of nv vectors of V elements.  Rows of at most `lanes`
+// vectors: a group takes kLoads rows at once; longer ones: kLoads vectors of one row at once.
+template <typename T, typename I, int V, bool SHORT>
+__global__ void __launch_bounds__(256) embedding_kernel(const void* ids, const T* table, int64_t table_st, T* y,
+                                                        int64_t y_st, int64_t N, int64_t rows, int nv, int lanes,
+                                                        float scale) {
+  const int per_block = 256 / lanes, group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
+  Cell<T, V> cell[kLoads];
+  if constexpr (SHORT) {
+    const int64_t n0 = (int64_t)blockIdx.x * per_block * kLoads + group;
+    int64_t id[kLoads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t n = n0 + u * per_block;
+      id[u] = n < N ? id_at<I>(ids, n) : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const bool ok = id[u] >= 0 && id[u] < rows;
+      if (!ok) atomicCAS(&g_dev_error, 0, kBadId);
+      cell[u].load(table + (ok ? id[u] * table_st : 0) + lane * V, ok && lane < nv && n0 + u * per_block < N);
+      id[u] = ok;
+    }
+    if (lane >= nv) return;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t n = n0 + u * per_block;
+      if (n < N) cell[u].store(y + n * y_st + lane * V, id[u] ? scale : __int_as_float(0x7fffffff));
+    }
+  } else {
+    const int64_t n = (int64_t)blockIdx.x * per_block + group;
+    if (n >= N) return;
+    const int64_t id = id_at<I>(ids, n);
+    const bool ok = id >= 0 && id < rows;
+    if (!ok) atomicCAS(&g_dev_error, 0, kBadId);
+    const T* src = table + (ok ? id * table_st : 0);
+    T* dst = y + n * y_st;
+    const float by = ok ? scale : __int_as_float(0x7fffffff);
+    for (int c0 = lane; c0 < nv; c0 += lanes * kLoads) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const int c = c0 + u * lanes;
+        cell[u].load(src + (int64_t)(c < nv ? c : 0) * V, ok && c < nv);
+      }
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const int c = c0 + u * lanes;
+        if (c < nv) cell[u].store(dst + (int64_t)c * V, by);
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------- sort by id
-constexpr int kSortThreads = 256, kSortWarps = kSortThreads / 32, kMaxBins = 512;
-constexpr int kTileLeast = 1024, kMostTiles = 128;
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMaxBins = 512;
+constexpr int kMostTiles = 128;
+constexpr int kOneTile = 4096;  // tokens that one CTA sorts in shared memory
 
 struct SortPlan {
   int passes, bits;      // digit passes and bits of a digit
-  int tiles;             // tiles of `tile` tokens, a multiple of 256
+  int tiles;             // tiles of `tile` tokens, a multiple of kSortThreads
   int64_t tile;
 };
 
@@ -107,33 +140,38 @@ __global__ void __launch_bounds__(kSortThreads) embedding_count_kernel(const voi
   }
 }
 
-// One digit's pass: (key, token) pairs move to their place by (digit, tile, place in the tile).  A tile's
-// place for each digit follows from all tiles' counts, which its CTA adds up itself.
-template <typename I>
-__global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const void* ids, const uint2* from, uint2* to,
-                                                                      int64_t N, int64_t rows, int64_t skip,
-                                                                      SortPlan p, int pass, unsigned* counts) {
-  __shared__ unsigned base[kMaxBins];                 // where the next of each digit goes
-  __shared__ unsigned part[kSortWarps][kMaxBins];     // a round's counts, warp by warp
-  __shared__ unsigned sums[kSortWarps];
-  const int bins = 1 << p.bits, shift = pass * p.bits;
+// Ranks of a round's tokens (one a thread) among those of the same digit, in the threads' order: a lane's place in
+// its warp, the warps before it (part: counts, then running sums), and base[digit], which then moves on.
+// d = bins: no token.  Every thread of the CTA calls it.
+__device__ __forceinline__ unsigned round_place(int d, int bins, unsigned* base, unsigned short (*part)[kMaxBins]) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const unsigned* table = counts + (int64_t)pass * p.tiles * bins;
-  unsigned* next = pass + 1 < p.passes ? counts + (int64_t)(pass + 1) * p.tiles * bins : nullptr;
-  // digits 2 * thread and 2 * thread + 1: the tokens of all tiles, and those of the tiles before this one
-  unsigned all[2] = {0, 0}, before[2] = {0, 0};
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int d = threadIdx.x * 2 + e;
-    if (d >= bins) continue;
+  for (int i = lane; i < bins / 2; i += 32) reinterpret_cast<unsigned*>(part[warp])[i] = 0;
+  __syncwarp();
+  const unsigned same = __match_any_sync(0xffffffffu, d);
+  const int rank = __popc(same & ((1u << lane) - 1));
+  if (d < bins && rank == 0) part[warp][d] = (unsigned short)__popc(same);
+  __syncthreads();
+  if ((int)threadIdx.x < bins) {
+    unsigned sum = base[threadIdx.x];
 #pragma unroll 8
-    for (int t = 0; t < p.tiles; ++t) {
-      const unsigned c = table[(int64_t)t * bins + d];
-      all[e] += c;
-      before[e] += t < (int)blockIdx.x ? c : 0;
+    for (int w = 0; w < kSortWarps; ++w) {
+      const unsigned c = part[w][threadIdx.x];
+      part[w][threadIdx.x] = (unsigned short)(sum - base[threadIdx.x]);
+      sum += c;
     }
+    base[kMaxBins + threadIdx.x] = sum;  // the next round's
   }
-  unsigned x = all[0] + all[1];  // running sum over the digits
+  __syncthreads();
+  const unsigned at = d < bins ? base[d] + part[warp][d] + rank : 0;
+  __syncthreads();
+  if ((int)threadIdx.x < bins) base[threadIdx.x] = base[kMaxBins + threadIdx.x];
+  return at;  // the caller synchronises before the next round
+}
+
+// base[d] = the tokens of lower digits, from counts c of a thread's digit (thread < bins)
+__device__ __forceinline__ unsigned lower_digits(unsigned c, unsigned* sums) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  unsigned x = c;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
@@ -141,38 +179,93 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const void
   }
   if (lane == 31) sums[warp] = x;
   __syncthreads();
-  unsigned lower = x - all[0] - all[1];
+  unsigned lower = x - c;
   for (int w = 0; w < warp; ++w) lower += sums[w];
-  if (threadIdx.x * 2 < bins) {
-    base[threadIdx.x * 2] = lower + before[0];
-    base[threadIdx.x * 2 + 1] = lower + all[0] + before[1];
+  return lower;
+}
+
+// One digit's pass: (key, token) pairs move to their place by (digit, tile, place in the tile).  A tile's
+// place for each digit follows from all tiles' counts, which its CTA adds up itself.
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const void* ids, const uint2* from, uint2* to,
+                                                                      int64_t N, int64_t rows, int64_t skip,
+                                                                      SortPlan p, int pass, unsigned* counts) {
+  __shared__ unsigned base[2 * kMaxBins], sums[kSortWarps];
+  __shared__ __align__(4) unsigned short part[kSortWarps][kMaxBins];
+  const int bins = 1 << p.bits, shift = pass * p.bits;
+  const unsigned* table = counts + (int64_t)pass * p.tiles * bins;
+  unsigned* next = pass + 1 < p.passes ? counts + (int64_t)(pass + 1) * p.tiles * bins : nullptr;
+  wait_for_previous();
+  unsigned all = 0, before = 0;
+  if ((int)threadIdx.x < bins) {
+#pragma unroll 16
+    for (int t = 0; t < p.tiles; ++t) {
+      const unsigned c = table[(int64_t)t * bins + threadIdx.x];
+      all += c;
+      before += t < (int)blockIdx.x ? c : 0;
+    }
   }
+  const unsigned lower = lower_digits(all, sums);
+  if ((int)threadIdx.x < bins) base[threadIdx.x] = lower + before;
   const int64_t begin = blockIdx.x * p.tile, end = min(N, begin + p.tile);
   for (int64_t n0 = begin; n0 < end; n0 += kSortThreads) {
-    for (int i = threadIdx.x; i < bins * kSortWarps; i += kSortThreads) part[i / bins][i % bins] = 0;
     const int64_t n = n0 + threadIdx.x;
     uint2 e = make_uint2(0, 0);
     if (n < end) e = pass == 0 ? make_uint2(sort_key<I>(ids, n, rows, skip), (unsigned)n) : from[n];
-    const int d = n < end ? (int)((e.x >> shift) & (unsigned)(bins - 1)) : bins;  // bins: no token
-    const unsigned same = __match_any_sync(0xffffffffu, d);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    __syncthreads();
-    if (d < bins && rank == 0) part[warp][d] = __popc(same);
-    __syncthreads();
+    const int d = n < end ? (int)((e.x >> shift) & (unsigned)(bins - 1)) : bins;
+    const unsigned at = round_place(d, bins, base, part);
     if (d < bins) {
-      unsigned at = base[d] + rank;
-      for (int w = 0; w < warp; ++w) at += part[w][d];
       to[at] = e;
       if (next) atomicAdd(&next[(int64_t)(at / p.tile) * bins + ((e.x >> (shift + p.bits)) & (unsigned)(bins - 1))], 1u);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < bins; i += kSortThreads) {
-      unsigned c = 0;
+  }
+}
+
+// All passes of up to kOneTile tokens by one CTA, in shared memory.
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) embedding_sort_one_kernel(const void* ids, uint2* to, int N,
+                                                                          int64_t rows, int64_t skip, SortPlan p) {
+  constexpr int kRounds = kOneTile / kSortThreads;
+  extern __shared__ uint2 sorted[];
+  __shared__ unsigned base[2 * kMaxBins], sums[kSortWarps], count[kMaxBins];
+  __shared__ __align__(4) unsigned short part[kSortWarps][kMaxBins];
+  const int bins = 1 << p.bits;
+  uint2 e[kRounds];
 #pragma unroll
-      for (int w = 0; w < kSortWarps; ++w) c += part[w][i];
-      base[i] += c;
+  for (int i = 0; i < kRounds; ++i) {
+    const int n = i * kSortThreads + threadIdx.x;
+    if (n < N) e[i] = make_uint2(sort_key<I>(ids, n, rows, skip), (unsigned)n);
+  }
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const int shift = pass * p.bits;
+    for (int i = threadIdx.x; i < bins; i += kSortThreads) count[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i)
+      if (i * kSortThreads + (int)threadIdx.x < N) atomicAdd(&count[(e[i].x >> shift) & (unsigned)(bins - 1)], 1u);
+    __syncthreads();
+    const unsigned lower = lower_digits((int)threadIdx.x < bins ? count[threadIdx.x] : 0, sums);
+    if ((int)threadIdx.x < bins) base[threadIdx.x] = lower;
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      if (i * kSortThreads >= N) break;
+      const int d = i * kSortThreads + (int)threadIdx.x < N ? (int)((e[i].x >> shift) & (unsigned)(bins - 1)) : bins;
+      const unsigned at = round_place(d, bins, base, part);
+      if (d < bins) sorted[at] = e[i];
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int n = i * kSortThreads + threadIdx.x;
+      if (n < N) e[i] = sorted[n];
     }
     __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int n = i * kSortThreads + threadIdx.x;
+    if (n < N) to[n] = e[i];
   }
 }
 
@@ -182,33 +275,57 @@ struct SumPlan {
   int64_t items, parts;
 };
 
-// tokens among the first d items: the most t with key[t - 1] <= d - t
+// Tokens among the first d items: the most t with key[t - 1] <= d - t.  A warp looks at 32 places at a time.
 __device__ __forceinline__ int64_t merge_split(const uint2* sorted, int64_t N, int64_t rows, int64_t d) {
+  const int lane = threadIdx.x % 32;
   int64_t lo = d > rows ? d - rows : 0, hi = d < N ? d : N;
   while (lo < hi) {
-    const int64_t t = (lo + hi + 1) / 2;
-    if ((int64_t)sorted[t - 1].x <= d - t) lo = t;
-    else hi = t - 1;
+    const int64_t step = (hi - lo + 31) / 32, t = min(lo + (lane + 1) * step, hi);
+    const unsigned yes = __ballot_sync(0xffffffffu, (int64_t)sorted[t - 1].x <= d - t);
+    const int k = __popc(yes);  // the first k places
+    if (k == 32) {
+      lo = hi;
+    } else {
+      hi = min(lo + (k + 1) * step, hi) - 1;
+      lo = lo + k * step;
+    }
   }
   return lo;
 }
 
-// V consecutive elements of a lane (V = 1: 8 elements 32 apart)
+// V consecutive elements of a lane (VEC false: 8 elements 32 apart), as they are fetched and as sums
 template <typename T, bool VEC> struct Cols {
   static constexpr int N = VEC ? Vec<T>::N : 8;
   static constexpr int kWarp = 32 * N;  // columns of a warp
+  struct Raw { uint4 w[VEC ? 1 : sizeof(T) / 2]; };
 };
 template <typename T, bool VEC>
-__device__ __forceinline__ void col_load(const T* row, int c0, int lane, int D, float* f) {
+__device__ __forceinline__ typename Cols<T, VEC>::Raw col_load(const T* row, int c0, int lane, int D, bool in) {
+  typename Cols<T, VEC>::Raw f;
   if constexpr (VEC) {
     const int c = c0 + lane * Vec<T>::N;
-    unpack16<T>(ldg16_pred(row + (c < D ? c : 0), c < D), f);
+    f.w[0] = ldg16_pred(row + (c < D ? c : 0), in && c < D);
   } else {
+    T* e = reinterpret_cast<T*>(f.w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int c = c0 + i * 32 + lane;
-      f[i] = c < D ? to_f(row[c]) : 0.f;
+      e[i] = in && c < D ? row[c] : from_f<T>(0.f);
     }
+  }
+  return f;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void col_add(float* acc, const typename Cols<T, VEC>::Raw& f) {
+  if constexpr (VEC) {
+    float x[Vec<T>::N];
+    unpack16<T>(f.w[0], x);
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) acc[i] += x[i];
+  } else {
+    const T* e = reinterpret_cast<const T*>(f.w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] += to_f(e[i]);
   }
 }
 template <typename T, bool VEC>
@@ -230,8 +347,10 @@ __device__ __forceinline__ float* part_at(float* p, int64_t u, int lane) {
   return p + ((u * gridDim.y + blockIdx.y) * 32 + lane) * N;
 }
 
-constexpr int kSumWarps = 4, kRowsAhead = 4;
+constexpr int kSumWarps = 4, kRowsAhead = 8;
 
+// A warp's part: its tokens' rows are fetched kRowsAhead at a time, whatever rows of the table they belong to; a
+// token of a later row first ends the rows before it.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kSumWarps * 32) embedding_sum_kernel(const uint2* sorted, const T* dy, int64_t dy_st,
                                                                        T* dtable, int64_t d_st, int64_t N,
@@ -242,40 +361,18 @@ __global__ void __launch_bounds__(kSumWarps * 32) embedding_sum_kernel(const uin
   const int lane = threadIdx.x % 32, c0 = blockIdx.y * C::kWarp;
   const int64_t u = (int64_t)blockIdx.x * kSumWarps + threadIdx.x / 32;
   if (u >= p.parts) return;
+  wait_for_previous();
   const int64_t d0 = u * p.items, d1 = min(d0 + p.items, rows + N);
   int64_t t = merge_split(sorted, N, rows, d0);
   const int64_t t_end = merge_split(sorted, N, rows, d1), r_end = d1 - t_end;
   int64_t r = d0 - t;
   // the first row began in an earlier part
-  bool begun = t > 0 && (int64_t)sorted[t - 1].x == r;
-  int head = -1, tail = -1;
+  bool begun = t > 0 && r < rows && (int64_t)sorted[t - 1].x == r;
+  int head = -1;
   float acc[C::N];
 #pragma unroll
   for (int i = 0; i < C::N; ++i) acc[i] = 0.f;
-  bool any = false;
-  while (r < rows) {  // behind the last row: the tokens that take no part
-    // a window of tokens: those of row r are the first k of it
-    const int64_t m = t + lane;
-    const uint2 e = m < t_end ? sorted[m] : make_uint2(0xffffffffu, 0);
-    const unsigned mine = __ballot_sync(0xffffffffu, m < t_end && (int64_t)e.x == r);
-    const int k = __popc(mine);
-    for (int j = 0; j < k; j += kRowsAhead) {
-      float f[kRowsAhead][C::N];
-#pragma unroll
-      for (int a = 0; a < kRowsAhead; ++a) {
-        const unsigned n = __shfl_sync(0xffffffffu, e.y, min(j + a, k - 1));
-        if (j + a < k) col_load<T, VEC>(dy + (int64_t)n * dy_st, c0, lane, D, f[a]);
-      }
-#pragma unroll
-      for (int a = 0; a < kRowsAhead; ++a)
-        if (j + a < k)
-#pragma unroll
-          for (int i = 0; i < C::N; ++i) acc[i] += f[a][i];
-    }
-    t += k;
-    any = any || k > 0;
-    if (k == 32) continue;  // the row may go on
-    if (r >= r_end) break;
+  auto end_row = [&] {
     if (begun) {
       head = (int)r;
 #pragma unroll
@@ -287,9 +384,39 @@ __global__ void __launch_bounds__(kSumWarps * 32) embedding_sum_kernel(const uin
     }
 #pragma unroll
     for (int i = 0; i < C::N; ++i) acc[i] = 0.f;
-    begun = any = false;
+    begun = false;
     ++r;
+  };
+  bool any = false;  // the current row has tokens here
+  for (int64_t w = t; w < t_end; w += 32) {
+    const uint2 e = w + lane < t_end ? sorted[w + lane] : make_uint2((unsigned)rows, 0);
+    const int n = (int)min((int64_t)32, t_end - w);
+    for (int j = 0; j < n; j += kRowsAhead) {
+      typename C::Raw f[kRowsAhead];
+#pragma unroll
+      for (int a = 0; a < kRowsAhead; ++a) {
+        const unsigned token = __shfl_sync(0xffffffffu, e.y, (j + a) & 31);
+        const bool in = j + a < n && __shfl_sync(0xffffffffu, e.x, (j + a) & 31) < (unsigned)rows;
+        f[a] = col_load<T, VEC>(dy + (int64_t)token * dy_st, c0, lane, D, in);
+      }
+#pragma unroll
+      for (int a = 0; a < kRowsAhead; ++a) {
+        const int64_t key = __shfl_sync(0xffffffffu, e.x, (j + a) & 31);
+        if (j + a >= n || key >= rows) break;
+        while (r < key) {
+          end_row();
+          any = false;
+        }
+        col_add<T, VEC>(acc, f[a]);
+        any = true;
+      }
+    }
   }
+  while (r < r_end) {
+    end_row();
+    any = false;
+  }
+  int tail = -1;
   if (r < rows && (any || begun)) {  // the row goes on in the next part
     tail = (int)r;
 #pragma unroll
@@ -302,46 +429,72 @@ __global__ void __launch_bounds__(kSumWarps * 32) embedding_sum_kernel(const uin
 }
 
 // Rows cut by the parts' borders: where a part ended such a row, the parts before it that hold the row's
-// beginning are added in order (8 warps take every eighth, and their sums are added in order), then its own.
+// beginning are added in order, then its own.  A warp for a part; where a row took more than kManyParts, the CTA's
+// eight warps take every eighth, and their sums are added in order.
+constexpr int kManyParts = 16;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) embedding_cut_kernel(T* dtable, int64_t d_st, int D, float scale, int64_t parts,
                                                             const int* heads, const int* tails, float* head_sums,
                                                             float* tail_sums) {
   using C = Cols<T, VEC>;
-  __shared__ float s[8][32][C::N];
-  const int64_t u = blockIdx.x;
-  const int head = heads[u];
-  if (head < 0) return;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  int64_t first = u - 1;  // the part in which the row began
-  for (int64_t f0 = u - 1;; f0 -= 32) {
-    const int64_t f = f0 - lane;
-    const bool through = f >= 0 && tails[f] < -1;
-    const unsigned m = __ballot_sync(0xffffffffu, !through);
-    if (m != 0) {
-      first = f0 - (__ffs(m) - 1);
-      break;
+  __shared__ float s[8][32][C::N + 1];
+  __shared__ int64_t many[8];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, c0 = blockIdx.y * C::kWarp;
+  const int64_t u = (int64_t)blockIdx.x * 8 + warp;
+  wait_for_previous();
+  const int head = u < parts ? heads[u] : -1;
+  int64_t first = u;  // the part in which the row began
+  if (head >= 0) {
+    for (int64_t f0 = u - 1;; f0 -= 32) {
+      const int64_t f = f0 - lane;
+      const unsigned m = __ballot_sync(0xffffffffu, f < 0 || tails[f] >= -1);
+      if (m != 0) {
+        first = f0 - (__ffs(m) - 1);
+        break;
+      }
     }
   }
+  const bool long_row = u - first > kManyParts;
+  if (lane == 0) many[warp] = long_row ? first : -1;
   float acc[C::N];
+  if (head >= 0 && !long_row) {
 #pragma unroll
-  for (int i = 0; i < C::N; ++i) acc[i] = 0.f;
+    for (int i = 0; i < C::N; ++i) acc[i] = 0.f;
 #pragma unroll 4
-  for (int64_t f = first + warp; f < u; f += 8) {
-    const float* q = part_at<C::N>(tail_sums, f, lane);
+    for (int64_t f = first; f <= u; ++f) {
+      const float* q = part_at<C::N>(f == u ? head_sums : tail_sums, f, lane);
 #pragma unroll
-    for (int i = 0; i < C::N; ++i) acc[i] += q[i];
+      for (int i = 0; i < C::N; ++i) acc[i] += q[i];
+    }
+#pragma unroll
+    for (int i = 0; i < C::N; ++i) acc[i] *= scale;
+    col_store<T, VEC>(dtable + head * d_st, c0, lane, D, acc);
   }
-#pragma unroll
-  for (int i = 0; i < C::N; ++i) s[warp][lane][i] = acc[i];
   __syncthreads();
-  if (warp != 0) return;
+  for (int k = 0; k < 8; ++k) {
+    const int64_t from = many[k], to = (int64_t)blockIdx.x * 8 + k;
+    if (from < 0) continue;
 #pragma unroll
-  for (int i = 0; i < C::N; ++i) {
-    for (int w = 1; w < 8; ++w) acc[i] += s[w][lane][i];
-    acc[i] = scale * (acc[i] + part_at<C::N>(head_sums, u, lane)[i]);
+    for (int i = 0; i < C::N; ++i) acc[i] = 0.f;
+#pragma unroll 8
+    for (int64_t f = from + warp; f < to; f += 8) {
+      const float* q = part_at<C::N>(tail_sums, f, lane);
+#pragma unroll
+      for (int i = 0; i < C::N; ++i) acc[i] += q[i];
+    }
+    __syncthreads();  // the sums of the row before this one are read
+#pragma unroll
+    for (int i = 0; i < C::N; ++i) s[warp][lane][i] = acc[i];
+    __syncthreads();
+    if (warp != k) continue;
+#pragma unroll
+    for (int i = 0; i < C::N; ++i) {
+      float sum = 0.f;
+      for (int w = 0; w < 8; ++w) sum += s[w][lane][i];
+      acc[i] = scale * (sum + part_at<C::N>(head_sums, to, lane)[i]);
+    }
+    col_store<T, VEC>(dtable + head * d_st, c0, lane, D, acc);
   }
-  col_store<T, VEC>(dtable + head * d_st, blockIdx.y * C::kWarp, lane, D, acc);
 }
 
 // ---------------------------------------------------------------- plans
@@ -352,16 +505,16 @@ static SortPlan sort_plan(int64_t N, int64_t rows) {
   p.passes = (bits + 8) / 9;
   p.bits = (bits + p.passes - 1) / p.passes;
   const int64_t least = (N + kMostTiles - 1) / kMostTiles;
-  p.tile = least <= kTileLeast ? kTileLeast : (least + kSortThreads - 1) / kSortThreads * kSortThreads;
+  p.tile = least <= kSortThreads ? kSortThreads : (least + kSortThreads - 1) / kSortThreads * kSortThreads;
   p.tiles = (int)((N + p.tile - 1) / p.tile);
   return p;
 }
-// Parts for a few waves of warps; at least 16 items, so that a part's search and partial sums stay small
-// beside its rows.
-static SumPlan sum_plan(int64_t N, int64_t rows) {
-  const int64_t total = N + rows;
-  int64_t items = (total + 4095) / 4096;
-  if (items < 16) items = 16;
+// Parts for two waves of warps over the column blocks; at least 8 items, so that a part's search and partial sums
+// stay small beside its rows.
+static SumPlan sum_plan(int64_t N, int64_t rows, int64_t D) {
+  const int64_t total = N + rows, cols = (D + 255) / 256, parts = 148 * 64 / cols > 148 ? 148 * 64 / cols : 148;
+  int64_t items = (total + parts - 1) / parts;
+  if (items < 8) items = 8;
   return {items, (total + items - 1) / items};
 }
 static int64_t padded_cols(int64_t D) { return (D + 255) / 256 * 256; }
@@ -370,7 +523,7 @@ static size_t up(size_t n) { return (n + 255) / 256 * 256; }
 struct Ws { size_t counts, a, b, heads, tails, head_sums, tail_sums, end; };
 static Ws layout(int64_t N, int64_t rows, int64_t D) {
   const SortPlan sp = sort_plan(N, rows);
-  const SumPlan su = sum_plan(N, rows);
+  const SumPlan su = sum_plan(N, rows, D);
   Ws w;
   w.counts = 0;
   w.a = up((size_t)sp.passes * sp.tiles * (size_t(1) << sp.bits) * 4);
@@ -403,28 +556,31 @@ static int lookup(const void* ids, const void* table, int64_t table_st, void* y,
   constexpr int V = Vec<T>::N;
   const bool vec = vectors(table, table_st, D, sizeof(T)) && vectors(y, y_st, D, sizeof(T));
   const int nv = (int)(vec ? D / V : D);
-  const int64_t blocks = (N * nv + 256 * kLoads - 1) / (256 * kLoads);
-  if (blocks >= (int64_t(1) << 31)) return fail(HDC_E_SHAPE, "embedding: N=%lld x D=%lld is too large", (long long)N, (long long)D);
-  auto t = static_cast<const T*>(table);
-  auto o = static_cast<T*>(y);
-  if (vec) embedding_kernel<T, I, V><<<(unsigned)blocks, 256, 0, s>>>(ids, t, table_st, o, y_st, N, rows, nv, scale);
-  else embedding_kernel<T, I, 1><<<(unsigned)blocks, 256, 0, s>>>(ids, t, table_st, o, y_st, N, rows, nv, scale);
+  int lanes = 1;
+  while (lanes < nv && lanes < 32) lanes *= 2;
+  const int64_t rows_per_block = 256 / lanes * (nv <= lanes ? kLoads : 1), blocks = (N + rows_per_block - 1) / rows_per_block;
+  auto go = [&](auto kernel) {
+    kernel<<<(unsigned)blocks, 256, 0, s>>>(ids, static_cast<const T*>(table), table_st, static_cast<T*>(y), y_st, N, rows, nv,
+                                            lanes, scale);
+  };
+  if (vec) nv <= lanes ? go(embedding_kernel<T, I, V, true>) : go(embedding_kernel<T, I, V, false>);
+  else nv <= lanes ? go(embedding_kernel<T, I, 1, true>) : go(embedding_kernel<T, I, 1, false>);
   return launch_status("embedding_kernel");
 }
 
 template <typename T, bool VEC>
 static int sums(const uint2* sorted, const void* dy, int64_t dy_st, void* dtable, int64_t d_st, int64_t N, int64_t rows,
                 int64_t D, float scale, char* w, const Ws& at, cudaStream_t s) {
-  const SumPlan p = sum_plan(N, rows);
+  const SumPlan p = sum_plan(N, rows, D);
   const unsigned cols = (unsigned)((D + Cols<T, VEC>::kWarp - 1) / Cols<T, VEC>::kWarp);
   int *heads = reinterpret_cast<int*>(w + at.heads), *tails = reinterpret_cast<int*>(w + at.tails);
   float *hs = reinterpret_cast<float*>(w + at.head_sums), *ts = reinterpret_cast<float*>(w + at.tail_sums);
-  embedding_sum_kernel<T, VEC><<<dim3((unsigned)((p.parts + kSumWarps - 1) / kSumWarps), cols), kSumWarps * 32, 0, s>>>(
-      sorted, static_cast<const T*>(dy), dy_st, static_cast<T*>(dtable), d_st, N, rows, (int)D, scale, p, heads, tails,
-      hs, ts);
+  launch_dependent(embedding_sum_kernel<T, VEC>, dim3((unsigned)((p.parts + kSumWarps - 1) / kSumWarps), cols), kSumWarps * 32, 0,
+                   s, sorted, static_cast<const T*>(dy), dy_st, static_cast<T*>(dtable), d_st, N, rows, (int)D, scale, p, heads,
+                   tails, hs, ts);
   if (int e = launch_status("embedding_sum_kernel")) return e;
-  embedding_cut_kernel<T, VEC><<<dim3((unsigned)p.parts, cols), 256, 0, s>>>(static_cast<T*>(dtable), d_st, (int)D, scale,
-                                                                            p.parts, heads, tails, hs, ts);
+  launch_dependent(embedding_cut_kernel<T, VEC>, dim3((unsigned)((p.parts + 7) / 8), cols), 256, 0, s, static_cast<T*>(dtable),
+                   d_st, (int)D, scale, p.parts, static_cast<const int*>(heads), static_cast<const int*>(tails), hs, ts);
   return launch_status("embedding_cut_kernel");
 }
 
@@ -435,16 +591,28 @@ static int gradient(const void* ids, const void* dy, int64_t dy_st, void* dtable
   const Ws at = layout(N, rows, D);
   auto counts = reinterpret_cast<unsigned*>(w + at.counts);
   uint2* buf[2] = {reinterpret_cast<uint2*>(w + at.a), reinterpret_cast<uint2*>(w + at.b)};
-  if (N > 0) {
+  const bool one = N <= kOneTile;
+  if (one && N > 0) {
+    static std::atomic<uint64_t> ready{0};  // devices whose limit of shared memory is set
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+      cudaFuncSetAttribute(embedding_sort_one_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, kOneTile * 8);
+      ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    embedding_sort_one_kernel<I><<<1, kSortThreads, kOneTile * 8, s>>>(ids, buf[0], (int)N, rows, skip, p);
+    if (int e = launch_status("embedding_sort_one_kernel")) return e;
+  } else if (N > 0) {
     embedding_count_kernel<I><<<p.tiles, kSortThreads, 0, s>>>(ids, N, rows, skip, p, counts);
     if (int e = launch_status("embedding_count_kernel")) return e;
     for (int k = 0; k < p.passes; ++k) {
-      embedding_sort_kernel<I><<<p.tiles, kSortThreads, 0, s>>>(ids, buf[(k + 1) % 2], buf[k % 2], N, rows, skip, p, k,
-                                                               counts);
+      launch_dependent(embedding_sort_kernel<I>, dim3(p.tiles), kSortThreads, 0, s, ids, static_cast<const uint2*>(buf[(k + 1) % 2]),
+                       buf[k % 2], N, rows, skip, p, k, counts);
       if (int e = launch_status("embedding_sort_kernel")) return e;
     }
   }
-  const uint2* sorted = buf[(p.passes + 1) % 2];
+  const uint2* sorted = one ? buf[0] : buf[(p.passes + 1) % 2];
   return vectors(dy, dy_st, D, sizeof(T)) && vectors(dtable, d_st, D, sizeof(T))
              ? sums<T, true>(sorted, dy, dy_st, dtable, d_st, N, rows, D, scale, w, at, s)
              : sums<T, false>(sorted, dy, dy_st, dtable, d_st, N, rows, D, scale, w, at, s);
