@@ -2,22 +2,28 @@
 //   norm = sqrt(sum over all tensors and elements of g^2),  out = g * min(1, max_norm / (norm + 1e-6)).
 //
 // Bound by traffic: the gradients are read for the norm, and read and written to be scaled.  All tensors
-// are cut into pieces of kPiece elements; a kernel's CTAs take the pieces in turn, whatever tensor they
-// belong to, so a launch serves up to kTensors tensors of mixed sizes and types.  The table of tensors
-// is a kernel argument: nothing is copied to the device beforehand, and a captured call needs no memory
-// of the host's.  The second kernel walks the pieces backwards, since L2 (126 MB) still holds the ones
-// that were read last; gradients that stay as they are, in place, it does not touch.
-// Sums: a thread adds the squares of kPiece / 256 elements in fp32, and those sums in 64 bits; the CTAs'
+// are cut into pieces of 16 KB; a kernel's CTAs share the pieces, whatever tensor they belong to, so a
+// launch serves up to kTensors tensors of mixed sizes and types.  The table of tensors is a kernel
+// argument: nothing is copied to the device beforehand, and a captured call needs no memory of the
+// host's.  Gradients that stay as they are, in place, the second kernel does not touch.
+// 76.5 M bf16 gradients into other buffers: 83 us for 459 MB, 5.5 TB/s; 190 M bf16 and 0.2 M fp32 204 us.  Reads
+// beside writes go no faster whatever the number of CTAs (2 to 6 per SM), the size of a piece or a second
+// piece in flight: what helps is less traffic, so the second kernel walks the pieces backwards and
+// finds the last 64 MB in L2 (86 and 211 us without; 32, 80 and 100 MB are no better).
+// Sums: a thread adds the squares of a piece's 16 or 32 elements in fp32, and those sums in 64 bits; the CTAs'
 // sums are added in a fixed order.  Where squares leave fp32's range (|g| above 1e18 or all below 1e-16)
 // a thread takes its elements again in 64 bits.
 #include <algorithm>
 #include <memory>
 
 #include "common.cuh"
+#include "vec.cuh"
 
 namespace hdc {
 
-constexpr int kTensors = 512, kThreads = 256, kPiece = 8192, kCtas = 148 * 4;
+constexpr int kTensors = 512, kThreads = 256, kVecs = 4, kPerSm = 4, kCtas = 148 * kPerSm;
+constexpr int kKeep = 4096;  // the last pieces, 64 MB, that the first kernel asks L2 to keep for the second
+template <typename T> constexpr int kPiece = kThreads * kVecs * Vec<T>::N;  // elements: 16 KB
 
 struct ClipTable {
   const void* in[kTensors];
@@ -34,68 +40,123 @@ template <typename T> __host__ __device__ inline int64_t lead(const void* p, int
   return n < k ? n : k;
 }
 
-// One piece as a thread sees it: 16-byte vectors, then at most two single elements (before the first
-// vector of the tensor's first piece, and behind the last one).
-template <typename T> struct Piece {
-  static constexpr int V = Vec<T>::N, kVecs = kPiece / V / kThreads;
-  const T* p;
-  int64_t begin, end, head, tail;  // head, tail: a single element's index, or -1
-  int vecs;
-  __device__ __forceinline__ Piece(const void* q, int64_t n, int piece) {
-    p = static_cast<const T*>(q);
-    const int64_t k = lead<T>(q, n);
-    begin = k + (int64_t)piece * kPiece;
-    end = min(n, begin + kPiece);
-    vecs = (int)((end - begin) / V);
-    head = piece == 0 && (int)threadIdx.x < k ? (int)threadIdx.x : -1;
-    tail = begin + (int64_t)vecs * V + threadIdx.x;
-    if (tail >= end) tail = -1;
+// The pieces of a CTA, every gridDim-th (the CTAs together read one stretch of memory), forwards or backwards, and
+// the tensor of each.
+struct Walk {
+  const ClipTable& t;
+  int i, step, k, pieces;
+  __device__ __forceinline__ Walk(const ClipTable& table, bool backwards) : t(table), pieces(table.first[table.tensors]) {
+    step = backwards ? -(int)gridDim.x : (int)gridDim.x;
+    i = backwards ? pieces - 1 - (int)blockIdx.x : (int)blockIdx.x;
+    k = backwards ? t.tensors - 1 : 0;
+    find();
   }
-  // element index of vector i, or -1
-  __device__ __forceinline__ int64_t at(int i) const {
-    const int v = i * kThreads + threadIdx.x;
-    return v < vecs ? begin + (int64_t)v * V : -1;
+  __device__ __forceinline__ bool more() const { return i >= 0 && i < pieces; }
+  __device__ __forceinline__ void find() {
+    if (!more()) return;
+    while (i >= t.first[k + 1]) ++k;
+    while (i < t.first[k]) --k;
+  }
+  __device__ __forceinline__ void next() {
+    i += step;
+    find();
+  }
+};
+struct Place {
+  const char* in;  // the piece's first 16-byte vector
+  char* out;       // the same element of the output
+  int vecs;        // whole vectors; behind the last piece: -1
+  int head, tail;  // single elements before the first vector (in a tensor's first piece) and behind the last
+  int bf16;
+  bool together;   // in and out reach 16-byte boundaries together
+  __device__ __forceinline__ explicit Place(const Walk& w) : vecs(-1) {
+    if (!w.more()) return;
+    bf16 = w.t.bf16[w.k];
+    const int es = bf16 ? 2 : 4, per = bf16 ? kPiece<__nv_bfloat16> : kPiece<float>;
+    const void* p = w.t.in[w.k];
+    const int64_t n = w.t.n[w.k];
+    const int piece = w.i - w.t.first[w.k];
+    const int64_t k = bf16 ? lead<__nv_bfloat16>(p, n) : lead<float>(p, n), begin = k + (int64_t)piece * per;
+    const int count = (int)min((int64_t)per, n - begin);
+    in = static_cast<const char*>(p) + begin * es;
+    out = static_cast<char*>(w.t.out[w.k]) + begin * es;
+    vecs = count * es / 16;
+    head = piece == 0 ? (int)k : 0;
+    tail = count - vecs * (16 / es);
+    together = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  }
+  // the element that a thread has beside the vectors, as a distance in elements from `in`, or no = kNone
+  static constexpr int kNone = 1 << 30;
+  __device__ __forceinline__ int single() const {
+    const int i = (int)threadIdx.x;
+    return i < head ? i - head : i < head + tail ? vecs * (bf16 ? 8 : 4) + i - head : kNone;
   }
 };
 
-__device__ __forceinline__ int tensor_of(const ClipTable& t, int piece) {
-  int lo = 0, hi = t.tensors - 1;
-  while (lo < hi) {
-    const int m = (lo + hi + 1) / 2;
-    if (t.first[m] <= piece) lo = m;
-    else hi = m - 1;
-  }
-  return lo;
+// A piece's values in registers; zeros where there are none.
+// 16 bytes that L2 keeps or lets go, by the policy
+__device__ __forceinline__ uint4 ldg16_hint(const void* p, uint64_t policy) {
+  uint4 r;
+  asm volatile("ld.global.nc.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p), "l"(policy));
+  return r;
 }
-
-template <typename T> __device__ __forceinline__ double squares(const void* q, int64_t n, int piece) {
-  using P = Piece<T>;
-  const P p(q, n, piece);
-  uint4 w[P::kVecs];
+struct Held {
+  uint4 w[kVecs];
+  float one;
+  __device__ __forceinline__ void load(const Place& p, uint64_t policy) {
+    const char* q = p.in + threadIdx.x * 16;
+    if (p.vecs == kThreads * kVecs) {
 #pragma unroll
-  for (int i = 0; i < P::kVecs; ++i) w[i] = ldg16_pred(p.at(i) < 0 ? p.p : p.p + p.at(i), p.at(i) >= 0);
-  const float h = p.head >= 0 ? to_f(p.p[p.head]) : 0.f, t = p.tail >= 0 ? to_f(p.p[p.tail]) : 0.f;
-  float s = fmaf(h, h, t * t), most = fmaxf(fabsf(h), fabsf(t));
+      for (int i = 0; i < kVecs; ++i) w[i] = ldg16_hint(q + i * kThreads * 16, policy);
+    } else {
 #pragma unroll
-  for (int i = 0; i < P::kVecs; ++i) {
-    float x[P::V];
-    unpack16<T>(w[i], x);
-#pragma unroll
-    for (int j = 0; j < P::V; ++j) {
-      s = fmaf(x[j], x[j], s);
-      most = fmaxf(most, fabsf(x[j]));
+      for (int i = 0; i < kVecs; ++i) {
+        const bool in = i * kThreads + (int)threadIdx.x < p.vecs;
+        w[i] = ldg16_pred(in ? q + i * kThreads * 16 : p.in, in);
+      }
+    }
+    one = 0.f;
+    if (p.head + p.tail > 0) {
+      const int at = p.single();
+      if (at != Place::kNone)
+        one = p.bf16 ? to_f(reinterpret_cast<const __nv_bfloat16*>(p.in)[at]) : reinterpret_cast<const float*>(p.in)[at];
     }
   }
-  if (most < 1e18f && (s > 1e-32f || most == 0.f) && s == s) return s;
-  double d = (double)h * h + (double)t * t;
+};
+
+// x^2 of two values added to two sums
+__device__ __forceinline__ void add_squares(uint64_t& s, float x, float y) {
+  const uint64_t v = pair_bits(x, y);
+  asm("fma.rn.f32x2 %0, %1, %1, %0;" : "+l"(s) : "l"(v));
+}
+template <typename T> __device__ __forceinline__ double squares(const Held& v) {
+  constexpr int V = Vec<T>::N;
+  uint64_t s2[2] = {0, 0};
+  uint32_t bits = __float_as_uint(v.one);
 #pragma unroll
-  for (int i = 0; i < P::kVecs; ++i) {
-    float x[P::V];
-    unpack16<T>(w[i], x);
+  for (int i = 0; i < kVecs; ++i) {
+    float x[V];
+    unpack16<T>(v.w[i], x);
 #pragma unroll
-    for (int j = 0; j < P::V; ++j) d += (double)x[j] * x[j];
+    for (int j = 0; j < V; j += 2) add_squares(s2[j / 2 & 1], x[j], x[j + 1]);
+    bits |= v.w[i].x | v.w[i].y | v.w[i].z | v.w[i].w;
   }
-  return d;
+  float a, b, c, d;
+  bits_pair(s2[0], a, b);
+  bits_pair(s2[1], c, d);
+  const float s = fmaf(v.one, v.one, (a + b) + (c + d));
+  // all zeros, or squares well inside fp32's range
+  if ((s > 1e-32f && s < 3e38f) || (bits & (sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu)) == 0) return s;
+  double e = (double)v.one * v.one;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    float x[V];
+    unpack16<T>(v.w[i], x);
+#pragma unroll
+    for (int j = 0; j < V; ++j) e += (double)x[j] * x[j];
+  }
+  return e;
 }
 
 __device__ __forceinline__ double cta_sum(double v) {
@@ -110,65 +171,86 @@ __device__ __forceinline__ double cta_sum(double v) {
   return r;
 }
 
-__global__ void __launch_bounds__(kThreads) grad_squares_kernel(const __grid_constant__ ClipTable t, double* sums) {
+// The place of the next piece is looked up while a piece's values are on their way.
+__global__ void __launch_bounds__(kThreads, kPerSm) grad_squares_kernel(const __grid_constant__ ClipTable t, double* sums,
+                                                                        int keep_from) {
+  let_next_start();
   double d = 0;
-  const int pieces = t.first[t.tensors];
-  for (int i = blockIdx.x; i < pieces; i += gridDim.x) {
-    const int k = tensor_of(t, i);
-    d += t.bf16[k] ? squares<__nv_bfloat16>(t.in[k], t.n[k], i - t.first[k])
-                   : squares<float>(t.in[k], t.n[k], i - t.first[k]);
+  Walk w(t, false);
+  uint64_t stay, go;
+  asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(stay));
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(go));
+  for (Place at(w); at.vecs >= 0;) {
+    Held v;
+    v.load(at, w.i >= keep_from ? stay : go);
+    const int bf16 = at.bf16;
+    w.next();
+    at = Place(w);
+    d += bf16 ? squares<__nv_bfloat16>(v) : squares<float>(v);
   }
   d = cta_sum(d);
   if (threadIdx.x == 0) sums[blockIdx.x] = d;
 }
 
-template <typename T> __device__ __forceinline__ void scale_piece(const void* q, void* out, int64_t n, int piece, float by) {
-  using P = Piece<T>;
-  const P p(q, n, piece);
-  T* o = static_cast<T*>(out);
-  if (((reinterpret_cast<uintptr_t>(q) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
-    // the two do not reach 16-byte boundaries together
-    const int64_t b = piece == 0 ? 0 : p.begin;
-    for (int64_t i = b + threadIdx.x; i < p.end; i += kThreads) o[i] = from_f<T>(to_f(p.p[i]) * by);
-    return;
+// Written values need not stay in L2: what this kernel has not read yet should.
+__device__ __forceinline__ void stg16_stream(void* p, const uint4& v) {
+  asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+template <typename T> __device__ __forceinline__ void scale_piece(const Held& v, const Place& p, float by) {
+  constexpr int V = Vec<T>::N;
+  if (p.head + p.tail > 0) {
+    const int at = p.single();
+    if (at != Place::kNone) reinterpret_cast<T*>(p.out)[at] = from_f<T>(v.one * by);
   }
-  uint4 w[P::kVecs];
+  char* q = p.out + threadIdx.x * 16;
 #pragma unroll
-  for (int i = 0; i < P::kVecs; ++i)
-    if (p.at(i) >= 0) w[i] = *reinterpret_cast<const uint4*>(p.p + p.at(i));
-  if (p.head >= 0) o[p.head] = from_f<T>(to_f(p.p[p.head]) * by);
-  if (p.tail >= 0) o[p.tail] = from_f<T>(to_f(p.p[p.tail]) * by);
+  for (int i = 0; i < kVecs; ++i) {
+    if (i * kThreads + (int)threadIdx.x >= p.vecs) continue;
+    float x[V];
+    unpack16<T>(v.w[i], x);
 #pragma unroll
-  for (int i = 0; i < P::kVecs; ++i) {
-    if (p.at(i) < 0) continue;
-    float x[P::V];
-    unpack16<T>(w[i], x);
+    for (int j = 0; j < V; j += 2) {
+      uint64_t r;
+      asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(x[j], x[j + 1])), "l"(pair_bits(by, by)));
+      bits_pair(r, x[j], x[j + 1]);
+    }
+    if (p.together) {
+      stg16_stream(q + i * kThreads * 16, pack16<T>(x));
+    } else {
+      T* o = reinterpret_cast<T*>(q + i * kThreads * 16);
 #pragma unroll
-    for (int j = 0; j < P::V; ++j) x[j] *= by;
-    stg16(o + p.at(i), pack16<T>(x));
+      for (int j = 0; j < V; ++j) o[j] = from_f<T>(x[j]);
+    }
   }
 }
 
-__global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_constant__ ClipTable t, const double* sums,
-                                                              int n_sums, float max_norm, float* norm_out) {
+__global__ void __launch_bounds__(kThreads, kPerSm) grad_scale_kernel(const __grid_constant__ ClipTable t, const double* sums,
+                                                                      int n_sums, float max_norm, float* norm_out) {
+  wait_for_previous();
   double d = 0;
   for (int i = threadIdx.x; i < n_sums; i += kThreads) d += sums[i];
   const double norm = sqrt(cta_sum(d));
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   const double c = (double)max_norm / (norm + 1e-6);
   const float by = c >= 1.0 ? 1.f : (float)c;  // NaN stays
-  const int pieces = t.first[t.tensors];
-  for (int j = blockIdx.x; j < pieces; j += gridDim.x) {
-    const int i = pieces - 1 - j, k = tensor_of(t, i);
-    if (by == 1.f && t.in[k] == t.out[k]) continue;
-    if (t.bf16[k]) scale_piece<__nv_bfloat16>(t.in[k], t.out[k], t.n[k], i - t.first[k], by);
-    else scale_piece<float>(t.in[k], t.out[k], t.n[k], i - t.first[k], by);
+  uint64_t go;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(go));
+  Walk w(t, true);
+  for (Place at(w); at.vecs >= 0;) {
+    const Place p = at;
+    const bool skip = by == 1.f && p.in == p.out;  // it stays as it is
+    Held v;
+    if (!skip) v.load(p, go);
+    w.next();
+    at = Place(w);
+    if (!skip) p.bf16 ? scale_piece<__nv_bfloat16>(v, p, by) : scale_piece<float>(v, p, by);
   }
 }
 
 static int64_t pieces_of(const void* p, int64_t n, int dtype) {
-  const int64_t m = n - (dtype == HDC_F32 ? lead<float>(p, n) : lead<__nv_bfloat16>(p, n));
-  return m <= kPiece ? 1 : (m + kPiece - 1) / kPiece;
+  const bool f32 = dtype == HDC_F32;
+  const int64_t m = n - (f32 ? lead<float>(p, n) : lead<__nv_bfloat16>(p, n)), per = f32 ? kPiece<float> : kPiece<__nv_bfloat16>;
+  return m <= per ? 1 : (m + per - 1) / per;
 }
 
 struct Span { uintptr_t begin, end; int tensor, out; };
@@ -240,12 +322,14 @@ static int clip(int64_t n, const int* dtypes, const void* const* grads, void* co
       const int grid = (int)std::min<int64_t>(kCtas, pieces);
       if (pass == 0) {
         if (grid == 0) continue;
-        grad_squares_kernel<<<grid, kThreads, 0, s>>>(*t, sums + used);
+        const int keep_from = outs && g + 1 == groups ? (int)pieces - kKeep : (int)pieces;
+        grad_squares_kernel<<<grid, kThreads, 0, s>>>(*t, sums + used, keep_from);
         used += grid;
         if (int e = launch_status("grad_squares_kernel")) return e;
       } else if (g == 0 || (grid > 0 && outs)) {
         if (!outs) t->tensors = t->first[0] = 0;
-        grad_scale_kernel<<<outs && grid > 0 ? grid : 1, kThreads, 0, s>>>(*t, sums, used, max_norm, g == 0 ? norm : nullptr);
+        launch_dependent(grad_scale_kernel, dim3(outs && grid > 0 ? grid : 1), kThreads, 0, s, *t, static_cast<const double*>(sums),
+                         used, max_norm, g == 0 ? norm : nullptr);
         if (int e = launch_status("grad_scale_kernel")) return e;
       }
     }

@@ -1,6 +1,9 @@
 // Decayed linear attention: entry points, the joining of segments, and the single-token step.
 // The mathematics stands in decay_attn.cuh.
+#include <type_traits>
+
 #include "decay_attn.cuh"
+#include "vec.cuh"
 
 namespace hdc {
 
@@ -15,11 +18,13 @@ __global__ void __launch_bounds__(128) attn_join_kernel(float* states, const flo
   const int64_t bh = blockIdx.x;
   const int i = (blockIdx.y * blockDim.x + threadIdx.x) * V;
   if (i >= DD) return;
+  let_next_start();
   const float d = g[bh % H];
   const float whole = decay_pow(d, seg), rest = decay_pow(d, L - (nseg - 1) * seg);
   float run[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) run[e] = from ? from[bh * DD + i + e] : 0.f;
+  wait_for_previous();
   float* s = states + bh * nseg * DD + i;
   for (int n0 = 0; n0 < nseg; n0 += kAhead) {
     float own[kAhead][V];
@@ -50,64 +55,74 @@ __global__ void __launch_bounds__(128) attn_join_kernel(float* states, const flo
 }
 
 // ---------------------------------------------------------------- one token
-// S <- e S + k v', o = scale q' S.  A CTA per state and 4 * kCols columns: a thread has 4 columns of
-// every kRows-th row, all its loads in flight at once; the rows' parts of o are added in shared memory.
-// Bound by the state's traffic (read and written once) at large batches, by one load's latency and the
-// launch at small ones.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(128) attn_step_kernel(AttnView q, AttnView k, AttnView v, AttnView o, const float* g,
+// S <- e S + k v', o = scale q' S.  256 threads take whole states, one after another in memory: CG lanes of 4
+// columns side by side, the others every RG-th row, their loads in flight at once; the rows' parts of o are added in
+// shared memory.  Bound by the state's traffic (read and written once) at large batches, by one load's latency
+// and the launch at small ones: 12 states of 64 x 64 2.6 us.
+template <typename T, int CG, bool VEC>
+__global__ void __launch_bounds__(256) attn_step_kernel(AttnView q, AttnView k, AttnView v, AttnView o, const float* g,
                                                         const float* state, float* state_out, float scale, int H,
-                                                        int D) {
-  constexpr int kCols = 8, kRows = 16;
-  __shared__ float part[kRows][kCols * 4 + 1];
-  const int64_t bh = blockIdx.x;
-  const int b = (int)(bh / H), h = (int)(bh % H);
-  const int cg = threadIdx.x % kCols, rg = threadIdx.x / kCols;
-  const int c = (blockIdx.y * kCols + cg) * 4;
-  const T* qp = static_cast<const T*>(q.p) + b * q.sb + h * q.sh;
-  const T* kp = static_cast<const T*>(k.p) + b * k.sb + h * k.sh;
-  const T* vp = static_cast<const T*>(v.p) + b * v.sb + h * v.sh;
-  const float e = expf(g[h]);
-  float vv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+                                                        int D, int64_t states) {
+  constexpr int RG = CG == 32 ? 8 : 16, PER = 256 / (CG * RG), ROWS = CG * 4 / RG, AHEAD = ROWS < 8 ? ROWS : 8;
+  __shared__ float part[PER][RG][CG * 4 + 4];
+  const int own = threadIdx.x / (CG * RG), rg = threadIdx.x / CG % RG, c = threadIdx.x % CG * 4;
+  const int64_t bh = (int64_t)blockIdx.x * PER + own;
+  const bool there = bh < states;
+  const int b = there ? (int)(bh / H) : 0, h = there ? (int)(bh % H) : 0;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  if (there && c < D) {
+    const T* qp = static_cast<const T*>(q.p) + b * q.sb + h * q.sh;
+    const T* kp = static_cast<const T*>(k.p) + b * k.sb + h * k.sh;
+    const T* vp = static_cast<const T*>(v.p) + b * v.sb + h * v.sh;
+    const float* s = state + bh * D * D + c;
+    float* t = state_out + bh * D * D + c;
+    const int cols = min(4, D - c);
+    const float e = expf(g[h]);
+    float vv[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) vv[j] = c + j < D ? to_f(vp[c + j]) : 0.f;
-  const float* s = state + bh * D * D;
-  float* t = state_out + bh * D * D;
+    for (int j = 0; j < 4; ++j) vv[j] = j < cols ? to_f(vp[c + j]) : 0.f;
 #pragma unroll
-  for (int i = 0; i < 128 / kRows; ++i) {
-    const int r = rg + i * kRows;
-    if (r >= D) continue;
-    const float kk = to_f(kp[r]), qq = to_f(qp[r]);
-    float x[4];
-    if constexpr (VEC) {
-      if (c >= D) continue;
-      const float4 w = *reinterpret_cast<const float4*>(s + r * D + c);
-      x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
-    } else {
+    for (int i0 = 0; i0 < ROWS; i0 += AHEAD) {
+      float x[AHEAD][4], kk[AHEAD], qq[AHEAD];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = c + j < D ? s[r * D + c + j] : 0.f;
-    }
+      for (int i = 0; i < AHEAD; ++i) {
+        const int r = rg + (i0 + i) * RG;
+        if (r >= D) continue;
+        if constexpr (VEC) {
+          *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(s + r * D);
+        } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] = fmaf(e, x[j], kk * vv[j]);
-      acc[j] = fmaf(qq, x[j], acc[j]);
-    }
-    if constexpr (VEC) {
-      *reinterpret_cast<float4*>(t + r * D + c) = make_float4(x[0], x[1], x[2], x[3]);
-    } else {
+          for (int j = 0; j < 4; ++j) x[i][j] = j < cols ? s[r * D + j] : 0.f;
+        }
+        kk[i] = to_f(kp[r]);
+        qq[i] = to_f(qp[r]);
+      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c + j < D) t[r * D + c + j] = x[j];
+      for (int i = 0; i < AHEAD; ++i) {
+        const int r = rg + (i0 + i) * RG;
+        if (r >= D) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[i][j] = fmaf(e, x[i][j], kk[i] * vv[j]);
+          acc[j] = fmaf(qq[i], x[i][j], acc[j]);
+        }
+        if constexpr (VEC) {
+          *reinterpret_cast<float4*>(t + r * D) = *reinterpret_cast<const float4*>(x[i]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < cols) t[r * D + j] = x[i][j];
+        }
+      }
     }
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) part[rg][cg * 4 + j] = acc[j];
+  *reinterpret_cast<float4*>(&part[own][rg][c]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
   __syncthreads();
-  const int col = blockIdx.y * kCols * 4 + threadIdx.x;
-  if (threadIdx.x >= kCols * 4 || col >= D) return;
+  const int col = threadIdx.x % (CG * RG);
+  if (!there || col >= D) return;
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) sum += part[i][threadIdx.x];
+  for (int i = 0; i < RG; ++i) sum += part[own][i][col];
   static_cast<T*>(const_cast<void*>(o.p))[b * o.sb + h * o.sh + col] = from_f<T>(scale * sum);
 }
 
@@ -173,8 +188,8 @@ static int join(float* states, const float* from, float* to, const AttnParams& p
   const bool vec = p.D % 2 == 0 && aligned16(states) && aligned16(from);
   const int per = vec ? 512 : 128;
   const dim3 grid((unsigned)bh, (unsigned)((DD + per - 1) / per));
-  if (vec) attn_join_kernel<4><<<grid, 128, 0, s>>>(states, from, to, p.g, p.H, p.L, DD, p.nseg, p.seg, backwards);
-  else attn_join_kernel<1><<<grid, 128, 0, s>>>(states, from, to, p.g, p.H, p.L, DD, p.nseg, p.seg, backwards);
+  launch_dependent(vec ? attn_join_kernel<4> : attn_join_kernel<1>, grid, 128, 0, s, states, from, to, p.g, p.H, p.L, DD, p.nseg,
+                   p.seg, backwards);
   return launch_status("attn_join_kernel");
 }
 
@@ -282,12 +297,20 @@ extern "C" int hdc_decay_attn_step(int dtype, const void* q, int64_t q_sb, int64
   const AttnView Q{q, q_sb, 0, q_sh}, K{k, k_sb, 0, k_sh}, V{v, v_sb, 0, v_sh}, O{o, o_sb, 0, o_sh};
   if (!heads_apart(O, B, 1, H, D)) return fail(HDC_E_SHAPE, "decay_attn_step: rows of o overlap");
   auto s = reinterpret_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)(B * H), (unsigned)((D + 31) / 32));
   const bool vec = D % 4 == 0 && aligned16(state) && aligned16(state_out);
-  auto launch = [&](auto kernel) {
-    kernel<<<grid, 128, 0, s>>>(Q, K, V, O, log_decay, state, state_out, scale, (int)H, (int)D);
+  const int64_t n = B * H;
+  auto launch = [&](auto kernel, int per) {
+    kernel<<<(unsigned)((n + per - 1) / per), 256, 0, s>>>(Q, K, V, O, log_decay, state, state_out, scale, (int)H, (int)D, n);
   };
-  if (dtype == HDC_F32) vec ? launch(attn_step_kernel<float, true>) : launch(attn_step_kernel<float, false>);
-  else vec ? launch(attn_step_kernel<__nv_bfloat16, true>) : launch(attn_step_kernel<__nv_bfloat16, false>);
+  auto sized = [&](auto t, auto vec_) {
+    using T = decltype(t);
+    constexpr bool kVec = decltype(vec_)::value;
+    if (D <= 16) launch(attn_step_kernel<T, 4, kVec>, 4);
+    else if (D <= 32) launch(attn_step_kernel<T, 8, kVec>, 2);
+    else if (D <= 64) launch(attn_step_kernel<T, 16, kVec>, 1);
+    else launch(attn_step_kernel<T, 32, kVec>, 1);
+  };
+  if (dtype == HDC_F32) vec ? sized(float(), std::true_type()) : sized(float(), std::false_type());
+  else vec ? sized(__nv_bfloat16(), std::true_type()) : sized(__nv_bfloat16(), std::false_type());
   return launch_status("attn_step_kernel");
 }

@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
   const bf16* zp = static_cast<const bf16*>(a.z.p) + b * a.z.sb + h * a.z.sh;
   const bf16* xp = OUT ? static_cast<const bf16*>(a.x.p) + b * a.x.sb + h * a.x.sh : nullptr;
 
+  let_next_start();
   const float gd = p.g[h];
   for (int i = threadIdx.x; i < 2 * kAttnChunk; i += T) {
     if (i <= kAttnChunk) pw[i] = decay_pow(gd, i);
@@ -167,6 +168,8 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   load(0);
+  // the tensors were there before the sums' kernel began; the states come from the kernel before this one
+  if (OUT) wait_for_previous();
 
   // the warp's part of the state: rows sr + g (+ 8), columns sc + 8 n + 2 c (+ 1)
   const int sr = DP == 32 ? (warp & 1) * 16 : warp * 16, sc = DP == 32 ? (warp >> 1) * 16 : 0;
@@ -417,7 +420,9 @@ static int launch(const AttnParams& p, int64_t bh, int passes, cudaStream_t s) {
     cudaFuncSetAttribute(attn_mma_kernel<DP, OUT, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  attn_mma_kernel<DP, OUT, CB><<<dim3((unsigned)(bh * p.nseg), 1, passes), Sh::kThreads, smem, s>>>(p);
+  const dim3 grid((unsigned)(bh * p.nseg), 1, passes);
+  if (OUT) launch_dependent(attn_mma_kernel<DP, OUT, CB>, grid, Sh::kThreads, smem, s, p);
+  else attn_mma_kernel<DP, OUT, CB><<<grid, Sh::kThreads, smem, s>>>(p);
   return launch_status(OUT ? "attn_mma_kernel" : "attn_mma_kernel (sums)");
 }
 

@@ -2,6 +2,7 @@
 #include <atomic>
 
 #include "decay_attn.cuh"
+#include "vec.cuh"
 
 namespace hdc {
 
@@ -42,7 +43,9 @@ __global__ void __launch_bounds__(256) attn_simt_kernel(AttnParams p) {
   const int begin = seg * p.seg, end = min(p.L, begin + p.seg);
   const int64_t ax = b * a.x.sb + h * a.x.sh, ay = b * a.y.sb + h * a.y.sh, az = b * a.z.sb + h * a.z.sh;
   float* state = a.states + (bh * p.nseg + seg) * D * D;
+  let_next_start();
   for (int i = threadIdx.x; i <= kAttnChunk; i += 256) pw[i] = decay_pow(p.g[h], i);
+  if (OUT) wait_for_previous();  // the states come from the kernel before this one
   for (int i = threadIdx.x; i < DP * DP; i += 256) {
     const int r = i / DP, c = i % DP;
     float x = 0.f;
@@ -165,7 +168,9 @@ static int attn_launch(const AttnParams& p, int64_t bh, int passes, cudaStream_t
     cudaFuncSetAttribute(attn_simt_kernel<DP, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  attn_simt_kernel<DP, OUT><<<dim3((unsigned)(bh * p.nseg), 1, passes), 256, smem, s>>>(p);
+  const dim3 grid((unsigned)(bh * p.nseg), 1, passes);
+  if (OUT) launch_dependent(attn_simt_kernel<DP, OUT>, grid, 256, smem, s, p);
+  else attn_simt_kernel<DP, OUT><<<grid, 256, smem, s>>>(p);
   return launch_status(OUT ? "attn_simt_kernel" : "attn_simt_kernel (sums)");
 }
 

@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_count_kernel(const voi
                                                                        int64_t skip, SortPlan p, unsigned* counts) {
   __shared__ unsigned c[kMaxBins];
   const int bins = 1 << p.bits;
+  let_next_start();
   for (int i = threadIdx.x; i < bins; i += kSortThreads) c[i] = 0;
   __syncthreads();
   const int64_t begin = blockIdx.x * p.tile, end = min(N, begin + p.tile);
@@ -195,6 +196,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const void
   const int bins = 1 << p.bits, shift = pass * p.bits;
   const unsigned* table = counts + (int64_t)pass * p.tiles * bins;
   unsigned* next = pass + 1 < p.passes ? counts + (int64_t)(pass + 1) * p.tiles * bins : nullptr;
+  let_next_start();
   wait_for_previous();
   unsigned all = 0, before = 0;
   if ((int)threadIdx.x < bins) {
@@ -231,6 +233,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_one_kernel(const 
   __shared__ unsigned base[2 * kMaxBins], sums[kSortWarps], count[kMaxBins];
   __shared__ __align__(4) unsigned short part[kSortWarps][kMaxBins];
   const int bins = 1 << p.bits;
+  let_next_start();
   uint2 e[kRounds];
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) {
@@ -360,6 +363,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) embedding_sum_kernel(const uin
   using C = Cols<T, VEC>;
   const int lane = threadIdx.x % 32, c0 = blockIdx.y * C::kWarp;
   const int64_t u = (int64_t)blockIdx.x * kSumWarps + threadIdx.x / 32;
+  let_next_start();
   if (u >= p.parts) return;
   wait_for_previous();
   const int64_t d0 = u * p.items, d1 = min(d0 + p.items, rows + N);
