@@ -87,10 +87,10 @@ SIGNATURES = {
     "hdc_group_norm_bwd_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64]),
     "hdc_group_norm_bwd": (c_int, [c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp,
                                    c_i64, c_i64, c_vp, c_vp, c_vp, c_size, c_i64, c_i64, c_i64, c_i64, c_int, c_vp]),
-    "hdc_decay_attn_segments": (c_i64, [c_i64, c_i64, c_i64]),
+    "hdc_decay_attn_state_slots": (c_i64, [c_int, c_i64, c_i64, c_i64, c_i64]),
     "hdc_decay_attn_fwd": (c_int, [c_int, *[c_vp, c_i64, c_i64, c_i64] * 3, c_vp, c_vp, c_float, c_vp, c_i64, c_i64,
                                    c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp]),
-    "hdc_decay_attn_bwd_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64]),
+    "hdc_decay_attn_bwd_workspace_bytes": (c_size, [c_int, c_i64, c_i64, c_i64, c_i64]),
     "hdc_decay_attn_bwd": (c_int, [c_int, *[c_vp, c_i64, c_i64, c_i64] * 4, c_vp, c_vp, c_vp, c_float,
                                    *[c_vp, c_i64, c_i64, c_i64] * 3, c_vp, c_vp, c_size, c_i64, c_i64, c_i64, c_i64,
                                    c_vp]),

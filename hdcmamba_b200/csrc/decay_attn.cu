@@ -128,25 +128,30 @@ __global__ void __launch_bounds__(256) attn_step_kernel(AttnView q, AttnView k, 
 
 // ---------------------------------------------------------------- plans and checks
 // Tokens of a segment, a function of the sizes alone (so that a forward and its gradient agree, and
-// results do not depend on the device's SM count): enough segments for some kCtas CTAs.
-static int64_t attn_seg(int64_t B, int64_t L, int64_t H) {
+// results do not depend on the device's SM count): enough segments for some kCtas CTAs, or one where a single
+// launch over all chunks takes no longer than the three over segments.  Forward in us, one segment and several
+// (bf16: 16 heads of 32 128 tokens 7 and 13, 257 12 and 12, 512 17 and 13; 12 heads of 64 257 tokens 17 and 13; 128 heads of 64 257 tokens 19 and 29,
+// 1024 45 and 53; 4 heads of 128 128 tokens 19 and 25, 257 35 and 25.  fp32: 12 heads of 64 64 tokens 19 and 19, 128
+// 33 and 25; 128 heads of 64 257 tokens 72 and 78, 384 90 and 78).
+static int64_t attn_seg(int dtype, int64_t B, int64_t L, int64_t H, int64_t D) {
   constexpr int64_t kCtas = 148 * 3;
-  const int64_t chunks = (L + kAttnChunk - 1) / kAttnChunk;
-  if (chunks < 1 || B < 1 || H < 1) return kAttnChunk;
-  int64_t want = kCtas / (B * H);
+  const int64_t chunks = (L + kAttnChunk - 1) / kAttnChunk, heads = B * H;
+  if (chunks < 1 || heads < 1) return kAttnChunk;
+  const int64_t alone = dtype == HDC_F32 ? 1 + heads / 32 : D <= 64 ? 4 + heads / 10 : 2 + heads / 20;
+  int64_t want = chunks <= alone ? 1 : kCtas / heads;
   if (want < 1) want = 1;
   if (want > chunks) want = chunks;
   return (chunks + want - 1) / want * kAttnChunk;
 }
-static int64_t attn_nseg(int64_t B, int64_t L, int64_t H) {
-  const int64_t seg = attn_seg(B, L, H);
+static int64_t attn_nseg(int dtype, int64_t B, int64_t L, int64_t H, int64_t D) {
+  const int64_t seg = attn_seg(dtype, B, L, H, D);
   return (L + seg - 1) / seg;
 }
 
 static int attn_check(const char* what, int dtype, int64_t B, int64_t L, int64_t H, int64_t D) {
   if (dtype != HDC_F32 && dtype != HDC_BF16) return fail(HDC_E_DTYPE, "%s: dtype %d", what, dtype);
   if (B < 0 || L < 0 || H < 1 || D < 1 || D > 128 || L > (int64_t(1) << 30) || B > (int64_t(1) << 30) ||
-      H > (int64_t(1) << 20) || B * H * attn_nseg(B, L, H) >= (int64_t(1) << 31))
+      H > (int64_t(1) << 20) || B * H * attn_nseg(dtype, B, L, H, D) >= (int64_t(1) << 31))
     return fail(HDC_E_SHAPE, "%s: B=%lld, L=%lld in [0, 2^30], H=%lld in [1, 2^20], D=%lld in [1, 128]", what,
                 (long long)B, (long long)L, (long long)H, (long long)D);
   return 0;
@@ -204,8 +209,13 @@ static int copy_state(const char* what, const float* from, float* to, int64_t n,
 
 using namespace hdc;
 
-extern "C" int64_t hdc_decay_attn_segments(int64_t B, int64_t L, int64_t H) {
-  return L < 1 || B < 1 || H < 1 ? 0 : attn_nseg(B, L, H);
+extern "C" int64_t hdc_decay_attn_state_slots(int dtype, int64_t B, int64_t L, int64_t H, int64_t D) {
+  return L < 1 || B < 1 || H < 1 || D < 1 ? 0 : attn_nseg(dtype, B, L, H, D);
+}
+
+static void plan(AttnParams& p, int dtype, const float* log_decay, int64_t B, int64_t L, int64_t H, int64_t D) {
+  p.g = log_decay; p.H = (int)H; p.L = (int)L; p.D = (int)D;
+  p.seg = (int)attn_seg(dtype, B, L, H, D); p.nseg = (int)attn_nseg(dtype, B, L, H, D);
 }
 
 extern "C" int hdc_decay_attn_fwd(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,
@@ -221,24 +231,28 @@ extern "C" int hdc_decay_attn_fwd(int dtype, const void* q, int64_t q_sb, int64_
       off_type(states, HDC_F32))
     return fail(HDC_E_ALIGN, "decay_attn: a pointer is not aligned to its type");
   if (L == 0) return copy_state("decay_attn", state_in, state_out, B * H * D * D, s);
-  if (!q || !k || !v || !o || !log_decay || !states) return fail(HDC_E_NULL, "decay_attn: null pointer");
+  AttnParams p{};
+  plan(p, dtype, log_decay, B, L, H, D);
+  if (!q || !k || !v || !o || !log_decay || (!states && p.nseg > 1)) return fail(HDC_E_NULL, "decay_attn: null pointer");
   auto view = [&](const void* t, int64_t sb, int64_t st, int64_t sh) { return view_of(t, sb, st, sh, B, L, H); };
   const AttnView Q = view(q, q_sb, q_st, q_sh), K = view(k, k_sb, k_st, k_sh), V = view(v, v_sb, v_st, v_sh),
                  O = view(o, o_sb, o_st, o_sh);
   if (!heads_apart(O, B, L, H, D)) return fail(HDC_E_SHAPE, "decay_attn: rows of o overlap");
-  AttnParams p{};
-  p.g = log_decay; p.H = (int)H; p.L = (int)L; p.D = (int)D;
-  p.seg = (int)attn_seg(B, L, H); p.nseg = (int)attn_nseg(B, L, H);
-  p.pass[0] = {Q, K, V, O, states, 0, 0, scale, scale, 1.f};
+  p.pass[0] = {Q, K, V, O, states, state_in, state_out, 0, 0, scale, scale, 1.f};
   const int64_t bh = B * H;
   const bool f32 = dtype == HDC_F32;
-  if (int e = f32 ? attn_sums_f32(p, bh, s) : attn_sums_bf16(p, bh, s)) return e;
-  if (int e = join(states, state_in, state_out, p, bh, 0, s)) return e;
+  if (p.nseg > 1) {
+    if (int e = f32 ? attn_sums_f32(p, bh, s) : attn_sums_bf16(p, bh, s)) return e;
+    if (int e = join(states, state_in, state_out, p, bh, 0, s)) return e;
+  } else if (states) {  // what enters the one segment, for the gradient
+    if (int e = copy_state("decay_attn", state_in, states, bh * D * D, s)) return e;
+  }
   return f32 ? attn_out_f32(p, bh, 1, s) : attn_out_bf16(p, bh, 1, s);
 }
 
-extern "C" size_t hdc_decay_attn_bwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t D) {
-  return L < 1 || B < 1 || H < 1 || D < 1 ? 0 : (size_t)(B * H * attn_nseg(B, L, H)) * D * D * 4;
+extern "C" size_t hdc_decay_attn_bwd_workspace_bytes(int dtype, int64_t B, int64_t L, int64_t H, int64_t D) {
+  const int64_t slots = hdc_decay_attn_state_slots(dtype, B, L, H, D);
+  return slots > 1 ? (size_t)(B * H * slots) * D * D * 4 : 0;
 }
 
 extern "C" int hdc_decay_attn_bwd(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,
@@ -259,8 +273,8 @@ extern "C" int hdc_decay_attn_bwd(int dtype, const void* q, int64_t q_sb, int64_
   if (L == 0) return copy_state("decay_attn_bwd", dstate_out, dstate_in, B * H * D * D, s);
   if (!q || !k || !v || !dout || !dq || !dk || !dv || !log_decay || !states)
     return fail(HDC_E_NULL, "decay_attn_bwd: null pointer");
-  const size_t need = hdc_decay_attn_bwd_workspace_bytes(B, L, H, D);
-  if (!workspace || workspace_bytes < need)
+  const size_t need = hdc_decay_attn_bwd_workspace_bytes(dtype, B, L, H, D);
+  if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(HDC_E_WORKSPACE, "decay_attn_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   if (!aligned16(workspace)) return fail(HDC_E_ALIGN, "decay_attn_bwd: the workspace is not 16-byte aligned");
   auto view = [&](const void* t, int64_t sb, int64_t st, int64_t sh) { return view_of(t, sb, st, sh, B, L, H); };
@@ -271,15 +285,16 @@ extern "C" int hdc_decay_attn_bwd(int dtype, const void* q, int64_t q_sb, int64_
     return fail(HDC_E_SHAPE, "decay_attn_bwd: rows of dq, dk or dv overlap");
   float* grads = static_cast<float*>(workspace);
   AttnParams p{};
-  p.g = log_decay; p.H = (int)H; p.L = (int)L; p.D = (int)D;
-  p.seg = (int)attn_seg(B, L, H); p.nseg = (int)attn_nseg(B, L, H);
+  plan(p, dtype, log_decay, B, L, H, D);
   const int64_t bh = B * H;
   const bool f32 = dtype == HDC_F32;
-  p.pass[0] = {K, Q, DO, DV, grads, 0, 1, scale, 1.f, scale};
-  if (int e = f32 ? attn_sums_f32(p, bh, s) : attn_sums_bf16(p, bh, s)) return e;
-  if (int e = join(grads, dstate_out, dstate_in, p, bh, 1, s)) return e;
-  p.pass[1] = {V, DO, Q, DK, grads, 1, 1, scale, 1.f, scale};
-  p.pass[2] = {DO, V, K, DQ, const_cast<float*>(states), 1, 0, scale, scale, 1.f};
+  p.pass[0] = {K, Q, DO, DV, grads, dstate_out, dstate_in, 0, 1, scale, 1.f, scale};
+  p.pass[1] = {V, DO, Q, DK, grads, dstate_out, nullptr, 1, 1, scale, 1.f, scale};
+  p.pass[2] = {DO, V, K, DQ, const_cast<float*>(states), states, nullptr, 1, 0, scale, scale, 1.f};
+  if (p.nseg > 1) {
+    if (int e = f32 ? attn_sums_f32(p, bh, s) : attn_sums_bf16(p, bh, s)) return e;
+    if (int e = join(grads, dstate_out, dstate_in, p, bh, 1, s)) return e;
+  }
   return f32 ? attn_out_f32(p, bh, 3, s) : attn_out_bf16(p, bh, 3, s);
 }
 

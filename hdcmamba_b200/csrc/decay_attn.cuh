@@ -13,7 +13,9 @@
 //   R <- e^n R + sum_j su up(j) y_j z_j',
 // with in(i) = e^(i+1), up(j) = e^(n-1-j) forwards and in(i) = e^(n-1-i), up(j) = e^(j+1) backwards.
 // A first kernel sums every segment's own state, a second joins the segments, a third writes the
-// outputs; no kernel waits for another CTA, and results do not depend on timing.
+// outputs; a sequence of one segment needs the third alone, which then writes the state behind it too.  No
+// kernel waits for another CTA, and results do not depend on timing.  (Joining up to eight segments in the third
+// kernel instead costs it registers and time: 8 x 4096 x 16 heads of 64 with gradient 544 us for 457.)
 #pragma once
 #include "common.cuh"
 
@@ -29,6 +31,10 @@ struct AttnView {
 struct AttnPass {
   AttnView x, y, z, out;
   float* states;  // [B * H][nseg][D * D]: the state that enters each segment (the sums' kernel: each segment's own)
+  // a sequence of one segment (p.nseg == 1): the state that enters it (NULL: zeros) and, unless NULL, where the one
+  // that leaves it goes
+  const float* from;
+  float* to;
   int transposed, backwards;
   float sa, si, su;
   int out_vec;  // out takes 16-byte stores
@@ -42,6 +48,12 @@ struct AttnParams {
 
 // exp(g d), 1 for d = 0 whatever g is
 __device__ __forceinline__ float decay_pow(float g, int d) { return d == 0 ? 1.f : expf(g * (float)d); }
+
+// the state that enters a CTA's segment, or NULL for zeros
+__device__ __forceinline__ const float* entering(const AttnParams& p, const AttnPass& a, int64_t bh, int seg) {
+  const int64_t DD = (int64_t)p.D * p.D;
+  return p.nseg > 1 ? a.states + (bh * p.nseg + seg) * DD : a.from ? a.from + bh * DD : nullptr;
+}
 
 // csrc/decay_attn_f32.cu, csrc/decay_attn_bf16.cu: the segments' own states (pass 0), and passes' outputs
 int attn_sums_f32(AttnParams& p, int64_t bh, cudaStream_t s);

@@ -7,10 +7,10 @@
 // S becomes P in registers: an accumulator tile has the layout of the next product's operand.
 //
 // Roundings.  P and the copy of R are rounded to bf16 once, as the result is; sums and states stay fp32.  The
-// weighted tokens up(j) y_j would add a third rounding to every state: they are split into bf16 parts, two where
-// only outputs follow (2^-17), three in the segments' sums, from which the fp32 state that the caller gets is
-// made (2^-25).  Those sums are also added up chunk by chunk outside the tensor cores, whose own sums of many
-// steps lose low bits one-sidedly.
+// weighted tokens up(j) y_j would add a third rounding to every state: they are split into two bf16 parts (2^-17), and
+// into three (2^-25) where the fp32 state that the caller gets is made of them: in a sequence of one segment, and in
+// those segments' sums that reach the end of the pass with more than a quarter left.  Sums for such a state are
+// also added up chunk by chunk outside the tensor cores, whose own sums of many steps lose low bits one-sidedly.
 //
 // Why not tcgen05: with heads of 64 a chunk's products are 64 x 64 x 64, each needed by the next within some
 // hundred ns; through tensor memory every one of them costs a round trip (commit, wait, load, convert, store),
@@ -72,6 +72,9 @@ template <bool FIRST, typename A, typename B> __device__ __forceinline__ auto& f
   else return b;
 }
 
+// What a kernel computes: segments' sums; outputs; outputs and the state behind a sequence of one segment.
+constexpr int kSums = 0, kOutputs = 1, kWhole = 2;
+
 template <int DP> struct AttnShape {
   static constexpr int kWarps = DP == 128 ? 8 : 4;
   static constexpr int kThreads = kWarps * 32;
@@ -80,7 +83,7 @@ template <int DP> struct AttnShape {
   static constexpr int kOutCols = DP == 128 ? 64 : DP;            // a warp's columns of the outputs (16 tokens)
   static constexpr int tiles(bool out) { return out ? 3 : 2; }    // of a stage
   static constexpr int smem(bool out) { return 2 * tiles(out) * kTile + (out ? 2 * DP * kPitch<DP> : 0); }
-  static constexpr int ctas(bool out) { return DP == 128 ? 1 : out ? 3 : 4; }
+  static constexpr int ctas(int mode) { return DP == 128 ? 1 : mode == kWhole ? 2 : mode == kOutputs ? 3 : 4; }
 };
 
 // One tile's rows, n of them from p on, to shared memory, zeros behind them.  CB: bytes that every row's pieces
@@ -122,11 +125,12 @@ __device__ __forceinline__ void load_tile(char* s, const bf16* p, int64_t st, in
   }
 }
 
-template <int DP, bool OUT, int CB>
-__global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(OUT)) attn_mma_kernel(const __grid_constant__ AttnParams p) {
+template <int DP, int MODE, int CB>
+__global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(MODE)) attn_mma_kernel(const __grid_constant__ AttnParams p) {
   using Sh = AttnShape<DP>;
+  constexpr bool OUT = MODE != kSums, EXACT = MODE != kOutputs;
   constexpr int T = Sh::kThreads, KD = DP / 16, SN = Sh::kStateCols / 8, ON = Sh::kOutCols / 8, PT = kPitch<DP>;
-  constexpr int SPLITS = OUT ? 2 : 3, STAGE = Sh::tiles(OUT) * Sh::kTile;
+  constexpr int SPLITS = EXACT ? 3 : 2, STAGE = Sh::tiles(OUT) * Sh::kTile;
   extern __shared__ uint4 smem16[];
   __shared__ float pw[kAttnChunk + 1];
   // in(i) si and up(j) su of a whole chunk; a short one of n tokens reads the one that counts from the chunk's
@@ -169,7 +173,7 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
   };
   load(0);
   // the tensors were there before the sums' kernel began; the states come from the kernel before this one
-  if (OUT) wait_for_previous();
+  if (OUT && p.nseg > 1) wait_for_previous();
 
   // the warp's part of the state: rows sr + g (+ 8), columns sc + 8 n + 2 c (+ 1)
   const int sr = DP == 32 ? (warp & 1) * 16 : warp * 16, sc = DP == 32 ? (warp >> 1) * 16 : 0;
@@ -177,7 +181,7 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
   // lower ones have more tiles on their side of the diagonal and a warp's number decides its sub-partition
   const int r = (warp + blockIdx.x) % 4, oc = DP == 128 ? (warp >> 2) * 64 : 0;
   float R[SN][4];
-  float* state = a.states + (bh * p.nseg + seg) * D * D;
+  const float* state = OUT ? entering(p, a, bh, seg) : nullptr;
   auto keep_copy = [&](int q) {  // bf16(R) for the next chunk's product
     char* rb = rbuf + (q & 1) * DP * PT + (sr + g) * PT + sc * 2 + c * 4;
 #pragma unroll
@@ -190,7 +194,7 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int row = sr + g + 8 * (e >> 1), col = sc + 8 * n + 2 * c + (e & 1);
-      R[n][e] = OUT && row < D && col < D ? (a.transposed ? state[col * D + row] : state[row * D + col]) : 0.f;
+      R[n][e] = OUT && state && row < D && col < D ? (a.transposed ? state[col * D + row] : state[row * D + col]) : 0.f;
     }
   // factors of P: on the diagonal's two tiles every element has its own; elsewhere decay^|i - j| is a power that
   // a tile shares times one of four (both at most 1: no power of a strong decay overflows)
@@ -211,6 +215,9 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
   const float* far = pw + (back ? -16 * r - 15 : 16 * r - 7);
   // one chunk: few products, whose roundings would not average out in the outputs, so P is split as well
   const bool fine = p.L <= kAttnChunk;
+
+  // whether the weighted tokens' third part counts
+  const bool third = EXACT && a.to && (OUT || decay_pow(gd, back ? begin : p.L - end) > 0.25f);
 
   // a lane's address of four 8 x 8 blocks: rows first (la), or columns first (lb)
   const uint32_t la = (lane % 8 + 8 * ((lane / 8) % 2)) * PT + lane / 16 * 16;
@@ -252,15 +259,15 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
         scale2(O[n][2], O[n][3], f1, f1);
       }
     }
-    // the state decays over the chunk; the sums' kernel adds a chunk's products up apart
+    // the state decays over the chunk; where it is exact a chunk's products are added up apart
     const float keep = pw[n_rows];
-    float U[OUT ? 1 : SN][4];
+    float U[EXACT ? SN : 1][4];
 #pragma unroll
     for (int n = 0; n < SN; ++n) {
       scale2(R[n][0], R[n][1], keep, keep);
       scale2(R[n][2], R[n][3], keep, keep);
     }
-    auto& acc = first_if<OUT>(R, U);
+    auto& acc = first_if<!EXACT>(R, U);
     const float* up = update + 2 * c + (back ? 0 : shift);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -323,17 +330,20 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
         scale2(lo, hi, up[16 * s + 4 * (e & 2)], up[16 * s + 4 * (e & 2) + 1]);
 #pragma unroll
         for (int k = 0; k < SPLITS; ++k) {
+          if (k == 2 && !third) break;
           part[k][e] = pack2(lo, hi);
           if (k + 1 < SPLITS) less2(lo, hi, part[k][e]);
         }
       }
 #pragma unroll
-      for (int k = SPLITS - 1; k >= 0; --k)
+      for (int k = 0; k < SPLITS; ++k) {
+        if (k == 2 && !third) break;
 #pragma unroll
         for (int n = 0; n < SN; ++n) {
-          if (!OUT && s == 0 && k == SPLITS - 1) mma0(acc[n], part[k], z[n][0], z[n][1]);
+          if (EXACT && s == 0 && k == 0) mma0(acc[n], part[k], z[n][0], z[n][1]);
           else mma(acc[n], part[k], z[n][0], z[n][1]);
         }
+      }
       if constexpr (OUT) {
         if (mine) {
 #pragma unroll
@@ -354,12 +364,13 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
         }
       }
     }
-    if constexpr (!OUT) {
+    if constexpr (EXACT) {
 #pragma unroll
       for (int n = 0; n < SN; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) R[n][e] += U[n][e];
-    } else {
+    }
+    if constexpr (OUT) {
       if (q + 1 < chunks) keep_copy(q + 1);
       bf16* out = static_cast<bf16*>(const_cast<void*>(a.out.p)) + b * a.out.sb + h * a.out.sh + (int64_t)t0 * a.out.st;
       // through the strip's own rows of X, which no other warp reads (wide heads: the strip's second warp)
@@ -391,13 +402,15 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(O
       }
     }
   }
-  if constexpr (!OUT) {
+  if constexpr (EXACT) {  // a segment's own sum, or the state behind a sequence of one segment
+    float* to = !OUT ? a.states + (bh * p.nseg + seg) * D * D : a.to ? a.to + bh * D * D : nullptr;
+    if (!to) return;
 #pragma unroll
     for (int n = 0; n < SN; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int row = sr + g + 8 * (e >> 1), col = sc + 8 * n + 2 * c + (e & 1);
-        if (row < D && col < D) state[row * D + col] = R[n][e];
+        if (row < D && col < D) to[row * D + col] = R[n][e];
       }
   }
 }
@@ -408,43 +421,45 @@ static int bytes_at_once(const AttnView& v, int D) {
   return at % 16 == 0 ? 16 : at % 4 == 0 ? 4 : 2;
 }
 
-template <int DP, bool OUT, int CB>
+template <int DP, int MODE, int CB>
 static int launch(const AttnParams& p, int64_t bh, int passes, cudaStream_t s) {
   using Sh = AttnShape<DP>;
-  constexpr int smem = Sh::smem(OUT);
+  constexpr int smem = Sh::smem(MODE != kSums);
   static std::atomic<uint64_t> ready{0};  // devices whose limit of shared memory is set
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = uint64_t(1) << (dev & 63);
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    cudaFuncSetAttribute(attn_mma_kernel<DP, OUT, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaFuncSetAttribute(attn_mma_kernel<DP, MODE, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
   const dim3 grid((unsigned)(bh * p.nseg), 1, passes);
-  if (OUT) launch_dependent(attn_mma_kernel<DP, OUT, CB>, grid, Sh::kThreads, smem, s, p);
-  else attn_mma_kernel<DP, OUT, CB><<<grid, Sh::kThreads, smem, s>>>(p);
-  return launch_status(OUT ? "attn_mma_kernel" : "attn_mma_kernel (sums)");
+  if (MODE == kOutputs && p.nseg > 1) launch_dependent(attn_mma_kernel<DP, MODE, CB>, grid, Sh::kThreads, smem, s, p);
+  else attn_mma_kernel<DP, MODE, CB><<<grid, Sh::kThreads, smem, s>>>(p);
+  return launch_status(MODE == kSums ? "attn_mma_kernel (sums)" : "attn_mma_kernel");
 }
 
-template <bool OUT>
+template <int MODE>
 static int run(AttnParams& p, int64_t bh, int passes, cudaStream_t s) {
   int cb = 16;
   for (int i = 0; i < passes; ++i) {
     AttnPass& a = p.pass[i];
     cb = min(cb, min(bytes_at_once(a.y, p.D), bytes_at_once(a.z, p.D)));
-    if (OUT) cb = min(cb, bytes_at_once(a.x, p.D));
-    a.out_vec = OUT && bytes_at_once(a.out, p.D) == 16;
+    if (MODE != kSums) cb = min(cb, bytes_at_once(a.x, p.D));
+    a.out_vec = MODE != kSums && bytes_at_once(a.out, p.D) == 16;
   }
   auto sized = [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
-    return cb == 16 ? launch<DP, OUT, 16>(p, bh, passes, s)
-           : cb == 4 ? launch<DP, OUT, 4>(p, bh, passes, s) : launch<DP, OUT, 2>(p, bh, passes, s);
+    return cb == 16 ? launch<DP, MODE, 16>(p, bh, passes, s)
+           : cb == 4 ? launch<DP, MODE, 4>(p, bh, passes, s) : launch<DP, MODE, 2>(p, bh, passes, s);
   };
   return p.D <= 32   ? sized(std::integral_constant<int, 32>())
          : p.D <= 64 ? sized(std::integral_constant<int, 64>()) : sized(std::integral_constant<int, 128>());
 }
 
-int attn_sums_bf16(AttnParams& p, int64_t bh, cudaStream_t s) { return run<false>(p, bh, 1, s); }
-int attn_out_bf16(AttnParams& p, int64_t bh, int passes, cudaStream_t s) { return run<true>(p, bh, passes, s); }
+int attn_sums_bf16(AttnParams& p, int64_t bh, cudaStream_t s) { return run<kSums>(p, bh, 1, s); }
+int attn_out_bf16(AttnParams& p, int64_t bh, int passes, cudaStream_t s) {
+  return p.nseg == 1 && p.pass[0].to ? run<kWhole>(p, bh, passes, s) : run<kOutputs>(p, bh, passes, s);
+}
 
 }  // namespace hdc

@@ -70,7 +70,9 @@ __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(c
   const float* xp = OUT ? static_cast<const float*>(a.x.p) + b * a.x.sb + h * a.x.sh : nullptr;
   const float* yp = static_cast<const float*>(a.y.p) + b * a.y.sb + h * a.y.sh;
   const float* zp = static_cast<const float*>(a.z.p) + b * a.z.sb + h * a.z.sh;
-  float* state = a.states + (bh * p.nseg + seg) * D * D;
+  const float* state = OUT ? entering(p, a, bh, seg) : nullptr;
+  // the state behind the segment goes: a segment's own sum, or the state behind a sequence of one segment
+  float* to = !OUT ? a.states + (bh * p.nseg + seg) * D * D : p.nseg == 1 && a.to ? a.to + bh * D * D : nullptr;
   const int chunks = (end - begin + kAttnChunk - 1) / kAttnChunk;
   let_next_start();
   for (int i = threadIdx.x; i <= kAttnChunk; i += 256) pw[i] = decay_pow(p.g[h], i);
@@ -84,7 +86,7 @@ __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(c
       if (OUT) wait_for_previous();  // the states come from the kernel before this one
       for (int i = threadIdx.x; i < KD * KD; i += 256) {
         const int r = i / KD, c = i % KD;
-        R[i] = OUT && r < D && c < D ? (a.transposed ? state[c * D + r] : state[r * D + c]) : 0.f;
+        R[i] = OUT && state && r < D && c < D ? (a.transposed ? state[c * D + r] : state[r * D + c]) : 0.f;
       }
     }
     __syncthreads();
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(c
           }
         }
     }
-    if (!OUT || q + 1 < chunks) {
+    if (to || q + 1 < chunks) {
       // R = e^n R + sum up(j) y_j z_j': rows 2 ty + 32 k, columns 2 tx + 32 m (+ 1)
       const int ty = threadIdx.x / 16;
       uint64_t r[2 * G][G];
@@ -216,9 +218,9 @@ __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(c
           *reinterpret_cast<uint64_t*>(R + (ty * 2 + 32 * (k / 2) + k % 2) * KD + tx * 2 + 32 * m) = r[k][m];
     }
   }
-  if (!OUT) {
+  if (to) {
     __syncthreads();
-    for (int i = threadIdx.x; i < D * D; i += 256) state[i] = R[i / D * KD + i % D];
+    for (int i = threadIdx.x; i < D * D; i += 256) to[i] = R[i / D * KD + i % D];
   }
 }
 
@@ -233,7 +235,7 @@ template <int G, bool OUT, bool VEC> static int launch(const AttnParams& p, int6
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
   const dim3 grid((unsigned)(bh * p.nseg), 1, passes);
-  if (OUT) launch_dependent(attn_f32_kernel<G, OUT, VEC>, grid, 256, smem, s, p);
+  if (OUT && p.nseg > 1) launch_dependent(attn_f32_kernel<G, OUT, VEC>, grid, 256, smem, s, p);
   else attn_f32_kernel<G, OUT, VEC><<<grid, 256, smem, s>>>(p);
   return launch_status(OUT ? "attn_f32_kernel" : "attn_f32_kernel (sums)");
 }

@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -68,9 +69,8 @@ struct On {
 Tensor make(at::IntArrayRef shape, const Tensor& like, at::ScalarType type) {
   return at::empty(shape, like.options().dtype(type).requires_grad(false));
 }
-Tensor workspace(size_t bytes, const Tensor& like) {
-  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte).requires_grad(false));
-}
+// Scratch memory of the current stream, given back at the end of the call (to kernels that come later there).
+c10::DataPtr workspace(size_t bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(bytes); }
 
 // ---------------------------------------------------------------- linear attention with a decay for each head
 void is_heads(const Tensor& t, const Tensor& q, const char* what) {
@@ -112,7 +112,7 @@ struct Out {
   Tensor o, state, states;
 };
 Out attn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, double scale,
-                 const Maybe& state, const Maybe& out) {
+                 const Maybe& state, const Maybe& out, bool want_states) {
   Attn a(q, k, v, log_decay, 4);
   is_state(state, q, "state");
   if (out) {
@@ -125,10 +125,12 @@ Out attn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
   Out r;
   r.o = out ? *out : make({a.B, a.L, a.H, a.D}, q, q.scalar_type());
   r.state = make({a.B, a.H, a.D, a.D}, q, at::kFloat);
-  r.states = make({a.B, a.H, hdc_decay_attn_segments(a.B, a.L, a.H), a.D, a.D}, q, at::kFloat);
+  const int64_t n = hdc_decay_attn_state_slots(a.code, a.B, a.L, a.H, a.D);
+  if (want_states || n > 1) r.states = make({a.B, a.H, n, a.D, a.D}, q, at::kFloat);
   done("hdc_decay_attn_fwd",
        hdc_decay_attn_fwd(a.code, VIEW(q), VIEW(k), VIEW(v), ptr<float>(a.g), ptr<float>(state), (float)scale, VIEW(r.o),
-                          ptr<float>(r.state), ptr<float>(r.states), a.B, a.L, a.H, a.D, on.stream));
+                          ptr<float>(r.state), r.states.defined() ? ptr<float>(r.states) : nullptr, a.B, a.L, a.H, a.D,
+                          on.stream));
   return r;
 }
 
@@ -141,7 +143,7 @@ Grads attn_backward(Tensor dout, const Tensor& q, const Tensor& k, const Tensor&
   same_type(q, dout);
   TORCH_CHECK_VALUE(dout.sizes() == q.sizes(), "do must be ", q.sizes(), ", got ", dout.sizes());
   is_state(dstate, q, "dstate");
-  const int64_t n = hdc_decay_attn_segments(a.B, a.L, a.H);
+  const int64_t n = hdc_decay_attn_state_slots(a.code, a.B, a.L, a.H, a.D);
   TORCH_CHECK_VALUE(states.scalar_type() == at::kFloat && states.is_contiguous() &&
                         states.sizes() == at::IntArrayRef({a.B, a.H, n, a.D, a.D}),
                     "states must be a contiguous fp32 [", a.B, ", ", a.H, ", ", n, ", ", a.D, ", ", a.D, "] tensor");
@@ -152,12 +154,12 @@ Grads attn_backward(Tensor dout, const Tensor& q, const Tensor& k, const Tensor&
   Grads r;
   for (Tensor* t : {&r.dq, &r.dk, &r.dv}) *t = make({a.B, a.L, a.H, a.D}, q, q.scalar_type());
   if (need_dstate) r.dstate = make({a.B, a.H, a.D, a.D}, q, at::kFloat);
-  const size_t bytes = hdc_decay_attn_bwd_workspace_bytes(a.B, a.L, a.H, a.D);
-  const Tensor ws = workspace(bytes, q);
+  const size_t bytes = hdc_decay_attn_bwd_workspace_bytes(a.code, a.B, a.L, a.H, a.D);
+  const auto ws = workspace(bytes);
   done("hdc_decay_attn_bwd",
        hdc_decay_attn_bwd(a.code, VIEW(q), VIEW(k), VIEW(v), VIEW(dout), ptr<float>(a.g), ptr<float>(states),
                           ptr<float>(dstate), (float)scale, VIEW(r.dq), VIEW(r.dk), VIEW(r.dv),
-                          need_dstate ? ptr<float>(r.dstate) : nullptr, ptr(ws), bytes, a.B, a.L, a.H, a.D, on.stream));
+                          need_dstate ? ptr<float>(r.dstate) : nullptr, ws.get(), bytes, a.B, a.L, a.H, a.D, on.stream));
   return r;
 }
 
@@ -179,7 +181,7 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["state_type"] = state ? (int64_t)state->scalar_type() : (int64_t)-1;
     const Maybe s = state ? Maybe(state->to(at::kFloat).contiguous()) : std::nullopt;
-    Out r = attn_forward(q, k, v, log_decay, scale, s, std::nullopt);
+    Out r = attn_forward(q, k, v, log_decay, scale, s, std::nullopt, true);
     ctx->save_for_backward({q, k, v, log_decay, r.states});
     return {r.o, r.state};
   }
@@ -245,9 +247,9 @@ Tensor lookup_backward(const Tensor& dy, const Tensor& ids, int64_t rows, double
   Tensor g = dy.dim() == 2 ? dy : dy.reshape({-1, D});
   if (D > 1 && g.stride(1) != 1) g = g.contiguous();
   const size_t n = hdc_embedding_bwd_workspace_bytes(i.numel(), rows, D);
-  const Tensor ws = workspace(n, dy);
+  const auto ws = workspace(n);
   done("hdc_embedding_bwd", hdc_embedding_bwd(code, ptr(i), bytes, ptr(g), g.stride(0), ptr(d), d.stride(0), (float)scale,
-                                              skip, ptr(ws), n, i.numel(), rows, D, on.stream));
+                                              skip, ws.get(), n, i.numel(), rows, D, on.stream));
   return d;
 }
 
@@ -316,8 +318,9 @@ PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 PyObject* py_attn(PyObject* const* a) {
-  const Out r = attn_forward(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), number(a[4]), maybe(a[5]), maybe(a[6]));
-  return truth(a[7]) ? tuple(r.o, r.state, r.states) : tuple(r.o, r.state);
+  const bool states = truth(a[7]);
+  const Out r = attn_forward(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), number(a[4]), maybe(a[5]), maybe(a[6]), states);
+  return states ? tuple(r.o, r.state, r.states) : tuple(r.o, r.state);
 }
 PyObject* py_attn_bwd(PyObject* const* a) {
   const Grads r = attn_backward(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]), tensor(a[5]),
@@ -396,12 +399,12 @@ PyObject* py_clip(PyObject* const* a) {
   On on(grads.first);
   const Tensor norm = make({}, grads.first, at::kFloat);
   const size_t bytes = hdc_clip_grads_workspace_bytes(n);
-  const Tensor ws = workspace(bytes, grads.first);
+  const auto ws = workspace(bytes);
   const bool scale = a[1] != Py_None;
   void* const* to = out ? out->at.data() : grads.at.data();
   done("hdc_clip_grads", hdc_clip_grads(n, grads.codes.data(), const_cast<const void* const*>(grads.at.data()),
                                         scale ? to : nullptr, grads.sizes.data(), scale ? (float)number(a[1]) : 0.f,
-                                        ptr<float>(norm), ptr(ws), bytes, on.stream));
+                                        ptr<float>(norm), ws.get(), bytes, on.stream));
   return wrap(norm);
 }
 PyObject* py_set_error(PyObject*, PyObject* type) {

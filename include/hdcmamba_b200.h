@@ -462,23 +462,24 @@ int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_t dy_sn, in
  * row i belonging to k's element i.  Products of bf16 tensors run on the tensor cores with fp32 sums; a
  * token's infinities and NaN may also reach the up to 63 tokens before it.
  *   state_in, state_out : NULL or fp32 [B, H, D, D]; may be the same.
- *   states : fp32 [B, H, hdc_decay_attn_segments(B, L, H), D, D]: the states between the sequence's
- *            segments, which the gradient starts from.
+ *   states : fp32 [B, H, hdc_decay_attn_state_slots(dtype, B, L, H, D), D, D]: states between the parts that
+ *            the sequence is cut into, which the gradient starts from; may be NULL where there is one slot and
+ *            no gradient follows.
  * hdc_decay_attn_bwd: states as the forward left them; dstate_out NULL or the gradient of state_out;
- *   writes dq, dk, dv and, unless NULL, dstate_in (may be dstate_out).  workspace:
+ *   writes dq, dk, dv and, unless NULL, dstate_in (not overlapping dstate_out).  workspace:
  *   hdc_decay_attn_bwd_workspace_bytes, 16-byte aligned.
  * hdc_decay_attn_step: one token per sequence, q [B, H, D] (strides q_sb, q_sh); state_out may be state.
- * D in [1, 128], B, L in [0, 2^30], H in [1, 2^20], B * H * segments < 2^31.  Rows of o, dq, dk and dv must
+ * D in [1, 128], B, L in [0, 2^30], H in [1, 2^20], B * H * slots < 2^31.  Rows of o, dq, dk and dv must
  * not overlap, nor the outputs the inputs.  Pointers need their type's alignment; 16-byte aligned heads
  * take the wide loads.  Results do not depend on timing.
  */
-int64_t hdc_decay_attn_segments(int64_t B, int64_t L, int64_t H);
+int64_t hdc_decay_attn_state_slots(int dtype, int64_t B, int64_t L, int64_t H, int64_t D);
 int hdc_decay_attn_fwd(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,
                        int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
                        int64_t v_sh, const float* log_decay, const float* state_in, float scale, void* o,
                        int64_t o_sb, int64_t o_st, int64_t o_sh, float* state_out, float* states, int64_t B,
                        int64_t L, int64_t H, int64_t D, hdc_stream_t stream);
-size_t hdc_decay_attn_bwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t D);
+size_t hdc_decay_attn_bwd_workspace_bytes(int dtype, int64_t B, int64_t L, int64_t H, int64_t D);
 int hdc_decay_attn_bwd(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,
                        int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
                        int64_t v_sh, const void* dout, int64_t do_sb, int64_t do_st, int64_t do_sh,

@@ -45,7 +45,7 @@ def test_attention_refusals():
     for kw in bad:
         with pytest.raises((ValueError, TypeError)):
             ops.decay_attention(**(dict(q=q, k=q, v=q, log_decay=g) | kw))
-    n = ops._size("hdc_decay_attn_segments", 2, 5, 3)
+    n = ops._size("hdc_decay_attn_state_slots", 0, 2, 5, 3, 8)
     st = torch.zeros(2, 3, n, 8, 8)
     for kw in (dict(do=q.bfloat16()), dict(do=q[:, :4]), dict(states=st[:, :2]), dict(states=st.double()),
                dict(dstate=s[:1])):
@@ -117,7 +117,7 @@ def test_c_checks_attention():
     assert attn_fwd(dtype=2) == -1
     assert attn_fwd(D=129) == -2 and attn_fwd(D=0) == -2 and attn_fwd(H=0) == -2 and attn_fwd(L=-1) == -2 and attn_fwd(B=-1) == -2
     assert attn_fwd(L=2 ** 30 + 1) == -2 and attn_fwd(B=2 ** 30, H=4) == -2
-    assert attn_fwd(q=None) == -4 and attn_fwd(states=None) == -4 and attn_fwd(g=None) == -4 and attn_fwd(o=None) == -4
+    assert attn_fwd(q=None) == -4 and attn_fwd(L=4096, st=(1 << 20, 32, 8), ost=(1 << 20, 32, 8), states=None) == -4 and attn_fwd(g=None) == -4 and attn_fwd(o=None) == -4
     assert attn_fwd(q=A + 1) == -3 and attn_fwd(states=A + 2) == -3 and attn_fwd(dtype=0, o=A + 2) == -3
     # rows of o that overlap: each of the three strides too short
     for ost in ((64, 32, 7), (64, 31, 8), (63, 32, 8), (0, 32, 8), (64, 0, 8), (8, 8, 8)):
@@ -130,9 +130,12 @@ def test_c_checks_attention():
         return rc("hdc_decay_attn_bwd", v["dtype"], A, *st, A, *st, A, *st, A, *st, A, v["states"], None, 1.0, v["dq"], *v["dst"],
                   v["dk"], *v["dst"], v["dv"], *v["dst"], None, v["ws"], v["n"], v["B"], v["L"], v["H"], v["D"], None)[0]
 
-    need = _lib.load().hdc_decay_attn_bwd_workspace_bytes(2, 2, 4, 8)
-    assert need == 2 * 4 * 64 * 4
-    assert bwd(n=need - 1) == -5 and bwd(ws=None) == -5 and bwd(ws=A + 8) == -3 and bwd(dq=None) == -4 and bwd(states=None) == -4
+    assert _lib.load().hdc_decay_attn_bwd_workspace_bytes(1, 2, 2, 4, 8) == 0  # one segment
+    need = _lib.load().hdc_decay_attn_bwd_workspace_bytes(1, 2, 4096, 4, 8)
+    assert need == 2 * 4 * 64 * 4 * _lib.load().hdc_decay_attn_state_slots(1, 2, 4096, 4, 8) > 0
+    long = dict(L=4096, dst=(1 << 20, 32, 8))
+    assert bwd(n=need - 1, **long) == -5 and bwd(ws=None, **long) == -5 and bwd(ws=A + 8, **long) == -3
+    assert bwd(dq=None) == -4 and bwd(states=None) == -4
     assert bwd(dst=(64, 32, 4)) == -2 and bwd(dtype=7) == -1 and bwd(B=0) == 0
 
     def step(**kw):
@@ -144,12 +147,14 @@ def test_c_checks_attention():
     assert step(ost=(32, 4)) == -2 and step(ost=(0, 8)) == -2 and step(B=0) == 0
 
 
-def test_segments_are_a_function_of_the_sizes():
-    n = _lib.load().hdc_decay_attn_segments
-    for B, L, H in ((1, 1, 1), (1, 64, 1), (1, 65, 1), (1, 32768, 12), (8, 4096, 16), (1000, 1000, 16), (1, 1 << 30, 1)):
-        s = n(B, L, H)
-        assert 1 <= s <= -(-L // 64) and B * H * s <= max(B * H, 2048), (B, L, H, s)
-    assert n(1, 0, 1) == 0 and n(0, 5, 1) == 0
+def test_state_slots_are_a_function_of_the_sizes():
+    n = _lib.load().hdc_decay_attn_state_slots
+    for dtype in (0, 1):
+        for B, L, H in ((1, 1, 1), (1, 64, 1), (1, 65, 1), (1, 32768, 12), (8, 4096, 16), (1000, 1000, 16), (1, 1 << 30, 1)):
+            for D in (1, 64, 128):
+                s = n(dtype, B, L, H, D)
+                assert 1 <= s <= -(-L // 64) + 1 and B * H * s <= max(2 * B * H, 2048), (B, L, H, D, s)
+        assert n(dtype, 1, 0, 1, 64) == 0 and n(dtype, 0, 5, 1, 64) == 0
 
 
 def test_c_checks_embedding():
