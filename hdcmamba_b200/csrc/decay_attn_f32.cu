@@ -15,9 +15,10 @@
 namespace hdc {
 
 template <int G> struct F32Shape {
-  static constexpr int kD = 32 * G, kY = kD + 4, kP = kAttnChunk + 4;  // row pitches: X, Z and R; Y; P
+  // row pitches: X and Z; Y; R (transposed states are stored four rows apart); P
+  static constexpr int kD = 32 * G, kY = kD + 4, kR = kD + 2, kP = kAttnChunk + 4;
   static constexpr int kX = kAttnChunk * (kD > kP ? kD : kP);          // X, and P in its place
-  static constexpr int smem(bool out) { return 4 * ((out ? kX : 0) + kAttnChunk * (kY + kD) + kD * kD); }
+  static constexpr int smem(bool out) { return 4 * ((out ? kX : 0) + kAttnChunk * (kY + kD) + kD * kR); }
   static constexpr int ctas(bool out) { return G == 4 ? 1 : G == 3 ? 2 : 3; }
 };
 
@@ -47,16 +48,41 @@ __device__ __forceinline__ void load_rows(float* s, int pitch, const float* p, i
   }
 }
 
+// A state (NULL: zeros) to shared memory; zeros in the rows and columns from D on.
+template <int KD, bool VEC>
+__device__ __forceinline__ void load_state(float* R, int pitch, const float* state, int transposed, int D) {
+  constexpr int E = VEC ? 4 : 1, PER = KD / E;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < KD * PER; i += 256) {
+    const int r = i / PER, c = i % PER * E;  // of the state in memory
+    const bool in = state && r < D && c < D;
+    float x[E];
+    if constexpr (VEC) {
+      // written by the kernel before this one: not through the read-only path
+      *reinterpret_cast<float4*>(x) = in ? *reinterpret_cast<const float4*>(state + r * D + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+      x[0] = in ? state[r * D + c] : 0.f;
+    }
+    if (transposed) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) R[(c + e) * pitch + r] = x[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) R[r * pitch + c + e] = x[e];
+    }
+  }
+}
+
 template <int G, bool OUT, bool VEC>
 __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(const __grid_constant__ AttnParams p) {
   using Sh = F32Shape<G>;
-  constexpr int KD = Sh::kD, PY = Sh::kY, PP = Sh::kP;
+  constexpr int KD = Sh::kD, PY = Sh::kY, PR = Sh::kR, PP = Sh::kP;
   extern __shared__ float4 smem4[];
-  float* R = reinterpret_cast<float*>(smem4);
-  float* Z = R + KD * KD;
+  float* Z = reinterpret_cast<float*>(smem4);
   float* Y = Z + kAttnChunk * KD;
   float* X = Y + kAttnChunk * PY;
   float* P = X;
+  float* R = OUT ? X + Sh::kX : X;
   __shared__ float pw[kAttnChunk + 1];
   const AttnPass& a = p.pass[blockIdx.z];
   const int D = p.D, DR = (D + 3) & ~3, back = a.backwards;
@@ -84,10 +110,7 @@ __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(c
     if (OUT) load_rows<KD, VEC>(X, KD, xp + (int64_t)t0 * a.x.st, a.x.st, n, D);
     if (q == 0) {
       if (OUT) wait_for_previous();  // the states come from the kernel before this one
-      for (int i = threadIdx.x; i < KD * KD; i += 256) {
-        const int r = i / KD, c = i % KD;
-        R[i] = OUT && state && r < D && c < D ? (a.transposed ? state[c * D + r] : state[r * D + c]) : 0.f;
-      }
+      load_state<KD, VEC>(R, PR, OUT ? state : nullptr, a.transposed, D);
     }
     __syncthreads();
     if constexpr (OUT) {
@@ -101,7 +124,7 @@ __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(c
         for (int k = 0; k < 4; ++k) {
           uint64_t w[G];
 #pragma unroll
-          for (int m = 0; m < G; ++m) w[m] = two(R + (d + k) * KD + tx * 2 + 32 * m);
+          for (int m = 0; m < G; ++m) w[m] = two(R + (d + k) * PR + tx * 2 + 32 * m);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float x = k == 0 ? u[i].x : k == 1 ? u[i].y : k == 2 ? u[i].z : u[i].w;
@@ -189,7 +212,7 @@ __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(c
       for (int k = 0; k < 2 * G; ++k)
 #pragma unroll
         for (int m = 0; m < G; ++m) {
-          r[k][m] = two(R + (ty * 2 + 32 * (k / 2) + k % 2) * KD + tx * 2 + 32 * m);
+          r[k][m] = two(R + (ty * 2 + 32 * (k / 2) + k % 2) * PR + tx * 2 + 32 * m);
           mul2(r[k][m], pw[n]);
         }
 #pragma unroll 4
@@ -215,12 +238,12 @@ __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(c
       for (int k = 0; k < 2 * G; ++k)
 #pragma unroll
         for (int m = 0; m < G; ++m)
-          *reinterpret_cast<uint64_t*>(R + (ty * 2 + 32 * (k / 2) + k % 2) * KD + tx * 2 + 32 * m) = r[k][m];
+          *reinterpret_cast<uint64_t*>(R + (ty * 2 + 32 * (k / 2) + k % 2) * PR + tx * 2 + 32 * m) = r[k][m];
     }
   }
   if (to) {
     __syncthreads();
-    for (int i = threadIdx.x; i < D * D; i += 256) to[i] = R[i / D * KD + i % D];
+    for (int i = threadIdx.x; i < D * D; i += 256) to[i] = R[i / D * PR + i % D];
   }
 }
 
@@ -249,7 +272,8 @@ template <bool OUT> static int run(AttnParams& p, int64_t bh, int passes, cudaSt
   bool vec = true;
   for (int i = 0; i < passes; ++i) {
     AttnPass& a = p.pass[i];
-    vec = vec && vectors(a.y, p.D) && vectors(a.z, p.D) && (!OUT || vectors(a.x, p.D));
+    // (a state's rows of D values: D * 4 bytes are looked at with the tensors')
+    vec = vec && aligned16(a.states) && aligned16(a.from) && vectors(a.y, p.D) && vectors(a.z, p.D) && (!OUT || vectors(a.x, p.D));
     a.out_vec = OUT && vectors(a.out, p.D);
   }
   auto sized = [&](auto g) {

@@ -23,6 +23,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
+from .lm import embed
 
 
 @dataclass
@@ -131,7 +132,7 @@ def _step_block(blk, st, x, pos_dev):
 @torch.no_grad()
 def prefill(lm, ids):
     """Logits of the prompt ids [B, L] (as ``lm(ids)``) and the decode state after it."""
-    h = ops.embedding(ids, lm.embedding.weight)
+    h = embed(lm.embedding, ids)
     state = DecodeState(pos_dev=torch.zeros(1, dtype=torch.int32, device=ids.device),
                         chunk=_blocks(lm)[0].chunk_size)
     for blk in _blocks(lm):
@@ -145,7 +146,7 @@ def prefill(lm, ids):
 @torch.no_grad()
 def decode_step(lm, state, ids):
     """Logits [B, vocab] of one new token per sequence (ids [B]); advances ``state``."""
-    h = ops.embedding(ids, lm.embedding.weight)
+    h = embed(lm.embedding, ids)
     for blk, st in zip(_blocks(lm), state.layers):
         h = _step_block(blk, st, h, state.pos_dev)
     state.pos_dev.add_(1).remainder_(state.chunk)  # on the device: the step replays as a CUDA graph

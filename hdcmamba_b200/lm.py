@@ -21,6 +21,16 @@ from .model import HdcMamba9v3Block, HdcMamba9v3Model, final_layer_norm
 from .training import embedding
 
 
+def embed(module, ids):
+    """``module(ids)``: through the framework's lookup for an ``nn.Embedding`` as it comes (no renormalised
+    rows, sparse or frequency-scaled gradients, hooks), in fp32 or bf16; otherwise the module itself."""
+    w = module.weight
+    if (type(module) is nn.Embedding and module.max_norm is None and not module.scale_grad_by_freq and not module.sparse
+            and not module._forward_hooks and not module._forward_pre_hooks and w.dtype in (torch.float32, torch.bfloat16)):
+        return embedding(ids, w, padding_idx=module.padding_idx)
+    return module(ids)
+
+
 class HdcMambaLM(nn.Module):
     """Embedding -> blocks (or HdcMamba9v3Model) -> LayerNorm -> tied head."""
 
@@ -39,7 +49,7 @@ class HdcMambaLM(nn.Module):
         self.norm = nn.LayerNorm(d_model)
 
     def hidden(self, ids):
-        h = embedding(ids, self.embedding.weight)  # a fresh activation: the layers update it in place
+        h = embed(self.embedding, ids)  # a fresh activation: the layers update it in place
         if self.use_model:
             return self.backbone._forward(h, owns_input=True)
         for layer in self.layers:

@@ -813,7 +813,7 @@ def decay_attention(q, k, v, log_decay, scale=1.0, state=None, out=None, return_
     q, k, v: [B, L, H, D] views (unit stride within a head; slices of a projection, and expanded
     ones for heads that share k or v, need no copy), D from 1 to 128; L may be 0.  log_decay: [H],
     constants <= 0.  state: optional contiguous fp32 [B, H, D, D] before the first token.  out:
-    optional [B, L, H, D] view.  Returns (o, the state after the last token) and, if
+    optional [B, L, H, D] view, apart from the inputs.  Returns (o, the state after the last token) and, if
     ``return_states``, the states that ``decay_attention_bwd`` needs.  For autograd use
     ``recurrent.decay_attention``."""
     return _lib.host().decay_attention(q, k, v, log_decay, scale, state, out, return_states)
