@@ -12,10 +12,10 @@
 // those segments' sums that reach the end of the pass with more than a quarter left.  Sums for such a state are
 // also added up chunk by chunk outside the tensor cores, whose own sums of many steps lose low bits one-sidedly.
 //
-// Why not tcgen05: with heads of 64 a chunk's products are 64 x 64 x 64, each needed by the next within some
-// hundred ns; through tensor memory every one of them costs a round trip (commit, wait, load, convert, store),
-// as the slot kernels' 6 us per 256 tokens show, while here three or more CTAs per SM overlap theirs in registers.
-// 136 products of m16n8k16 per chunk and warp come to 24 us for 32768 x 12 heads of 64, whose bytes take 31 us.
+// Bound by mma.sync: one m16n8k16 takes 16 cycles of a sub-partition (512 multiply-adds per clock and SM), so the
+// 136 of a chunk and warp come to 52 us for 32768 x 12 heads of 64, and the 64 to 96 of the sums to 23 to 34; measured
+// 63 and 33, at 201 and 101 MB (31 and 15 us).  Three chunks in flight instead of two change nothing; all four
+// products with a whole square instead of its causal part cost 6 us more.
 #include <atomic>
 
 #include "decay_attn.cuh"
