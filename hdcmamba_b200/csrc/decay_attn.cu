@@ -134,13 +134,19 @@ __global__ void __launch_bounds__(256) attn_step_kernel(AttnView q, AttnView k, 
 // 1024 45 and 53; 4 heads of 128 128 tokens 19 and 25, 257 35 and 25.  fp32: 12 heads of 64 64 tokens 19 and 19, 128
 // 33 and 25; 128 heads of 64 257 tokens 72 and 78, 384 90 and 78).
 static int64_t attn_seg(int dtype, int64_t B, int64_t L, int64_t H, int64_t D) {
-  constexpr int64_t kCtas = 148 * 3;
+  const bool tc = dtype == HDC_BF16 && D > 32 && D <= 64;
+  const int64_t kCtas = 148 * (tc ? 2 : 3);
   const int64_t chunks = (L + kAttnChunk - 1) / kAttnChunk, heads = B * H;
   if (chunks < 1 || heads < 1) return kAttnChunk;
   const int64_t alone = dtype == HDC_F32 ? 1 + heads / 32 : D <= 64 ? 4 + heads / 10 : 2 + heads / 20;
   int64_t want = chunks <= alone ? 1 : kCtas / heads;
   if (want < 1) want = 1;
   if (want > chunks) want = chunks;
+  if (tc && want > 1) {
+    const int64_t pairs = (chunks + 1) / 2;
+    if (want > pairs) want = pairs;
+    return (pairs + want - 1) / want * 2 * kAttnChunk;
+  }
   return (chunks + want - 1) / want * kAttnChunk;
 }
 static int64_t attn_nseg(int dtype, int64_t B, int64_t L, int64_t H, int64_t D) {

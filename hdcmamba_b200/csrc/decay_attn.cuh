@@ -60,5 +60,8 @@ int attn_sums_f32(AttnParams& p, int64_t bh, cudaStream_t s);
 int attn_out_f32(AttnParams& p, int64_t bh, int passes, cudaStream_t s);
 int attn_sums_bf16(AttnParams& p, int64_t bh, cudaStream_t s);
 int attn_out_bf16(AttnParams& p, int64_t bh, int passes, cudaStream_t s);
+// csrc/decay_attn_tc.cu: outputs of several segments of whole 128 tokens (but for the last one's end), heads of at
+// most 64 whose rows allow 16-byte copies; false where a tensor's strides do not suit it
+bool attn_out_tc(const AttnParams& p, int64_t bh, int passes, cudaStream_t s, int* status);
 
 }  // namespace hdc

@@ -448,6 +448,10 @@ static int run(AttnParams& p, int64_t bh, int passes, cudaStream_t s) {
     if (MODE != kSums) cb = min(cb, bytes_at_once(a.x, p.D));
     a.out_vec = MODE != kSums && bytes_at_once(a.out, p.D) == 16;
   }
+  if (MODE == kOutputs && p.nseg > 1 && p.seg % 128 == 0 && cb == 16 && p.D > 32 && p.D <= 64) {
+    int status = 0;
+    if (attn_out_tc(p, bh, passes, s, &status)) return status;
+  }
   auto sized = [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     return cb == 16 ? launch<DP, MODE, 16>(p, bh, passes, s)

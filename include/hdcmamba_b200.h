@@ -460,7 +460,7 @@ int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_t dy_sn, in
  * q + b*q_sb + t*q_st + h*q_sh + d (elements; any strides, 0 for heads that share k or v), the others
  * likewise.  log_decay fp32 [H], constants (no gradient), meant to be <= 0.  States fp32 [B, H, D, D],
  * row i belonging to k's element i.  Products of bf16 tensors run on the tensor cores with fp32 sums; a
- * token's infinities and NaN may also reach the other tokens of the 64 with which it is computed.
+ * token's infinities and NaN may also reach the other tokens of the up to 128 with which it is computed.
  *   state_in, state_out : NULL or fp32 [B, H, D, D]; may be the same.
  *   states : fp32 [B, H, hdc_decay_attn_state_slots(dtype, B, L, H, D), D, D]: states between the parts that
  *            the sequence is cut into, which the gradient starts from; may be NULL where there is one slot and

@@ -102,6 +102,31 @@ def test_views(dtype, D):
     assert torch.equal(dq, dq2)
 
 
+@pytest.mark.parametrize("D", [40, 48, 56, 64])
+@pytest.mark.parametrize("L", [449, 768, 1100])
+def test_long_views(D, L):
+    """Several segments of 128-token chunks: slices of a projection, permuted tensors, shared heads, an output view."""
+    B, H = 1, 4
+    g = torch.Generator().manual_seed(L + D)
+    ld = torch.tensor([-0.002, -0.1, -0.7, -0.02]).cuda()
+    do = torch.randn(B, L, H, D, generator=g).to(BF16).cuda()
+    s, ds = (torch.randn(B, H, D, D, generator=g).cuda() for _ in range(2))
+    proj = torch.randn(B, L, 8 + 3 * H * D, generator=g).to(BF16).cuda()
+    q, k, v = (proj[..., 8 + i * H * D:8 + (i + 1) * H * D].unflatten(-1, (H, D)) for i in range(3))
+    both(q, k, v, ld, s, do, ds)
+    q, k, v = (torch.randn(B, H, L, D, generator=g).to(BF16).cuda().transpose(1, 2) for _ in range(3))
+    both(q, k, v, ld, None, do.transpose(1, 2).contiguous().transpose(1, 2), None)
+    one = torch.randn(B, L, 1, D, generator=g).to(BF16).cuda().expand(B, L, H, D)
+    o, e = ops.decay_attention(q, one, v, ld, 0.3)
+    check_forward(o, e, q, one, v, ld, 0.3, None, True)
+    buf = torch.full((B, L + 20, H, D + 16), 7.0, device="cuda", dtype=BF16)
+    for lead in (8, 4):  # 16-byte stores and single ones
+        o2, _ = ops.decay_attention(q, k, v, ld, 0.3, out=buf[:, 10:10 + L, :, lead:lead + D])
+        assert torch.equal(o2, ops.decay_attention(q, k, v, ld, 0.3)[0])
+        o2.fill_(7)
+        assert (buf == 7).all()
+
+
 def test_out_view_leaves_the_rest():
     q, k, v, ld, s, _, _ = make(BF16, 2, 70, 3, 40)
     buf = torch.full((2, 90, 3, 48), 7.0, device="cuda", dtype=BF16)
@@ -265,14 +290,15 @@ def test_offsets_past_32_bits():
 
 
 def test_non_finite_tokens_stay_in_their_sequence():
-    """Infinities and NaN of a token reach its own batch and head, from at most 63 tokens before it on."""
+    """Infinities and NaN of a token reach its own batch and head, from at most 127 tokens before it on (a chunk's
+    tokens are computed together: zeros of the causal mask times infinity)."""
     q, k, v, ld, _, _, _ = make(BF16, 2, 300, 2, 64, seed=17)
     want, _ = ops.decay_attention(q, k, v, ld)
     v[0, 200, 1, 3] = float("nan")
     k[0, 210, 1, 5] = float("inf")
     got, _ = ops.decay_attention(q, k, v, ld)
     assert torch.equal(got[1], want[1]) and torch.equal(got[0, :, 0], want[0, :, 0])
-    assert torch.equal(got[0, :137, 1], want[0, :137, 1]) and torch.isnan(got[0, 200:, 1, 3]).all()
+    assert torch.equal(got[0, :73, 1], want[0, :73, 1]) and torch.isnan(got[0, 200:, 1, 3]).all()
 
 
 def test_no_device_error():
