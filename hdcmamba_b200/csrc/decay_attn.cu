@@ -127,22 +127,30 @@ __global__ void __launch_bounds__(256) attn_step_kernel(AttnView q, AttnView k, 
 }
 
 // ---------------------------------------------------------------- plans and checks
-// Tokens of a segment, a function of the sizes alone (so that a forward and its gradient agree, and
-// results do not depend on the device's SM count): enough segments for some kCtas CTAs, or one where a single
-// launch over all chunks takes no longer than the three over segments.  Forward in us, one segment and several
-// (bf16: 16 heads of 32 128 tokens 7 and 13, 257 12 and 12, 512 17 and 13; 12 heads of 64 257 tokens 17 and 13; 128 heads of 64 257 tokens 19 and 29,
-// 1024 45 and 53; 4 heads of 128 128 tokens 19 and 25, 257 35 and 25.  fp32: 12 heads of 64 64 tokens 19 and 19, 128
-// 33 and 25; 128 heads of 64 257 tokens 72 and 78, 384 90 and 78).
+// Whether the outputs come from the tcgen05 kernel: heads of 33 to 64 in bf16, and enough tokens that its longer
+// chunks pay.  Forward in us with it and without: 12 heads 1024 tokens 18 and 17, 2048 21 and 21, 16384 56 and 56; 4 heads
+// 1024 tokens 15 and 12, 4096 17 and 20; 32 heads 768 tokens 21 and 19, 1024 21 and 23, 16384 119 and 134; 128 heads 4096
+// tokens 135 and 147.
+static bool attn_wide(int dtype, int64_t heads, int64_t chunks, int64_t D) {
+  return dtype == HDC_BF16 && D > 32 && D <= 64 && (chunks >= 32 || heads * chunks >= 512);
+}
+
+// Tokens of a segment, a function of the sizes alone (so that a forward and its gradient agree, and results do not
+// depend on the device's SM count): enough segments for the CTAs that 148 SMs hold, or one where a single launch
+// over all chunks takes no longer than the three over segments.  Forward in us, one segment and several (bf16:
+// 16 heads of 32 128 tokens 7 and 13, 257 12 and 12, 512 17 and 13; 128 heads of 64 257 tokens 19 and 29, 1024 45 and 53;
+// 4 heads of 128 128 tokens 19 and 25, 257 35 and 25.  fp32: 12 heads of 64 64 tokens 19 and 19, 128 33 and 25; 128
+// heads of 64 257 tokens 72 and 78, 384 90 and 78).
 static int64_t attn_seg(int dtype, int64_t B, int64_t L, int64_t H, int64_t D) {
-  const bool tc = dtype == HDC_BF16 && D > 32 && D <= 64;
-  const int64_t kCtas = 148 * (tc ? 2 : 3);
   const int64_t chunks = (L + kAttnChunk - 1) / kAttnChunk, heads = B * H;
   if (chunks < 1 || heads < 1) return kAttnChunk;
+  const bool wide = attn_wide(dtype, heads, chunks, D);
+  const int64_t ctas = 148 * (wide ? 2 : 3);
   const int64_t alone = dtype == HDC_F32 ? 1 + heads / 32 : D <= 64 ? 4 + heads / 10 : 2 + heads / 20;
-  int64_t want = chunks <= alone ? 1 : kCtas / heads;
+  int64_t want = chunks <= alone ? 1 : ctas / heads;
   if (want < 1) want = 1;
   if (want > chunks) want = chunks;
-  if (tc && want > 1) {
+  if (wide && want > 1) {  // whole 128 tokens
     const int64_t pairs = (chunks + 1) / 2;
     if (want > pairs) want = pairs;
     return (pairs + want - 1) / want * 2 * kAttnChunk;
@@ -222,6 +230,7 @@ extern "C" int64_t hdc_decay_attn_state_slots(int dtype, int64_t B, int64_t L, i
 static void plan(AttnParams& p, int dtype, const float* log_decay, int64_t B, int64_t L, int64_t H, int64_t D) {
   p.g = log_decay; p.H = (int)H; p.L = (int)L; p.D = (int)D;
   p.seg = (int)attn_seg(dtype, B, L, H, D); p.nseg = (int)attn_nseg(dtype, B, L, H, D);
+  p.wide = p.nseg > 1 && attn_wide(dtype, B * H, (L + kAttnChunk - 1) / kAttnChunk, D);
 }
 
 extern "C" int hdc_decay_attn_fwd(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,

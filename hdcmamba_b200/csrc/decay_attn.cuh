@@ -44,6 +44,7 @@ struct AttnParams {
   AttnPass pass[3];
   const float* g;
   int H, L, D, nseg, seg;  // seg: tokens of a segment, whole chunks
+  int wide;                // segments of whole 128 tokens, outputs by the tcgen05 kernel where strides allow it
 };
 
 // exp(g d), 1 for d = 0 whatever g is

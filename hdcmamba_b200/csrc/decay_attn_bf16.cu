@@ -9,8 +9,9 @@
 // Roundings.  P and the copy of R are rounded to bf16 once, as the result is; sums and states stay fp32.  The
 // weighted tokens up(j) y_j would add a third rounding to every state: they are split into two bf16 parts (2^-17), and
 // into three (2^-25) where the fp32 state that the caller gets is made of them: in a sequence of one segment, and in
-// those segments' sums that reach the end of the pass with more than a quarter left.  Sums for such a state are
-// also added up chunk by chunk outside the tensor cores, whose own sums of many steps lose low bits one-sidedly.
+// those segments' sums of which more than 2^-8 is left at the end of the pass (the others' 2^-17 is 2^-25 there; a
+// quarter was too much, where the few tokens behind it happened to be small).  Sums for such a state are also added up
+// chunk by chunk outside the tensor cores, whose own sums of many steps lose low bits one-sidedly.
 //
 // Bound by mma.sync: one m16n8k16 takes 16 cycles of a sub-partition (512 multiply-adds per clock and SM), so the
 // 136 of a chunk and warp come to 52 us for 32768 x 12 heads of 64, and the 64 to 96 of the sums to 23 to 34; measured
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(M
   const bool fine = p.L <= kAttnChunk;
 
   // whether the weighted tokens' third part counts
-  const bool third = EXACT && a.to && (OUT || decay_pow(gd, back ? begin : p.L - end) > 0.25f);
+  const bool third = EXACT && a.to && (OUT || decay_pow(gd, back ? begin : p.L - end) > 0x1p-8f);
 
   // a lane's address of four 8 x 8 blocks: rows first (la), or columns first (lb)
   const uint32_t la = (lane % 8 + 8 * ((lane / 8) % 2)) * PT + lane / 16 * 16;
@@ -448,7 +449,7 @@ static int run(AttnParams& p, int64_t bh, int passes, cudaStream_t s) {
     if (MODE != kSums) cb = min(cb, bytes_at_once(a.x, p.D));
     a.out_vec = MODE != kSums && bytes_at_once(a.out, p.D) == 16;
   }
-  if (MODE == kOutputs && p.nseg > 1 && p.seg % 128 == 0 && cb == 16 && p.D > 32 && p.D <= 64) {
+  if (MODE == kOutputs && p.wide && cb == 16) {
     int status = 0;
     if (attn_out_tc(p, bh, passes, s, &status)) return status;
   }

@@ -47,7 +47,7 @@ def test_head_sizes(dtype, D):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("B,L,H,D", [(1, 1000, 1, 64), (1, 2049, 2, 32), (3, 700, 5, 24), (1, 640, 3, 128), (30, 200, 16, 16),
+@pytest.mark.parametrize("B,L,H,D", [(1, 1000, 1, 64), (1, 2049, 2, 32), (3, 700, 5, 24), (1, 640, 3, 128), (30, 200, 16, 16), (2, 1025, 20, 64), (1, 4000, 9, 40),
                                      (1, 1, 1, 1), (500, 3, 1, 8)])
 def test_segments(dtype, B, L, H, D):
     """Sequences cut into several segments, the last one short, and more heads than CTAs."""
@@ -57,9 +57,10 @@ def test_segments(dtype, B, L, H, D):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("decay", [0.0, -1e-4, -3.0, -40.0, -200.0, float("-inf")])
 def test_decays(dtype, decay):
-    """Heads that forget nothing, and heads that remember nothing."""
-    q, k, v, ld, s, do, ds = make(dtype, 2, 200, 2, 64, state=True, seed=5, decay=decay)
-    both(q, k, v, ld, s, do, ds)
+    """Heads that forget nothing, and heads that remember nothing; one segment and several, of both chunk lengths."""
+    for L in (200, 500, 2060) if dtype == BF16 else (200,):
+        q, k, v, ld, s, do, ds = make(dtype, 1, L, 2, 64, state=True, seed=5, decay=decay)
+        both(q, k, v, ld, s, do, ds)
 
 
 def test_each_head_has_its_own_decay():
@@ -103,12 +104,12 @@ def test_views(dtype, D):
 
 
 @pytest.mark.parametrize("D", [40, 48, 56, 64])
-@pytest.mark.parametrize("L", [449, 768, 1100])
+@pytest.mark.parametrize("L", [449, 1100, 2050, 2176])
 def test_long_views(D, L):
-    """Several segments of 128-token chunks: slices of a projection, permuted tensors, shared heads, an output view."""
-    B, H = 1, 4
+    """Several segments, from 2048 tokens on of 128-token chunks: slices of a projection, permuted tensors, shared heads, an output view."""
+    B, H = (1, 4) if L < 2000 else (2, 2)
     g = torch.Generator().manual_seed(L + D)
-    ld = torch.tensor([-0.002, -0.1, -0.7, -0.02]).cuda()
+    ld = torch.tensor([-0.002, -0.7, -0.1, -0.02][:H]).cuda()
     do = torch.randn(B, L, H, D, generator=g).to(BF16).cuda()
     s, ds = (torch.randn(B, H, D, D, generator=g).cuda() for _ in range(2))
     proj = torch.randn(B, L, 8 + 3 * H * D, generator=g).to(BF16).cuda()
@@ -238,8 +239,9 @@ def test_empty():
         assert ops.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s)[0].shape == (0, 3, 16)
 
 
-def test_same_bits_again_on_another_stream_and_from_two_graphs():
-    q, k, v, ld, s, do, ds = make(BF16, 2, 900, 4, 64, state=True, seed=13)
+@pytest.mark.parametrize("L", [130, 900, 2100])
+def test_same_bits_again_on_another_stream_and_from_two_graphs(L):
+    q, k, v, ld, s, do, ds = make(BF16, 2, L, 4, 64, state=True, seed=13)
     leaves = [x.detach().requires_grad_() for x in (q, k, v)]
 
     def run():
@@ -289,16 +291,26 @@ def test_offsets_past_32_bits():
     assert torch.equal(want, x)
 
 
-def test_non_finite_tokens_stay_in_their_sequence():
+@pytest.mark.parametrize("L", [300, 2100])
+def test_non_finite_tokens_stay_in_their_sequence(L):
     """Infinities and NaN of a token reach its own batch and head, from at most 127 tokens before it on (a chunk's
     tokens are computed together: zeros of the causal mask times infinity)."""
-    q, k, v, ld, _, _, _ = make(BF16, 2, 300, 2, 64, seed=17)
+    q, k, v, ld, _, _, _ = make(BF16, 2, L, 2, 64, seed=17)
     want, _ = ops.decay_attention(q, k, v, ld)
     v[0, 200, 1, 3] = float("nan")
     k[0, 210, 1, 5] = float("inf")
     got, _ = ops.decay_attention(q, k, v, ld)
     assert torch.equal(got[1], want[1]) and torch.equal(got[0, :, 0], want[0, :, 0])
     assert torch.equal(got[0, :73, 1], want[0, :73, 1]) and torch.isnan(got[0, 200:, 1, 3]).all()
+
+
+def test_the_same_tensors_again_after_a_view_that_tma_does_not_take():
+    """Strides past what a tensor map holds and heads that share memory go another way, with the same roundings."""
+    q, k, v, ld, _, _, _ = make(BF16, 1, 2100, 2, 64, seed=19)
+    one = k[:, :, :1]
+    a, ea = ops.decay_attention(q, one.expand(-1, -1, 2, -1), v, ld, 0.3)
+    b, eb = ops.decay_attention(q, one.repeat(1, 1, 2, 1), v, ld, 0.3)
+    assert (a.float() - b.float()).norm() <= 2 * 2 ** -8 * b.float().norm() and torch.equal(ea, eb)
 
 
 def test_no_device_error():
