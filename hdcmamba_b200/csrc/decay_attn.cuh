@@ -7,7 +7,7 @@
 //   out_t = x_t' M_t,   M a decayed sum of y_t z_t' forwards or backwards in time:
 //   o (x, y, z) = (q, k, v);  dq = (do, v, k), M = S';  dv backwards = (k, q, do), M = G;  dk backwards = (v, do, q), M = G'.
 //
-// Time is cut into chunks of 64 tokens and those into segments.  With R the state that enters a chunk
+// Time is cut into chunks of 64 tokens (128 in decay_attn_tc.cu) and segments of whole chunks.  With R the state that enters a chunk
 // of n tokens (i, j local indices),
 //   out_i = si in(i) x_i' R + sum_j sa e^|i-j| (x_i' y_j) z_j   over j <= i (backwards j >= i),
 //   R <- e^n R + sum_j su up(j) y_j z_j',

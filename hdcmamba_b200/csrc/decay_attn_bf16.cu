@@ -15,7 +15,7 @@
 //
 // Bound by mma.sync: one m16n8k16 takes 16 cycles of a sub-partition (512 multiply-adds per clock and SM), so the
 // 136 of a chunk and warp come to 52 us for 32768 x 12 heads of 64, and the 64 to 96 of the sums to 23 to 34; measured
-// 63 and 33, at 201 and 101 MB (31 and 15 us).  Three chunks in flight instead of two change nothing; all four
+// 63 and 33, at 201 and 101 MB (31 and 15 us).  (Outputs of many tokens with heads of 33 to 64: decay_attn_tc.cu.)  Three chunks in flight instead of two change nothing; all four
 // products with a whole square instead of its causal part cost 6 us more.
 #include <atomic>
 

@@ -9,7 +9,9 @@
 //   o = in(i) O1 + O2,  R <- e^n R + U hi + U lo         the state stays in the registers of half the threads
 // and the next chunk's X and Y are loaded once S is done, Z once O2 and U are.  Roundings as in
 // decay_attn_bf16.cu, whose m16n8k16 products (512 multiply-adds per clock and SM) bound the same work at 52 us for
-// 32768 x 12 heads of 64.
+// 32768 x 12 heads of 64.  Measured there 62 us (63), and 215 us (247) for the three passes of the gradient at 8 x 4096 x
+// 16 heads; bytes 31 and 72 us.  Bound by a chunk's chain of dependent steps, 10 500 cycles with two CTAs on an SM (the
+// tensor pipe is busy 17%): weighting Y 1200, P 1800, O2's eight products 1200, the rest read-outs, barriers and loads.
 //
 // Tensor memory, 256 columns: S in [0, 128); P, packed, over the first half of each thread pair's own 64 columns
 // (piece k of 16 tokens comes to columns that pieces up to k have left); O1 and then O2 in [128, 192); U in [192, 256).

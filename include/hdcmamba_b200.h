@@ -471,7 +471,8 @@ int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_t dy_sn, in
  * hdc_decay_attn_step: one token per sequence, q [B, H, D] (strides q_sb, q_sh); state_out may be state.
  * D in [1, 128], B, L in [0, 2^30], H in [1, 2^20], B * H * slots < 2^31.  Rows of o, dq, dk and dv must
  * not overlap, nor the outputs the inputs.  Pointers need their type's alignment; 16-byte aligned heads
- * take the wide loads.  Results do not depend on timing.
+ * take the wide loads.  Results do not depend on timing.  Waits for a kernel's own loads and products are
+ * bounded: 81 through hdc_device_error() if one runs out (never expected).
  */
 int64_t hdc_decay_attn_state_slots(int dtype, int64_t B, int64_t L, int64_t H, int64_t D);
 int hdc_decay_attn_fwd(int dtype, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,

@@ -129,3 +129,71 @@ def test_the_lm_looks_its_rows_up():
     assert torch.equal(seen[0], lm.embedding.weight[ids])
     lm(ids).float().sum().backward()
     assert lm.embedding.weight.grad.isfinite().all()
+
+
+def test_two_threads_at_once():
+    """Calls from two host threads on streams of their own."""
+    import threading
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(2, 300, 2, 64, generator=g).cuda().bfloat16()
+    ld = torch.tensor([-0.02, -0.3]).cuda()
+    ids = torch.randint(0, V, (5000,), generator=g).cuda()
+    dy = torch.randn(5000, 64, generator=g).cuda()
+    xs = [torch.randn(9999, generator=g).cuda() for _ in range(3)]
+    torch.cuda.synchronize()
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                leaf = q.clone().requires_grad_()
+                o, e = recurrent.decay_attention(leaf, q, q, ld)
+                r = [o.detach(), e.detach(), *torch.autograd.grad(o, [leaf], q), ops.embedding_bwd(dy, ids, V), ops.clip_grads(xs, None)]
+        s.synchronize()
+        return r
+
+    want, got = work(), [None, None]
+
+    def run(i):
+        got[i] = work()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for r in got:
+        assert r is not None and all(torch.equal(a, b) for a, b in zip(want, r))
+
+
+def test_refusals_of_the_library_raise():
+    from hdcmamba_b200 import _lib
+    x = torch.ones(100, device="cuda")
+    for grads, out in (([x, x], None), ([x[:60], x[50:]], None), ([x[:50], x[50:]], [x[50:], x[:50]])):
+        with pytest.raises(_lib.HdcError, match="overlaps"):
+            ops.clip_grads(grads, 1.0, out=out)
+    with pytest.raises(_lib.HdcError, match="max_norm"):
+        ops.clip_grads([x], -1.0)
+    q = torch.zeros(1, 4, 2, 8, device="cuda")
+    with pytest.raises(_lib.HdcError, match="overlap"):
+        ops.decay_attention(q, q, q, torch.zeros(2, device="cuda"), out=q[:, :1].expand(1, 4, 2, 8))
+    with pytest.raises(RuntimeError, match="CPU"):
+        ops.decay_attention(q, q.cpu(), q, torch.zeros(2, device="cuda"))
+    with pytest.raises(RuntimeError, match="CPU"):
+        ops.embedding(torch.zeros(3, dtype=torch.int64), q[0, 0])
+    assert (x == 1).all()
+
+
+def test_a_sequence_of_a_quarter_million_tokens():
+    """Against two halves of it, joined by the state: the same bounds as for the definition (two roundings to bf16)."""
+    g = torch.Generator().manual_seed(5)
+    L = 262144 + 37
+    q, k, v = (torch.randn(1, L, 1, 64, generator=g).cuda().bfloat16() for _ in range(3))
+    ld = torch.tensor([-0.0005]).cuda()
+    o, e = ops.decay_attention(q, k, v, ld, 0.1)
+    cut = 100001
+    a, m = ops.decay_attention(q[:, :cut], k[:, :cut], v[:, :cut], ld, 0.1)
+    b, n = ops.decay_attention(q[:, cut:], k[:, cut:], v[:, cut:], ld, 0.1, m)
+    both = torch.cat([a, b], 1).float()
+    assert (o.float() - both).norm() <= 2 * 2 * 2 ** -8 * both.norm()
+    assert (e - n).norm() <= 2 * 64 * 2.0 ** -24 * n.norm()
