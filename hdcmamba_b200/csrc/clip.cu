@@ -93,7 +93,6 @@ struct Place {
   }
 };
 
-// A piece's values in registers; zeros where there are none.
 // 16 bytes that L2 keeps or lets go, by the policy
 __device__ __forceinline__ uint4 ldg16_hint(const void* p, uint64_t policy) {
   uint4 r;
@@ -101,6 +100,7 @@ __device__ __forceinline__ uint4 ldg16_hint(const void* p, uint64_t policy) {
                : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p), "l"(policy));
   return r;
 }
+// A piece's values in registers; zeros where there are none.
 struct Held {
   uint4 w[kVecs];
   float one;
