@@ -132,16 +132,13 @@ __global__ void __launch_bounds__(kTcThreads, 2) attn_tc_kernel(const __grid_con
   }
   keep_copy();
 
-  for (int q = 0; q < chunks; ++q) {
+  int q = 0;
+  for (; q < chunks; ++q) {
     const int t0 = chunk_at(q), n = min(kTcTokens, end - t0), shift = kTcTokens - n;
     const bool last = q + 1 == chunks;
     const uint32_t ph = q & 1;
     __syncthreads();
-    if (s_late) {  // a wait has run out: no load is left on its way when the CTA ends
-      mbar_wait_warp(&bars[3], ph, kTcCode);
-      mbar_wait_warp(&bars[4], ph, kTcCode);
-      break;
-    }
+    if (s_late) break;
     if (!mbar_wait_warp(&bars[3], ph, kTcCode)) s_late = 1;
     if (issues) {
       tc_fence_after();
@@ -296,6 +293,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) attn_tc_kernel(const __grid_con
         if (r < n && c < D) to[r * a.out.st + c] = *reinterpret_cast<const __nv_bfloat16*>(tiles + 3 * kTcTile + sw128_off(r, c));
       }
     }
+  }
+  __syncthreads();
+  if (s_late) {  // a wait has run out: no load is left on its way when the CTA ends
+    const uint32_t ph = min(q, chunks - 1) & 1;
+    mbar_wait_warp(&bars[3], ph, kTcCode);
+    mbar_wait_warp(&bars[4], ph, kTcCode);
   }
   __syncthreads();
   if (warp == 0) tmem_dealloc(tmem, 256);
