@@ -384,6 +384,8 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(M
         for (int e = 0; e < 2; ++e)
           *reinterpret_cast<uint32_t*>(Xs + (g + 8 * e) * PT + n * 16 + c * 4) = pack2(O[n][2 * e], O[n][2 * e + 1]);
       __syncwarp();
+      // X's columns from D on become zeros again: an output there is infinity times zero where a token is not finite,
+      // and would meet every token of the chunk that takes these tiles next
       if (a.out_vec) {
         const int col = lane % ON * 8;
         if (oc + col < D) {
@@ -393,12 +395,15 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(M
             if (16 * r + row < n_rows)
               stg16(out + (16 * r + row) * a.out.st + oc + col, *reinterpret_cast<const uint4*>(Xs + row * PT + col * 2));
           }
+        } else {
+          for (int row = lane / ON; row < 16; row += 32 / ON) *reinterpret_cast<uint4*>(Xs + row * PT + col * 2) = make_uint4(0, 0, 0, 0);
         }
       } else {
         for (int i = lane; i < 16 * 8 * ON; i += 32) {
           const int row = i / (8 * ON), col = i % (8 * ON);
-          if (16 * r + row < n_rows && oc + col < D)
-            out[(16 * r + row) * a.out.st + oc + col] = *reinterpret_cast<const bf16*>(Xs + row * PT + col * 2);
+          bf16* at = reinterpret_cast<bf16*>(Xs + row * PT + col * 2);
+          if (oc + col >= D) *at = __float2bfloat16(0.f);
+          else if (16 * r + row < n_rows) out[(16 * r + row) * a.out.st + oc + col] = *at;
         }
       }
     }
