@@ -361,8 +361,10 @@ PyObject* py_embedding_train(PyObject* const* a) {
   return wrap(Embedding::apply(tensor(a[1]), tensor(a[0]), number(a[2]), a[3] == Py_None ? (int64_t)-1 : whole(a[3])));
 }
 
-// a sequence's tensors: contiguous, of one device; their addresses, types and sizes
+// a sequence's tensors: contiguous, of one device; their addresses, types and sizes.  It holds the tensors: a
+// generator's would otherwise be gone before the kernels are launched, and their memory another tensor's.
 struct List {
+  std::vector<Tensor> tensors;
   std::vector<void*> at;
   std::vector<int> codes;
   std::vector<int64_t> sizes;
@@ -372,6 +374,7 @@ struct List {
     if (!s) throw python_error();
     const std::unique_ptr<PyObject, void (*)(PyObject*)> hold(s, [](PyObject* o) { Py_DECREF(o); });
     const Py_ssize_t n = PySequence_Fast_GET_SIZE(s);
+    tensors.reserve(n);
     at.reserve(n);
     codes.reserve(n);
     sizes.reserve(n);
@@ -381,6 +384,7 @@ struct List {
       TORCH_CHECK_VALUE(t.device() == first.device(), "tensors must be on one device (", first.device(), ", got ", t.device(), ")");
       TORCH_CHECK_VALUE(t.layout() == at::kStrided && t.is_contiguous(), "clip_grads needs contiguous tensors");
       codes.push_back(code_of(t));
+      tensors.push_back(t);
       at.push_back(t.data_ptr());
       sizes.push_back(t.numel());
     }
