@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(mc::NT, 1)
     uint8_t* sK = base + st * 2 * TILE;
     uint8_t* sV = sK + TILE;
     if (PERSTEP && warp < G && g + 1 < ngroups) chunk_cumlog_load<CT>(mc_log_a(p, b, h, n0, g + 1, warp), p.H, la_next);
-    if (!mbar_wait_warp(&bars[st], (fph >> st) & 1u, 71)) { ok = false; break; }
+    if (!mbar_wait_warp(&bars[st], (fph >> st) & 1u, 70)) { ok = false; break; }
     fph ^= 1u << st;
     if (tid == 0) pending &= ~(1 << st);
     // k~ = bf16(bf16(phi(k)) kdec_j) in place, four 16-byte pieces per thread

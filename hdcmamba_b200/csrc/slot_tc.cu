@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(spipe::NT, 1)
       constexpr uint32_t idU = idesc_bf16_f32(64, 64, true, true);
       for (int n = n0; n < n1; ++n) {
         const int i = n - n0, st = i % NS, ub = i & 1;
-        if (!mbar_wait(&bars[B_PREP + st], (uint32_t)((i / NS) & 1), 71)) break;
+        if (!mbar_wait(&bars[B_PREP + st], (uint32_t)((i / NS) & 1), 70)) break;
         if (i >= 2 && !mbar_wait(&bars[B_UFREE + ub], (uint32_t)(((i >> 1) - 1) & 1), 72)) break;
         tc_fence_after();
         const uint64_t dK = sdesc_sw128(smem_u32(sK(st)), 0, 1024), dV = sdesc_sw128(smem_u32(sV(st)), 0, 1024);
