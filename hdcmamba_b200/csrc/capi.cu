@@ -46,13 +46,21 @@ void register_dev_error_reader(int (*reader)(int reset)) {
 
 }  // namespace hdc
 
+// Each translation unit has a word of its own.  A wait that ran out (a call's outputs are invalid) comes before an
+// id outside a table (one row is NaN), which then stays for the next call.
 extern "C" int hdc_device_error(int reset) {
-  int first = 0;
+  constexpr int kBadId = 71;  // embedding.cu, whose word holds nothing else
+  int first = 0, id = 0;
   for (int i = 0; i < hdc::g_n_err_readers; ++i) {
-    const int v = hdc::g_err_readers[i](reset);
-    if (v != 0 && first == 0) first = v;
+    const int v = hdc::g_err_readers[i](0);
+    if (v == kBadId) id = v;
+    else if (v != 0 && first == 0) first = v;
+    if (reset && v != 0 && v != kBadId) hdc::g_err_readers[i](1);
   }
-  return first;
+  if (first != 0 || id == 0) return first;
+  if (reset)
+    for (int i = 0; i < hdc::g_n_err_readers; ++i) hdc::g_err_readers[i](1);
+  return id;
 }
 
 extern "C" int hdc_version(void) { return 100; }

@@ -50,15 +50,19 @@ def _same_dtype(ref, *ts):
 def check_device():
     """Synchronise the current device and raise HdcError if a bounded wait inside a kernel has run
     out since the last check (the error is cleared): the outputs of the call that waited are
-    invalid.  An ``embedding`` that met an id outside its table is reported likewise.  Kernels
-    report both on the device only, so a training loop calls this once in a while (say with each
-    checkpoint)."""
+    invalid.  An ``embedding`` that met an id outside its table is reported likewise (where both
+    have happened, by the check after the one that reports the wait).  Kernels report both on the
+    device only, so a training loop calls this once in a while (say with each checkpoint)."""
     torch.cuda.synchronize()
     code = _lib.load().hdc_device_error(1)
-    if code == 71:
-        raise _lib.HdcError("an embedding met an id outside its table (code 71): its row is NaN and takes no part in the gradient")
     if code != 0:
-        raise _lib.HdcError(f"a bounded wait inside a kernel has run out (code {code}); the outputs of that call are invalid")
+        raise _lib.HdcError(_device_error_text(code))
+
+
+def _device_error_text(code):
+    if code == 71:
+        return "an embedding met an id outside its table (code 71): its row is NaN and takes no part in the gradient"
+    return f"a bounded wait inside a kernel has run out (code {code}); the outputs of that call are invalid"
 
 
 # ------------------------------------------------------------------ LN + conv

@@ -128,8 +128,11 @@ class SequenceParallel:
         if not isinstance(self.k, CudaKernels):
             return
         from . import _lib
+        from .ops import _device_error_text
         torch.cuda.synchronize()
         code = _lib.load().hdc_device_error(1)
+        if code == 71:
+            raise _lib.HdcError(f"rank {self.rank}: {_device_error_text(code)}")
         if code != 0:
             raise _lib.HdcError(f"rank {self.rank}: a bounded device wait timed out (code {code}); "
                                 "the sequence-parallel forward's output is invalid")

@@ -294,9 +294,10 @@ int hdc_slot_scan_fwd_path(int dtype, const void* q, const void* k, const void* 
                            hdc_stream_t stream);
 
 /*
- * Device-side error word of the tcgen05 kernels: 0, or the code of a bounded wait
- * (mbarrier) that timed out after ~2 s.  Synchronous; reset != 0 clears it.
- * Returns -1 if the word could not be read.
+ * Device-side error word: 0, or the code of a bounded wait (mbarrier, flag) inside a kernel that ran
+ * out after ~2 s, or 71 for an embedding's id outside its table.  Synchronous; reset != 0 clears it.
+ * A wait's code comes before 71, which then stays for the next call.  Returns -1 if the word could
+ * not be read.
  */
 int hdc_device_error(int reset);
 
