@@ -24,11 +24,15 @@ from .training import embedding
 def embed(module, ids):
     """``module(ids)``: through the framework's lookup for an ``nn.Embedding`` as it comes (no renormalised
     rows, sparse or frequency-scaled gradients, hooks), in fp32 or bf16; otherwise the module itself."""
-    w = module.weight
-    if (type(module) is nn.Embedding and module.max_norm is None and not module.scale_grad_by_freq and not module.sparse
-            and not module._forward_hooks and not module._forward_pre_hooks and w.dtype in (torch.float32, torch.bfloat16)):
-        return embedding(ids, w, padding_idx=module.padding_idx)
+    if type(module) is nn.Embedding and _is_plain(module):
+        return embedding(ids, module.weight, padding_idx=module.padding_idx)
     return module(ids)
+
+
+def _is_plain(module):
+    return (module.max_norm is None and not module.scale_grad_by_freq and not module.sparse
+            and not module._forward_hooks and not module._forward_pre_hooks
+            and module.weight.dtype in (torch.float32, torch.bfloat16))
 
 
 class HdcMambaLM(nn.Module):

@@ -3,7 +3,6 @@ import pytest
 import torch
 import torch.nn as nn
 
-from hdcmamba_b200 import ops
 from hdcmamba_b200.lm import embed
 
 pytestmark = pytest.mark.gpu
