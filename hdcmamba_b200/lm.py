@@ -21,18 +21,29 @@ from .model import HdcMamba9v3Block, HdcMamba9v3Model, final_layer_norm
 from .training import embedding
 
 
+_forward = nn.Embedding.forward
+
+
 def embed(module, ids):
     """``module(ids)``: through the framework's lookup for an ``nn.Embedding`` as it comes (no renormalised
-    rows, sparse or frequency-scaled gradients, hooks), in fp32 or bf16; otherwise the module itself."""
-    if type(module) is nn.Embedding and _is_plain(module):
+    rows, sparse or frequency-scaled gradients, and nothing that would see or change the module's call), in
+    fp32 or bf16; otherwise the module itself."""
+    if type(module) is nn.Embedding and _is_plain(module) and not _is_watched(module):
         return embedding(ids, module.weight, padding_idx=module.padding_idx)
     return module(ids)
 
 
 def _is_plain(module):
     return (module.max_norm is None and not module.scale_grad_by_freq and not module.sparse
-            and not module._forward_hooks and not module._forward_pre_hooks
             and module.weight.dtype in (torch.float32, torch.bfloat16))
+
+
+def _is_watched(module):
+    """Hooks of the module or of all modules, a forward that is not the class's own (offloading, adapters,
+    ``module.compile()``), modes that see every operation."""
+    return (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+            or nn.modules.module._has_any_global_hook() or "forward" in module.__dict__ or nn.Embedding.forward is not _forward
+            or module._compiled_call_impl is not None or torch._C._len_torch_function_stack() or torch._C._len_torch_dispatch_stack())
 
 
 class HdcMambaLM(nn.Module):

@@ -30,3 +30,56 @@ def test_modules_of_other_kinds():
     assert torch.equal(embed(m, ids), m(ids))
     f = table().weight.detach()
     assert torch.equal(embed(lambda i: f[i], ids), f[ids])
+
+
+def test_hooks_of_every_kind_are_called():
+    """Forward and backward hooks of the module, and those that are registered for all modules."""
+    ids = torch.tensor(IDS).cuda()
+    for name in ("register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook", "register_full_backward_pre_hook"):
+        for owner in ("module", "all"):
+            m, called = table(), []
+            if owner == "module":
+                handle = getattr(m, name)(lambda *a: called.append(1))
+            else:
+                name_all = name.replace("register_", "register_module_")
+                if not hasattr(nn.modules.module, name_all):
+                    continue
+                handle = getattr(nn.modules.module, name_all)(lambda *a: called.append(1))
+            embed(m, ids).sum().backward()
+            handle.remove()
+            assert called, (name, owner)
+
+
+def test_a_forward_of_the_instance_or_of_the_class():
+    ids = torch.tensor(IDS).cuda()
+    m = table()
+    m.forward = lambda i: nn.functional.embedding(i, m.weight) + 1
+    assert torch.equal(embed(m, ids), m.weight[ids] + 1)
+    m, was = table(), nn.Embedding.forward
+    try:
+        nn.Embedding.forward = lambda self, i: was(self, i) + 2
+        assert torch.equal(embed(m, ids), m.weight[ids] + 2)
+    finally:
+        nn.Embedding.forward = was
+
+
+def test_modes_see_the_lookup():
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+    ids, m, seen = torch.tensor(IDS).cuda(), table(), []
+
+    class Functions(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            seen.append(getattr(func, "__name__", ""))
+            return func(*args, **(kwargs or {}))
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    for mode in (Functions, Dispatch):
+        seen.clear()
+        with mode():
+            y = embed(m, ids)
+        assert torch.equal(y, m.weight[ids]) and any("embedding" in s for s in seen), (mode, seen)
