@@ -209,6 +209,14 @@ void is_table(const Tensor& t, const char* what) {
   TORCH_CHECK_VALUE(t.size(1) == 1 || t.stride(1) == 1, what, " needs a unit column stride");
 }
 
+// whether `lookup` takes these: what nn.Embedding allows beyond is left to it
+bool takes(const Tensor& ids, const Tensor& w) {
+  return (w.scalar_type() == at::kFloat || w.scalar_type() == at::kBFloat16) && w.is_cuda() && w.dim() == 2 && w.stride(1) == 1 &&
+         w.size(0) >= 1 && w.size(0) <= (int64_t(1) << 30) && w.size(1) >= 1 && w.size(1) <= 65536 &&
+         (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) && ids.device() == w.device() &&
+         ids.numel() <= (int64_t(1) << 30);
+}
+
 Tensor lookup(const Tensor& ids, const Tensor& weight, double scale, const Maybe& out) {
   const int code = code_of(weight), bytes = id_bytes(ids);
   is_table(weight, "weight");
@@ -354,6 +362,7 @@ PyObject* py_attn_step(PyObject* const* p) {
   return tuple(o, next);
 }
 PyObject* py_embedding(PyObject* const* a) { return wrap(lookup(tensor(a[0]), tensor(a[1]), number(a[2]), maybe(a[3]))); }
+PyObject* py_embedding_takes(PyObject* const* a) { return PyBool_FromLong(takes(tensor(a[0]), tensor(a[1]))); }
 PyObject* py_embedding_bwd(PyObject* const* a) {
   return wrap(lookup_backward(tensor(a[0]), tensor(a[1]), whole(a[2]), number(a[3]), a[4] == Py_None ? -1 : whole(a[4]), maybe(a[5])));
 }
@@ -427,6 +436,7 @@ PyMethodDef g_methods[] = {
     method<6, py_attn_train>("decay_attention_train"),
     method<8, py_attn_step>("decay_attention_step"),
     method<4, py_embedding>("embedding"),
+    method<2, py_embedding_takes>("embedding_takes"),
     method<6, py_embedding_bwd>("embedding_bwd"),
     method<4, py_embedding_train>("embedding_train"),
     method<3, py_clip>("clip_grads"),

@@ -17,6 +17,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import _lib
 from .model import HdcMamba9v3Block, HdcMamba9v3Model, final_layer_norm
 from .training import embedding
 
@@ -28,14 +29,15 @@ def embed(module, ids):
     """``module(ids)``: through the framework's lookup for an ``nn.Embedding`` as it comes (no renormalised
     rows, sparse or frequency-scaled gradients, and nothing that would see or change the module's call), in
     fp32 or bf16; otherwise the module itself."""
-    if type(module) is nn.Embedding and _is_plain(module) and not _is_watched(module):
+    if type(module) is nn.Embedding and _is_plain(module, ids) and not _is_watched(module):
         return embedding(ids, module.weight, padding_idx=module.padding_idx)
     return module(ids)
 
 
-def _is_plain(module):
+def _is_plain(module, ids):
+    """The module does what the lookup does, with a table and ids that the lookup takes."""
     return (module.max_norm is None and not module.scale_grad_by_freq and not module.sparse
-            and module.weight.dtype in (torch.float32, torch.bfloat16))
+            and _lib.host().embedding_takes(ids, module.weight))
 
 
 def _is_watched(module):

@@ -83,3 +83,20 @@ def test_modes_see_the_lookup():
         with mode():
             y = embed(m, ids)
         assert torch.equal(y, m.weight[ids]) and any("embedding" in s for s in seen), (mode, seen)
+
+
+def test_tables_that_the_kernel_does_not_take():
+    """Rows whose elements lie apart, rows wider than the kernel's, host tables."""
+    ids = torch.tensor(IDS).cuda()
+    m = table()
+    m.weight = nn.Parameter(m.weight.detach().t().contiguous().t())
+    assert torch.equal(embed(m, ids), m.weight[ids])
+    embed(m, ids).sum().backward()
+    want = torch.zeros(20, 16, device="cuda").index_add_(0, ids.flatten(), torch.ones(6, 16, device="cuda"))
+    assert torch.equal(m.weight.grad, want)
+    m = nn.Embedding(3, 65537, device="cuda", dtype=torch.bfloat16)
+    assert torch.equal(embed(m, ids % 3), m.weight[ids % 3])
+    m = nn.Embedding(20, 16)
+    assert torch.equal(embed(m, ids.cpu()), m.weight[ids.cpu()])
+    with pytest.raises(RuntimeError):
+        embed(table(), ids.float())
