@@ -165,8 +165,8 @@ Grads attn_backward(Tensor dout, const Tensor& q, const Tensor& k, const Tensor&
 
 void first_order_only() {
   TORCH_CHECK(!at::GradMode::is_enabled(),
-              "hdcmamba_b200: norm_conv1d, gated_scan, group_norm_act, decay_attention and embedding are differentiable "
-              "once (create_graph=False)");
+              "hdcmamba_b200: norm_conv1d, gated_scan, group_norm_act and decay_attention are differentiable once "
+              "(create_graph=False)");
 }
 
 using torch::autograd::AutogradContext;
@@ -261,6 +261,9 @@ Tensor lookup_backward(const Tensor& dy, const Tensor& ids, int64_t rows, double
   return d;
 }
 
+// The lookup is linear in its table and its gradient linear in dy, so that each is the other's derivative.
+Variable embedding_grad(const Variable& dy, const Tensor& ids, int64_t rows, double scale, int64_t skip);
+
 // (weight, ids, scale, padding id or -1) -> rows; gradient for weight
 struct Embedding : torch::autograd::Function<Embedding> {
   static Variable forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale, int64_t skip) {
@@ -271,13 +274,36 @@ struct Embedding : torch::autograd::Function<Embedding> {
     return lookup(ids, weight, scale, std::nullopt);
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) {
-    first_order_only();
     auto& s = ctx->saved_data;
-    return {lookup_backward(d[0], ctx->get_saved_variables()[0], s["rows"].toInt(), s["scale"].toDouble(),
-                            s["skip"].toInt(), std::nullopt),
+    return {embedding_grad(d[0], ctx->get_saved_variables()[0], s["rows"].toInt(), s["scale"].toDouble(), s["skip"].toInt()),
             Variable(), Variable(), Variable()};
   }
 };
+
+// (dy, ids, rows, scale, padding id or -1) -> the table's gradient; gradient for dy: that of the padding's tokens is zero
+struct EmbeddingGrad : torch::autograd::Function<EmbeddingGrad> {
+  static Variable forward(AutogradContext* ctx, const Tensor& dy, const Tensor& ids, int64_t rows, double scale, int64_t skip) {
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["skip"] = skip;
+    ctx->save_for_backward({ids});
+    return lookup_backward(dy, ids, rows, scale, skip, std::nullopt);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list d) {
+    const Tensor ids = ctx->get_saved_variables()[0];
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const int64_t skip = ctx->saved_data["skip"].toInt();
+    const Tensor table = d[0].size(1) == 1 || d[0].stride(1) == 1 ? d[0] : d[0].contiguous();
+    Variable ddy = at::GradMode::is_enabled() && table.requires_grad() ? Embedding::apply(table, ids, scale, skip)
+                                                                       : lookup(ids, table, scale, std::nullopt);
+    if (skip >= 0) ddy = ddy.masked_fill(ids.eq(skip).unsqueeze(-1), 0);
+    return {ddy, Variable(), Variable(), Variable(), Variable()};
+  }
+};
+
+Variable embedding_grad(const Variable& dy, const Tensor& ids, int64_t rows, double scale, int64_t skip) {
+  if (at::GradMode::is_enabled() && dy.requires_grad()) return EmbeddingGrad::apply(dy, ids, rows, scale, skip);
+  return lookup_backward(dy, ids, rows, scale, skip, std::nullopt);
+}
 
 // ---------------------------------------------------------------- Python
 const Tensor& tensor(PyObject* o) {

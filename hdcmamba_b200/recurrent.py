@@ -33,8 +33,8 @@ __all__ = ["norm_conv1d", "gated_scan", "group_norm_act", "decay_attention", "No
 def _first_order_only():
     """Gradients of the gradients are not implemented: an error rather than missing terms."""
     if torch.is_grad_enabled():  # only with create_graph=True
-        raise RuntimeError("hdcmamba_b200: norm_conv1d, gated_scan, group_norm_act, decay_attention and embedding are "
-                           "differentiable once (create_graph=False)")
+        raise RuntimeError("hdcmamba_b200: norm_conv1d, gated_scan, group_norm_act and decay_attention are differentiable "
+                           "once (create_graph=False)")
 
 
 class NormConv1dFunction(torch.autograd.Function):

@@ -17,7 +17,7 @@ __all__ = ["embedding", "clip_grad_norm_"]
 
 
 def embedding(ids, weight, scale=1.0, padding_idx=None):
-    """Differentiable ``ops.embedding``: ids.shape + [D].  ``padding_idx``: an id whose tokens take no
+    """Differentiable ``ops.embedding`` (any number of times): ids.shape + [D].  ``padding_idx``: an id whose tokens take no
     part in the gradient (their rows are looked up like any other)."""
     _require_cuda(ids)
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:

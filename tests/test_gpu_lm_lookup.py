@@ -3,6 +3,7 @@ import pytest
 import torch
 import torch.nn as nn
 
+from hdcmamba_b200 import training
 from hdcmamba_b200.lm import embed
 
 pytestmark = pytest.mark.gpu
@@ -100,3 +101,32 @@ def test_tables_that_the_kernel_does_not_take():
     assert torch.equal(embed(m, ids.cpu()), m.weight[ids.cpu()])
     with pytest.raises(RuntimeError):
         embed(table(), ids.float())
+
+
+@pytest.mark.parametrize("padding_idx", [None, 3])
+def test_gradients_of_the_gradients(padding_idx):
+    """The lookup is linear in its table: as with the module, derivatives of every order."""
+    ids = torch.tensor(IDS).cuda()
+    m = table(padding_idx=padding_idx)
+    m.weight.data.normal_()
+
+    def chain(look):
+        w = m.weight
+        (g,) = torch.autograd.grad((look(m, ids) ** 3).sum(), [w], create_graph=True)
+        (h,) = torch.autograd.grad((g ** 2).sum(), [w], create_graph=True)
+        (t,) = torch.autograd.grad((h * torch.arange(16, device="cuda")).sum(), [w])
+        return g, h, t
+
+    for a, b in zip(chain(embed), chain(lambda mod, i: mod(i))):
+        assert (a - b).abs().max() <= 2.0 ** -24 * 64 * b.abs().max()  # some ten products and sums of up to four terms
+
+
+def test_gradients_of_the_scaled_lookup_against_differences():
+    ids = torch.tensor(IDS).cuda()
+    w = torch.randn(20, 16, generator=torch.Generator().manual_seed(1)).cuda().requires_grad_()
+    u, v = (torch.randn(s, generator=torch.Generator().manual_seed(2)).cuda() for s in ((2, 3, 16), (20, 16)))
+    dy = u.clone().requires_grad_()
+    (g,) = torch.autograd.grad(training.embedding(ids, w, scale=1.5, padding_idx=1), [w], dy, create_graph=True)
+    (d,) = torch.autograd.grad(g, [dy], v)
+    want = 1.5 * v[ids] * (ids != 1)[..., None]
+    assert torch.equal(d, want)
