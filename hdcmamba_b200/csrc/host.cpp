@@ -209,9 +209,13 @@ void is_table(const Tensor& t, const char* what) {
   TORCH_CHECK_VALUE(t.size(1) == 1 || t.stride(1) == 1, what, " needs a unit column stride");
 }
 
+// A tensor with memory of its own and no tangent: not a transform's or a subclass's stand-in for one.
+bool ordinary(const Tensor& t) {
+  return t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch() && !t._fw_grad(0).defined();
+}
 // whether `lookup` takes these: what nn.Embedding allows beyond is left to it
 bool takes(const Tensor& ids, const Tensor& w) {
-  return (w.scalar_type() == at::kFloat || w.scalar_type() == at::kBFloat16) && w.is_cuda() && w.dim() == 2 && w.stride(1) == 1 &&
+  return ordinary(ids) && ordinary(w) && (w.scalar_type() == at::kFloat || w.scalar_type() == at::kBFloat16) && w.is_cuda() && w.dim() == 2 && w.stride(1) == 1 &&
          w.size(0) >= 1 && w.size(0) <= (int64_t(1) << 30) && w.size(1) >= 1 && w.size(1) <= 65536 &&
          (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) && ids.device() == w.device() &&
          ids.numel() <= (int64_t(1) << 30);

@@ -17,6 +17,15 @@ def table(**kw):
 IDS = [[3, 1, 3], [7, 0, 19]]
 
 
+class Lookup(nn.Module):
+    def __init__(self, m):
+        super().__init__()
+        self.m = m
+
+    def forward(self, ids):
+        return embed(self.m, ids)
+
+
 def test_modules_of_other_kinds():
     class Sum(nn.Module):
         def __init__(self):
@@ -130,3 +139,26 @@ def test_gradients_of_the_scaled_lookup_against_differences():
     (d,) = torch.autograd.grad(g, [dy], v)
     want = 1.5 * v[ids] * (ids != 1)[..., None]
     assert torch.equal(d, want)
+
+
+def test_tangents_and_transforms():
+    """Forward-mode derivatives and torch.func's transforms go through the module."""
+    import torch.autograd.forward_ad as fwd
+    ids, m = torch.tensor(IDS).cuda(), table()
+    t = torch.randn_like(m.weight)
+    with fwd.dual_level():
+        w = fwd.make_dual(m.weight.detach(), t)
+        del m._parameters["weight"]
+        m.weight = w
+        assert torch.equal(fwd.unpack_dual(embed(m, ids)).tangent, t[ids])
+    m = table()
+
+    def loss(w):
+        y = torch.func.functional_call(Lookup(m), {"m.weight": w}, (ids,))
+        return (y ** 2).sum()
+
+    g = torch.func.grad(loss)(m.weight.detach())
+    want = torch.zeros_like(g).index_add_(0, ids.flatten(), 2 * m.weight.detach()[ids.flatten()])
+    assert (g - want).abs().max() <= 2.0 ** -22 * want.abs().max()
+    many = torch.stack([m.weight.detach(), 2 * m.weight.detach()])
+    assert torch.equal(torch.vmap(lambda w: torch.func.functional_call(Lookup(m), {"m.weight": w}, (ids,)))(many), many[:, ids])
