@@ -22,6 +22,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 from .model import _require_cuda
@@ -35,6 +36,12 @@ def _first_order_only():
     if torch.is_grad_enabled():  # only with create_graph=True
         raise RuntimeError("hdcmamba_b200: norm_conv1d, gated_scan, group_norm_act and decay_attention are differentiable "
                            "once (create_graph=False)")
+
+
+def _no_tangents(*tensors):
+    """Forward-mode derivatives are not implemented: an error rather than a tangent that is lost."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("hdcmamba_b200: the operators have no forward-mode derivatives (a dual tensor was passed)")
 
 
 class NormConv1dFunction(torch.autograd.Function):
@@ -59,6 +66,7 @@ def norm_conv1d(x, norm, conv):
     parameters of an ``nn.LayerNorm`` and an ``nn.Conv1d``; rows before the sequence are zeros
     before the norm."""
     _require_cuda(x)
+    _no_tangents(x, norm.weight, norm.bias, conv.weight, conv.bias)
     params = [p.to(x.dtype) for p in (norm.weight, norm.bias, conv.weight.squeeze(1), conv.bias)]
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params)):
         return NormConv1dFunction.apply(x, *params, norm.eps)
@@ -100,6 +108,7 @@ def gated_scan(projs, A_log, d_state, h0=None, reset=None):
     """Differentiable ``ops.gated_scan``: (y, h_last).  ``h0`` and ``h_last`` carry gradients,
     so a sequence can be trained window by window."""
     _require_cuda(projs)
+    _no_tangents(projs, A_log, h0)
     if torch.is_grad_enabled() and (projs.requires_grad or A_log.requires_grad or
                                     (h0 is not None and h0.requires_grad)):
         return GatedScanFunction.apply(projs, A_log, h0, reset, d_state)
@@ -132,6 +141,7 @@ class GroupNormActFunction(torch.autograd.Function):
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none"):
     """Differentiable ``ops.group_norm_act``."""
     _require_cuda(x)
+    _no_tangents(x, weight, bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return GroupNormActFunction.apply(x, weight, bias, num_groups, eps, act)
     return ops.group_norm_act(x, num_groups, weight, bias, eps=eps, act=act)
@@ -141,6 +151,7 @@ def decay_attention(q, k, v, log_decay, scale=1.0, state=None):
     """Differentiable ``ops.decay_attention``: (o, state after the last token).  The states carry
     gradients, so a sequence can be trained window by window; the decays are constants."""
     _require_cuda(q)
+    _no_tangents(q, k, v, log_decay, state)
     if log_decay.requires_grad:
         raise ValueError("decay_attention has no gradient for log_decay: pass a constant (log_decay.detach())")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or

@@ -12,6 +12,7 @@ import torch
 
 from . import _lib, ops
 from .model import _require_cuda
+from .recurrent import _no_tangents
 
 __all__ = ["embedding", "clip_grad_norm_"]
 
@@ -20,6 +21,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     """Differentiable ``ops.embedding`` (any number of times): ids.shape + [D].  ``padding_idx``: an id whose tokens take no
     part in the gradient (their rows are looked up like any other)."""
     _require_cuda(ids)
+    _no_tangents(weight)
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"padding_idx {padding_idx} is outside the table of {weight.shape[0]} rows")
     if torch.is_grad_enabled() and weight.requires_grad:
