@@ -151,6 +151,9 @@ def host():
         load()
         if not os.path.exists(os.path.join(HERE, "_host.so")):
             raise OSError(f"{HERE}/_host.so is missing: build it with `python -m hdcmamba_b200.build`")
+        from . import build
+        if not build.host_matches():
+            raise OSError(f"{HERE}/_host.so was compiled against another torch or Python: build it with `python -m hdcmamba_b200.build`")
         from . import _host as m
         m.set_error(HdcError)
         _host = m

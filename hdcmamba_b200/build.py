@@ -6,6 +6,7 @@ Both are built in-tree, next to this file, so that they travel with the source t
 import argparse
 import concurrent.futures as cf
 import os
+import platform
 import shutil
 import subprocess
 import sys
@@ -45,7 +46,21 @@ def up_to_date():
     if not os.path.exists(LIB) or not os.path.exists(HOST):
         return False
     t = min(os.path.getmtime(LIB), os.path.getmtime(HOST))
-    return all(os.path.getmtime(f) <= t for f in _deps() if os.path.exists(f))
+    return all(os.path.getmtime(f) <= t for f in _deps() if os.path.exists(f)) and host_matches()
+
+
+def host_tag():
+    """What the host module is compiled against, as it stands in the module."""
+    import torch
+    return (f"hdcmamba_b200._host for torch {torch.__version__}, C++ ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, "
+            f"Python {'.'.join(platform.python_version().split('.')[:2])};")
+
+
+def host_matches():
+    """Whether ``_host.so`` was compiled against this torch and Python; read from the file, since loading another's
+    may end in undefined symbols or in objects of another layout."""
+    with open(HOST, "rb") as f:
+        return host_tag().encode() in f.read()
 
 
 def host_command(obj):
@@ -55,7 +70,7 @@ def host_command(obj):
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
     dirs = (root, os.path.join(root, "torch", "csrc", "api", "include"), cuda, sysconfig.get_paths()["include"])
     return ["g++", "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-            *[f"-I{d}" for d in dirs], "-c", HOST_SRC, "-o", obj], os.path.join(os.path.dirname(torch.__file__), "lib")
+            f'-DHDC_HOST_TAG="{host_tag()}"', *[f"-I{d}" for d in dirs], "-c", HOST_SRC, "-o", obj], os.path.join(os.path.dirname(torch.__file__), "lib")
 
 
 def build(force=False, jobs=None, verbose=False, extra=()):

@@ -20,6 +20,9 @@
 
 #include "../../include/hdcmamba_b200.h"
 
+// what this module was compiled against (hdcmamba_b200/build.py reads it from the file)
+extern "C" __attribute__((used, visibility("default"))) const char hdc_host_tag[] = HDC_HOST_TAG;
+
 namespace {
 
 using at::Tensor;
