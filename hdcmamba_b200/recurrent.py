@@ -152,7 +152,7 @@ def decay_attention(q, k, v, log_decay, scale=1.0, state=None):
     gradients, so a sequence can be trained window by window; the decays are constants."""
     _require_cuda(q)
     _no_tangents(q, k, v, log_decay, state)
-    if log_decay.requires_grad:
+    if torch.is_grad_enabled() and log_decay.requires_grad:
         raise ValueError("decay_attention has no gradient for log_decay: pass a constant (log_decay.detach())")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                     (state is not None and state.requires_grad)):
