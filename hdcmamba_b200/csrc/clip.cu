@@ -93,27 +93,33 @@ struct Place {
   }
 };
 
-// 16 bytes that L2 keeps or lets go, by the policy
-__device__ __forceinline__ uint4 ldg16_hint(const void* p, uint64_t policy) {
+// 16 bytes that L2 keeps or lets go, by the policy.  RO: nothing writes them while the kernel runs; the kernel that
+// scales may do so in place, and loads them the ordinary way.
+template <bool RO> __device__ __forceinline__ uint4 ldg16_hint(const void* p, uint64_t policy) {
   uint4 r;
-  asm volatile("ld.global.nc.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p), "l"(policy));
+  if constexpr (RO) {
+    asm volatile("ld.global.nc.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p), "l"(policy));
+  } else {
+    asm volatile("ld.global.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p), "l"(policy) : "memory");
+  }
   return r;
 }
 // A piece's values in registers; zeros where there are none.
 struct Held {
   uint4 w[kVecs];
   float one;
-  __device__ __forceinline__ void load(const Place& p, uint64_t policy) {
+  template <bool RO> __device__ __forceinline__ void load(const Place& p, uint64_t policy) {
     const char* q = p.in + threadIdx.x * 16;
     if (p.vecs == kThreads * kVecs) {
 #pragma unroll
-      for (int i = 0; i < kVecs; ++i) w[i] = ldg16_hint(q + i * kThreads * 16, policy);
+      for (int i = 0; i < kVecs; ++i) w[i] = ldg16_hint<RO>(q + i * kThreads * 16, policy);
     } else {
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) {
-        const bool in = i * kThreads + (int)threadIdx.x < p.vecs;
-        w[i] = ldg16_pred(in ? q + i * kThreads * 16 : p.in, in);
+        w[i] = make_uint4(0, 0, 0, 0);
+        if (i * kThreads + (int)threadIdx.x < p.vecs) w[i] = ldg16_hint<RO>(q + i * kThreads * 16, policy);
       }
     }
     one = 0.f;
@@ -182,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) grad_squares_kernel(const __
   asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(go));
   for (Place at(w); at.vecs >= 0;) {
     Held v;
-    v.load(at, w.i >= keep_from ? stay : go);
+    v.load<true>(at, w.i >= keep_from ? stay : go);
     const int bf16 = at.bf16;
     w.next();
     at = Place(w);
@@ -240,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) grad_scale_kernel(const __gr
     const Place p = at;
     const bool skip = by == 1.f && p.in == p.out;  // it stays as it is
     Held v;
-    if (!skip) v.load(p, go);
+    if (!skip) v.load<false>(p, go);
     w.next();
     at = Place(w);
     if (!skip) p.bf16 ? scale_piece<__nv_bfloat16>(v, p, by) : scale_piece<float>(v, p, by);
