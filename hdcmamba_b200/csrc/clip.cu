@@ -6,10 +6,12 @@
 // launch serves up to kTensors tensors of mixed sizes and types.  The table of tensors is a kernel
 // argument: nothing is copied to the device beforehand, and a captured call needs no memory of the
 // host's.  Gradients that stay as they are, in place, the second kernel does not touch.
-// 76.5 M bf16 gradients into other buffers: 83 us for 459 MB, 5.5 TB/s; 190 M bf16 and 0.2 M fp32 204 us.  Reads
-// beside writes go no faster whatever the number of CTAs (2 to 6 per SM), the size of a piece or a second
-// piece in flight: what helps is less traffic, so the second kernel walks the pieces backwards and
-// finds the last 64 MB in L2 (86 and 211 us without; 32, 80 and 100 MB are no better).
+// 76.5 M bf16 gradients into other buffers: 76 us for 459 MB, 6.0 TB/s, in place 78 us; 190 M 190 us.  Reads beside
+// writes go no faster whatever the number of CTAs (2 to 6 per SM), the size of a piece or a second piece in flight: what
+// helps is less traffic, so the second kernel walks the pieces backwards and finds the last 64 MB in L2, which the first
+// one loads the ordinary way and all others as the first to let go (86 and 211 us without; 32, 80 and 100 MB are no better).
+// Asking L2 to keep the 64 MB above all else gains nothing here (77, 80 and 192 us), and where the second kernel has
+// nothing to read it would bind half of L2 for what comes later: a kernel over 100 MB that are in L2 35 us for 31.
 // Sums: a thread adds the squares of a piece's 16 or 32 elements in fp32, and those sums in 64 bits; the CTAs'
 // sums are added in a fixed order.  Where squares leave fp32's range (|g| above 1e18 or all below 1e-16)
 // a thread takes its elements again in 64 bits.
@@ -22,7 +24,7 @@
 namespace hdc {
 
 constexpr int kTensors = 512, kThreads = 256, kVecs = 4, kPerSm = 4, kCtas = 148 * kPerSm;
-constexpr int kKeep = 4096;  // the last pieces, 64 MB, that the first kernel asks L2 to keep for the second
+constexpr int kKeep = 4096;  // the last pieces, 64 MB, that stay in L2 from the first kernel to the second
 template <typename T> constexpr int kPiece = kThreads * kVecs * Vec<T>::N;  // elements: 16 KB
 
 struct ClipTable {
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) grad_squares_kernel(const __
   double d = 0;
   Walk w(t, false);
   uint64_t stay, go;
-  asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(stay));
+  asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(stay));
   asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(go));
   for (Place at(w); at.vecs >= 0;) {
     Held v;
