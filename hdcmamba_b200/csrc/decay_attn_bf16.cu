@@ -62,6 +62,9 @@ __device__ __forceinline__ void scale2(float& x, float& y, float f, float h) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_bits(x, y)), "l"(pair_bits(f, h)));
   bits_pair(r, x, y);
 }
+__device__ __forceinline__ void fma2(uint64_t& s, uint64_t a, uint64_t b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(s) : "l"(a), "l"(b));
+}
 // (x, y) minus the two bf16 values of v
 __device__ __forceinline__ void less2(float& x, float& y, uint32_t v) {
   uint64_t r;
@@ -225,6 +228,8 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(M
   const uint32_t lb = (lane % 8 + 8 * (lane / 16)) * PT + (lane / 8) % 2 * 16;
   const uint32_t tiles_at = shared_at(tiles), rbuf_at = shared_at(rbuf) + la + oc * 2;
 
+  uint64_t odd[2] = {0, 0};  // not finite where one of the thread's outputs is not
+
   for (int q = 0; q < chunks; ++q) {
     const int t0 = chunk_at(q), n_rows = min(kAttnChunk, end - t0), shift = kAttnChunk - n_rows;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -372,6 +377,8 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(M
         for (int e = 0; e < 4; ++e) R[n][e] += U[n][e];
     }
     if constexpr (OUT) {
+#pragma unroll
+      for (int n = 0; n < ON; ++n) fma2(odd[n & 1], pair_bits(O[n][0], O[n][1]), pair_bits(O[n][2], O[n][3]));
       if (q + 1 < chunks) keep_copy(q + 1);
       bf16* out = static_cast<bf16*>(const_cast<void*>(a.out.p)) + b * a.out.sb + h * a.out.sh + (int64_t)t0 * a.out.st;
       // through the strip's own rows of X, which no other warp reads (wide heads: the strip's second warp)
@@ -408,9 +415,8 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(M
       }
     }
   }
-  if constexpr (EXACT) {  // a segment's own sum, or the state behind a sequence of one segment
-    float* to = !OUT ? a.states + (bh * p.nseg + seg) * D * D : a.to ? a.to + bh * D * D : nullptr;
-    if (!to) return;
+  float* const to = !EXACT ? nullptr : !OUT ? a.states + (bh * p.nseg + seg) * D * D : a.to ? a.to + bh * D * D : nullptr;
+  auto leave = [&] {  // a segment's own sum, or the state behind a sequence of one segment
 #pragma unroll
     for (int n = 0; n < SN; ++n)
 #pragma unroll
@@ -418,6 +424,19 @@ __global__ void __launch_bounds__(AttnShape<DP>::kThreads, AttnShape<DP>::ctas(M
         const int row = sr + g + 8 * (e >> 1), col = sc + 8 * n + 2 * c + (e & 1);
         if (row < D && col < D) to[row * D + col] = R[n][e];
       }
+  };
+  const bool later = OUT && a.to == a.from;  // it takes the place of the one before the sequence, which may be read again
+  if (EXACT && to && !later) leave();
+  if constexpr (OUT) {
+    if (!__syncthreads_or(!all_finite(odd[0]) || !all_finite(odd[1]))) {
+      if (EXACT && to && later) leave();
+      return;
+    }
+    float* const M = reinterpret_cast<float*>(smem16);
+    state_for_recurrence(p, a, bh, seg, M);
+    __syncthreads();
+    if (EXACT && to && later) leave();
+    by_recurrence<bf16>(p, a, bh, seg, M);
   }
 }
 

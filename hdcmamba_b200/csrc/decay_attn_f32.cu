@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(c
   float* P = X;
   float* R = OUT ? X + Sh::kX : X;
   __shared__ float pw[kAttnChunk + 1];
+  __shared__ int s_odd;  // an output is not finite
   const AttnPass& a = p.pass[blockIdx.z];
   const int D = p.D, DR = (D + 3) & ~3, back = a.backwards;
   const int64_t bh = blockIdx.x / p.nseg;
@@ -101,8 +102,8 @@ __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(c
   float* to = !OUT ? a.states + (bh * p.nseg + seg) * D * D : p.nseg == 1 && a.to ? a.to + bh * D * D : nullptr;
   const int chunks = (end - begin + kAttnChunk - 1) / kAttnChunk;
   let_next_start();
+  if (OUT && threadIdx.x == 0) s_odd = 0;
   for (int i = threadIdx.x; i <= kAttnChunk; i += 256) pw[i] = decay_pow(p.g[h], i);
-
   for (int q = 0; q < chunks; ++q) {
     const int t0 = begin + (back ? chunks - 1 - q : q) * kAttnChunk, n = min(kAttnChunk, end - t0);
     load_rows<KD, VEC>(Y, PY, yp + (int64_t)t0 * a.y.st, a.y.st, n, D);
@@ -186,6 +187,13 @@ __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(c
           }
         }
       }
+      uint64_t odd[2] = {0, 0};
+#pragma unroll
+      for (int m = 0; m < G; ++m) {
+        fma2(odd[0], o[0][m], o[1][m]);
+        fma2(odd[1], o[2][m], o[3][m]);
+      }
+      if (!all_finite(odd[0]) || !all_finite(odd[1])) s_odd = 1;
       float* out = static_cast<float*>(const_cast<void*>(a.out.p)) + b * a.out.sb + h * a.out.sh + (int64_t)t0 * a.out.st;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -241,10 +249,15 @@ __global__ void __launch_bounds__(256, F32Shape<G>::ctas(OUT)) attn_f32_kernel(c
           *reinterpret_cast<uint64_t*>(R + (ty * 2 + 32 * (k / 2) + k % 2) * PR + tx * 2 + 32 * m) = r[k][m];
     }
   }
-  if (to) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < D * D; i += 256) to[i] = R[i / D * PR + i % D];
+  __syncthreads();
+  const bool redo = OUT && s_odd != 0;
+  if (redo) {  // (in the place of Z and Y)
+    state_for_recurrence(p, a, bh, seg, Z);
+    __syncthreads();  // the state behind the sequence may take the place of the one before it
   }
+  if (to)
+    for (int i = threadIdx.x; i < D * D; i += 256) to[i] = R[i / D * PR + i % D];
+  if (redo) by_recurrence<float>(p, a, bh, seg, Z);
 }
 
 template <int G, bool OUT, bool VEC> static int launch(const AttnParams& p, int64_t bh, int passes, cudaStream_t s) {

@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) attn_tc_kernel(const __grid_con
   // products: S and O1; O2; U.  Loads: X and Y; Z
   __shared__ __align__(8) uint64_t bars[5];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_late;
+  __shared__ int s_late, s_odd;  // a wait has run out; an output is not finite
   // powers of the decay; in(i) si and up(j) su of a whole chunk (a short one of n tokens reads the one that counts
   // from the chunk's end 128 - n further on); sa e^|i - j| at 127 + (j - i), zeros on the masked side
   __shared__ float pw[kTcTokens + 1], entry[2 * kTcTokens], update[2 * kTcTokens], apart[2 * kTcTokens];
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) attn_tc_kernel(const __grid_con
   if (threadIdx.x == 0) {
     for (int i = 0; i < 5; ++i) mbar_init(&bars[i], 1);
     fence_mbar_init();
-    s_late = 0;
+    s_late = s_odd = 0;
   }
   const float gd = p.g[h];
   for (int i = threadIdx.x; i < 2 * kTcTokens; i += kTcThreads) {
@@ -238,6 +238,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) attn_tc_kernel(const __grid_con
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         out[i] = f2_to_bf2(f2_add(f2_make(o[2 * i], o[2 * i + 1]), f2_make(o2[2 * i], o2[2 * i + 1])));
+      uint64_t odd = f2_make(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) odd = f2_fma(f2_make(o2[i], o2[i + 1]), f2_make(o2[i + 2], o2[i + 3]), odd);
+      if (!all_finite(odd)) s_odd = 1;
     }
     if (!last) {
       if (!mbar_wait_warp(&bars[2], ph, kTcCode)) s_late = 1;
@@ -302,6 +306,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) attn_tc_kernel(const __grid_con
   }
   __syncthreads();
   if (warp == 0) tmem_dealloc(tmem, 256);
+  if (s_odd && !s_late) {
+    float* M = reinterpret_cast<float*>(tiles);
+    state_for_recurrence(p, a, bh, seg, M);
+    __syncthreads();
+    by_recurrence<__nv_bfloat16>(p, a, bh, seg, M);
+  }
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,

@@ -460,8 +460,9 @@ int hdc_group_norm_bwd(int dtype, int p_dtype, const void* dy, int64_t dy_sn, in
  * dtype is that of q, k, v, o, dout, dq, dk, dv: element (b, t, h, d) of q at
  * q + b*q_sb + t*q_st + h*q_sh + d (elements; any strides, 0 for heads that share k or v), the others
  * likewise.  log_decay fp32 [H], constants (no gradient), meant to be <= 0.  States fp32 [B, H, D, D],
- * row i belonging to k's element i.  Products of bf16 tensors run on the tensor cores with fp32 sums; a
- * token's infinities and NaN may also reach the other tokens of the up to 128 with which it is computed.
+ * row i belonging to k's element i.  Products of bf16 tensors run on the tensor cores with fp32 sums.  A
+ * token's infinities and NaN reach the outputs that it reaches in the recurrence (in the gradient: those that it
+ * reaches through the states and their gradients), and no others.
  *   state_in, state_out : NULL or fp32 [B, H, D, D]; may be the same.
  *   states : fp32 [B, H, hdc_decay_attn_state_slots(dtype, B, L, H, D), D, D]: states between the parts that
  *            the sequence is cut into, which the gradient starts from; may be NULL where there is one slot and
