@@ -69,6 +69,11 @@ struct On {
         stream(reinterpret_cast<hdc_stream_t>(c10::cuda::getCurrentCUDAStream(t.device().index()).stream())) {}
 };
 
+// A tensor of the caller's that the call has written: autograd must not take what it saved of it before for what it was.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor make(at::IntArrayRef shape, const Tensor& like, at::ScalarType type) {
   return at::empty(shape, like.options().dtype(type).requires_grad(false));
 }
@@ -134,6 +139,7 @@ Out attn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
        hdc_decay_attn_fwd(a.code, VIEW(q), VIEW(k), VIEW(v), ptr<float>(a.g), ptr<float>(state), (float)scale, VIEW(r.o),
                           ptr<float>(r.state), r.states.defined() ? ptr<float>(r.states) : nullptr, a.B, a.L, a.H, a.D,
                           on.stream));
+  if (out) written(r.o);
   return r;
 }
 
@@ -241,6 +247,7 @@ Tensor lookup(const Tensor& ids, const Tensor& weight, double scale, const Maybe
   Tensor y = out ? *out : make(shape, weight, weight.scalar_type());
   done("hdc_embedding_fwd", hdc_embedding_fwd(code, ptr(i), bytes, ptr(weight), weight.stride(0), ptr(y), D, (float)scale,
                                               i.numel(), rows, D, on.stream));
+  if (out) written(y);
   return y;
 }
 
@@ -265,6 +272,7 @@ Tensor lookup_backward(const Tensor& dy, const Tensor& ids, int64_t rows, double
   const auto ws = workspace(n);
   done("hdc_embedding_bwd", hdc_embedding_bwd(code, ptr(i), bytes, ptr(g), g.stride(0), ptr(d), d.stride(0), (float)scale,
                                               skip, ws.get(), n, i.numel(), rows, D, on.stream));
+  if (out) written(d);
   return d;
 }
 
@@ -392,6 +400,8 @@ PyObject* py_attn_step(PyObject* const* p) {
        hdc_decay_attn_step(a.code, ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0),
                            v.stride(1), ptr<float>(a.g), ptr<float>(state), (float)scale, ptr(o), o.stride(0), o.stride(1),
                            ptr<float>(next), a.B, a.H, a.D, on.stream));
+  if (out) written(o);
+  written(next);
   return tuple(o, next);
 }
 PyObject* py_embedding(PyObject* const* a) { return wrap(lookup(tensor(a[0]), tensor(a[1]), number(a[2]), maybe(a[3]))); }
@@ -451,6 +461,8 @@ PyObject* py_clip(PyObject* const* a) {
   done("hdc_clip_grads", hdc_clip_grads(n, grads.codes.data(), const_cast<const void* const*>(grads.at.data()),
                                         scale ? to : nullptr, grads.sizes.data(), scale ? (float)number(a[1]) : 0.f,
                                         ptr<float>(norm), ws.get(), bytes, on.stream));
+  if (scale)
+    for (const Tensor& t : (out ? *out : grads).tensors) written(t);
   return wrap(norm);
 }
 PyObject* py_set_error(PyObject*, PyObject* type) {
