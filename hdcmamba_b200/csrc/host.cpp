@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -55,6 +56,15 @@ void on_device(const Tensor& ref, std::initializer_list<const Tensor*> rest) {
       TORCH_CHECK(t->is_cuda(), "hdcmamba_b200 kernels run on CUDA tensors only (got a CPU tensor)");
       TORCH_CHECK_VALUE(t->device() == ref.device(), "tensors are on ", ref.device(), " and ", t->device());
     }
+}
+// An output lies apart from what the call reads, as far as the two tell (views with gaps: unless they begin alike).
+void apart(const Tensor& out, std::initializer_list<const Tensor*> inputs, const char* what) {
+  for (const Tensor* t : inputs) {
+    if (!t || !t->defined() || !out.is_alias_of(*t) || out.numel() == 0 || t->numel() == 0) continue;
+    const auto s = at::get_overlap_status(out, *t);
+    if (out.data_ptr() == t->data_ptr() || s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial)
+      throw Failure(std::string("hdcmamba_b200: ") + what + " overlaps an input");
+  }
 }
 const Tensor* at_of(const Maybe& t) { return t ? &*t : nullptr; }
 template <typename T = void> T* ptr(const Tensor& t) { return static_cast<T*>(t.data_ptr()); }
@@ -126,6 +136,7 @@ Out attn_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
   if (out) {
     same_type(q, *out);
     is_heads(*out, q, "out");
+    apart(*out, {&q, &k, &v, &log_decay, at_of(state)}, "out");
   }
   on_device(q, {&k, &v, &log_decay, at_of(state), at_of(out)});
   On on(q);
@@ -240,6 +251,7 @@ Tensor lookup(const Tensor& ids, const Tensor& weight, double scale, const Maybe
     same_type(weight, *out);
     TORCH_CHECK_VALUE(out->sizes() == at::IntArrayRef(shape) && out->is_contiguous(), "out must be a contiguous ",
                       at::IntArrayRef(shape), " tensor");
+    apart(*out, {&ids, &weight}, "out");
   }
   on_device(weight, {&ids, at_of(out)});
   On on(weight);
@@ -261,6 +273,7 @@ Tensor lookup_backward(const Tensor& dy, const Tensor& ids, int64_t rows, double
     same_type(dy, *out);
     TORCH_CHECK_VALUE(out->sizes() == at::IntArrayRef({rows, D}), "out must be [", rows, ", ", D, "]");
     is_table(*out, "out");
+    apart(*out, {&dy, &ids}, "out");
   }
   on_device(dy, {&ids, at_of(out)});
   On on(dy);
@@ -390,12 +403,15 @@ PyObject* py_attn_step(PyObject* const* p) {
   if (out) {
     same_type(q, *out);
     is_heads(*out, q, "out");
+    apart(*out, {&q, &k, &v, &g, &state, at_of(state_out)}, "out");
   }
+  const Tensor& next = state_out ? *state_out : state;
+  apart(next, {&q, &k, &v, &g}, "the new state");
+  if (state_out && state_out->data_ptr() != state.data_ptr()) apart(next, {&state}, "state_out");
   on_device(q, {&k, &v, &g, &state, at_of(out), at_of(state_out)});
   On on(q);
   a.decays();
   const Tensor o = out ? *out : make({a.B, a.H, a.D}, q, q.scalar_type());
-  const Tensor& next = state_out ? *state_out : state;
   done("hdc_decay_attn_step",
        hdc_decay_attn_step(a.code, ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0),
                            v.stride(1), ptr<float>(a.g), ptr<float>(state), (float)scale, ptr(o), o.stride(0), o.stride(1),

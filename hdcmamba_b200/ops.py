@@ -834,7 +834,7 @@ def decay_attention_bwd(do, q, k, v, log_decay, states, scale=1.0, dstate=None, 
 def decay_attention_step(q, k, v, log_decay, state, scale=1.0, out=None, state_out=None):
     """One token per sequence of ``decay_attention`` (hdc_decay_attn_step): q, k, v [B, H, D] views (unit
     stride within a head), state contiguous fp32 [B, H, D, D], updated in place unless ``state_out`` is
-    given.  Returns (o [B, H, D], the new state)."""
+    given (the state itself, or apart from it).  out: optional [B, H, D] view, apart from all others.  Returns (o [B, H, D], the new state)."""
     return _lib.host().decay_attention_step(q, k, v, log_decay, state, scale, out, state_out)
 
 
@@ -842,7 +842,7 @@ def decay_attention_step(q, k, v, log_decay, state, scale=1.0, out=None, state_o
 def embedding(ids, weight, scale=1.0, out=None):
     """Rows of ``weight`` [rows, D] (unit column stride) by ``ids`` (int64 or int32, any shape), times
     ``scale`` (hdc_embedding_fwd; the LM wrappers' nn.Embedding, train.py:116-137): ids.shape + [D] in
-    weight's type.  out: optional contiguous tensor of that shape.  An id outside the table gives a row
+    weight's type.  out: optional contiguous tensor of that shape, apart from the inputs.  An id outside the table gives a row
     of NaN and an error in ``check_device``.  For autograd use ``training.embedding``."""
     return _lib.host().embedding(ids, weight, scale, out)
 
@@ -851,7 +851,8 @@ def embedding_bwd(dy, ids, rows, scale=1.0, padding_idx=None, out=None):
     """Gradient of ``embedding`` for its table of ``rows`` rows (hdc_embedding_bwd): dy ids.shape + [D].
     Tokens are sorted by id and each row's sum is taken in their order in fp32, so the result does not
     depend on timing; rows that no token has are zeros.  padding_idx: optional id that takes no part.
-    out: optional [rows, D] view (unit column stride).  Returns [rows, D] in dy's type."""
+    out: optional [rows, D] view (unit column stride), apart from the inputs.  Returns [rows, D] in dy's
+    type."""
     return _lib.host().embedding_bwd(dy, ids, rows, scale, padding_idx, out)
 
 

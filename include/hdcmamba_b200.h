@@ -504,8 +504,8 @@ int hdc_decay_attn_step(int dtype, const void* q, int64_t q_sb, int64_t q_sh, co
  *         of the gradient, and 71 through hdc_device_error().
  *   table : row v at table + v*table_st (elements); y, dy, dtable likewise.
  *   skip_id : an id that takes no part in the gradient (padding); -1 for none.
- * N, rows in [0 or 1, 2^30], D in [1, 65536].  Rows of y and of dtable must not overlap.  Pointers need
- * their type's alignment; 16-byte aligned rows take the wide loads.  workspace:
+ * N, rows in [0 or 1, 2^30], D in [1, 65536].  Rows of y and of dtable must not overlap, nor the outputs
+ * the inputs.  Pointers need their type's alignment; 16-byte aligned rows take the wide loads.  workspace:
  * hdc_embedding_bwd_workspace_bytes, 16-byte aligned.
  */
 int hdc_embedding_fwd(int dtype, const void* ids, int id_bytes, const void* table, int64_t table_st, void* y,
