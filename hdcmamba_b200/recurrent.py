@@ -157,7 +157,7 @@ def decay_attention(q, k, v, log_decay, scale=1.0, state=None):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                     (state is not None and state.requires_grad)):
         return _lib.host().decay_attention_train(q, k, v, log_decay, state, scale)  # a C++ autograd node
-    return ops.decay_attention(q, k, v, log_decay, scale, state)
+    return ops.decay_attention(q, k, v, log_decay, scale, state.float().contiguous() if state is not None else None)
 
 
 @dataclass
