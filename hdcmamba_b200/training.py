@@ -34,11 +34,10 @@ def clip_grad_norm_(parameters, max_norm):
     """Scale the gradients of ``parameters`` (a tensor or an iterable) in place so that the norm over all
     of them is at most ``max_norm``; returns the norm before (fp32 on the device, which the host does
     not wait for).  Gradients are fp32 or bf16, mixed as they come; parameters without one are left out."""
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
-        return torch.zeros(())
+        return torch.zeros((), device=parameters[0].device if parameters else None)
     if all(g.is_contiguous() for g in grads):
         return ops.clip_grads(grads, max_norm)
     # gradients in another order of memory: scaled in a copy

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from hdcmamba_b200 import ops
+from hdcmamba_b200 import ops, training
 
 pytestmark = pytest.mark.gpu
 
@@ -19,3 +19,11 @@ def test_in_place_and_elsewhere(dtype, lead):
     n1 = ops.clip_grads(grads, 2.0, out=other)
     n2 = ops.clip_grads(grads, 2.0)
     assert torch.equal(n1, n2) and all(torch.equal(a, b) for a, b in zip(grads, other))
+
+
+def test_the_norm_of_no_gradients_is_on_the_parameters_device():
+    p = torch.nn.Parameter(torch.ones(3, device="cuda"))
+    for params in (p, [p], iter([p])):
+        norm = training.clip_grad_norm_(params, 1.0)
+        assert norm.device == p.device and norm.dtype == torch.float32 and norm == 0
+    assert training.clip_grad_norm_([], 1.0) == 0
