@@ -235,7 +235,8 @@ bool ordinary(const Tensor& t) {
 }
 // whether `lookup` takes these: what nn.Embedding allows beyond is left to it
 bool takes(const Tensor& ids, const Tensor& w) {
-  return ordinary(ids) && ordinary(w) && (w.scalar_type() == at::kFloat || w.scalar_type() == at::kBFloat16) && w.is_cuda() && w.dim() == 2 && w.stride(1) == 1 &&
+  return ordinary(ids) && ordinary(w) && (w.scalar_type() == at::kFloat || w.scalar_type() == at::kBFloat16) && w.is_cuda() &&
+         w.dim() == 2 && w.stride(1) == 1 &&
          w.size(0) >= 1 && w.size(0) <= (int64_t(1) << 30) && w.size(1) >= 1 && w.size(1) <= 65536 &&
          (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) && ids.device() == w.device() &&
          ids.numel() <= (int64_t(1) << 30);
@@ -421,7 +422,10 @@ PyObject* py_attn_step(PyObject* const* p) {
   return tuple(o, next);
 }
 PyObject* py_embedding(PyObject* const* a) { return wrap(lookup(tensor(a[0]), tensor(a[1]), number(a[2]), maybe(a[3]))); }
-PyObject* py_embedding_takes(PyObject* const* a) { return PyBool_FromLong(takes(tensor(a[0]), tensor(a[1]))); }
+// (subclasses of Tensor, but for Parameter, may mean something else by a lookup)
+PyObject* py_embedding_takes(PyObject* const* a) {
+  return PyBool_FromLong(THPVariable_CheckExact(a[0]) && THPVariable_CheckExact(a[1]) && takes(tensor(a[0]), tensor(a[1])));
+}
 PyObject* py_embedding_bwd(PyObject* const* a) {
   return wrap(lookup_backward(tensor(a[0]), tensor(a[1]), whole(a[2]), number(a[3]), a[4] == Py_None ? -1 : whole(a[4]), maybe(a[5])));
 }

@@ -162,3 +162,23 @@ def test_tangents_and_transforms():
     assert (g - want).abs().max() <= 2.0 ** -22 * want.abs().max()
     many = torch.stack([m.weight.detach(), 2 * m.weight.detach()])
     assert torch.equal(torch.vmap(lambda w: torch.func.functional_call(Lookup(m), {"m.weight": w}, (ids,)))(many), many[:, ids])
+
+
+def test_tensor_subclasses_see_the_lookup():
+    seen = []
+
+    class Watched(torch.Tensor):
+        @classmethod
+        def __torch_function__(cls, func, types, args=(), kwargs=None):
+            seen.append(getattr(func, "__name__", ""))
+            return super().__torch_function__(func, types, args, kwargs or {})
+
+    ids, m = torch.tensor(IDS).cuda(), table()
+    for which in ("ids", "weight"):
+        seen.clear()
+        if which == "weight":
+            w = m.weight.detach().as_subclass(Watched)
+            del m._parameters["weight"]
+            m.weight = w
+        y = embed(m, ids.as_subclass(Watched) if which == "ids" else ids)
+        assert isinstance(y, Watched) and "embedding" in seen, (which, seen)
