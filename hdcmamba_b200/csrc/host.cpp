@@ -321,15 +321,30 @@ struct EmbeddingGrad : torch::autograd::Function<EmbeddingGrad> {
     const Tensor ids = ctx->get_saved_variables()[0];
     const double scale = ctx->saved_data["scale"].toDouble();
     const int64_t skip = ctx->saved_data["skip"].toInt();
-    const Tensor table = d[0].size(1) == 1 || d[0].stride(1) == 1 ? d[0] : d[0].contiguous();
-    Variable ddy = at::GradMode::is_enabled() && table.requires_grad() ? Embedding::apply(table, ids, scale, skip)
-                                                                       : lookup(ids, table, scale, std::nullopt);
+    Variable ddy;
+    if (!d[0].has_storage()) {  // a transform's stand-in for several
+      auto shape = ids.sizes().vec();
+      shape.push_back(d[0].size(1));
+      ddy = d[0].index_select(0, ids.reshape({-1})).reshape(shape);
+      if (scale != 1.0) ddy = ddy * scale;
+    } else {
+      const Tensor table = d[0].size(1) == 1 || d[0].stride(1) == 1 ? d[0] : d[0].contiguous();
+      ddy = at::GradMode::is_enabled() && table.requires_grad() ? Embedding::apply(table, ids, scale, skip)
+                                                                : lookup(ids, table, scale, std::nullopt);
+    }
     if (skip >= 0) ddy = ddy.masked_fill(ids.eq(skip).unsqueeze(-1), 0);
     return {ddy, Variable(), Variable(), Variable(), Variable()};
   }
 };
 
 Variable embedding_grad(const Variable& dy, const Tensor& ids, int64_t rows, double scale, int64_t skip) {
+  if (!dy.has_storage()) {  // a transform's stand-in for several (is_grads_batched): operations that it can take apart
+    const int64_t D = dy.size(-1);
+    Tensor terms = dy.to(at::kFloat) * scale;
+    if (skip >= 0) terms = terms.masked_fill(ids.eq(skip).unsqueeze(-1), 0);
+    const Tensor zeros = at::zeros({rows, D}, ids.options().dtype(at::kFloat));
+    return zeros.index_add(0, ids.reshape({-1}), terms.reshape({-1, D})).to(dy.scalar_type());
+  }
   if (at::GradMode::is_enabled() && dy.requires_grad()) return EmbeddingGrad::apply(dy, ids, rows, scale, skip);
   return lookup_backward(dy, ids, rows, scale, skip, std::nullopt);
 }

@@ -182,3 +182,23 @@ def test_tensor_subclasses_see_the_lookup():
             m.weight = w
         y = embed(m, ids.as_subclass(Watched) if which == "ids" else ids)
         assert isinstance(y, Watched) and "embedding" in seen, (which, seen)
+
+
+@pytest.mark.parametrize("padding_idx", [None, 3])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_batched_gradients(padding_idx, dtype):
+    """Several gradients at once (is_grads_batched), as the module gives them."""
+    ids = torch.tensor(IDS).cuda()
+    m = table(padding_idx=padding_idx).to(dtype)
+    dy = torch.randn(4, 2, 3, 16, generator=torch.Generator().manual_seed(1)).cuda().to(dtype)
+    one = [torch.autograd.grad(embed(m, ids), [m.weight], d)[0] for d in dy]
+    (got,) = torch.autograd.grad(embed(m, ids), [m.weight], dy, is_grads_batched=True)
+    tol = 2 ** -8 if dtype == torch.bfloat16 else 2.0 ** -23  # sums of two terms, rounded once
+    assert (got - torch.stack(one)).abs().max() <= tol * got.abs().max()
+    # the gradient's own gradient, batched
+    y = dy[0].clone().requires_grad_()
+    (g,) = torch.autograd.grad(embed(m, ids), [m.weight], y, create_graph=True)
+    v = torch.randn(3, 20, 16, generator=torch.Generator().manual_seed(2)).cuda().to(dtype)
+    (d,) = torch.autograd.grad(g, [y], v, is_grads_batched=True)
+    want = v[:, ids] * (1 if padding_idx is None else (ids != padding_idx)[..., None])
+    assert torch.equal(d, want)
